@@ -283,6 +283,15 @@ spl_status spl_argmax(spl_engine *engine, int32_t vocab_limit, int32_t *ids);
  * descending order, the lower index first among equal values; ids and values [logit rows][k] on the host. Rows with
  * fewer than k values above -inf end in (0, -inf) entries, as the reference's untouched slots do. */
 spl_status spl_topk(spl_engine *engine, int32_t vocab_limit, int32_t k, int32_t *ids, float *values);
+/* Sampler.sample (Sampler.swift:128-156) for every logit row of the last step, on the device and over the whole of [0, vocab_limit): `settings` and
+ * `uniform` (numbers in [0, 1), say from spl_sampler_uniform) one a row, ids one a row. The values stand in descending order, the
+ * lower index first among equal ones; with w = exp((x - max x) / temperature) the first top_k stay (<= 0: all), of those the smallest
+ * prefix whose w reaches top_p of their sum (>= 1: all), of those the ones with w >= min_p (<= 0: all; above 1 taken as 1), and the
+ * token is the first whose running sum of w reaches uniform times the sum of what stays. temperature <= 0 takes the largest value.
+ * NaN and -inf are never picked; a row without any other value gives id 0. Sums are formed so that the token is the definition's in
+ * 64 bits and the same in every run. vocab_limit is at most 524,288. */
+typedef struct spl_sampling { float temperature; int32_t top_k; float top_p, min_p; } spl_sampling;
+spl_status spl_sample(spl_engine *engine, int32_t vocab_limit, const spl_sampling *settings, const float *uniform, int32_t *ids);
 spl_status spl_slot_reset(spl_engine *engine, int32_t slot);                                  /* Engine.resetSlot */
 spl_status spl_verify_discard(spl_engine *engine, int32_t slot);                              /* Engine.discardVerify */
 spl_status spl_verify_accept(spl_engine *engine, int32_t slot, int32_t rows, int32_t token_count); /* Engine.acceptVerify */
@@ -394,6 +403,55 @@ spl_status spl_pass_embed(spl_engine *engine, const uint32_t *device_tokens, int
 /* Engine.mlpIn: out = bf16(silu(gate x in) * (up x in)) as fp32 rows; scratch [rows][gate rows] holds up x in. */
 spl_status spl_pass_mlp_in(spl_engine *engine, const spl_tensor *gate, const spl_tensor *up, const float *device_in, int32_t rows, float *device_out, float *device_scratch);
 spl_status spl_pass_wait(spl_engine *engine);
+/* spl_sample's rule on logits of the caller's, fp32 [rows][ld] on the device; settings and uniform numbers are device arrays of one element
+ * a row, and a null array of settings stands for temperature 1, or for a filter that is off. Queued on `stream`, as the calls below. */
+spl_status spl_pass_sample(spl_engine *engine, const float *device_logits, int32_t rows, int64_t ld, int32_t vocab_limit, const float *device_temperature,
+                           const int32_t *device_top_k, const float *device_top_p, const float *device_min_p, const float *device_uniform, int32_t *device_ids, void *stream);
+
+/* ---- A paged cache of the caller's own --------------------------------------------------------
+ * The attention of a pass over the caller's own tensors (DraftModel keeps a K/V store and an attention of its own beside the
+ * engine's primitives, DraftModel.swift:418-468, Sources/Shaders/draft.metal:59-100): keys and values of any number of sequences in pages of
+ * 16-bit elements that the caller owns, K and V in buffers of the same layout. A spl_paged describes one layer shape and holds a batch:
+ *   spl_paged_batch   once a pass: which sequences have how many new tokens, how long they are with them, and their pages
+ *   spl_paged_append  once a layer: queries, keys and values of the new tokens, normed (where weights are given) and rotated at their
+ *                     positions; keys and values into the cache, queries to rows of the cache's type
+ *   spl_paged_attend  once a layer: the new rows' attention over everything cached
+ * Row r of a pass is the r-th new token, sequence after sequence; sequence s's new tokens are the last rows[s] of its lengths[s].
+ * Rows past the batch's are neither read nor written. `stream` is a cudaStream_t, null for the engine's stream (the
+ * other spl_pass_ calls'); cudaStreamLegacy is the default stream. Calls on one spl_paged are ordered by the caller: one stream at a time, or events between
+ * them. append and attend allocate nothing and may be captured into a graph; such a graph may be replayed after another spl_paged_batch of the same
+ * rows per sequence (lengths and pages may differ). Two graphs, or two streams, that may run at the same time need a spl_paged each.
+ * An attention block that gives up a wait is reported by the next spl_pass_wait (after the caller has synchronised its stream). */
+enum { SPL_F32 = 0, SPL_F16 = 1, SPL_BF16 = 2 };
+typedef struct spl_paged spl_paged;
+typedef struct spl_paged_config {
+    int32_t heads, kv_heads, head_dim;                   /* head_dim 64, 128 or 256; heads a multiple of kv_heads, at most 64 times it */
+    int32_t dtype;                                       /* of cache and queries: SPL_F16 or SPL_BF16 */
+    int32_t page_tokens, pages;                          /* 16, 32, 64, 128 or 256 tokens a page; pages of the cache */
+    int64_t page_stride, head_stride, token_stride;      /* elements; [page][kv head][token][channel] or [page][token][kv head][channel], multiples of 8 */
+    int32_t rotary_dim;                                  /* channels i and i + rotary_dim / 2 turn by position * rope_theta^(-2 i / rotary_dim) */
+    float rope_theta;
+    float scale;                                         /* of the scores; 0: 1 / sqrt(head_dim) */
+    int32_t causal;                                      /* 0: a row sees all of its sequence (a block of rows that see each other) */
+    int32_t window;                                      /* > 0: a row at position i sees no token before i - window + 1 */
+    int32_t max_sequences, max_rows, max_context;        /* of a batch; max_context tokens a sequence */
+} spl_paged_config;
+spl_status spl_paged_create(spl_engine *engine, const spl_paged_config *config, spl_paged **out);
+/* Waits for the device: calls may be queued on streams of the caller's. Destroy it before its engine. */
+void spl_paged_destroy(spl_paged *paged);
+/* Host arrays: rows[sequences], lengths[sequences] (new tokens included; rows[s] may be 0), page_table[sequences][table_ld] of which the
+ * first ceil(lengths[s] / page_tokens) entries are read. Everything is checked here (SPL_ERR_INVALID_ROWS, SPL_ERR_CONTEXT_EXCEEDED; the batch set
+ * before stays), copied on `stream`, and may be changed when the call returns. Not during a stream capture. */
+spl_status spl_paged_batch(spl_paged *paged, int32_t sequences, const int32_t *rows, const int32_t *lengths, const int32_t *page_table, int32_t table_ld, void *stream);
+/* Rows of `type` (SPL_F32, SPL_F16, SPL_BF16) with row strides in elements (even; rows begin on a boundary of two elements): q [rows][heads][head_dim],
+ * k and v [rows][kv_heads][head_dim]. q_norm and k_norm (spl_tensor_create_vector of head_dim, may be null): x * rsqrt(mean x^2 + eps) * weight
+ * over a head's channels, before the rotation. q_out [rows][heads][head_dim] of the cache's type. A batch in which two sequences
+ * would write to one page is refused. */
+spl_status spl_paged_append(spl_paged *paged, int32_t type, const void *device_q, int64_t q_ld, const void *device_k, int64_t k_ld, const void *device_v, int64_t v_ld,
+                            const spl_tensor *q_norm, const spl_tensor *k_norm, void *device_q_out, void *device_k_cache, void *device_v_cache, void *stream);
+/* q [rows][heads][head_dim] of the cache's type; out the same shape, out_type SPL_F32 or the cache's type. Scores, softmax statistics and sums are fp32, a
+ * probability is rounded to the cache's type before it meets the values. Buffers begin on 16-byte boundaries. */
+spl_status spl_paged_attend(spl_paged *paged, const void *device_q, const void *device_k_cache, const void *device_v_cache, int32_t out_type, void *device_out, void *stream);
 
 /* ---- The DFlash 2 block-diffusion drafter (Sources/SploshRuntime/DraftModel.swift) -----------------
  * A draft pass proposes a whole block at once: [anchor, mask x (block - 1)] through a few non-causal layers that attend

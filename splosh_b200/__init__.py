@@ -8,6 +8,7 @@ from .engine import (Engine, EngineConfig, EngineRow, EngineError, Geometry, Hos
                      gemm_q4, gemm_gguf, greedy_accept, library_path, Sampler, Planner, PackSession)
 
 from .draft import DraftModel, DraftConfig, DraftRequest, DraftProposal
+from .paged import PagedAttention
 
-__all__ = ["DraftModel", "DraftConfig", "DraftRequest", "DraftProposal", "Engine", "EngineConfig", "EngineRow", "EngineError", "Geometry", "Host", "StepStats", "tiny_geometry",
+__all__ = ["PagedAttention", "DraftModel", "DraftConfig", "DraftRequest", "DraftProposal", "Engine", "EngineConfig", "EngineRow", "EngineError", "Geometry", "Host", "StepStats", "tiny_geometry",
            "b27_geometry", "gemm_q4", "gemm_gguf", "greedy_accept", "library_path", "Sampler", "Planner", "PackSession"]

@@ -2126,3 +2126,4 @@ spl_status spl_pass_wait(spl_engine *e) {
 }  // extern "C"
 
 #include "spl_draft_impl.cuh"
+#include "spl_paged_impl.cuh"

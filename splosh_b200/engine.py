@@ -243,6 +243,13 @@ def lib():
             "spl_debug_profile_read": (i32, [vp, i32, C.POINTER(C.c_double), C.POINTER(C.c_int64), C.POINTER(C.c_double)]),
             "spl_op_gemm_q4": (i32, [i32, vp, vp, vp, i32, i32, vp, i32, vp, vp]),
             "spl_gemm_q4_static": (i32, [vp, i32, i32, vp, i32, vp, vp, vp]),
+            "spl_sample": (i32, [vp, i32, vp, vp, vp]),
+            "spl_pass_sample": (i32, [vp, vp, i32, C.c_int64, i32, vp, vp, vp, vp, vp, vp, vp]),
+            "spl_paged_create": (i32, [vp, vp, C.POINTER(vp)]),
+            "spl_paged_destroy": (None, [vp]),
+            "spl_paged_batch": (i32, [vp, i32, vp, vp, vp, i32, vp]),
+            "spl_paged_append": (i32, [vp, i32, vp, C.c_int64, vp, C.c_int64, vp, C.c_int64, vp, vp, vp, vp, vp, vp]),
+            "spl_paged_attend": (i32, [vp, vp, vp, vp, i32, vp, vp]),
             "spl_draft_create": (i32, [vp, vp, vp]),
             "spl_draft_destroy": (None, [vp]),
             "spl_draft_set_tensor": (i32, [vp, C.c_char_p, vp, i32, i32]),
@@ -273,6 +280,11 @@ EXPORTS = None  # filled by tests from include/splosh_cuda.h
 
 def _ptr(a):
     return a.ctypes.data_as(C.c_void_p)
+
+
+def stream_handle(stream):
+    """A cudaStream_t as an integer: None for the engine's own stream, 0 (what torch calls its default stream) for the legacy default stream."""
+    return None if stream is None else int(stream) or 1
 
 
 def _rows_array(rows):
@@ -525,6 +537,11 @@ class Engine:
     def pass_mlp_in(self, gate, up, device_in, rows, device_out, device_scratch):
         self._check(lib().spl_pass_mlp_in(self.handle, gate, up, C.c_void_p(device_in), rows, C.c_void_p(device_out), C.c_void_p(device_scratch)))
 
+    def pass_sample(self, device_logits, rows, ld, vocab_limit, device_ids, device_uniform, temperature=None, top_k=None, top_p=None, min_p=None, stream=None):
+        """A token a row from fp32 logits on the device (spl_pass_sample); the settings are addresses of one value a row, or None."""
+        self._check(lib().spl_pass_sample(self.handle, device_logits, rows, ld, vocab_limit, temperature, top_k, top_p, min_p, device_uniform, device_ids,
+                                          stream_handle(stream)))
+
     def pass_wait(self):
         self._check(lib().spl_pass_wait(self.handle))
 
@@ -678,6 +695,20 @@ class Engine:
         ids = np.zeros((n, k), np.int32); values = np.zeros((n, k), np.float32)
         self._check(lib().spl_topk(self.handle, vocab_limit or self.g.vocab, k, _ptr(ids), _ptr(values)))
         return ids[:self.last_logit_rows], values[:self.last_logit_rows]
+
+    def sample(self, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, vocab_limit=None):
+        """A token for every logit row of the last step, drawn on the device from the whole vocabulary (spl_sample): `uniform` one number
+        in [0, 1) a row, the settings one value for all rows or one a row."""
+        n = self.last_logit_rows
+        uniform = np.ascontiguousarray(uniform, np.float32)
+        if uniform.shape != (n,):
+            raise EngineError(10, f"{n} uniform numbers are needed, one a logit row")
+        settings = np.zeros(max(n, 1), [("temperature", np.float32), ("top_k", np.int32), ("top_p", np.float32), ("min_p", np.float32)])
+        for name, value in (("temperature", temperature), ("top_k", top_k), ("top_p", top_p), ("min_p", min_p)):
+            settings[name][:n] = value
+        ids = np.zeros(max(n, 1), np.int32)
+        self._check(lib().spl_sample(self.handle, vocab_limit or self.g.vocab, _ptr(settings), _ptr(uniform), _ptr(ids)))
+        return ids[:n]
 
     def enable_features(self, layers=None, enabled=True):
         """Engine.step(captureFeatures:) (Engine.swift:1316): keep the residual stream after the listed blocks

@@ -1,0 +1,270 @@
+"""The paged cache of the caller's own: append and attention against plain 64-bit implementations, over types, head layouts, page sizes, lengths from one
+token on, windows, padding, streams and graphs. What may not be read is NaN."""
+import numpy as np
+import pytest
+import torch
+
+import splosh_b200 as S
+from helpers import observed
+from paged_reference import Scene, TYPES, check_attention, half_step
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def engine():
+    e = S.Engine(S.tiny_geometry(), S.EngineConfig(max_slots=1, max_rows=64, kv_pages=4, max_context=512))
+    yield e
+    e.close()
+
+
+def bf16_bits(x):
+    return x.to(torch.bfloat16).view(torch.int16).numpy().view(np.uint16)
+
+
+# ---- attention -----------------------------------------------------------------------------------
+def attend(engine, scene, out_dtype=None, stream=None, paged=None):
+    paged = paged or scene.paged(engine, S.PagedAttention)
+    out = torch.full((scene.total + 1, scene.heads, scene.head_dim), 7.0, device="cuda", dtype=TYPES[out_dtype or scene.dtype])
+    torch.cuda.synchronize()
+    paged.batch(scene.rows, scene.lengths, scene.table, stream=stream)
+    paged.attend(scene.dq.data_ptr(), scene.k.data_ptr(), scene.v.data_ptr(), out.data_ptr(), out_dtype=out_dtype, stream=stream)
+    engine.pass_wait()
+    torch.cuda.synchronize()
+    assert (out[scene.total:] == 7.0).all()              # rows behind the last sequence stay
+    return out[:scene.total]
+
+
+SHAPES = [(8, 2, 128), (24, 4, 256), (6, 6, 64), (16, 1, 128), (5, 1, 64), (12, 2, 256), (32, 1, 64)]
+
+
+@pytest.mark.parametrize("heads,kv_heads,head_dim", SHAPES)
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("out_dtype", ["same", "f32"])
+def test_head_shapes_and_types(engine, heads, kv_heads, head_dim, dtype, out_dtype):
+    scene = Scene(heads + head_dim, heads, kv_heads, head_dim, [1, 0, 7, 3], [1, 40, 150, 301], dtype=dtype)
+    out = dtype if out_dtype == "same" else "f32"
+    worst = check_attention(scene, attend(engine, scene, out), out)
+    observed(f"paged attention {heads}/{kv_heads}/{head_dim} {dtype} -> {out}: {worst:.2f} of the bound")
+
+
+@pytest.mark.parametrize("page_tokens", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("layout", ["head", "token"])
+@pytest.mark.parametrize("head_dim", [64, 128, 256])
+def test_page_sizes_and_layouts(engine, page_tokens, layout, head_dim):
+    scene = Scene(page_tokens + head_dim, 4, 2, head_dim, [2, 1, 5], [page_tokens, page_tokens + 1, 3 * page_tokens - 1], page_tokens=page_tokens, layout=layout)
+    check_attention(scene, attend(engine, scene, "f32"), "f32")
+
+
+@pytest.mark.parametrize("length", [1, 2, 15, 16, 17, 63, 64, 65, 127, 128, 129, 255, 256, 257, 383, 511, 640, 1000])
+@pytest.mark.parametrize("head_dim", [64, 128, 256])
+def test_lengths_around_tiles_and_pages(engine, length, head_dim):
+    scene = Scene(length, 4, 1, head_dim, [min(length, 3), 1], [length, length], page_tokens=64)
+    check_attention(scene, attend(engine, scene), "bf16")
+
+
+@pytest.mark.parametrize("rows,lengths", [([130], [130]), ([301, 1, 1], [301, 77, 500]), ([97], [700]), ([33, 34, 35], [33, 99, 290]), ([16] * 9, [16 + 37 * i for i in range(9)])])
+@pytest.mark.parametrize("heads,kv_heads,head_dim,dtype", [(6, 1, 256, "bf16"), (8, 2, 128, "fp16"), (3, 1, 64, "bf16")])
+def test_prompts_chunks_and_mixed_batches(engine, rows, lengths, heads, kv_heads, head_dim, dtype):
+    scene = Scene(sum(lengths), heads, kv_heads, head_dim, rows, lengths, page_tokens=16, dtype=dtype, layout="token")
+    check_attention(scene, attend(engine, scene), dtype)
+
+
+@pytest.mark.parametrize("window", [1, 2, 63, 64, 129, 300])
+@pytest.mark.parametrize("causal", [True, False])
+def test_windows_and_blocks_that_see_themselves(engine, window, causal):
+    scene = Scene(window, 8, 2, 128, [16, 1, 40], [300, 150, 40], page_tokens=32, causal=causal, window=window)
+    check_attention(scene, attend(engine, scene, "f32"), "f32")
+
+
+@pytest.mark.parametrize("head_dim", [64, 128, 256])
+def test_long_contexts_of_few_rows(engine, head_dim):
+    scene = Scene(9, 4, 1, head_dim, [1, 4], [9001, 5000], page_tokens=128)
+    check_attention(scene, attend(engine, scene), "bf16")
+
+
+def test_scores_far_apart_and_a_maximum_that_keeps_rising(engine):
+    """Keys that grow with the position raise a row's maximum tile after tile; large queries make most probabilities vanish."""
+    for dtype in ("bf16", "fp16"):
+        scene = Scene(3, 4, 2, 128, [4, 200], [900, 700], page_tokens=64, dtype=dtype)
+        for s, (keys, _) in enumerate(scene.tokens):
+            factor = torch.linspace(0.1, 12.0, keys.shape[0]).to(TYPES[dtype]).double()[:, None, None]
+            keys.copy_((keys * factor).to(TYPES[dtype]).double())
+            for i in range(-(-keys.shape[0] // 64)):
+                part = keys[i * 64:(i + 1) * 64]
+                scene.k[scene.table[s, i], :, :part.shape[0]] = part.transpose(0, 1).to(TYPES[dtype]).cuda()
+        check_attention(scene, attend(engine, scene, "f32"), "f32")
+
+
+def test_what_the_mask_hides_may_be_anything(engine):
+    """Infinities in tokens that a row does not see: behind the last token, in front of the window."""
+    scene = Scene(5, 4, 1, 128, [1, 1], [200, 77], page_tokens=64, window=50)
+    want, _ = scene.expected()
+    for s, length in enumerate(scene.lengths):
+        for cache in (scene.k, scene.v):
+            for token in range(length - 50):
+                cache[scene.table[s, token // 64], :, token % 64] = float("inf") if token % 2 else float("nan")
+    check_attention(scene, attend(engine, scene, "f32"), "f32")
+
+
+def test_strides_of_a_cache_that_holds_keys_and_values_side_by_side(engine):
+    """K and V of a page next to each other, and the layers' pages interleaved: every stride larger than the data."""
+    scene = Scene(11, 4, 2, 128, [3, 1], [90, 33], page_tokens=32)
+    wide = torch.full((scene.pages, 3, 2, 32, 128 + 64), float("nan"), device="cuda", dtype=torch.bfloat16)
+    wide[:, 1, :, :, :128], wide[:, 2, :, :, :128] = scene.k, scene.v
+    paged = S.PagedAttention(engine, 4, 2, 128, scene.pages, page_tokens=32, strides=(wide.stride(0), wide.stride(2), wide.stride(3)), max_sequences=2, max_rows=4, max_context=96)
+    scene.k, scene.v = wide[:, 1], wide[:, 2]
+    check_attention(scene, attend(engine, scene, paged=paged), "bf16")
+
+
+def test_pages_shared_by_sequences(engine):
+    """Two sequences that begin with the same pages read the same tokens."""
+    scene = Scene(21, 4, 2, 128, [1, 1], [64, 70], page_tokens=32)
+    table = scene.table.copy()
+    table[0, :2] = table[1, :2]
+    scene.table = table
+    scene.tokens[0] = tuple(x[:64] for x in scene.tokens[1])
+    check_attention(scene, attend(engine, scene), "bf16")
+
+
+def test_runs_are_equal_to_the_bit_and_streams_do_not_matter(engine):
+    scene = Scene(2, 24, 4, 256, [1, 8, 50], [3000, 777, 50], page_tokens=256)
+    first = attend(engine, scene)
+    again = attend(engine, scene)
+    side = torch.cuda.Stream()
+    other = attend(engine, scene, stream=side.cuda_stream)
+    legacy = attend(engine, scene, stream=0)
+    assert torch.equal(first, again) and torch.equal(first, other) and torch.equal(first, legacy)
+
+
+def test_a_captured_graph_follows_the_batch(engine):
+    """The graph of a decode step, replayed with longer sequences in other pages."""
+    scenes = [Scene(30 + i, 8, 2, 128, [1, 2], lengths, page_tokens=32, spare_pages=40 - sum(-(-n // 32) for n in lengths)) for i, lengths in enumerate(([40, 33], [41, 600], [1, 2]))]
+    paged = S.PagedAttention(engine, 8, 2, 128, 40, page_tokens=32, scale=scenes[0].scale, max_sequences=2, max_rows=3, max_context=700)
+    q, k, v = (torch.empty_like(x) for x in (scenes[0].dq, scenes[0].k, scenes[0].v))
+    out = torch.zeros((3, 8, 128), device="cuda", dtype=torch.bfloat16)
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    paged.batch(scenes[0].rows, scenes[0].lengths, scenes[0].table, stream=stream.cuda_stream)
+    with torch.cuda.graph(graph, stream=stream):
+        paged.attend(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), stream=stream.cuda_stream)
+        with pytest.raises(S.EngineError) as caught:
+            paged.batch(scenes[0].rows, scenes[0].lengths, scenes[0].table, stream=stream.cuda_stream)
+        assert caught.value.case == "invalidArgument" and "capture" in str(caught.value)
+    for scene in scenes:
+        with torch.cuda.stream(stream):
+            q.copy_(scene.dq); k.copy_(scene.k); v.copy_(scene.v)
+            paged.batch(scene.rows, scene.lengths, scene.table, stream=stream.cuda_stream)
+            graph.replay()
+        stream.synchronize()
+        check_attention(scene, out, "bf16")
+
+
+# ---- append --------------------------------------------------------------------------------------
+def expected_append(x, position, rotary, theta, weight, eps):
+    """[rows][heads][head_dim] in 64 bits, and the bound on the 32-bit arithmetic in front of the rounding."""
+    y = x.double()
+    if weight is not None:
+        y = y / torch.sqrt((y * y).mean(-1, keepdim=True) + eps) * weight.double()
+    z, wide = y.clone(), y.abs().clone()
+    half = rotary // 2
+    for i in range(half):
+        angle = position.double() * float(theta) ** (-2.0 * i / rotary)
+        c, s = torch.cos(angle)[:, None], torch.sin(angle)[:, None]
+        z[..., i], z[..., i + half] = y[..., i] * c - y[..., i + half] * s, y[..., i + half] * c + y[..., i] * s
+        wide[..., i] = wide[..., i + half] = y[..., i].abs() + y[..., i + half].abs()
+    # Norm: the sum's relative error is below 16 steps of 2^-24 for 256 terms in eight serial and five tree additions, root, quotient and two products
+    # five more; turn: angle within 2^-23 turns (2^-20 of the values), sine and cosine and three operations a few steps.
+    return z, wide * 2.0 ** -19
+
+
+@pytest.mark.parametrize("heads,kv_heads,head_dim", [(8, 2, 128), (24, 4, 256), (3, 3, 64), (1, 1, 64), (40, 8, 128)])
+@pytest.mark.parametrize("rotary", [0, 2, 6, "quarter", "whole"])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("source,norm,layout", [("f32", True, "head"), ("f32", False, "token"), ("fp16", False, "head"), ("bf16", True, "token")])
+def test_append(engine, heads, kv_heads, head_dim, rotary, dtype, source, norm, layout):
+    rotary = {"quarter": head_dim // 4, "whole": head_dim}.get(rotary, rotary)
+    rows, lengths, page = [1, 0, 5, 20], [200001, 9, 5, 60], 32
+    theta = 1e6
+    seed = heads + head_dim + rotary
+    g = torch.Generator().manual_seed(seed)
+    total, pages = sum(rows), 8
+    table = np.full((4, -(-200001 // page)), 0, np.int32)      # a long sequence whose earlier tokens lie in one page (they are not touched)
+    table[0, 200000 // page] = 5
+    table[1, 0], table[2, 0], table[3, :2] = 6, 1, (4, 2)
+    width = heads + 2 * kv_heads
+    x = torch.randn((total, width + 1, head_dim), generator=g).to(TYPES[source])
+    wq, wk = (1.0 + 0.2 * torch.randn(head_dim, generator=g)).to(torch.bfloat16), (1.0 + 0.2 * torch.randn(head_dim, generator=g)).to(torch.bfloat16)
+    shape = (pages, kv_heads, page, head_dim) if layout == "head" else (pages, page, kv_heads, head_dim)
+    k, v = torch.full(shape, 3.0, device="cuda", dtype=TYPES[dtype]), torch.full(shape, 3.0, device="cuda", dtype=TYPES[dtype])
+    q = torch.full((total + 1, heads, head_dim), 3.0, device="cuda", dtype=TYPES[dtype])
+    dx = x.cuda()
+    paged = S.PagedAttention(engine, heads, kv_heads, head_dim, pages, page_tokens=page, dtype=dtype, layout=layout, rotary_dim=rotary, rope_theta=theta, max_sequences=4, max_rows=total,
+                             max_context=200001)
+    norms = [engine.tensor_vector(bf16_bits(w)) for w in (wq, wk)] if norm else [None, None]
+    torch.cuda.synchronize()
+    paged.batch(rows, lengths, table)
+    size, base = x.element_size(), dx.data_ptr()
+    paged.append(base, base + size * heads * head_dim, base + size * (heads + kv_heads) * head_dim, q.data_ptr(), k.data_ptr(), v.data_ptr(), dtype=source, ld=(width + 1) * head_dim,
+                 q_norm=norms[0], k_norm=norms[1])
+    engine.pass_wait()
+    for t in norms:
+        if t:
+            engine.tensor_destroy(t)
+    sequence = np.repeat(np.arange(4), rows)
+    position = np.concatenate([np.arange(n - r, n) for r, n in zip(rows, lengths)])
+    eps = engine.g.eps
+    want = [expected_append(x[:, a:b], torch.from_numpy(position), r, theta, w if norm and w is not None else None, eps)
+            for a, b, r, w in ((0, heads, rotary, wq), (heads, heads + kv_heads, rotary, wk), (heads + kv_heads, width, 0, None))]
+    kk, vv = (c.cpu() if layout == "head" else c.cpu().transpose(1, 2) for c in (k, v))
+    touched = torch.zeros((pages, page), dtype=torch.bool)
+    page_of, slot_of = table[sequence, position // page], position % page
+    touched[page_of, slot_of] = True
+    got = [q[:total].cpu(), kk[page_of, :, slot_of], vv[page_of, :, slot_of]]
+    for name, g_, (w_, e_) in zip("qkv", got, want):
+        bound = e_ + half_step(dtype) * (w_.abs() + e_) + 2.0 ** -25
+        worst = ((g_.double() - w_).abs() / bound).max().item()
+        assert worst <= 1.0, (name, worst)
+    assert (q[total:] == 3.0).all() and (kk.transpose(1, 2)[~touched] == 3.0).all() and (vv.transpose(1, 2)[~touched] == 3.0).all()
+
+
+def test_refusals(engine):
+    def make(**more):
+        args = dict(heads=4, kv_heads=2, head_dim=128, pages=8, page_tokens=32, max_sequences=2, max_rows=4, max_context=128)
+        args.update(more)
+        return S.PagedAttention(engine, **args)
+    for bad in (dict(head_dim=96), dict(heads=5), dict(heads=130, kv_heads=2), dict(page_tokens=48), dict(page_tokens=512), dict(pages=0), dict(rotary_dim=130), dict(rotary_dim=3), dict(window=-1),
+                dict(dtype="f32"), dict(max_rows=0), dict(max_sequences=0), dict(max_context=0), dict(scale=-1.0), dict(scale=float("nan")), dict(rotary_dim=64, rope_theta=0.0),
+                dict(strides=(8192, 4096, 64)), dict(strides=(8192, 4100, 128)), dict(strides=(4096, 4096, 128)), dict(layout="channel"), dict(dtype="int8")):
+        with pytest.raises(S.EngineError) as caught:
+            make(**bad)
+        assert caught.value.case == "invalidArgument", bad
+    paged = make()
+    buffer = torch.zeros(1 << 16, device="cuda")
+    a = buffer.data_ptr()
+    with pytest.raises(S.EngineError) as caught:
+        paged.attend(a, a, a, a)
+    assert "no batch" in str(caught.value)
+    good = ([1, 1], [33, 20], np.array([[0, 1], [2, 3]], np.int32))
+    paged.batch(*good)
+    for case, rows, lengths, table in (("invalidRows", [2, 1], [1, 20], good[2]), ("invalidRows", [-1, 1], [33, 20], good[2]), ("contextExceeded", [1, 1], [129, 20], np.zeros((2, 5), np.int32)),
+                                       ("invalidRows", [1, 1], [33, 20], np.array([[0, 8], [2, 3]], np.int32)), ("invalidRows", [1, 1], [33, 20], np.array([[0, -1], [2, 3]], np.int32)),
+                                       ("invalidRows", [1, 1], [33, 20], np.array([[0], [2]], np.int32)), ("invalidRows", [0, 0], [33, 20], good[2]), ("invalidRows", [3, 2], [33, 20], good[2]),
+                                       ("invalidRows", [1, 1, 1], [1, 1, 1], np.array([[0], [1], [2]], np.int32))):
+        with pytest.raises(S.EngineError) as caught:
+            paged.batch(rows, lengths, table)
+        assert caught.value.case == case, (rows, lengths)
+    for call in (lambda: paged.attend(a + 8, a, a, a), lambda: paged.attend(a, a + 2, a, a), lambda: paged.attend(a, a, a, a + 4), lambda: paged.attend(a, a, a, a, out_dtype="fp16"),
+                 lambda: paged.append(a + 4, a, a, a, a, a), lambda: paged.append(a, a, a, a, a, a, ld=100), lambda: paged.append(a, a, a, a, a, a, ld=1025), lambda: paged.attend(None, a, a, a)):
+        with pytest.raises(S.EngineError) as caught:
+            call()
+        assert caught.value.case == "invalidArgument"
+    vector = engine.tensor_vector(np.zeros(64, np.uint16))
+    with pytest.raises(S.EngineError):
+        paged.append(a, a, a, a, a, a, q_norm=vector)
+    engine.tensor_destroy(vector)
+    # One page that two sequences would write to: attention may read it, append refuses.
+    paged.batch([1, 1], [33, 20], np.array([[0, 1], [1, 3]], np.int32))
+    with pytest.raises(S.EngineError) as caught:
+        paged.append(a, a, a, a, a, a)
+    assert "one page" in str(caught.value)
+    paged.close()
