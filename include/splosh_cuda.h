@@ -452,6 +452,15 @@ spl_status spl_paged_append(spl_paged *paged, int32_t type, const void *device_q
 /* q [rows][heads][head_dim] of the cache's type; out the same shape, out_type SPL_F32 or the cache's type. Scores, softmax statistics and sums are fp32, a
  * probability is rounded to the cache's type before it meets the values. Buffers begin on 16-byte boundaries. */
 spl_status spl_paged_attend(spl_paged *paged, const void *device_q, const void *device_k_cache, const void *device_v_cache, int32_t out_type, void *device_out, void *stream);
+/* What spl_paged_create and spl_paged_batch would say, without an engine or a GPU (sequences 0: the configuration alone); the reason in
+ * `message`. *shared_write (may be null): append would refuse the batch. */
+spl_status spl_paged_check(const spl_paged_config *config, int32_t sequences, const int32_t *rows, const int32_t *lengths, const int32_t *page_table, int32_t table_ld, int32_t *shared_write,
+                           char *message, size_t message_bytes);
+/* Tests: how a batch's attention is dealt to `blocks` blocks. block_begin[blocks + 1]; items[][8]: sequence, its first row, kv head, first packed query row and their
+ * count, first and last tile of 128 tokens, slot of partial sums (-1: none); merges[blocks][8]: first row, kv head, first packed query row, count, first slot,
+ * slots. Host arithmetic, no device needed. */
+spl_status spl_debug_paged_plan(const spl_paged_config *config, int32_t blocks, int32_t sequences, const int32_t *rows, const int32_t *lengths, int32_t *block_begin, int32_t *items, int32_t items_capacity,
+                                int32_t *item_count, int32_t *merges, int32_t *merge_count);
 
 /* ---- The DFlash 2 block-diffusion drafter (Sources/SploshRuntime/DraftModel.swift) -----------------
  * A draft pass proposes a whole block at once: [anchor, mask x (block - 1)] through a few non-causal layers that attend

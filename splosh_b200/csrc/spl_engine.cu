@@ -733,6 +733,7 @@ spl_status finish_step(spl_engine *e, spl_step_stats *stats) {
         std::memcpy(flag, e->tables_host + e->tables_words, sizeof flag);
         if (flag[0]) {
             cudaMemset(e->tc_error, 0, sizeof flag);
+            if (flag[0] >= 200) return e->fail(SPL_ERR_TIMEOUT, "a paged attention block gave up waiting (warp " + std::to_string(flag[0] - 200) + "; wait " + std::to_string(flag[1]) + ")");
             if (flag[0] >= 100) return e->fail(SPL_ERR_TIMEOUT, "an attention scan block gave up waiting (warp " + std::to_string(flag[0] - 100) + ")");
             // The wait that ran out first: 10 weight copy for a free stage; 20, 21 activation copy for a free tile of means, a free
             // stage; 30-37 tensor-core issue (two warps) for a tile of means, activations, converted weights;
@@ -2118,6 +2119,7 @@ spl_status spl_pass_wait(spl_engine *e) {
     SPL_CUDA(cudaMemcpy(flag, e->tc_error, sizeof flag, cudaMemcpyDeviceToHost));
     if (flag[0]) {
         cudaMemset(e->tc_error, 0, sizeof flag);
+        if (flag[0] >= 200) return e->fail(SPL_ERR_TIMEOUT, "a paged attention block gave up waiting (warp " + std::to_string(flag[0] - 200) + "; wait " + std::to_string(flag[1]) + ")");
         return e->fail(SPL_ERR_TIMEOUT, "a GEMM block of the pass gave up waiting (warp " + std::to_string(flag[0] - 1) + "; first wait " + std::to_string(flag[1]) + ")");
     }
     return SPL_OK;

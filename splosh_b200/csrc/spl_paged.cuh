@@ -10,7 +10,11 @@
 // A batch: sequence s has rows[s] new tokens, the last of its lengths[s]; row r of a pass belongs to sequence row_sequence[r] and
 // sits at position row_position[r]. Token t of sequence s is in page table[s * max_pages + t / page_tokens].
 #pragma once
+#include <cuda.h>
+
+#include "spl_attention.cuh"
 #include "spl_common.cuh"
+#include "spl_paged_plan.h"
 
 struct SplPagedShape {
     int heads, kv_heads, group, head_dim, page_tokens, max_pages;
@@ -20,7 +24,7 @@ struct SplPagedShape {
 };
 // The batch as the kernels read it (device memory).
 struct SplPagedTables {
-    const int *counts;            // rows, sequences
+    const int *counts;            // rows, sequences, merges
     const int *row_sequence, *row_position;
     const int *rows, *lengths;    // per sequence
     const int *table;             // [sequences][max_pages]
@@ -116,50 +120,371 @@ spl_paged_append_kernel(SplPagedRows in, const uint16_t *__restrict__ q_norm, co
 }
 
 // ---- attention --------------------------------------------------------------------------------
-// Tokens that the row at `position` of a sequence of `length` tokens sees: [first, last).
-__host__ __device__ __forceinline__ int spl_paged_first(const SplPagedShape &s, int position) { return s.window > 0 && position + 1 > s.window ? position + 1 - s.window : 0; }
-__host__ __device__ __forceinline__ int spl_paged_last(const SplPagedShape &s, int position, int length) { return s.causal ? position + 1 : length; }
+// o = sum_j p_j v_j / sum_j p_j with p_j = exp(scale q.k_j - m), in one pass over the tokens with a running reference m.
+//
+// A block takes pieces (SplPagedItem) of 128 packed query rows (the new tokens of a sequence times the heads that share a kv head: single
+// tokens, verify blocks and prompt chunks are one kernel) against tiles of 128 tokens. Per tile
+//   S[128 rows x 128 tokens]   = Q[128 x HD] K^T          A = Q, B = K          (shared memory, K-major)
+//   O[128 rows x HD]          += P[128 x 128] V           A = P (tensor memory), B = V (shared memory, tokens along the contraction)
+// with the softmax between them. Keys and values come as chunks of 128 tokens x 64 channels (16 KB, 128-byte swizzle), one ring for both in the
+// order the products take them: K of tile 0; K of tile i + 1, V of tile i; ... A page smaller than a tile is a copy of its own, so page sizes and
+// head layouts are the tensor map's business alone.
+//
+// Warps 0-7 softmax (thread: a row and half of the tile's tokens; the pair of warps of 32 rows agrees on the maximum), warp 8 copies, warp 9 issues
+// both products: S of tile i + 1 runs under the softmax of tile i. The reference is raised only when a row's maximum exceeds it by 2^8, so the sums in
+// tensor memory are rescaled a few times a piece, not every tile. Rows that are not there cost no softmax work.
+// Tensor memory: S / P two buffers of 128 columns (P, 16 bits, over the S it came from), O HD columns from 256.
+//
+// Rounding: P to the cache's type (what the tensor core takes beside V); S, m, the sums of P and O are fp32. In fp16 P is scaled by 2^7 (the factor
+// cancels), so that probabilities down to 2^-21 of the reference keep all bits and one 2^8 above it stays finite.
+//
+// What is masked may be anything: a masked score is replaced before it is used, and because 0 x inf is no number, tokens that no row of the piece
+// sees (behind the sequence's last token, in front of the window) have their values zeroed in shared memory or are left out of the product.
+#define SPL_PAGED_THREADS 320
+#define SPL_PAGED_CHUNK 16384
+#define SPL_PAGED_HEADROOM 8.0f
+__host__ __device__ constexpr int spl_paged_ring(int hd) { return hd == 256 ? 9 : hd == 128 ? 11 : 12; }
+__host__ __device__ constexpr size_t spl_paged_smem_bytes(int hd) {
+    return 1024 + size_t(hd / 64 + spl_paged_ring(hd)) * SPL_PAGED_CHUNK + 2 * 2 * 128 * 4 /* maxima */ + 2 * 128 * 4 /* sums */ + 256 /* barriers */;
+}
 
-// o = sum_j p_j v_j / sum_j p_j, p_j = exp(scale q.k_j - m), one pass with the running maximum m. A warp a (row, head), a lane the
-// channels 64j + 2 lane and the next. Grid (ceil(heads / 4), rows), 128 threads.
-template <bool BF16, bool F32_OUT>
-__global__ void __launch_bounds__(128)
-spl_paged_attend_kernel(const uint16_t *__restrict__ q, const uint16_t *__restrict__ k_cache, const uint16_t *__restrict__ v_cache, SplPagedTables t, SplPagedShape s, void *out) {
-    spl_grid_begin();
-    const int row = blockIdx.y, head = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31, hd = s.head_dim;
-    if (row >= t.counts[0] || head >= s.heads) return;
-    const int sequence = t.row_sequence[row], position = t.row_position[row];
-    const int first = spl_paged_first(s, position), last = spl_paged_last(s, position, t.lengths[sequence]);
-    const int *pages = t.table + size_t(sequence) * s.max_pages;
-    float2 x[4], acc[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        acc[j] = make_float2(0.0f, 0.0f);
-        if (64 * j < hd) x[j] = spl_load_pair<BF16 ? 2 : 1>(q, (size_t(row) * s.heads + head) * hd + 64 * j + 2 * lane);
+// Tokens that the row at `position` of a sequence of `length` tokens sees: [first, last).
+__device__ __forceinline__ int spl_paged_first(const SplPagedShape &s, int position) { return s.window > 0 && position + 1 > s.window ? position + 1 - s.window : 0; }
+__device__ __forceinline__ int spl_paged_last(const SplPagedShape &s, int position, int length) { return s.causal ? position + 1 : length; }
+
+// D[tmem] (+)= A[smem] * B[smem]; one thread issues.
+__device__ __forceinline__ void spl_tc_mma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n"
+                 ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+}
+// The instruction descriptor of spl_tc_idesc for either type; the value product's B has its tokens (the contraction) in rows: MN-major.
+__host__ __device__ constexpr uint32_t spl_paged_idesc(int n, bool bf16, bool b_mn) {
+    return spl_tc_idesc(n) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (b_mn ? 1u << 16 : 0u);
+}
+__device__ __forceinline__ void spl_tc_ld32(uint32_t (&r)[32], uint32_t taddr) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+                 "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+                 "tcgen05.wait::ld.sync.aligned;\n"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+                   "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+                   "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
+                   "=r"(r[31]) : "r"(taddr));
+}
+// A box of a tensor map into shared memory; the innermost coordinate is a multiple of 64 elements.
+__device__ __forceinline__ void spl_tma_load4(void *smem, const CUtensorMap *map, int x, int token, int head, int page, uint64_t *bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];\n"
+                 ::"r"(spl_smem_addr(smem)), "l"(map), "r"(x), "r"(token), "r"(head), "r"(page), "r"(spl_smem_addr(bar)) : "memory");
+}
+// The two warps of 32 rows (w and w + 4): barriers 1 to 4.
+__device__ __forceinline__ void spl_paged_pair_barrier(int quarter) {
+    if (quarter == 0) spl_named_barrier<1, 64>();
+    else if (quarter == 1) spl_named_barrier<2, 64>();
+    else if (quarter == 2) spl_named_barrier<3, 64>();
+    else spl_named_barrier<4, 64>();
+}
+
+struct SplPagedAttend {
+    const uint16_t *q; void *out; int out_f32;
+    const SplPagedItem *items; const int *block_begin;
+    float *partial;              // [slot][slot_rows][HD] sums
+    float2 *partial_ml;          // [slot][slot_rows] reference (log2), sum of p
+    int slot_rows;
+    int *error_flag;
+};
+
+template <int HD, bool BF16>
+__global__ void __launch_bounds__(SPL_PAGED_THREADS, 1)
+spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, SplPagedTables t, SplPagedShape s, SplPagedAttend a) {
+    constexpr int C = HD / 64, NST = spl_paged_ring(HD), CHUNK = SPL_PAGED_CHUNK;
+    constexpr float PBIAS = BF16 ? 0.0f : 7.0f;
+    extern __shared__ unsigned char spl_paged_raw[];
+    unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(spl_paged_raw) + 1023) & ~uintptr_t(1023));
+    unsigned char *q_tile = smem, *ring = q_tile + C * CHUNK;
+    float *xmax = reinterpret_cast<float *>(ring + NST * CHUNK);      // [tile parity][half][row]
+    float *xsum = xmax + 2 * 2 * 128;                                 // [half][row]
+    uint64_t *bars = reinterpret_cast<uint64_t *>(xsum + 2 * 128);
+    uint64_t *full = bars, *empty = full + NST, *s_full = empty + NST, *p_full = s_full + 2, *o_done = p_full + 2, *q_full = o_done + 1, *drained = q_full + 1;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drained + 1);
+    volatile int *abort = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    if (tid == 0) {
+        for (int i = 0; i < NST; ++i) { spl_mbar_init(&full[i], 1); spl_mbar_init(&empty[i], 1); }
+        for (int i = 0; i < 2; ++i) { spl_mbar_init(&s_full[i], 1); spl_mbar_init(&p_full[i], 8); }
+        spl_mbar_init(o_done, 1); spl_mbar_init(q_full, 8); spl_mbar_init(drained, 1);
+        *abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
-    float m = -INFINITY, sum = 0.0f;
-    for (int token = first; token < last; ++token) {
-        const size_t at = size_t(pages[token / s.page_tokens]) * s.page_stride + size_t(head / s.group) * s.head_stride + size_t(token % s.page_tokens) * s.token_stride + 2 * lane;
-        float dot = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) if (64 * j < hd) { const float2 y = spl_load_pair<BF16 ? 2 : 1>(k_cache, at + 64 * j); dot += x[j].x * y.x + x[j].y * y.y; }
-        const float score = spl_warp_sum(dot) * s.scale;
-        if (score > m) {
-            const float f = expf(m - score);
-            m = score; sum *= f;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) { acc[j].x *= f; acc[j].y *= f; }
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(spl_smem_addr(tmem_slot)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+    }
+    spl_tc_fence_before();
+    __syncthreads();
+    spl_tc_fence_after();
+    const uint32_t tmem = *tmem_slot, tmem_o = tmem + 256;
+    spl_grid_begin();
+    const int item0 = a.block_begin[blockIdx.x], item1 = a.block_begin[blockIdx.x + 1];
+    // A role whose wait ran out goes through the rest of its loops without waiting: barriers among warps are met by all of them whatever happened.
+    bool ok = true;
+    auto gave_up = [&](int code) { ok = false; if (!*abort && lane == 0) { spl_note_wait(a.error_flag, code, 0); a.error_flag[0] = 200 + warp; } *abort = 1; };
+
+    if (warp == 8) {
+        // ---- copies. Lane b brings the tile's b-th page (or its half of a page of 256); a chunk's barrier counts the pages that hold tokens.
+        const int box = min(s.page_tokens, 128), boxes = 128 / box;
+        int n = 0;                                            // chunks so far
+        auto bring = [&](const CUtensorMap *map, const SplPagedItem &it, int tile, int page, int present) {
+            for (int c = 0; c < C; ++c, ++n) {
+                const int st = n % NST;
+                if (ok && !spl_mbar_wait_warp(&empty[st], ((n / NST) & 1) ^ 1, const_cast<const int *>(abort))) gave_up(60);
+                if (!ok) return;
+                if (lane == 0) spl_mbar_expect_tx(&full[st], uint32_t(present * box) * 128);
+                __syncwarp();
+                if (lane < present)
+                    spl_tma_load4(ring + st * CHUNK + lane * box * 128, map, c * 64, s.page_tokens > 128 ? (tile & 1) * 128 : 0, it.kv_head, page, &full[st]);
+            }
+        };
+        for (int i = item0; i < item1 && ok; ++i) {
+            const SplPagedItem it = a.items[i];
+            const int length = t.lengths[it.sequence];
+            const int *pages = t.table + size_t(it.sequence) * s.max_pages;
+            auto present_of = [&](int tile) { return min(boxes, (length - tile * 128 + box - 1) / box); };
+            auto page_of = [&](int tile) { return tile < it.tile_end && lane < present_of(tile) ? pages[s.page_tokens > 128 ? tile >> 1 : tile * boxes + lane] : 0; };
+            int page = page_of(it.tile_begin), ahead = page_of(it.tile_begin + 1);
+            bring(&k_map, it, it.tile_begin, page, present_of(it.tile_begin));
+            for (int tile = it.tile_begin; tile < it.tile_end && ok; ++tile) {
+                const int later = page_of(tile + 2);
+                if (tile + 1 < it.tile_end) bring(&k_map, it, tile + 1, ahead, present_of(tile + 1));
+                if (ok) bring(&v_map, it, tile, page, present_of(tile));
+                page = ahead; ahead = later;
+            }
         }
-        const float p = expf(score - m);
-        sum += p;
+        // Nothing may still be on its way into the block's shared memory when it is handed on.
+        for (int st = 0; st < NST && st < n; ++st) { const int last = st + (n - 1 - st) / NST * NST; spl_mbar_wait(&full[st], (last / NST) & 1); }
+    } else if (warp == 9) {
+        // ---- both products, one elected lane of a converged warp.
+        constexpr uint32_t s_idesc = spl_paged_idesc(128, BF16, false), o_idesc = spl_paged_idesc(64, BF16, true);
+        const uint64_t q_desc = spl_tc_desc_sw128(spl_smem_addr(q_tile)), ring_desc = spl_tc_desc_sw128(spl_smem_addr(ring));
+        int n = 0, tiles = 0, pieces = 0;                     // chunks, tiles and pieces so far
+        // Scores of tile number `at` of this block. They go where the P of tile at - 2 lies, which has to have been read (a piece's first tile: all products before
+        // it are over, since its queries are there).
+        auto scores = [&](int at, bool first) {
+            if (ok && !first && at >= 2 && !spl_mbar_wait_warp(o_done, (at - 2) & 1, const_cast<const int *>(abort))) gave_up(61);
+            for (int c = 0; c < C; ++c, ++n) {
+                const int st = n % NST;
+                if (ok && !spl_mbar_wait_warp(&full[st], (n / NST) & 1, const_cast<const int *>(abort))) gave_up(62);
+                if (!ok) return;
+                spl_tc_fence_after();
+                if (spl_elect_one()) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) if (64 * j < hd) { const float2 y = spl_load_pair<BF16 ? 2 : 1>(v_cache, at + 64 * j); acc[j].x += p * y.x; acc[j].y += p * y.y; }
+                    for (int ks = 0; ks < 4; ++ks)
+                        spl_tc_mma_ss(tmem + (at & 1) * 128, q_desc + uint64_t((c * CHUNK + ks * 32) >> 4), ring_desc + uint64_t((st * CHUNK + ks * 32) >> 4), s_idesc, c + ks > 0 ? 1u : 0u);
+                    spl_tc_commit(&empty[st]);
+                    if (c == C - 1) spl_tc_commit(&s_full[at & 1]);
+                }
+                __syncwarp();
+            }
+        };
+        for (int i = item0; i < item1 && ok; ++i, ++pieces) {
+            const SplPagedItem it = a.items[i];
+            const int base = t.lengths[it.sequence] - t.rows[it.sequence];
+            // Tokens that some row of the piece sees.
+            const int seen_first = spl_paged_first(s, base + it.q0 / s.group), seen_last = spl_paged_last(s, base + (it.q0 + it.q_count - 1) / s.group, t.lengths[it.sequence]);
+            if (ok && !spl_mbar_wait_warp(q_full, pieces & 1, const_cast<const int *>(abort))) gave_up(63);
+            if (!ok) break;
+            scores(tiles, true);
+            for (int tile = it.tile_begin; tile < it.tile_end && ok; ++tile, ++tiles) {
+                if (tile + 1 < it.tile_end) scores(tiles + 1, false);
+                if (ok && !spl_mbar_wait_warp(&p_full[tiles & 1], (tiles >> 1) & 1, const_cast<const int *>(abort))) gave_up(64);
+                const int from = max(0, seen_first - tile * 128), to = min(128, seen_last - tile * 128), k0 = from / 16, k1 = (to + 15) / 16;
+                for (int c = 0; c < C && ok; ++c, ++n) {
+                    const int st = n % NST;
+                    if (!spl_mbar_wait_warp(&full[st], (n / NST) & 1, const_cast<const int *>(abort))) { gave_up(65); break; }
+                    if (from % 16 || to % 16) {
+                        // Values of unseen tokens in the first and last groups of sixteen: zero, whatever the cache holds there.
+                        unsigned char *rows = ring + st * CHUNK;
+                        const int before = from % 16 * 8, after = (16 - to % 16) % 16 * 8;
+                        for (int z = lane; z < before + after; z += 32)
+                            *reinterpret_cast<uint4 *>(rows + (z < before ? k0 * 2048 + z * 16 : to * 128 + (z - before) * 16)) = make_uint4(0, 0, 0, 0);
+                        spl_fence_proxy_async();
+                        __syncwarp();
+                    }
+                    spl_tc_fence_after();
+                    if (spl_elect_one()) {
+                        for (int ks = k0; ks < k1; ++ks)
+                            spl_tc_mma_ts(tmem_o + c * 64, tmem + (tiles & 1) * 128 + ks * 8, ring_desc + uint64_t((st * CHUNK + ks * 2048) >> 4), o_idesc, tile > it.tile_begin || ks > k0 ? 1u : 0u);
+                        spl_tc_commit(&empty[st]);
+                        if (c == C - 1) spl_tc_commit(o_done);
+                    }
+                    __syncwarp();
+                }
+            }
+        }
+        // No product may still read shared or write tensor memory when they are handed on.
+        if (spl_elect_one()) spl_tc_commit(drained);
+        __syncwarp();
+        spl_mbar_wait(drained, 0);
+    } else {
+        // ---- softmax: row r of the piece, tokens [64 half, 64 half + 64) of a tile.
+        const int quarter = warp & 3, half = warp >> 2, r = quarter * 32 + lane;
+        const uint32_t lanes = uint32_t(quarter * 32) << 16;
+        const float c = s.scale * 1.4426950408889634f;
+        int tiles = 0;
+        for (int i = item0; i < item1; ++i) {
+            const SplPagedItem it = a.items[i];
+            const int length = t.lengths[it.sequence], base = length - t.rows[it.sequence];
+            const bool busy = quarter * 32 < it.q_count;             // whether this warp's rows hold a query
+            // Queries into the swizzled operand tile, zero where there is none: 16-byte pieces of eight channels.
+            for (int idx = tid; idx < 128 * (HD / 8); idx += 256) {
+                const int m = idx / (HD / 8), piece = idx % (HD / 8), packed = it.q0 + m;
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (m < it.q_count)
+                    v = *reinterpret_cast<const uint4 *>(a.q + (size_t(it.row0 + packed / s.group) * s.heads + it.kv_head * s.group + packed % s.group) * HD + piece * 8);
+                *reinterpret_cast<uint4 *>(q_tile + (piece >> 3) * CHUNK + spl_sw128_offset(m, (piece & 7) * 8)) = v;
+            }
+            spl_fence_proxy_async();
+            spl_tc_fence_before();
+            __syncwarp();
+            if (lane == 0) spl_mbar_arrive(q_full);
+            const int position = base + (it.q0 + min(r, it.q_count - 1)) / s.group;
+            const int first = spl_paged_first(s, position), last = spl_paged_last(s, position, length);
+            float ref = -INFINITY, sum = 0.0f;
+            for (int tile = it.tile_begin; tile < it.tile_end; ++tile, ++tiles) {
+                const int buf = tiles & 1;
+                if (ok && !spl_mbar_wait_warp(&s_full[buf], (tiles >> 1) & 1, const_cast<const int *>(abort))) gave_up(66);
+                if (busy) {
+                    spl_tc_fence_after();
+                    const uint32_t at = tmem + lanes + buf * 128;
+                    uint32_t x0[32], x1[32];
+                    spl_tc_ld32(x0, at + half * 64);
+                    spl_tc_ld32(x1, at + half * 64 + 32);
+                    const int t0 = tile * 128 + half * 64;
+                    // Masked scores are -inf; a tile that all rows see whole has none.
+                    if (__any_sync(0xffffffffu, t0 < first || t0 + 64 > last)) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            if (t0 + j < first || t0 + j >= last) x0[j] = 0xff800000u;
+                            if (t0 + 32 + j < first || t0 + 32 + j >= last) x1[j] = 0xff800000u;
+                        }
+                    }
+                    float m = -INFINITY;
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) m = fmaxf(m, fmaxf(__uint_as_float(x0[j]), __uint_as_float(x1[j])));
+                    xmax[(buf * 2 + half) * 128 + r] = m;
+                    spl_paged_pair_barrier(quarter);
+                    m = fmaxf(m, xmax[(buf * 2 + (half ^ 1)) * 128 + r]) * c;
+                    const bool raise = m > ref + SPL_PAGED_HEADROOM;
+                    if (__any_sync(0xffffffffu, raise)) {
+                        const float factor = raise ? exp2f(ref - m) : 1.0f;
+                        if (tile > it.tile_begin) {
+                            // The product before has to be done with these sums; the next waits for this warp's probabilities.
+                            if (ok && !spl_mbar_wait_warp(o_done, (tiles - 1) & 1, const_cast<const int *>(abort))) gave_up(67);
+                            spl_tc_fence_after();
+#pragma unroll 1
+                            for (int o = 0; o < HD / 2; o += 16) {
+                                uint32_t y[16];
+                                spl_tc_ld16(y, tmem_o + lanes + half * (HD / 2) + o);
+#pragma unroll
+                                for (int j = 0; j < 16; ++j) y[j] = __float_as_uint(__uint_as_float(y[j]) * factor);
+                                spl_tc_st16(tmem_o + lanes + half * (HD / 2) + o, y);
+                            }
+                        }
+                        if (raise) { sum *= factor; ref = m; }
+                    }
+                    const float offset = (ref == -INFINITY ? 0.0f : -ref) + PBIAS;      // a row that has seen nothing yet: all its scores are -inf
+                    float part = 0.0f;
+                    uint32_t p[32];
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        const float p0 = spl_ex2(fmaf(__uint_as_float(x0[2 * j]), c, offset)), p1 = spl_ex2(fmaf(__uint_as_float(x0[2 * j + 1]), c, offset));
+                        const float p2 = spl_ex2(fmaf(__uint_as_float(x1[2 * j]), c, offset)), p3 = spl_ex2(fmaf(__uint_as_float(x1[2 * j + 1]), c, offset));
+                        part += (p0 + p1) + (p2 + p3);
+                        p[j] = spl_pack16<BF16>(p0, p1); p[16 + j] = spl_pack16<BF16>(p2, p3);
+                    }
+                    sum += part;
+                    spl_tc_st32(at + half * 32, p);
+                    spl_tc_st_wait();
+                    spl_tc_fence_before();
+                }
+                __syncwarp();
+                if (lane == 0) spl_mbar_arrive(&p_full[buf]);
+            }
+            // The piece's sums.
+            if (ok && !spl_mbar_wait_warp(o_done, (tiles - 1) & 1, const_cast<const int *>(abort))) gave_up(68);
+            if (busy) {
+                spl_tc_fence_after();
+                xsum[half * 128 + r] = sum;
+                spl_paged_pair_barrier(quarter);
+                sum += xsum[(half ^ 1) * 128 + r];
+                const bool here = r < it.q_count;
+                const int packed = it.q0 + r;
+                const size_t place = (size_t(it.row0 + packed / s.group) * s.heads + it.kv_head * s.group + packed % s.group) * HD + half * (HD / 2);
+                const size_t slot_row = size_t(it.slot) * a.slot_rows + r;
+                const float inv = it.slot < 0 ? 1.0f / sum : 1.0f;
+#pragma unroll 1
+                for (int o = 0; o < HD / 2; o += 16) {
+                    uint32_t y[16];
+                    spl_tc_ld16(y, tmem_o + lanes + half * (HD / 2) + o);
+                    if (!here) continue;
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) y[j] = __float_as_uint(__uint_as_float(y[j]) * inv);
+                    if (it.slot >= 0 || a.out_f32) {
+                        float *dst = it.slot >= 0 ? a.partial + slot_row * HD + half * (HD / 2) + o : static_cast<float *>(a.out) + place + o;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4 *>(dst + 4 * j) = make_uint4(y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]);
+                    } else {
+                        uint32_t w[8];
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) w[j] = spl_pack16<BF16>(__uint_as_float(y[2 * j]), __uint_as_float(y[2 * j + 1]));
+                        uint4 *dst = reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.out) + place + o);
+                        dst[0] = make_uint4(w[0], w[1], w[2], w[3]); dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
+                    }
+                }
+                if (here && it.slot >= 0 && half == 0) a.partial_ml[slot_row] = make_float2(ref, sum);
+                spl_paged_pair_barrier(quarter);              // the sums in shared memory are read before the next piece's
+            }
+        }
+    }
+    spl_tc_fence_before();
+    __syncthreads();
+    spl_tc_fence_after();
+    if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512) : "memory");
+}
+
+// The pieces of a tile of query rows joined: o = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s. Grid (blocks of the attention, row groups of eight), 256 threads: a warp a row.
+template <int HD, bool BF16>
+__global__ void __launch_bounds__(256)
+spl_paged_merge_kernel(const int *__restrict__ counts, const SplPagedMerge *__restrict__ merges, SplPagedShape s, const float *__restrict__ partial, const float2 *__restrict__ partial_ml,
+                       int slot_rows, void *out, int out_f32) {
+    spl_grid_begin();
+    if (int(blockIdx.x) >= counts[2]) return;
+    const SplPagedMerge mg = merges[blockIdx.x];
+    const int r = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (r >= mg.q_count) return;
+    float m = -INFINITY;
+    for (int n = 0; n < mg.slots; ++n) m = fmaxf(m, partial_ml[size_t(mg.slot + n) * slot_rows + r].x);
+    float2 acc[HD / 64];
+    float sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < HD / 64; ++j) acc[j] = make_float2(0.0f, 0.0f);
+    for (int n = 0; n < mg.slots; ++n) {
+        const size_t row = size_t(mg.slot + n) * slot_rows + r;
+        const float2 ml = partial_ml[row];
+        if (ml.x == -INFINITY) continue;                      // a piece of whose tokens this row sees none
+        const float f = exp2f(ml.x - m);
+        sum += f * ml.y;
+#pragma unroll
+        for (int j = 0; j < HD / 64; ++j) {
+            const float2 v = *reinterpret_cast<const float2 *>(partial + row * HD + 64 * j + 2 * lane);
+            acc[j].x += f * v.x; acc[j].y += f * v.y;
+        }
     }
     const float inv = 1.0f / sum;
+    const int packed = mg.q0 + r;
+    const size_t place = (size_t(mg.row0 + packed / s.group) * s.heads + mg.kv_head * s.group + packed % s.group) * HD;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) if (64 * j < hd) {
-        const size_t at = (size_t(row) * s.heads + head) * hd + 64 * j + 2 * lane;
-        if constexpr (F32_OUT) *reinterpret_cast<float2 *>(static_cast<float *>(out) + at) = make_float2(acc[j].x * inv, acc[j].y * inv);
-        else *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(out) + at) = spl_pack16<BF16>(acc[j].x * inv, acc[j].y * inv);
+    for (int j = 0; j < HD / 64; ++j) {
+        if (out_f32) *reinterpret_cast<float2 *>(static_cast<float *>(out) + place + 64 * j + 2 * lane) = make_float2(acc[j].x * inv, acc[j].y * inv);
+        else *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(out) + place + 64 * j + 2 * lane) = spl_pack16<BF16>(acc[j].x * inv, acc[j].y * inv);
     }
 }

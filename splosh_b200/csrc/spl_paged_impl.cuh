@@ -14,13 +14,23 @@ struct SplDeviceScope {
     ~SplDeviceScope() { if (before >= 0) cudaSetDevice(before); }
 };
 
+typedef CUresult (*SplEncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
 struct spl_paged {
     spl_engine *e = nullptr;
     spl_paged_config c;
     SplPagedShape shape{};
     int max_pages = 0;
-    // Device tables in one block, filled by one copy from one of two pinned blocks (the other may still be on its way).
-    size_t words = 0;
+    SplEncodeTiled encode = nullptr;
+    // Device tables in one block, filled from one of two pinned blocks (the other's copy may still be on its way): counts, block_begin, merges and items of
+    // the attention's plan; then the batch. Places do not depend on the batch, so a captured graph finds the next one's.
+    size_t words = 0, begin_at = 16, merges_at = 0, items_at = 0, batch_at = 0;
+    SplPagedPlan plan;
+    // Partial sums of query rows whose tokens several blocks share.
+    int slot_rows = 0;
+    float *partial = nullptr;
+    float2 *partial_ml = nullptr;
     int *tables_dev = nullptr, *tables_host[2] = {};
     cudaEvent_t copied[2] = {};
     int turn = 0;
@@ -31,9 +41,9 @@ struct spl_paged {
     std::vector<uint8_t> written;      // scratch of the check for pages that two sequences would write
 
     SplPagedTables tables() const {
-        const int *t = tables_dev;
+        const int *t = tables_dev + batch_at;
         SplPagedTables out;
-        out.counts = t; t += 16;
+        out.counts = tables_dev;
         out.row_sequence = t; t += c.max_rows; out.row_position = t; t += c.max_rows;
         out.rows = t; t += c.max_sequences; out.lengths = t; t += c.max_sequences;
         out.table = t;
@@ -41,36 +51,42 @@ struct spl_paged {
     }
 };
 
+template <int HD> static bool paged_configure_dim() {
+    const int bytes = int(spl_paged_smem_bytes(HD));
+    return cudaFuncSetAttribute(spl_paged_attend_kernel<HD, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess &&
+           cudaFuncSetAttribute(spl_paged_attend_kernel<HD, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess;
+}
+// (The opt-in is a property of the current device.)
+static bool paged_configure(int head_dim) { return head_dim == 64 ? paged_configure_dim<64>() : head_dim == 128 ? paged_configure_dim<128>() : paged_configure_dim<256>(); }
+
 static spl_status paged_create(spl_engine *e, const spl_paged_config *cp, spl_paged *p) {
     const spl_paged_config &c = p->c = *cp;
-    auto refuse = [&](const char *text) { return e->fail(SPL_ERR_INVALID_ARGUMENT, std::string("spl_paged_create: ") + text); };
-    if (c.head_dim != 64 && c.head_dim != 128 && c.head_dim != 256) return refuse("heads are 64, 128 or 256 channels wide");
-    if (c.heads < 1 || c.kv_heads < 1 || c.heads % c.kv_heads || c.heads > 1024 || c.heads / c.kv_heads > 64) return refuse("heads must be a multiple of kv_heads, at most 1024 and 64 a kv head");
-    if (c.dtype != SPL_F16 && c.dtype != SPL_BF16) return refuse("the cache holds fp16 or bf16");
-    if (c.page_tokens != 16 && c.page_tokens != 32 && c.page_tokens != 64 && c.page_tokens != 128 && c.page_tokens != 256) return refuse("pages hold 16, 32, 64, 128 or 256 tokens");
-    if (c.pages < 1) return refuse("no pages");
-    const int64_t d = c.head_dim, ps = c.page_stride, hs = c.head_stride, ts = c.token_stride;
-    if (ps % 8 || hs % 8 || ts % 8) return refuse("strides must be multiples of 8 elements");
-    const bool token_inside = ts >= d && hs >= ts * c.page_tokens && ps >= hs * c.kv_heads, head_inside = hs >= d && ts >= hs * c.kv_heads && ps >= ts * c.page_tokens;
-    if (!token_inside && !head_inside) return refuse("strides must be those of [page][kv head][token][channel] or [page][token][kv head][channel], rows not overlapping");
-    if (ps > (int64_t(1) << 38) || ps > (int64_t(1) << 60) / c.pages) return refuse("the cache is too large");
-    if (c.rotary_dim < 0 || c.rotary_dim > c.head_dim || c.rotary_dim % 2) return refuse("rotary_dim must be even and at most head_dim");
-    if (c.rotary_dim && !(c.rope_theta > 0.0f && std::isfinite(c.rope_theta))) return refuse("rope_theta must be positive");
-    if (!(c.scale >= 0.0f) || !std::isfinite(c.scale)) return refuse("scale must be positive, or 0 for 1 / sqrt(head_dim)");
-    if (c.window < 0) return refuse("window must be 0 (none) or a number of tokens");
-    if (c.max_sequences < 1 || c.max_rows < 1 || c.max_context < 1 || c.max_context > (1 << 30) || c.max_rows > (1 << 20) || c.max_sequences > (1 << 16)) return refuse("max_sequences, max_rows or max_context out of range");
+    if (const char *wrong = spl_paged_config_error(c)) return e->fail(SPL_ERR_INVALID_ARGUMENT, std::string("spl_paged_create: ") + wrong);
     p->max_pages = (c.max_context + c.page_tokens - 1) / c.page_tokens;
-    if (int64_t(p->max_pages) * c.max_sequences > (int64_t(1) << 28)) return refuse("the page table is too large");
     p->e = e;
-    p->shape = SplPagedShape{c.heads, c.kv_heads, c.heads / c.kv_heads, c.head_dim, c.page_tokens, p->max_pages, ps, hs, ts, c.rotary_dim, c.causal != 0, c.window,
+    p->shape = SplPagedShape{c.heads, c.kv_heads, c.heads / c.kv_heads, c.head_dim, c.page_tokens, p->max_pages, c.page_stride, c.head_stride, c.token_stride, c.rotary_dim, c.causal != 0, c.window,
                              c.scale > 0.0f ? c.scale : float(1.0 / std::sqrt(double(c.head_dim)))};
-    p->words = 16 + size_t(c.max_rows) * 2 + size_t(c.max_sequences) * 2 + size_t(p->max_pages) * c.max_sequences;
+    const size_t blocks = size_t(e->sms), items = size_t(spl_paged_items_max(c, e->sms));
+    p->merges_at = p->begin_at + (blocks + 1 + 3) / 4 * 4;
+    p->items_at = p->merges_at + blocks * (sizeof(SplPagedMerge) / 4);
+    p->batch_at = p->items_at + items * (sizeof(SplPagedItem) / 4);
+    p->words = p->batch_at + size_t(c.max_rows) * 2 + size_t(c.max_sequences) * 2 + size_t(p->max_pages) * c.max_sequences;
     p->written.assign(size_t(c.pages), 0);
     SPL_CUDA(cudaMalloc(reinterpret_cast<void **>(&p->tables_dev), p->words * 4));
     for (int i = 0; i < 2; ++i) {
         SPL_CUDA(cudaMallocHost(reinterpret_cast<void **>(&p->tables_host[i]), p->words * 4));
         SPL_CUDA(cudaEventCreateWithFlags(&p->copied[i], cudaEventDisableTiming));
     }
+    p->slot_rows = int(std::min<int64_t>(SPL_PAGED_TILE, int64_t(c.max_rows) * p->shape.group));
+    const size_t slot_rows = size_t(spl_paged_slots_max(e->sms)) * p->slot_rows;
+    SPL_CUDA(cudaMalloc(reinterpret_cast<void **>(&p->partial), slot_rows * c.head_dim * 4));
+    SPL_CUDA(cudaMalloc(reinterpret_cast<void **>(&p->partial_ml), slot_rows * sizeof(float2)));
+    cudaDriverEntryPointQueryResult found;
+    void *encode = nullptr;
+    SPL_CUDA(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &encode, 12000, cudaEnableDefault, &found));
+    if (found != cudaDriverEntryPointSuccess || !encode) return e->fail(SPL_ERR_UNSUPPORTED_DEVICE, "spl_paged_create: the driver has no tensor maps");
+    p->encode = reinterpret_cast<SplEncodeTiled>(encode);
+    if (!paged_configure(c.head_dim)) return e->fail(SPL_ERR_UNSUPPORTED_DEVICE, "spl_paged_create: the kernel's shared-memory opt-in failed");
     std::vector<double> turns(size_t(std::max(1, c.rotary_dim / 2)), 0.0);
     for (int i = 0; i < c.rotary_dim / 2; ++i) turns[i] = std::pow(double(c.rope_theta), -2.0 * i / c.rotary_dim) / 6.283185307179586476925;
     SPL_CUDA(cudaMalloc(reinterpret_cast<void **>(&p->turns), turns.size() * 8));
@@ -79,7 +95,7 @@ static spl_status paged_create(spl_engine *e, const spl_paged_config *cp, spl_pa
 }
 
 static void paged_release(spl_paged *p) {
-    cudaFree(p->tables_dev); cudaFree(p->turns);
+    cudaFree(p->tables_dev); cudaFree(p->turns); cudaFree(p->partial); cudaFree(p->partial_ml);
     for (int i = 0; i < 2; ++i) { if (p->tables_host[i]) cudaFreeHost(p->tables_host[i]); if (p->copied[i]) cudaEventDestroy(p->copied[i]); }
     delete p;
 }
@@ -89,46 +105,34 @@ static cudaStream_t paged_stream(const spl_engine *e, void *stream) { return str
 static spl_status paged_batch(spl_paged *p, int32_t sequences, const int32_t *rows, const int32_t *lengths, const int32_t *table, int32_t table_ld, cudaStream_t stream) {
     spl_engine *e = p->e;
     const spl_paged_config &c = p->c;
-    auto refuse = [&](spl_status s, const std::string &text) { return e->fail(s, "spl_paged_batch: " + text); };
-    if (sequences < 1 || sequences > c.max_sequences) return refuse(SPL_ERR_INVALID_ROWS, "the number of sequences is outside the limit");
-    int64_t total = 0;
-    for (int s = 0; s < sequences; ++s) {
-        if (rows[s] < 0 || lengths[s] < rows[s]) return refuse(SPL_ERR_INVALID_ROWS, "sequence " + std::to_string(s) + " has more new rows than tokens");
-        if (lengths[s] > c.max_context) return refuse(SPL_ERR_CONTEXT_EXCEEDED, "sequence " + std::to_string(s) + " is longer than max_context");
-        total += rows[s];
-        const int used = (lengths[s] + c.page_tokens - 1) / c.page_tokens;
-        if (used > table_ld) return refuse(SPL_ERR_INVALID_ROWS, "sequence " + std::to_string(s) + " has more pages than the table's rows");
-        for (int i = 0; i < used; ++i) {
-            const int page = table[size_t(s) * table_ld + i];
-            if (page < 0 || page >= c.pages) return refuse(SPL_ERR_INVALID_ROWS, "page " + std::to_string(i) + " of sequence " + std::to_string(s) + " is not a page of the cache");
-        }
-    }
-    if (total < 1 || total > c.max_rows) return refuse(SPL_ERR_INVALID_ROWS, "the number of rows is outside the limit");
+    std::string why;
+    bool shared = false;
+    const spl_status taken = spl_paged_batch_check(c, sequences, rows, lengths, table, table_ld, p->written, &shared, &why);
+    if (taken != SPL_OK) return e->fail(taken, "spl_paged_batch: " + why);
     cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
     SPL_CUDA(cudaStreamIsCapturing(stream, &capture));
-    if (capture != cudaStreamCaptureStatusNone) return refuse(SPL_ERR_INVALID_ARGUMENT, "a batch is set outside a capture");
-    // Pages that two sequences would write to (or one twice): append refuses such a batch.
-    bool shared = false;
-    auto each_written = [&](auto &&visit) {
-        for (int s = 0; s < sequences; ++s)
-            if (rows[s]) for (int i = (lengths[s] - rows[s]) / c.page_tokens; i <= (lengths[s] - 1) / c.page_tokens; ++i) visit(table[size_t(s) * table_ld + i]);
-    };
-    each_written([&](int page) { shared = shared || p->written[page]; p->written[page] = 1; });
-    each_written([&](int page) { p->written[page] = 0; });
+    if (capture != cudaStreamCaptureStatusNone) return e->fail(SPL_ERR_INVALID_ARGUMENT, "spl_paged_batch: a batch is set outside a capture");
+    int64_t total = 0;
+    for (int s = 0; s < sequences; ++s) total += rows[s];
+    spl_paged_plan(c, e->sms, sequences, rows, lengths, p->plan);
     const int turn = p->turn;
     SPL_CUDA(cudaEventSynchronize(p->copied[turn]));      // this block's last copy
     int *w = p->tables_host[turn];
     std::memset(w, 0, 16 * 4);
-    w[0] = int(total); w[1] = sequences;
-    int *row_sequence = w + 16, *row_position = row_sequence + c.max_rows, *seq_rows = row_position + c.max_rows, *seq_lengths = seq_rows + c.max_sequences, *pages = seq_lengths + c.max_sequences;
+    w[0] = int(total); w[1] = sequences; w[2] = int(p->plan.merges.size());
+    std::memcpy(w + p->begin_at, p->plan.block_begin.data(), p->plan.block_begin.size() * 4);
+    if (!p->plan.merges.empty()) std::memcpy(w + p->merges_at, p->plan.merges.data(), p->plan.merges.size() * sizeof(SplPagedMerge));
+    std::memcpy(w + p->items_at, p->plan.items.data(), p->plan.items.size() * sizeof(SplPagedItem));
+    int *row_sequence = w + p->batch_at, *row_position = row_sequence + c.max_rows, *seq_rows = row_position + c.max_rows, *seq_lengths = seq_rows + c.max_sequences, *pages = seq_lengths + c.max_sequences;
     for (int s = 0, r = 0; s < sequences; ++s) {
         for (int i = 0; i < rows[s]; ++i, ++r) { row_sequence[r] = s; row_position[r] = lengths[s] - rows[s] + i; }
         seq_rows[s] = rows[s]; seq_lengths[s] = lengths[s];
         const int used = (lengths[s] + c.page_tokens - 1) / c.page_tokens;
         if (used) std::memcpy(pages + size_t(s) * p->max_pages, table + size_t(s) * table_ld, size_t(used) * 4);
     }
-    const size_t used_words = size_t(pages - w) + size_t(sequences) * p->max_pages;
-    SPL_CUDA(cudaMemcpyAsync(p->tables_dev, w, used_words * 4, cudaMemcpyHostToDevice, stream));
+    const size_t planned = p->items_at + p->plan.items.size() * (sizeof(SplPagedItem) / 4), used = size_t(pages - w) + size_t(sequences) * p->max_pages - p->batch_at;
+    SPL_CUDA(cudaMemcpyAsync(p->tables_dev, w, planned * 4, cudaMemcpyHostToDevice, stream));
+    SPL_CUDA(cudaMemcpyAsync(p->tables_dev + p->batch_at, w + p->batch_at, used * 4, cudaMemcpyHostToDevice, stream));
     SPL_CUDA(cudaEventRecord(p->copied[turn], stream));
     p->turn ^= 1;
     p->rows = int(total); p->sequences = sequences; p->shared_write = shared; p->ready = true;
@@ -143,6 +147,23 @@ template <int TYPE> static void launch_append(const spl_paged *p, const SplPaged
         launch_step(spl_paged_append_kernel<TYPE, true>, grid, dim3(256), 0, stream, in, q_norm, k_norm, (const double *)p->turns, p->tables(), p->shape, p->e->g.eps, q, k, v);
     else
         launch_step(spl_paged_append_kernel<TYPE, false>, grid, dim3(256), 0, stream, in, q_norm, k_norm, (const double *)p->turns, p->tables(), p->shape, p->e->g.eps, q, k, v);
+}
+
+// The cache as a tensor (channel, token in page, kv head, page) in boxes of 64 channels by a page's tokens (at most a tile's).
+static bool paged_map(const spl_paged *p, const void *cache, CUtensorMap *map) {
+    const spl_paged_config &c = p->c;
+    const cuuint64_t dims[4] = {cuuint64_t(c.head_dim), cuuint64_t(c.page_tokens), cuuint64_t(c.kv_heads), cuuint64_t(c.pages)};
+    const cuuint64_t strides[3] = {cuuint64_t(c.token_stride) * 2, cuuint64_t(c.head_stride) * 2, cuuint64_t(c.page_stride) * 2};
+    const cuuint32_t box[4] = {64, cuuint32_t(std::min(c.page_tokens, SPL_PAGED_TILE)), 1, 1}, steps[4] = {1, 1, 1, 1};
+    return p->encode(map, c.dtype == SPL_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void *>(cache), dims, strides, box, steps,
+                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int HD, bool BF16> static void launch_attend(const spl_paged *p, const CUtensorMap &k_map, const CUtensorMap &v_map, const SplPagedAttend &a, cudaStream_t stream) {
+    launch_step(spl_paged_attend_kernel<HD, BF16>, dim3(p->e->sms), dim3(SPL_PAGED_THREADS), spl_paged_smem_bytes(HD), stream, k_map, v_map, p->tables(), p->shape, a);
+    // Always launched: a captured graph's next batch may have pieces to join where this one has none.
+    launch_step(spl_paged_merge_kernel<HD, BF16>, dim3(p->e->sms, (p->slot_rows + 7) / 8), dim3(256), 0, stream, (const int *)p->tables_dev,
+                reinterpret_cast<const SplPagedMerge *>(p->tables_dev + p->merges_at), p->shape, (const float *)p->partial, (const float2 *)p->partial_ml, p->slot_rows, a.out, a.out_f32);
 }
 
 static bool misaligned(const void *p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes != 0; }
@@ -214,16 +235,15 @@ spl_status spl_paged_attend(spl_paged *p, const void *device_q, const void *devi
     if (out_type != SPL_F32 && out_type != c.dtype) return refuse("outputs are fp32 or of the cache's type");
     if (misaligned(device_q, 16) || misaligned(device_k_cache, 16) || misaligned(device_v_cache, 16) || misaligned(device_out, 16)) return refuse("all buffers begin on a 16-byte boundary");
     const SplDeviceScope scope(e->device);
-    const dim3 grid((c.heads + 3) / 4, p->rows);
-    const uint16_t *q = static_cast<const uint16_t *>(device_q), *k = static_cast<const uint16_t *>(device_k_cache), *v = static_cast<const uint16_t *>(device_v_cache);
+    CUtensorMap k_map, v_map;
+    if (!paged_map(p, device_k_cache, &k_map) || !paged_map(p, device_v_cache, &v_map)) return refuse("the driver takes no tensor map of this cache");
+    const SplPagedAttend a{static_cast<const uint16_t *>(device_q), device_out, out_type == SPL_F32, reinterpret_cast<const SplPagedItem *>(p->tables_dev + p->items_at), p->tables_dev + p->begin_at,
+                           p->partial, p->partial_ml, p->slot_rows, e->tc_error};
     cudaStream_t st = paged_stream(e, stream);
-    if (c.dtype == SPL_BF16) {
-        if (out_type == SPL_F32) launch_step(spl_paged_attend_kernel<true, true>, grid, dim3(128), 0, st, q, k, v, p->tables(), p->shape, device_out);
-        else launch_step(spl_paged_attend_kernel<true, false>, grid, dim3(128), 0, st, q, k, v, p->tables(), p->shape, device_out);
-    } else {
-        if (out_type == SPL_F32) launch_step(spl_paged_attend_kernel<false, true>, grid, dim3(128), 0, st, q, k, v, p->tables(), p->shape, device_out);
-        else launch_step(spl_paged_attend_kernel<false, false>, grid, dim3(128), 0, st, q, k, v, p->tables(), p->shape, device_out);
-    }
+    const bool bf16 = c.dtype == SPL_BF16;
+    if (c.head_dim == 64) { if (bf16) launch_attend<64, true>(p, k_map, v_map, a, st); else launch_attend<64, false>(p, k_map, v_map, a, st); }
+    else if (c.head_dim == 128) { if (bf16) launch_attend<128, true>(p, k_map, v_map, a, st); else launch_attend<128, false>(p, k_map, v_map, a, st); }
+    else { if (bf16) launch_attend<256, true>(p, k_map, v_map, a, st); else launch_attend<256, false>(p, k_map, v_map, a, st); }
     return check_launch(e, "spl_paged_attend");
 }
 
@@ -261,6 +281,40 @@ spl_status spl_sample(spl_engine *e, int32_t vocab_limit, const spl_sampling *se
     SPL_CUDA(cudaStreamSynchronize(e->stream));
     std::memcpy(ids, e->topk_host + 5 * rows, size_t(rows) * 4);
     return SPL_OK;
+}
+
+// Host arithmetic, no device needed.
+spl_status spl_paged_check(const spl_paged_config *config, int32_t sequences, const int32_t *rows, const int32_t *lengths, const int32_t *page_table, int32_t table_ld, int32_t *shared_write,
+                           char *message, size_t message_bytes) {
+    if (!config || (sequences && (!rows || !lengths || !page_table)) || table_ld < 0) return SPL_ERR_INVALID_ARGUMENT;
+    auto say = [&](const std::string &text) { if (message && message_bytes) { const size_t n = std::min(message_bytes - 1, text.size()); std::memcpy(message, text.data(), n); message[n] = 0; } };
+    say("");
+    try {
+        if (const char *wrong = spl_paged_config_error(*config)) { say(wrong); return SPL_ERR_INVALID_ARGUMENT; }
+        if (!sequences) return SPL_OK;
+        std::vector<uint8_t> written;
+        std::string why;
+        bool shared = false;
+        const spl_status s = spl_paged_batch_check(*config, sequences, rows, lengths, page_table, table_ld, written, &shared, &why);
+        say(why);
+        if (s == SPL_OK && shared_write) *shared_write = shared;
+        return s;
+    } catch (const std::bad_alloc &) { return SPL_ERR_ALLOCATION_FAILED; }
+}
+
+spl_status spl_debug_paged_plan(const spl_paged_config *config, int32_t blocks, int32_t sequences, const int32_t *rows, const int32_t *lengths, int32_t *block_begin, int32_t *items, int32_t items_capacity,
+                                int32_t *item_count, int32_t *merges, int32_t *merge_count) {
+    if (!config || !rows || !lengths || !block_begin || !items || !item_count || !merges || !merge_count || blocks < 1 || sequences < 1 || spl_paged_config_error(*config)) return SPL_ERR_INVALID_ARGUMENT;
+    try {
+        SplPagedPlan plan;
+        spl_paged_plan(*config, blocks, sequences, rows, lengths, plan);
+        if (plan.items.size() > size_t(std::max(items_capacity, 0)) || plan.merges.size() > size_t(blocks)) return SPL_ERR_ALLOCATION_FAILED;
+        std::memcpy(block_begin, plan.block_begin.data(), plan.block_begin.size() * 4);
+        std::memcpy(items, plan.items.data(), plan.items.size() * sizeof(SplPagedItem));
+        if (!plan.merges.empty()) std::memcpy(merges, plan.merges.data(), plan.merges.size() * sizeof(SplPagedMerge));
+        *item_count = int32_t(plan.items.size()); *merge_count = int32_t(plan.merges.size());
+        return SPL_OK;
+    } catch (const std::bad_alloc &) { return SPL_ERR_ALLOCATION_FAILED; }
 }
 
 }  // extern "C"

@@ -1,0 +1,147 @@
+// spl_paged_plan.h — the host arithmetic of the paged cache: which configurations and batches are taken, and how a batch's attention
+// is dealt to the blocks of a launch. No device needed.
+#pragma once
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <string>
+#include <vector>
+
+#include "../../include/splosh_cuda.h"
+
+#define SPL_PAGED_TILE 128            // tokens a tile; packed query rows a block
+
+// A block's piece of work: packed query rows [q0, q0 + q_count) of a sequence (packed row i is the sequence's new token i / group, head i % group of
+// the kv head) against the tokens [tile_begin * 128, tile_end * 128). slot >= 0: the piece is one of several of its rows and leaves
+// partial sums there.
+struct SplPagedItem { int32_t sequence, row0, kv_head, q0, q_count, tile_begin, tile_end, slot; };
+// Rows whose pieces' partial sums are to be joined: slots [slot, slot + slots).
+struct SplPagedMerge { int32_t row0, kv_head, q0, q_count, slot, slots, reserved[2]; };
+
+struct SplPagedPlan {
+    std::vector<SplPagedItem> items;
+    std::vector<int32_t> block_begin;         // [blocks + 1]: a block's items
+    std::vector<SplPagedMerge> merges;
+};
+
+// Most items and merges that a configuration's batches come to: a block's boundary cuts at most one tile of query rows.
+inline int64_t spl_paged_items_max(const spl_paged_config &c, int blocks) {
+    const int64_t group = c.heads / c.kv_heads;
+    return c.kv_heads * (int64_t(c.max_rows) * group / SPL_PAGED_TILE + std::min(c.max_sequences, c.max_rows)) + blocks;
+}
+
+inline int spl_paged_first_token(const spl_paged_config &c, int position) { return c.window > 0 && position + 1 > c.window ? position + 1 - c.window : 0; }
+
+// Why a configuration is refused, or null.
+inline const char *spl_paged_config_error(const spl_paged_config &c) {
+    if (c.head_dim != 64 && c.head_dim != 128 && c.head_dim != 256) return "heads are 64, 128 or 256 channels wide";
+    if (c.heads < 1 || c.kv_heads < 1 || c.heads % c.kv_heads || c.heads > 1024 || c.heads / c.kv_heads > 64) return "heads must be a multiple of kv_heads, at most 1024 and 64 a kv head";
+    if (c.dtype != SPL_F16 && c.dtype != SPL_BF16) return "the cache holds fp16 or bf16";
+    if (c.page_tokens != 16 && c.page_tokens != 32 && c.page_tokens != 64 && c.page_tokens != 128 && c.page_tokens != 256) return "pages hold 16, 32, 64, 128 or 256 tokens";
+    if (c.pages < 1) return "no pages";
+    const int64_t d = c.head_dim, ps = c.page_stride, hs = c.head_stride, ts = c.token_stride, most = int64_t(1) << 38;
+    if (ps % 8 || hs % 8 || ts % 8) return "strides must be multiples of 8 elements";
+    if (ps <= 0 || hs <= 0 || ts <= 0 || ps > most || hs > most || ts > most || ps > (int64_t(1) << 50) / c.pages) return "strides are out of range";
+    const bool token_inside = ts >= d && hs >= ts * c.page_tokens && ps >= hs * c.kv_heads, head_inside = hs >= d && ts >= hs * c.kv_heads && ps >= ts * c.page_tokens;
+    if (!token_inside && !head_inside) return "strides must be those of [page][kv head][token][channel] or [page][token][kv head][channel], rows not overlapping";
+    if (c.rotary_dim < 0 || c.rotary_dim > c.head_dim || c.rotary_dim % 2) return "rotary_dim must be even and at most head_dim";
+    if (c.rotary_dim && !(c.rope_theta > 0.0f && std::isfinite(c.rope_theta))) return "rope_theta must be positive";
+    if (!(c.scale >= 0.0f) || !std::isfinite(c.scale)) return "scale must be positive, or 0 for 1 / sqrt(head_dim)";
+    if (c.window < 0) return "window must be 0 (none) or a number of tokens";
+    if (c.max_sequences < 1 || c.max_rows < 1 || c.max_context < 1 || c.max_context > (1 << 30) || c.max_rows > (1 << 20) || c.max_sequences > (1 << 16))
+        return "max_sequences, max_rows or max_context out of range";
+    if (int64_t((c.max_context + c.page_tokens - 1) / c.page_tokens) * c.max_sequences > (int64_t(1) << 28)) return "the page table is too large";
+    return nullptr;
+}
+
+// Whether a batch is taken; `why` says what is wrong with one that is not. `shared_write`: two sequences' new tokens share a page (or a
+// sequence's page table holds one twice among those it writes to).
+inline spl_status spl_paged_batch_check(const spl_paged_config &c, int32_t sequences, const int32_t *rows, const int32_t *lengths, const int32_t *table, int32_t table_ld,
+                                        std::vector<uint8_t> &written, bool *shared_write, std::string *why) {
+    auto refuse = [&](spl_status s, const std::string &text) { *why = text; return s; };
+    if (sequences < 1 || sequences > c.max_sequences) return refuse(SPL_ERR_INVALID_ROWS, "the number of sequences is outside the limit");
+    int64_t total = 0;
+    for (int s = 0; s < sequences; ++s) {
+        const std::string name = "sequence " + std::to_string(s);
+        if (rows[s] < 0 || lengths[s] < rows[s]) return refuse(SPL_ERR_INVALID_ROWS, name + " has more new rows than tokens");
+        if (lengths[s] > c.max_context) return refuse(SPL_ERR_CONTEXT_EXCEEDED, name + " is longer than max_context");
+        total += rows[s];
+        const int used = (lengths[s] + c.page_tokens - 1) / c.page_tokens;
+        if (used > table_ld) return refuse(SPL_ERR_INVALID_ROWS, name + " has more pages than the table's rows");
+        for (int i = 0; i < used; ++i) {
+            const int page = table[size_t(s) * table_ld + i];
+            if (page < 0 || page >= c.pages) return refuse(SPL_ERR_INVALID_ROWS, "page " + std::to_string(i) + " of " + name + " is not a page of the cache");
+        }
+    }
+    if (total < 1 || total > c.max_rows) return refuse(SPL_ERR_INVALID_ROWS, "the number of rows is outside the limit");
+    bool shared = false;
+    auto each_written = [&](auto &&visit) {
+        for (int s = 0; s < sequences; ++s)
+            if (rows[s]) for (int i = (lengths[s] - rows[s]) / c.page_tokens; i <= (lengths[s] - 1) / c.page_tokens; ++i) visit(table[size_t(s) * table_ld + i]);
+    };
+    written.resize(size_t(c.pages), 0);
+    each_written([&](int page) { shared = shared || written[page]; written[page] = 1; });
+    each_written([&](int page) { written[page] = 0; });
+    *shared_write = shared;
+    return SPL_OK;
+}
+
+// The tiles of all (sequence, kv head, 128 packed rows) in a line, cut in one stretch a block of equal cost, a piece costing its tiles and
+// SPL_PAGED_PIECE_COST more (queries in, the pipeline's start, the output). The pieces of a tile of rows that a cut goes through are joined afterwards.
+// (Whole tiles of rows, longest first, leave the last round of blocks idle for prompts and most of the GPU for decode steps of few sequences; a stretch a
+// block has neither.)
+#define SPL_PAGED_PIECE_COST 2
+inline void spl_paged_plan(const spl_paged_config &c, int blocks, int32_t sequences, const int32_t *rows, const int32_t *lengths, SplPagedPlan &plan) {
+    const int group = c.heads / c.kv_heads, tile = SPL_PAGED_TILE;
+    std::vector<SplPagedItem> &units = plan.items;
+    std::vector<SplPagedItem> whole;
+    int64_t tiles = 0;
+    int longest = 0;
+    for (int s = 0, row0 = 0; s < sequences; row0 += rows[s], ++s)
+        for (int h = 0; h < c.kv_heads; ++h)
+            for (int q0 = 0; q0 < rows[s] * group; q0 += tile) {
+                const int count = std::min(tile, rows[s] * group - q0), base = lengths[s] - rows[s];
+                const int first = spl_paged_first_token(c, base + q0 / group), last = c.causal ? base + (q0 + count - 1) / group + 1 : lengths[s];
+                const SplPagedItem u{s, row0, h, q0, count, first / tile, (last + tile - 1) / tile, -1};
+                tiles += u.tile_end - u.tile_begin;
+                longest = std::max(longest, u.tile_end - u.tile_begin);
+                whole.push_back(u);
+            }
+    // The least stretch that makes do with the blocks there are.
+    auto blocks_for = [&](int64_t stretch) {
+        int64_t used = 1, left = stretch;
+        for (const SplPagedItem &u : whole)
+            for (int64_t t = u.tile_end - u.tile_begin; t > 0;) {
+                if (left <= SPL_PAGED_PIECE_COST) { ++used; left = stretch; }
+                const int64_t take = std::min(t, left - SPL_PAGED_PIECE_COST);
+                t -= take; left -= take + SPL_PAGED_PIECE_COST;
+            }
+        return used;
+    };
+    int64_t low = SPL_PAGED_PIECE_COST + 1, high = std::max<int64_t>(low, tiles + int64_t(whole.size()) * SPL_PAGED_PIECE_COST);
+    while (low < high) { const int64_t mid = (low + high) / 2; if (blocks_for(mid) <= blocks) high = mid; else low = mid + 1; }
+    units.clear(); plan.merges.clear();
+    plan.block_begin.assign(1, 0);
+    int64_t left = low;
+    int slots = 0;
+    for (const SplPagedItem &u : whole) {
+        const size_t piece0 = units.size();
+        for (int t = u.tile_begin; t < u.tile_end;) {
+            if (left <= SPL_PAGED_PIECE_COST) { plan.block_begin.push_back(int32_t(units.size())); left = low; }
+            const int take = int(std::min<int64_t>(u.tile_end - t, left - SPL_PAGED_PIECE_COST));
+            SplPagedItem piece = u;
+            piece.tile_begin = t; piece.tile_end = t + take;
+            units.push_back(piece);
+            t += take; left -= take + SPL_PAGED_PIECE_COST;
+        }
+        const int pieces = int(units.size() - piece0);
+        if (pieces > 1) {
+            plan.merges.push_back(SplPagedMerge{u.row0, u.kv_head, u.q0, u.q_count, slots, pieces, {0, 0}});
+            for (size_t i = piece0; i < units.size(); ++i) units[i].slot = slots++;
+        }
+    }
+    plan.block_begin.resize(size_t(blocks) + 1, int32_t(units.size()));
+    plan.block_begin[blocks] = int32_t(units.size());
+}
+// Slots that a plan of `blocks` stretches takes at most: each cut between two blocks makes two pieces of one.
+inline int spl_paged_slots_max(int blocks) { return 2 * blocks; }

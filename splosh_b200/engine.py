@@ -250,6 +250,8 @@ def lib():
             "spl_paged_batch": (i32, [vp, i32, vp, vp, vp, i32, vp]),
             "spl_paged_append": (i32, [vp, i32, vp, C.c_int64, vp, C.c_int64, vp, C.c_int64, vp, vp, vp, vp, vp, vp]),
             "spl_paged_attend": (i32, [vp, vp, vp, vp, i32, vp, vp]),
+            "spl_paged_check": (i32, [vp, i32, vp, vp, vp, i32, vp, C.c_char_p, C.c_size_t]),
+            "spl_debug_paged_plan": (i32, [vp, i32, i32, vp, vp, vp, vp, i32, vp, vp, vp]),
             "spl_draft_create": (i32, [vp, vp, vp]),
             "spl_draft_destroy": (None, [vp]),
             "spl_draft_set_tensor": (i32, [vp, C.c_char_p, vp, i32, i32]),

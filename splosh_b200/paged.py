@@ -23,6 +23,47 @@ def _type(name):
     return TYPES[name]
 
 
+def _config(heads, kv_heads, head_dim, pages, page_tokens=256, dtype="bf16", layout="head", strides=None, rotary_dim=0, rope_theta=10000.0, scale=0.0, causal=True, window=0,
+            max_sequences=8, max_rows=64, max_context=32768):
+    if strides is None:
+        if layout not in ("head", "token"):
+            raise EngineError(10, f"no such layout: {layout}; head or token")
+        page = kv_heads * page_tokens * head_dim
+        strides = (page, page_tokens * head_dim, head_dim) if layout == "head" else (page, head_dim, kv_heads * head_dim)
+    return _Config(heads, kv_heads, head_dim, _type(dtype), page_tokens, pages, *strides, rotary_dim, rope_theta, scale, int(causal), window, max_sequences, max_rows, max_context)
+
+
+def _batch(rows, lengths, page_table):
+    rows, lengths, table = (np.ascontiguousarray(x, np.int32) for x in (rows, lengths, page_table))
+    if rows.ndim != 1 or lengths.shape != rows.shape or table.ndim != 2 or table.shape[0] != rows.shape[0]:
+        raise EngineError(10, "rows and lengths are one number a sequence, the page table one row a sequence")
+    return rows, lengths, table
+
+
+def paged_check(rows=(), lengths=(), page_table=None, **config):
+    """What PagedAttention and its batch would say to these arguments, without a GPU (spl_paged_check): whether append would refuse the batch."""
+    cfg, message, shared = _config(**config), C.create_string_buffer(256), C.c_int32(0)
+    rows, lengths, table = _batch(rows, lengths, np.zeros((len(rows), 0), np.int32) if page_table is None else page_table)
+    status = lib().spl_paged_check(C.byref(cfg), rows.shape[0], _ptr(rows), _ptr(lengths), _ptr(table), table.shape[1], C.byref(shared), message, len(message))
+    if status:
+        raise EngineError(status, message.value.decode() or "spl_paged_check refused its arguments")
+    return bool(shared.value)
+
+
+def debug_paged_plan(rows, lengths, blocks=148, **config):
+    """How a batch's attention is dealt to the blocks of a launch (spl_debug_paged_plan): (block_begin, items, merges)."""
+    cfg = _config(**config)
+    rows, lengths = np.ascontiguousarray(rows, np.int32), np.ascontiguousarray(lengths, np.int32)
+    group = cfg.heads // cfg.kv_heads
+    capacity = cfg.kv_heads * (int(rows.sum()) * group // 128 + len(rows)) + blocks
+    begin, items, merges = np.zeros(blocks + 1, np.int32), np.zeros((capacity, 8), np.int32), np.zeros((blocks, 8), np.int32)
+    item_count, merge_count = C.c_int32(0), C.c_int32(0)
+    status = lib().spl_debug_paged_plan(C.byref(cfg), blocks, len(rows), _ptr(rows), _ptr(lengths), _ptr(begin), _ptr(items), capacity, C.byref(item_count), _ptr(merges), C.byref(merge_count))
+    if status:
+        raise EngineError(status, "spl_debug_paged_plan refused its arguments")
+    return begin, items[:item_count.value], merges[:merge_count.value]
+
+
 class PagedAttention:
     """One layer shape and the batch of a pass (spl_paged). The cache is the caller's: K and V each `pages` pages in the layout "head"
     ([page][kv head][token][channel]) or "token" ([page][token][kv head][channel]), or with `strides` (page, head, token) in elements."""
@@ -31,12 +72,7 @@ class PagedAttention:
                  causal=True, window=0, max_sequences=8, max_rows=64, max_context=32768):
         self.handle, self.engine, self.dtype = None, engine, dtype
         self.q_width, self.kv_width = heads * head_dim, kv_heads * head_dim
-        if strides is None:
-            if layout not in ("head", "token"):
-                raise EngineError(10, f"no such layout: {layout}; head or token")
-            page = kv_heads * page_tokens * head_dim
-            strides = (page, page_tokens * head_dim, head_dim) if layout == "head" else (page, head_dim, kv_heads * head_dim)
-        cfg = _Config(heads, kv_heads, head_dim, _type(dtype), page_tokens, pages, *strides, rotary_dim, rope_theta, scale, int(causal), window, max_sequences, max_rows, max_context)
+        cfg = _config(heads, kv_heads, head_dim, pages, page_tokens, dtype, layout, strides, rotary_dim, rope_theta, scale, causal, window, max_sequences, max_rows, max_context)
         handle = C.c_void_p()
         engine._check(lib().spl_paged_create(engine.handle, C.byref(cfg), C.byref(handle)))
         self.handle = handle
@@ -52,9 +88,7 @@ class PagedAttention:
 
     def batch(self, rows, lengths, page_table, stream=None):
         """The sequences of a pass: new tokens and length (with them) of each, and its pages (int32 [sequences][pages of the longest])."""
-        rows, lengths, table = (np.ascontiguousarray(x, np.int32) for x in (rows, lengths, page_table))
-        if rows.ndim != 1 or lengths.shape != rows.shape or table.ndim != 2 or table.shape[0] != rows.shape[0]:
-            raise EngineError(10, "rows and lengths are one number a sequence, the page table one row a sequence")
+        rows, lengths, table = _batch(rows, lengths, page_table)
         self.engine._check(lib().spl_paged_batch(self.handle, rows.shape[0], _ptr(rows), _ptr(lengths), _ptr(table), table.shape[1], stream_handle(stream)))
 
     def append(self, q, k, v, q_out, k_cache, v_cache, dtype="f32", ld=None, q_norm=None, k_norm=None, stream=None):
