@@ -145,7 +145,7 @@ spl_paged_append_kernel(SplPagedRows in, const uint16_t *__restrict__ q_norm, co
 #define SPL_PAGED_HEADROOM 8.0f
 __host__ __device__ constexpr int spl_paged_ring(int hd) { return hd == 256 ? 9 : hd == 128 ? 11 : 12; }
 __host__ __device__ constexpr size_t spl_paged_smem_bytes(int hd) {
-    return 1024 + size_t(hd / 64 + spl_paged_ring(hd)) * SPL_PAGED_CHUNK + 2 * 2 * 128 * 4 /* maxima */ + 2 * 128 * 4 /* sums */ + 256 /* barriers */;
+    return 1024 + size_t(hd / 64 + spl_paged_ring(hd)) * SPL_PAGED_CHUNK + 2 * 2 * 128 * 4 /* maxima */ + 2 * 128 * 4 /* sums */ + 512 /* barriers */;
 }
 
 // Tokens that the row at `position` of a sequence of `length` tokens sees: [first, last).
@@ -203,15 +203,15 @@ spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
     float *xmax = reinterpret_cast<float *>(ring + NST * CHUNK);      // [tile parity][half][row]
     float *xsum = xmax + 2 * 2 * 128;                                 // [half][row]
     uint64_t *bars = reinterpret_cast<uint64_t *>(xsum + 2 * 128);
-    uint64_t *full = bars, *empty = full + NST, *s_full = empty + NST, *p_full = s_full + 2, *o_done = p_full + 2, *q_full = o_done + 1, *drained = q_full + 1;
+    uint64_t *full = bars, *empty = full + NST, *s_full = empty + NST, *p_full = s_full + 2, *o_done = p_full + 2, *q_full = o_done + 2, *drained = q_full + 1;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drained + 1);
     volatile int *abort = reinterpret_cast<volatile int *>(tmem_slot + 1);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     if (tid == 0) {
         for (int i = 0; i < NST; ++i) { spl_mbar_init(&full[i], 1); spl_mbar_init(&empty[i], 1); }
-        for (int i = 0; i < 2; ++i) { spl_mbar_init(&s_full[i], 1); spl_mbar_init(&p_full[i], 8); }
-        spl_mbar_init(o_done, 1); spl_mbar_init(q_full, 8); spl_mbar_init(drained, 1);
+        for (int i = 0; i < 2; ++i) { spl_mbar_init(&s_full[i], 1); spl_mbar_init(&p_full[i], 8); spl_mbar_init(&o_done[i], 1); }
+        spl_mbar_init(q_full, 8); spl_mbar_init(drained, 1);
         *abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
@@ -225,6 +225,8 @@ spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
     const uint32_t tmem = *tmem_slot, tmem_o = tmem + 256;
     spl_grid_begin();
     const int item0 = a.block_begin[blockIdx.x], item1 = a.block_begin[blockIdx.x + 1];
+    // A wait tells a phase from the one before it and no more, so a barrier is waited for only by roles that know its last but one use to be over: S, P and O have one a tile
+    // parity (tile i's S is issued after the product of tile i - 2 was waited for; whoever has seen that S may wait for the product of tile i - 1 or i).
     // A role whose wait ran out goes through the rest of its loops without waiting: barriers among warps are met by all of them whatever happened.
     bool ok = true;
     auto gave_up = [&](int code) { ok = false; if (!*abort && lane == 0) { spl_note_wait(a.error_flag, code, 0); a.error_flag[0] = 200 + warp; } *abort = 1; };
@@ -266,10 +268,9 @@ spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
         constexpr uint32_t s_idesc = spl_paged_idesc(128, BF16, false), o_idesc = spl_paged_idesc(64, BF16, true);
         const uint64_t q_desc = spl_tc_desc_sw128(spl_smem_addr(q_tile)), ring_desc = spl_tc_desc_sw128(spl_smem_addr(ring));
         int n = 0, tiles = 0, pieces = 0;                     // chunks, tiles and pieces so far
-        // Scores of tile number `at` of this block. They go where the P of tile at - 2 lies, which has to have been read (a piece's first tile: all products before
-        // it are over, since its queries are there).
-        auto scores = [&](int at, bool first) {
-            if (ok && !first && at >= 2 && !spl_mbar_wait_warp(o_done, (at - 2) & 1, const_cast<const int *>(abort))) gave_up(61);
+        // Scores of tile number `at` of this block. They go where the P of tile at - 2 lies, which has to have been read.
+        auto scores = [&](int at) {
+            if (ok && at >= 2 && !spl_mbar_wait_warp(&o_done[at & 1], ((at - 2) >> 1) & 1, const_cast<const int *>(abort))) gave_up(61);
             for (int c = 0; c < C; ++c, ++n) {
                 const int st = n % NST;
                 if (ok && !spl_mbar_wait_warp(&full[st], (n / NST) & 1, const_cast<const int *>(abort))) gave_up(62);
@@ -292,9 +293,9 @@ spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
             const int seen_first = spl_paged_first(s, base + it.q0 / s.group), seen_last = spl_paged_last(s, base + (it.q0 + it.q_count - 1) / s.group, t.lengths[it.sequence]);
             if (ok && !spl_mbar_wait_warp(q_full, pieces & 1, const_cast<const int *>(abort))) gave_up(63);
             if (!ok) break;
-            scores(tiles, true);
+            scores(tiles);
             for (int tile = it.tile_begin; tile < it.tile_end && ok; ++tile, ++tiles) {
-                if (tile + 1 < it.tile_end) scores(tiles + 1, false);
+                if (tile + 1 < it.tile_end) scores(tiles + 1);
                 if (ok && !spl_mbar_wait_warp(&p_full[tiles & 1], (tiles >> 1) & 1, const_cast<const int *>(abort))) gave_up(64);
                 const int from = max(0, seen_first - tile * 128), to = min(128, seen_last - tile * 128), k0 = from / 16, k1 = (to + 15) / 16;
                 for (int c = 0; c < C && ok; ++c, ++n) {
@@ -314,7 +315,7 @@ spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
                         for (int ks = k0; ks < k1; ++ks)
                             spl_tc_mma_ts(tmem_o + c * 64, tmem + (tiles & 1) * 128 + ks * 8, ring_desc + uint64_t((st * CHUNK + ks * 2048) >> 4), o_idesc, tile > it.tile_begin || ks > k0 ? 1u : 0u);
                         spl_tc_commit(&empty[st]);
-                        if (c == C - 1) spl_tc_commit(o_done);
+                        if (c == C - 1) spl_tc_commit(&o_done[tiles & 1]);
                     }
                     __syncwarp();
                 }
@@ -378,7 +379,7 @@ spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
                         const float factor = raise ? exp2f(ref - m) : 1.0f;
                         if (tile > it.tile_begin) {
                             // The product before has to be done with these sums; the next waits for this warp's probabilities.
-                            if (ok && !spl_mbar_wait_warp(o_done, (tiles - 1) & 1, const_cast<const int *>(abort))) gave_up(67);
+                            if (ok && !spl_mbar_wait_warp(&o_done[(tiles - 1) & 1], ((tiles - 1) >> 1) & 1, const_cast<const int *>(abort))) gave_up(67);
                             spl_tc_fence_after();
 #pragma unroll 1
                             for (int o = 0; o < HD / 2; o += 16) {
@@ -410,7 +411,7 @@ spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
                 if (lane == 0) spl_mbar_arrive(&p_full[buf]);
             }
             // The piece's sums.
-            if (ok && !spl_mbar_wait_warp(o_done, (tiles - 1) & 1, const_cast<const int *>(abort))) gave_up(68);
+            if (ok && !spl_mbar_wait_warp(&o_done[(tiles - 1) & 1], ((tiles - 1) >> 1) & 1, const_cast<const int *>(abort))) gave_up(68);
             if (busy) {
                 spl_tc_fence_after();
                 xsum[half * 128 + r] = sum;
@@ -425,10 +426,10 @@ spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
                 for (int o = 0; o < HD / 2; o += 16) {
                     uint32_t y[16];
                     spl_tc_ld16(y, tmem_o + lanes + half * (HD / 2) + o);
-                    if (!here) continue;
 #pragma unroll
                     for (int j = 0; j < 16; ++j) y[j] = __float_as_uint(__uint_as_float(y[j]) * inv);
-                    if (it.slot >= 0 || a.out_f32) {
+                    if (!here) {
+                    } else if (it.slot >= 0 || a.out_f32) {
                         float *dst = it.slot >= 0 ? a.partial + slot_row * HD + half * (HD / 2) + o : static_cast<float *>(a.out) + place + o;
 #pragma unroll
                         for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4 *>(dst + 4 * j) = make_uint4(y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]);
@@ -439,6 +440,7 @@ spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
                         uint4 *dst = reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.out) + place + o);
                         dst[0] = make_uint4(w[0], w[1], w[2], w[3]); dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
                     }
+                    __syncwarp();
                 }
                 if (here && it.slot >= 0 && half == 0) a.partial_ml[slot_row] = make_float2(ref, sum);
                 spl_paged_pair_barrier(quarter);              // the sums in shared memory are read before the next piece's

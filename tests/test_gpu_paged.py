@@ -70,6 +70,18 @@ def test_prompts_chunks_and_mixed_batches(engine, rows, lengths, heads, kv_heads
     check_attention(scene, attend(engine, scene), dtype)
 
 
+@pytest.mark.parametrize("head_dim,dtype", [(64, "bf16"), (64, "fp16"), (128, "bf16"), (128, "fp16"), (256, "bf16"), (256, "fp16")])
+@pytest.mark.parametrize("count,around", [(149, 256), (200, 300), (40, 1000), (300, 20)])
+def test_blocks_of_several_tiles_and_pieces(engine, head_dim, dtype, count, around):
+    """More tiles than blocks: a block takes several tiles of one sequence and pieces of several sequences, one after the other."""
+    lengths = [around] * count if around == 256 else [around + (37 * i) % around for i in range(count)]
+    scene = Scene(count, 2, 1, head_dim, [1 + i % 2 for i in range(count)], lengths, page_tokens=64, dtype=dtype)
+    check_attention(scene, attend(engine, scene, "f32"), "f32")
+    again = attend(engine, scene, "f32")
+    for _ in range(5):
+        assert torch.equal(attend(engine, scene, "f32"), again)
+
+
 @pytest.mark.parametrize("window", [1, 2, 63, 64, 129, 300])
 @pytest.mark.parametrize("causal", [True, False])
 def test_windows_and_blocks_that_see_themselves(engine, window, causal):
