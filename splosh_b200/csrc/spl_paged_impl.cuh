@@ -166,6 +166,25 @@ template <int HD, bool BF16> static void launch_attend(const spl_paged *p, const
                 reinterpret_cast<const SplPagedMerge *>(p->tables_dev + p->merges_at), p->shape, (const float *)p->partial, (const float2 *)p->partial_ml, p->slot_rows, a.out, a.out_f32);
 }
 
+// A cluster of blocks a row, as many as hold the row in shared memory (at most eight; more values than that are read in every pass).
+static spl_status launch_sample(spl_engine *e, const SplSampleArgs &args, int rows, cudaStream_t stream) {
+    int blocks = 1;
+    while (blocks < SPL_SAMPLE_CLUSTER && blocks * SPL_SAMPLE_STRETCH < args.limit) blocks *= 2;
+    while (blocks > 1 && e->clusters[blocks] < 1) blocks /= 2;      // (a size the device cannot hold)
+    const bool held = blocks * SPL_SAMPLE_STRETCH >= args.limit;
+    void (*kernel)(SplSampleArgs) = held ? spl_sample_kernel<true> : spl_sample_kernel<false>;
+    const size_t smem = sizeof(SplSampleShared) + (held ? size_t(std::min(args.limit, SPL_SAMPLE_STRETCH)) * 4 : 0);
+    SPL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(SplSampleShared) + SPL_SAMPLE_STRETCH * 4)));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(blocks, rows); cfg.blockDim = dim3(1024); cfg.dynamicSmemBytes = smem; cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization; attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension; attr[1].val.clusterDim.x = blocks; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr; cfg.numAttrs = 2;
+    SPL_CUDA(cudaLaunchKernelEx(&cfg, kernel, args));
+    return SPL_OK;
+}
+
 static bool misaligned(const void *p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes != 0; }
 
 extern "C" {
@@ -255,8 +274,7 @@ spl_status spl_pass_sample(spl_engine *e, const float *device_logits, int32_t ro
     if (vocab_limit < 1 || vocab_limit > SPL_SAMPLE_VOCAB || ld < vocab_limit) return e->fail(SPL_ERR_INVALID_ARGUMENT, "spl_pass_sample: vocab_limit must be 1 ... 524288 and at most the rows' stride");
     const SplDeviceScope scope(e->device);
     const SplSampleArgs args{device_logits, ld, vocab_limit, device_temperature, device_top_k, device_top_p, device_min_p, device_uniform, device_ids};
-    launch_step(spl_sample_kernel, dim3(rows), dim3(1024), 0, paged_stream(e, stream), args);
-    return check_launch(e, "spl_pass_sample");
+    return launch_sample(e, args, rows, paged_stream(e, stream));
 }
 
 spl_status spl_sample(spl_engine *e, int32_t vocab_limit, const spl_sampling *settings, const float *uniform, int32_t *ids) {
@@ -274,8 +292,7 @@ spl_status spl_sample(spl_engine *e, int32_t vocab_limit, const spl_sampling *se
     }
     SPL_CUDA(cudaMemcpyAsync(d, w, size_t(rows) * 20, cudaMemcpyHostToDevice, e->stream));
     const SplSampleArgs args{e->logits, e->logits_ld, vocab_limit, d, reinterpret_cast<const int *>(d) + rows, d + 2 * rows, d + 3 * rows, d + 4 * rows, reinterpret_cast<int *>(d) + 5 * rows};
-    launch_step(spl_sample_kernel, dim3(rows), dim3(1024), 0, e->stream, args);
-    const spl_status launched = check_launch(e, "spl_sample");
+    const spl_status launched = launch_sample(e, args, rows, e->stream);
     if (launched != SPL_OK) return launched;
     SPL_CUDA(cudaMemcpyAsync(e->topk_host + 5 * rows, d + 5 * rows, size_t(rows) * 4, cudaMemcpyDeviceToHost, e->stream));
     SPL_CUDA(cudaStreamSynchronize(e->stream));

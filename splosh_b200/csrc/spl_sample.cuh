@@ -6,13 +6,15 @@
 //   top-p   of those the smallest prefix whose w reaches p times their sum        (p >= 1: all)
 //   min-p   of those the ones with w >= m                                         (m <= 0: all)
 //   draw    the first whose running sum of w reaches u times the sum of what stays
-// T <= 0 takes the largest value. Everything that stays is a prefix of the order, so nothing is sorted: a cut is found
-// by its place or by its weight, eight bits of the values' keys at a time.
+// T <= 0 takes the largest value. Everything that stays is a prefix of the order, so a row is never sorted: a place in the order
+// (the k-th, the one where the weight reaches p, the draw) lies in one bin of a histogram over the values, and only that bin's values are.
 //
 // The token has to be the definition's, so the sums have to be right where a boundary between tokens is close: 32-bit sums of a flat
 // vocabulary of 250K would pick another token in one row of fifty. Weights are formed in 64-bit floating point and summed as whole numbers of
 // 2^-44 (the largest is 2^44, 2^19 of them fit 64 bits): the sums do not depend on the order of the additions.
 #pragma once
+#include <cooperative_groups.h>
+
 #include "spl_elementwise.cuh"
 
 #define SPL_SAMPLE_UNIT 17592186044416.0       // 2^44
@@ -25,38 +27,83 @@ struct SplSampleArgs {
 };
 
 __device__ __forceinline__ float spl_topk_value(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key); }
-// The weight of a value, a whole number of 2^-44. (inf - inf is no number: the maximum itself has weight one.)
+// The weight of a value, a whole number of 2^-44. (inf - inf is no number: the maximum itself has weight one, beside an infinite one nothing has any.)
 __device__ __forceinline__ unsigned long long spl_sample_weight(float x, float max, double inv_t) {
     if (x == max) return 1ull << 44;
+    if (max == INFINITY || !(x > -INFINITY)) return 0ull;
     return static_cast<unsigned long long>(exp((double(x) - double(max)) * inv_t) * SPL_SAMPLE_UNIT + 0.5);
 }
 
-// Grid (rows), 1,024 threads.
-__global__ void __launch_bounds__(1024)
-spl_sample_kernel(SplSampleArgs a) {
-    __shared__ unsigned long long mass[256];
-    __shared__ unsigned int count[256], warp_count[32];
-    __shared__ unsigned long long found_before;
-    __shared__ unsigned int found_digit, shared_max;
-    spl_grid_begin();
-    const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const float *x = a.logits + size_t(row) * a.ld;
-    const float t = a.temperature ? a.temperature[row] : 1.0f, p = a.top_p ? a.top_p[row] : 1.0f, u = a.uniform[row];
-    const float m = a.min_p ? fminf(a.min_p[row], 1.0f) : 0.0f;
-    const int k = a.top_k ? a.top_k[row] : 0;
-    if (tid == 0) shared_max = 0u;
-    __syncthreads();
-    uint32_t top = 0u;
-    for (int i = tid; i < a.limit; i += 1024) top = max(top, spl_topk_key(x[i]));
-    top = __reduce_max_sync(0xffffffffu, top);
-    if (lane == 0) atomicMax(&shared_max, top);
-    __syncthreads();
-    top = shared_max;
-    if (top == 0u) { if (tid == 0) a.ids[row] = 0; return; }                 // nothing to pick from: as an untouched slot of a top-k
-    const float max_value = spl_topk_value(top);
-    const bool greedy = !(t > 0.0f);
-    const double inv_t = greedy ? 1.0 : 1.0 / double(t);
 
+// A cluster of blocks a row, 32,768 values a block in shared memory (a vocabulary of more than eight blocks' is read anew in every pass): the row comes
+// from memory once. The histogram has 2,048 bins of 1/64 in (max - x) / T, so that bins hold a few hundred values where a vocabulary's are densest; what is
+// 31.98 and more below the maximum has no weight in whole numbers of 2^-44 and is the last bin. The first block of the cluster adds the blocks' bins, finds the bin
+// that a place lies in, and sorts that bin's values, which the blocks have set aside:
+//   top-k         counts; the bins down to the k-th value's are sorted whole where they fit (SPL_SAMPLE_LIST), and everything else is decided on
+//                 that list; a larger k sorts its own bin alone and leaves a cut for what follows
+//   then          weights; the bins of top-p's place and of min-p's bound are sorted for the exact end of what stays, and then the draw's bin
+// A bin of more values than the list holds (equal logits, very high temperatures) leaves the row to the first block, which finds places eight bits of
+// the values' keys at a time (spl_sample_slow).
+#define SPL_SAMPLE_BINS 2048
+#define SPL_SAMPLE_LIST 4096
+#define SPL_SAMPLE_STRETCH 32768
+#define SPL_SAMPLE_CLUSTER 8
+
+struct SplSampleShared {
+    unsigned int lo[SPL_SAMPLE_BINS], hi[SPL_SAMPLE_BINS];      // the bins: counts in lo, or weights in both
+    unsigned long long list[SPL_SAMPLE_LIST];                   // values set aside: key << 32 | ~index, so that descending order is the definition's
+    unsigned long long sums[SPL_SAMPLE_LIST];                   // running sums of bins or of the sorted list (first block)
+    unsigned long long best[SPL_SAMPLE_CLUSTER];                // the blocks' largest values
+    unsigned long long warp_sum[32], value[4];
+    unsigned int listed, found;
+    // The first block's decision, in every block: which bins to set aside, or what has been decided.
+    int step, first_bin, last_bin;
+    unsigned long long cut;
+};
+enum { SPL_SAMPLE_DONE = 0, SPL_SAMPLE_FINISH, SPL_SAMPLE_CUT, SPL_SAMPLE_END, SPL_SAMPLE_DRAW, SPL_SAMPLE_WEIGH, SPL_SAMPLE_SLOW };
+
+struct SplSampleRow { float t, p, u, m, max_value, bin_scale; double inv_t; unsigned long long least; int k; };
+
+__device__ __forceinline__ unsigned long long spl_sample_entry(uint32_t key, uint32_t index) { return (unsigned long long)key << 32 | uint32_t(~index); }
+
+// Sum over the block's threads before this one (exclusive), and of all in *total.
+__device__ __forceinline__ unsigned long long spl_sample_scan(unsigned long long v, SplSampleShared &sh, unsigned long long *total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    unsigned long long run = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const unsigned long long y = __shfl_up_sync(0xffffffffu, run, o); if (lane >= o) run += y; }
+    __syncthreads();
+    if (lane == 31) sh.warp_sum[warp] = run;
+    __syncthreads();
+    if (warp == 0) {
+        unsigned long long w = sh.warp_sum[lane];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) { const unsigned long long y = __shfl_up_sync(0xffffffffu, w, o); if (lane >= o) w += y; }
+        sh.warp_sum[lane] = w;
+    }
+    __syncthreads();
+    *total = sh.warp_sum[31];
+    return (warp ? sh.warp_sum[warp - 1] : 0ull) + run - v;
+}
+// The first place of [0, n) whose sums[] reaches `target` (n: none); the sums do not fall. All threads get it.
+__device__ __forceinline__ int spl_sample_place(SplSampleShared &sh, int n, unsigned long long target) {
+    __syncthreads();
+    if (threadIdx.x == 0) sh.found = unsigned(n);
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += 1024) if (sh.sums[i] >= target && (i == 0 || sh.sums[i - 1] < target)) sh.found = unsigned(i);
+    __syncthreads();
+    return int(sh.found);
+}
+__device__ __forceinline__ unsigned long long spl_sample_target(float fraction, unsigned long long sum) {
+    return fraction > 0.0f ? min(sum, (unsigned long long)ceil(double(fraction) * double(sum))) : 0ull;
+}
+
+// Places found on the row itself, eight bits of the keys at a time, by one block.
+__device__ __noinline__ void spl_sample_slow(const SplSampleArgs &a, const SplSampleRow &r, SplSampleShared &sh, int row) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const float *x = a.logits + size_t(row) * a.ld;
+    unsigned long long *mass = sh.sums;
+    unsigned int *count = sh.lo, *warp_count = sh.hi;
     // What stays: keys above cut_key, and of cut_key itself the cut_ties lowest indices; and weights of at least `least`.
     uint32_t cut_key = 1u;
     unsigned long long cut_ties = ~0ull, least = 0ull;
@@ -66,20 +113,25 @@ spl_sample_kernel(SplSampleArgs a) {
         uint32_t prefix = 0u;
         unsigned long long before = 0ull;
         for (int shift = 24; shift >= 0; shift -= 8) {
+            __syncthreads();
             if (tid < 256) { mass[tid] = 0ull; count[tid] = 0u; }
             __syncthreads();
-            for (int i = tid; i < a.limit; i += 1024) {
-                const float v = x[i];
+            for (int base = 0; base < a.limit; base += 1024) {
+                const int i = base + tid;
+                const float v = i < a.limit ? x[i] : -INFINITY;
                 const uint32_t key = spl_topk_key(v);
-                if (key < cut_key || key == 0u || (shift < 24 && (key >> (shift + 8)) != prefix)) continue;
-                const uint32_t digit = key >> shift & 255u;
-                if (by_count) atomicAdd(&count[digit], 1u);
-                else {
-                    const unsigned long long w = spl_sample_weight(v, max_value, inv_t);
-                    if (w < least) continue;
-                    atomicAdd(&mass[digit], w);
-                    atomicAdd(&count[digit], 1u);
-                }
+                const unsigned long long w = by_count ? 1ull : spl_sample_weight(v, r.max_value, r.inv_t);
+                const bool counts = key >= cut_key && key != 0u && (shift == 24 || (key >> (shift + 8)) == prefix) && (by_count || w >= least);
+                const unsigned int votes = __ballot_sync(0xffffffffu, counts);
+                if (!votes) continue;
+                const uint32_t digit = key >> shift & 255u, first = __shfl_sync(0xffffffffu, digit, __ffs(votes) - 1);
+                // Rows come here because many values are equal: those of a warp are added before they meet the others'.
+                if (__all_sync(0xffffffffu, !counts || digit == first)) {
+                    unsigned long long sum = counts ? w : 0ull;
+#pragma unroll
+                    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                    if (lane == 0) { atomicAdd(&mass[first], sum); atomicAdd(&count[first], __popc(votes)); }
+                } else if (counts) { atomicAdd(&mass[digit], w); atomicAdd(&count[digit], 1u); }
             }
             __syncthreads();
             if (tid == 0) {
@@ -87,28 +139,27 @@ spl_sample_kernel(SplSampleArgs a) {
                 int last = -1;
                 for (int d = 255; d >= 0; --d) {
                     if (!count[d]) continue;
-                    const uint32_t reached = prefix << 8 | uint32_t(d);
-                    unsigned long long here = by_count ? count[d] : mass[d];
+                    unsigned long long here = mass[d];
                     // The key that an earlier cut goes through keeps only its lowest indices.
-                    if (!by_count && shift == 0 && reached == cut_key && count[d] > cut_ties) here = mass[d] / count[d] * cut_ties;
+                    if (shift == 0 && (prefix << 8 | uint32_t(d)) == cut_key && count[d] > cut_ties) here = mass[d] / count[d] * cut_ties;
                     last = d;
-                    found_before = sum;
+                    sh.value[0] = sum;
                     sum += here;
                     if (sum >= target) break;
                 }
-                found_digit = uint32_t(last);
+                sh.found = unsigned(last);
             }
             __syncthreads();
-            prefix = prefix << 8 | found_digit;
-            before = found_before;
-            __syncthreads();
+            prefix = prefix << 8 | sh.found;
+            before = sh.value[0];
         }
         *key_out = prefix;
-        const unsigned long long each = by_count ? 1ull : spl_sample_weight(spl_topk_value(prefix), max_value, inv_t);
+        const unsigned long long each = by_count ? 1ull : spl_sample_weight(spl_topk_value(prefix), r.max_value, r.inv_t);
         *ties_out = target <= before + 1ull || each == 0ull ? 1ull : (target - before + each - 1ull) / each;
     };
     // The weight of all that stays.
     auto total = [&]() {
+        __syncthreads();
         if (tid == 0) { mass[0] = 0ull; count[0] = 0u; }
         __syncthreads();
         unsigned long long sum = 0ull;
@@ -118,39 +169,33 @@ spl_sample_kernel(SplSampleArgs a) {
             const uint32_t key = spl_topk_key(v);
             if (key < cut_key || key == 0u) continue;
             if (key == cut_key) { ++ties; continue; }
-            const unsigned long long w = spl_sample_weight(v, max_value, inv_t);
+            const unsigned long long w = spl_sample_weight(v, r.max_value, r.inv_t);
             if (w >= least) sum += w;
         }
         if (sum) atomicAdd(&mass[0], sum);
         if (ties) atomicAdd(&count[0], ties);
         __syncthreads();
-        const unsigned long long each = spl_sample_weight(spl_topk_value(cut_key), max_value, inv_t);
+        const unsigned long long each = spl_sample_weight(spl_topk_value(cut_key), r.max_value, r.inv_t);
         sum = mass[0];
         if (count[0] && each >= least) sum += each * min((unsigned long long)count[0], cut_ties);
-        __syncthreads();
         return sum;
     };
-    uint32_t pick_key = top;
-    unsigned long long pick_tie = 1ull;
-    if (!greedy) {
-        if (k > 0 && k < a.limit) find(true, (unsigned long long)k, &cut_key, &cut_ties);
-        if (p < 1.0f) {
-            const unsigned long long target = p > 0.0f ? (unsigned long long)ceil(double(p) * double(total())) : 0ull;
-            uint32_t key; unsigned long long ties;
-            find(false, target, &key, &ties);
-            if (key > cut_key || ties < cut_ties) { cut_key = key; cut_ties = ties; }
-        }
-        if (m > 0.0f) least = (unsigned long long)ceil(double(m) * SPL_SAMPLE_UNIT);
-        const unsigned long long all = total();
-        const unsigned long long target = u > 0.0f ? min(all, (unsigned long long)ceil(double(u) * double(all))) : 0ull;
-        find(false, target, &pick_key, &pick_tie);
+    if (r.k > 0 && r.k < a.limit) find(true, (unsigned long long)r.k, &cut_key, &cut_ties);
+    if (r.p < 1.0f) {
+        uint32_t key; unsigned long long ties;
+        find(false, spl_sample_target(r.p, total()), &key, &ties);
+        if (key > cut_key || ties < cut_ties) { cut_key = key; cut_ties = ties; }
     }
+    least = r.least;
+    uint32_t pick_key; unsigned long long pick_tie;
+    find(false, spl_sample_target(r.u, total()), &pick_key, &pick_tie);
     // The pick_tie-th lowest index of pick_key: the block walks the row in order.
     unsigned long long seen = 0ull;
     for (int base = 0; base < a.limit; base += 1024) {
         const int i = base + tid;
         const bool hit = i < a.limit && spl_topk_key(x[i]) == pick_key;
         const unsigned int votes = __ballot_sync(0xffffffffu, hit);
+        __syncthreads();
         if (lane == 0) warp_count[warp] = __popc(votes);
         __syncthreads();
         unsigned int before = 0u, all = 0u;
@@ -158,6 +203,303 @@ spl_sample_kernel(SplSampleArgs a) {
         if (hit && seen + before + __popc(votes & ((1u << lane) - 1u)) + 1u == pick_tie) a.ids[row] = i;
         seen += all;
         if (seen >= pick_tie) return;
-        __syncthreads();
     }
+}
+
+// The first block: the blocks' lists into its own, sorted, with running sums of weights that begin at `base`. Returns the entries, or -1 where
+// they do not fit.
+__device__ __forceinline__ int spl_sample_sorted(SplSampleShared &sh, cooperative_groups::cluster_group &cluster, int blocks, const SplSampleRow &r, unsigned long long base) {
+    const int tid = threadIdx.x;
+    unsigned int n = sh.listed;
+    for (int b = 1; b < blocks; ++b) {
+        const SplSampleShared *peer = cluster.map_shared_rank(&sh, b);
+        const unsigned int more = peer->listed;
+        if (n + more <= SPL_SAMPLE_LIST) for (unsigned int i = tid; i < more; i += 1024) sh.list[n + i] = peer->list[i];
+        n += more;
+    }
+    if (n > SPL_SAMPLE_LIST) return -1;
+    unsigned int width = 2;
+    while (width < n) width <<= 1;
+    __syncthreads();
+    for (unsigned int i = n + tid; i < width; i += 1024) sh.list[i] = 0ull;
+    for (unsigned int size = 2; size <= width; size <<= 1)
+        for (unsigned int stride = size >> 1; stride > 0; stride >>= 1) {
+            __syncthreads();
+            for (unsigned int q = tid; q < width / 2; q += 1024) {
+                const unsigned int i = 2 * q - (q & (stride - 1)), j = i + stride;
+                const unsigned long long x = sh.list[i], y = sh.list[j];
+                if ((x < y) == ((i & size) == 0)) { sh.list[i] = y; sh.list[j] = x; }
+            }
+        }
+    __syncthreads();
+    unsigned long long w[SPL_SAMPLE_LIST / 1024], run = 0ull, all;
+    const int per = width <= 1024 ? 1 : int(width / 1024);
+#pragma unroll
+    for (int e = 0; e < SPL_SAMPLE_LIST / 1024; ++e) {
+        const unsigned int i = tid * per + e;
+        w[e] = e < per && i < n ? spl_sample_weight(spl_topk_value(uint32_t(sh.list[i] >> 32)), r.max_value, r.inv_t) : 0ull;
+        run += w[e];
+    }
+    run = base + spl_sample_scan(run, sh, &all);
+#pragma unroll
+    for (int e = 0; e < SPL_SAMPLE_LIST / 1024; ++e) {
+        run += w[e];
+        const unsigned int i = tid * per + e;
+        if (e < per && i < n) sh.sums[i] = run;
+    }
+    __syncthreads();
+    return int(n);
+}
+
+// Grid (blocks a row, rows) in clusters of a row's blocks, 1,024 threads.
+template <bool HELD>
+__global__ void __launch_bounds__(1024, 1)
+spl_sample_kernel(SplSampleArgs a) {
+    namespace cg = cooperative_groups;
+    extern __shared__ __align__(128) unsigned char spl_sample_raw[];
+    SplSampleShared &sh = *reinterpret_cast<SplSampleShared *>(spl_sample_raw);
+    cg::cluster_group cluster = cg::this_cluster();
+    spl_grid_begin();
+    const int row = blockIdx.y, rank = blockIdx.x, blocks = gridDim.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const float *x = a.logits + size_t(row) * a.ld;
+    const int stretch = HELD ? SPL_SAMPLE_STRETCH : ((a.limit + blocks - 1) / blocks + 1023) / 1024 * 1024, begin = rank * stretch, end = min(a.limit, begin + stretch);
+    float *held = reinterpret_cast<float *>(spl_sample_raw + sizeof(SplSampleShared));
+    const float *mine = x + begin;
+    const int count = max(0, end - begin);
+    asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");      // (a block's shared memory may be reached when it has begun)
+    // Every thread of the block runs f(value, index) for its values, a warp's in step.
+    auto each = [&](auto &&f) {
+#pragma unroll 4
+        for (int base = 0; base < count; base += 1024) {
+            const int i = base + tid;
+            f(i < count ? (HELD ? held[i] : mine[i]) : -INFINITY, begin + i);
+        }
+    };
+    SplSampleRow r;
+    r.t = a.temperature ? a.temperature[row] : 1.0f; r.p = a.top_p ? a.top_p[row] : 1.0f; r.u = a.uniform[row];
+    r.m = a.min_p ? fminf(a.min_p[row], 1.0f) : 0.0f; r.k = a.top_k ? a.top_k[row] : 0;
+    r.least = r.m > 0.0f ? (unsigned long long)ceil(double(r.m) * SPL_SAMPLE_UNIT) : 0ull;
+
+    // The largest value and its lowest index.
+    {
+        uint32_t key = 0u, index = 0u;
+#pragma unroll 8
+        for (int i = tid; i < count; i += 1024) {
+            const float value = mine[i];
+            if (HELD) held[i] = value;
+            const uint32_t y = spl_topk_key(value);
+            if (y > key) { key = y; index = uint32_t(begin + i); }
+        }
+        const uint32_t all = __reduce_max_sync(0xffffffffu, key);
+        const uint32_t first = __reduce_min_sync(0xffffffffu, key == all ? index : 0xffffffffu);
+        if (lane == 0) sh.warp_sum[warp] = spl_sample_entry(all, first);
+        for (int i = tid; i < SPL_SAMPLE_BINS; i += 1024) { sh.lo[i] = 0u; sh.hi[i] = 0u; }
+        if (tid == 0) sh.listed = 0u;
+        __syncthreads();
+        unsigned long long best = 0ull;
+        if (warp == 0) {
+            best = sh.warp_sum[lane];
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+        }
+        asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+        if (warp == 0 && lane < blocks) cluster.map_shared_rank(&sh, lane)->best[rank] = best;
+        cluster.sync();
+    }
+    unsigned long long top = sh.best[0];
+    for (int b = 1; b < blocks; ++b) top = max(top, sh.best[b]);
+    const bool nothing = (top >> 32) == 0ull;          // id 0, as an untouched slot of a top-k
+    if (nothing || !(r.t > 0.0f)) {
+        if (rank == 0 && tid == 0) a.ids[row] = nothing ? 0 : int32_t(~uint32_t(top));
+        return;
+    }
+    r.max_value = spl_topk_value(uint32_t(top >> 32));
+    r.inv_t = 1.0 / double(r.t);
+    r.bin_scale = fminf(128.0f / r.t, 3.0e38f);
+    const bool endless = r.max_value == INFINITY;
+    // The bin of a value that may be picked (halved values do not overflow; rounding keeps the order).
+    auto bin_of = [&](float value) {
+        if (value == r.max_value) return 0;
+        return endless ? SPL_SAMPLE_BINS - 1 : int(fminf((0.5f * r.max_value - 0.5f * value) * r.bin_scale, float(SPL_SAMPLE_BINS - 1)));
+    };
+    unsigned long long cut = 0ull;                     // entries below it are out
+    auto set_aside = [&](int first_bin, int last_bin) {
+        each([&](float value, int i) {
+            const uint32_t key = spl_topk_key(value);
+            if (key == 0u) return;
+            const int b = bin_of(value);
+            if (b < first_bin || b > last_bin) return;
+            const unsigned long long entry = spl_sample_entry(key, uint32_t(i));
+            if (entry < cut) return;
+            const unsigned int at = atomicAdd(&sh.listed, 1u);
+            if (at < SPL_SAMPLE_LIST) sh.list[at] = entry;
+        });
+        cluster.sync();
+    };
+    // The first block's decision goes to all of them; what their lists held has been read.
+    auto decide = [&](int step, int first_bin, int last_bin, unsigned long long new_cut) {
+        __syncthreads();
+        if (tid < blocks) {
+            SplSampleShared *peer = cluster.map_shared_rank(&sh, tid);
+            peer->step = step; peer->first_bin = first_bin; peer->last_bin = last_bin; peer->cut = new_cut; peer->listed = 0u;
+        }
+    };
+    int step = SPL_SAMPLE_WEIGH;
+    if (r.k > 0 && r.k < a.limit) {
+        unsigned int last = 0u;                        // values of the last bin are many: counted apart
+        each([&](float value, int) {
+            if (spl_topk_key(value) == 0u) return;
+            const int b = bin_of(value);
+            if (b == SPL_SAMPLE_BINS - 1) ++last; else atomicAdd(&sh.lo[b], 1u);
+        });
+        last = __reduce_add_sync(0xffffffffu, last);
+        if (lane == 0 && last) atomicAdd(&sh.lo[SPL_SAMPLE_BINS - 1], last);
+        cluster.sync();
+        if (rank == 0) {
+            unsigned long long c0 = 0ull, c1 = 0ull, all;
+            for (int b = 0; b < blocks; ++b) { const SplSampleShared *peer = cluster.map_shared_rank(&sh, b); c0 += peer->lo[2 * tid]; c1 += peer->lo[2 * tid + 1]; }
+            const unsigned long long before = spl_sample_scan(c0 + c1, sh, &all);
+            sh.sums[2 * tid] = before + c0; sh.sums[2 * tid + 1] = before + c0 + c1;
+            const int b = spl_sample_place(sh, SPL_SAMPLE_BINS, (unsigned long long)r.k);
+            if (b == SPL_SAMPLE_BINS) decide(SPL_SAMPLE_WEIGH, 0, 0, 0ull);                                     // fewer values than k
+            else if (sh.sums[b] <= SPL_SAMPLE_LIST) decide(SPL_SAMPLE_FINISH, 0, b, 0ull);
+            else {
+                if (tid == 0) sh.value[1] = b ? sh.sums[b - 1] : 0ull;
+                decide(SPL_SAMPLE_CUT, b, b, 0ull);
+            }
+        }
+        cluster.sync();
+        step = sh.step;
+        if (step != SPL_SAMPLE_WEIGH) {
+            set_aside(sh.first_bin, sh.last_bin);
+            if (rank == 0) {
+                const int n = spl_sample_sorted(sh, cluster, blocks, r, 0ull);
+                if (n < 0) decide(SPL_SAMPLE_SLOW, 0, 0, 0ull);
+                else if (step == SPL_SAMPLE_CUT) decide(SPL_SAMPLE_WEIGH, 0, 0, sh.list[r.k - int(sh.value[1]) - 1]);
+                else {
+                    int stay = min(n, r.k);
+                    if (r.p < 1.0f) stay = min(stay, spl_sample_place(sh, stay, spl_sample_target(r.p, sh.sums[stay - 1])) + 1);
+                    if (r.least) {
+                        // Weights do not rise along the list.
+                        __syncthreads();
+                        if (tid == 0) sh.found = unsigned(stay);
+                        __syncthreads();
+                        for (int i = tid; i < stay; i += 1024)
+                            if (sh.sums[i] - (i ? sh.sums[i - 1] : 0ull) < r.least && (i == 0 || sh.sums[i - 1] - (i > 1 ? sh.sums[i - 2] : 0ull) >= r.least)) sh.found = unsigned(i);
+                        __syncthreads();
+                        stay = int(sh.found);
+                    }
+                    const int pick = spl_sample_place(sh, stay, spl_sample_target(r.u, sh.sums[stay - 1]));
+                    if (tid == 0) a.ids[row] = int32_t(~uint32_t(sh.list[pick]));
+                    decide(SPL_SAMPLE_DONE, 0, 0, 0ull);
+                }
+            }
+            cluster.sync();
+            step = sh.step;
+            cut = sh.cut;
+        }
+    }
+    if (step == SPL_SAMPLE_WEIGH) {
+        for (int i = tid; i < SPL_SAMPLE_BINS; i += 1024) { sh.lo[i] = 0u; sh.hi[i] = 0u; }
+        __syncthreads();
+        each([&](float value, int i) {
+            const uint32_t key = spl_topk_key(value);
+            if (key == 0u || (cut && spl_sample_entry(key, uint32_t(i)) < cut)) return;
+            const int b = bin_of(value);
+            if (b == SPL_SAMPLE_BINS - 1) return;
+            const unsigned long long w = spl_sample_weight(value, r.max_value, r.inv_t);
+            // Two words a bin, the carry taken by whoever makes the lower one overflow.
+            const unsigned int low = unsigned(w), was = atomicAdd(&sh.lo[b], low), high = unsigned(w >> 32) + (was + low < was ? 1u : 0u);
+            if (high) atomicAdd(&sh.hi[b], high);
+        });
+        cluster.sync();
+        // The first block: what stays ends in the bins [c0, c1], or nowhere before the last value.
+        int c0 = SPL_SAMPLE_BINS, c1 = -1, p_bin = SPL_SAMPLE_BINS;
+        unsigned long long p_target = 0ull, all = 0ull;
+        if (rank == 0) {
+            unsigned long long w0 = 0ull, w1 = 0ull;
+            for (int b = 0; b < blocks; ++b) {
+                const SplSampleShared *peer = cluster.map_shared_rank(&sh, b);
+                w0 += (unsigned long long)peer->hi[2 * tid] << 32 | peer->lo[2 * tid];
+                w1 += (unsigned long long)peer->hi[2 * tid + 1] << 32 | peer->lo[2 * tid + 1];
+            }
+            const unsigned long long before = spl_sample_scan(w0 + w1, sh, &all);
+            // (The list's sums take the same place later: the bins' sums go where the bins were.)
+            __syncthreads();
+            sh.sums[2 * tid] = before + w0; sh.sums[2 * tid + 1] = before + w0 + w1;
+            if (r.p < 1.0f) { p_target = spl_sample_target(r.p, all); p_bin = spl_sample_place(sh, SPL_SAMPLE_BINS, p_target); }
+            if (p_bin < SPL_SAMPLE_BINS) c0 = c1 = p_bin;
+            if (r.least) {
+                // Weights of m lie -ln m below the maximum; the bins next to that one may hold some, too, for the rounding of their place.
+                const int m_bin = int(fminf(fmaxf(-logf(r.m) * 64.0f, 0.0f), float(SPL_SAMPLE_BINS - 2))), m0 = max(m_bin - 1, 0), m1 = m_bin + 1;
+                if (p_bin > m1) { c0 = m0; c1 = m1; p_bin = SPL_SAMPLE_BINS; }      // top-p's place comes later
+                else if (p_bin >= m0) { c0 = m0; c1 = m1; }
+            }
+            if (c1 >= 0) decide(SPL_SAMPLE_END, c0, c1, cut);
+            else {
+                const int b = spl_sample_place(sh, SPL_SAMPLE_BINS, spl_sample_target(r.u, all));
+                decide(SPL_SAMPLE_DRAW, b, b, cut);
+            }
+            // The bins' sums are kept for the draw (the bins have been read).
+            __syncthreads();
+            unsigned long long *kept = reinterpret_cast<unsigned long long *>(sh.lo);      // lo and hi
+            for (int i = tid; i < SPL_SAMPLE_BINS; i += 1024) kept[i] = sh.sums[i];
+        }
+        cluster.sync();
+        step = sh.step;
+        const unsigned long long *kept = reinterpret_cast<const unsigned long long *>(sh.lo);
+        unsigned long long target = rank == 0 && step == SPL_SAMPLE_DRAW ? spl_sample_target(r.u, all) : 0ull;
+        if (step == SPL_SAMPLE_END) {
+            set_aside(sh.first_bin, sh.last_bin);
+            if (rank == 0) {
+                const unsigned long long base = c0 ? kept[c0 - 1] : 0ull;
+                const int n = spl_sample_sorted(sh, cluster, blocks, r, base);
+                if (n < 0) decide(SPL_SAMPLE_SLOW, 0, 0, 0ull);
+                else {
+                    int stay = n;
+                    if (p_bin < SPL_SAMPLE_BINS && n) stay = min(n, spl_sample_place(sh, n, p_target) + 1);
+                    if (r.least) {
+                        __syncthreads();
+                        if (tid == 0) sh.found = unsigned(stay);
+                        __syncthreads();
+                        for (int i = tid; i < stay; i += 1024) {
+                            const unsigned long long w = sh.sums[i] - (i ? sh.sums[i - 1] : base), previous = i ? sh.sums[i - 1] - (i > 1 ? sh.sums[i - 2] : base) : ~0ull;
+                            if (w < r.least && previous >= r.least) sh.found = unsigned(i);
+                        }
+                        __syncthreads();
+                        stay = int(sh.found);
+                    }
+                    target = spl_sample_target(r.u, stay ? sh.sums[stay - 1] : base);
+                    if (target > base || base == 0ull) {
+                        const int pick = spl_sample_place(sh, stay, target);
+                        if (tid == 0) a.ids[row] = int32_t(~uint32_t(sh.list[pick]));
+                        decide(SPL_SAMPLE_DONE, 0, 0, 0ull);
+                    } else {
+                        __syncthreads();
+                        for (int i = tid; i < SPL_SAMPLE_BINS; i += 1024) sh.sums[i] = kept[i];
+                        const int b = spl_sample_place(sh, SPL_SAMPLE_BINS, target);
+                        decide(SPL_SAMPLE_DRAW, b, b, cut);
+                    }
+                }
+            }
+            cluster.sync();
+            step = sh.step;
+        }
+        if (step == SPL_SAMPLE_DRAW) {
+            const int b = sh.first_bin;
+            set_aside(b, b);
+            if (rank == 0) {
+                const int n = spl_sample_sorted(sh, cluster, blocks, r, b ? kept[b - 1] : 0ull);
+                if (n < 0) decide(SPL_SAMPLE_SLOW, 0, 0, 0ull);
+                else {
+                    const int pick = spl_sample_place(sh, n, target);
+                    if (tid == 0) a.ids[row] = int32_t(~uint32_t(sh.list[pick]));
+                    decide(SPL_SAMPLE_DONE, 0, 0, 0ull);
+                }
+            }
+            cluster.sync();
+            step = sh.step;
+        }
+    }
+    if (step == SPL_SAMPLE_SLOW && rank == 0) spl_sample_slow(a, r, sh, row);
 }

@@ -86,6 +86,32 @@ def test_ties_go_to_the_lowest_index(engine):
         assert np.array_equal(device_sample(engine, x, width, settings, u), expected(x, width, settings, u))
 
 
+@pytest.mark.parametrize("temperature", [1e-3, 0.3, 3.0, 20.0, 1e4])
+def test_bins_of_few_and_of_very_many_values(engine, temperature):
+    """At low temperatures nearly everything lies in the last bin, at high ones everything in the first, which no list holds."""
+    rng = np.random.default_rng(6)
+    for width in (9000, 100003):
+        x, u = logits(rng, 7, width), rng.random(7).astype(np.float32)
+        for k, p, m in ((0, 1.0, 0.0), (0, 0.9, 0.0), (5000, 0.99, 0.0), (8000, 1.0, 0.3), (0, 0.5, 0.7), (30, 0.9, 0.2)):
+            assert np.array_equal(device_sample(engine, x, width, (temperature, k, p, m), u), expected(x, width, (temperature, k, p, m), u)), (k, p, m)
+
+
+@pytest.mark.parametrize("k", [2000, 4096, 4097, 6000, 20000, 70000])
+def test_a_large_top_k_and_the_other_filters_on_what_it_leaves(engine, k):
+    rng = np.random.default_rng(k)
+    x, u = logits(rng, 8, 80000), rng.random(8).astype(np.float32)
+    for settings in ((1.0, k, 1.0, 0.0), (1.0, k, 0.999, 0.0), (0.8, k, 0.7, 0.01), (2.0, k, 1.0, 0.02)):
+        assert np.array_equal(device_sample(engine, x, 80000, settings, u), expected(x, 80000, settings, u)), settings
+
+
+@pytest.mark.parametrize("width", [262144, 262145, 400001, 524288])
+def test_vocabularies_at_and_past_what_a_cluster_holds(engine, width):
+    rng = np.random.default_rng(width)
+    x, u = logits(rng, 3, width), rng.random(3).astype(np.float32)
+    for settings in ((None, None, None, None), (0.8, 50, 0.9, 0.01), (1.0, 9000, 0.95, 0.0), (0.0, None, None, None)):
+        assert np.array_equal(device_sample(engine, x, width, settings, u), expected(x, width, settings, u)), settings
+
+
 def test_values_that_are_never_picked(engine):
     rng = np.random.default_rng(8)
     width = 3000
