@@ -166,14 +166,15 @@ template <int HD, bool BF16> static void launch_attend(const spl_paged *p, const
                 reinterpret_cast<const SplPagedMerge *>(p->tables_dev + p->merges_at), p->shape, (const float *)p->partial, (const float2 *)p->partial_ml, p->slot_rows, a.out, a.out_f32);
 }
 
-// A cluster of blocks a row, as many as hold the row in shared memory (at most eight; more values than that are read in every pass).
+// A cluster of blocks a row: as many as hold the row in shared memory (at most eight; more values than that are read in every pass), and more where
+// SMs would be idle and each still has 4,096 values (one row of 32,000 takes ... in one block).
 static spl_status launch_sample(spl_engine *e, const SplSampleArgs &args, int rows, cudaStream_t stream) {
     int blocks = 1;
-    while (blocks < SPL_SAMPLE_CLUSTER && blocks * SPL_SAMPLE_STRETCH < args.limit) blocks *= 2;
+    while (blocks < SPL_SAMPLE_CLUSTER && (blocks * SPL_SAMPLE_STRETCH < args.limit || (rows * blocks * 2 <= e->sms && blocks * 8192 <= args.limit))) blocks *= 2;
     while (blocks > 1 && e->clusters[blocks] < 1) blocks /= 2;      // (a size the device cannot hold)
     const bool held = blocks * SPL_SAMPLE_STRETCH >= args.limit;
     void (*kernel)(SplSampleArgs) = held ? spl_sample_kernel<true> : spl_sample_kernel<false>;
-    const size_t smem = sizeof(SplSampleShared) + (held ? size_t(std::min(args.limit, SPL_SAMPLE_STRETCH)) * 4 : 0);
+    const size_t smem = sizeof(SplSampleShared) + (held ? size_t(((args.limit + blocks - 1) / blocks + 31) / 32 * 32) * 4 : 0);      // a block's stretch, as the kernel forms it
     SPL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(SplSampleShared) + SPL_SAMPLE_STRETCH * 4)));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(blocks, rows); cfg.blockDim = dim3(1024); cfg.dynamicSmemBytes = smem; cfg.stream = stream;
@@ -181,8 +182,8 @@ static spl_status launch_sample(spl_engine *e, const SplSampleArgs &args, int ro
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization; attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension; attr[1].val.clusterDim.x = blocks; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr; cfg.numAttrs = 2;
-    SPL_CUDA(cudaLaunchKernelEx(&cfg, kernel, args));
-    return SPL_OK;
+    cudaLaunchKernelEx(&cfg, kernel, args);
+    return check_launch(e, "sampling");
 }
 
 static bool misaligned(const void *p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes != 0; }

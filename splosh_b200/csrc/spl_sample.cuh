@@ -27,13 +27,27 @@ struct SplSampleArgs {
 };
 
 __device__ __forceinline__ float spl_topk_value(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key); }
-// The weight of a value, a whole number of 2^-44. (inf - inf is no number: the maximum itself has weight one, beside an infinite one nothing has any.)
-__device__ __forceinline__ unsigned long long spl_sample_weight(float x, float max, double inv_t) {
-    if (x == max) return 1ull << 44;
-    if (max == INFINITY || !(x > -INFINITY)) return 0ull;
-    return static_cast<unsigned long long>(exp((double(x) - double(max)) * inv_t) * SPL_SAMPLE_UNIT + 0.5);
+// The weight of a value, a whole number of 2^-44: 2^44 exp(z), z = (x - max) / T <= 0, rounded. With n = rint(64 z / ln 2) and f = z - n ln 2 / 64 (at most
+// 0.0055 in size), exp(z) = 2^(n / 64) exp(f): the power from a table of 64 (powers[j] = 2^(j / 64)) and an exponent, exp(f) its series to f^5 (the next term is 4e-17), all in
+// 64 bits; 2^52 added leaves the rounded whole number in the low bits. scale = 64 / (T ln 2). (inf - inf is no number: the maximum itself has weight one, beside an
+// infinite one nothing has any. Below -32 nothing is left of 2^44.)
+struct SplSampleWeigh { float max; double scale; const double *powers; };
+__device__ __forceinline__ unsigned long long spl_sample_weight(float x, const SplSampleWeigh &w) {
+    if (x == w.max) return 1ull << 44;
+    const double y = (double(x) - double(w.max)) * w.scale;
+    if (!(y > -32.0 * 64.0 / 0.693147180559945309417) || w.max == INFINITY) return 0ull;
+    const double magic = 6755399441055744.0, shifted = y + magic;               // 1.5 * 2^52: the low word of the sum is n
+    const int n = __double2loint(shifted);
+    const double f = (y - (shifted - magic)) * (0.693147180559945309417 / 64.0);
+    double e = fma(f, 1.0 / 120.0, 1.0 / 24.0);
+    e = fma(f, e, 1.0 / 6.0);
+    e = fma(f, e, 0.5);
+    e = fma(f, e, 1.0);
+    e = fma(f, e, 1.0);
+    const double power = w.powers[n & 63];
+    const double scaled = __hiloint2double(__double2hiint(power) + ((n >> 6) + 44) * (1 << 20), __double2loint(power));      // 2^(44 + n / 64), at least 2^-3
+    return (unsigned long long)__double_as_longlong(fma(scaled, e, 4503599627370496.0)) & ((1ull << 52) - 1ull);
 }
-
 
 // A cluster of blocks a row, 32,768 values a block in shared memory (a vocabulary of more than eight blocks' is read anew in every pass): the row comes
 // from memory once. The histogram has 2,048 bins of 1/64 in (max - x) / T, so that bins hold a few hundred values where a vocabulary's are densest; what is
@@ -55,6 +69,7 @@ struct SplSampleShared {
     unsigned long long sums[SPL_SAMPLE_LIST];                   // running sums of bins or of the sorted list (first block)
     unsigned long long best[SPL_SAMPLE_CLUSTER];                // the blocks' largest values
     unsigned long long warp_sum[32], value[4];
+    double powers[64];                                          // 2^(j / 64)
     unsigned int listed, found;
     // The first block's decision, in every block: which bins to set aside, or what has been decided.
     int step, first_bin, last_bin;
@@ -62,7 +77,7 @@ struct SplSampleShared {
 };
 enum { SPL_SAMPLE_DONE = 0, SPL_SAMPLE_FINISH, SPL_SAMPLE_CUT, SPL_SAMPLE_END, SPL_SAMPLE_DRAW, SPL_SAMPLE_WEIGH, SPL_SAMPLE_SLOW };
 
-struct SplSampleRow { float t, p, u, m, max_value, bin_scale; double inv_t; unsigned long long least; int k; };
+struct SplSampleRow { float t, p, u, m, bin_scale; SplSampleWeigh w; unsigned long long least; int k; };
 
 __device__ __forceinline__ unsigned long long spl_sample_entry(uint32_t key, uint32_t index) { return (unsigned long long)key << 32 | uint32_t(~index); }
 
@@ -120,7 +135,7 @@ __device__ __noinline__ void spl_sample_slow(const SplSampleArgs &a, const SplSa
                 const int i = base + tid;
                 const float v = i < a.limit ? x[i] : -INFINITY;
                 const uint32_t key = spl_topk_key(v);
-                const unsigned long long w = by_count ? 1ull : spl_sample_weight(v, r.max_value, r.inv_t);
+                const unsigned long long w = by_count ? 1ull : spl_sample_weight(v, r.w);
                 const bool counts = key >= cut_key && key != 0u && (shift == 24 || (key >> (shift + 8)) == prefix) && (by_count || w >= least);
                 const unsigned int votes = __ballot_sync(0xffffffffu, counts);
                 if (!votes) continue;
@@ -154,7 +169,7 @@ __device__ __noinline__ void spl_sample_slow(const SplSampleArgs &a, const SplSa
             before = sh.value[0];
         }
         *key_out = prefix;
-        const unsigned long long each = by_count ? 1ull : spl_sample_weight(spl_topk_value(prefix), r.max_value, r.inv_t);
+        const unsigned long long each = by_count ? 1ull : spl_sample_weight(spl_topk_value(prefix), r.w);
         *ties_out = target <= before + 1ull || each == 0ull ? 1ull : (target - before + each - 1ull) / each;
     };
     // The weight of all that stays.
@@ -169,13 +184,13 @@ __device__ __noinline__ void spl_sample_slow(const SplSampleArgs &a, const SplSa
             const uint32_t key = spl_topk_key(v);
             if (key < cut_key || key == 0u) continue;
             if (key == cut_key) { ++ties; continue; }
-            const unsigned long long w = spl_sample_weight(v, r.max_value, r.inv_t);
+            const unsigned long long w = spl_sample_weight(v, r.w);
             if (w >= least) sum += w;
         }
         if (sum) atomicAdd(&mass[0], sum);
         if (ties) atomicAdd(&count[0], ties);
         __syncthreads();
-        const unsigned long long each = spl_sample_weight(spl_topk_value(cut_key), r.max_value, r.inv_t);
+        const unsigned long long each = spl_sample_weight(spl_topk_value(cut_key), r.w);
         sum = mass[0];
         if (count[0] && each >= least) sum += each * min((unsigned long long)count[0], cut_ties);
         return sum;
@@ -209,21 +224,49 @@ __device__ __noinline__ void spl_sample_slow(const SplSampleArgs &a, const SplSa
 // The first block: the blocks' lists into its own, sorted, with running sums of weights that begin at `base`. Returns the entries, or -1 where
 // they do not fit.
 __device__ __forceinline__ int spl_sample_sorted(SplSampleShared &sh, cooperative_groups::cluster_group &cluster, int blocks, const SplSampleRow &r, unsigned long long base) {
-    const int tid = threadIdx.x;
-    unsigned int n = sh.listed;
-    for (int b = 1; b < blocks; ++b) {
-        const SplSampleShared *peer = cluster.map_shared_rank(&sh, b);
-        const unsigned int more = peer->listed;
-        if (n + more <= SPL_SAMPLE_LIST) for (unsigned int i = tid; i < more; i += 1024) sh.list[n + i] = peer->list[i];
-        n += more;
-    }
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    // Each warp works out where the blocks' lists go; the lists of the others are copied side by side, four warps each.
+    unsigned int n = lane < blocks ? cluster.map_shared_rank(&sh, lane)->listed : 0u;
+    const unsigned int mine = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const unsigned int y = __shfl_up_sync(0xffffffffu, n, o); if (lane >= o) n += y; }
+    const unsigned int from = warp / 4, start = __shfl_sync(0xffffffffu, n - mine, from), more = __shfl_sync(0xffffffffu, mine, from);
+    n = __shfl_sync(0xffffffffu, n, 31);
     if (n > SPL_SAMPLE_LIST) return -1;
-    unsigned int width = 2;
+    if (from > 0 && int(from) < blocks) {
+        const SplSampleShared *peer = cluster.map_shared_rank(&sh, from);
+        for (unsigned int i = (warp & 3) * 32 + lane; i < more; i += 128) sh.list[start + i] = peer->list[i];
+    }
+    unsigned int width = 32;
     while (width < n) width <<= 1;
-    __syncthreads();
     for (unsigned int i = n + tid; i < width; i += 1024) sh.list[i] = 0ull;
-    for (unsigned int size = 2; size <= width; size <<= 1)
-        for (unsigned int stride = size >> 1; stride > 0; stride >>= 1) {
+    __syncthreads();
+    // Bitonic, descending: what meets within 32 entries in registers, the rest through shared memory.
+    auto within = [&](unsigned int size, unsigned int first_stride) {
+        for (unsigned int i = tid; i < width; i += 1024) {
+            unsigned long long v = sh.list[i];
+            for (unsigned int stride = first_stride; stride > 0; stride >>= 1) {
+                const unsigned long long other = __shfl_xor_sync(0xffffffffu, v, stride);
+                const bool larger = ((i & stride) == 0) == ((i & size) == 0);      // this entry takes the larger of the two
+                v = (v > other) == larger ? v : other;
+            }
+            sh.list[i] = v;
+        }
+    };
+    for (unsigned int i = tid; i < width; i += 1024) {
+        unsigned long long v = sh.list[i];
+#pragma unroll
+        for (unsigned int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+            for (unsigned int stride = size >> 1; stride > 0; stride >>= 1) {
+                const unsigned long long other = __shfl_xor_sync(0xffffffffu, v, stride);
+                const bool larger = ((i & stride) == 0) == ((i & size) == 0);
+                v = (v > other) == larger ? v : other;
+            }
+        sh.list[i] = v;
+    }
+    for (unsigned int size = 64; size <= width; size <<= 1) {
+        for (unsigned int stride = size >> 1; stride >= 32; stride >>= 1) {
             __syncthreads();
             for (unsigned int q = tid; q < width / 2; q += 1024) {
                 const unsigned int i = 2 * q - (q & (stride - 1)), j = i + stride;
@@ -231,13 +274,16 @@ __device__ __forceinline__ int spl_sample_sorted(SplSampleShared &sh, cooperativ
                 if ((x < y) == ((i & size) == 0)) { sh.list[i] = y; sh.list[j] = x; }
             }
         }
+        __syncthreads();
+        within(size, 16);
+    }
     __syncthreads();
     unsigned long long w[SPL_SAMPLE_LIST / 1024], run = 0ull, all;
     const int per = width <= 1024 ? 1 : int(width / 1024);
 #pragma unroll
     for (int e = 0; e < SPL_SAMPLE_LIST / 1024; ++e) {
         const unsigned int i = tid * per + e;
-        w[e] = e < per && i < n ? spl_sample_weight(spl_topk_value(uint32_t(sh.list[i] >> 32)), r.max_value, r.inv_t) : 0ull;
+        w[e] = e < per && i < n ? spl_sample_weight(spl_topk_value(uint32_t(sh.list[i] >> 32)), r.w) : 0ull;
         run += w[e];
     }
     run = base + spl_sample_scan(run, sh, &all);
@@ -262,7 +308,7 @@ spl_sample_kernel(SplSampleArgs a) {
     spl_grid_begin();
     const int row = blockIdx.y, rank = blockIdx.x, blocks = gridDim.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const float *x = a.logits + size_t(row) * a.ld;
-    const int stretch = HELD ? SPL_SAMPLE_STRETCH : ((a.limit + blocks - 1) / blocks + 1023) / 1024 * 1024, begin = rank * stretch, end = min(a.limit, begin + stretch);
+    const int stretch = ((a.limit + blocks - 1) / blocks + 31) / 32 * 32, begin = rank * stretch, end = min(a.limit, begin + stretch);
     float *held = reinterpret_cast<float *>(spl_sample_raw + sizeof(SplSampleShared));
     const float *mine = x + begin;
     const int count = max(0, end - begin);
@@ -283,18 +329,24 @@ spl_sample_kernel(SplSampleArgs a) {
     // The largest value and its lowest index.
     {
         uint32_t key = 0u, index = 0u;
-#pragma unroll 8
-        for (int i = tid; i < count; i += 1024) {
-            const float value = mine[i];
-            if (HELD) held[i] = value;
-            const uint32_t y = spl_topk_key(value);
-            if (y > key) { key = y; index = uint32_t(begin + i); }
+        for (int base = 0; base < count; base += 16 * 1024) {      // sixteen loads on their way
+            float value[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) { const int i = base + e * 1024 + tid; value[e] = i < count ? mine[i] : -INFINITY; }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int i = base + e * 1024 + tid;
+                if (HELD && i < count) held[i] = value[e];
+                const uint32_t y = spl_topk_key(value[e]);
+                if (y > key) { key = y; index = uint32_t(begin + i); }
+            }
         }
         const uint32_t all = __reduce_max_sync(0xffffffffu, key);
         const uint32_t first = __reduce_min_sync(0xffffffffu, key == all ? index : 0xffffffffu);
         if (lane == 0) sh.warp_sum[warp] = spl_sample_entry(all, first);
         for (int i = tid; i < SPL_SAMPLE_BINS; i += 1024) { sh.lo[i] = 0u; sh.hi[i] = 0u; }
         if (tid == 0) sh.listed = 0u;
+        if (tid < 64) sh.powers[tid] = exp2(double(tid) / 64.0);
         __syncthreads();
         unsigned long long best = 0ull;
         if (warp == 0) {
@@ -313,18 +365,23 @@ spl_sample_kernel(SplSampleArgs a) {
         if (rank == 0 && tid == 0) a.ids[row] = nothing ? 0 : int32_t(~uint32_t(top));
         return;
     }
-    r.max_value = spl_topk_value(uint32_t(top >> 32));
-    r.inv_t = 1.0 / double(r.t);
+    r.w.max = spl_topk_value(uint32_t(top >> 32));
+    r.w.scale = 64.0 / 0.693147180559945309417 / double(r.t);
+    r.w.powers = sh.powers;
     r.bin_scale = fminf(128.0f / r.t, 3.0e38f);
-    const bool endless = r.max_value == INFINITY;
+    const bool endless = r.w.max == INFINITY;
     // The bin of a value that may be picked (halved values do not overflow; rounding keeps the order).
     auto bin_of = [&](float value) {
-        if (value == r.max_value) return 0;
-        return endless ? SPL_SAMPLE_BINS - 1 : int(fminf((0.5f * r.max_value - 0.5f * value) * r.bin_scale, float(SPL_SAMPLE_BINS - 1)));
+        if (value == r.w.max) return 0;
+        return endless ? SPL_SAMPLE_BINS - 1 : int(fminf((0.5f * r.w.max - 0.5f * value) * r.bin_scale, float(SPL_SAMPLE_BINS - 1)));
     };
     unsigned long long cut = 0ull;                     // entries below it are out
     auto set_aside = [&](int first_bin, int last_bin) {
+        // Most values are told by two comparisons: bounds a bin and the roundings outside the bins asked for.
+        const float width = r.t / 64.0f, slack = width + 1e-6f * fabsf(r.w.max), high = r.w.max - float(first_bin) * width + slack;
+        const float low = last_bin == SPL_SAMPLE_BINS - 1 ? -INFINITY : r.w.max - float(last_bin + 1) * width - slack;
         each([&](float value, int i) {
+            if (value > high || value < low) return;
             const uint32_t key = spl_topk_key(value);
             if (key == 0u) return;
             const int b = bin_of(value);
@@ -357,7 +414,12 @@ spl_sample_kernel(SplSampleArgs a) {
         cluster.sync();
         if (rank == 0) {
             unsigned long long c0 = 0ull, c1 = 0ull, all;
-            for (int b = 0; b < blocks; ++b) { const SplSampleShared *peer = cluster.map_shared_rank(&sh, b); c0 += peer->lo[2 * tid]; c1 += peer->lo[2 * tid + 1]; }
+            // (A block past the last is the first again, left out: the loads of all are on their way together.)
+#pragma unroll
+            for (int b = 0; b < SPL_SAMPLE_CLUSTER; ++b) {
+                const uint2 y = *reinterpret_cast<const uint2 *>(&cluster.map_shared_rank(&sh, b < blocks ? b : 0)->lo[2 * tid]);
+                if (b < blocks) { c0 += y.x; c1 += y.y; }
+            }
             const unsigned long long before = spl_sample_scan(c0 + c1, sh, &all);
             sh.sums[2 * tid] = before + c0; sh.sums[2 * tid + 1] = before + c0 + c1;
             const int b = spl_sample_place(sh, SPL_SAMPLE_BINS, (unsigned long long)r.k);
@@ -407,7 +469,7 @@ spl_sample_kernel(SplSampleArgs a) {
             if (key == 0u || (cut && spl_sample_entry(key, uint32_t(i)) < cut)) return;
             const int b = bin_of(value);
             if (b == SPL_SAMPLE_BINS - 1) return;
-            const unsigned long long w = spl_sample_weight(value, r.max_value, r.inv_t);
+            const unsigned long long w = spl_sample_weight(value, r.w);
             // Two words a bin, the carry taken by whoever makes the lower one overflow.
             const unsigned int low = unsigned(w), was = atomicAdd(&sh.lo[b], low), high = unsigned(w >> 32) + (was + low < was ? 1u : 0u);
             if (high) atomicAdd(&sh.hi[b], high);
@@ -418,10 +480,11 @@ spl_sample_kernel(SplSampleArgs a) {
         unsigned long long p_target = 0ull, all = 0ull;
         if (rank == 0) {
             unsigned long long w0 = 0ull, w1 = 0ull;
-            for (int b = 0; b < blocks; ++b) {
-                const SplSampleShared *peer = cluster.map_shared_rank(&sh, b);
-                w0 += (unsigned long long)peer->hi[2 * tid] << 32 | peer->lo[2 * tid];
-                w1 += (unsigned long long)peer->hi[2 * tid + 1] << 32 | peer->lo[2 * tid + 1];
+#pragma unroll
+            for (int b = 0; b < SPL_SAMPLE_CLUSTER; ++b) {
+                const SplSampleShared *peer = cluster.map_shared_rank(&sh, b < blocks ? b : 0);
+                const uint2 low = *reinterpret_cast<const uint2 *>(&peer->lo[2 * tid]), high = *reinterpret_cast<const uint2 *>(&peer->hi[2 * tid]);
+                if (b < blocks) { w0 += (unsigned long long)high.x << 32 | low.x; w1 += (unsigned long long)high.y << 32 | low.y; }
             }
             const unsigned long long before = spl_sample_scan(w0 + w1, sh, &all);
             // (The list's sums take the same place later: the bins' sums go where the bins were.)
