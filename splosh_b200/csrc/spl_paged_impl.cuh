@@ -166,13 +166,24 @@ template <int HD, bool BF16> static void launch_attend(const spl_paged *p, const
                 reinterpret_cast<const SplPagedMerge *>(p->tables_dev + p->merges_at), p->shape, (const float *)p->partial, (const float2 *)p->partial_ml, p->slot_rows, a.out, a.out_f32);
 }
 
-// A cluster of blocks a row: as many as hold the row in shared memory (at most eight; more values than that are read in every pass), and more where
-// SMs would be idle and each still has 4,096 values (one row of 32,000 takes ... in one block).
+// The blocks of a row's cluster: a wave of clusters costs some 14 us of meetings and sorting whatever a block's share, and 19 us for 32,768 values a block (they fit
+// its shared memory; a larger share is read from L2 in every pass, at the same pace). 64 rows of 248,077 take 132 us in four waves of clusters of eight and @64@ in
+// one wave of pairs; twelve rows 42 us in eights, @12@ in pairs.
+static int sample_blocks(const spl_engine *e, int rows, int limit) {
+    int best = 1;
+    double least = 0.0;
+    for (int blocks = 1; blocks <= SPL_SAMPLE_CLUSTER; blocks *= 2) {
+        const int resident = e->clusters[blocks];
+        if (resident < 1) continue;      // a size the device cannot hold
+        const double cost = double((rows + resident - 1) / resident) * (14.0 + 19.0 * ((limit + blocks - 1) / blocks) / SPL_SAMPLE_STRETCH);
+        if (blocks == 1 || cost < least) { best = blocks; least = cost; }
+    }
+    return best;
+}
+
 static spl_status launch_sample(spl_engine *e, const SplSampleArgs &args, int rows, cudaStream_t stream) {
-    int blocks = 1;
-    while (blocks < SPL_SAMPLE_CLUSTER && (blocks * SPL_SAMPLE_STRETCH < args.limit || (rows * blocks * 2 <= e->sms && blocks * 8192 <= args.limit))) blocks *= 2;
-    while (blocks > 1 && e->clusters[blocks] < 1) blocks /= 2;      // (a size the device cannot hold)
-    const bool held = blocks * SPL_SAMPLE_STRETCH >= args.limit;
+    const int blocks = sample_blocks(e, rows, args.limit);
+    const bool held = blocks * SPL_SAMPLE_STRETCH >= args.limit;      // a block's share fits its shared memory
     void (*kernel)(SplSampleArgs) = held ? spl_sample_kernel<true> : spl_sample_kernel<false>;
     const size_t smem = sizeof(SplSampleShared) + (held ? size_t(((args.limit + blocks - 1) / blocks + 31) / 32 * 32) * 4 : 0);      // a block's stretch, as the kernel forms it
     SPL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(SplSampleShared) + SPL_SAMPLE_STRETCH * 4)));

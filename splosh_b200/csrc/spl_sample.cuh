@@ -32,25 +32,30 @@ __device__ __forceinline__ float spl_topk_value(uint32_t key) { return __uint_as
 // 64 bits; 2^52 added leaves the rounded whole number in the low bits. scale = 64 / (T ln 2). (inf - inf is no number: the maximum itself has weight one, beside an
 // infinite one nothing has any. Below -32 nothing is left of 2^44.)
 struct SplSampleWeigh { float max; double scale; const double *powers; };
+// (The value is the maximum or less than 33 below it times T.)
+__device__ __forceinline__ unsigned long long spl_sample_weight_near(float x, const SplSampleWeigh &w) {
+    const double d = double(x) - double(w.max);
+    const double magic = 6755399441055744.0, shifted = fma(d, w.scale, magic);      // 1.5 * 2^52: the low word of the sum is n
+    const int n = __double2loint(shifted);
+    const double g = fma(d, w.scale, magic - shifted);                              // f = g ln 2 / 64; the series in g
+    constexpr double c = 0.693147180559945309417 / 64.0;
+    double e = fma(g, c * c * c * c * c / 120.0, c * c * c * c / 24.0);
+    e = fma(g, e, c * c * c / 6.0);
+    e = fma(g, e, c * c / 2.0);
+    e = fma(g, e, c);
+    e = fma(g, e, 1.0);
+    const double power = w.powers[n & 63];
+    const double scaled = __hiloint2double(__double2hiint(power) + ((n >> 6) + 44) * (1 << 20), __double2loint(power));      // 2^(44 + n / 64), at least 2^-4
+    return (unsigned long long)__double_as_longlong(fma(scaled, e, 4503599627370496.0)) & ((1ull << 52) - 1ull);
+}
 __device__ __forceinline__ unsigned long long spl_sample_weight(float x, const SplSampleWeigh &w) {
     if (x == w.max) return 1ull << 44;
-    const double y = (double(x) - double(w.max)) * w.scale;
-    if (!(y > -32.0 * 64.0 / 0.693147180559945309417) || w.max == INFINITY) return 0ull;
-    const double magic = 6755399441055744.0, shifted = y + magic;               // 1.5 * 2^52: the low word of the sum is n
-    const int n = __double2loint(shifted);
-    const double f = (y - (shifted - magic)) * (0.693147180559945309417 / 64.0);
-    double e = fma(f, 1.0 / 120.0, 1.0 / 24.0);
-    e = fma(f, e, 1.0 / 6.0);
-    e = fma(f, e, 0.5);
-    e = fma(f, e, 1.0);
-    e = fma(f, e, 1.0);
-    const double power = w.powers[n & 63];
-    const double scaled = __hiloint2double(__double2hiint(power) + ((n >> 6) + 44) * (1 << 20), __double2loint(power));      // 2^(44 + n / 64), at least 2^-3
-    return (unsigned long long)__double_as_longlong(fma(scaled, e, 4503599627370496.0)) & ((1ull << 52) - 1ull);
+    if (w.max == INFINITY || !((double(x) - double(w.max)) * w.scale > -32.0 * 64.0 / 0.693147180559945309417)) return 0ull;
+    return spl_sample_weight_near(x, w);
 }
 
 // A cluster of blocks a row, 32,768 values a block in shared memory (a vocabulary of more than eight blocks' is read anew in every pass): the row comes
-// from memory once. The histogram has 2,048 bins of 1/64 in (max - x) / T, so that bins hold a few hundred values where a vocabulary's are densest; what is
+// from memory once. The histogram has 4,096 bins of 1/128 in (max - x) / T, so that bins hold a few hundred values where a vocabulary's are densest; what is
 // 31.98 and more below the maximum has no weight in whole numbers of 2^-44 and is the last bin. The first block of the cluster adds the blocks' bins, finds the bin
 // that a place lies in, and sorts that bin's values, which the blocks have set aside:
 //   top-k         counts; the bins down to the k-th value's are sorted whole where they fit (SPL_SAMPLE_LIST), and everything else is decided on
@@ -58,12 +63,13 @@ __device__ __forceinline__ unsigned long long spl_sample_weight(float x, const S
 //   then          weights; the bins of top-p's place and of min-p's bound are sorted for the exact end of what stays, and then the draw's bin
 // A bin of more values than the list holds (equal logits, very high temperatures) leaves the row to the first block, which finds places eight bits of
 // the values' keys at a time (spl_sample_slow).
-#define SPL_SAMPLE_BINS 2048
+#define SPL_SAMPLE_BINS 4096
+#define SPL_SAMPLE_BINS_NAT 128.0f             // bins a natural unit of (max - x) / T
 #define SPL_SAMPLE_LIST 4096
 #define SPL_SAMPLE_STRETCH 32768
 #define SPL_SAMPLE_CLUSTER 8
 
-struct SplSampleShared {
+struct __align__(128) SplSampleShared {
     unsigned int lo[SPL_SAMPLE_BINS], hi[SPL_SAMPLE_BINS];      // the bins: counts in lo, or weights in both
     unsigned long long list[SPL_SAMPLE_LIST];                   // values set aside: key << 32 | ~index, so that descending order is the definition's
     unsigned long long sums[SPL_SAMPLE_LIST];                   // running sums of bins or of the sorted list (first block)
@@ -72,7 +78,7 @@ struct SplSampleShared {
     double powers[64];                                          // 2^(j / 64)
     unsigned int listed, found;
     // The first block's decision, in every block: which bins to set aside, or what has been decided.
-    int step, first_bin, last_bin;
+    int step, first_bin, last_bin, also_bin;
     unsigned long long cut;
 };
 enum { SPL_SAMPLE_DONE = 0, SPL_SAMPLE_FINISH, SPL_SAMPLE_CUT, SPL_SAMPLE_END, SPL_SAMPLE_DRAW, SPL_SAMPLE_WEIGH, SPL_SAMPLE_SLOW };
@@ -99,6 +105,34 @@ __device__ __forceinline__ unsigned long long spl_sample_scan(unsigned long long
     __syncthreads();
     *total = sh.warp_sum[31];
     return (warp ? sh.warp_sum[warp - 1] : 0ull) + run - v;
+}
+// A block's share of the bins, all blocks' added, into the first block's sums. (A block past the last is the first again, left out: the loads of all are on
+// their way together.)
+__device__ __forceinline__ void spl_sample_add_blocks(SplSampleShared &sh, cooperative_groups::cluster_group &cluster, int rank, int blocks) {
+    const int share = SPL_SAMPLE_BINS / blocks;
+    unsigned long long *sums = cluster.map_shared_rank(&sh, 0)->sums;
+    for (int i = rank * share + threadIdx.x; i < (rank + 1) * share; i += 1024) {
+        unsigned int lo[SPL_SAMPLE_CLUSTER], hi[SPL_SAMPLE_CLUSTER];
+#pragma unroll
+        for (int b = 0; b < SPL_SAMPLE_CLUSTER; ++b) {
+            const SplSampleShared *peer = cluster.map_shared_rank(&sh, b < blocks ? b : 0);
+            lo[b] = peer->lo[i]; hi[b] = peer->hi[i];
+        }
+        unsigned long long sum = 0ull;
+#pragma unroll
+        for (int b = 0; b < SPL_SAMPLE_CLUSTER; ++b) if (b < blocks) sum += (unsigned long long)hi[b] << 32 | lo[b];
+        sums[i] = sum;
+    }
+}
+// The first block's sums of bins into running sums.
+__device__ __forceinline__ void spl_sample_running(SplSampleShared &sh, unsigned long long *total) {
+    unsigned long long v[SPL_SAMPLE_BINS / 1024], run = 0ull;
+#pragma unroll
+    for (int q = 0; q < SPL_SAMPLE_BINS / 1024; ++q) { v[q] = sh.sums[SPL_SAMPLE_BINS / 1024 * threadIdx.x + q]; run += v[q]; }
+    run = spl_sample_scan(run, sh, total);
+#pragma unroll
+    for (int q = 0; q < SPL_SAMPLE_BINS / 1024; ++q) { run += v[q]; sh.sums[SPL_SAMPLE_BINS / 1024 * threadIdx.x + q] = run; }
+    __syncthreads();
 }
 // The first place of [0, n) whose sums[] reaches `target` (n: none); the sums do not fall. All threads get it.
 __device__ __forceinline__ int spl_sample_place(SplSampleShared &sh, int n, unsigned long long target) {
@@ -313,12 +347,23 @@ spl_sample_kernel(SplSampleArgs a) {
     const float *mine = x + begin;
     const int count = max(0, end - begin);
     asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");      // (a block's shared memory may be reached when it has begun)
-    // Every thread of the block runs f(value, index) for its values, a warp's in step.
+    // Every thread of the block runs f(four values, index of the first, step of the index) for its values; past the row's end a value is -inf.
     auto each = [&](auto &&f) {
-#pragma unroll 4
-        for (int base = 0; base < count; base += 1024) {
-            const int i = base + tid;
-            f(i < count ? (HELD ? held[i] : mine[i]) : -INFINITY, begin + i);
+        if constexpr (HELD) {
+#pragma unroll 2
+            for (int i = 4 * tid; i < stretch; i += 4096) {
+                const float4 four = *reinterpret_cast<const float4 *>(held + i);
+                const float value[4] = {four.x, four.y, four.z, four.w};
+                f(value, begin + i, 1);
+            }
+        } else {
+#pragma unroll 2
+            for (int i = tid; i < count; i += 4096) {
+                float value[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) value[q] = i + q * 1024 < count ? mine[i + q * 1024] : -INFINITY;
+                f(value, begin + i, 1024);
+            }
         }
     };
     SplSampleRow r;
@@ -329,14 +374,14 @@ spl_sample_kernel(SplSampleArgs a) {
     // The largest value and its lowest index.
     {
         uint32_t key = 0u, index = 0u;
-        for (int base = 0; base < count; base += 16 * 1024) {      // sixteen loads on their way
+        for (int base = 0; base < (HELD ? stretch : count); base += 16 * 1024) {      // sixteen loads on their way
             float value[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) { const int i = base + e * 1024 + tid; value[e] = i < count ? mine[i] : -INFINITY; }
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 const int i = base + e * 1024 + tid;
-                if (HELD && i < count) held[i] = value[e];
+                if (HELD && i < stretch) held[i] = value[e];
                 const uint32_t y = spl_topk_key(value[e]);
                 if (y > key) { key = y; index = uint32_t(begin + i); }
             }
@@ -368,60 +413,64 @@ spl_sample_kernel(SplSampleArgs a) {
     r.w.max = spl_topk_value(uint32_t(top >> 32));
     r.w.scale = 64.0 / 0.693147180559945309417 / double(r.t);
     r.w.powers = sh.powers;
-    r.bin_scale = fminf(128.0f / r.t, 3.0e38f);
-    const bool endless = r.w.max == INFINITY;
-    // The bin of a value that may be picked (halved values do not overflow; rounding keeps the order).
+    r.bin_scale = fminf(2.0f * SPL_SAMPLE_BINS_NAT / r.t, 3.0e38f);
+    // The bin of a value that may be picked: halved values do not overflow, and rounding keeps the order (it may put a value in the next bin, no more). Beside an
+    // infinite maximum the finite values are binned as beside the largest one (they have no weight).
+    const float half_max = 0.5f * fminf(r.w.max, 3.402823466e38f);
     auto bin_of = [&](float value) {
-        if (value == r.w.max) return 0;
-        return endless ? SPL_SAMPLE_BINS - 1 : int(fminf((0.5f * r.w.max - 0.5f * value) * r.bin_scale, float(SPL_SAMPLE_BINS - 1)));
+        return __float_as_int(fminf(fmaxf(fmaf(-0.5f, value, half_max) * r.bin_scale, 0.0f), float(SPL_SAMPLE_BINS - 1)) + 8388608.0f) & (SPL_SAMPLE_BINS - 1);
     };
     unsigned long long cut = 0ull;                     // entries below it are out
-    auto set_aside = [&](int first_bin, int last_bin) {
-        // Most values are told by two comparisons: bounds a bin and the roundings outside the bins asked for.
-        const float width = r.t / 64.0f, slack = width + 1e-6f * fabsf(r.w.max), high = r.w.max - float(first_bin) * width + slack;
-        const float low = last_bin == SPL_SAMPLE_BINS - 1 ? -INFINITY : r.w.max - float(last_bin + 1) * width - slack;
-        each([&](float value, int i) {
-            if (value > high || value < low) return;
+    // The values of the bins [first, last] and of bin `also` (in front of them, or negative) into the block's list.
+    auto set_aside = [&](int first, int last, int also) {
+        // Most values are told by comparisons: bounds a bin and the roundings outside the bins asked for.
+        const float width = r.t / SPL_SAMPLE_BINS_NAT, slack = 2.0f * width + 1e-6f * fabsf(r.w.max);
+        auto top_of = [&](int b) { return r.w.max - float(b) * width + slack; };
+        auto bottom_of = [&](int b) { return b == SPL_SAMPLE_BINS - 1 ? -INFINITY : r.w.max - float(b + 1) * width - slack; };
+        const float high = top_of(first), low = bottom_of(last), also_high = also < 0 ? -INFINITY : top_of(also), also_low = also < 0 ? INFINITY : bottom_of(also);
+        auto near = [&](float value) { return !(value > high || value < low) || !(value > also_high || value < also_low); };
+        auto keep = [&](float value, int i) {
             const uint32_t key = spl_topk_key(value);
-            if (key == 0u) return;
             const int b = bin_of(value);
-            if (b < first_bin || b > last_bin) return;
+            if (key == 0u || ((b < first || b > last) && b != also)) return;
             const unsigned long long entry = spl_sample_entry(key, uint32_t(i));
             if (entry < cut) return;
             const unsigned int at = atomicAdd(&sh.listed, 1u);
             if (at < SPL_SAMPLE_LIST) sh.list[at] = entry;
+        };
+        each([&](const float (&value)[4], int i, int step) {
+            if (!(near(value[0]) | near(value[1]) | near(value[2]) | near(value[3]))) return;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) keep(value[q], i + q * step);
         });
         cluster.sync();
     };
     // The first block's decision goes to all of them; what their lists held has been read.
-    auto decide = [&](int step, int first_bin, int last_bin, unsigned long long new_cut) {
+    auto decide = [&](int step, int first_bin, int last_bin, unsigned long long new_cut, int also_bin = -1) {
         __syncthreads();
         if (tid < blocks) {
             SplSampleShared *peer = cluster.map_shared_rank(&sh, tid);
-            peer->step = step; peer->first_bin = first_bin; peer->last_bin = last_bin; peer->cut = new_cut; peer->listed = 0u;
+            peer->step = step; peer->first_bin = first_bin; peer->last_bin = last_bin; peer->also_bin = also_bin; peer->cut = new_cut; peer->listed = 0u;
         }
     };
     int step = SPL_SAMPLE_WEIGH;
     if (r.k > 0 && r.k < a.limit) {
         unsigned int last = 0u;                        // values of the last bin are many: counted apart
-        each([&](float value, int) {
-            if (spl_topk_key(value) == 0u) return;
-            const int b = bin_of(value);
-            if (b == SPL_SAMPLE_BINS - 1) ++last; else atomicAdd(&sh.lo[b], 1u);
+        each([&](const float (&value)[4], int, int) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int b = bin_of(value[q]);
+                if (value[q] > -INFINITY) { if (b == SPL_SAMPLE_BINS - 1) ++last; else atomicAdd(&sh.lo[b], 1u); }
+            }
         });
         last = __reduce_add_sync(0xffffffffu, last);
         if (lane == 0 && last) atomicAdd(&sh.lo[SPL_SAMPLE_BINS - 1], last);
         cluster.sync();
+        spl_sample_add_blocks(sh, cluster, rank, blocks);
+        cluster.sync();
         if (rank == 0) {
-            unsigned long long c0 = 0ull, c1 = 0ull, all;
-            // (A block past the last is the first again, left out: the loads of all are on their way together.)
-#pragma unroll
-            for (int b = 0; b < SPL_SAMPLE_CLUSTER; ++b) {
-                const uint2 y = *reinterpret_cast<const uint2 *>(&cluster.map_shared_rank(&sh, b < blocks ? b : 0)->lo[2 * tid]);
-                if (b < blocks) { c0 += y.x; c1 += y.y; }
-            }
-            const unsigned long long before = spl_sample_scan(c0 + c1, sh, &all);
-            sh.sums[2 * tid] = before + c0; sh.sums[2 * tid + 1] = before + c0 + c1;
+            unsigned long long all;
+            spl_sample_running(sh, &all);
             const int b = spl_sample_place(sh, SPL_SAMPLE_BINS, (unsigned long long)r.k);
             if (b == SPL_SAMPLE_BINS) decide(SPL_SAMPLE_WEIGH, 0, 0, 0ull);                                     // fewer values than k
             else if (sh.sums[b] <= SPL_SAMPLE_LIST) decide(SPL_SAMPLE_FINISH, 0, b, 0ull);
@@ -433,7 +482,7 @@ spl_sample_kernel(SplSampleArgs a) {
         cluster.sync();
         step = sh.step;
         if (step != SPL_SAMPLE_WEIGH) {
-            set_aside(sh.first_bin, sh.last_bin);
+            set_aside(sh.first_bin, sh.last_bin, -1);
             if (rank == 0) {
                 const int n = spl_sample_sorted(sh, cluster, blocks, r, 0ull);
                 if (n < 0) decide(SPL_SAMPLE_SLOW, 0, 0, 0ull);
@@ -464,78 +513,107 @@ spl_sample_kernel(SplSampleArgs a) {
     if (step == SPL_SAMPLE_WEIGH) {
         for (int i = tid; i < SPL_SAMPLE_BINS; i += 1024) { sh.lo[i] = 0u; sh.hi[i] = 0u; }
         __syncthreads();
-        each([&](float value, int i) {
-            const uint32_t key = spl_topk_key(value);
-            if (key == 0u || (cut && spl_sample_entry(key, uint32_t(i)) < cut)) return;
-            const int b = bin_of(value);
-            if (b == SPL_SAMPLE_BINS - 1) return;
-            const unsigned long long w = spl_sample_weight(value, r.w);
-            // Two words a bin, the carry taken by whoever makes the lower one overflow.
-            const unsigned int low = unsigned(w), was = atomicAdd(&sh.lo[b], low), high = unsigned(w >> 32) + (was + low < was ? 1u : 0u);
-            if (high) atomicAdd(&sh.hi[b], high);
+        each([&](const float (&value)[4], int i, int step) {
+            // The four weights side by side (a weight is a chain of ten 64-bit operations), whatever of them counts.
+            unsigned long long w[4];
+            int b[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) { b[q] = bin_of(value[q]); w[q] = spl_sample_weight_near(value[q], r.w); }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const uint32_t key = spl_topk_key(value[q]);
+                if (b[q] == SPL_SAMPLE_BINS - 1 || key == 0u || (cut && spl_sample_entry(key, uint32_t(i + q * step)) < cut)) continue;
+                if (r.w.max == INFINITY) { if (value[q] != r.w.max) continue; w[q] = 1ull << 44; }
+                // Two words a bin, the carry taken by whoever makes the lower one overflow.
+                const unsigned int low = unsigned(w[q]), was = atomicAdd(&sh.lo[b[q]], low), high = unsigned(w[q] >> 32) + (was + low < was ? 1u : 0u);
+                if (high) atomicAdd(&sh.hi[b[q]], high);
+            }
         });
         cluster.sync();
+        spl_sample_add_blocks(sh, cluster, rank, blocks);
+        cluster.sync();
         // The first block: what stays ends in the bins [c0, c1], or nowhere before the last value.
-        int c0 = SPL_SAMPLE_BINS, c1 = -1, p_bin = SPL_SAMPLE_BINS;
+        int c0 = SPL_SAMPLE_BINS, c1 = -1, p_bin = SPL_SAMPLE_BINS, also = -1;
         unsigned long long p_target = 0ull, all = 0ull;
         if (rank == 0) {
-            unsigned long long w0 = 0ull, w1 = 0ull;
-#pragma unroll
-            for (int b = 0; b < SPL_SAMPLE_CLUSTER; ++b) {
-                const SplSampleShared *peer = cluster.map_shared_rank(&sh, b < blocks ? b : 0);
-                const uint2 low = *reinterpret_cast<const uint2 *>(&peer->lo[2 * tid]), high = *reinterpret_cast<const uint2 *>(&peer->hi[2 * tid]);
-                if (b < blocks) { w0 += (unsigned long long)high.x << 32 | low.x; w1 += (unsigned long long)high.y << 32 | low.y; }
-            }
-            const unsigned long long before = spl_sample_scan(w0 + w1, sh, &all);
-            // (The list's sums take the same place later: the bins' sums go where the bins were.)
-            __syncthreads();
-            sh.sums[2 * tid] = before + w0; sh.sums[2 * tid + 1] = before + w0 + w1;
+            spl_sample_running(sh, &all);
+            // The bins' sums, here for the places below and, where the bins were, for the draw.
+            unsigned long long *keep = reinterpret_cast<unsigned long long *>(sh.lo);      // lo and hi
+            for (int i = tid; i < SPL_SAMPLE_BINS; i += 1024) keep[i] = sh.sums[i];
             if (r.p < 1.0f) { p_target = spl_sample_target(r.p, all); p_bin = spl_sample_place(sh, SPL_SAMPLE_BINS, p_target); }
             if (p_bin < SPL_SAMPLE_BINS) c0 = c1 = p_bin;
             if (r.least) {
                 // Weights of m lie -ln m below the maximum; the bins next to that one may hold some, too, for the rounding of their place.
-                const int m_bin = int(fminf(fmaxf(-logf(r.m) * 64.0f, 0.0f), float(SPL_SAMPLE_BINS - 2))), m0 = max(m_bin - 1, 0), m1 = m_bin + 1;
+                const int m_bin = int(fminf(fmaxf(-logf(r.m) * SPL_SAMPLE_BINS_NAT, 0.0f), float(SPL_SAMPLE_BINS - 2))), m0 = max(m_bin - 1, 0), m1 = m_bin + 1;
                 if (p_bin > m1) { c0 = m0; c1 = m1; p_bin = SPL_SAMPLE_BINS; }      // top-p's place comes later
                 else if (p_bin >= m0) { c0 = m0; c1 = m1; }
             }
-            if (c1 >= 0) decide(SPL_SAMPLE_END, c0, c1, cut);
-            else {
+            if (c1 >= 0) {
+                // Whatever of the bins [c0, c1] stays, the draw mostly lies in one and the same bin: set aside with them, it is found in the same list.
+                const unsigned long long least_sum = c0 ? sh.sums[c0 - 1] : 0ull;
+                const int d0 = spl_sample_place(sh, SPL_SAMPLE_BINS, spl_sample_target(r.u, least_sum)), d1 = spl_sample_place(sh, SPL_SAMPLE_BINS, spl_sample_target(r.u, sh.sums[c1]));
+                if (d0 == d1 && d1 < c0) also = d1;
+                decide(SPL_SAMPLE_END, c0, c1, cut, also);
+            } else {
                 const int b = spl_sample_place(sh, SPL_SAMPLE_BINS, spl_sample_target(r.u, all));
                 decide(SPL_SAMPLE_DRAW, b, b, cut);
             }
-            // The bins' sums are kept for the draw (the bins have been read).
-            __syncthreads();
-            unsigned long long *kept = reinterpret_cast<unsigned long long *>(sh.lo);      // lo and hi
-            for (int i = tid; i < SPL_SAMPLE_BINS; i += 1024) kept[i] = sh.sums[i];
         }
         cluster.sync();
         step = sh.step;
         const unsigned long long *kept = reinterpret_cast<const unsigned long long *>(sh.lo);
         unsigned long long target = rank == 0 && step == SPL_SAMPLE_DRAW ? spl_sample_target(r.u, all) : 0ull;
         if (step == SPL_SAMPLE_END) {
-            set_aside(sh.first_bin, sh.last_bin);
+            set_aside(sh.first_bin, sh.last_bin, sh.also_bin);
             if (rank == 0) {
-                const unsigned long long base = c0 ? kept[c0 - 1] : 0ull;
-                const int n = spl_sample_sorted(sh, cluster, blocks, r, base);
+                // The list: the draw's bin where it came along (entries [0, front)), then the bins what stays ends in, running sums from `base`.
+                const unsigned long long base = c0 ? kept[c0 - 1] : 0ull, also_base = also > 0 ? kept[also - 1] : 0ull, also_sum = also < 0 ? 0ull : kept[also] - also_base;
+                const int n = spl_sample_sorted(sh, cluster, blocks, r, base - also_sum);
                 if (n < 0) decide(SPL_SAMPLE_SLOW, 0, 0, 0ull);
                 else {
+                    int front = 0;
+                    if (also >= 0) {
+                        __syncthreads();
+                        if (tid == 0) sh.found = unsigned(n);
+                        __syncthreads();
+                        for (int i = tid; i < n; i += 1024) {
+                            auto in_front = [&](int e) { return bin_of(spl_topk_value(uint32_t(sh.list[e] >> 32))) == also; };
+                            if (!in_front(i) && (i == 0 || in_front(i - 1))) sh.found = unsigned(i);
+                        }
+                        __syncthreads();
+                        front = int(sh.found);
+                    }
                     int stay = n;
-                    if (p_bin < SPL_SAMPLE_BINS && n) stay = min(n, spl_sample_place(sh, n, p_target) + 1);
+                    if (p_bin < SPL_SAMPLE_BINS && n > front) {
+                        __syncthreads();
+                        if (tid == 0) sh.found = unsigned(n);
+                        __syncthreads();
+                        for (int i = front + tid; i < n; i += 1024) if (sh.sums[i] >= p_target && (i == front || sh.sums[i - 1] < p_target)) sh.found = unsigned(i);
+                        __syncthreads();
+                        stay = min(n, int(sh.found) + 1);
+                    }
                     if (r.least) {
                         __syncthreads();
                         if (tid == 0) sh.found = unsigned(stay);
                         __syncthreads();
-                        for (int i = tid; i < stay; i += 1024) {
-                            const unsigned long long w = sh.sums[i] - (i ? sh.sums[i - 1] : base), previous = i ? sh.sums[i - 1] - (i > 1 ? sh.sums[i - 2] : base) : ~0ull;
-                            if (w < r.least && previous >= r.least) sh.found = unsigned(i);
-                        }
+                        auto weight_of = [&](int e) { return spl_sample_weight(spl_topk_value(uint32_t(sh.list[e] >> 32)), r.w); };      // does not rise along the list
+                        for (int i = front + tid; i < stay; i += 1024) if (weight_of(i) < r.least && (i == front || weight_of(i - 1) >= r.least)) sh.found = unsigned(i);
                         __syncthreads();
                         stay = int(sh.found);
                     }
-                    target = spl_sample_target(r.u, stay ? sh.sums[stay - 1] : base);
-                    if (target > base || base == 0ull) {
-                        const int pick = spl_sample_place(sh, stay, target);
-                        if (tid == 0) a.ids[row] = int32_t(~uint32_t(sh.list[pick]));
+                    target = spl_sample_target(r.u, stay > front ? sh.sums[stay - 1] : base);
+                    int from = -1, to = stay;
+                    unsigned long long shift = 0ull;
+                    if (target > base || base == 0ull) from = front;
+                    else if (also >= 0 && target > also_base && target <= also_base + also_sum) { from = 0; to = front; shift = base - also_sum - also_base; }
+                    else if (also == 0) { from = 0; to = front; shift = base - also_sum; }      // a target of nothing: the first value
+                    if (from >= 0) {
+                        __syncthreads();
+                        if (tid == 0) sh.found = unsigned(to - 1);
+                        __syncthreads();
+                        for (int i = from + tid; i < to; i += 1024) if (sh.sums[i] - shift >= target && (i == from || sh.sums[i - 1] - shift < target)) sh.found = unsigned(i);
+                        __syncthreads();
+                        if (tid == 0) a.ids[row] = int32_t(~uint32_t(sh.list[sh.found]));
                         decide(SPL_SAMPLE_DONE, 0, 0, 0ull);
                     } else {
                         __syncthreads();
@@ -550,7 +628,7 @@ spl_sample_kernel(SplSampleArgs a) {
         }
         if (step == SPL_SAMPLE_DRAW) {
             const int b = sh.first_bin;
-            set_aside(b, b);
+            set_aside(b, b, -1);
             if (rank == 0) {
                 const int n = spl_sample_sorted(sh, cluster, blocks, r, b ? kept[b - 1] : 0ull);
                 if (n < 0) decide(SPL_SAMPLE_SLOW, 0, 0, 0ull);
