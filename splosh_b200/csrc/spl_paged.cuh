@@ -126,9 +126,11 @@ spl_paged_append_kernel(SplPagedRows in, const uint16_t *__restrict__ q_norm, co
 // tokens, verify blocks and prompt chunks are one kernel) against tiles of 128 tokens. Per tile
 //   S[128 rows x 128 tokens]   = Q[128 x HD] K^T          A = Q, B = K          (shared memory, K-major)
 //   O[128 rows x HD]          += P[128 x 128] V           A = P (tensor memory), B = V (shared memory, tokens along the contraction)
-// with the softmax between them. Keys and values come as chunks of 128 tokens x 64 channels (16 KB, 128-byte swizzle), one ring for both in the
-// order the products take them: K of tile 0; K of tile i + 1, V of tile i; ... A page smaller than a tile is a copy of its own, so page sizes and
-// head layouts are the tensor map's business alone.
+// with the softmax between them. Keys come as chunks of 128 tokens x 64 channels, values as chunks of 8192 / HD tokens x all channels (16 KB each, 128-byte
+// swizzle), one ring for both in the order the products take them: K of tile 0; K of tile i + 1, V of tile i; ... A page smaller than a chunk's tokens is a copy
+// of its own, so page sizes and head layouts are the tensor maps' business alone.
+// An instruction of the value product spans all HD columns of O: with values in chunks of 64 channels it took HD / 64 times as many instructions of 64 columns, and the
+// issuing warp (some 100 cycles an instruction) was the block's pace: 5,000 of 6,450 cycles a tile at HD = 256.
 //
 // Warps 0-7 softmax (thread: a row and half of the tile's tokens; the pair of warps of 32 rows agrees on the maximum), warp 8 copies, warp 9 issues
 // both products: S of tile i + 1 runs under the softmax of tile i. The reference is raised only when a row's maximum exceeds it by 2^8, so the sums in
@@ -170,6 +172,14 @@ __device__ __forceinline__ void spl_tc_ld32(uint32_t (&r)[32], uint32_t taddr) {
                    "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
                    "=r"(r[31]) : "r"(taddr));
 }
+__device__ __forceinline__ void spl_tma_load5(void *smem, const CUtensorMap *map, int x, int token, int block, int head, int page, uint64_t *bar) {
+    asm volatile("cp.async.bulk.tensor.5d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];\n"
+                 ::"r"(spl_smem_addr(smem)), "l"(map), "r"(x), "r"(token), "r"(block), "r"(head), "r"(page), "r"(spl_smem_addr(bar)) : "memory");
+}
+// MN-major, 128-byte swizzle: rows of 64 elements (128 bytes) along the contraction, eight-row groups 1,024 bytes apart, the next 64 elements of a row `block_bytes` on.
+__device__ __forceinline__ uint64_t spl_tc_desc_mn_sw128(uint32_t smem_byte_addr, uint32_t block_bytes) {
+    return (spl_tc_desc_sw128(smem_byte_addr) & ~(uint64_t(0x3FFF) << 16)) | uint64_t(block_bytes >> 4) << 16;
+}
 // A box of a tensor map into shared memory; the innermost coordinate is a multiple of 64 elements.
 __device__ __forceinline__ void spl_tma_load4(void *smem, const CUtensorMap *map, int x, int token, int head, int page, uint64_t *bar) {
     asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];\n"
@@ -195,7 +205,7 @@ struct SplPagedAttend {
 template <int HD, bool BF16>
 __global__ void __launch_bounds__(SPL_PAGED_THREADS, 1)
 spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, SplPagedTables t, SplPagedShape s, SplPagedAttend a) {
-    constexpr int C = HD / 64, NST = spl_paged_ring(HD), CHUNK = SPL_PAGED_CHUNK;
+    constexpr int C = HD / 64, VT = 128 / C, NST = spl_paged_ring(HD), CHUNK = SPL_PAGED_CHUNK;      // VT: tokens a chunk of values
     constexpr float PBIAS = BF16 ? 0.0f : 7.0f;
     extern __shared__ unsigned char spl_paged_raw[];
     unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(spl_paged_raw) + 1023) & ~uintptr_t(1023));
@@ -235,15 +245,29 @@ spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
         // ---- copies. Lane b brings the tile's b-th page (or its half of a page of 256); a chunk's barrier counts the pages that hold tokens.
         const int box = min(s.page_tokens, 128), boxes = 128 / box;
         int n = 0;                                            // chunks so far
-        auto bring = [&](const CUtensorMap *map, const SplPagedItem &it, int tile, int page, int present) {
+        auto next = [&]() {                                   // room for a chunk
+            if (ok && !spl_mbar_wait_warp(&empty[n % NST], ((n / NST) & 1) ^ 1, const_cast<const int *>(abort))) gave_up(60);
+            return ok;
+        };
+        // Lane b holds the page of the tile's b-th box of tokens; `present` of them hold tokens. inside: where a tile begins in a page of 256.
+        auto bring_k = [&](const SplPagedItem &it, int inside, int page, int present) {
             for (int c = 0; c < C; ++c, ++n) {
+                if (!next()) return;
                 const int st = n % NST;
-                if (ok && !spl_mbar_wait_warp(&empty[st], ((n / NST) & 1) ^ 1, const_cast<const int *>(abort))) gave_up(60);
-                if (!ok) return;
                 if (lane == 0) spl_mbar_expect_tx(&full[st], uint32_t(present * box) * 128);
                 __syncwarp();
-                if (lane < present)
-                    spl_tma_load4(ring + st * CHUNK + lane * box * 128, map, c * 64, s.page_tokens > 128 ? (tile & 1) * 128 : 0, it.kv_head, page, &full[st]);
+                if (lane < present) spl_tma_load4(ring + st * CHUNK + lane * box * 128, &k_map, c * 64, inside, it.kv_head, page, &full[st]);
+            }
+        };
+        const int vbox = min(s.page_tokens, VT), vboxes = VT / vbox, per_page = box / vbox;      // boxes a chunk of values, boxes a lane's page
+        auto bring_v = [&](const SplPagedItem &it, int inside, int page, int tokens) {
+            for (int c = 0; c < C; ++c, ++n) {
+                if (!next()) return;
+                const int st = n % NST, b = c * vboxes + lane;                                  // lane's box of the tile
+                const int there = min(vboxes, max(0, (tokens - c * VT + vbox - 1) / vbox)), from = __shfl_sync(0xffffffffu, page, lane < vboxes ? b / per_page : 0);
+                if (lane == 0) spl_mbar_expect_tx(&full[st], uint32_t(there) * vbox * HD * 2);
+                __syncwarp();
+                if (lane < there) spl_tma_load5(ring + st * CHUNK + lane * vbox * HD * 2, &v_map, 0, inside + b % per_page * vbox, 0, it.kv_head, from, &full[st]);
             }
         };
         for (int i = item0; i < item1 && ok; ++i) {
@@ -252,12 +276,13 @@ spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
             const int *pages = t.table + size_t(it.sequence) * s.max_pages;
             auto present_of = [&](int tile) { return min(boxes, (length - tile * 128 + box - 1) / box); };
             auto page_of = [&](int tile) { return tile < it.tile_end && lane < present_of(tile) ? pages[s.page_tokens > 128 ? tile >> 1 : tile * boxes + lane] : 0; };
+            auto inside_of = [&](int tile) { return s.page_tokens > 128 ? (tile & 1) * 128 : 0; };
             int page = page_of(it.tile_begin), ahead = page_of(it.tile_begin + 1);
-            bring(&k_map, it, it.tile_begin, page, present_of(it.tile_begin));
+            bring_k(it, inside_of(it.tile_begin), page, present_of(it.tile_begin));
             for (int tile = it.tile_begin; tile < it.tile_end && ok; ++tile) {
                 const int later = page_of(tile + 2);
-                if (tile + 1 < it.tile_end) bring(&k_map, it, tile + 1, ahead, present_of(tile + 1));
-                if (ok) bring(&v_map, it, tile, page, present_of(tile));
+                if (tile + 1 < it.tile_end) bring_k(it, inside_of(tile + 1), ahead, present_of(tile + 1));
+                if (ok) bring_v(it, inside_of(tile), page, min(128, length - tile * 128));
                 page = ahead; ahead = later;
             }
         }
@@ -265,8 +290,10 @@ spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
         for (int st = 0; st < NST && st < n; ++st) { const int last = st + (n - 1 - st) / NST * NST; spl_mbar_wait(&full[st], (last / NST) & 1); }
     } else if (warp == 9) {
         // ---- both products, one elected lane of a converged warp.
-        constexpr uint32_t s_idesc = spl_paged_idesc(128, BF16, false), o_idesc = spl_paged_idesc(64, BF16, true);
-        const uint64_t q_desc = spl_tc_desc_sw128(spl_smem_addr(q_tile)), ring_desc = spl_tc_desc_sw128(spl_smem_addr(ring));
+        constexpr uint32_t s_idesc = spl_paged_idesc(128, BF16, false), o_idesc = spl_paged_idesc(HD, BF16, true);
+        const int vbox = min(s.page_tokens, VT);
+        const uint64_t q_desc = spl_tc_desc_sw128(spl_smem_addr(q_tile)), ring_desc = spl_tc_desc_sw128(spl_smem_addr(ring)), v_desc = spl_tc_desc_mn_sw128(spl_smem_addr(ring), vbox * 128);
+        const uint32_t v_box_step = uint32_t(vbox) * HD * 2, vlog = 31 - __clz(vbox);
         int n = 0, tiles = 0, pieces = 0;                     // chunks, tiles and pieces so far
         // Scores of tile number `at` of this block. They go where the P of tile at - 2 lies, which has to have been read.
         auto scores = [&](int at) {
@@ -297,23 +324,34 @@ spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
             for (int tile = it.tile_begin; tile < it.tile_end && ok; ++tile, ++tiles) {
                 if (tile + 1 < it.tile_end) scores(tiles + 1);
                 if (ok && !spl_mbar_wait_warp(&p_full[tiles & 1], (tiles >> 1) & 1, const_cast<const int *>(abort))) gave_up(64);
-                const int from = max(0, seen_first - tile * 128), to = min(128, seen_last - tile * 128), k0 = from / 16, k1 = (to + 15) / 16;
+                const int from = max(0, seen_first - tile * 128), to = min(128, seen_last - tile * 128);
+                const uint32_t p_at = tmem + (tiles & 1) * 128;
                 for (int c = 0; c < C && ok; ++c, ++n) {
                     const int st = n % NST;
                     if (!spl_mbar_wait_warp(&full[st], (n / NST) & 1, const_cast<const int *>(abort))) { gave_up(65); break; }
-                    if (from % 16 || to % 16) {
+                    const int f = min(max(from - c * VT, 0), VT), e = min(max(to - c * VT, 0), VT), k0 = f / 16, k1 = (e + 15) / 16;      // the chunk's tokens that some row sees
+                    if (f % 16 || e % 16) {
                         // Values of unseen tokens in the first and last groups of sixteen: zero, whatever the cache holds there.
-                        unsigned char *rows = ring + st * CHUNK;
-                        const int before = from % 16 * 8, after = (16 - to % 16) % 16 * 8;
-                        for (int z = lane; z < before + after; z += 32)
-                            *reinterpret_cast<uint4 *>(rows + (z < before ? k0 * 2048 + z * 16 : to * 128 + (z - before) * 16)) = make_uint4(0, 0, 0, 0);
+                        const int before = f % 16, after = (16 - e % 16) % 16;
+                        for (int z = lane; z < (before + after) * C * 8; z += 32) {
+                            const int row = z / (C * 8), token = row < before ? k0 * 16 + row : e + row - before, piece = z % (C * 8);
+                            *reinterpret_cast<uint4 *>(ring + st * CHUNK + token / vbox * v_box_step + (piece >> 3) * vbox * 128 + token % vbox * 128 + (piece & 7) * 16) = make_uint4(0, 0, 0, 0);
+                        }
                         spl_fence_proxy_async();
                         __syncwarp();
                     }
                     spl_tc_fence_after();
+                    const uint64_t chunk = v_desc + uint64_t((st * CHUNK) >> 4);
+                    // The piece's first product overwrites what O held.
+                    const uint32_t onto = tile > it.tile_begin || c * VT + k0 * 16 > from / 16 * 16 ? 1u : 0u;
                     if (spl_elect_one()) {
-                        for (int ks = k0; ks < k1; ++ks)
-                            spl_tc_mma_ts(tmem_o + c * 64, tmem + (tiles & 1) * 128 + ks * 8, ring_desc + uint64_t((st * CHUNK + ks * 2048) >> 4), o_idesc, tile > it.tile_begin || ks > k0 ? 1u : 0u);
+                        auto place = [&](int ks) { return chunk + uint64_t((((ks * 16) >> vlog) * v_box_step + ((ks * 16) & (vbox - 1)) * 128) >> 4); };
+                        if (k0 == 0 && k1 == VT / 16) {
+#pragma unroll
+                            for (int ks = 0; ks < VT / 16; ++ks) spl_tc_mma_ts(tmem_o, p_at + (c * (VT / 16) + ks) * 8, place(ks), o_idesc, ks > 0 ? 1u : onto);
+                        } else {
+                            for (int ks = k0; ks < k1; ++ks) spl_tc_mma_ts(tmem_o, p_at + (c * (VT / 16) + ks) * 8, place(ks), o_idesc, ks > k0 ? 1u : onto);
+                        }
                         spl_tc_commit(&empty[st]);
                         if (c == C - 1) spl_tc_commit(&o_done[tiles & 1]);
                     }

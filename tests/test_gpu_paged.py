@@ -280,3 +280,17 @@ def test_refusals(engine):
         paged.append(a, a, a, a, a, a)
     assert "one page" in str(caught.value)
     paged.close()
+
+
+@pytest.mark.parametrize("head_dim", [64, 128, 256])
+@pytest.mark.parametrize("page_tokens", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("window", [64, 65, 96, 100, 128, 200])
+def test_windows_that_begin_anywhere_in_a_tile(engine, head_dim, page_tokens, window):
+    """The first chunks of a piece's first tile are left out, and its first product begins in the middle of a chunk or at its start; everything in front is NaN."""
+    lengths = [256, 300, 129, 192]
+    scene = Scene(window + page_tokens, 2, 1, head_dim, [1] * 4, lengths, page_tokens=page_tokens, window=window)
+    for cache in (scene.k, scene.v):
+        for s, length in enumerate(lengths):
+            for token in range(length - window):
+                cache[scene.table[s, token // page_tokens], :, token % page_tokens] = float("nan")
+    check_attention(scene, attend(engine, scene, "f32"), "f32")
