@@ -154,10 +154,18 @@ __host__ __device__ constexpr size_t spl_paged_smem_bytes(int hd) {
 __device__ __forceinline__ int spl_paged_first(const SplPagedShape &s, int position) { return s.window > 0 && position + 1 > s.window ? position + 1 - s.window : 0; }
 __device__ __forceinline__ int spl_paged_last(const SplPagedShape &s, int position, int length) { return s.causal ? position + 1 : length; }
 
-// D[tmem] (+)= A[smem] * B[smem]; one thread issues.
-__device__ __forceinline__ void spl_tc_mma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n"
-                 ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+// D[tmem] (+)= A * B with A and B in shared memory, or A in tensor memory; issued by the lane with `elected` set, in the converged warp's control flow: descriptors are
+// formed in uniform registers, which a branch around the instructions prevents (150 cycles an instruction).
+__device__ __forceinline__ void spl_tc_mma_ss_if(uint32_t elected, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n .reg .pred p, e;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 e, %5, 0;\n @e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n"
+                 ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(elected) : "memory");
+}
+__device__ __forceinline__ void spl_tc_mma_ts_if(uint32_t elected, uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n .reg .pred p, e;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 e, %5, 0;\n @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
+                 ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(elected) : "memory");
+}
+__device__ __forceinline__ void spl_tc_commit_if(uint32_t elected, uint64_t *bar) {
+    asm volatile("{\n .reg .pred e;\n setp.ne.b32 e, %1, 0;\n @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(spl_smem_addr(bar)), "r"(elected) : "memory");
 }
 // The instruction descriptor of spl_tc_idesc for either type; the value product's B has its tokens (the contraction) in rows: MN-major.
 __host__ __device__ constexpr uint32_t spl_paged_idesc(int n, bool bf16, bool b_mn) {
@@ -294,23 +302,22 @@ spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
         const int vbox = min(s.page_tokens, VT);
         const uint64_t q_desc = spl_tc_desc_sw128(spl_smem_addr(q_tile)), ring_desc = spl_tc_desc_sw128(spl_smem_addr(ring)), v_desc = spl_tc_desc_mn_sw128(spl_smem_addr(ring), vbox * 128);
         const uint32_t v_box_step = uint32_t(vbox) * HD * 2, vlog = 31 - __clz(vbox);
+        const uint32_t elected = spl_elect_one() ? 1u : 0u;
         int n = 0, tiles = 0, pieces = 0;                     // chunks, tiles and pieces so far
         // Scores of tile number `at` of this block. They go where the P of tile at - 2 lies, which has to have been read.
         auto scores = [&](int at) {
             if (ok && at >= 2 && !spl_mbar_wait_warp(&o_done[at & 1], ((at - 2) >> 1) & 1, const_cast<const int *>(abort))) gave_up(61);
+#pragma unroll
             for (int c = 0; c < C; ++c, ++n) {
                 const int st = n % NST;
                 if (ok && !spl_mbar_wait_warp(&full[st], (n / NST) & 1, const_cast<const int *>(abort))) gave_up(62);
                 if (!ok) return;
                 spl_tc_fence_after();
-                if (spl_elect_one()) {
 #pragma unroll
-                    for (int ks = 0; ks < 4; ++ks)
-                        spl_tc_mma_ss(tmem + (at & 1) * 128, q_desc + uint64_t((c * CHUNK + ks * 32) >> 4), ring_desc + uint64_t((st * CHUNK + ks * 32) >> 4), s_idesc, c + ks > 0 ? 1u : 0u);
-                    spl_tc_commit(&empty[st]);
-                    if (c == C - 1) spl_tc_commit(&s_full[at & 1]);
-                }
-                __syncwarp();
+                for (int ks = 0; ks < 4; ++ks)
+                    spl_tc_mma_ss_if(elected, tmem + (at & 1) * 128, q_desc + uint64_t((c * CHUNK + ks * 32) >> 4), ring_desc + uint64_t((st * CHUNK + ks * 32) >> 4), s_idesc, c + ks > 0 ? 1u : 0u);
+                spl_tc_commit_if(elected, &empty[st]);
+                if (c == C - 1) spl_tc_commit_if(elected, &s_full[at & 1]);
             }
         };
         for (int i = item0; i < item1 && ok; ++i, ++pieces) {
@@ -344,24 +351,20 @@ spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
                     const uint64_t chunk = v_desc + uint64_t((st * CHUNK) >> 4);
                     // The piece's first product overwrites what O held.
                     const uint32_t onto = tile > it.tile_begin || c * VT + k0 * 16 > from / 16 * 16 ? 1u : 0u;
-                    if (spl_elect_one()) {
-                        auto place = [&](int ks) { return chunk + uint64_t((((ks * 16) >> vlog) * v_box_step + ((ks * 16) & (vbox - 1)) * 128) >> 4); };
-                        if (k0 == 0 && k1 == VT / 16) {
+                    auto place = [&](int ks) { return chunk + uint64_t((((ks * 16) >> vlog) * v_box_step + ((ks * 16) & (vbox - 1)) * 128) >> 4); };
+                    if (k0 == 0 && k1 == VT / 16) {
 #pragma unroll
-                            for (int ks = 0; ks < VT / 16; ++ks) spl_tc_mma_ts(tmem_o, p_at + (c * (VT / 16) + ks) * 8, place(ks), o_idesc, ks > 0 ? 1u : onto);
-                        } else {
-                            for (int ks = k0; ks < k1; ++ks) spl_tc_mma_ts(tmem_o, p_at + (c * (VT / 16) + ks) * 8, place(ks), o_idesc, ks > k0 ? 1u : onto);
-                        }
-                        spl_tc_commit(&empty[st]);
-                        if (c == C - 1) spl_tc_commit(&o_done[tiles & 1]);
+                        for (int ks = 0; ks < VT / 16; ++ks) spl_tc_mma_ts_if(elected, tmem_o, p_at + (c * (VT / 16) + ks) * 8, place(ks), o_idesc, ks > 0 ? 1u : onto);
+                    } else {
+                        for (int ks = k0; ks < k1; ++ks) spl_tc_mma_ts_if(elected, tmem_o, p_at + (c * (VT / 16) + ks) * 8, place(ks), o_idesc, ks > k0 ? 1u : onto);
                     }
-                    __syncwarp();
+                    spl_tc_commit_if(elected, &empty[st]);
+                    if (c == C - 1) spl_tc_commit_if(elected, &o_done[tiles & 1]);
                 }
             }
         }
         // No product may still read shared or write tensor memory when they are handed on.
-        if (spl_elect_one()) spl_tc_commit(drained);
-        __syncwarp();
+        spl_tc_commit_if(elected, drained);
         spl_mbar_wait(drained, 0);
     } else {
         // ---- softmax: row r of the piece, tokens [64 half, 64 half + 64) of a tile.
