@@ -126,8 +126,8 @@ spl_paged_append_kernel(SplPagedRows in, const uint16_t *__restrict__ q_norm, co
 // tokens, verify blocks and prompt chunks are one kernel) against tiles of 128 tokens. Per tile
 //   S[128 rows x 128 tokens]   = Q[128 x HD] K^T          A = Q, B = K          (shared memory, K-major)
 //   O[128 rows x HD]          += P[128 x 128] V           A = P (tensor memory), B = V (shared memory, tokens along the contraction)
-// with the softmax between them. Keys come as chunks of 128 tokens x 64 channels, values as chunks of 8192 / HD tokens x all channels (16 KB each, 128-byte
-// swizzle), one ring for both in the order the products take them: K of tile 0; K of tile i + 1, V of tile i; ... A page smaller than a chunk's tokens is a copy
+// with the softmax between them. Keys come as chunks of 128 tokens x up to 128 channels, values as chunks of up to 128 tokens x all channels (a tile at HD of 64
+// and 128, half a tile at 256; 128-byte swizzle), one ring for both in the order the products take them: K of tile 0; K of tile i + 1, V of tile i; ... A page smaller than a chunk's tokens is a copy
 // of its own, so page sizes and head layouts are the tensor maps' business alone.
 // An instruction of the value product spans all HD columns of O: with values in chunks of 64 channels it took HD / 64 times as many instructions of 64 columns, and the
 // issuing warp (some 100 cycles an instruction) was the block's pace: 5,000 of 6,450 cycles a tile at HD = 256.
@@ -143,11 +143,11 @@ spl_paged_append_kernel(SplPagedRows in, const uint16_t *__restrict__ q_norm, co
 // What is masked may be anything: a masked score is replaced before it is used, and because 0 x inf is no number, tokens that no row of the piece
 // sees (behind the sequence's last token, in front of the window) have their values zeroed in shared memory or are left out of the product.
 #define SPL_PAGED_THREADS 320
-#define SPL_PAGED_CHUNK 16384
 #define SPL_PAGED_HEADROOM 8.0f
-__host__ __device__ constexpr int spl_paged_ring(int hd) { return hd == 256 ? 9 : hd == 128 ? 11 : 12; }
+__host__ __device__ constexpr int spl_paged_chunk(int hd) { return hd == 64 ? 16384 : 32768; }
+__host__ __device__ constexpr int spl_paged_ring(int hd) { return hd == 256 ? 4 : hd == 128 ? 5 : 12; }
 __host__ __device__ constexpr size_t spl_paged_smem_bytes(int hd) {
-    return 1024 + size_t(hd / 64 + spl_paged_ring(hd)) * SPL_PAGED_CHUNK + 2 * 2 * 128 * 4 /* maxima */ + 2 * 128 * 4 /* sums */ + 512 /* barriers */;
+    return 1024 + size_t(hd) * 256 + size_t(spl_paged_ring(hd)) * spl_paged_chunk(hd) + 2 * 2 * 128 * 4 /* maxima */ + 2 * 128 * 4 /* sums */ + 512 /* barriers */;
 }
 
 // Tokens that the row at `position` of a sequence of `length` tokens sees: [first, last).
@@ -213,11 +213,11 @@ struct SplPagedAttend {
 template <int HD, bool BF16>
 __global__ void __launch_bounds__(SPL_PAGED_THREADS, 1)
 spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, SplPagedTables t, SplPagedShape s, SplPagedAttend a) {
-    constexpr int C = HD / 64, VT = 128 / C, NST = spl_paged_ring(HD), CHUNK = SPL_PAGED_CHUNK;      // VT: tokens a chunk of values
+    constexpr int C = HD / 64, NST = spl_paged_ring(HD), CHUNK = spl_paged_chunk(HD), PARTS = HD * 256 / CHUNK, KB = C / PARTS, VT = 128 / PARTS;      // chunks a tile; blocks of 64 channels in one of keys, tokens in one of values
     constexpr float PBIAS = BF16 ? 0.0f : 7.0f;
     extern __shared__ unsigned char spl_paged_raw[];
     unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(spl_paged_raw) + 1023) & ~uintptr_t(1023));
-    unsigned char *q_tile = smem, *ring = q_tile + C * CHUNK;
+    unsigned char *q_tile = smem, *ring = q_tile + HD * 256;
     float *xmax = reinterpret_cast<float *>(ring + NST * CHUNK);      // [tile parity][half][row]
     float *xsum = xmax + 2 * 2 * 128;                                 // [half][row]
     uint64_t *bars = reinterpret_cast<uint64_t *>(xsum + 2 * 128);
@@ -259,17 +259,18 @@ spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
         };
         // Lane b holds the page of the tile's b-th box of tokens; `present` of them hold tokens. inside: where a tile begins in a page of 256.
         auto bring_k = [&](const SplPagedItem &it, int inside, int page, int present) {
-            for (int c = 0; c < C; ++c, ++n) {
+            const int block = lane / boxes, b = lane % boxes, from = __shfl_sync(0xffffffffu, page, b);      // a lane a box of 64 channels by a page's tokens
+            for (int c = 0; c < PARTS; ++c, ++n) {
                 if (!next()) return;
                 const int st = n % NST;
-                if (lane == 0) spl_mbar_expect_tx(&full[st], uint32_t(present * box) * 128);
+                if (lane == 0) spl_mbar_expect_tx(&full[st], uint32_t(present * box) * 128 * KB);
                 __syncwarp();
-                if (lane < present) spl_tma_load4(ring + st * CHUNK + lane * box * 128, &k_map, c * 64, inside, it.kv_head, page, &full[st]);
+                if (block < KB && b < present) spl_tma_load4(ring + st * CHUNK + block * 16384 + b * box * 128, &k_map, (c * KB + block) * 64, inside, it.kv_head, from, &full[st]);
             }
         };
         const int vbox = min(s.page_tokens, VT), vboxes = VT / vbox, per_page = box / vbox;      // boxes a chunk of values, boxes a lane's page
         auto bring_v = [&](const SplPagedItem &it, int inside, int page, int tokens) {
-            for (int c = 0; c < C; ++c, ++n) {
+            for (int c = 0; c < PARTS; ++c, ++n) {
                 if (!next()) return;
                 const int st = n % NST, b = c * vboxes + lane;                                  // lane's box of the tile
                 const int there = min(vboxes, max(0, (tokens - c * VT + vbox - 1) / vbox)), from = __shfl_sync(0xffffffffu, page, lane < vboxes ? b / per_page : 0);
@@ -308,16 +309,17 @@ spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
         auto scores = [&](int at) {
             if (ok && at >= 2 && !spl_mbar_wait_warp(&o_done[at & 1], ((at - 2) >> 1) & 1, const_cast<const int *>(abort))) gave_up(61);
 #pragma unroll
-            for (int c = 0; c < C; ++c, ++n) {
+            for (int c = 0; c < PARTS; ++c, ++n) {
                 const int st = n % NST;
                 if (ok && !spl_mbar_wait_warp(&full[st], (n / NST) & 1, const_cast<const int *>(abort))) gave_up(62);
                 if (!ok) return;
                 spl_tc_fence_after();
 #pragma unroll
-                for (int ks = 0; ks < 4; ++ks)
-                    spl_tc_mma_ss_if(elected, tmem + (at & 1) * 128, q_desc + uint64_t((c * CHUNK + ks * 32) >> 4), ring_desc + uint64_t((st * CHUNK + ks * 32) >> 4), s_idesc, c + ks > 0 ? 1u : 0u);
+                for (int ks = 0; ks < 4 * KB; ++ks)
+                    spl_tc_mma_ss_if(elected, tmem + (at & 1) * 128, q_desc + uint64_t(((c * KB + ks / 4) * 16384 + ks % 4 * 32) >> 4), ring_desc + uint64_t((st * CHUNK + ks / 4 * 16384 + ks % 4 * 32) >> 4),
+                                     s_idesc, c + ks > 0 ? 1u : 0u);
                 spl_tc_commit_if(elected, &empty[st]);
-                if (c == C - 1) spl_tc_commit_if(elected, &s_full[at & 1]);
+                if (c == PARTS - 1) spl_tc_commit_if(elected, &s_full[at & 1]);
             }
         };
         for (int i = item0; i < item1 && ok; ++i, ++pieces) {
@@ -333,7 +335,7 @@ spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
                 if (ok && !spl_mbar_wait_warp(&p_full[tiles & 1], (tiles >> 1) & 1, const_cast<const int *>(abort))) gave_up(64);
                 const int from = max(0, seen_first - tile * 128), to = min(128, seen_last - tile * 128);
                 const uint32_t p_at = tmem + (tiles & 1) * 128;
-                for (int c = 0; c < C && ok; ++c, ++n) {
+                for (int c = 0; c < PARTS && ok; ++c, ++n) {
                     const int st = n % NST;
                     if (!spl_mbar_wait_warp(&full[st], (n / NST) & 1, const_cast<const int *>(abort))) { gave_up(65); break; }
                     const int f = min(max(from - c * VT, 0), VT), e = min(max(to - c * VT, 0), VT), k0 = f / 16, k1 = (e + 15) / 16;      // the chunk's tokens that some row sees
@@ -359,7 +361,7 @@ spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
                         for (int ks = k0; ks < k1; ++ks) spl_tc_mma_ts_if(elected, tmem_o, p_at + (c * (VT / 16) + ks) * 8, place(ks), o_idesc, ks > k0 ? 1u : onto);
                     }
                     spl_tc_commit_if(elected, &empty[st]);
-                    if (c == C - 1) spl_tc_commit_if(elected, &o_done[tiles & 1]);
+                    if (c == PARTS - 1) spl_tc_commit_if(elected, &o_done[tiles & 1]);
                 }
             }
         }
@@ -382,7 +384,7 @@ spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
                 uint4 v = make_uint4(0, 0, 0, 0);
                 if (m < it.q_count)
                     v = *reinterpret_cast<const uint4 *>(a.q + (size_t(it.row0 + packed / s.group) * s.heads + it.kv_head * s.group + packed % s.group) * HD + piece * 8);
-                *reinterpret_cast<uint4 *>(q_tile + (piece >> 3) * CHUNK + spl_sw128_offset(m, (piece & 7) * 8)) = v;
+                *reinterpret_cast<uint4 *>(q_tile + (piece >> 3) * 16384 + spl_sw128_offset(m, (piece & 7) * 8)) = v;
             }
             spl_fence_proxy_async();
             spl_tc_fence_before();

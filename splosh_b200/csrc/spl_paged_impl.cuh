@@ -160,7 +160,7 @@ static bool paged_map(const spl_paged *p, const void *cache, bool values, CUtens
     void *base = const_cast<void *>(cache);
     if (values) {
         const cuuint64_t dims[5] = {64, tokens, d / 64, heads, pages}, strides[4] = {ts, 128, hs, ps};
-        const cuuint32_t box[5] = {64, cuuint32_t(std::min(c.page_tokens, 8192 / c.head_dim)), cuuint32_t(d / 64), 1, 1};
+        const cuuint32_t box[5] = {64, cuuint32_t(std::min(c.page_tokens, spl_paged_chunk(c.head_dim) / (2 * c.head_dim))), cuuint32_t(d / 64), 1, 1};
         return p->encode(map, type, 5, base, dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
     }
     const cuuint64_t dims[4] = {d, tokens, heads, pages}, strides[3] = {ts, hs, ps};
