@@ -224,7 +224,9 @@ spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
     uint64_t *full = bars, *empty = full + NST, *s_full = empty + NST, *p_full = s_full + 2, *o_done = p_full + 2, *q_full = o_done + 2, *drained = q_full + 1;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drained + 1);
     volatile int *abort = reinterpret_cast<volatile int *>(tmem_slot + 1);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    // (Broadcasts tell the compiler what is the same in a warp: the issuing warp's descriptors then stay in uniform registers.)
+    auto uniform = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
+    const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
 
     if (tid == 0) {
         for (int i = 0; i < NST; ++i) { spl_mbar_init(&full[i], 1); spl_mbar_init(&empty[i], 1); }
@@ -240,9 +242,9 @@ spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
     spl_tc_fence_before();
     __syncthreads();
     spl_tc_fence_after();
-    const uint32_t tmem = *tmem_slot, tmem_o = tmem + 256;
+    const uint32_t tmem = uint32_t(uniform(int(*tmem_slot))), tmem_o = tmem + 256;
     spl_grid_begin();
-    const int item0 = a.block_begin[blockIdx.x], item1 = a.block_begin[blockIdx.x + 1];
+    const int item0 = uniform(a.block_begin[blockIdx.x]), item1 = uniform(a.block_begin[blockIdx.x + 1]);
     // A wait tells a phase from the one before it and no more, so a barrier is waited for only by roles that know its last but one use to be over: S, P and O have one a tile
     // parity (tile i's S is issued after the product of tile i - 2 was waited for; whoever has seen that S may wait for the product of tile i - 1 or i).
     // A role whose wait ran out goes through the rest of its loops without waiting: barriers among warps are met by all of them whatever happened.
@@ -324,14 +326,15 @@ spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
         };
         for (int i = item0; i < item1 && ok; ++i, ++pieces) {
             const SplPagedItem it = a.items[i];
+            const int tile_begin = uniform(it.tile_begin), tile_end = uniform(it.tile_end);
             const int base = t.lengths[it.sequence] - t.rows[it.sequence];
             // Tokens that some row of the piece sees.
-            const int seen_first = spl_paged_first(s, base + it.q0 / s.group), seen_last = spl_paged_last(s, base + (it.q0 + it.q_count - 1) / s.group, t.lengths[it.sequence]);
+            const int seen_first = uniform(spl_paged_first(s, base + it.q0 / s.group)), seen_last = uniform(spl_paged_last(s, base + (it.q0 + it.q_count - 1) / s.group, t.lengths[it.sequence]));
             if (ok && !spl_mbar_wait_warp(q_full, pieces & 1, const_cast<const int *>(abort))) gave_up(63);
             if (!ok) break;
             scores(tiles);
-            for (int tile = it.tile_begin; tile < it.tile_end && ok; ++tile, ++tiles) {
-                if (tile + 1 < it.tile_end) scores(tiles + 1);
+            for (int tile = tile_begin; tile < tile_end && ok; ++tile, ++tiles) {
+                if (tile + 1 < tile_end) scores(tiles + 1);
                 if (ok && !spl_mbar_wait_warp(&p_full[tiles & 1], (tiles >> 1) & 1, const_cast<const int *>(abort))) gave_up(64);
                 const int from = max(0, seen_first - tile * 128), to = min(128, seen_last - tile * 128);
                 const uint32_t p_at = tmem + (tiles & 1) * 128;
@@ -352,7 +355,7 @@ spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
                     spl_tc_fence_after();
                     const uint64_t chunk = v_desc + uint64_t((st * CHUNK) >> 4);
                     // The piece's first product overwrites what O held.
-                    const uint32_t onto = tile > it.tile_begin || c * VT + k0 * 16 > from / 16 * 16 ? 1u : 0u;
+                    const uint32_t onto = tile > tile_begin || c * VT + k0 * 16 > from / 16 * 16 ? 1u : 0u;
                     auto place = [&](int ks) { return chunk + uint64_t((((ks * 16) >> vlog) * v_box_step + ((ks * 16) & (vbox - 1)) * 128) >> 4); };
                     if (k0 == 0 && k1 == VT / 16) {
 #pragma unroll
