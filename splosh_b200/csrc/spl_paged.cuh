@@ -127,13 +127,14 @@ spl_paged_append_kernel(SplPagedRows in, const uint16_t *__restrict__ q_norm, co
 //   S[128 rows x 128 tokens]   = Q[128 x HD] K^T          A = Q, B = K          (shared memory, K-major)
 //   O[128 rows x HD]          += P[128 x 128] V           A = P (tensor memory), B = V (shared memory, tokens along the contraction)
 // with the softmax between them. Keys come as chunks of 128 tokens x up to 128 channels, values as chunks of up to 128 tokens x all channels (a tile at HD of 64
-// and 128, half a tile at 256; 128-byte swizzle), one ring for both in the order the products take them: K of tile 0; K of tile i + 1, V of tile i; ... A page smaller than a chunk's tokens is a copy
+// and 128, half a tile at 256; 128-byte swizzle), a ring for each (a ring's barriers tell a phase from the one before it and no more, so a ring has one reader); they are asked for in the
+// order the products take them: K of tile 0; K of tile i + 1, V of tile i; ... A page smaller than a chunk's tokens is a copy
 // of its own, so page sizes and head layouts are the tensor maps' business alone.
 // An instruction of the value product spans all HD columns of O: with values in chunks of 64 channels it took HD / 64 times as many instructions of 64 columns, and the
 // issuing warp (some 100 cycles an instruction) was the block's pace: 5,000 of 6,450 cycles a tile at HD = 256.
 //
-// Warps 0-7 softmax (thread: a row and half of the tile's tokens; the pair of warps of 32 rows agrees on the maximum), warp 8 copies, warp 9 issues
-// both products: S of tile i + 1 runs under the softmax of tile i. The reference is raised only when a row's maximum exceeds it by 2^8, so the sums in
+// Warps 0-7 softmax (thread: a row and half of the tile's tokens; the pair of warps of 32 rows agrees on the maximum), warp 8 copies, warps 9 and
+// 10 issue the products: S of tile i + 1 runs under the softmax of tile i. The reference is raised only when a row's maximum exceeds it by 2^8, so the sums in
 // tensor memory are rescaled a few times a piece, not every tile. Rows that are not there cost no softmax work.
 // Tensor memory: S / P two buffers of 128 columns (P, 16 bits, over the S it came from), O HD columns from 256.
 //
@@ -142,10 +143,12 @@ spl_paged_append_kernel(SplPagedRows in, const uint16_t *__restrict__ q_norm, co
 //
 // What is masked may be anything: a masked score is replaced before it is used, and because 0 x inf is no number, tokens that no row of the piece
 // sees (behind the sequence's last token, in front of the window) have their values zeroed in shared memory or are left out of the product.
-#define SPL_PAGED_THREADS 320
+#define SPL_PAGED_THREADS 352
 #define SPL_PAGED_HEADROOM 8.0f
 __host__ __device__ constexpr int spl_paged_chunk(int hd) { return hd == 64 ? 16384 : 32768; }
-__host__ __device__ constexpr int spl_paged_ring(int hd) { return hd == 256 ? 4 : hd == 128 ? 5 : 12; }
+__host__ __device__ constexpr int spl_paged_ring_k(int hd) { return hd == 256 ? 2 : hd == 128 ? 3 : 6; }
+__host__ __device__ constexpr int spl_paged_ring_v(int hd) { return hd == 64 ? 6 : 2; }
+__host__ __device__ constexpr int spl_paged_ring(int hd) { return spl_paged_ring_k(hd) + spl_paged_ring_v(hd); }
 __host__ __device__ constexpr size_t spl_paged_smem_bytes(int hd) {
     return 1024 + size_t(hd) * 256 + size_t(spl_paged_ring(hd)) * spl_paged_chunk(hd) + 2 * 2 * 128 * 4 /* maxima */ + 2 * 128 * 4 /* sums */ + 512 /* barriers */;
 }
@@ -213,25 +216,25 @@ struct SplPagedAttend {
 template <int HD, bool BF16>
 __global__ void __launch_bounds__(SPL_PAGED_THREADS, 1)
 spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, SplPagedTables t, SplPagedShape s, SplPagedAttend a) {
-    constexpr int C = HD / 64, NST = spl_paged_ring(HD), CHUNK = spl_paged_chunk(HD), PARTS = HD * 256 / CHUNK, KB = C / PARTS, VT = 128 / PARTS;      // chunks a tile; blocks of 64 channels in one of keys, tokens in one of values
+    constexpr int C = HD / 64, NK = spl_paged_ring_k(HD), NV = spl_paged_ring_v(HD), CHUNK = spl_paged_chunk(HD), PARTS = HD * 256 / CHUNK, KB = C / PARTS, VT = 128 / PARTS;      // chunks a tile; blocks of 64 channels in one of keys, tokens in one of values
     constexpr float PBIAS = BF16 ? 0.0f : 7.0f;
     extern __shared__ unsigned char spl_paged_raw[];
     unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(spl_paged_raw) + 1023) & ~uintptr_t(1023));
-    unsigned char *q_tile = smem, *ring = q_tile + HD * 256;
-    float *xmax = reinterpret_cast<float *>(ring + NST * CHUNK);      // [tile parity][half][row]
+    unsigned char *q_tile = smem, *ring = q_tile + HD * 256, *v_ring = ring + NK * CHUNK;
+    float *xmax = reinterpret_cast<float *>(v_ring + NV * CHUNK);      // [tile parity][half][row]
     float *xsum = xmax + 2 * 2 * 128;                                 // [half][row]
     uint64_t *bars = reinterpret_cast<uint64_t *>(xsum + 2 * 128);
-    uint64_t *full = bars, *empty = full + NST, *s_full = empty + NST, *p_full = s_full + 2, *o_done = p_full + 2, *q_full = o_done + 2, *drained = q_full + 1;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drained + 1);
+    uint64_t *full_k = bars, *empty_k = full_k + NK, *full_v = empty_k + NK, *empty_v = full_v + NV, *s_full = empty_v + NV, *p_full = s_full + 2, *o_done = p_full + 2, *q_full = o_done + 2, *drained = q_full + 1;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drained + 2);
     volatile int *abort = reinterpret_cast<volatile int *>(tmem_slot + 1);
     // (Broadcasts tell the compiler what is the same in a warp: the issuing warp's descriptors then stay in uniform registers.)
     auto uniform = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
     const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
 
     if (tid == 0) {
-        for (int i = 0; i < NST; ++i) { spl_mbar_init(&full[i], 1); spl_mbar_init(&empty[i], 1); }
+        for (int i = 0; i < 2 * NK + 2 * NV; ++i) spl_mbar_init(&bars[i], 1);
         for (int i = 0; i < 2; ++i) { spl_mbar_init(&s_full[i], 1); spl_mbar_init(&p_full[i], 8); spl_mbar_init(&o_done[i], 1); }
-        spl_mbar_init(q_full, 8); spl_mbar_init(drained, 1);
+        spl_mbar_init(q_full, 8); spl_mbar_init(&drained[0], 1); spl_mbar_init(&drained[1], 1);
         *abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
@@ -254,31 +257,31 @@ spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
     if (warp == 8) {
         // ---- copies. Lane b brings the tile's b-th page (or its half of a page of 256); a chunk's barrier counts the pages that hold tokens.
         const int box = min(s.page_tokens, 128), boxes = 128 / box;
-        int n = 0;                                            // chunks so far
-        auto next = [&]() {                                   // room for a chunk
-            if (ok && !spl_mbar_wait_warp(&empty[n % NST], ((n / NST) & 1) ^ 1, const_cast<const int *>(abort))) gave_up(60);
+        int nk = 0, nv = 0;                                   // chunks so far
+        auto room = [&](uint64_t *empty, int n, int slots) {
+            if (ok && !spl_mbar_wait_warp(&empty[n % slots], ((n / slots) & 1) ^ 1, const_cast<const int *>(abort))) gave_up(60);
             return ok;
         };
         // Lane b holds the page of the tile's b-th box of tokens; `present` of them hold tokens. inside: where a tile begins in a page of 256.
         auto bring_k = [&](const SplPagedItem &it, int inside, int page, int present) {
             const int block = lane / boxes, b = lane % boxes, from = __shfl_sync(0xffffffffu, page, b);      // a lane a box of 64 channels by a page's tokens
-            for (int c = 0; c < PARTS; ++c, ++n) {
-                if (!next()) return;
-                const int st = n % NST;
-                if (lane == 0) spl_mbar_expect_tx(&full[st], uint32_t(present * box) * 128 * KB);
+            for (int c = 0; c < PARTS; ++c, ++nk) {
+                if (!room(empty_k, nk, NK)) return;
+                const int st = nk % NK;
+                if (lane == 0) spl_mbar_expect_tx(&full_k[st], uint32_t(present * box) * 128 * KB);
                 __syncwarp();
-                if (block < KB && b < present) spl_tma_load4(ring + st * CHUNK + block * 16384 + b * box * 128, &k_map, (c * KB + block) * 64, inside, it.kv_head, from, &full[st]);
+                if (block < KB && b < present) spl_tma_load4(ring + st * CHUNK + block * 16384 + b * box * 128, &k_map, (c * KB + block) * 64, inside, it.kv_head, from, &full_k[st]);
             }
         };
         const int vbox = min(s.page_tokens, VT), vboxes = VT / vbox, per_page = box / vbox;      // boxes a chunk of values, boxes a lane's page
         auto bring_v = [&](const SplPagedItem &it, int inside, int page, int tokens) {
-            for (int c = 0; c < PARTS; ++c, ++n) {
-                if (!next()) return;
-                const int st = n % NST, b = c * vboxes + lane;                                  // lane's box of the tile
+            for (int c = 0; c < PARTS; ++c, ++nv) {
+                if (!room(empty_v, nv, NV)) return;
+                const int st = nv % NV, b = c * vboxes + lane;                                  // lane's box of the tile
                 const int there = min(vboxes, max(0, (tokens - c * VT + vbox - 1) / vbox)), from = __shfl_sync(0xffffffffu, page, lane < vboxes ? b / per_page : 0);
-                if (lane == 0) spl_mbar_expect_tx(&full[st], uint32_t(there) * vbox * HD * 2);
+                if (lane == 0) spl_mbar_expect_tx(&full_v[st], uint32_t(there) * vbox * HD * 2);
                 __syncwarp();
-                if (lane < there) spl_tma_load5(ring + st * CHUNK + lane * vbox * HD * 2, &v_map, 0, inside + b % per_page * vbox, 0, it.kv_head, from, &full[st]);
+                if (lane < there) spl_tma_load5(v_ring + st * CHUNK + lane * vbox * HD * 2, &v_map, 0, inside + b % per_page * vbox, 0, it.kv_head, from, &full_v[st]);
             }
         };
         for (int i = item0; i < item1 && ok; ++i) {
@@ -298,79 +301,86 @@ spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
             }
         }
         // Nothing may still be on its way into the block's shared memory when it is handed on.
-        for (int st = 0; st < NST && st < n; ++st) { const int last = st + (n - 1 - st) / NST * NST; spl_mbar_wait(&full[st], (last / NST) & 1); }
-    } else if (warp == 9) {
-        // ---- both products, one elected lane of a converged warp.
+        for (int st = 0; st < NK && st < nk; ++st) spl_mbar_wait(&full_k[st], ((st + (nk - 1 - st) / NK * NK) / NK) & 1);
+        for (int st = 0; st < NV && st < nv; ++st) spl_mbar_wait(&full_v[st], ((st + (nv - 1 - st) / NV * NV) / NV) & 1);
+    } else if (warp == 9 || warp == 10) {
+        // ---- the products, a warp each (a wait is 110 cycles even when it is over: in one warp six a tile were a third of its time), issued by one elected lane of
+        // a converged warp.
+        const uint32_t elected = spl_elect_one() ? 1u : 0u;
+        const bool first_product = warp == 9;
         constexpr uint32_t s_idesc = spl_paged_idesc(128, BF16, false), o_idesc = spl_paged_idesc(HD, BF16, true);
         const int vbox = min(s.page_tokens, VT);
-        const uint64_t q_desc = spl_tc_desc_sw128(spl_smem_addr(q_tile)), ring_desc = spl_tc_desc_sw128(spl_smem_addr(ring)), v_desc = spl_tc_desc_mn_sw128(spl_smem_addr(ring), vbox * 128);
+        const uint64_t q_desc = spl_tc_desc_sw128(spl_smem_addr(q_tile)), ring_desc = spl_tc_desc_sw128(spl_smem_addr(ring)), v_desc = spl_tc_desc_mn_sw128(spl_smem_addr(v_ring), vbox * 128);
         const uint32_t v_box_step = uint32_t(vbox) * HD * 2, vlog = 31 - __clz(vbox);
-        const uint32_t elected = spl_elect_one() ? 1u : 0u;
-        int n = 0, tiles = 0, pieces = 0;                     // chunks, tiles and pieces so far
-        // Scores of tile number `at` of this block. They go where the P of tile at - 2 lies, which has to have been read.
-        auto scores = [&](int at) {
-            if (ok && at >= 2 && !spl_mbar_wait_warp(&o_done[at & 1], ((at - 2) >> 1) & 1, const_cast<const int *>(abort))) gave_up(61);
-#pragma unroll
-            for (int c = 0; c < PARTS; ++c, ++n) {
-                const int st = n % NST;
-                if (ok && !spl_mbar_wait_warp(&full[st], (n / NST) & 1, const_cast<const int *>(abort))) gave_up(62);
-                if (!ok) return;
-                spl_tc_fence_after();
-#pragma unroll
-                for (int ks = 0; ks < 4 * KB; ++ks)
-                    spl_tc_mma_ss_if(elected, tmem + (at & 1) * 128, q_desc + uint64_t(((c * KB + ks / 4) * 16384 + ks % 4 * 32) >> 4), ring_desc + uint64_t((st * CHUNK + ks / 4 * 16384 + ks % 4 * 32) >> 4),
-                                     s_idesc, c + ks > 0 ? 1u : 0u);
-                spl_tc_commit_if(elected, &empty[st]);
-                if (c == PARTS - 1) spl_tc_commit_if(elected, &s_full[at & 1]);
-            }
-        };
-        for (int i = item0; i < item1 && ok; ++i, ++pieces) {
+        int n = 0, tiles = 0;                                 // chunks of its ring and tiles so far
+        for (int i = item0; i < item1 && ok; ++i) {
             const SplPagedItem it = a.items[i];
-            const int tile_begin = uniform(it.tile_begin), tile_end = uniform(it.tile_end);
-            const int base = t.lengths[it.sequence] - t.rows[it.sequence];
-            // Tokens that some row of the piece sees.
-            const int seen_first = uniform(spl_paged_first(s, base + it.q0 / s.group)), seen_last = uniform(spl_paged_last(s, base + (it.q0 + it.q_count - 1) / s.group, t.lengths[it.sequence]));
-            if (ok && !spl_mbar_wait_warp(q_full, pieces & 1, const_cast<const int *>(abort))) gave_up(63);
-            if (!ok) break;
-            scores(tiles);
-            for (int tile = tile_begin; tile < tile_end && ok; ++tile, ++tiles) {
-                if (tile + 1 < tile_end) scores(tiles + 1);
-                if (ok && !spl_mbar_wait_warp(&p_full[tiles & 1], (tiles >> 1) & 1, const_cast<const int *>(abort))) gave_up(64);
-                const int from = max(0, seen_first - tile * 128), to = min(128, seen_last - tile * 128);
-                const uint32_t p_at = tmem + (tiles & 1) * 128;
-                for (int c = 0; c < PARTS && ok; ++c, ++n) {
-                    const int st = n % NST;
-                    if (!spl_mbar_wait_warp(&full[st], (n / NST) & 1, const_cast<const int *>(abort))) { gave_up(65); break; }
-                    const int f = min(max(from - c * VT, 0), VT), e = min(max(to - c * VT, 0), VT), k0 = f / 16, k1 = (e + 15) / 16;      // the chunk's tokens that some row sees
-                    if (f % 16 || e % 16) {
-                        // Values of unseen tokens in the first and last groups of sixteen: zero, whatever the cache holds there.
-                        const int before = f % 16, after = (16 - e % 16) % 16;
-                        for (int z = lane; z < (before + after) * C * 8; z += 32) {
-                            const int row = z / (C * 8), token = row < before ? k0 * 16 + row : e + row - before, piece = z % (C * 8);
-                            *reinterpret_cast<uint4 *>(ring + st * CHUNK + token / vbox * v_box_step + (piece >> 3) * vbox * 128 + token % vbox * 128 + (piece & 7) * 16) = make_uint4(0, 0, 0, 0);
-                        }
-                        spl_fence_proxy_async();
-                        __syncwarp();
-                    }
-                    spl_tc_fence_after();
-                    const uint64_t chunk = v_desc + uint64_t((st * CHUNK) >> 4);
-                    // The piece's first product overwrites what O held.
-                    const uint32_t onto = tile > tile_begin || c * VT + k0 * 16 > from / 16 * 16 ? 1u : 0u;
-                    auto place = [&](int ks) { return chunk + uint64_t((((ks * 16) >> vlog) * v_box_step + ((ks * 16) & (vbox - 1)) * 128) >> 4); };
-                    if (k0 == 0 && k1 == VT / 16) {
+            const int tile_begin = uniform(it.tile_begin), count = uniform(it.tile_end) - tile_begin;
+            if (first_product) {
+                if (!spl_mbar_wait_warp(q_full, (i - item0) & 1, const_cast<const int *>(abort))) { gave_up(63); break; }
+                for (int tile = 0; tile < count && ok; ++tile) {
+                    const int at = tiles + tile;
+                    // The first keys may be there long before the place of the scores is: it held the P of tile at - 2, which has to have been read.
+                    if (!spl_mbar_wait_warp(&full_k[n % NK], (n / NK) & 1, const_cast<const int *>(abort))) { gave_up(62); break; }
+                    if (at >= 2 && !spl_mbar_wait_warp(&o_done[at & 1], ((at - 2) >> 1) & 1, const_cast<const int *>(abort))) { gave_up(61); break; }
 #pragma unroll
-                        for (int ks = 0; ks < VT / 16; ++ks) spl_tc_mma_ts_if(elected, tmem_o, p_at + (c * (VT / 16) + ks) * 8, place(ks), o_idesc, ks > 0 ? 1u : onto);
-                    } else {
-                        for (int ks = k0; ks < k1; ++ks) spl_tc_mma_ts_if(elected, tmem_o, p_at + (c * (VT / 16) + ks) * 8, place(ks), o_idesc, ks > k0 ? 1u : onto);
+                    for (int c = 0; c < PARTS; ++c, ++n) {
+                        const int st = n % NK;
+                        if (c > 0 && ok && !spl_mbar_wait_warp(&full_k[st], (n / NK) & 1, const_cast<const int *>(abort))) gave_up(62);
+                        if (!ok) break;
+                        spl_tc_fence_after();
+#pragma unroll
+                        for (int ks = 0; ks < 4 * KB; ++ks)
+                            spl_tc_mma_ss_if(elected, tmem + (at & 1) * 128, q_desc + uint64_t(((c * KB + ks / 4) * 16384 + ks % 4 * 32) >> 4),
+                                             ring_desc + uint64_t((st * CHUNK + ks / 4 * 16384 + ks % 4 * 32) >> 4), s_idesc, c + ks > 0 ? 1u : 0u);
+                        spl_tc_commit_if(elected, &empty_k[st]);
+                        if (c == PARTS - 1) spl_tc_commit_if(elected, &s_full[at & 1]);
                     }
-                    spl_tc_commit_if(elected, &empty[st]);
-                    if (c == PARTS - 1) spl_tc_commit_if(elected, &o_done[tiles & 1]);
+                }
+            } else {
+                const int base = t.lengths[it.sequence] - t.rows[it.sequence];
+                // Tokens that some row of the piece sees.
+                const int seen_first = uniform(spl_paged_first(s, base + it.q0 / s.group)), seen_last = uniform(spl_paged_last(s, base + (it.q0 + it.q_count - 1) / s.group, t.lengths[it.sequence]));
+                for (int tile = 0; tile < count && ok; ++tile) {
+                    const int at = tiles + tile, token0 = (tile_begin + tile) * 128;
+                    const int from = max(0, seen_first - token0), to = min(128, seen_last - token0);
+                    const uint32_t p_at = tmem + (at & 1) * 128;
+                    for (int c = 0; c < PARTS && ok; ++c, ++n) {
+                        const int st = n % NV;
+                        if (!spl_mbar_wait_warp(&full_v[st], (n / NV) & 1, const_cast<const int *>(abort))) { gave_up(65); break; }
+                        const int f = min(max(from - c * VT, 0), VT), e = min(max(to - c * VT, 0), VT), k0 = f / 16, k1 = (e + 15) / 16;      // the chunk's tokens that some row sees
+                        if (f % 16 || e % 16) {
+                            // Values of unseen tokens in the first and last groups of sixteen: zero, whatever the cache holds there.
+                            const int before = f % 16, after = (16 - e % 16) % 16;
+                            for (int z = lane; z < (before + after) * C * 8; z += 32) {
+                                const int row = z / (C * 8), token = row < before ? k0 * 16 + row : e + row - before, piece = z % (C * 8);
+                                *reinterpret_cast<uint4 *>(v_ring + st * CHUNK + token / vbox * v_box_step + (piece >> 3) * vbox * 128 + token % vbox * 128 + (piece & 7) * 16) = make_uint4(0, 0, 0, 0);
+                            }
+                            spl_fence_proxy_async();
+                            __syncwarp();
+                        }
+                        if (c == 0 && !spl_mbar_wait_warp(&p_full[at & 1], (at >> 1) & 1, const_cast<const int *>(abort))) { gave_up(64); break; }
+                        spl_tc_fence_after();
+                        const uint64_t chunk = v_desc + uint64_t((st * CHUNK) >> 4);
+                        // The piece's first product overwrites what O held.
+                        const uint32_t onto = tile > 0 || c * VT + k0 * 16 > from / 16 * 16 ? 1u : 0u;
+                        auto place = [&](int ks) { return chunk + uint64_t((((ks * 16) >> vlog) * v_box_step + ((ks * 16) & (vbox - 1)) * 128) >> 4); };
+                        if (k0 == 0 && k1 == VT / 16) {
+#pragma unroll
+                            for (int ks = 0; ks < VT / 16; ++ks) spl_tc_mma_ts_if(elected, tmem_o, p_at + (c * (VT / 16) + ks) * 8, place(ks), o_idesc, ks > 0 ? 1u : onto);
+                        } else {
+                            for (int ks = k0; ks < k1; ++ks) spl_tc_mma_ts_if(elected, tmem_o, p_at + (c * (VT / 16) + ks) * 8, place(ks), o_idesc, ks > k0 ? 1u : onto);
+                        }
+                        spl_tc_commit_if(elected, &empty_v[st]);
+                        if (c == PARTS - 1) spl_tc_commit_if(elected, &o_done[at & 1]);
+                    }
                 }
             }
+            tiles += count;
         }
         // No product may still read shared or write tensor memory when they are handed on.
-        spl_tc_commit_if(elected, drained);
-        spl_mbar_wait(drained, 0);
+        spl_tc_commit_if(elected, &drained[first_product ? 0 : 1]);
+        spl_mbar_wait(&drained[first_product ? 0 : 1], 0);
     } else {
         // ---- softmax: row r of the piece, tokens [64 half, 64 half + 64) of a tile.
         const int quarter = warp & 3, half = warp >> 2, r = quarter * 32 + lane;
