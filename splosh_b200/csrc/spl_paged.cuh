@@ -24,7 +24,7 @@ struct SplPagedShape {
 };
 // The batch as the kernels read it (device memory).
 struct SplPagedTables {
-    const int *counts;            // rows, sequences, merges
+    const int *counts;            // rows, sequences
     const int *row_sequence, *row_position;
     const int *rows, *lengths;    // per sequence
     const int *table;             // [sequences][max_pages]
@@ -146,11 +146,11 @@ spl_paged_append_kernel(SplPagedRows in, const uint16_t *__restrict__ q_norm, co
 #define SPL_PAGED_THREADS 352
 #define SPL_PAGED_HEADROOM 8.0f
 __host__ __device__ constexpr int spl_paged_chunk(int hd) { return hd == 64 ? 16384 : 32768; }
-__host__ __device__ constexpr int spl_paged_ring_k(int hd) { return hd == 256 ? 2 : hd == 128 ? 3 : 6; }
+__host__ __device__ constexpr int spl_paged_ring_k(int hd) { return hd == 64 ? 6 : 3; }
 __host__ __device__ constexpr int spl_paged_ring_v(int hd) { return hd == 64 ? 6 : 2; }
 __host__ __device__ constexpr int spl_paged_ring(int hd) { return spl_paged_ring_k(hd) + spl_paged_ring_v(hd); }
 __host__ __device__ constexpr size_t spl_paged_smem_bytes(int hd) {
-    return 1024 + size_t(hd) * 256 + size_t(spl_paged_ring(hd)) * spl_paged_chunk(hd) + 2 * 2 * 128 * 4 /* maxima */ + 2 * 128 * 4 /* sums */ + 512 /* barriers */;
+    return size_t(hd) * 256 + size_t(spl_paged_ring(hd)) * spl_paged_chunk(hd) + 2 * 2 * 128 * 4 /* maxima, sums */ + 512 /* barriers */;
 }
 
 // Tokens that the row at `position` of a sequence of `length` tokens sees: [first, last).
@@ -183,6 +183,7 @@ __device__ __forceinline__ void spl_tc_ld32(uint32_t (&r)[32], uint32_t taddr) {
                    "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
                    "=r"(r[31]) : "r"(taddr));
 }
+__device__ __forceinline__ void spl_tma_prefetch(const CUtensorMap *map) { asm volatile("prefetch.tensormap [%0];\n" ::"l"(map) : "memory"); }
 __device__ __forceinline__ void spl_tma_load5(void *smem, const CUtensorMap *map, int x, int token, int block, int head, int page, uint64_t *bar) {
     asm volatile("cp.async.bulk.tensor.5d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];\n"
                  ::"r"(spl_smem_addr(smem)), "l"(map), "r"(x), "r"(token), "r"(block), "r"(head), "r"(page), "r"(spl_smem_addr(bar)) : "memory");
@@ -206,27 +207,67 @@ __device__ __forceinline__ void spl_paged_pair_barrier(int quarter) {
 
 struct SplPagedAttend {
     const uint16_t *q; void *out; int out_f32;
-    const SplPagedItem *items; const int *block_begin;
+    const SplPagedItem *starts, *items; const int *block_begin; int *arrived;
     float *partial;              // [slot][slot_rows][HD] sums
     float2 *partial_ml;          // [slot][slot_rows] reference (log2), sum of p
     int slot_rows;
     int *error_flag;
 };
 
+// The pieces of a tile of query rows joined: o = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s. Eight warps, a warp a row, four pieces' sums on their way.
+template <int HD, bool BF16>
+__device__ __forceinline__ void spl_paged_join(const SplPagedShape &s, const SplPagedAttend &a, const SplPagedItem &it, int row0, int head0, uint32_t per_group) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int r = warp; r < it.q_count; r += 8) {
+        float m = -INFINITY;
+        for (int n = lane; n < it.pieces; n += 32) m = fmaxf(m, __ldcg(&a.partial_ml[size_t(it.slot0 + n) * a.slot_rows + r]).x);
+        m = spl_warp_max(m);
+        float2 acc[HD / 64];
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < HD / 64; ++j) acc[j] = make_float2(0.0f, 0.0f);
+        for (int n0 = 0; n0 < it.pieces; n0 += 4) {
+            float2 ml[4], v[4][HD / 64];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const size_t row = size_t(it.slot0 + min(n0 + u, it.pieces - 1)) * a.slot_rows + r;
+                ml[u] = __ldcg(&a.partial_ml[row]);
+#pragma unroll
+                for (int j = 0; j < HD / 64; ++j) v[u][j] = __ldcg(reinterpret_cast<const float2 *>(a.partial + row * HD + 64 * j + 2 * lane));
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                if (n0 + u >= it.pieces || ml[u].x == -INFINITY) continue;      // (a piece of whose tokens this row sees none)
+                const float f = exp2f(ml[u].x - m);
+                sum += f * ml[u].y;
+#pragma unroll
+                for (int j = 0; j < HD / 64; ++j) { acc[j].x += f * v[u][j].x; acc[j].y += f * v[u][j].y; }
+            }
+        }
+        const float inv = 1.0f / sum;
+        const int x = head0 + r, row = int(x * per_group >> 16);
+        const size_t place = (size_t(row0 + row) * s.heads + it.kv_head * s.group + x - row * s.group) * HD;
+#pragma unroll
+        for (int j = 0; j < HD / 64; ++j) {
+            if (a.out_f32) *reinterpret_cast<float2 *>(static_cast<float *>(a.out) + place + 64 * j + 2 * lane) = make_float2(acc[j].x * inv, acc[j].y * inv);
+            else *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(a.out) + place + 64 * j + 2 * lane) = spl_pack16<BF16>(acc[j].x * inv, acc[j].y * inv);
+        }
+    }
+}
+
 template <int HD, bool BF16>
 __global__ void __launch_bounds__(SPL_PAGED_THREADS, 1)
 spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, SplPagedTables t, SplPagedShape s, SplPagedAttend a) {
     constexpr int C = HD / 64, NK = spl_paged_ring_k(HD), NV = spl_paged_ring_v(HD), CHUNK = spl_paged_chunk(HD), PARTS = HD * 256 / CHUNK, KB = C / PARTS, VT = 128 / PARTS;      // chunks a tile; blocks of 64 channels in one of keys, tokens in one of values
     constexpr float PBIAS = BF16 ? 0.0f : 7.0f;
-    extern __shared__ unsigned char spl_paged_raw[];
-    unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(spl_paged_raw) + 1023) & ~uintptr_t(1023));
-    unsigned char *q_tile = smem, *ring = q_tile + HD * 256, *v_ring = ring + NK * CHUNK;
+    extern __shared__ __align__(1024) unsigned char spl_paged_raw[];
+    if (spl_smem_addr(spl_paged_raw) % 1024) { if (threadIdx.x == 0) a.error_flag[0] = 299; return; }      // (the swizzle's unit; there is no room to round up)
+    unsigned char *q_tile = spl_paged_raw, *ring = q_tile + HD * 256, *v_ring = ring + NK * CHUNK;
     float *xmax = reinterpret_cast<float *>(v_ring + NV * CHUNK);      // [tile parity][half][row]
-    float *xsum = xmax + 2 * 2 * 128;                                 // [half][row]
-    uint64_t *bars = reinterpret_cast<uint64_t *>(xsum + 2 * 128);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(xmax + 2 * 2 * 128);
     uint64_t *full_k = bars, *empty_k = full_k + NK, *full_v = empty_k + NK, *empty_v = full_v + NV, *s_full = empty_v + NV, *p_full = s_full + 2, *o_done = p_full + 2, *q_full = o_done + 2, *drained = q_full + 1;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drained + 2);
-    volatile int *abort = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    volatile int *abort = reinterpret_cast<volatile int *>(tmem_slot + 1), *joins = abort + 1;
     // (Broadcasts tell the compiler what is the same in a warp: the issuing warp's descriptors then stay in uniform registers.)
     auto uniform = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
     const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
@@ -238,6 +279,7 @@ spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
         *abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
+    if (tid == 256) { spl_tma_prefetch(&k_map); spl_tma_prefetch(&v_map); }
     if (warp == 9) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(spl_smem_addr(tmem_slot)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
@@ -247,7 +289,10 @@ spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
     spl_tc_fence_after();
     const uint32_t tmem = uint32_t(uniform(int(*tmem_slot))), tmem_o = tmem + 256;
     spl_grid_begin();
+    // (The first item comes with the block's range, not after it.)
+    const SplPagedItem first_item = a.starts[blockIdx.x];
     const int item0 = uniform(a.block_begin[blockIdx.x]), item1 = uniform(a.block_begin[blockIdx.x + 1]);
+    auto item_at = [&](int i) { return i == item0 ? first_item : a.items[i]; };
     // A wait tells a phase from the one before it and no more, so a barrier is waited for only by roles that know its last but one use to be over: S, P and O have one a tile
     // parity (tile i's S is issued after the product of tile i - 2 was waited for; whoever has seen that S may wait for the product of tile i - 1 or i).
     // A role whose wait ran out goes through the rest of its loops without waiting: barriers among warps are met by all of them whatever happened.
@@ -285,8 +330,8 @@ spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
             }
         };
         for (int i = item0; i < item1 && ok; ++i) {
-            const SplPagedItem it = a.items[i];
-            const int length = t.lengths[it.sequence];
+            const SplPagedItem it = item_at(i);
+            const int length = it.length;
             const int *pages = t.table + size_t(it.sequence) * s.max_pages;
             auto present_of = [&](int tile) { return min(boxes, (length - tile * 128 + box - 1) / box); };
             auto page_of = [&](int tile) { return tile < it.tile_end && lane < present_of(tile) ? pages[s.page_tokens > 128 ? tile >> 1 : tile * boxes + lane] : 0; };
@@ -314,7 +359,7 @@ spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
         const uint32_t v_box_step = uint32_t(vbox) * HD * 2, vlog = 31 - __clz(vbox);
         int n = 0, tiles = 0;                                 // chunks of its ring and tiles so far
         for (int i = item0; i < item1 && ok; ++i) {
-            const SplPagedItem it = a.items[i];
+            const SplPagedItem it = item_at(i);
             const int tile_begin = uniform(it.tile_begin), count = uniform(it.tile_end) - tile_begin;
             if (first_product) {
                 if (!spl_mbar_wait_warp(q_full, (i - item0) & 1, const_cast<const int *>(abort))) { gave_up(63); break; }
@@ -338,9 +383,8 @@ spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
                     }
                 }
             } else {
-                const int base = t.lengths[it.sequence] - t.rows[it.sequence];
                 // Tokens that some row of the piece sees.
-                const int seen_first = uniform(spl_paged_first(s, base + it.q0 / s.group)), seen_last = uniform(spl_paged_last(s, base + (it.q0 + it.q_count - 1) / s.group, t.lengths[it.sequence]));
+                const int seen_first = uniform(spl_paged_first(s, it.base + it.q0 / s.group)), seen_last = uniform(spl_paged_last(s, it.base + (it.q0 + it.q_count - 1) / s.group, it.length));
                 for (int tile = 0; tile < count && ok; ++tile) {
                     const int at = tiles + tile, token0 = (tile_begin + tile) * 128;
                     const int from = max(0, seen_first - token0), to = min(128, seen_last - token0);
@@ -386,25 +430,37 @@ spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
         const int quarter = warp & 3, half = warp >> 2, r = quarter * 32 + lane;
         const uint32_t lanes = uint32_t(quarter * 32) << 16;
         const float c = s.scale * 1.4426950408889634f;
+        const uint32_t per_group = (65536u + s.group - 1) / s.group;      // x / group = x * per_group >> 16 for x below 192
         int tiles = 0;
-        for (int i = item0; i < item1; ++i) {
-            const SplPagedItem it = a.items[i];
-            const int length = t.lengths[it.sequence], base = length - t.rows[it.sequence];
-            const bool busy = quarter * 32 < it.q_count;             // whether this warp's rows hold a query
-            // Queries into the swizzled operand tile, zero where there is none: 16-byte pieces of eight channels.
-            for (int idx = tid; idx < 128 * (HD / 8); idx += 256) {
-                const int m = idx / (HD / 8), piece = idx % (HD / 8), packed = it.q0 + m;
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (m < it.q_count)
-                    v = *reinterpret_cast<const uint4 *>(a.q + (size_t(it.row0 + packed / s.group) * s.heads + it.kv_head * s.group + packed % s.group) * HD + piece * 8);
-                *reinterpret_cast<uint4 *>(q_tile + (piece >> 3) * 16384 + spl_sw128_offset(m, (piece & 7) * 8)) = v;
+        // A piece's queries into the swizzled operand tile: 16-byte pieces of eight channels, eight on their way a thread. (What lies in rows without a query does not reach the others.)
+        auto bring_q = [&](const SplPagedItem &it) {
+            const int row0 = it.row0 + it.q0 / s.group, head0 = it.q0 % s.group, pieces = it.q_count * (HD / 8);
+            for (int base = tid; base < pieces; base += 8 * 256) {
+                uint4 v[8];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    const int idx = base + u * 256, x = head0 + idx / (HD / 8), row = int(x * per_group >> 16);
+                    if (idx < pieces) v[u] = *reinterpret_cast<const uint4 *>(a.q + (size_t(row0 + row) * s.heads + it.kv_head * s.group + (x - row * s.group)) * HD + idx % (HD / 8) * 8);
+                }
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    const int idx = base + u * 256, piece = idx % (HD / 8);
+                    if (idx < pieces) *reinterpret_cast<uint4 *>(q_tile + (piece >> 3) * 16384 + spl_sw128_offset(idx / (HD / 8), (piece & 7) * 8)) = v[u];
+                }
             }
             spl_fence_proxy_async();
             spl_tc_fence_before();
             __syncwarp();
             if (lane == 0) spl_mbar_arrive(q_full);
-            const int position = base + (it.q0 + min(r, it.q_count - 1)) / s.group;
-            const int first = spl_paged_first(s, position), last = spl_paged_last(s, position, length);
+        };
+        SplPagedItem it = first_item;
+        if (item0 < item1) bring_q(it);
+        for (int i = item0; i < item1; ++i) {
+            const bool busy = quarter * 32 < it.q_count;             // whether this warp's rows hold a query
+            const SplPagedItem next = i + 1 < item1 ? a.items[i + 1] : it;
+            const int row0 = it.row0 + it.q0 / s.group, mine = it.q0 % s.group + min(r, it.q_count - 1), row = int(mine * per_group >> 16), head = it.kv_head * s.group + mine - row * s.group;
+            const int position = it.base + it.q0 / s.group + row;
+            const int first = spl_paged_first(s, position), last = spl_paged_last(s, position, it.length);
             float ref = -INFINITY, sum = 0.0f;
             for (int tile = it.tile_begin; tile < it.tile_end; ++tile, ++tiles) {
                 const int buf = tiles & 1;
@@ -466,83 +522,68 @@ spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
                 __syncwarp();
                 if (lane == 0) spl_mbar_arrive(&p_full[buf]);
             }
+            // The next piece's queries: all scores of this one have been seen, so its own are no longer read. (O is overwritten by a product that waits for this warp.)
+            if (i + 1 < item1) bring_q(next);
             // The piece's sums.
             if (ok && !spl_mbar_wait_warp(&o_done[(tiles - 1) & 1], ((tiles - 1) >> 1) & 1, const_cast<const int *>(abort))) gave_up(68);
+            const size_t slot_row = size_t(it.slot) * a.slot_rows + r;
             if (busy) {
                 spl_tc_fence_after();
+                // (Exchanged where the maxima of the tile before the last were: nobody reads those any more.)
+                float *xsum = xmax + (tiles & 1) * 2 * 128;
                 xsum[half * 128 + r] = sum;
                 spl_paged_pair_barrier(quarter);
                 sum += xsum[(half ^ 1) * 128 + r];
                 const bool here = r < it.q_count;
-                const int packed = it.q0 + r;
-                const size_t place = (size_t(it.row0 + packed / s.group) * s.heads + it.kv_head * s.group + packed % s.group) * HD + half * (HD / 2);
-                const size_t slot_row = size_t(it.slot) * a.slot_rows + r;
+                const size_t place = (size_t(row0 + row) * s.heads + head) * HD + half * (HD / 2);
                 const float inv = it.slot < 0 ? 1.0f / sum : 1.0f;
 #pragma unroll 1
-                for (int o = 0; o < HD / 2; o += 16) {
-                    uint32_t y[16];
-                    spl_tc_ld16(y, tmem_o + lanes + half * (HD / 2) + o);
+                for (int o = 0; o < HD / 2; o += 32) {
+                    uint32_t y[32];
+                    spl_tc_ld32(y, tmem_o + lanes + half * (HD / 2) + o);
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) y[j] = __float_as_uint(__uint_as_float(y[j]) * inv);
+                    for (int j = 0; j < 32; ++j) y[j] = __float_as_uint(__uint_as_float(y[j]) * inv);
                     if (!here) {
                     } else if (it.slot >= 0 || a.out_f32) {
                         float *dst = it.slot >= 0 ? a.partial + slot_row * HD + half * (HD / 2) + o : static_cast<float *>(a.out) + place + o;
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4 *>(dst + 4 * j) = make_uint4(y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]);
+                        for (int j = 0; j < 8; ++j) *reinterpret_cast<uint4 *>(dst + 4 * j) = make_uint4(y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]);
                     } else {
-                        uint32_t w[8];
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) w[j] = spl_pack16<BF16>(__uint_as_float(y[2 * j]), __uint_as_float(y[2 * j + 1]));
                         uint4 *dst = reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.out) + place + o);
-                        dst[0] = make_uint4(w[0], w[1], w[2], w[3]); dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            uint32_t w[4];
+#pragma unroll
+                            for (int u = 0; u < 4; ++u) w[u] = spl_pack16<BF16>(__uint_as_float(y[8 * j + 2 * u]), __uint_as_float(y[8 * j + 2 * u + 1]));
+                            dst[j] = make_uint4(w[0], w[1], w[2], w[3]);
+                        }
                     }
                     __syncwarp();
                 }
                 if (here && it.slot >= 0 && half == 0) a.partial_ml[slot_row] = make_float2(ref, sum);
+                spl_tc_fence_before();
                 spl_paged_pair_barrier(quarter);              // the sums in shared memory are read before the next piece's
             }
+            if (it.slot >= 0) {
+                // Whichever block is the last to leave a piece of these rows joins them, in the order of the pieces whoever it is.
+                __threadfence();
+                spl_named_barrier<5, 256>();
+                if (tid == 0) {
+                    const bool all = atomicAdd(&a.arrived[it.merge], 1) == it.pieces - 1;
+                    if (all) a.arrived[it.merge] = 0;          // for the next launch
+                    *joins = all;
+                }
+                spl_named_barrier<5, 256>();
+                if (*joins) {
+                    __threadfence();
+                    spl_paged_join<HD, BF16>(s, a, it, row0, it.q0 % s.group, per_group);
+                }
+            }
+            it = next;
         }
     }
     spl_tc_fence_before();
     __syncthreads();
     spl_tc_fence_after();
     if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512) : "memory");
-}
-
-// The pieces of a tile of query rows joined: o = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s. Grid (blocks of the attention, row groups of eight), 256 threads: a warp a row.
-template <int HD, bool BF16>
-__global__ void __launch_bounds__(256)
-spl_paged_merge_kernel(const int *__restrict__ counts, const SplPagedMerge *__restrict__ merges, SplPagedShape s, const float *__restrict__ partial, const float2 *__restrict__ partial_ml,
-                       int slot_rows, void *out, int out_f32) {
-    spl_grid_begin();
-    if (int(blockIdx.x) >= counts[2]) return;
-    const SplPagedMerge mg = merges[blockIdx.x];
-    const int r = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (r >= mg.q_count) return;
-    float m = -INFINITY;
-    for (int n = 0; n < mg.slots; ++n) m = fmaxf(m, partial_ml[size_t(mg.slot + n) * slot_rows + r].x);
-    float2 acc[HD / 64];
-    float sum = 0.0f;
-#pragma unroll
-    for (int j = 0; j < HD / 64; ++j) acc[j] = make_float2(0.0f, 0.0f);
-    for (int n = 0; n < mg.slots; ++n) {
-        const size_t row = size_t(mg.slot + n) * slot_rows + r;
-        const float2 ml = partial_ml[row];
-        if (ml.x == -INFINITY) continue;                      // a piece of whose tokens this row sees none
-        const float f = exp2f(ml.x - m);
-        sum += f * ml.y;
-#pragma unroll
-        for (int j = 0; j < HD / 64; ++j) {
-            const float2 v = *reinterpret_cast<const float2 *>(partial + row * HD + 64 * j + 2 * lane);
-            acc[j].x += f * v.x; acc[j].y += f * v.y;
-        }
-    }
-    const float inv = 1.0f / sum;
-    const int packed = mg.q0 + r;
-    const size_t place = (size_t(mg.row0 + packed / s.group) * s.heads + mg.kv_head * s.group + packed % s.group) * HD;
-#pragma unroll
-    for (int j = 0; j < HD / 64; ++j) {
-        if (out_f32) *reinterpret_cast<float2 *>(static_cast<float *>(out) + place + 64 * j + 2 * lane) = make_float2(acc[j].x * inv, acc[j].y * inv);
-        else *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(out) + place + 64 * j + 2 * lane) = spl_pack16<BF16>(acc[j].x * inv, acc[j].y * inv);
-    }
 }

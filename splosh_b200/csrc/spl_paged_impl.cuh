@@ -23,9 +23,9 @@ struct spl_paged {
     SplPagedShape shape{};
     int max_pages = 0;
     SplEncodeTiled encode = nullptr;
-    // Device tables in one block, filled from one of two pinned blocks (the other's copy may still be on its way): counts, block_begin, merges and items of
-    // the attention's plan; then the batch. Places do not depend on the batch, so a captured graph finds the next one's.
-    size_t words = 0, begin_at = 16, merges_at = 0, items_at = 0, batch_at = 0;
+    // Device tables in one block, filled from one of two pinned blocks (the other's copy may still be on its way): counts, the attention's plan (block_begin, the pieces that
+    // have arrived of each merge: none, the blocks' first items, items); then the batch. Places do not depend on the batch, so a captured graph finds the next one's.
+    size_t words = 0, begin_at = 16, arrived_at = 0, starts_at = 0, items_at = 0, batch_at = 0;
     SplPagedPlan plan;
     // Partial sums of query rows whose tokens several blocks share.
     int slot_rows = 0;
@@ -67,8 +67,9 @@ static spl_status paged_create(spl_engine *e, const spl_paged_config *cp, spl_pa
     p->shape = SplPagedShape{c.heads, c.kv_heads, c.heads / c.kv_heads, c.head_dim, c.page_tokens, p->max_pages, c.page_stride, c.head_stride, c.token_stride, c.rotary_dim, c.causal != 0, c.window,
                              c.scale > 0.0f ? c.scale : float(1.0 / std::sqrt(double(c.head_dim)))};
     const size_t blocks = size_t(e->sms), items = size_t(spl_paged_items_max(c, e->sms));
-    p->merges_at = p->begin_at + (blocks + 1 + 3) / 4 * 4;
-    p->items_at = p->merges_at + blocks * (sizeof(SplPagedMerge) / 4);
+    p->arrived_at = p->begin_at + (blocks + 1 + 3) / 4 * 4;
+    p->starts_at = p->arrived_at + (blocks + 3) / 4 * 4;
+    p->items_at = p->starts_at + blocks * (sizeof(SplPagedItem) / 4);
     p->batch_at = p->items_at + items * (sizeof(SplPagedItem) / 4);
     p->words = p->batch_at + size_t(c.max_rows) * 2 + size_t(c.max_sequences) * 2 + size_t(p->max_pages) * c.max_sequences;
     p->written.assign(size_t(c.pages), 0);
@@ -119,9 +120,10 @@ static spl_status paged_batch(spl_paged *p, int32_t sequences, const int32_t *ro
     SPL_CUDA(cudaEventSynchronize(p->copied[turn]));      // this block's last copy
     int *w = p->tables_host[turn];
     std::memset(w, 0, 16 * 4);
-    w[0] = int(total); w[1] = sequences; w[2] = int(p->plan.merges.size());
+    w[0] = int(total); w[1] = sequences;
     std::memcpy(w + p->begin_at, p->plan.block_begin.data(), p->plan.block_begin.size() * 4);
-    if (!p->plan.merges.empty()) std::memcpy(w + p->merges_at, p->plan.merges.data(), p->plan.merges.size() * sizeof(SplPagedMerge));
+    std::memset(w + p->arrived_at, 0, size_t(e->sms) * 4);
+    std::memcpy(w + p->starts_at, p->plan.starts.data(), p->plan.starts.size() * sizeof(SplPagedItem));
     std::memcpy(w + p->items_at, p->plan.items.data(), p->plan.items.size() * sizeof(SplPagedItem));
     int *row_sequence = w + p->batch_at, *row_position = row_sequence + c.max_rows, *seq_rows = row_position + c.max_rows, *seq_lengths = seq_rows + c.max_sequences, *pages = seq_lengths + c.max_sequences;
     for (int s = 0, r = 0; s < sequences; ++s) {
@@ -170,9 +172,6 @@ static bool paged_map(const spl_paged *p, const void *cache, bool values, CUtens
 
 template <int HD, bool BF16> static void launch_attend(const spl_paged *p, const CUtensorMap &k_map, const CUtensorMap &v_map, const SplPagedAttend &a, cudaStream_t stream) {
     launch_step(spl_paged_attend_kernel<HD, BF16>, dim3(p->e->sms), dim3(SPL_PAGED_THREADS), spl_paged_smem_bytes(HD), stream, k_map, v_map, p->tables(), p->shape, a);
-    // Always launched: a captured graph's next batch may have pieces to join where this one has none.
-    launch_step(spl_paged_merge_kernel<HD, BF16>, dim3(p->e->sms, (p->slot_rows + 7) / 8), dim3(256), 0, stream, (const int *)p->tables_dev,
-                reinterpret_cast<const SplPagedMerge *>(p->tables_dev + p->merges_at), p->shape, (const float *)p->partial, (const float2 *)p->partial_ml, p->slot_rows, a.out, a.out_f32);
 }
 
 // The blocks of a row's cluster: a wave of clusters costs some 14 us of meetings and sorting whatever a block's share, and 19 us for 32,768 values a block (they fit
@@ -277,8 +276,8 @@ spl_status spl_paged_attend(spl_paged *p, const void *device_q, const void *devi
     const SplDeviceScope scope(e->device);
     CUtensorMap k_map, v_map;
     if (!paged_map(p, device_k_cache, false, &k_map) || !paged_map(p, device_v_cache, true, &v_map)) return refuse("the driver takes no tensor map of this cache");
-    const SplPagedAttend a{static_cast<const uint16_t *>(device_q), device_out, out_type == SPL_F32, reinterpret_cast<const SplPagedItem *>(p->tables_dev + p->items_at), p->tables_dev + p->begin_at,
-                           p->partial, p->partial_ml, p->slot_rows, e->tc_error};
+    const SplPagedAttend a{static_cast<const uint16_t *>(device_q), device_out, out_type == SPL_F32, reinterpret_cast<const SplPagedItem *>(p->tables_dev + p->starts_at),
+                           reinterpret_cast<const SplPagedItem *>(p->tables_dev + p->items_at), p->tables_dev + p->begin_at, p->tables_dev + p->arrived_at, p->partial, p->partial_ml, p->slot_rows, e->tc_error};
     cudaStream_t st = paged_stream(e, stream);
     const bool bf16 = c.dtype == SPL_BF16;
     if (c.head_dim == 64) { if (bf16) launch_attend<64, true>(p, k_map, v_map, a, st); else launch_attend<64, false>(p, k_map, v_map, a, st); }
@@ -346,11 +345,15 @@ spl_status spl_debug_paged_plan(const spl_paged_config *config, int32_t blocks, 
     try {
         SplPagedPlan plan;
         spl_paged_plan(*config, blocks, sequences, rows, lengths, plan);
-        if (plan.items.size() > size_t(std::max(items_capacity, 0)) || plan.merges.size() > size_t(blocks)) return SPL_ERR_ALLOCATION_FAILED;
+        if (plan.items.size() > size_t(std::max(items_capacity, 0)) || plan.merges > blocks) return SPL_ERR_ALLOCATION_FAILED;
         std::memcpy(block_begin, plan.block_begin.data(), plan.block_begin.size() * 4);
-        std::memcpy(items, plan.items.data(), plan.items.size() * sizeof(SplPagedItem));
-        if (!plan.merges.empty()) std::memcpy(merges, plan.merges.data(), plan.merges.size() * sizeof(SplPagedMerge));
-        *item_count = int32_t(plan.items.size()); *merge_count = int32_t(plan.merges.size());
+        for (size_t i = 0; i < plan.items.size(); ++i) {
+            const SplPagedItem &it = plan.items[i];
+            std::memcpy(items + 8 * i, &it, 8 * 4);
+            const int32_t merge[8] = {it.row0, it.kv_head, it.q0, it.q_count, it.slot0, it.pieces, it.length, it.base};
+            if (it.merge >= 0) std::memcpy(merges + 8 * it.merge, merge, sizeof merge);
+        }
+        *item_count = int32_t(plan.items.size()); *merge_count = plan.merges;
         return SPL_OK;
     } catch (const std::bad_alloc &) { return SPL_ERR_ALLOCATION_FAILED; }
 }

@@ -13,18 +13,18 @@
 
 // A block's piece of work: packed query rows [q0, q0 + q_count) of a sequence (packed row i is the sequence's new token i / group, head i % group of
 // the kv head) against the tokens [tile_begin * 128, tile_end * 128). slot >= 0: the piece is one of several of its rows and leaves
-// partial sums there.
-struct SplPagedItem { int32_t sequence, row0, kv_head, q0, q_count, tile_begin, tile_end, slot; };
-// Rows whose pieces' partial sums are to be joined: slots [slot, slot + slots).
-struct SplPagedMerge { int32_t row0, kv_head, q0, q_count, slot, slots, reserved[2]; };
+// partial sums there; the `pieces` of its rows, merge number `merge`, have the slots from slot0 on. length: the sequence's tokens; base: the position of
+// its first new one.
+struct alignas(16) SplPagedItem { int32_t sequence, row0, kv_head, q0, q_count, tile_begin, tile_end, slot, length, base, merge, pieces, slot0, reserved[3]; };
 
 struct SplPagedPlan {
     std::vector<SplPagedItem> items;
     std::vector<int32_t> block_begin;         // [blocks + 1]: a block's items
-    std::vector<SplPagedMerge> merges;
+    std::vector<SplPagedItem> starts;         // [blocks]: a block's first item (none: no tiles)
+    int merges = 0;
 };
 
-// Most items and merges that a configuration's batches come to: a block's boundary cuts at most one tile of query rows.
+// Most items that a configuration's batches come to: a block's boundary cuts at most one tile of query rows.
 inline int64_t spl_paged_items_max(const spl_paged_config &c, int blocks) {
     const int64_t group = c.heads / c.kv_heads;
     return c.kv_heads * (int64_t(c.max_rows) * group / SPL_PAGED_TILE + std::min(c.max_sequences, c.max_rows)) + blocks;
@@ -102,7 +102,7 @@ inline void spl_paged_plan(const spl_paged_config &c, int blocks, int32_t sequen
             for (int q0 = 0; q0 < rows[s] * group; q0 += tile) {
                 const int count = std::min(tile, rows[s] * group - q0), base = lengths[s] - rows[s];
                 const int first = spl_paged_first_token(c, base + q0 / group), last = c.causal ? base + (q0 + count - 1) / group + 1 : lengths[s];
-                const SplPagedItem u{s, row0, h, q0, count, first / tile, (last + tile - 1) / tile, -1};
+                const SplPagedItem u{s, row0, h, q0, count, first / tile, (last + tile - 1) / tile, -1, lengths[s], base, -1, 1, 0, {0, 0, 0}};
                 tiles += u.tile_end - u.tile_begin;
                 longest = std::max(longest, u.tile_end - u.tile_begin);
                 whole.push_back(u);
@@ -120,7 +120,7 @@ inline void spl_paged_plan(const spl_paged_config &c, int blocks, int32_t sequen
     };
     int64_t low = SPL_PAGED_PIECE_COST + 1, high = std::max<int64_t>(low, tiles + int64_t(whole.size()) * SPL_PAGED_PIECE_COST);
     while (low < high) { const int64_t mid = (low + high) / 2; if (blocks_for(mid) <= blocks) high = mid; else low = mid + 1; }
-    units.clear(); plan.merges.clear();
+    units.clear(); plan.merges = 0;
     plan.block_begin.assign(1, 0);
     int64_t left = low;
     int slots = 0;
@@ -136,12 +136,14 @@ inline void spl_paged_plan(const spl_paged_config &c, int blocks, int32_t sequen
         }
         const int pieces = int(units.size() - piece0);
         if (pieces > 1) {
-            plan.merges.push_back(SplPagedMerge{u.row0, u.kv_head, u.q0, u.q_count, slots, pieces, {0, 0}});
-            for (size_t i = piece0; i < units.size(); ++i) units[i].slot = slots++;
+            for (size_t i = piece0; i < units.size(); ++i) { units[i].slot = slots + int(i - piece0); units[i].slot0 = slots; units[i].pieces = pieces; units[i].merge = plan.merges; }
+            slots += pieces; ++plan.merges;
         }
     }
     plan.block_begin.resize(size_t(blocks) + 1, int32_t(units.size()));
     plan.block_begin[blocks] = int32_t(units.size());
+    plan.starts.assign(size_t(blocks), SplPagedItem{});
+    for (int b = 0; b < blocks; ++b) if (plan.block_begin[b] < plan.block_begin[b + 1]) plan.starts[b] = units[plan.block_begin[b]];
 }
 // Slots that a plan of `blocks` stretches takes at most: each cut between two blocks makes two pieces of one.
 inline int spl_paged_slots_max(int blocks) { return 2 * blocks; }
