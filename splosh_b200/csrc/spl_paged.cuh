@@ -214,45 +214,76 @@ struct SplPagedAttend {
     int *error_flag;
 };
 
-// The pieces of a tile of query rows joined: o = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s. Eight warps, a warp a row, four pieces' sums on their way.
-template <int HD, bool BF16>
-__device__ __forceinline__ void spl_paged_join(const SplPagedShape &s, const SplPagedAttend &a, const SplPagedItem &it, int row0, int head0, uint32_t per_group) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (int r = warp; r < it.q_count; r += 8) {
-        float m = -INFINITY;
-        for (int n = lane; n < it.pieces; n += 32) m = fmaxf(m, __ldcg(&a.partial_ml[size_t(it.slot0 + n) * a.slot_rows + r]).x);
-        m = spl_warp_max(m);
-        float2 acc[HD / 64];
-        float sum = 0.0f;
+// The pieces of a tile of query rows joined by 256 threads: o = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s. First m and 1 / sum of every row, to shared memory (`scratch`,
+// 256 floats); then the sums, four channels a thread, as many on their way as there are registers for: UP groups of 1024 channels times UN pieces.
+template <int HD, bool BF16, int UP, int UN>
+__device__ __forceinline__ void spl_paged_join_sums(const SplPagedShape &s, const SplPagedAttend &a, const SplPagedItem &it, int row0, int head0, uint32_t per_group, const float *scratch) {
+    const int fours = it.q_count * (HD / 4);
+    for (int base = threadIdx.x; base < fours; base += UP * 256) {
+        float4 acc[UP];
 #pragma unroll
-        for (int j = 0; j < HD / 64; ++j) acc[j] = make_float2(0.0f, 0.0f);
-        for (int n0 = 0; n0 < it.pieces; n0 += 4) {
-            float2 ml[4], v[4][HD / 64];
+        for (int u = 0; u < UP; ++u) acc[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int n0 = 0; n0 < it.pieces; n0 += UN) {
+            float4 v[UP][UN];
+            float ref[UP][UN];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const size_t row = size_t(it.slot0 + min(n0 + u, it.pieces - 1)) * a.slot_rows + r;
-                ml[u] = __ldcg(&a.partial_ml[row]);
+            for (int u = 0; u < UP; ++u)
 #pragma unroll
-                for (int j = 0; j < HD / 64; ++j) v[u][j] = __ldcg(reinterpret_cast<const float2 *>(a.partial + row * HD + 64 * j + 2 * lane));
-            }
+                for (int n = 0; n < UN; ++n) {
+                    const int idx = min(base + u * 256, fours - 1), r = idx / (HD / 4);
+                    const size_t row = size_t(it.slot0 + min(n0 + n, it.pieces - 1)) * a.slot_rows + r;
+                    v[u][n] = __ldcg(reinterpret_cast<const float4 *>(a.partial + row * HD) + idx % (HD / 4));
+                    ref[u][n] = __ldcg(&a.partial_ml[row].x);
+                }
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                if (n0 + u >= it.pieces || ml[u].x == -INFINITY) continue;      // (a piece of whose tokens this row sees none)
-                const float f = exp2f(ml[u].x - m);
-                sum += f * ml[u].y;
+            for (int u = 0; u < UP; ++u)
 #pragma unroll
-                for (int j = 0; j < HD / 64; ++j) { acc[j].x += f * v[u][j].x; acc[j].y += f * v[u][j].y; }
-            }
+                for (int n = 0; n < UN; ++n) {
+                    const int r = min(base + u * 256, fours - 1) / (HD / 4);
+                    if (n0 + n >= it.pieces || ref[u][n] == -INFINITY) continue;      // (a piece of whose tokens this row sees none)
+                    const float f = exp2f(ref[u][n] - scratch[r]);
+                    acc[u].x += f * v[u][n].x; acc[u].y += f * v[u][n].y; acc[u].z += f * v[u][n].z; acc[u].w += f * v[u][n].w;
+                }
         }
-        const float inv = 1.0f / sum;
-        const int x = head0 + r, row = int(x * per_group >> 16);
-        const size_t place = (size_t(row0 + row) * s.heads + it.kv_head * s.group + x - row * s.group) * HD;
 #pragma unroll
-        for (int j = 0; j < HD / 64; ++j) {
-            if (a.out_f32) *reinterpret_cast<float2 *>(static_cast<float *>(a.out) + place + 64 * j + 2 * lane) = make_float2(acc[j].x * inv, acc[j].y * inv);
-            else *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(a.out) + place + 64 * j + 2 * lane) = spl_pack16<BF16>(acc[j].x * inv, acc[j].y * inv);
+        for (int u = 0; u < UP; ++u) {
+            const int idx = base + u * 256;
+            if (idx >= fours) continue;
+            const int r = idx / (HD / 4), x = head0 + r, row = int(x * per_group >> 16);
+            const float inv = scratch[128 + r];
+            const size_t place = (size_t(row0 + row) * s.heads + it.kv_head * s.group + x - row * s.group) * HD + idx % (HD / 4) * 4;
+            if (a.out_f32) *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + place) = make_float4(acc[u].x * inv, acc[u].y * inv, acc[u].z * inv, acc[u].w * inv);
+            else *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + place) = make_uint2(spl_pack16<BF16>(acc[u].x * inv, acc[u].y * inv), spl_pack16<BF16>(acc[u].z * inv, acc[u].w * inv));
         }
     }
+}
+template <int HD, bool BF16>
+__device__ __forceinline__ void spl_paged_join(const SplPagedShape &s, const SplPagedAttend &a, const SplPagedItem &it, int row0, int head0, uint32_t per_group, float *scratch) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    auto at = [&](int n, int r) { return __ldcg(&a.partial_ml[size_t(it.slot0 + n) * a.slot_rows + r]); };
+    if (it.pieces <= 4) {                                     // a thread a row
+        const int r = threadIdx.x;
+        if (r < it.q_count) {
+            float2 ml[4];
+#pragma unroll
+            for (int n = 0; n < 4; ++n) ml[n] = n < it.pieces ? at(n, r) : make_float2(-INFINITY, 0.0f);
+            const float m = fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x));
+            float sum = 0.0f;
+#pragma unroll
+            for (int n = 0; n < 4; ++n) if (ml[n].x > -INFINITY) sum += exp2f(ml[n].x - m) * ml[n].y;
+            scratch[r] = m; scratch[128 + r] = 1.0f / sum;
+        }
+    } else for (int r = warp; r < it.q_count; r += 8) {       // a warp a row
+        float m = -INFINITY, sum = 0.0f;
+        for (int n = lane; n < it.pieces; n += 32) m = fmaxf(m, at(n, r).x);
+        m = spl_warp_max(m);
+        for (int n = lane; n < it.pieces; n += 32) { const float2 ml = at(n, r); if (ml.x > -INFINITY) sum += exp2f(ml.x - m) * ml.y; }
+        sum = spl_warp_sum(sum);
+        if (lane == 0) { scratch[r] = m; scratch[128 + r] = 1.0f / sum; }
+    }
+    spl_named_barrier<5, 256>();
+    if (it.pieces <= 2) spl_paged_join_sums<HD, BF16, 6, 2>(s, a, it, row0, head0, per_group, scratch);
+    else spl_paged_join_sums<HD, BF16, 2, 6>(s, a, it, row0, head0, per_group, scratch);
 }
 
 template <int HD, bool BF16>
@@ -576,7 +607,8 @@ spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
                 spl_named_barrier<5, 256>();
                 if (*joins) {
                     __threadfence();
-                    spl_paged_join<HD, BF16>(s, a, it, row0, it.q0 % s.group, per_group);
+                    spl_paged_join<HD, BF16>(s, a, it, row0, it.q0 % s.group, per_group, xmax + (tiles & 1) * 2 * 128);
+                    spl_named_barrier<5, 256>();               // before the next piece's maxima
                 }
             }
             it = next;

@@ -86,11 +86,26 @@ inline spl_status spl_paged_batch_check(const spl_paged_config &c, int32_t seque
     return SPL_OK;
 }
 
-// The tiles of all (sequence, kv head, 128 packed rows) in a line, cut in one stretch a block of equal cost, a piece costing its tiles and
-// SPL_PAGED_PIECE_COST more (queries in, the pipeline's start, the output). The pieces of a tile of rows that a cut goes through are joined afterwards.
-// (Whole tiles of rows, longest first, leave the last round of blocks idle for prompts and most of the GPU for decode steps of few sequences; a stretch a
-// block has neither.)
+// The tiles of all (sequence, kv head, 128 packed rows) in a line, cut in one stretch a block of equal cost. In tiles: a piece costs its tiles and
+// SPL_PAGED_PIECE_COST more (the first keys' way, the output), and a piece of a cut unit what leaving and joining partial sums takes, which goes by the rows.
+// Units of many rows are cut only into pieces that are worth it. (Whole units, longest first, leave the last round of blocks idle for prompts and most of the GPU for
+// decode steps of few sequences; stretches that cut everything spent 25 of 47 us on joining 1-tile pieces of 128 rows in a step of six decoding sessions and a
+// 301-token prompt.)
 #define SPL_PAGED_PIECE_COST 2
+inline int spl_paged_cut_cost(int q_count) { return q_count <= 16 ? 0 : q_count <= 64 ? 1 : 2; }
+inline int spl_paged_cut_least(int q_count) { return q_count <= 16 ? 1 : q_count <= 64 ? 3 : 5; }      // tiles a piece
+// What a block that has `left` of its stretch takes of the `t` tiles left of a unit (cut: some have gone to another block): 0, some, or all; -1: the stretch is too short
+// for this unit's pieces.
+inline int64_t spl_paged_take(int64_t t, int64_t left, int64_t stretch, int q_count, bool cut) {
+    const int64_t piece = SPL_PAGED_PIECE_COST + (cut ? spl_paged_cut_cost(q_count) : 0);
+    if (t + piece <= left) return t;
+    const int64_t least = spl_paged_cut_least(q_count), some = left - SPL_PAGED_PIECE_COST - spl_paged_cut_cost(q_count);
+    if (t >= 2 * least) {
+        if (some >= least) return std::min(some, t - least);    // (a rest is a piece, too)
+        return left == stretch ? -1 : 0;
+    }
+    return left == stretch ? t : 0;                             // not worth a cut: whole, in a block of its own at the worst
+}
 inline void spl_paged_plan(const spl_paged_config &c, int blocks, int32_t sequences, const int32_t *rows, const int32_t *lengths, SplPagedPlan &plan) {
     const int group = c.heads / c.kv_heads, tile = SPL_PAGED_TILE;
     std::vector<SplPagedItem> &units = plan.items;
@@ -111,14 +126,16 @@ inline void spl_paged_plan(const spl_paged_config &c, int blocks, int32_t sequen
     auto blocks_for = [&](int64_t stretch) {
         int64_t used = 1, left = stretch;
         for (const SplPagedItem &u : whole)
-            for (int64_t t = u.tile_end - u.tile_begin; t > 0;) {
-                if (left <= SPL_PAGED_PIECE_COST) { ++used; left = stretch; }
-                const int64_t take = std::min(t, left - SPL_PAGED_PIECE_COST);
-                t -= take; left -= take + SPL_PAGED_PIECE_COST;
+            for (int64_t t = u.tile_end - u.tile_begin, all = t; t > 0;) {
+                const int64_t take = spl_paged_take(t, left, stretch, u.q_count, t < all);
+                if (take < 0) return int64_t(blocks) + 1;
+                if (!take) { if (++used > blocks) return used; left = stretch; continue; }
+                left -= take + SPL_PAGED_PIECE_COST + (take < all ? spl_paged_cut_cost(u.q_count) : 0);
+                t -= take;
             }
         return used;
     };
-    int64_t low = SPL_PAGED_PIECE_COST + 1, high = std::max<int64_t>(low, tiles + int64_t(whole.size()) * SPL_PAGED_PIECE_COST);
+    int64_t low = SPL_PAGED_PIECE_COST + 1, high = std::max<int64_t>(low, tiles + int64_t(whole.size()) * (SPL_PAGED_PIECE_COST + 2));
     while (low < high) { const int64_t mid = (low + high) / 2; if (blocks_for(mid) <= blocks) high = mid; else low = mid + 1; }
     units.clear(); plan.merges = 0;
     plan.block_begin.assign(1, 0);
@@ -126,13 +143,15 @@ inline void spl_paged_plan(const spl_paged_config &c, int blocks, int32_t sequen
     int slots = 0;
     for (const SplPagedItem &u : whole) {
         const size_t piece0 = units.size();
+        const int all = u.tile_end - u.tile_begin;
         for (int t = u.tile_begin; t < u.tile_end;) {
-            if (left <= SPL_PAGED_PIECE_COST) { plan.block_begin.push_back(int32_t(units.size())); left = low; }
-            const int take = int(std::min<int64_t>(u.tile_end - t, left - SPL_PAGED_PIECE_COST));
+            const int take = int(spl_paged_take(u.tile_end - t, left, low, u.q_count, t > u.tile_begin));
+            if (!take) { plan.block_begin.push_back(int32_t(units.size())); left = low; continue; }
             SplPagedItem piece = u;
             piece.tile_begin = t; piece.tile_end = t + take;
             units.push_back(piece);
-            t += take; left -= take + SPL_PAGED_PIECE_COST;
+            left -= take + SPL_PAGED_PIECE_COST + (take < all ? spl_paged_cut_cost(u.q_count) : 0);
+            t += take;
         }
         const int pieces = int(units.size() - piece0);
         if (pieces > 1) {
@@ -145,5 +164,5 @@ inline void spl_paged_plan(const spl_paged_config &c, int blocks, int32_t sequen
     plan.starts.assign(size_t(blocks), SplPagedItem{});
     for (int b = 0; b < blocks; ++b) if (plan.block_begin[b] < plan.block_begin[b + 1]) plan.starts[b] = units[plan.block_begin[b]];
 }
-// Slots that a plan of `blocks` stretches takes at most: each cut between two blocks makes two pieces of one.
+// Slots that a plan of `blocks` stretches takes at most: a unit is cut only where a block ends, and each such cut makes two pieces of one.
 inline int spl_paged_slots_max(int blocks) { return 2 * blocks; }

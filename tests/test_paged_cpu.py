@@ -89,7 +89,22 @@ def test_every_visible_tile_is_done_once(seed):
             assert slots == joined.pop((starts[s], h, q0, count))
             used += slots
     assert not joined and sorted(used) == list(range(len(used))) and len(used) <= 2 * blocks and len(merges) <= blocks
-    load = [sum(int(i[6] - i[5]) + 2 for i in items[a:b]) for a, b in zip(begin, begin[1:])]
-    total = sum(int(i[6] - i[5]) for i in items)
-    whole = sum(1 for _ in expected)
-    assert max(load) <= (total + 2 * (whole + blocks)) / blocks + 3 or max(load) <= 3
+    # A block's load: its tiles, two more a piece and the joining; no block carries much more than its share, or than the least that is not cut.
+    def cost(item):
+        rows_there = 0 if item[7] < 0 or item[4] <= 16 else 1 if item[4] <= 64 else 2
+        return int(item[6] - item[5]) + 2 + rows_there
+    load = [sum(cost(i) for i in items[a:b]) for a, b in zip(begin, begin[1:])]
+    share = (sum(int(i[6] - i[5]) for i in items) + 4 * (len(expected) + blocks)) / blocks
+    assert max(load) <= 2 * share + 14
+    for (s, h, q0, count), pieces in done.items():
+        if len(pieces) > 1:
+            assert min(t1 - t0 for t0, t1, _ in pieces) >= (1 if count <= 16 else 3 if count <= 64 else 5)
+
+
+def test_a_single_sequence_is_spread_over_the_blocks():
+    """One decoding session: pieces of a tile or two on as many blocks; one long prompt: every block within two percent of its share."""
+    begin, items, _ = debug_paged_plan([1], [1024], heads=8, kv_heads=2, head_dim=128, pages=1, max_sequences=1, max_rows=1, max_context=1024)
+    assert len(items) == 16 and (np.diff(begin) <= 1).all()
+    begin, items, _ = debug_paged_plan([2048], [26624], heads=24, kv_heads=4, head_dim=256, pages=1, max_sequences=1, max_rows=2048, max_context=1 << 16)
+    tiles = np.array([sum(int(i[6] - i[5]) for i in items[a:b]) for a, b in zip(begin, begin[1:])])
+    assert tiles.max() <= 1.02 * tiles.mean()
