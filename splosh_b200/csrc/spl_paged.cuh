@@ -136,7 +136,8 @@ spl_paged_append_kernel(SplPagedRows in, const uint16_t *__restrict__ q_norm, co
 // Warps 0-7 softmax (thread: a row and half of the tile's tokens; the pair of warps of 32 rows agrees on the maximum), warp 8 copies, warps 9 and
 // 10 issue the products: S of tile i + 1 runs under the softmax of tile i. The reference is raised only when a row's maximum exceeds it by 2^8, so the sums in
 // tensor memory are rescaled a few times a piece, not every tile. Rows that are not there cost no softmax work.
-// Tensor memory: S / P two buffers of 128 columns (P, 16 bits, over the S it came from), O HD columns from 256.
+// Tensor memory: S / P two buffers of 128 columns (P, 16 bits, over the S it came from), O HD columns from 256. (At HD = 128 there is room for P beside S: with the next tile's
+// scores loaded under a tile's exponentials 2,048 rows over 8,192 tokens of 32/8 heads took 303 us instead of 264, with two groups of four warps taking turns at the tiles 282.)
 //
 // Rounding: P to the cache's type (what the tensor core takes beside V); S, m, the sums of P and O are fp32. In fp16 P is scaled by 2^7 (the factor
 // cancels), so that probabilities down to 2^-21 of the reference keep all bits and one 2^8 above it stays finite.
@@ -261,6 +262,50 @@ template <int HD, bool BF16>
 __device__ __forceinline__ void spl_paged_join(const SplPagedShape &s, const SplPagedAttend &a, const SplPagedItem &it, int row0, int head0, uint32_t per_group, float *scratch) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     auto at = [&](int n, int r) { return __ldcg(&a.partial_ml[size_t(it.slot0 + n) * a.slot_rows + r]); };
+    if (it.q_count <= 8) {
+        // A row a warp (a single token's heads): nothing to exchange. A running reference, eight pieces on their way.
+        if (warp >= it.q_count) return;
+        const int x = head0 + warp, row = int(x * per_group >> 16);
+        float2 acc[HD / 64];
+        float m = -INFINITY, sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < HD / 64; ++j) acc[j] = make_float2(0.0f, 0.0f);
+        for (int n0 = 0; n0 < it.pieces; n0 += 8) {
+            float2 ml[8], v[8][HD / 64];
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+                const int p = min(n0 + n, it.pieces - 1);
+                ml[n] = at(p, warp);
+#pragma unroll
+                for (int j = 0; j < HD / 64; ++j) v[n][j] = __ldcg(reinterpret_cast<const float2 *>(a.partial + (size_t(it.slot0 + p) * a.slot_rows + warp) * HD + 64 * j + 2 * lane));
+            }
+            float now = m;
+#pragma unroll
+            for (int n = 0; n < 8; ++n) if (n0 + n < it.pieces) now = fmaxf(now, ml[n].x);
+            if (now == -INFINITY) continue;
+            const float old = exp2f(m - now);
+            sum *= old;
+#pragma unroll
+            for (int j = 0; j < HD / 64; ++j) { acc[j].x *= old; acc[j].y *= old; }
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+                if (n0 + n >= it.pieces || ml[n].x == -INFINITY) continue;      // (a piece of whose tokens this row sees none)
+                const float f = exp2f(ml[n].x - now);
+                sum += f * ml[n].y;
+#pragma unroll
+                for (int j = 0; j < HD / 64; ++j) { acc[j].x += f * v[n][j].x; acc[j].y += f * v[n][j].y; }
+            }
+            m = now;
+        }
+        const float inv = 1.0f / sum;
+        const size_t place = (size_t(row0 + row) * s.heads + it.kv_head * s.group + x - row * s.group) * HD;
+#pragma unroll
+        for (int j = 0; j < HD / 64; ++j) {
+            if (a.out_f32) *reinterpret_cast<float2 *>(static_cast<float *>(a.out) + place + 64 * j + 2 * lane) = make_float2(acc[j].x * inv, acc[j].y * inv);
+            else *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(a.out) + place + 64 * j + 2 * lane) = spl_pack16<BF16>(acc[j].x * inv, acc[j].y * inv);
+        }
+        return;
+    }
     if (it.pieces <= 4) {                                     // a thread a row
         const int r = threadIdx.x;
         if (r < it.q_count) {
@@ -511,9 +556,13 @@ spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
                             if (t0 + 32 + j < first || t0 + 32 + j >= last) x1[j] = 0xff800000u;
                         }
                     }
-                    float m = -INFINITY;
+                    float m = -INFINITY, n = -INFINITY;
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) m = fmaxf(m, fmaxf(__uint_as_float(x0[j]), __uint_as_float(x1[j])));
+                    for (int j = 0; j < 32; j += 2) {
+                        m = fmaxf(m, fmaxf(__uint_as_float(x0[j]), __uint_as_float(x0[j + 1])));
+                        n = fmaxf(n, fmaxf(__uint_as_float(x1[j]), __uint_as_float(x1[j + 1])));
+                    }
+                    m = fmaxf(m, n);
                     xmax[(buf * 2 + half) * 128 + r] = m;
                     spl_paged_pair_barrier(quarter);
                     m = fmaxf(m, xmax[(buf * 2 + (half ^ 1)) * 128 + r]) * c;
@@ -536,16 +585,17 @@ spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
                         if (raise) { sum *= factor; ref = m; }
                     }
                     const float offset = (ref == -INFINITY ? 0.0f : -ref) + PBIAS;      // a row that has seen nothing yet: all its scores are -inf
-                    float part = 0.0f;
+                    const float2 c2 = make_float2(c, c), offset2 = make_float2(offset, offset);
+                    float2 part = make_float2(0.0f, 0.0f);
                     uint32_t p[32];
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const float p0 = spl_ex2(fmaf(__uint_as_float(x0[2 * j]), c, offset)), p1 = spl_ex2(fmaf(__uint_as_float(x0[2 * j + 1]), c, offset));
-                        const float p2 = spl_ex2(fmaf(__uint_as_float(x1[2 * j]), c, offset)), p3 = spl_ex2(fmaf(__uint_as_float(x1[2 * j + 1]), c, offset));
-                        part += (p0 + p1) + (p2 + p3);
-                        p[j] = spl_pack16<BF16>(p0, p1); p[16 + j] = spl_pack16<BF16>(p2, p3);
+                    for (int j = 0; j < 32; ++j) {
+                        const uint32_t *x = j < 16 ? x0 + 2 * j : x1 + 2 * (j - 16);
+                        const float2 z = spl_fma2(make_float2(__uint_as_float(x[0]), __uint_as_float(x[1])), c2, offset2), e = make_float2(spl_ex2(z.x), spl_ex2(z.y));
+                        part = spl_add2(part, e);
+                        p[j] = spl_pack16<BF16>(e.x, e.y);
                     }
-                    sum += part;
+                    sum += part.x + part.y;
                     spl_tc_st32(at + half * 32, p);
                     spl_tc_st_wait();
                     spl_tc_fence_before();
