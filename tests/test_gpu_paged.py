@@ -119,6 +119,30 @@ def test_what_the_mask_hides_may_be_anything(engine):
     check_attention(scene, attend(engine, scene, "f32"), "f32")
 
 
+def test_what_is_no_number_in_a_token_that_is_seen_shows(engine):
+    """A NaN in one key or value reaches exactly the rows that see it, in any place of a tile."""
+    for place in (0, 1, 2, 3, 67, 130):
+        for which in ("k", "v"):
+            scene = Scene(place, 2, 1, 128, [140], [140], page_tokens=64)
+            getattr(scene, which)[scene.table[0, place // 64], 0, place % 64, 5] = float("nan")
+            out = attend(engine, scene, "f32")
+            assert out[place:].isnan().any(-1).all()
+            if which == "k":
+                assert not out[:place].isnan().any()
+
+
+def test_a_masked_tokens_values_do_not_count_however_large(engine):
+    """Later tokens of a chunk with values near the type's end: a weight of nothing, not of next to nothing."""
+    scene = Scene(17, 2, 1, 128, [100], [100], page_tokens=64)
+    keys, values = scene.tokens[0]
+    values[50:] = 3e38
+    for token in range(50, 100):
+        scene.v[scene.table[0, token // 64], :, token % 64] = 3e38
+    out = attend(engine, scene, "f32")[:50].double().cpu()
+    want, bound = scene.expected()
+    assert ((out - want[:50]).abs() <= bound[:50]).all()
+
+
 def test_strides_of_a_cache_that_holds_keys_and_values_side_by_side(engine):
     """K and V of a page next to each other, and the layers' pages interleaved: every stride larger than the data."""
     scene = Scene(11, 4, 2, 128, [3, 1], [90, 33], page_tokens=32)
