@@ -50,11 +50,13 @@ template <int TYPE> __device__ __forceinline__ float2 spl_load_pair(const void *
 // by the angle position * theta^(-2i / rotary); queries to their rows, keys and values to their place in the cache, all rounded once to
 // 16 bits. The angle is formed in 64 bits as turns (position * theta^(-2i/rotary) / 2 pi): at position 200,000 a 32-bit product is
 // off by 6e-3 of a radian, a 64-bit one by 1e-11; what is left of the whole turns fits 32 bits.
-// Grid (rows, head ranges), 256 threads: the angles' sines and cosines once a block, then a warp a head.
+// Grid (rows, head ranges), 256 threads: the angles' sines and cosines once a block, then a warp a head, the next head's channels on their way. Bound: the instructions of a head (some
+// 300; half the issue slots), then HBM: 2,048 rows of 24/4 heads of 256 (101 MB) 24 us at 48 registers, 29 without the loads ahead. With weights and angles in registers (250 instructions, but
+// three blocks an SM instead of five) 29, blocks that stay for several rows 27.
 struct SplPagedRows { const void *q, *k, *v; long long q_ld, k_ld, v_ld; };
 
 template <int TYPE, bool BF16>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 5)
 spl_paged_append_kernel(SplPagedRows in, const uint16_t *__restrict__ q_norm, const uint16_t *__restrict__ k_norm, const double *__restrict__ turns,
                         SplPagedTables t, SplPagedShape s, float eps, uint16_t *q_out, uint16_t *k_cache, uint16_t *v_cache) {
     __shared__ float2 turn[128];                 // (cos, sin) of channel pair i
@@ -70,26 +72,36 @@ spl_paged_append_kernel(SplPagedRows in, const uint16_t *__restrict__ q_norm, co
         sincospif(2.0f * float(a - rint(a)), &sn, &cs);
         turn[threadIdx.x] = make_float2(cs, sn);
     }
-    __syncthreads();
     const int page = t.table[size_t(sequence) * s.max_pages + position / s.page_tokens];
     const size_t place = size_t(page) * s.page_stride + size_t(position % s.page_tokens) * s.token_stride;
     float *mine = reinterpret_cast<float *>(vector[warp]);
     const int per = (vectors + gridDim.y - 1) / gridDim.y, last = min(vectors, int(blockIdx.y + 1) * per);
-    for (int n = blockIdx.y * per + warp; n < last; n += 8) {
+    // A head's channels 64 j + 2 lane and the next; the next head's are on their way meanwhile.
+    auto load = [&](int n, float2 (&x)[4]) {
+        const bool is_q = n < s.heads, is_v = n >= s.heads + s.kv_heads;
+        const void *src = is_q ? in.q : is_v ? in.v : in.k;
+        const size_t from = size_t(row) * (is_q ? in.q_ld : is_v ? in.v_ld : in.k_ld) + size_t(is_q ? n : is_v ? n - s.heads - s.kv_heads : n - s.heads) * hd + 2 * lane;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) if (64 * j < hd) x[j] = spl_load_pair<TYPE>(src, from + 64 * j);
+    };
+    float2 ahead[4];
+    const int begin = blockIdx.y * per + warp;
+    if (begin < last) load(begin, ahead);
+    __syncthreads();
+    for (int n = begin; n < last; n += 8) {
         const bool is_q = n < s.heads, is_v = n >= s.heads + s.kv_heads;
         const int head = is_q ? n : is_v ? n - s.heads - s.kv_heads : n - s.heads;
-        const void *src = is_q ? in.q : is_v ? in.v : in.k;
-        const size_t from = size_t(row) * (is_q ? in.q_ld : is_v ? in.v_ld : in.k_ld) + size_t(head) * hd + 2 * lane;
         uint16_t *dst = is_q ? q_out + (size_t(row) * s.heads + head) * hd : (is_v ? v_cache : k_cache) + place + size_t(head) * s.head_stride;
         const uint16_t *weight = is_q ? q_norm : is_v ? nullptr : k_norm;
         float2 x[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) if (64 * j < hd) x[j] = spl_load_pair<TYPE>(src, from + 64 * j);
+        for (int j = 0; j < 4; ++j) x[j] = ahead[j];
+        if (n + 8 < last) load(n + 8, ahead);
         if (weight) {
             float ss = 0.0f;
 #pragma unroll
             for (int j = 0; j < 4; ++j) if (64 * j < hd) ss += x[j].x * x[j].x + x[j].y * x[j].y;
-            const float inv = 1.0f / sqrtf(spl_warp_sum(ss) / float(hd) + eps);
+            const float inv = rsqrtf(spl_warp_sum(ss) / float(hd) + eps);
 #pragma unroll
             for (int j = 0; j < 4; ++j) if (64 * j < hd) {
                 const uint32_t w = *reinterpret_cast<const uint32_t *>(weight + 64 * j + 2 * lane);
