@@ -513,7 +513,10 @@ spl_sample_kernel(SplSampleArgs a) {
     if (step == SPL_SAMPLE_WEIGH) {
         for (int i = tid; i < SPL_SAMPLE_BINS; i += 1024) { sh.lo[i] = 0u; sh.hi[i] = 0u; }
         __syncthreads();
+        // Values that cannot count are passed over: without top-p nothing below min-p's bound is in any sum (a bin and the roundings of slack).
+        const float least_value = r.least && !(r.p < 1.0f) ? r.w.max - (-logf(r.m) + 4.0f / SPL_SAMPLE_BINS_NAT) * r.t - 1e-6f * fabsf(r.w.max) : -INFINITY;
         each([&](const float (&value)[4], int i, int step) {
+            if (!(value[0] >= least_value) & !(value[1] >= least_value) & !(value[2] >= least_value) & !(value[3] >= least_value)) return;
             // The four weights side by side (a weight is a chain of ten 64-bit operations), whatever of them counts.
             unsigned long long w[4];
             int b[4];
@@ -521,8 +524,8 @@ spl_sample_kernel(SplSampleArgs a) {
             for (int q = 0; q < 4; ++q) { b[q] = bin_of(value[q]); w[q] = spl_sample_weight_near(value[q], r.w); }
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                const uint32_t key = spl_topk_key(value[q]);
-                if (b[q] == SPL_SAMPLE_BINS - 1 || key == 0u || (cut && spl_sample_entry(key, uint32_t(i + q * step)) < cut)) continue;
+                if (!(value[q] > -INFINITY) || b[q] == SPL_SAMPLE_BINS - 1) continue;
+                if (cut && spl_sample_entry(spl_topk_key(value[q]), uint32_t(i + q * step)) < cut) continue;
                 if (r.w.max == INFINITY) { if (value[q] != r.w.max) continue; w[q] = 1ull << 44; }
                 // Two words a bin, the carry taken by whoever makes the lower one overflow.
                 const unsigned int low = unsigned(w[q]), was = atomicAdd(&sh.lo[b[q]], low), high = unsigned(w[q] >> 32) + (was + low < was ? 1u : 0u);
