@@ -357,12 +357,12 @@ spl_sample_kernel(SplSampleArgs a) {
                 f(value, begin + i, 1);
             }
         } else {
-#pragma unroll 2
-            for (int i = tid; i < count; i += 4096) {
-                float value[4];
+            for (int i = tid; i < count; i += 16384) {          // sixteen loads on their way
+                float value[4][4];
 #pragma unroll
-                for (int q = 0; q < 4; ++q) value[q] = i + q * 1024 < count ? mine[i + q * 1024] : -INFINITY;
-                f(value, begin + i, 1024);
+                for (int q = 0; q < 16; ++q) value[q / 4][q % 4] = i + q * 1024 < count ? mine[i + q * 1024] : -INFINITY;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) f(value[q], begin + i + q * 4096, 1024);
             }
         }
     };
