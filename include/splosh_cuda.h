@@ -445,12 +445,14 @@ void spl_paged_destroy(spl_paged *paged);
 spl_status spl_paged_batch(spl_paged *paged, int32_t sequences, const int32_t *rows, const int32_t *lengths, const int32_t *page_table, int32_t table_ld, void *stream);
 /* Rows of `type` (SPL_F32, SPL_F16, SPL_BF16) with row strides in elements (even; rows begin on a boundary of two elements): q [rows][heads][head_dim],
  * k and v [rows][kv_heads][head_dim]. q_norm and k_norm (spl_tensor_create_vector of head_dim, may be null): x * rsqrt(mean x^2 + eps) * weight
- * over a head's channels, before the rotation. q_out [rows][heads][head_dim] of the cache's type. A batch in which two sequences
+ * over a head's channels (the geometry's eps), before the rotation. q_out [rows][heads][head_dim] of the cache's type. A batch in which two sequences
  * would write to one page is refused. */
 spl_status spl_paged_append(spl_paged *paged, int32_t type, const void *device_q, int64_t q_ld, const void *device_k, int64_t k_ld, const void *device_v, int64_t v_ld,
                             const spl_tensor *q_norm, const spl_tensor *k_norm, void *device_q_out, void *device_k_cache, void *device_v_cache, void *stream);
 /* q [rows][heads][head_dim] of the cache's type; out the same shape, out_type SPL_F32 or the cache's type. Scores, softmax statistics and sums are fp32, a
- * probability is rounded to the cache's type before it meets the values. Buffers begin on 16-byte boundaries. */
+ * probability is rounded to the cache's type before it meets the values. Buffers begin on 16-byte boundaries. What the cache holds behind a sequence's last token,
+ * or in front of every row's window, may be anything. (Page table entries in front of a window still name pages of the cache.) A NaN or infinity among a token's
+ * values reaches the rows that see the token, and may reach earlier rows of the same chunk of that sequence. */
 spl_status spl_paged_attend(spl_paged *paged, const void *device_q, const void *device_k_cache, const void *device_v_cache, int32_t out_type, void *device_out, void *stream);
 /* What spl_paged_create and spl_paged_batch would say, without an engine or a GPU (sequences 0: the configuration alone); the reason in
  * `message`. *shared_write (may be null): append would refuse the batch. */

@@ -368,7 +368,7 @@ spl_sample_kernel(SplSampleArgs a) {
     };
     SplSampleRow r;
     r.t = a.temperature ? a.temperature[row] : 1.0f; r.p = a.top_p ? a.top_p[row] : 1.0f; r.u = a.uniform[row];
-    r.m = a.min_p ? fminf(a.min_p[row], 1.0f) : 0.0f; r.k = a.top_k ? a.top_k[row] : 0;
+    r.m = a.min_p && a.min_p[row] > 0.0f ? fminf(a.min_p[row], 1.0f) : 0.0f; r.k = a.top_k ? a.top_k[row] : 0;
     r.least = r.m > 0.0f ? (unsigned long long)ceil(double(r.m) * SPL_SAMPLE_UNIT) : 0ull;
 
     // The largest value and its lowest index.

@@ -86,17 +86,22 @@ class PagedAttention:
     def __del__(self):
         self.close()
 
+    def _handle(self):
+        if not self.handle or not self.engine.handle:
+            raise EngineError(10, "the engine or this object is closed")
+        return self.handle
+
     def batch(self, rows, lengths, page_table, stream=None):
         """The sequences of a pass: new tokens and length (with them) of each, and its pages (int32 [sequences][pages of the longest])."""
         rows, lengths, table = _batch(rows, lengths, page_table)
-        self.engine._check(lib().spl_paged_batch(self.handle, rows.shape[0], _ptr(rows), _ptr(lengths), _ptr(table), table.shape[1], stream_handle(stream)))
+        self.engine._check(lib().spl_paged_batch(self._handle(), rows.shape[0], _ptr(rows), _ptr(lengths), _ptr(table), table.shape[1], stream_handle(stream)))
 
     def append(self, q, k, v, q_out, k_cache, v_cache, dtype="f32", ld=None, q_norm=None, k_norm=None, stream=None):
         """Rows of `dtype` at the addresses q, k, v (row stride `ld` elements for all three, or a triple; None: each contiguous) -> rotated queries at q_out,
         keys and values in the cache. q_norm and k_norm are tensors of Engine.tensor_vector."""
         q_ld, k_ld, v_ld = (self.q_width, self.kv_width, self.kv_width) if ld is None else (ld,) * 3 if np.isscalar(ld) else ld
-        self.engine._check(lib().spl_paged_append(self.handle, _type(dtype), q, q_ld, k, k_ld, v, v_ld, q_norm, k_norm, q_out, k_cache, v_cache, stream_handle(stream)))
+        self.engine._check(lib().spl_paged_append(self._handle(), _type(dtype), q, q_ld, k, k_ld, v, v_ld, q_norm, k_norm, q_out, k_cache, v_cache, stream_handle(stream)))
 
     def attend(self, q, k_cache, v_cache, out, out_dtype=None, stream=None):
         """The batch's rows over the cache: q and out [rows][heads][head_dim], out of the cache's type or "f32"."""
-        self.engine._check(lib().spl_paged_attend(self.handle, q, k_cache, v_cache, _type(out_dtype or self.dtype), out, stream_handle(stream)))
+        self.engine._check(lib().spl_paged_attend(self._handle(), q, k_cache, v_cache, _type(out_dtype or self.dtype), out, stream_handle(stream)))
