@@ -78,7 +78,7 @@ struct __align__(128) SplSampleShared {
     double powers[64];                                          // 2^(j / 64)
     unsigned int listed, found;
     // The first block's decision, in every block: which bins to set aside, or what has been decided.
-    int step, first_bin, last_bin, also_bin;
+    int step, first_bin, last_bin, also_first, also_last;
     unsigned long long cut;
 };
 enum { SPL_SAMPLE_DONE = 0, SPL_SAMPLE_FINISH, SPL_SAMPLE_CUT, SPL_SAMPLE_END, SPL_SAMPLE_DRAW, SPL_SAMPLE_WEIGH, SPL_SAMPLE_SLOW };
@@ -415,24 +415,24 @@ spl_sample_kernel(SplSampleArgs a) {
     r.w.powers = sh.powers;
     r.bin_scale = fminf(2.0f * SPL_SAMPLE_BINS_NAT / r.t, 3.0e38f);
     // The bin of a value that may be picked: halved values do not overflow, and rounding keeps the order (it may put a value in the next bin, no more). Beside an
-    // infinite maximum the finite values are binned as beside the largest one (they have no weight).
+    // infinite maximum the finite values are binned as beside the largest one (they have no weight), and the infinite ones come to bin 0 by way of -inf.
     const float half_max = 0.5f * fminf(r.w.max, 3.402823466e38f);
     auto bin_of = [&](float value) {
-        return __float_as_int(fminf(fmaxf(fmaf(-0.5f, value, half_max) * r.bin_scale, 0.0f), float(SPL_SAMPLE_BINS - 1)) + 8388608.0f) & (SPL_SAMPLE_BINS - 1);
+        return __float_as_int(fminf(fmaf(-0.5f, value, half_max) * r.bin_scale, float(SPL_SAMPLE_BINS - 1)) + 8388608.0f) & (SPL_SAMPLE_BINS - 1);
     };
     unsigned long long cut = 0ull;                     // entries below it are out
-    // The values of the bins [first, last] and of bin `also` (in front of them, or negative) into the block's list.
-    auto set_aside = [&](int first, int last, int also) {
+    // The values of the bins [first, last] and [also_first, also_last] (in front of them; none where also_first is negative) into the block's list.
+    auto set_aside = [&](int first, int last, int also_first, int also_last) {
         // Most values are told by comparisons: bounds a bin and the roundings outside the bins asked for.
         const float width = r.t / SPL_SAMPLE_BINS_NAT, slack = 2.0f * width + 1e-6f * fabsf(r.w.max);
         auto top_of = [&](int b) { return r.w.max - float(b) * width + slack; };
         auto bottom_of = [&](int b) { return b == SPL_SAMPLE_BINS - 1 ? -INFINITY : r.w.max - float(b + 1) * width - slack; };
-        const float high = top_of(first), low = bottom_of(last), also_high = also < 0 ? -INFINITY : top_of(also), also_low = also < 0 ? INFINITY : bottom_of(also);
+        const float high = top_of(first), low = bottom_of(last), also_high = also_first < 0 ? -INFINITY : top_of(also_first), also_low = also_first < 0 ? INFINITY : bottom_of(also_last);
         auto near = [&](float value) { return !(value > high || value < low) || !(value > also_high || value < also_low); };
         auto keep = [&](float value, int i) {
             const uint32_t key = spl_topk_key(value);
             const int b = bin_of(value);
-            if (key == 0u || ((b < first || b > last) && b != also)) return;
+            if (key == 0u || ((b < first || b > last) && (also_first < 0 || b < also_first || b > also_last))) return;
             const unsigned long long entry = spl_sample_entry(key, uint32_t(i));
             if (entry < cut) return;
             const unsigned int at = atomicAdd(&sh.listed, 1u);
@@ -446,11 +446,11 @@ spl_sample_kernel(SplSampleArgs a) {
         cluster.sync();
     };
     // The first block's decision goes to all of them; what their lists held has been read.
-    auto decide = [&](int step, int first_bin, int last_bin, unsigned long long new_cut, int also_bin = -1) {
+    auto decide = [&](int step, int first_bin, int last_bin, unsigned long long new_cut, int also_first = -1, int also_last = -1) {
         __syncthreads();
         if (tid < blocks) {
             SplSampleShared *peer = cluster.map_shared_rank(&sh, tid);
-            peer->step = step; peer->first_bin = first_bin; peer->last_bin = last_bin; peer->also_bin = also_bin; peer->cut = new_cut; peer->listed = 0u;
+            peer->step = step; peer->first_bin = first_bin; peer->last_bin = last_bin; peer->also_first = also_first; peer->also_last = also_last; peer->cut = new_cut; peer->listed = 0u;
         }
     };
     int step = SPL_SAMPLE_WEIGH;
@@ -482,7 +482,7 @@ spl_sample_kernel(SplSampleArgs a) {
         cluster.sync();
         step = sh.step;
         if (step != SPL_SAMPLE_WEIGH) {
-            set_aside(sh.first_bin, sh.last_bin, -1);
+            set_aside(sh.first_bin, sh.last_bin, -1, -1);
             if (rank == 0) {
                 const int n = spl_sample_sorted(sh, cluster, blocks, r, 0ull);
                 if (n < 0) decide(SPL_SAMPLE_SLOW, 0, 0, 0ull);
@@ -536,7 +536,7 @@ spl_sample_kernel(SplSampleArgs a) {
         spl_sample_add_blocks(sh, cluster, rank, blocks);
         cluster.sync();
         // The first block: what stays ends in the bins [c0, c1], or nowhere before the last value.
-        int c0 = SPL_SAMPLE_BINS, c1 = -1, p_bin = SPL_SAMPLE_BINS, also = -1;
+        int c0 = SPL_SAMPLE_BINS, c1 = -1, p_bin = SPL_SAMPLE_BINS, also = -1, also_last = -1;
         unsigned long long p_target = 0ull, all = 0ull;
         if (rank == 0) {
             spl_sample_running(sh, &all);
@@ -552,11 +552,12 @@ spl_sample_kernel(SplSampleArgs a) {
                 else if (p_bin >= m0) { c0 = m0; c1 = m1; }
             }
             if (c1 >= 0) {
-                // Whatever of the bins [c0, c1] stays, the draw mostly lies in one and the same bin: set aside with them, it is found in the same list.
+                // Whatever of the bins [c0, c1] stays, the draw mostly lies in one and the same bin, or one of a few: set aside with them, it is found in the same list. (With one bin
+                // alone a fifth of the rows of a vocabulary of 248,077 needed another turn.)
                 const unsigned long long least_sum = c0 ? sh.sums[c0 - 1] : 0ull;
                 const int d0 = spl_sample_place(sh, SPL_SAMPLE_BINS, spl_sample_target(r.u, least_sum)), d1 = spl_sample_place(sh, SPL_SAMPLE_BINS, spl_sample_target(r.u, sh.sums[c1]));
-                if (d0 == d1 && d1 < c0) also = d1;
-                decide(SPL_SAMPLE_END, c0, c1, cut, also);
+                if (d0 < c0 && min(d1, c0 - 1) - d0 < 8) { also = d0; also_last = min(d1, c0 - 1); }
+                decide(SPL_SAMPLE_END, c0, c1, cut, also, also_last);
             } else {
                 const int b = spl_sample_place(sh, SPL_SAMPLE_BINS, spl_sample_target(r.u, all));
                 decide(SPL_SAMPLE_DRAW, b, b, cut);
@@ -567,10 +568,10 @@ spl_sample_kernel(SplSampleArgs a) {
         const unsigned long long *kept = reinterpret_cast<const unsigned long long *>(sh.lo);
         unsigned long long target = rank == 0 && step == SPL_SAMPLE_DRAW ? spl_sample_target(r.u, all) : 0ull;
         if (step == SPL_SAMPLE_END) {
-            set_aside(sh.first_bin, sh.last_bin, sh.also_bin);
+            set_aside(sh.first_bin, sh.last_bin, sh.also_first, sh.also_last);
             if (rank == 0) {
-                // The list: the draw's bin where it came along (entries [0, front)), then the bins what stays ends in, running sums from `base`.
-                const unsigned long long base = c0 ? kept[c0 - 1] : 0ull, also_base = also > 0 ? kept[also - 1] : 0ull, also_sum = also < 0 ? 0ull : kept[also] - also_base;
+                // The list: the draw's bins where they came along (entries [0, front)), then the bins what stays ends in, running sums from `base`.
+                const unsigned long long base = c0 ? kept[c0 - 1] : 0ull, also_base = also > 0 ? kept[also - 1] : 0ull, also_sum = also < 0 ? 0ull : kept[also_last] - also_base;
                 const int n = spl_sample_sorted(sh, cluster, blocks, r, base - also_sum);
                 if (n < 0) decide(SPL_SAMPLE_SLOW, 0, 0, 0ull);
                 else {
@@ -580,7 +581,7 @@ spl_sample_kernel(SplSampleArgs a) {
                         if (tid == 0) sh.found = unsigned(n);
                         __syncthreads();
                         for (int i = tid; i < n; i += 1024) {
-                            auto in_front = [&](int e) { return bin_of(spl_topk_value(uint32_t(sh.list[e] >> 32))) == also; };
+                            auto in_front = [&](int e) { return bin_of(spl_topk_value(uint32_t(sh.list[e] >> 32))) <= also_last; };
                             if (!in_front(i) && (i == 0 || in_front(i - 1))) sh.found = unsigned(i);
                         }
                         __syncthreads();
@@ -631,7 +632,7 @@ spl_sample_kernel(SplSampleArgs a) {
         }
         if (step == SPL_SAMPLE_DRAW) {
             const int b = sh.first_bin;
-            set_aside(b, b, -1);
+            set_aside(b, b, -1, -1);
             if (rank == 0) {
                 const int n = spl_sample_sorted(sh, cluster, blocks, r, b ? kept[b - 1] : 0ull);
                 if (n < 0) decide(SPL_SAMPLE_SLOW, 0, 0, 0ull);
