@@ -145,8 +145,8 @@ spl_paged_append_kernel(SplPagedRows in, const uint16_t *__restrict__ q_norm, co
 // An instruction of the value product spans all HD columns of O: with values in chunks of 64 channels it took HD / 64 times as many instructions of 64 columns, and the
 // issuing warp (some 100 cycles an instruction) was the block's pace: 5,000 of 6,450 cycles a tile at HD = 256.
 //
-// Warps 0-7 softmax (thread: a row and half of the tile's tokens; the pair of warps of 32 rows agrees on the maximum), warp 8 copies, warps 9 and
-// 10 issue the products: S of tile i + 1 runs under the softmax of tile i. The reference is raised only when a row's maximum exceeds it by 2^8, so the sums in
+// Warps 0-7 softmax (thread: a row and half of the tile's tokens; the pair of warps of 32 rows agrees on the maximum), warps 8 and 11 copy (a chunk is
+// some 800 cycles of waiting and asking: with one warp for both that was the block's pace at HD = 256), warps 9 and 10 issue the products: S of tile i + 1 runs under the softmax of tile i. The reference is raised only when a row's maximum exceeds it by 2^8, so the sums in
 // tensor memory are rescaled a few times a piece, not every tile. Rows that are not there cost no softmax work.
 // Tensor memory: S / P two buffers of 128 columns (P, 16 bits, over the S it came from), O HD columns from 256. (At HD = 128 there is room for P beside S: with the next tile's
 // scores loaded under a tile's exponentials 2,048 rows over 8,192 tokens of 32/8 heads took 303 us instead of 264, with two groups of four warps taking turns at the tiles 282.)
@@ -156,11 +156,11 @@ spl_paged_append_kernel(SplPagedRows in, const uint16_t *__restrict__ q_norm, co
 //
 // What is masked may be anything: a masked score is replaced before it is used, and because 0 x inf is no number, tokens that no row of the piece
 // sees (behind the sequence's last token, in front of the window) have their values zeroed in shared memory or are left out of the product.
-#define SPL_PAGED_THREADS 352
+#define SPL_PAGED_THREADS 384
 #define SPL_PAGED_HEADROOM 8.0f
 __host__ __device__ constexpr int spl_paged_chunk(int hd) { return hd == 64 ? 16384 : 32768; }
 __host__ __device__ constexpr int spl_paged_ring_k(int hd) { return hd == 64 ? 6 : 3; }
-__host__ __device__ constexpr int spl_paged_ring_v(int hd) { return hd == 64 ? 6 : 2; }
+__host__ __device__ constexpr int spl_paged_ring_v(int hd) { return hd == 64 ? 6 : hd == 128 ? 3 : 2; }
 __host__ __device__ constexpr int spl_paged_ring(int hd) { return spl_paged_ring_k(hd) + spl_paged_ring_v(hd); }
 __host__ __device__ constexpr size_t spl_paged_smem_bytes(int hd) {
     return size_t(hd) * 256 + size_t(spl_paged_ring(hd)) * spl_paged_chunk(hd) + 2 * 2 * 128 * 4 /* maxima, sums */ + 512 /* barriers */;
@@ -402,55 +402,52 @@ spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
     bool ok = true;
     auto gave_up = [&](int code) { ok = false; if (!*abort && lane == 0) { spl_note_wait(a.error_flag, code, 0); a.error_flag[0] = 200 + warp; } *abort = 1; };
 
-    if (warp == 8) {
-        // ---- copies. Lane b brings the tile's b-th page (or its half of a page of 256); a chunk's barrier counts the pages that hold tokens.
+    if (warp == 8 || warp == 11) {
+        // ---- copies, keys (warp 8) and values (warp 11). Lane b holds the page of the tile's b-th box of tokens (a page, or half a page of 256); a chunk's barrier counts the boxes that hold tokens.
         const int box = min(s.page_tokens, 128), boxes = 128 / box;
-        int nk = 0, nv = 0;                                   // chunks so far
-        auto room = [&](uint64_t *empty, int n, int slots) {
-            if (ok && !spl_mbar_wait_warp(&empty[n % slots], ((n / slots) & 1) ^ 1, const_cast<const int *>(abort))) gave_up(60);
+        const bool keys = warp == 8;
+        uint64_t *full = keys ? full_k : full_v, *empty = keys ? empty_k : empty_v;
+        const int slots = keys ? NK : NV;
+        int n = 0, st = 0;                                    // chunks so far, and the next one's place
+        auto room = [&]() {
+            if (ok && !spl_mbar_wait_warp(&empty[st], ((n / slots) & 1) ^ 1, const_cast<const int *>(abort))) gave_up(60);
             return ok;
         };
-        // Lane b holds the page of the tile's b-th box of tokens; `present` of them hold tokens. inside: where a tile begins in a page of 256.
-        auto bring_k = [&](const SplPagedItem &it, int inside, int page, int present) {
-            const int block = lane / boxes, b = lane % boxes, from = __shfl_sync(0xffffffffu, page, b);      // a lane a box of 64 channels by a page's tokens
-            for (int c = 0; c < PARTS; ++c, ++nk) {
-                if (!room(empty_k, nk, NK)) return;
-                const int st = nk % NK;
-                if (lane == 0) spl_mbar_expect_tx(&full_k[st], uint32_t(present * box) * 128 * KB);
-                __syncwarp();
-                if (block < KB && b < present) spl_tma_load4(ring + st * CHUNK + block * 16384 + b * box * 128, &k_map, (c * KB + block) * 64, inside, it.kv_head, from, &full_k[st]);
-            }
-        };
-        const int vbox = min(s.page_tokens, VT), vboxes = VT / vbox, per_page = box / vbox;      // boxes a chunk of values, boxes a lane's page
-        auto bring_v = [&](const SplPagedItem &it, int inside, int page, int tokens) {
-            for (int c = 0; c < PARTS; ++c, ++nv) {
-                if (!room(empty_v, nv, NV)) return;
-                const int st = nv % NV, b = c * vboxes + lane;                                  // lane's box of the tile
-                const int there = min(vboxes, max(0, (tokens - c * VT + vbox - 1) / vbox)), from = __shfl_sync(0xffffffffu, page, lane < vboxes ? b / per_page : 0);
-                if (lane == 0) spl_mbar_expect_tx(&full_v[st], uint32_t(there) * vbox * HD * 2);
-                __syncwarp();
-                if (lane < there) spl_tma_load5(v_ring + st * CHUNK + lane * vbox * HD * 2, &v_map, 0, inside + b % per_page * vbox, 0, it.kv_head, from, &full_v[st]);
-            }
-        };
+        const int block = lane / boxes, b = lane % boxes;                                       // keys: a lane a box of 64 channels by a page's tokens
+        const int vbox = min(s.page_tokens, VT), vboxes = VT / vbox, per_page = box / vbox;      // values: boxes a chunk, boxes a lane's page
         for (int i = item0; i < item1 && ok; ++i) {
             const SplPagedItem it = item_at(i);
             const int length = it.length;
             const int *pages = t.table + size_t(it.sequence) * s.max_pages;
-            auto present_of = [&](int tile) { return min(boxes, (length - tile * 128 + box - 1) / box); };
-            auto page_of = [&](int tile) { return tile < it.tile_end && lane < present_of(tile) ? pages[s.page_tokens > 128 ? tile >> 1 : tile * boxes + lane] : 0; };
-            auto inside_of = [&](int tile) { return s.page_tokens > 128 ? (tile & 1) * 128 : 0; };
-            int page = page_of(it.tile_begin), ahead = page_of(it.tile_begin + 1);
-            bring_k(it, inside_of(it.tile_begin), page, present_of(it.tile_begin));
+            auto page_of = [&](int tile) {
+                return tile < it.tile_end && lane < min(boxes, (length - tile * 128 + box - 1) / box) ? pages[s.page_tokens > 128 ? tile >> 1 : tile * boxes + lane] : 0;
+            };
+            int page = page_of(it.tile_begin);
             for (int tile = it.tile_begin; tile < it.tile_end && ok; ++tile) {
-                const int later = page_of(tile + 2);
-                if (tile + 1 < it.tile_end) bring_k(it, inside_of(tile + 1), ahead, present_of(tile + 1));
-                if (ok) bring_v(it, inside_of(tile), page, min(128, length - tile * 128));
-                page = ahead; ahead = later;
+                const int ahead = page_of(tile + 1), inside = s.page_tokens > 128 ? (tile & 1) * 128 : 0, tokens = min(128, length - tile * 128);
+                if (keys) {
+                    const int present = (tokens + box - 1) / box, from = __shfl_sync(0xffffffffu, page, b);
+                    for (int c = 0; c < PARTS && room(); ++c) {
+                        if (lane == 0) spl_mbar_expect_tx(&full[st], uint32_t(present * box) * 128 * KB);
+                        __syncwarp();
+                        if (block < KB && b < present) spl_tma_load4(ring + st * CHUNK + block * 16384 + b * box * 128, &k_map, (c * KB + block) * 64, inside, it.kv_head, from, &full[st]);
+                        ++n; st = st + 1 == slots ? 0 : st + 1;
+                    }
+                } else {
+                    for (int c = 0; c < PARTS && room(); ++c) {
+                        const int v = c * vboxes + lane;                                        // lane's box of the tile
+                        const int there = min(vboxes, max(0, (tokens - c * VT + vbox - 1) / vbox)), from = __shfl_sync(0xffffffffu, page, lane < vboxes ? v / per_page : 0);
+                        if (lane == 0) spl_mbar_expect_tx(&full[st], uint32_t(there) * vbox * HD * 2);
+                        __syncwarp();
+                        if (lane < there) spl_tma_load5(v_ring + st * CHUNK + lane * vbox * HD * 2, &v_map, 0, inside + v % per_page * vbox, 0, it.kv_head, from, &full[st]);
+                        ++n; st = st + 1 == slots ? 0 : st + 1;
+                    }
+                }
+                page = ahead;
             }
         }
         // Nothing may still be on its way into the block's shared memory when it is handed on.
-        for (int st = 0; st < NK && st < nk; ++st) spl_mbar_wait(&full_k[st], ((st + (nk - 1 - st) / NK * NK) / NK) & 1);
-        for (int st = 0; st < NV && st < nv; ++st) spl_mbar_wait(&full_v[st], ((st + (nv - 1 - st) / NV * NV) / NV) & 1);
+        for (int z = 0; z < slots && z < n; ++z) spl_mbar_wait(&full[z], ((z + (n - 1 - z) / slots * slots) / slots) & 1);
     } else if (warp == 9 || warp == 10) {
         // ---- the products, a warp each (a wait is 110 cycles even when it is over: in one warp six a tile were a third of its time), issued by one elected lane of
         // a converged warp.
@@ -528,7 +525,7 @@ spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
         // No product may still read shared or write tensor memory when they are handed on.
         spl_tc_commit_if(elected, &drained[first_product ? 0 : 1]);
         spl_mbar_wait(&drained[first_product ? 0 : 1], 0);
-    } else {
+    } else if (warp < 8) {
         // ---- softmax: row r of the piece, tokens [64 half, 64 half + 64) of a tile.
         const int quarter = warp & 3, half = warp >> 2, r = quarter * 32 + lane;
         const uint32_t lanes = uint32_t(quarter * 32) << 16;
