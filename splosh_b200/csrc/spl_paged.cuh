@@ -206,10 +206,6 @@ __device__ __forceinline__ uint64_t spl_tc_desc_mn_sw128(uint32_t smem_byte_addr
     return (spl_tc_desc_sw128(smem_byte_addr) & ~(uint64_t(0x3FFF) << 16)) | uint64_t(block_bytes >> 4) << 16;
 }
 // A box of a tensor map into shared memory; the innermost coordinate is a multiple of 64 elements.
-__device__ __forceinline__ void spl_tma_load4(void *smem, const CUtensorMap *map, int x, int token, int head, int page, uint64_t *bar) {
-    asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];\n"
-                 ::"r"(spl_smem_addr(smem)), "l"(map), "r"(x), "r"(token), "r"(head), "r"(page), "r"(spl_smem_addr(bar)) : "memory");
-}
 // The two warps of 32 rows (w and w + 4): barriers 1 to 4.
 __device__ __forceinline__ void spl_paged_pair_barrier(int quarter) {
     if (quarter == 0) spl_named_barrier<1, 64>();
@@ -413,7 +409,7 @@ spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
             if (ok && !spl_mbar_wait_warp(&empty[st], ((n / slots) & 1) ^ 1, const_cast<const int *>(abort))) gave_up(60);
             return ok;
         };
-        const int block = lane / boxes, b = lane % boxes;                                       // keys: a lane a box of 64 channels by a page's tokens
+        const int whole = boxes == 1 ? KB : 1, block = boxes == 1 ? lane * KB : lane / boxes, b = lane % boxes;      // keys: a lane a box of a page's tokens by 64 channels, or by the chunk's where that is a tile's tokens
         const int vbox = min(s.page_tokens, VT), vboxes = VT / vbox, per_page = box / vbox;      // values: boxes a chunk, boxes a lane's page
         for (int i = item0; i < item1 && ok; ++i) {
             const SplPagedItem it = item_at(i);
@@ -430,7 +426,7 @@ spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
                     for (int c = 0; c < PARTS && room(); ++c) {
                         if (lane == 0) spl_mbar_expect_tx(&full[st], uint32_t(present * box) * 128 * KB);
                         __syncwarp();
-                        if (block < KB && b < present) spl_tma_load4(ring + st * CHUNK + block * 16384 + b * box * 128, &k_map, (c * KB + block) * 64, inside, it.kv_head, from, &full[st]);
+                        if (block + whole <= KB && b < present) spl_tma_load5(ring + st * CHUNK + block * 16384 + b * box * 128, &k_map, 0, inside, c * KB + block, it.kv_head, from, &full[st]);
                         ++n; st = st + 1 == slots ? 0 : st + 1;
                     }
                 } else {

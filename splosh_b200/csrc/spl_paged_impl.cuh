@@ -151,23 +151,17 @@ template <int TYPE> static void launch_append(const spl_paged *p, const SplPaged
         launch_step(spl_paged_append_kernel<TYPE, false>, grid, dim3(256), 0, stream, in, q_norm, k_norm, (const double *)p->turns, p->tables(), p->shape, p->e->g.eps, q, k, v);
 }
 
-// The cache as a tensor for the copies of keys, (channel, token in page, kv head, page) in boxes of 64 channels by a page's tokens (at most a tile's), or of values,
-// (channel in block, token in page, block of 64 channels, kv head, page) in boxes of all channels by a page's tokens (at most a chunk's).
+// The cache as a tensor (channel in block, token in page, block of 64 channels, kv head, page) for the copies of values, in boxes of all channels by a page's tokens (at most a
+// chunk's), or of keys: of a page's tokens (at most a tile's) by 64 channels, or by a chunk's where the box is a tile's tokens.
 static bool paged_map(const spl_paged *p, const void *cache, bool values, CUtensorMap *map) {
     const spl_paged_config &c = p->c;
-    const cuuint64_t d = cuuint64_t(c.head_dim), tokens = cuuint64_t(c.page_tokens), heads = cuuint64_t(c.kv_heads), pages = cuuint64_t(c.pages);
-    const cuuint64_t ts = cuuint64_t(c.token_stride) * 2, hs = cuuint64_t(c.head_stride) * 2, ps = cuuint64_t(c.page_stride) * 2;
-    const CUtensorMapDataType type = c.dtype == SPL_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-    const cuuint32_t steps[5] = {1, 1, 1, 1, 1};
-    void *base = const_cast<void *>(cache);
-    if (values) {
-        const cuuint64_t dims[5] = {64, tokens, d / 64, heads, pages}, strides[4] = {ts, 128, hs, ps};
-        const cuuint32_t box[5] = {64, cuuint32_t(std::min(c.page_tokens, spl_paged_chunk(c.head_dim) / (2 * c.head_dim))), cuuint32_t(d / 64), 1, 1};
-        return p->encode(map, type, 5, base, dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-    }
-    const cuuint64_t dims[4] = {d, tokens, heads, pages}, strides[3] = {ts, hs, ps};
-    const cuuint32_t box[4] = {64, cuuint32_t(std::min(c.page_tokens, SPL_PAGED_TILE)), 1, 1};
-    return p->encode(map, type, 4, base, dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    const cuuint64_t d = cuuint64_t(c.head_dim), dims[5] = {64, cuuint64_t(c.page_tokens), d / 64, cuuint64_t(c.kv_heads), cuuint64_t(c.pages)};
+    const cuuint64_t strides[4] = {cuuint64_t(c.token_stride) * 2, 128, cuuint64_t(c.head_stride) * 2, cuuint64_t(c.page_stride) * 2};
+    const int chunk = spl_paged_chunk(c.head_dim), tokens = std::min(c.page_tokens, values ? chunk / (2 * c.head_dim) : SPL_PAGED_TILE);
+    const cuuint32_t blocks = values ? cuuint32_t(d / 64) : tokens == SPL_PAGED_TILE ? cuuint32_t(chunk / 16384) : 1u;
+    const cuuint32_t box[5] = {64, cuuint32_t(tokens), blocks, 1, 1}, steps[5] = {1, 1, 1, 1, 1};
+    return p->encode(map, c.dtype == SPL_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, const_cast<void *>(cache), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <int HD, bool BF16> static void launch_attend(const spl_paged *p, const CUtensorMap &k_map, const CUtensorMap &v_map, const SplPagedAttend &a, cudaStream_t stream) {
