@@ -50,84 +50,102 @@ template <int TYPE> __device__ __forceinline__ float2 spl_load_pair(const void *
 // by the angle position * theta^(-2i / rotary); queries to their rows, keys and values to their place in the cache, all rounded once to
 // 16 bits. The angle is formed in 64 bits as turns (position * theta^(-2i/rotary) / 2 pi): at position 200,000 a 32-bit product is
 // off by 6e-3 of a radian, a 64-bit one by 1e-11; what is left of the whole turns fits 32 bits.
-// Grid (rows, head ranges), 256 threads: the angles' sines and cosines once a block, then a warp a head, the next head's channels on their way. Bound: the instructions of a head (some
-// 300; half the issue slots), then HBM: 2,048 rows of 24/4 heads of 256 (101 MB) 24 us at 48 registers, 29 without the loads ahead. With weights and angles in registers (250 instructions, but
-// three blocks an SM instead of five) 29, blocks that stay for several rows 27.
+// Grid (rows, head ranges), 256 threads: the angles' sines and cosines once a block, then a warp a head, a lane the channels 64 j + 2 lane and the next, the next head's on their way.
+// A channel's partner is in another register or lane where rotary / 2 is a power of two from 2 on, else it comes by way of shared memory. Bound: the instructions of a head, then HBM: 2,048
+// rows of 24/4 heads of 256 (101 MB) took 25 us at 320 instructions a head, 21 at 250, a block's start among them.
 struct SplPagedRows { const void *q, *k, *v; long long q_ld, k_ld, v_ld; };
 
-template <int TYPE, bool BF16>
+template <int TYPE, bool BF16, int HD>
 __global__ void __launch_bounds__(256, 5)
 spl_paged_append_kernel(SplPagedRows in, const uint16_t *__restrict__ q_norm, const uint16_t *__restrict__ k_norm, const double *__restrict__ turns,
                         SplPagedTables t, SplPagedShape s, float eps, uint16_t *q_out, uint16_t *k_cache, uint16_t *v_cache) {
-    __shared__ float2 turn[128];                 // (cos, sin) of channel pair i
-    __shared__ float2 vector[8][128];
+    constexpr int J = HD / 64, SIZE = TYPE == 0 ? 4 : 2;
+    __shared__ __align__(16) float2 turn[128];   // (cos, sin) of channel pair i
+    __shared__ float2 vector[8][32 * J];
     spl_grid_begin();
-    const int row = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int half = s.rotary / 2, hd = s.head_dim, vectors = s.heads + 2 * s.kv_heads;
-    if (row >= t.counts[0]) return;
-    const int sequence = t.row_sequence[row], position = t.row_position[row];
+    const int row = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = s.rotary / 2, vectors = s.heads + 2 * s.kv_heads;
+    const int rows = t.counts[0], sequence = t.row_sequence[row], position = t.row_position[row];
+    if (row >= rows) return;
+    const int per = (vectors + gridDim.y - 1) / gridDim.y, begin = blockIdx.y * per + warp, last = min(vectors, int(blockIdx.y + 1) * per);
+    // Where head n of the row's queries, keys and values begins, for this lane.
+    const char *q_from = static_cast<const char *>(in.q) + (size_t(row) * in.q_ld + 2 * lane) * SIZE, *k_from = static_cast<const char *>(in.k) + (size_t(row) * in.k_ld + 2 * lane) * SIZE,
+               *v_from = static_cast<const char *>(in.v) + (size_t(row) * in.v_ld + 2 * lane) * SIZE;
+    auto load = [&](int n, float2 (&x)[J]) {
+        const int k = n - s.heads, v = k - s.kv_heads;
+        const char *from = k < 0 ? q_from + n * (HD * SIZE) : v < 0 ? k_from + k * (HD * SIZE) : v_from + v * (HD * SIZE);
+#pragma unroll
+        for (int j = 0; j < J; ++j) x[j] = spl_load_pair<TYPE>(from, 64 * j);
+    };
+    float2 ahead[J];
+    if (begin < last) load(begin, ahead);
+    const int page = t.table[size_t(sequence) * s.max_pages + position / s.page_tokens];
     if (threadIdx.x < half) {
         const double a = double(position) * turns[threadIdx.x];
         float sn, cs;
         sincospif(2.0f * float(a - rint(a)), &sn, &cs);
         turn[threadIdx.x] = make_float2(cs, sn);
     }
-    const int page = t.table[size_t(sequence) * s.max_pages + position / s.page_tokens];
-    const size_t place = size_t(page) * s.page_stride + size_t(position % s.page_tokens) * s.token_stride;
-    float *mine = reinterpret_cast<float *>(vector[warp]);
-    const int per = (vectors + gridDim.y - 1) / gridDim.y, last = min(vectors, int(blockIdx.y + 1) * per);
-    // A head's channels 64 j + 2 lane and the next; the next head's are on their way meanwhile.
-    auto load = [&](int n, float2 (&x)[4]) {
-        const bool is_q = n < s.heads, is_v = n >= s.heads + s.kv_heads;
-        const void *src = is_q ? in.q : is_v ? in.v : in.k;
-        const size_t from = size_t(row) * (is_q ? in.q_ld : is_v ? in.v_ld : in.k_ld) + size_t(is_q ? n : is_v ? n - s.heads - s.kv_heads : n - s.heads) * hd + 2 * lane;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) if (64 * j < hd) x[j] = spl_load_pair<TYPE>(src, from + 64 * j);
-    };
-    float2 ahead[4];
-    const int begin = blockIdx.y * per + warp;
-    if (begin < last) load(begin, ahead);
     __syncthreads();
+    const bool square = (half & (half - 1)) == 0 && half > 1;
+    const size_t place = size_t(page) * s.page_stride + size_t(position % s.page_tokens) * s.token_stride + 2 * lane;
+    uint16_t *q_to = q_out + size_t(row) * s.heads * HD + 2 * lane, *k_to = k_cache + place, *v_to = v_cache + place;
+    const uint16_t *held = nullptr;              // the weight in registers: a warp's queries come first, then its keys
+    float2 w[J];
     for (int n = begin; n < last; n += 8) {
-        const bool is_q = n < s.heads, is_v = n >= s.heads + s.kv_heads;
-        const int head = is_q ? n : is_v ? n - s.heads - s.kv_heads : n - s.heads;
-        uint16_t *dst = is_q ? q_out + (size_t(row) * s.heads + head) * hd : (is_v ? v_cache : k_cache) + place + size_t(head) * s.head_stride;
-        const uint16_t *weight = is_q ? q_norm : is_v ? nullptr : k_norm;
-        float2 x[4];
+        const int k = n - s.heads, v = k - s.kv_heads;
+        uint16_t *dst = k < 0 ? q_to + n * HD : v < 0 ? k_to + size_t(k) * s.head_stride : v_to + size_t(v) * s.head_stride;
+        float2 x[J];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = ahead[j];
+        for (int j = 0; j < J; ++j) x[j] = ahead[j];
         if (n + 8 < last) load(n + 8, ahead);
+        const uint16_t *weight = k < 0 ? q_norm : v < 0 ? k_norm : nullptr;
         if (weight) {
-            float ss = 0.0f;
+            if (weight != held) {
+                held = weight;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) if (64 * j < hd) ss += x[j].x * x[j].x + x[j].y * x[j].y;
-            const float inv = rsqrtf(spl_warp_sum(ss) / float(hd) + eps);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) if (64 * j < hd) {
-                const uint32_t w = *reinterpret_cast<const uint32_t *>(weight + 64 * j + 2 * lane);
-                x[j].x = x[j].x * inv * __uint_as_float(w << 16); x[j].y = x[j].y * inv * __uint_as_float(w & 0xffff0000u);
+                for (int j = 0; j < J; ++j) w[j] = spl_unpack16<true>(*reinterpret_cast<const uint32_t *>(weight + 64 * j + 2 * lane));
             }
+            float2 ss = make_float2(0.0f, 0.0f);
+#pragma unroll
+            for (int j = 0; j < J; ++j) ss = spl_fma2(x[j], x[j], ss);
+            const float inv = rsqrtf(spl_warp_sum(ss.x + ss.y) * (1.0f / HD) + eps);
+#pragma unroll
+            for (int j = 0; j < J; ++j) x[j] = spl_mul2(spl_mul2(x[j], make_float2(inv, inv)), w[j]);
         }
-        if (!is_v && half) {
-            __syncwarp();
+        if (v < 0 && half) {
+            if (square) {
+                float2 other[J];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) if (64 * j < s.rotary) vector[warp][32 * j + lane] = x[j];
-            __syncwarp();
+                for (int j = 0; j < J; ++j) {
+                    if (half >= 64) other[j] = half == 64 ? x[j ^ (J > 1 ? 1 : 0)] : x[j ^ (J > 2 ? 2 : 0)];
+                    else if (64 * j < s.rotary) other[j] = make_float2(__shfl_xor_sync(0xffffffffu, x[j].x, half / 2), __shfl_xor_sync(0xffffffffu, x[j].y, half / 2));
+                }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) if (64 * j < s.rotary) {
+                for (int j = 0; j < J; ++j) {
+                    const int i = 64 * j + 2 * lane;
+                    if (i < s.rotary) {          // (rotary and i are even: a lane's two channels turn together)
+                        const float4 a = *reinterpret_cast<const float4 *>(&turn[i & (half - 1)]);
+                        const float sign = i & half ? 1.0f : -1.0f;
+                        x[j] = make_float2(x[j].x * a.x + sign * other[j].x * a.y, x[j].y * a.z + sign * other[j].y * a.w);
+                    }
+                }
+            } else {
+                float *mine = reinterpret_cast<float *>(vector[warp]);
+                __syncwarp();
+#pragma unroll
+                for (int j = 0; j < J; ++j) vector[warp][32 * j + lane] = x[j];
+                __syncwarp();
                 auto turned = [&](int i, float own) {
                     if (i >= s.rotary) return own;
-                    const bool first = i < half;
-                    const float2 c = turn[first ? i : i - half];
-                    const float other = mine[first ? i + half : i - half];
-                    return first ? own * c.x - other * c.y : own * c.x + other * c.y;
+                    const float2 c = turn[i < half ? i : i - half];
+                    return i < half ? own * c.x - mine[i + half] * c.y : own * c.x + mine[i - half] * c.y;
                 };
-                const int i = 64 * j + 2 * lane;
-                x[j] = make_float2(turned(i, x[j].x), turned(i + 1, x[j].y));
+#pragma unroll
+                for (int j = 0; j < J; ++j) x[j] = make_float2(turned(64 * j + 2 * lane, x[j].x), turned(64 * j + 2 * lane + 1, x[j].y));
             }
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) if (64 * j < hd) *reinterpret_cast<uint32_t *>(dst + 64 * j + 2 * lane) = spl_pack16<BF16>(x[j].x, x[j].y);
+        for (int j = 0; j < J; ++j) *reinterpret_cast<uint32_t *>(dst + 64 * j) = spl_pack16<BF16>(x[j].x, x[j].y);
     }
 }
 

@@ -141,14 +141,17 @@ static spl_status paged_batch(spl_paged *p, int32_t sequences, const int32_t *ro
     return SPL_OK;
 }
 
-template <int TYPE> static void launch_append(const spl_paged *p, const SplPagedRows &in, const uint16_t *q_norm, const uint16_t *k_norm, uint16_t *q, uint16_t *k, uint16_t *v, cudaStream_t stream) {
+template <int TYPE, int HD> static void launch_append_dim(const spl_paged *p, const SplPagedRows &in, const uint16_t *q_norm, const uint16_t *k_norm, uint16_t *q, uint16_t *k, uint16_t *v, cudaStream_t stream) {
     // A warp a head of a row; few rows are spread over more blocks.
     const int vectors = p->c.heads + 2 * p->c.kv_heads, most = (vectors + 7) / 8;
     const dim3 grid(p->rows, std::max(1, std::min(most, (2 * p->e->sms + p->rows - 1) / p->rows)));
-    if (p->c.dtype == SPL_BF16)
-        launch_step(spl_paged_append_kernel<TYPE, true>, grid, dim3(256), 0, stream, in, q_norm, k_norm, (const double *)p->turns, p->tables(), p->shape, p->e->g.eps, q, k, v);
-    else
-        launch_step(spl_paged_append_kernel<TYPE, false>, grid, dim3(256), 0, stream, in, q_norm, k_norm, (const double *)p->turns, p->tables(), p->shape, p->e->g.eps, q, k, v);
+    launch_step(p->c.dtype == SPL_BF16 ? spl_paged_append_kernel<TYPE, true, HD> : spl_paged_append_kernel<TYPE, false, HD>, grid, dim3(256), 0, stream, in, q_norm, k_norm, (const double *)p->turns,
+                p->tables(), p->shape, p->e->g.eps, q, k, v);
+}
+template <int TYPE> static void launch_append(const spl_paged *p, const SplPagedRows &in, const uint16_t *q_norm, const uint16_t *k_norm, uint16_t *q, uint16_t *k, uint16_t *v, cudaStream_t stream) {
+    if (p->c.head_dim == 64) launch_append_dim<TYPE, 64>(p, in, q_norm, k_norm, q, k, v, stream);
+    else if (p->c.head_dim == 128) launch_append_dim<TYPE, 128>(p, in, q_norm, k_norm, q, k, v, stream);
+    else launch_append_dim<TYPE, 256>(p, in, q_norm, k_norm, q, k, v, stream);
 }
 
 // The cache as a tensor (channel in block, token in page, block of 64 channels, kv head, page) for the copies of values, in boxes of all channels by a page's tokens (at most a
@@ -169,8 +172,8 @@ template <int HD, bool BF16> static void launch_attend(const spl_paged *p, const
 }
 
 // The blocks of a row's cluster: a wave of clusters costs some 14 us of meetings and sorting whatever a block's share, and 19 us for 32,768 values a block (they fit
-// its shared memory; a larger share is read from L2 in every pass, at the same pace). 64 rows of 248,077 take 132 us in four waves of clusters of eight and @64@ in
-// one wave of pairs; twelve rows 42 us in eights, @12@ in pairs.
+// its shared memory; a larger share is read from L2 in every pass, at the same pace). With top-p over 248,077 values 64 rows take 98 us in one wave of pairs, 132 in two
+// waves of fours, 190 in four waves of eights; twelve rows 53 us in eights and 123 in pairs, everything cold.
 static int sample_blocks(const spl_engine *e, int rows, int limit) {
     int best = 1;
     double least = 0.0;
