@@ -421,7 +421,7 @@ spl_status spl_pass_sample(spl_engine *engine, const float *device_logits, int32
  * other spl_pass_ calls'); cudaStreamLegacy is the default stream. Calls on one spl_paged are ordered by the caller: one stream at a time, or events between
  * them. append and attend allocate nothing and may be captured into a graph; such a graph may be replayed after another spl_paged_batch of the same
  * rows per sequence (lengths and pages may differ). Two graphs, or two streams, that may run at the same time need a spl_paged each.
- * An attention block that gives up a wait is reported by the next spl_pass_wait (after the caller has synchronised its stream). */
+ * An attention block that gives up a wait is reported by the next spl_pass_wait (after the caller has synchronised its stream); the pass then begins anew with spl_paged_batch. */
 enum { SPL_F32 = 0, SPL_F16 = 1, SPL_BF16 = 2 };
 typedef struct spl_paged spl_paged;
 typedef struct spl_paged_config {

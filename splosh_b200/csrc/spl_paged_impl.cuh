@@ -23,9 +23,9 @@ struct spl_paged {
     SplPagedShape shape{};
     int max_pages = 0;
     SplEncodeTiled encode = nullptr;
-    // Device tables in one block, filled from one of two pinned blocks (the other's copy may still be on its way): counts, the attention's plan (block_begin, the pieces that
-    // have arrived of each merge: none, the blocks' first items, items); then the batch. Places do not depend on the batch, so a captured graph finds the next one's.
-    size_t words = 0, begin_at = 16, arrived_at = 0, starts_at = 0, items_at = 0, batch_at = 0;
+    // Device tables in one block, filled from one of two pinned blocks (the other's copy may still be on its way): counts, block_begin, the pieces that have arrived of each merge
+    // (none), the blocks' first items, the batch's rows and lengths, the plan's items, the page table. Places do not depend on the batch, so a captured graph finds the next one's.
+    size_t words = 0, begin_at = 16, arrived_at = 0, starts_at = 0, batch_at = 0, items_at = 0, table_at = 0;
     SplPagedPlan plan;
     // Partial sums of query rows whose tokens several blocks share.
     int slot_rows = 0;
@@ -45,8 +45,8 @@ struct spl_paged {
         SplPagedTables out;
         out.counts = tables_dev;
         out.row_sequence = t; t += c.max_rows; out.row_position = t; t += c.max_rows;
-        out.rows = t; t += c.max_sequences; out.lengths = t; t += c.max_sequences;
-        out.table = t;
+        out.rows = t; t += c.max_sequences; out.lengths = t;
+        out.table = tables_dev + table_at;
         return out;
     }
 };
@@ -69,35 +69,39 @@ static spl_status paged_create(spl_engine *e, const spl_paged_config *cp, spl_pa
     const size_t blocks = size_t(e->sms), items = size_t(spl_paged_items_max(c, e->sms));
     p->arrived_at = p->begin_at + (blocks + 1 + 3) / 4 * 4;
     p->starts_at = p->arrived_at + (blocks + 3) / 4 * 4;
-    p->items_at = p->starts_at + blocks * (sizeof(SplPagedItem) / 4);
-    p->batch_at = p->items_at + items * (sizeof(SplPagedItem) / 4);
-    p->words = p->batch_at + size_t(c.max_rows) * 2 + size_t(c.max_sequences) * 2 + size_t(p->max_pages) * c.max_sequences;
+    p->batch_at = p->starts_at + blocks * (sizeof(SplPagedItem) / 4);
+    p->items_at = (p->batch_at + size_t(c.max_rows) * 2 + size_t(c.max_sequences) * 2 + 3) / 4 * 4;
+    p->table_at = p->items_at + items * (sizeof(SplPagedItem) / 4);
+    p->words = p->table_at + size_t(p->max_pages) * c.max_sequences;
     p->written.assign(size_t(c.pages), 0);
-    SPL_CUDA(cudaMalloc(reinterpret_cast<void **>(&p->tables_dev), p->words * 4));
-    for (int i = 0; i < 2; ++i) {
-        SPL_CUDA(cudaMallocHost(reinterpret_cast<void **>(&p->tables_host[i]), p->words * 4));
-        SPL_CUDA(cudaEventCreateWithFlags(&p->copied[i], cudaEventDisableTiming));
-    }
     p->slot_rows = int(std::min<int64_t>(SPL_PAGED_TILE, int64_t(c.max_rows) * p->shape.group));
-    const size_t slot_rows = size_t(spl_paged_slots_max(e->sms)) * p->slot_rows;
-    SPL_CUDA(cudaMalloc(reinterpret_cast<void **>(&p->partial), slot_rows * c.head_dim * 4));
-    SPL_CUDA(cudaMalloc(reinterpret_cast<void **>(&p->partial_ml), slot_rows * sizeof(float2)));
+    // One block of device memory, one pinned one.
+    const size_t slot_rows = size_t(spl_paged_slots_max(e->sms)) * p->slot_rows, table_bytes = (p->words * 4 + 255) / 256 * 256, turn_bytes = 1024;
+    unsigned char *block = nullptr;
+    SPL_CUDA(cudaMalloc(reinterpret_cast<void **>(&block), table_bytes + turn_bytes + slot_rows * (size_t(c.head_dim) * 4 + sizeof(float2))));
+    p->tables_dev = reinterpret_cast<int *>(block);
+    p->turns = reinterpret_cast<double *>(block + table_bytes);
+    p->partial = reinterpret_cast<float *>(block + table_bytes + turn_bytes);
+    p->partial_ml = reinterpret_cast<float2 *>(p->partial + slot_rows * c.head_dim);
+    SPL_CUDA(cudaMallocHost(reinterpret_cast<void **>(&p->tables_host[0]), p->words * 8));
+    p->tables_host[1] = p->tables_host[0] + p->words;
+    for (cudaEvent_t &event : p->copied) SPL_CUDA(cudaEventCreateWithFlags(&event, cudaEventDisableTiming));
     cudaDriverEntryPointQueryResult found;
     void *encode = nullptr;
     SPL_CUDA(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &encode, 12000, cudaEnableDefault, &found));
     if (found != cudaDriverEntryPointSuccess || !encode) return e->fail(SPL_ERR_UNSUPPORTED_DEVICE, "spl_paged_create: the driver has no tensor maps");
     p->encode = reinterpret_cast<SplEncodeTiled>(encode);
     if (!paged_configure(c.head_dim)) return e->fail(SPL_ERR_UNSUPPORTED_DEVICE, "spl_paged_create: the kernel's shared-memory opt-in failed");
-    std::vector<double> turns(size_t(std::max(1, c.rotary_dim / 2)), 0.0);
+    double turns[128] = {};
     for (int i = 0; i < c.rotary_dim / 2; ++i) turns[i] = std::pow(double(c.rope_theta), -2.0 * i / c.rotary_dim) / 6.283185307179586476925;
-    SPL_CUDA(cudaMalloc(reinterpret_cast<void **>(&p->turns), turns.size() * 8));
-    SPL_CUDA(cudaMemcpy(p->turns, turns.data(), turns.size() * 8, cudaMemcpyHostToDevice));
+    SPL_CUDA(cudaMemcpy(p->turns, turns, sizeof turns, cudaMemcpyHostToDevice));
     return SPL_OK;
 }
 
 static void paged_release(spl_paged *p) {
-    cudaFree(p->tables_dev); cudaFree(p->turns); cudaFree(p->partial); cudaFree(p->partial_ml);
-    for (int i = 0; i < 2; ++i) { if (p->tables_host[i]) cudaFreeHost(p->tables_host[i]); if (p->copied[i]) cudaEventDestroy(p->copied[i]); }
+    cudaFree(p->tables_dev);
+    if (p->tables_host[0]) cudaFreeHost(p->tables_host[0]);
+    for (cudaEvent_t event : p->copied) if (event) cudaEventDestroy(event);
     delete p;
 }
 
@@ -125,16 +129,18 @@ static spl_status paged_batch(spl_paged *p, int32_t sequences, const int32_t *ro
     std::memset(w + p->arrived_at, 0, size_t(e->sms) * 4);
     std::memcpy(w + p->starts_at, p->plan.starts.data(), p->plan.starts.size() * sizeof(SplPagedItem));
     std::memcpy(w + p->items_at, p->plan.items.data(), p->plan.items.size() * sizeof(SplPagedItem));
-    int *row_sequence = w + p->batch_at, *row_position = row_sequence + c.max_rows, *seq_rows = row_position + c.max_rows, *seq_lengths = seq_rows + c.max_sequences, *pages = seq_lengths + c.max_sequences;
+    int *row_sequence = w + p->batch_at, *row_position = row_sequence + c.max_rows, *seq_rows = row_position + c.max_rows, *seq_lengths = seq_rows + c.max_sequences, *pages = w + p->table_at;
+    int longest = 1;
     for (int s = 0, r = 0; s < sequences; ++s) {
         for (int i = 0; i < rows[s]; ++i, ++r) { row_sequence[r] = s; row_position[r] = lengths[s] - rows[s] + i; }
         seq_rows[s] = rows[s]; seq_lengths[s] = lengths[s];
         const int used = (lengths[s] + c.page_tokens - 1) / c.page_tokens;
         if (used) std::memcpy(pages + size_t(s) * p->max_pages, table + size_t(s) * table_ld, size_t(used) * 4);
+        longest = std::max(longest, used);
     }
-    const size_t planned = p->items_at + p->plan.items.size() * (sizeof(SplPagedItem) / 4), used = size_t(pages - w) + size_t(sequences) * p->max_pages - p->batch_at;
+    const size_t planned = p->items_at + p->plan.items.size() * (sizeof(SplPagedItem) / 4), pitch = size_t(p->max_pages) * 4;
     SPL_CUDA(cudaMemcpyAsync(p->tables_dev, w, planned * 4, cudaMemcpyHostToDevice, stream));
-    SPL_CUDA(cudaMemcpyAsync(p->tables_dev + p->batch_at, w + p->batch_at, used * 4, cudaMemcpyHostToDevice, stream));
+    SPL_CUDA(cudaMemcpy2DAsync(p->tables_dev + p->table_at, pitch, pages, pitch, size_t(longest) * 4, size_t(sequences), cudaMemcpyHostToDevice, stream));
     SPL_CUDA(cudaEventRecord(p->copied[turn], stream));
     p->turn ^= 1;
     p->rows = int(total); p->sequences = sequences; p->shared_write = shared; p->ready = true;
@@ -172,8 +178,9 @@ template <int HD, bool BF16> static void launch_attend(const spl_paged *p, const
 }
 
 // The blocks of a row's cluster: a wave of clusters costs some 14 us of meetings and sorting whatever a block's share, and 19 us for 32,768 values a block (they fit
-// its shared memory; a larger share is read from L2 in every pass, at the same pace). With top-p over 248,077 values 64 rows take 98 us in one wave of pairs, 132 in two
-// waves of fours, 190 in four waves of eights; twelve rows 53 us in eights and 123 in pairs, everything cold.
+// its shared memory; a larger share is read from L2 in every pass, at the same pace). With top-p over 248,077 values, L2 flushed before each call, in blocks of 1, 2, 4
+// and 8: 12 rows take 158, 96, 65 and 45 us, 24 rows 158, 96, 65 and 82 (two waves of eights), 64 rows 180, 117, 125 and 190. Over 32,000, 151,936 and 248,077 values
+// and 1 to 128 rows, with top-p and with top-k, the rule's choice was the fastest of the four to within 2 us.
 static int sample_blocks(const spl_engine *e, int rows, int limit) {
     int best = 1;
     double least = 0.0;
@@ -210,13 +217,17 @@ spl_status spl_paged_create(spl_engine *e, const spl_paged_config *config, spl_p
     if (!e || !config || !out) return SPL_ERR_INVALID_ARGUMENT;
     SPL_NOT_IN_FLIGHT(e);
     const SplDeviceScope scope(e->device);
+    spl_paged *p = nullptr;
     try {
-        spl_paged *p = new spl_paged;
+        p = new spl_paged;
         const spl_status s = paged_create(e, config, p);
         if (s != SPL_OK) { cudaGetLastError(); paged_release(p); return s; }
         *out = p;
         return SPL_OK;
-    } catch (const std::bad_alloc &) { return SPL_ERR_ALLOCATION_FAILED; }
+    } catch (const std::bad_alloc &) {
+        if (p) paged_release(p);
+        return SPL_ERR_ALLOCATION_FAILED;
+    }
 }
 
 void spl_paged_destroy(spl_paged *p) {
