@@ -405,10 +405,19 @@ spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
     __syncthreads();
     spl_tc_fence_after();
     const uint32_t tmem = uint32_t(uniform(int(*tmem_slot))), tmem_o = tmem + 256;
+    // The block's range, its first item and the first tile's pages are there before the kernel in front is done: a batch is set by copies, which are over before the first kernel
+    // behind them begins. (The first item comes with the range, not after it.)
+    union { SplPagedItem item; int4 four[sizeof(SplPagedItem) / 16]; } first;
+#pragma unroll
+    for (int i = 0; i < int(sizeof(SplPagedItem) / 16); ++i) first.four[i] = __ldcg(reinterpret_cast<const int4 *>(a.starts + blockIdx.x) + i);
+    const SplPagedItem first_item = first.item;
+    const int item0 = uniform(__ldcg(a.block_begin + blockIdx.x)), item1 = uniform(__ldcg(a.block_begin + blockIdx.x + 1));
+    const int box = min(s.page_tokens, 128), boxes = 128 / box;      // a tile's boxes of tokens: a page, or half a page of 256
+    auto page_of = [&](const SplPagedItem &it, int tile) {
+        return tile < it.tile_end && lane < min(boxes, (it.length - tile * 128 + box - 1) / box) ? __ldcg(t.table + size_t(it.sequence) * s.max_pages + (s.page_tokens > 128 ? tile >> 1 : tile * boxes + lane)) : 0;
+    };
+    const int first_page = (warp == 8 || warp == 11) && item0 < item1 ? page_of(first_item, first_item.tile_begin) : 0;
     spl_grid_begin();
-    // (The first item comes with the block's range, not after it.)
-    const SplPagedItem first_item = a.starts[blockIdx.x];
-    const int item0 = uniform(a.block_begin[blockIdx.x]), item1 = uniform(a.block_begin[blockIdx.x + 1]);
     auto item_at = [&](int i) { return i == item0 ? first_item : a.items[i]; };
     // A wait tells a phase from the one before it and no more, so a barrier is waited for only by roles that know its last but one use to be over: S, P and O have one a tile
     // parity (tile i's S is issued after the product of tile i - 2 was waited for; whoever has seen that S may wait for the product of tile i - 1 or i).
@@ -417,8 +426,7 @@ spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
     auto gave_up = [&](int code) { ok = false; if (!*abort && lane == 0) { spl_note_wait(a.error_flag, code, 0); a.error_flag[0] = 200 + warp; } *abort = 1; };
 
     if (warp == 8 || warp == 11) {
-        // ---- copies, keys (warp 8) and values (warp 11). Lane b holds the page of the tile's b-th box of tokens (a page, or half a page of 256); a chunk's barrier counts the boxes that hold tokens.
-        const int box = min(s.page_tokens, 128), boxes = 128 / box;
+        // ---- copies, keys (warp 8) and values (warp 11). Lane b holds the page of the tile's b-th box of tokens; a chunk's barrier counts the boxes that hold tokens.
         const bool keys = warp == 8;
         uint64_t *full = keys ? full_k : full_v, *empty = keys ? empty_k : empty_v;
         const int slots = keys ? NK : NV;
@@ -432,13 +440,9 @@ spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
         for (int i = item0; i < item1 && ok; ++i) {
             const SplPagedItem it = item_at(i);
             const int length = it.length;
-            const int *pages = t.table + size_t(it.sequence) * s.max_pages;
-            auto page_of = [&](int tile) {
-                return tile < it.tile_end && lane < min(boxes, (length - tile * 128 + box - 1) / box) ? pages[s.page_tokens > 128 ? tile >> 1 : tile * boxes + lane] : 0;
-            };
-            int page = page_of(it.tile_begin);
+            int page = i == item0 ? first_page : page_of(it, it.tile_begin);
             for (int tile = it.tile_begin; tile < it.tile_end && ok; ++tile) {
-                const int ahead = page_of(tile + 1), inside = s.page_tokens > 128 ? (tile & 1) * 128 : 0, tokens = min(128, length - tile * 128);
+                const int ahead = page_of(it, tile + 1), inside = s.page_tokens > 128 ? (tile & 1) * 128 : 0, tokens = min(128, length - tile * 128);
                 if (keys) {
                     const int present = (tokens + box - 1) / box, from = __shfl_sync(0xffffffffu, page, b);
                     for (int c = 0; c < PARTS && room(); ++c) {
