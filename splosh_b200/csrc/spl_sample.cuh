@@ -339,7 +339,6 @@ spl_sample_kernel(SplSampleArgs a) {
     extern __shared__ __align__(128) unsigned char spl_sample_raw[];
     SplSampleShared &sh = *reinterpret_cast<SplSampleShared *>(spl_sample_raw);
     cg::cluster_group cluster = cg::this_cluster();
-    spl_grid_begin();
     const int row = blockIdx.y, rank = blockIdx.x, blocks = gridDim.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const float *x = a.logits + size_t(row) * a.ld;
     const int stretch = ((a.limit + blocks - 1) / blocks + 31) / 32 * 32, begin = rank * stretch, end = min(a.limit, begin + stretch);
@@ -347,6 +346,10 @@ spl_sample_kernel(SplSampleArgs a) {
     const float *mine = x + begin;
     const int count = max(0, end - begin);
     asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");      // (a block's shared memory may be reached when it has begun)
+    for (int i = tid; i < SPL_SAMPLE_BINS; i += 1024) { sh.lo[i] = 0u; sh.hi[i] = 0u; }
+    if (tid == 0) sh.listed = 0u;
+    if (tid < 64) sh.powers[tid] = exp2(double(tid) / 64.0);
+    spl_grid_begin();
     // Every thread of the block runs f(four values, index of the first, step of the index) for its values; past the row's end a value is -inf.
     auto each = [&](auto &&f) {
         if constexpr (HELD) {
@@ -389,9 +392,6 @@ spl_sample_kernel(SplSampleArgs a) {
         const uint32_t all = __reduce_max_sync(0xffffffffu, key);
         const uint32_t first = __reduce_min_sync(0xffffffffu, key == all ? index : 0xffffffffu);
         if (lane == 0) sh.warp_sum[warp] = spl_sample_entry(all, first);
-        for (int i = tid; i < SPL_SAMPLE_BINS; i += 1024) { sh.lo[i] = 0u; sh.hi[i] = 0u; }
-        if (tid == 0) sh.listed = 0u;
-        if (tid < 64) sh.powers[tid] = exp2(double(tid) / 64.0);
         __syncthreads();
         unsigned long long best = 0ull;
         if (warp == 0) {
