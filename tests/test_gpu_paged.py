@@ -195,6 +195,37 @@ def test_a_captured_graph_follows_the_batch(engine):
         check_attention(scene, out, "bf16")
 
 
+@pytest.mark.parametrize("page_tokens", [16, 256])
+def test_steps_without_a_wait_between_them(engine, page_tokens):
+    """Batch, append and attend queued one after the other, several sequences growing and leaving: what a step without waits reads is what the step before wrote, to the bit."""
+    heads, kv_heads, dim, steps, pages = 8, 2, 128, 24, 3 * (-(-400 // page_tokens))
+    g = torch.Generator().manual_seed(page_tokens)
+    x = torch.randn((steps, 2, 3, heads + 2 * kv_heads, dim), generator=g).cuda()
+    table = torch.randperm(pages, generator=g).numpy().astype(np.int32).reshape(3, -1)
+    start = torch.randn((2, pages, kv_heads, page_tokens, dim), generator=g).to(torch.bfloat16).cuda()
+
+    def run(wait):
+        paged = S.PagedAttention(engine, heads, kv_heads, dim, pages, page_tokens=page_tokens, rotary_dim=64, rope_theta=1e4, max_sequences=3, max_rows=3, max_context=400)
+        k, v = start[0].clone(), start[1].clone()
+        q, out = (torch.zeros((steps, 2, 3, heads, dim), device="cuda", dtype=torch.bfloat16) for _ in range(2))
+        torch.cuda.synchronize()
+        for step in range(steps):
+            lengths = [1 + step, 120 + step, (300 if step % 2 else 5) + step]
+            paged.batch([1, 1, 1], lengths, table)
+            for layer in range(2):                        # of one cache: the second writes what the first has read
+                row = x[step, layer].data_ptr()
+                paged.append(row, row + 4 * heads * dim, row + 4 * (heads + kv_heads) * dim, q[step, layer].data_ptr(), k.data_ptr(), v.data_ptr(), ld=(heads + 2 * kv_heads) * dim)
+                paged.attend(q[step, layer].data_ptr(), k.data_ptr(), v.data_ptr(), out[step, layer].data_ptr())
+                if wait:
+                    engine.pass_wait()
+        engine.pass_wait()
+        torch.cuda.synchronize()
+        return out, k, v
+
+    for a, b in zip(run(True), run(False)):
+        assert torch.equal(a, b)
+
+
 # ---- append --------------------------------------------------------------------------------------
 def expected_append(x, position, rotary, theta, weight, eps):
     """[rows][heads][head_dim] in 64 bits, and the bound on the 32-bit arithmetic in front of the rounding."""
