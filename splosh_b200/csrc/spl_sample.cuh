@@ -513,8 +513,9 @@ spl_sample_kernel(SplSampleArgs a) {
     if (step == SPL_SAMPLE_WEIGH) {
         for (int i = tid; i < SPL_SAMPLE_BINS; i += 1024) { sh.lo[i] = 0u; sh.hi[i] = 0u; }
         __syncthreads();
-        // Values that cannot count are passed over: without top-p nothing below min-p's bound is in any sum (a bin and the roundings of slack).
-        const float least_value = r.least && !(r.p < 1.0f) ? r.w.max - (-logf(r.m) + 4.0f / SPL_SAMPLE_BINS_NAT) * r.t - 1e-6f * fabsf(r.w.max) : -INFINITY;
+        // Values that cannot count are passed over: without top-p nothing below min-p's bound is in any sum (a bin and the roundings of slack). Beside an infinite maximum the bound
+        // would be no number, which nothing reaches: there all values are looked at.
+        const float least_value = r.least && !(r.p < 1.0f) && r.w.max < INFINITY ? r.w.max - (-logf(r.m) + 4.0f / SPL_SAMPLE_BINS_NAT) * r.t - 1e-6f * fabsf(r.w.max) : -INFINITY;
         each([&](const float (&value)[4], int i, int step) {
             if (!(value[0] >= least_value) & !(value[1] >= least_value) & !(value[2] >= least_value) & !(value[3] >= least_value)) return;
             // The four weights side by side (a weight is a chain of ten 64-bit operations), whatever of them counts.

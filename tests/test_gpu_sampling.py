@@ -188,3 +188,18 @@ def test_refusals(engine):
         engine.sample([0.5, 0.5])
     with pytest.raises(S.EngineError):
         engine.sample([0.5], vocab_limit=engine.g.vocab + 1)
+
+
+def test_infinite_values_share_the_weight_under_min_p(engine):
+    """Several infinite logits with min-p and nothing else that ends what stays, at every share of theirs: on rows of few values, on rows that hold fewer values than top-k, and behind a cut."""
+    rng = np.random.default_rng(21)
+    u = np.array([0.0, 0.1, 0.33, 0.34, 0.5, 0.66, 0.67, 0.9, 0.999], np.float32)
+    for width, at, settings in ((3000, [7, 90, 2000], (None, None, None, 0.05)), (3000, [7, 90, 2000], (0.7, None, None, 0.5)), (3000, [7, 90, 2000], (None, None, None, 1e-6)), (9500, [4, 5, 9000], (None, 9000, None, 0.05)),
+                                (20000, [0, 900, 19999], (1.0, 9000, 1.0, 0.05)), (248077, [1, 100000, 248000], (None, None, None, 0.9)), (3000, [17], (None, None, None, 0.05)), (3000, [7, 90], (None, 2, None, 0.05))):
+        x = logits(rng, len(u), width)
+        if width == 9500:
+            x[:, rng.random(width) < 0.5] = -np.inf
+        x[:, at] = np.inf
+        want = expected(x, width, settings, u)
+        assert set(want) <= set(at)
+        assert np.array_equal(device_sample(engine, x, width, settings, u), want), (width, settings)
