@@ -371,7 +371,8 @@ spl_sample_kernel(SplSampleArgs a) {
     };
     SplSampleRow r;
     r.t = a.temperature ? a.temperature[row] : 1.0f; r.p = a.top_p ? a.top_p[row] : 1.0f; r.u = a.uniform[row];
-    r.m = a.min_p && a.min_p[row] > 0.0f ? fminf(a.min_p[row], 1.0f) : 0.0f; r.k = a.top_k ? a.top_k[row] : 0;
+    // (At an infinite temperature every weight is one, or none beside an infinite value: min-p takes nothing away.)
+    r.m = a.min_p && a.min_p[row] > 0.0f && r.t < INFINITY ? fminf(a.min_p[row], 1.0f) : 0.0f; r.k = a.top_k ? a.top_k[row] : 0;
     r.least = r.m > 0.0f ? (unsigned long long)ceil(double(r.m) * SPL_SAMPLE_UNIT) : 0ull;
 
     // The largest value and its lowest index.
@@ -413,7 +414,7 @@ spl_sample_kernel(SplSampleArgs a) {
     r.w.max = spl_topk_value(uint32_t(top >> 32));
     r.w.scale = 64.0 / 0.693147180559945309417 / double(r.t);
     r.w.powers = sh.powers;
-    r.bin_scale = fminf(2.0f * SPL_SAMPLE_BINS_NAT / r.t, 3.0e38f);
+    r.bin_scale = fminf(fmaxf(2.0f * SPL_SAMPLE_BINS_NAT / r.t, 1.0e-38f), 3.0e38f);      // (never zero: an infinite value's bin would be no number at an infinite temperature)
     // The bin of a value that may be picked: halved values do not overflow, and rounding keeps the order (it may put a value in the next bin, no more). Beside an
     // infinite maximum the finite values are binned as beside the largest one (they have no weight), and the infinite ones come to bin 0 by way of -inf.
     const float half_max = 0.5f * fminf(r.w.max, 3.402823466e38f);

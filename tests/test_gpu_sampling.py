@@ -203,3 +203,20 @@ def test_infinite_values_share_the_weight_under_min_p(engine):
         want = expected(x, width, settings, u)
         assert set(want) <= set(at)
         assert np.array_equal(device_sample(engine, x, width, settings, u), want), (width, settings)
+
+
+def test_an_infinite_temperature_weighs_all_alike(engine):
+    """Every value's weight is one, but for -inf and NaN; beside infinite values the finite ones have none."""
+    rng = np.random.default_rng(22)
+    u = np.array([0.0, 0.1, 0.33, 0.34, 0.5, 0.66, 0.67, 0.9, 0.999], np.float32)
+    for width in (40, 3000, 9000):
+        x = logits(rng, len(u), width)
+        x[:, rng.random(width) < 0.3] = -np.inf
+        x[:, rng.random(width) < 0.1] = np.nan
+        x[0, 3:9] = [3.4e38, -3.4e38, 1e-40, -1e-40, 0.0, -0.0]
+        for settings in ((np.inf, None, None, None), (np.inf, 30, None, None), (np.inf, None, 0.25, None), (np.inf, None, None, 0.5), (np.inf, 20, 0.5, 1.0), (np.inf, 6000, 0.75, 0.1)):
+            assert np.array_equal(device_sample(engine, x, width, settings, u), expected(x, width, settings, u)), (width, settings)
+        x[:, [5, 20, 31]] = np.inf
+        for k, p, m, stay in ((None, None, None, 3), (None, None, 0.5, 3), (2, None, None, 2), (20, 0.5, 1.0, 2), (None, 0.25, None, 1), (6000, None, 0.1, 3), (None, None, 1.0, 3)):
+            want = [(5, 20, 31)[max(int(np.ceil(np.float64(v) * stay)) - 1, 0)] for v in u]
+            assert np.array_equal(device_sample(engine, x, width, (np.inf, k, p, m), u), want), (width, k, p, m)
