@@ -48,9 +48,13 @@ __device__ __forceinline__ unsigned long long spl_sample_weight_near(float x, co
     const double scaled = __hiloint2double(__double2hiint(power) + ((n >> 6) + 44) * (1 << 20), __double2loint(power));      // 2^(44 + n / 64), at least 2^-4
     return (unsigned long long)__double_as_longlong(fma(scaled, e, 4503599627370496.0)) & ((1ull << 52) - 1ull);
 }
+// Whether a value other than the maximum has no weight.
+__device__ __forceinline__ bool spl_sample_weightless(float x, const SplSampleWeigh &w) {
+    return w.max == INFINITY || !((double(x) - double(w.max)) * w.scale > -32.0 * 64.0 / 0.693147180559945309417);
+}
 __device__ __forceinline__ unsigned long long spl_sample_weight(float x, const SplSampleWeigh &w) {
     if (x == w.max) return 1ull << 44;
-    if (w.max == INFINITY || !((double(x) - double(w.max)) * w.scale > -32.0 * 64.0 / 0.693147180559945309417)) return 0ull;
+    if (spl_sample_weightless(x, w)) return 0ull;
     return spl_sample_weight_near(x, w);
 }
 
@@ -65,6 +69,7 @@ __device__ __forceinline__ unsigned long long spl_sample_weight(float x, const S
 // the values' keys at a time (spl_sample_slow).
 #define SPL_SAMPLE_BINS 4096
 #define SPL_SAMPLE_BINS_NAT 128.0f             // bins a natural unit of (max - x) / T
+#define SPL_SAMPLE_SCALE_MAX 3.0e38f           // of a row's bin_scale, twice the bins a unit of max - x: at temperatures below 8.6e-37 bins are wider, and values of no weight lie in front of the last one, too
 #define SPL_SAMPLE_LIST 4096
 #define SPL_SAMPLE_STRETCH 32768
 #define SPL_SAMPLE_CLUSTER 8
@@ -414,7 +419,7 @@ spl_sample_kernel(SplSampleArgs a) {
     r.w.max = spl_topk_value(uint32_t(top >> 32));
     r.w.scale = 64.0 / 0.693147180559945309417 / double(r.t);
     r.w.powers = sh.powers;
-    r.bin_scale = fminf(fmaxf(2.0f * SPL_SAMPLE_BINS_NAT / r.t, 1.0e-38f), 3.0e38f);      // (never zero: an infinite value's bin would be no number at an infinite temperature)
+    r.bin_scale = fminf(fmaxf(2.0f * SPL_SAMPLE_BINS_NAT / r.t, 1.0e-38f), SPL_SAMPLE_SCALE_MAX);      // (never zero: an infinite value's bin would be no number at an infinite temperature)
     // The bin of a value that may be picked: halved values do not overflow, and rounding keeps the order (it may put a value in the next bin, no more). Beside an
     // infinite maximum the finite values are binned as beside the largest one (they have no weight), and the infinite ones come to bin 0 by way of -inf.
     const float half_max = 0.5f * fminf(r.w.max, 3.402823466e38f);
@@ -425,7 +430,7 @@ spl_sample_kernel(SplSampleArgs a) {
     // The values of the bins [first, last] and [also_first, also_last] (in front of them; none where also_first is negative) into the block's list.
     auto set_aside = [&](int first, int last, int also_first, int also_last) {
         // Most values are told by comparisons: bounds a bin and the roundings outside the bins asked for.
-        const float width = r.t / SPL_SAMPLE_BINS_NAT, slack = 2.0f * width + 1e-6f * fabsf(r.w.max);
+        const float width = 2.0f / r.bin_scale, slack = 2.0f * width + 1e-6f * fabsf(r.w.max);
         auto top_of = [&](int b) { return r.w.max - float(b) * width + slack; };
         auto bottom_of = [&](int b) { return b == SPL_SAMPLE_BINS - 1 ? -INFINITY : r.w.max - float(b + 1) * width - slack; };
         const float high = top_of(first), low = bottom_of(last), also_high = also_first < 0 ? -INFINITY : top_of(also_first), also_low = also_first < 0 ? INFINITY : bottom_of(also_last);
@@ -517,6 +522,7 @@ spl_sample_kernel(SplSampleArgs a) {
         // Values that cannot count are passed over: without top-p nothing below min-p's bound is in any sum (a bin and the roundings of slack). Beside an infinite maximum the bound
         // would be no number, which nothing reaches: there all values are looked at.
         const float least_value = r.least && !(r.p < 1.0f) && r.w.max < INFINITY ? r.w.max - (-logf(r.m) + 4.0f / SPL_SAMPLE_BINS_NAT) * r.t - 1e-6f * fabsf(r.w.max) : -INFINITY;
+        const bool guarded = r.w.max == INFINITY || r.bin_scale == SPL_SAMPLE_SCALE_MAX;      // the last bin does not hold all values of no weight
         each([&](const float (&value)[4], int i, int step) {
             if (!(value[0] >= least_value) & !(value[1] >= least_value) & !(value[2] >= least_value) & !(value[3] >= least_value)) return;
             // The four weights side by side (a weight is a chain of ten 64-bit operations), whatever of them counts.
@@ -528,7 +534,7 @@ spl_sample_kernel(SplSampleArgs a) {
             for (int q = 0; q < 4; ++q) {
                 if (!(value[q] > -INFINITY) || b[q] == SPL_SAMPLE_BINS - 1) continue;
                 if (cut && spl_sample_entry(spl_topk_key(value[q]), uint32_t(i + q * step)) < cut) continue;
-                if (r.w.max == INFINITY) { if (value[q] != r.w.max) continue; w[q] = 1ull << 44; }
+                if (guarded) { if (value[q] == r.w.max) w[q] = 1ull << 44; else if (spl_sample_weightless(value[q], r.w)) continue; }
                 // Two words a bin, the carry taken by whoever makes the lower one overflow.
                 const unsigned int low = unsigned(w[q]), was = atomicAdd(&sh.lo[b[q]], low), high = unsigned(w[q] >> 32) + (was + low < was ? 1u : 0u);
                 if (high) atomicAdd(&sh.hi[b[q]], high);
@@ -549,7 +555,7 @@ spl_sample_kernel(SplSampleArgs a) {
             if (p_bin < SPL_SAMPLE_BINS) c0 = c1 = p_bin;
             if (r.least) {
                 // Weights of m lie -ln m below the maximum; the bins next to that one may hold some, too, for the rounding of their place.
-                const int m_bin = int(fminf(fmaxf(-logf(r.m) * SPL_SAMPLE_BINS_NAT, 0.0f), float(SPL_SAMPLE_BINS - 2))), m0 = max(m_bin - 1, 0), m1 = m_bin + 1;
+                const int m_bin = int(fminf(fmaxf(-logf(r.m) * (0.5f * r.bin_scale * r.t), 0.0f), float(SPL_SAMPLE_BINS - 2))), m0 = max(m_bin - 1, 0), m1 = m_bin + 1;
                 if (p_bin > m1) { c0 = m0; c1 = m1; p_bin = SPL_SAMPLE_BINS; }      // top-p's place comes later
                 else if (p_bin >= m0) { c0 = m0; c1 = m1; }
             }

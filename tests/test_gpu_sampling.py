@@ -220,3 +220,18 @@ def test_an_infinite_temperature_weighs_all_alike(engine):
         for k, p, m, stay in ((None, None, None, 3), (None, None, 0.5, 3), (2, None, None, 2), (20, 0.5, 1.0, 2), (None, 0.25, None, 1), (6000, None, 0.1, 3), (None, None, 1.0, 3)):
             want = [(5, 20, 31)[max(int(np.ceil(np.float64(v) * stay)) - 1, 0)] for v in u]
             assert np.array_equal(device_sample(engine, x, width, (np.inf, k, p, m), u), want), (width, k, p, m)
+
+
+@pytest.mark.parametrize("temperature", [1e-35, 8e-37, 1e-37, 3e-38, 1e-38, 1e-40, 1e-44])
+def test_temperatures_near_the_types_smallest(engine, temperature):
+    """Logits of the temperature's size, and some up to thousands of it below the maximum."""
+    rng = np.random.default_rng(23)
+    t = np.float32(temperature)
+    for width in (2000, 50000):
+        x = (rng.normal(0, 2, (9, width)) * np.float64(t)).astype(np.float32)
+        x[:, rng.integers(0, width, 20)] += (rng.uniform(4, 9, 20) * np.float64(t)).astype(np.float32)
+        x[:, ::3] = (-rng.uniform(20, 4000, x[:, ::3].shape) * np.float64(t)).astype(np.float32)
+        x[:, 1:300:9] = (x.max(1, keepdims=True).astype(np.float64) - np.linspace(1380.0, 1425.0, len(range(1, 300, 9))) * np.float64(t)).astype(np.float32)
+        u = rng.random(9).astype(np.float32)
+        for settings in ((t, None, None, None), (t, None, 0.9, None), (t, None, None, 0.05), (t, None, 0.95, 0.01), (t, 40, None, None), (t, 40, 0.9, 0.02), (t, 9000, 0.98, 0.001), (t, None, None, 1e-6)):
+            assert np.array_equal(device_sample(engine, x, width, settings, u), expected(x, width, settings, u)), (width, settings)
