@@ -478,8 +478,8 @@ spl_sample_kernel(SplSampleArgs a) {
             unsigned long long all;
             spl_sample_running(sh, &all);
             const int b = spl_sample_place(sh, SPL_SAMPLE_BINS, (unsigned long long)r.k);
-            if (b == SPL_SAMPLE_BINS) decide(SPL_SAMPLE_WEIGH, 0, 0, 0ull);                                     // fewer values than k
-            else if (sh.sums[b] <= SPL_SAMPLE_LIST) decide(SPL_SAMPLE_FINISH, 0, b, 0ull);
+            if (b < SPL_SAMPLE_BINS && sh.sums[b] <= SPL_SAMPLE_LIST) decide(SPL_SAMPLE_FINISH, 0, b, 0ull);
+            else if (b >= SPL_SAMPLE_BINS - 1) decide(SPL_SAMPLE_WEIGH, 0, 0, 0ull);      // fewer values than k, or fewer with a weight: a cut among those without takes nothing away
             else {
                 if (tid == 0) sh.value[1] = b ? sh.sums[b - 1] : 0ull;
                 decide(SPL_SAMPLE_CUT, b, b, 0ull);
@@ -555,7 +555,7 @@ spl_sample_kernel(SplSampleArgs a) {
             if (p_bin < SPL_SAMPLE_BINS) c0 = c1 = p_bin;
             if (r.least) {
                 // Weights of m lie -ln m below the maximum; the bins next to that one may hold some, too, for the rounding of their place.
-                const int m_bin = int(fminf(fmaxf(-logf(r.m) * (0.5f * r.bin_scale * r.t), 0.0f), float(SPL_SAMPLE_BINS - 2))), m0 = max(m_bin - 1, 0), m1 = m_bin + 1;
+                const int m_bin = int(fminf(fmaxf(-logf(r.m) * (0.5f * r.bin_scale * r.t), 0.0f), float(SPL_SAMPLE_BINS - 2))), m0 = max(m_bin - 1, 0), m1 = min(m_bin + 1, SPL_SAMPLE_BINS - 2);      // (the last bin's have no weight)
                 if (p_bin > m1) { c0 = m0; c1 = m1; p_bin = SPL_SAMPLE_BINS; }      // top-p's place comes later
                 else if (p_bin >= m0) { c0 = m0; c1 = m1; }
             }

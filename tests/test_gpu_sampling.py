@@ -235,3 +235,42 @@ def test_temperatures_near_the_types_smallest(engine, temperature):
         u = rng.random(9).astype(np.float32)
         for settings in ((t, None, None, None), (t, None, 0.9, None), (t, None, None, 0.05), (t, None, 0.95, 0.01), (t, 40, None, None), (t, 40, 0.9, 0.02), (t, 9000, 0.98, 0.001), (t, None, None, 1e-6)):
             assert np.array_equal(device_sample(engine, x, width, settings, u), expected(x, width, settings, u)), (width, settings)
+
+
+def fastest(engine, x, limit, settings, u, runs=8):
+    """The token of every row, and the shortest of some runs on the device, in us."""
+    rows = x.shape[0]
+    types = (np.float32, np.int32, np.float32, np.float32)
+    dx, du = torch.from_numpy(x).cuda(), torch.from_numpy(u).cuda()
+    buffers = [None if s is None else torch.from_numpy(np.ascontiguousarray(np.broadcast_to(s, rows), t)).cuda() for s, t in zip(settings, types)]
+    t, k, p, m = (None if b is None else b.data_ptr() for b in buffers)
+    ids, least = torch.zeros(rows, dtype=torch.int32, device="cuda"), float("inf")
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(runs):
+        begin, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        with torch.cuda.stream(stream):
+            begin.record()
+            engine.pass_sample(dx.data_ptr(), rows, x.shape[1], limit, ids.data_ptr(), du.data_ptr(), temperature=t, top_k=k, top_p=p, min_p=m, stream=stream.cuda_stream)
+            end.record()
+        end.synchronize()
+        least = min(least, begin.elapsed_time(end) * 1e3)
+    return ids.cpu().numpy(), least
+
+
+@pytest.fixture(scope="module")
+def large(engine):
+    """Twelve rows of 248,077 logits, and what sampling them takes where nothing is in the way."""
+    rng = np.random.default_rng(31)
+    x, u = logits(rng, 12, 248077), rng.random(12).astype(np.float32)
+    ids, ordinary = fastest(engine, x, 248077, (1.0, None, 0.95, None), u)
+    assert np.array_equal(ids, expected(x, 248077, (1.0, None, 0.95, None), u))
+    return x, u, ordinary
+
+
+@pytest.mark.parametrize("settings", [(0.1, 20, None, None), (0.2, 1000, None, None), (0.1, 50, 0.9, None), (0.1, None, None, 1e-14), (0.05, 100, None, 0.01), (0.1, None, 0.99, 1e-20)])
+def test_values_without_a_weight_do_not_slow_a_row_down(engine, large, settings):
+    x, u, ordinary = large
+    ids, took = fastest(engine, x, 248077, settings, u)
+    assert np.array_equal(ids, expected(x, 248077, settings, u))
+    assert took < 4 * ordinary
