@@ -575,13 +575,14 @@ spl_sample_kernel(SplSampleArgs a) {
         step = sh.step;
         const unsigned long long *kept = reinterpret_cast<const unsigned long long *>(sh.lo);
         unsigned long long target = rank == 0 && step == SPL_SAMPLE_DRAW ? spl_sample_target(r.u, all) : 0ull;
-        if (step == SPL_SAMPLE_END) {
+        while (step == SPL_SAMPLE_END) {                                               // (twice at most)
             set_aside(sh.first_bin, sh.last_bin, sh.also_first, sh.also_last);
             if (rank == 0) {
                 // The list: the draw's bins where they came along (entries [0, front)), then the bins what stays ends in, running sums from `base`.
                 const unsigned long long base = c0 ? kept[c0 - 1] : 0ull, also_base = also > 0 ? kept[also - 1] : 0ull, also_sum = also < 0 ? 0ull : kept[also_last] - also_base;
                 const int n = spl_sample_sorted(sh, cluster, blocks, r, base - also_sum);
-                if (n < 0) decide(SPL_SAMPLE_SLOW, 0, 0, 0ull);
+                if (n < 0 && also >= 0) { also = -1; decide(SPL_SAMPLE_END, c0, c1, cut); }      // too many together: the draw has a turn of its own
+                else if (n < 0) decide(SPL_SAMPLE_SLOW, 0, 0, 0ull);
                 else {
                     int front = 0;
                     if (also >= 0) {

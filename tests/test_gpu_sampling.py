@@ -274,3 +274,11 @@ def test_values_without_a_weight_do_not_slow_a_row_down(engine, large, settings)
     ids, took = fastest(engine, x, 248077, settings, u)
     assert np.array_equal(ids, expected(x, 248077, settings, u))
     assert took < 4 * ordinary
+
+
+@pytest.mark.parametrize("settings", [(3.0, None, 0.95, 0.02), (3.0, None, None, 0.05), (2.5, None, 0.95, 0.02)])
+def test_the_draws_bins_do_not_crowd_out_the_end(engine, large, settings):
+    x, u, ordinary = large
+    ids, took = fastest(engine, x, 248077, settings, u)
+    assert np.array_equal(ids, expected(x, 248077, settings, u))
+    assert took < 4 * ordinary
