@@ -349,3 +349,24 @@ def test_windows_that_begin_anywhere_in_a_tile(engine, head_dim, page_tokens, wi
             for token in range(length - window):
                 cache[scene.table[s, token // page_tokens], :, token % page_tokens] = float("nan")
     check_attention(scene, attend(engine, scene, "f32"), "f32")
+
+
+def test_a_new_object_rotates_by_its_own_table_at_once(engine):
+    """Append on a stream that waits for nobody, right behind the object's making: the table of angles is there. (Every object has another base, and often the memory of the one before.)"""
+    heads, kv_heads, dim, rows = 2, 1, 128, 4
+    g = torch.Generator().manual_seed(40)
+    x = torch.randn((rows, heads + 2 * kv_heads, dim), generator=g).cuda()
+    k, v = (torch.zeros((1, kv_heads, 16, dim), device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    stream, base = torch.cuda.Stream(), x.data_ptr()
+    for i in range(40):
+        q = torch.zeros((2, rows, heads, dim), device="cuda", dtype=torch.bfloat16)
+        torch.cuda.synchronize()
+        paged = S.PagedAttention(engine, heads, kv_heads, dim, 1, page_tokens=16, rotary_dim=dim, rope_theta=10.0 ** (1 + i % 7), max_sequences=1, max_rows=rows, max_context=16)
+        for n in range(2):
+            paged.batch([rows], [16], np.zeros((1, 1), np.int32), stream=stream.cuda_stream)
+            paged.append(base, base + 4 * heads * dim, base + 4 * (heads + kv_heads) * dim, q[n].data_ptr(), k.data_ptr(), v.data_ptr(), ld=(heads + 2 * kv_heads) * dim, stream=stream.cuda_stream)
+            torch.cuda.synchronize()
+        want, e = expected_append(x[:, :heads].cpu(), torch.arange(12, 16), dim, 10.0 ** (1 + i % 7), None, 0.0)
+        for got in q:
+            assert ((got.double().cpu() - want).abs() <= e + half_step("bf16") * (want.abs() + e)).all()
+        paged.close()
