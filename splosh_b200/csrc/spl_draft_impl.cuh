@@ -317,8 +317,7 @@ spl_status spl_draft_set_tensor(spl_draft *d, const char *name, const uint16_t *
         if (!shape(d->c.rank, H)) return wrong();
         d->hidden_projection.resize(size_t(rows) * inner);
         for (size_t i = 0; i < d->hidden_projection.size(); ++i) d->hidden_projection[i] = draft_bf16_float(bf16[i]);
-        SPL_CUDA(cudaMemcpy(d->projection_dev, d->hidden_projection.data(), d->hidden_projection.size() * 4, cudaMemcpyHostToDevice));
-        return SPL_OK;
+        return upload(e, d->projection_dev, d->hidden_projection.data(), d->hidden_projection.size() * 4);
     }
     if (n == "candidate_selector.predecessor_codebook" || n == "candidate_selector.successor_codebook") {
         if (!shape(d->vocab, d->c.rank)) return wrong();
@@ -431,8 +430,9 @@ spl_status spl_draft_import_context(spl_draft *d, int32_t slot, int32_t first, i
     const size_t per_slot = size_t(d->c.ring_capacity) * d->kv * 2;
     const uint8_t *in = static_cast<const uint8_t *>(rings);
     for (DraftLayer &L : d->layers) {
-        SPL_CUDA(cudaMemcpy(reinterpret_cast<uint8_t *>(L.k_ring) + slot * per_slot, in, per_slot, cudaMemcpyHostToDevice)); in += per_slot;
-        SPL_CUDA(cudaMemcpy(reinterpret_cast<uint8_t *>(L.v_ring) + slot * per_slot, in, per_slot, cudaMemcpyHostToDevice)); in += per_slot;
+        spl_status s = upload(e, reinterpret_cast<uint8_t *>(L.k_ring) + slot * per_slot, in, per_slot); in += per_slot;
+        if (s == SPL_OK) s = upload(e, reinterpret_cast<uint8_t *>(L.v_ring) + slot * per_slot, in, per_slot); in += per_slot;
+        if (s != SPL_OK) return s;
     }
     d->context_first[slot] = first; d->context_end[slot] = end;
     return SPL_OK;

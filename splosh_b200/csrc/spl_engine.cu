@@ -131,6 +131,14 @@ spl_status device_alloc(spl_engine *e, T **ptr, size_t count, size_t *account = 
     return SPL_OK;
 }
 
+// Host memory to the device, there when the call returns. (cudaMemcpy of pageable memory may return before the copy on the device is done, and only the legacy stream would wait
+// for it: neither the engine's stream nor one of the caller's need do so.)
+spl_status upload(spl_engine *e, void *dst, const void *src, size_t bytes) {
+    SPL_CUDA(cudaMemcpyAsync(dst, src, bytes, cudaMemcpyHostToDevice, e->stream));
+    SPL_CUDA(cudaStreamSynchronize(e->stream));
+    return SPL_OK;
+}
+
 int round16(int v) { return (v + 15) / 16 * 16; }
 
 struct Shapes {
@@ -873,7 +881,7 @@ spl_status create(const spl_geometry *gp, const spl_config *cp, spl_engine *e) {
         std::vector<float> freq(std::max(1, g.rotary_dim / 2));
         for (int i = 0; i < g.rotary_dim / 2; ++i) freq[i] = float(std::pow(double(g.rope_theta), -2.0 * double(i) / double(g.rotary_dim)));
         if ((s = device_alloc(e, &e->inv_freq, freq.size())) != SPL_OK) return s;
-        SPL_CUDA(cudaMemcpy(e->inv_freq, freq.data(), freq.size() * 4, cudaMemcpyHostToDevice));
+        if ((s = upload(e, e->inv_freq, freq.data(), freq.size() * 4)) != SPL_OK) return s;
     }
     // Session state.
     const size_t page_vecs = size_t(g.kv_heads) * SPL_PAGE_TOKENS;
@@ -1017,10 +1025,10 @@ spl_status spl_weights_set_q4(spl_engine *e, int32_t layer, int32_t kind, int32_
     SPL_CUDA(cudaSetDevice(e->device));
     if (layer < 0 && kind == SPL_Q4_EMBED) {
         if (rows != e->g.vocab || inner != e->g.hidden) return e->fail(SPL_ERR_INVALID_ARGUMENT, "embedding shape does not match the geometry");
-        SPL_CUDA(cudaMemcpy(e->embed_packed, packed, size_t(rows) * inner / 2, cudaMemcpyHostToDevice));
-        SPL_CUDA(cudaMemcpy(e->embed_scales, scales, size_t(rows) * inner / 32, cudaMemcpyHostToDevice));
-        SPL_CUDA(cudaMemcpy(e->embed_biases, biases, size_t(rows) * inner / 32, cudaMemcpyHostToDevice));
-        return SPL_OK;
+        spl_status s = upload(e, e->embed_packed, packed, size_t(rows) * inner / 2);
+        if (s == SPL_OK) s = upload(e, e->embed_scales, scales, size_t(rows) * inner / 32);
+        if (s == SPL_OK) s = upload(e, e->embed_biases, biases, size_t(rows) * inner / 32);
+        return s;
     }
     Placement pl;
     const spl_status s = place(e, layer, kind, &pl);
@@ -1041,8 +1049,7 @@ spl_status spl_weights_set_vector(spl_engine *e, int32_t layer, int32_t kind, co
         slot = &e->layers[layer].vec[kind];
     }
     if (!*slot) SPL_CUDA(cudaMalloc(reinterpret_cast<void **>(slot), size_t(count) * 2));
-    SPL_CUDA(cudaMemcpy(*slot, bf16, size_t(count) * 2, cudaMemcpyHostToDevice));
-    return SPL_OK;
+    return upload(e, *slot, bf16, size_t(count) * 2);
 }
 
 // The GGUF twin of a q4 device tensor of the engine.
@@ -1112,9 +1119,9 @@ spl_status spl_weights_set_gguf(spl_engine *e, int32_t layer, int32_t kind, int3
         const size_t bytes = size_t(rows) * (inner / 256) * spl_gguf_block_bytes(type);
         cudaFree(e->g_embed); e->g_embed = nullptr;
         SPL_CUDA(cudaMalloc(reinterpret_cast<void **>(&e->g_embed), bytes));
-        SPL_CUDA(cudaMemcpy(e->g_embed, blocks, bytes, cudaMemcpyHostToDevice));
-        e->g_embed_format = type;
-        return SPL_OK;
+        const spl_status s = upload(e, e->g_embed, blocks, bytes);
+        if (s == SPL_OK) e->g_embed_format = type;
+        return s;
     }
     Placement pl;
     const spl_status s = place(e, layer, kind, &pl);
@@ -2036,7 +2043,8 @@ spl_status spl_tensor_create_vector(spl_engine *e, const uint16_t *bf16, int32_t
     SPL_CUDA(cudaSetDevice(e->device));
     spl_tensor *t = new spl_tensor;
     if (cudaMalloc(reinterpret_cast<void **>(&t->vec), size_t(count) * 2) != cudaSuccess) { delete t; return e->fail(SPL_ERR_ALLOCATION_FAILED, "vector"); }
-    cudaMemcpy(t->vec, bf16, size_t(count) * 2, cudaMemcpyHostToDevice);
+    const spl_status s = upload(e, t->vec, bf16, size_t(count) * 2);
+    if (s != SPL_OK) { cudaFree(t->vec); delete t; return s; }
     t->count = count;
     *out = t;
     return SPL_OK;

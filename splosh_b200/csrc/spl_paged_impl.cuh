@@ -94,10 +94,7 @@ static spl_status paged_create(spl_engine *e, const spl_paged_config *cp, spl_pa
     if (!paged_configure(c.head_dim)) return e->fail(SPL_ERR_UNSUPPORTED_DEVICE, "spl_paged_create: the kernel's shared-memory opt-in failed");
     double turns[128] = {};
     for (int i = 0; i < c.rotary_dim / 2; ++i) turns[i] = std::pow(double(c.rope_theta), -2.0 * i / c.rotary_dim) / 6.283185307179586476925;
-    // On the engine's stream, and waited for: cudaMemcpy of pageable memory may return before the copy is done, and only the legacy stream would wait for it.
-    SPL_CUDA(cudaMemcpyAsync(p->turns, turns, sizeof turns, cudaMemcpyHostToDevice, e->stream));
-    SPL_CUDA(cudaStreamSynchronize(e->stream));
-    return SPL_OK;
+    return upload(e, p->turns, turns, sizeof turns);
 }
 
 static void paged_release(spl_paged *p) {

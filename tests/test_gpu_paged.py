@@ -370,3 +370,25 @@ def test_a_new_object_rotates_by_its_own_table_at_once(engine):
         for got in q:
             assert ((got.double().cpu() - want).abs() <= e + half_step("bf16") * (want.abs() + e)).all()
         paged.close()
+
+
+def test_a_new_norm_weight_is_there_at_once(engine):
+    """Append on a stream that waits for nobody, right behind the weight's making."""
+    heads, dim = 1, 256
+    g = torch.Generator().manual_seed(41)
+    x = torch.randn((1, heads + 2, dim), generator=g).cuda()
+    k, v = (torch.zeros((1, 1, 16, dim), device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    stream, base = torch.cuda.Stream(), x.data_ptr()
+    paged = S.PagedAttention(engine, heads, 1, dim, 1, page_tokens=16, max_sequences=1, max_rows=1, max_context=16)
+    paged.batch([1], [1], np.zeros((1, 1), np.int32), stream=stream.cuda_stream)
+    for i in range(40):
+        weight = (1.0 + 0.2 * torch.randn(dim, generator=g)).to(torch.bfloat16)
+        q = torch.zeros((1, heads, dim), device="cuda", dtype=torch.bfloat16)
+        torch.cuda.synchronize()
+        norm = engine.tensor_vector(bf16_bits(weight))
+        paged.append(base, base + 4 * dim, base + 8 * dim, q.data_ptr(), k.data_ptr(), v.data_ptr(), ld=(heads + 2) * dim, q_norm=norm, k_norm=norm, stream=stream.cuda_stream)
+        torch.cuda.synchronize()
+        engine.tensor_destroy(norm)
+        want, e = expected_append(x[:, :heads].cpu(), torch.zeros(1), 0, 1.0, weight, engine.g.eps)
+        assert ((q.double().cpu() - want).abs() <= e + half_step("bf16") * (want.abs() + e)).all()
+    paged.close()
