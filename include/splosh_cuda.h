@@ -437,7 +437,7 @@ typedef struct spl_paged_config {
     int32_t max_sequences, max_rows, max_context;        /* of a batch; max_context tokens a sequence */
 } spl_paged_config;
 spl_status spl_paged_create(spl_engine *engine, const spl_paged_config *config, spl_paged **out);
-/* Waits for the device: calls may be queued on streams of the caller's. Destroy it before its engine. */
+/* Waits for the device: calls may be queued on streams of the caller's. The engine may be gone by then; every other call needs it. */
 void spl_paged_destroy(spl_paged *paged);
 /* Host arrays: rows[sequences], lengths[sequences] (new tokens included; rows[s] may be 0), page_table[sequences][table_ld] of which the
  * first ceil(lengths[s] / page_tokens) entries are read. Everything is checked here (SPL_ERR_INVALID_ROWS, SPL_ERR_CONTEXT_EXCEEDED; the batch set

@@ -19,6 +19,7 @@ typedef CUresult (*SplEncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_
 
 struct spl_paged {
     spl_engine *e = nullptr;
+    int device = 0;                    // the engine's (which may be gone when this object is destroyed)
     spl_paged_config c;
     SplPagedShape shape{};
     int max_pages = 0;
@@ -63,7 +64,6 @@ static spl_status paged_create(spl_engine *e, const spl_paged_config *cp, spl_pa
     const spl_paged_config &c = p->c = *cp;
     if (const char *wrong = spl_paged_config_error(c)) return e->fail(SPL_ERR_INVALID_ARGUMENT, std::string("spl_paged_create: ") + wrong);
     p->max_pages = (c.max_context + c.page_tokens - 1) / c.page_tokens;
-    p->e = e;
     p->shape = SplPagedShape{c.heads, c.kv_heads, c.heads / c.kv_heads, c.head_dim, c.page_tokens, p->max_pages, c.page_stride, c.head_stride, c.token_stride, c.rotary_dim, c.causal != 0, c.window,
                              c.scale > 0.0f ? c.scale : float(1.0 / std::sqrt(double(c.head_dim)))};
     const size_t blocks = size_t(e->sms), items = size_t(spl_paged_items_max(c, e->sms));
@@ -219,6 +219,7 @@ spl_status spl_paged_create(spl_engine *e, const spl_paged_config *config, spl_p
     spl_paged *p = nullptr;
     try {
         p = new spl_paged;
+        p->e = e; p->device = e->device;
         const spl_status s = paged_create(e, config, p);
         if (s != SPL_OK) { cudaGetLastError(); paged_release(p); return s; }
         *out = p;
@@ -231,7 +232,7 @@ spl_status spl_paged_create(spl_engine *e, const spl_paged_config *config, spl_p
 
 void spl_paged_destroy(spl_paged *p) {
     if (!p) return;
-    const SplDeviceScope scope(p->e->device);
+    const SplDeviceScope scope(p->device);
     cudaDeviceSynchronize();          // calls may be queued on streams of the caller's
     paged_release(p);
 }

@@ -79,9 +79,7 @@ class PagedAttention:
 
     def close(self):
         if getattr(self, "handle", None):
-            if self.engine.handle:
-                lib().spl_paged_destroy(self.handle)
-            self.handle = None
+            lib().spl_paged_destroy(self.handle); self.handle = None
 
     def __del__(self):
         self.close()

@@ -224,3 +224,18 @@ def test_the_callers_device_stays_current_and_a_closed_engine_is_refused():
     with pytest.raises(S.EngineError):
         paged.batch([1], [1], np.zeros((1, 1), np.int32))
     paged.close()
+
+
+def test_an_object_closed_behind_its_engine_gives_its_memory_back():
+    def once():
+        e = S.Engine(S.tiny_geometry(), S.EngineConfig(max_slots=1, max_rows=8, kv_pages=1, max_context=256))
+        paged = S.PagedAttention(e, 24, 4, 256, 2, page_tokens=16, max_sequences=8, max_rows=64, max_context=32)      # 39 MB of partial sums
+        e.close()
+        paged.close()
+    once()
+    torch.cuda.synchronize()
+    before = torch.cuda.mem_get_info()[0]
+    for _ in range(3):
+        once()
+    torch.cuda.synchronize()
+    assert before - torch.cuda.mem_get_info()[0] < 20e6
