@@ -392,3 +392,40 @@ def test_a_new_norm_weight_is_there_at_once(engine):
         want, e = expected_append(x[:, :heads].cpu(), torch.zeros(1), 0, 1.0, weight, engine.g.eps)
         assert ((q.double().cpu() - want).abs() <= e + half_step("bf16") * (want.abs() + e)).all()
     paged.close()
+
+
+@pytest.mark.parametrize("behind", ["attention", "sampling", "torch", "nothing"])
+def test_a_batch_set_on_another_stream_with_events_between(engine, behind):
+    """The batch's copies lie behind a long wait on a stream of their own; attention on another stream, behind an event and behind a kernel of that stream, goes by the new batch: its blocks read
+    their range, pages and first tiles ahead of the kernel in front of them, never ahead of the event."""
+    heads, kv_heads, dim, pages = 8, 2, 128, 48
+    scenes = [Scene(60 + i, heads, kv_heads, dim, [1, 2, 1], lengths, page_tokens=32, spare_pages=pages - sum(-(-n // 32) for n in lengths)) for i, lengths in enumerate(([300, 33, 500], [41, 600, 2]))]
+    def new():
+        return S.PagedAttention(engine, heads, kv_heads, dim, pages, page_tokens=32, scale=scenes[0].scale, max_sequences=3, max_rows=4, max_context=700)
+    paged, other = new(), new()
+    want = [attend(engine, scene, "f32", paged=paged) for scene in scenes]      # (both batches have been set once: all tables hold valid numbers)
+    other.batch(scenes[0].rows, scenes[0].lengths, scenes[0].table)
+    out, side = torch.zeros((20, 4, heads, dim), device="cuda"), torch.zeros((4, heads, dim), device="cuda")
+    uniform, ids = torch.full((4,), 0.5, device="cuda"), torch.zeros(4, dtype=torch.int32, device="cuda")
+    engine.pass_wait()
+    setting, running = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for n in range(20):
+        scene = scenes[n % 2]
+        with torch.cuda.stream(setting):
+            torch.cuda._sleep(400_000)
+        paged.batch(scene.rows, scene.lengths, scene.table, stream=setting.cuda_stream)
+        if behind == "attention":
+            other.attend(scenes[0].dq.data_ptr(), scenes[0].k.data_ptr(), scenes[0].v.data_ptr(), side.data_ptr(), out_dtype="f32", stream=running.cuda_stream)
+        elif behind == "sampling":
+            engine.pass_sample(side.data_ptr(), 4, heads * dim, heads * dim, ids.data_ptr(), uniform.data_ptr(), stream=running.cuda_stream)
+        elif behind == "torch":
+            with torch.cuda.stream(running):
+                side.add_(1.0)
+        running.wait_stream(setting)
+        paged.attend(scene.dq.data_ptr(), scene.k.data_ptr(), scene.v.data_ptr(), out[n].data_ptr(), out_dtype="f32", stream=running.cuda_stream)
+        setting.wait_stream(running)
+    torch.cuda.synchronize()
+    engine.pass_wait()
+    for n in range(20):
+        assert torch.equal(out[n], want[n % 2]), n
