@@ -19,6 +19,7 @@
 #include "spl_gdn_chunk.cuh"
 #include "spl_gemm_tc.cuh"
 #include "spl_gemm_narrow.cuh"
+#include "spl_sample.cuh"
 #include "spl_host.h"
 
 namespace {
@@ -78,6 +79,7 @@ struct spl_engine {
     int gdn_chunk_min = SPL_GDN_CHUNK_MIN;      // ordinary runs at least this long take the chunked gated-delta scan (spl_debug_gdn_chunk_min)
     int gguf_block_rows = 0;      // test switch (spl_debug_gguf_block_rows)
     int sms = 148;
+    const int *sample_clusters = nullptr;      // the sampling kernel's (configure_sampling)
     const int *clusters = nullptr;     // clusters of 1 ... SPL_NARROW_CLUSTER blocks of the narrow GEMM that are resident at a time (configure_device)
     int rows_padded = 0, logit_rows_padded = 0;
     int *tc_error = nullptr;
@@ -281,6 +283,31 @@ bool configure_device(int device, int *sms, const int **clusters) {
         done[device] = true;
     }
     *sms = count[device];
+    *clusters = resident[device];
+    return true;
+}
+
+// The sampling kernel's shared-memory opt-in, and the clusters of 1, 2, 4 and 8 of its blocks that are resident at a time; once per device and process.
+bool configure_sampling(int device, const int **clusters) {
+    static bool done[64] = {};
+    static int resident[64][SPL_SAMPLE_CLUSTER + 1] = {};
+    if (device < 0 || device >= 64) return false;
+    if (!done[device]) {
+        const int most = int(sizeof(SplSampleShared) + SPL_SAMPLE_STRETCH * 4);
+        cudaFuncSetAttribute(spl_sample_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+        cudaFuncSetAttribute(spl_sample_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(SplSampleShared)));
+        for (int s = 1; s <= SPL_SAMPLE_CLUSTER; s *= 2) {
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3(s); cfg.blockDim = dim3(1024); cfg.dynamicSmemBytes = most;
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim.x = s; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+            cfg.attrs = attr; cfg.numAttrs = 1;
+            if (cudaOccupancyMaxActiveClusters(&resident[device][s], spl_sample_kernel<true>, &cfg) != cudaSuccess) { resident[device][s] = 0; cudaGetLastError(); }
+        }
+        if (cudaGetLastError() != cudaSuccess || resident[device][1] < 1) return false;
+        done[device] = true;
+    }
     *clusters = resident[device];
     return true;
 }
@@ -853,6 +880,7 @@ spl_status create(const spl_geometry *gp, const spl_config *cp, spl_engine *e) {
     e->device = cp->device;
     SPL_CUDA(cudaSetDevice(e->device));
     if (!configure_device(e->device, &e->sms, &e->clusters)) return e->fail(SPL_ERR_UNSUPPORTED_DEVICE, "unsupported device: the kernels' shared-memory opt-in failed");
+    if (!configure_sampling(e->device, &e->sample_clusters)) return e->fail(SPL_ERR_UNSUPPORTED_DEVICE, "unsupported device: the sampling kernel's shared-memory opt-in failed");
     spl_status hs = spl_host_create(gp, cp, &e->host);
     if (hs != SPL_OK) return e->fail(hs, "invalid engine configuration");
     e->c = e->host->config;

@@ -184,7 +184,7 @@ static int sample_blocks(const spl_engine *e, int rows, int limit) {
     int best = 1;
     double least = 0.0;
     for (int blocks = 1; blocks <= SPL_SAMPLE_CLUSTER; blocks *= 2) {
-        const int resident = e->clusters[blocks];
+        const int resident = e->sample_clusters[blocks];
         if (resident < 1) continue;      // a size the device cannot hold
         const double cost = double((rows + resident - 1) / resident) * (14.0 + 19.0 * ((limit + blocks - 1) / blocks) / SPL_SAMPLE_STRETCH);
         if (blocks == 1 || cost < least) { best = blocks; least = cost; }
@@ -197,7 +197,6 @@ static spl_status launch_sample(spl_engine *e, const SplSampleArgs &args, int ro
     const bool held = blocks * SPL_SAMPLE_STRETCH >= args.limit;      // a block's share fits its shared memory
     void (*kernel)(SplSampleArgs) = held ? spl_sample_kernel<true> : spl_sample_kernel<false>;
     const size_t smem = sizeof(SplSampleShared) + (held ? size_t(((args.limit + blocks - 1) / blocks + 31) / 32 * 32) * 4 : 0);      // a block's stretch, as the kernel forms it
-    SPL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(SplSampleShared) + SPL_SAMPLE_STRETCH * 4)));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(blocks, rows); cfg.blockDim = dim3(1024); cfg.dynamicSmemBytes = smem; cfg.stream = stream;
     cudaLaunchAttribute attr[2];
