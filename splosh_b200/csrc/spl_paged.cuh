@@ -7,8 +7,7 @@
 //
 // Cache: element (page, kv head, token in page, channel) of K and of V lies at
 //   page * page_stride + head * head_stride + token * token_stride + channel     (16-bit elements)
-// A batch: sequence s has rows[s] new tokens, the last of its lengths[s]; row r of a pass belongs to sequence row_sequence[r] and
-// sits at position row_position[r]. Token t of sequence s is in page table[s * max_pages + t / page_tokens].
+// A batch: row r of a pass belongs to sequence row_sequence[r] and sits at position row_position[r], the last of its sequence's rows at the sequence's last token. Token t of sequence s is in page table[s * max_pages + t / page_tokens].
 #pragma once
 #include <cuda.h>
 
@@ -24,9 +23,8 @@ struct SplPagedShape {
 };
 // The batch as the kernels read it (device memory).
 struct SplPagedTables {
-    const int *counts;            // rows, sequences
+    const int *count;             // rows
     const int *row_sequence, *row_position;
-    const int *rows, *lengths;    // per sequence
     const int *table;             // [sequences][max_pages]
 };
 
@@ -64,7 +62,7 @@ spl_paged_append_kernel(SplPagedRows in, const uint16_t *__restrict__ q_norm, co
     __shared__ float2 vector[8][32 * J];
     spl_grid_begin();
     const int row = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = s.rotary / 2, vectors = s.heads + 2 * s.kv_heads;
-    const int rows = t.counts[0], sequence = t.row_sequence[row], position = t.row_position[row];
+    const int rows = *t.count, sequence = t.row_sequence[row], position = t.row_position[row];
     if (row >= rows) return;
     const int per = (vectors + gridDim.y - 1) / gridDim.y, begin = blockIdx.y * per + warp, last = min(vectors, int(blockIdx.y + 1) * per);
     // Where head n of the row's queries, keys and values begins, for this lane.
@@ -227,7 +225,6 @@ __device__ __forceinline__ void spl_tma_prefetch5(const CUtensorMap *map, int x,
 __device__ __forceinline__ uint64_t spl_tc_desc_mn_sw128(uint32_t smem_byte_addr, uint32_t block_bytes) {
     return (spl_tc_desc_sw128(smem_byte_addr) & ~(uint64_t(0x3FFF) << 16)) | uint64_t(block_bytes >> 4) << 16;
 }
-// A box of a tensor map into shared memory; the innermost coordinate is a multiple of 64 elements.
 // The two warps of 32 rows (w and w + 4): barriers 1 to 4.
 __device__ __forceinline__ void spl_paged_pair_barrier(int quarter) {
     if (quarter == 0) spl_named_barrier<1, 64>();

@@ -24,8 +24,8 @@ struct spl_paged {
     SplPagedShape shape{};
     int max_pages = 0;
     SplEncodeTiled encode = nullptr;
-    // Device tables in one block, filled from one of two pinned blocks (the other's copy may still be on its way): counts, block_begin, the pieces that have arrived of each merge
-    // (none), the blocks' first items, the batch's rows and lengths, the plan's items, the page table. Places do not depend on the batch, so a captured graph finds the next one's.
+    // Device tables in one block, filled from one of two pinned blocks (the other's copy may still be on its way): the row count, block_begin, the pieces that have arrived of each merge
+    // (none), the blocks' first items, the rows' sequences and positions, the plan's items, the page table. Places do not depend on the batch, so a captured graph finds the next one's.
     size_t words = 0, begin_at = 16, arrived_at = 0, starts_at = 0, batch_at = 0, items_at = 0, table_at = 0;
     SplPagedPlan plan;
     // Partial sums of query rows whose tokens several blocks share.
@@ -37,16 +37,15 @@ struct spl_paged {
     int turn = 0;
     double *turns = nullptr;
     // The batch that was set last.
-    int rows = 0, sequences = 0;
+    int rows = 0;
     bool ready = false, shared_write = false;
     std::vector<uint8_t> written;      // scratch of the check for pages that two sequences would write
 
     SplPagedTables tables() const {
         const int *t = tables_dev + batch_at;
         SplPagedTables out;
-        out.counts = tables_dev;
-        out.row_sequence = t; t += c.max_rows; out.row_position = t; t += c.max_rows;
-        out.rows = t; t += c.max_sequences; out.lengths = t;
+        out.count = tables_dev;
+        out.row_sequence = t; out.row_position = t + c.max_rows;
         out.table = tables_dev + table_at;
         return out;
     }
@@ -70,7 +69,7 @@ static spl_status paged_create(spl_engine *e, const spl_paged_config *cp, spl_pa
     p->arrived_at = p->begin_at + (blocks + 1 + 3) / 4 * 4;
     p->starts_at = p->arrived_at + (blocks + 3) / 4 * 4;
     p->batch_at = p->starts_at + blocks * (sizeof(SplPagedItem) / 4);
-    p->items_at = (p->batch_at + size_t(c.max_rows) * 2 + size_t(c.max_sequences) * 2 + 3) / 4 * 4;
+    p->items_at = (p->batch_at + size_t(c.max_rows) * 2 + 3) / 4 * 4;
     p->table_at = p->items_at + items * (sizeof(SplPagedItem) / 4);
     p->words = p->table_at + size_t(p->max_pages) * c.max_sequences;
     p->written.assign(size_t(c.pages), 0);
@@ -123,16 +122,15 @@ static spl_status paged_batch(spl_paged *p, int32_t sequences, const int32_t *ro
     SPL_CUDA(cudaEventSynchronize(p->copied[turn]));      // this block's last copy
     int *w = p->tables_host[turn];
     std::memset(w, 0, 16 * 4);
-    w[0] = int(total); w[1] = sequences;
+    w[0] = int(total);
     std::memcpy(w + p->begin_at, p->plan.block_begin.data(), p->plan.block_begin.size() * 4);
     std::memset(w + p->arrived_at, 0, size_t(e->sms) * 4);
     std::memcpy(w + p->starts_at, p->plan.starts.data(), p->plan.starts.size() * sizeof(SplPagedItem));
     std::memcpy(w + p->items_at, p->plan.items.data(), p->plan.items.size() * sizeof(SplPagedItem));
-    int *row_sequence = w + p->batch_at, *row_position = row_sequence + c.max_rows, *seq_rows = row_position + c.max_rows, *seq_lengths = seq_rows + c.max_sequences, *pages = w + p->table_at;
+    int *row_sequence = w + p->batch_at, *row_position = row_sequence + c.max_rows, *pages = w + p->table_at;
     int longest = 1;
     for (int s = 0, r = 0; s < sequences; ++s) {
         for (int i = 0; i < rows[s]; ++i, ++r) { row_sequence[r] = s; row_position[r] = lengths[s] - rows[s] + i; }
-        seq_rows[s] = rows[s]; seq_lengths[s] = lengths[s];
         const int used = (lengths[s] + c.page_tokens - 1) / c.page_tokens;
         if (used) std::memcpy(pages + size_t(s) * p->max_pages, table + size_t(s) * table_ld, size_t(used) * 4);
         longest = std::max(longest, used);
@@ -142,7 +140,7 @@ static spl_status paged_batch(spl_paged *p, int32_t sequences, const int32_t *ro
     SPL_CUDA(cudaMemcpy2DAsync(p->tables_dev + p->table_at, pitch, pages, pitch, size_t(longest) * 4, size_t(sequences), cudaMemcpyHostToDevice, stream));
     SPL_CUDA(cudaEventRecord(p->copied[turn], stream));
     p->turn ^= 1;
-    p->rows = int(total); p->sequences = sequences; p->shared_write = shared; p->ready = true;
+    p->rows = int(total); p->shared_write = shared; p->ready = true;
     return SPL_OK;
 }
 
