@@ -288,8 +288,10 @@ spl_status spl_topk(spl_engine *engine, int32_t vocab_limit, int32_t k, int32_t 
  * lower index first among equal ones; with w = exp((x - max x) / temperature) the first top_k stay (<= 0: all), of those the smallest
  * prefix whose w reaches top_p of their sum (>= 1: all), of those the ones with w >= min_p (<= 0: all; above 1 taken as 1), and the
  * token is the first whose running sum of w reaches uniform times the sum of what stays. temperature <= 0 takes the largest value.
- * NaN and -inf are never picked; a row without any other value gives id 0. Sums are formed so that the token is the definition's in
- * 64 bits and the same in every run. vocab_limit is at most 524,288. */
+ * NaN and -inf are never picked; a row without any other value gives id 0; beside an infinite value the finite ones have no weight. A weight
+ * is a whole number of 2^-44 of the largest (none where (max x - x) / temperature is above 31.2), and these are summed exactly: the token is the same in every run, and the
+ * definition's wherever no boundary between tokens is nearer than n 2^-45 of the largest weight over n values (2^-26 at most). Rows in which more than 4,096 values lie where a
+ * place has to be found (a 128th of a unit of x / temperature: nearly flat rows of a large vocabulary) are right, too, but take milliseconds. vocab_limit is at most 524,288. */
 typedef struct spl_sampling { float temperature; int32_t top_k; float top_p, min_p; } spl_sampling;
 spl_status spl_sample(spl_engine *engine, int32_t vocab_limit, const spl_sampling *settings, const float *uniform, int32_t *ids);
 spl_status spl_slot_reset(spl_engine *engine, int32_t slot);                                  /* Engine.resetSlot */
@@ -420,7 +422,7 @@ spl_status spl_pass_sample(spl_engine *engine, const float *device_logits, int32
  * Rows past the batch's are neither read nor written. `stream` is a cudaStream_t, null for the engine's stream (the
  * other spl_pass_ calls'); cudaStreamLegacy is the default stream. Calls on one spl_paged are ordered by the caller: one stream at a time, or events between
  * them. append and attend allocate nothing and may be captured into a graph; such a graph may be replayed after another spl_paged_batch of the same
- * rows per sequence (lengths and pages may differ). Two graphs, or two streams, that may run at the same time need a spl_paged each.
+ * rows per sequence (lengths and pages may differ; what append refuses, such a replay does not see: check the batch's pages with spl_paged_check). Two graphs, or two streams, that may run at the same time need a spl_paged each.
  * An attention block that gives up a wait is reported by the next spl_pass_wait (after the caller has synchronised its stream); the pass then begins anew with spl_paged_batch. */
 enum { SPL_F32 = 0, SPL_F16 = 1, SPL_BF16 = 2 };
 typedef struct spl_paged spl_paged;
@@ -452,7 +454,7 @@ spl_status spl_paged_append(spl_paged *paged, int32_t type, const void *device_q
 /* q [rows][heads][head_dim] of the cache's type; out the same shape, out_type SPL_F32 or the cache's type. Scores, softmax statistics and sums are fp32, a
  * probability is rounded to the cache's type before it meets the values. Buffers begin on 16-byte boundaries. What the cache holds behind a sequence's last token,
  * or in front of every row's window, may be anything. (Page table entries in front of a window still name pages of the cache.) A NaN or infinity among a token's
- * values reaches the rows that see the token, and may reach earlier rows of the same chunk of that sequence. */
+ * values reaches the rows that see the token, and may reach other rows of the same chunk of that sequence (earlier ones, and later ones whose window the token has left). */
 spl_status spl_paged_attend(spl_paged *paged, const void *device_q, const void *device_k_cache, const void *device_v_cache, int32_t out_type, void *device_out, void *stream);
 /* What spl_paged_create and spl_paged_batch would say, without an engine or a GPU (sequences 0: the configuration alone); the reason in
  * `message`. *shared_write (may be null): append would refuse the batch. */

@@ -373,7 +373,8 @@ __device__ __forceinline__ void spl_paged_join(const SplPagedShape &s, const Spl
     else spl_paged_join_sums<HD, BF16, 2, 6>(s, a, it, row0, head0, per_group, scratch);
 }
 
-// Tiles a block asks for while the kernel in front ends: 0, 1, 2, 3 and 4 take 32.1, 31.0, 30.7, 31.0 and 31.6 us for 12 rows over 3,000 tokens of 24/4 heads of 256.
+// Tiles a block asks for while the kernel in front ends: 0 and 2 take 24.7 and 23.4 us for eight blocks of 16 rows over a window of 2,048 tokens of 32/8 heads of 128. (12 rows over 3,000 tokens of
+// 24/4 heads of 256: 33.2 and 33.1 where every call has other data; 0 to 4 take 32.1, 31.0, 30.7, 31.0 and 31.6 where they have the same.)
 #define SPL_PAGED_EARLY 2
 template <int HD, bool BF16>
 __global__ void __launch_bounds__(SPL_PAGED_THREADS, 1)

@@ -176,7 +176,7 @@ template <int HD, bool BF16> static void launch_attend(const spl_paged *p, const
 
 // The blocks of a row's cluster: a wave of clusters costs some 14 us of meetings and sorting whatever a block's share, and 19 us for 32,768 values a block (they fit
 // its shared memory; a larger share is read from L2 in every pass, at the same pace). With top-p over 248,077 values, L2 flushed before each call, in blocks of 1, 2, 4
-// and 8: 12 rows take 158, 96, 65 and 45 us, 24 rows 158, 96, 65 and 82 (two waves of eights), 64 rows 180, 117, 125 and 190. Over 32,000, 151,936 and 248,077 values
+// and 8: 12 rows take 156, 94, 64 and 45 us, 24 rows 162, 98, 70 and 84 (two waves of eights), 64 rows 166, 107, 129 and 193. Over 32,000, 151,936 and 248,077 values
 // and 1 to 128 rows, with top-p and with top-k, the rule's choice was the fastest of the four to within 2 us.
 static int sample_blocks(const spl_engine *e, int rows, int limit) {
     int best = 1;

@@ -11,7 +11,7 @@
 //
 // The token has to be the definition's, so the sums have to be right where a boundary between tokens is close: 32-bit sums of a flat
 // vocabulary of 250K would pick another token in one row of fifty. Weights are formed in 64-bit floating point and summed as whole numbers of
-// 2^-44 (the largest is 2^44, 2^19 of them fit 64 bits): the sums do not depend on the order of the additions.
+// 2^-44 (the largest is 2^44, 2^19 of them fit 64 bits): the sums do not depend on the order of the additions, and over n values they are off by at most n 2^-45 of the largest weight.
 #pragma once
 #include <cooperative_groups.h>
 
@@ -60,13 +60,14 @@ __device__ __forceinline__ unsigned long long spl_sample_weight(float x, const S
 
 // A cluster of blocks a row, 32,768 values a block in shared memory (a vocabulary of more than eight blocks' is read anew in every pass): the row comes
 // from memory once. The histogram has 4,096 bins of 1/128 in (max - x) / T, so that bins hold a few hundred values where a vocabulary's are densest; what is
-// 31.98 and more below the maximum has no weight in whole numbers of 2^-44 and is the last bin. The first block of the cluster adds the blocks' bins, finds the bin
+// 31.98 and more below the maximum has no weight in whole numbers of 2^-44 and is the last bin (no place that matters lies there, and it is never set aside but in a list that it fits). The first block of the cluster adds the blocks' bins, finds the bin
 // that a place lies in, and sorts that bin's values, which the blocks have set aside:
 //   top-k         counts; the bins down to the k-th value's are sorted whole where they fit (SPL_SAMPLE_LIST), and everything else is decided on
 //                 that list; a larger k sorts its own bin alone and leaves a cut for what follows
 //   then          weights; the bins of top-p's place and of min-p's bound are sorted for the exact end of what stays, and then the draw's bin
-// A bin of more values than the list holds (equal logits, very high temperatures) leaves the row to the first block, which finds places eight bits of
-// the values' keys at a time (spl_sample_slow).
+// Where top-p's and min-p's bins and the draw's do not fit one list together, the draw's come in a turn of their own. Bins that do not fit alone (equal logits, very high temperatures: more than
+// 4,096 values in a 128th of a unit, or in the three at min-p's bound) leave the row to the first block, which finds places eight bits of the
+// values' keys at a time (spl_sample_slow): 12 rows of 248,077 at temperature 10,000 with top-p take 7.2 ms, at 10 still 0.09.
 #define SPL_SAMPLE_BINS 4096
 #define SPL_SAMPLE_BINS_NAT 128.0f             // bins a natural unit of (max - x) / T
 #define SPL_SAMPLE_SCALE_MAX 3.0e38f           // of a row's bin_scale, twice the bins a unit of max - x: at temperatures below 8.6e-37 bins are wider, and values of no weight lie in front of the last one, too
