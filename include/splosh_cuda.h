@@ -290,7 +290,7 @@ spl_status spl_topk(spl_engine *engine, int32_t vocab_limit, int32_t k, int32_t 
  * token is the first whose running sum of w reaches uniform times the sum of what stays. temperature <= 0 takes the largest value.
  * NaN and -inf are never picked; a row without any other value gives id 0; beside an infinite value the finite ones have no weight. A weight
  * is a whole number of 2^-44 of the largest (none where (max x - x) / temperature is above 31.2), and these are summed exactly: the token is the same in every run, and the
- * definition's wherever no boundary between tokens is nearer than n 2^-45 of the largest weight over n values (2^-26 at most). Rows in which more than 4,096 values lie where a
+ * definition's wherever no boundary between tokens (min_p's: a weight within 2^-45 of it) is nearer than n 2^-45 of the largest weight over n values (2^-26 at most). Rows in which more than 4,096 values lie where a
  * place has to be found (a 128th of a unit of x / temperature: nearly flat rows of a large vocabulary) are right, too, but take milliseconds. vocab_limit is at most 524,288. */
 typedef struct spl_sampling { float temperature; int32_t top_k; float top_p, min_p; } spl_sampling;
 spl_status spl_sample(spl_engine *engine, int32_t vocab_limit, const spl_sampling *settings, const float *uniform, int32_t *ids);
