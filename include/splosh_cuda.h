@@ -410,6 +410,20 @@ spl_status spl_pass_wait(spl_engine *engine);
 spl_status spl_pass_sample(spl_engine *engine, const float *device_logits, int32_t rows, int64_t ld, int32_t vocab_limit, const float *device_temperature,
                            const int32_t *device_top_k, const float *device_top_p, const float *device_min_p, const float *device_uniform, int32_t *device_ids, void *stream);
 
+/* SpeculativeSampling.resolve (Sampler.swift:163-179) on the device, for whole blocks of drafted tokens and over the whole of [0, vocab_limit): fp32 logits [rows][ld] of `sequences` sequences, sequence s's rows are
+ * [device_first[s], device_first[s + 1]) (device_first holds sequences + 1 numbers). device_drafts[rows]: the token drafted to follow a row, negative for none (a block's last row); candidates [rows][candidates] and
+ * probabilities [rows][candidates], at most 64 a row: what the drafter picked it from (spl_draft_propose's; finite, none negative; one listed twice counts as listed first, one that is not a token of the vocabulary not at all),
+ * with candidates 0 the token was its only choice (a continuation found in the text, or a greedy drafter's). Settings are one a row as spl_pass_sample's and make the target's distribution p: the weights of what stays over their sum;
+ * uniform [rows][2] in [0, 1).
+ *   ids[rows]       -1 where uniform[0] * q(draft) < p(draft), q the draft's probability (0 where it is not a candidate); otherwise the token that takes its place: spl_sample's draw with uniform[1], in its order, from
+ *                   max(p - q, 0) over the sum of that, or from p where nothing is left of it. A row without a draft draws from p.
+ *   accepted, next  [sequences] the rows in front of the sequence's first whose id is not -1, and that id (-1: all are)
+ * Every row is answered, those behind a refused token, too. What spl_sample says of weights, of NaN and infinities, of ties and of rows that take milliseconds holds here; q is rounded to whole units of 2^-44 of the
+ * largest weight, as p is. Queued on `stream`; may be captured. */
+spl_status spl_pass_verify(spl_engine *engine, const float *device_logits, int32_t sequences, int32_t rows, int64_t ld, int32_t vocab_limit, const int32_t *device_first, const int32_t *device_drafts, int32_t candidates,
+                           const int32_t *device_candidates, const float *device_probabilities, const float *device_temperature, const int32_t *device_top_k, const float *device_top_p, const float *device_min_p,
+                           const float *device_uniform, int32_t *device_ids, int32_t *device_accepted, int32_t *device_next, void *stream);
+
 /* ---- A paged cache of the caller's own --------------------------------------------------------
  * The attention of a pass over the caller's own tensors (DraftModel keeps a K/V store and an attention of its own beside the
  * engine's primitives, DraftModel.swift:418-468, Sources/Shaders/draft.metal:59-100): keys and values of any number of sequences in pages of
@@ -424,13 +438,13 @@ spl_status spl_pass_sample(spl_engine *engine, const float *device_logits, int32
  * them. append and attend allocate nothing and may be captured into a graph; such a graph may be replayed after another spl_paged_batch of the same
  * rows per sequence (lengths and pages may differ; what append refuses, such a replay does not see: check the batch's pages with spl_paged_check). Two graphs, or two streams, that may run at the same time need a spl_paged each.
  * An attention block that gives up a wait is reported by the next spl_pass_wait (after the caller has synchronised its stream); the pass then begins anew with spl_paged_batch. */
-enum { SPL_F32 = 0, SPL_F16 = 1, SPL_BF16 = 2 };
+enum { SPL_F32 = 0, SPL_F16 = 1, SPL_BF16 = 2, SPL_E4M3 = 3 };
 typedef struct spl_paged spl_paged;
 typedef struct spl_paged_config {
     int32_t heads, kv_heads, head_dim;                   /* head_dim 64, 128 or 256; heads a multiple of kv_heads, at most 64 times it */
-    int32_t dtype;                                       /* of cache and queries: SPL_F16 or SPL_BF16 */
+    int32_t dtype;                                       /* of cache and queries: SPL_F16 or SPL_BF16; SPL_E4M3: a cache of 8-bit codes with scales, queries in bf16 */
     int32_t page_tokens, pages;                          /* 16, 32, 64, 128 or 256 tokens a page; pages of the cache */
-    int64_t page_stride, head_stride, token_stride;      /* elements; [page][kv head][token][channel] or [page][token][kv head][channel], multiples of 8 */
+    int64_t page_stride, head_stride, token_stride;      /* elements; [page][kv head][token][channel] or [page][token][kv head][channel], multiples of 16 bytes */
     int32_t rotary_dim;                                  /* channels i and i + rotary_dim / 2 turn by position * rope_theta^(-2 i / rotary_dim) */
     float rope_theta;
     float scale;                                         /* of the scores; 0: 1 / sqrt(head_dim) */
@@ -456,15 +470,39 @@ spl_status spl_paged_append(spl_paged *paged, int32_t type, const void *device_q
  * or in front of every row's window, may be anything. (Page table entries in front of a window still name pages of the cache.) A NaN or infinity among a token's
  * values reaches the rows that see the token, and may reach other rows of the same chunk of that sequence (earlier ones, and later ones whose window the token has left). */
 spl_status spl_paged_attend(spl_paged *paged, const void *device_q, const void *device_k_cache, const void *device_v_cache, int32_t out_type, void *device_out, void *stream);
+/* A cache of SPL_E4M3: a token's keys of one kv head are head_dim codes times one scale, its values likewise, at half the memory and traffic of 16 bits. The scales are the caller's, fp32 [pages][kv_heads][page_tokens]
+ * for keys and for values, on 16-byte boundaries; they are not negative. append takes scale = max |y| / 448 over the head's channels (at least 2^-100) and code = y / scale to nearest even, y what spl_paged_append
+ * would round to 16 bits; a head that holds an infinity or NaN is NaN for whoever sees its token. attend's queries and 16-bit outputs are bf16, its scores q.k * scale and sums fp32; a probability times its token's value
+ * scale is rounded to fp16, relative to the row's largest such product. In all else they are spl_paged_append and spl_paged_attend, which refuse a cache with scales as these refuse one without. */
+spl_status spl_paged_append_scaled(spl_paged *paged, int32_t type, const void *device_q, int64_t q_ld, const void *device_k, int64_t k_ld, const void *device_v, int64_t v_ld, const spl_tensor *q_norm,
+                                   const spl_tensor *k_norm, void *device_q_out, void *device_k_cache, void *device_v_cache, float *device_k_scale, float *device_v_scale, void *stream);
+spl_status spl_paged_attend_scaled(spl_paged *paged, const void *device_q, const void *device_k_cache, const void *device_v_cache, const float *device_k_scale, const float *device_v_scale, int32_t out_type,
+                                   void *device_out, void *stream);
+/* spl_paged_batch for sequences that begin with the same tokens (a system prompt, continuations of one prompt): group g is the batch's next group_sequences[g] sequences, whose first group_tokens[g] tokens
+ * lie in the same pages (whole pages, in front of every member's new rows, the same entries of the page table; SPL_ERR_INVALID_ROWS otherwise). Sequences behind the last group share nothing. attend then reads
+ * the whole tiles of 128 tokens of a shared prefix once for up to 128 packed rows (a row's heads that share a kv head) of its group instead of once a sequence, where that saves more than the joining costs: without a window, for sequences of at most 128
+ * packed rows. The results are the same to the rounding of fp32 sums. The first call sets device memory aside for it (two partial sums a packed row); a graph captured before or after may be replayed after batches with
+ * groups and without. */
+spl_status spl_paged_batch_shared(spl_paged *paged, int32_t sequences, const int32_t *rows, const int32_t *lengths, const int32_t *page_table, int32_t table_ld, int32_t groups, const int32_t *group_sequences,
+                                  const int32_t *group_tokens, void *stream);
 /* What spl_paged_create and spl_paged_batch would say, without an engine or a GPU (sequences 0: the configuration alone); the reason in
  * `message`. *shared_write (may be null): append would refuse the batch. */
 spl_status spl_paged_check(const spl_paged_config *config, int32_t sequences, const int32_t *rows, const int32_t *lengths, const int32_t *page_table, int32_t table_ld, int32_t *shared_write,
                            char *message, size_t message_bytes);
+/* spl_paged_check for a batch with groups. */
+spl_status spl_paged_check_shared(const spl_paged_config *config, int32_t sequences, const int32_t *rows, const int32_t *lengths, const int32_t *page_table, int32_t table_ld, int32_t groups,
+                                  const int32_t *group_sequences, const int32_t *group_tokens, int32_t *shared_write, char *message, size_t message_bytes);
 /* Tests: how a batch's attention is dealt to `blocks` blocks. block_begin[blocks + 1]; items[][8]: sequence, its first row, kv head, first packed query row and their
  * count, first and last tile of 128 tokens, slot of partial sums (-1: none); merges[blocks][8]: first row, kv head, first packed query row, count, first slot,
  * slots. Host arithmetic, no device needed. */
 spl_status spl_debug_paged_plan(const spl_paged_config *config, int32_t blocks, int32_t sequences, const int32_t *rows, const int32_t *lengths, int32_t *block_begin, int32_t *items, int32_t items_capacity,
                                 int32_t *item_count, int32_t *merges, int32_t *merge_count);
+
+/* Tests: the same for a batch with groups. items as above, but a slot is the first of the piece's rows of partial sums; records[][10]: first row, first packed query row, kv head, count, and twice the first row of partial
+ * sums, the step from piece to piece and the pieces (of the joint rows over the prefix, and of the sequence's own). joint: some sequences meet their prefix together. */
+spl_status spl_debug_paged_plan_shared(const spl_paged_config *config, int32_t blocks, int32_t sequences, const int32_t *rows, const int32_t *lengths, int32_t groups, const int32_t *group_sequences,
+                                       const int32_t *group_tokens, int32_t *block_begin, int32_t *items, int32_t items_capacity, int32_t *item_count, int32_t *records, int32_t records_capacity,
+                                       int32_t *record_count, int64_t *partial_rows, int32_t *joint);
 
 /* ---- The DFlash 2 block-diffusion drafter (Sources/SploshRuntime/DraftModel.swift) -----------------
  * A draft pass proposes a whole block at once: [anchor, mask x (block - 1)] through a few non-causal layers that attend

@@ -294,8 +294,10 @@ bool configure_sampling(int device, const int **clusters) {
     if (device < 0 || device >= 64) return false;
     if (!done[device]) {
         const int most = int(sizeof(SplSampleShared) + SPL_SAMPLE_STRETCH * 4);
-        cudaFuncSetAttribute(spl_sample_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
-        cudaFuncSetAttribute(spl_sample_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(SplSampleShared)));
+        cudaFuncSetAttribute(spl_sample_kernel<true, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+        cudaFuncSetAttribute(spl_sample_kernel<false, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(SplSampleShared)));
+        cudaFuncSetAttribute(spl_sample_kernel<true, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(most + spl_verify_bytes()));
+        cudaFuncSetAttribute(spl_sample_kernel<false, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(SplSampleShared) + spl_verify_bytes()));
         for (int s = 1; s <= SPL_SAMPLE_CLUSTER; s *= 2) {
             cudaLaunchConfig_t cfg = {};
             cfg.gridDim = dim3(s); cfg.blockDim = dim3(1024); cfg.dynamicSmemBytes = most;
@@ -303,7 +305,7 @@ bool configure_sampling(int device, const int **clusters) {
             attr[0].id = cudaLaunchAttributeClusterDimension;
             attr[0].val.clusterDim.x = s; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
             cfg.attrs = attr; cfg.numAttrs = 1;
-            if (cudaOccupancyMaxActiveClusters(&resident[device][s], spl_sample_kernel<true>, &cfg) != cudaSuccess) { resident[device][s] = 0; cudaGetLastError(); }
+            if (cudaOccupancyMaxActiveClusters(&resident[device][s], spl_sample_kernel<true, false>, &cfg) != cudaSuccess) { resident[device][s] = 0; cudaGetLastError(); }
         }
         if (cudaGetLastError() != cudaSuccess || resident[device][1] < 1) return false;
         done[device] = true;

@@ -51,12 +51,25 @@ template <int TYPE> __device__ __forceinline__ float2 spl_load_pair(const void *
 // Grid (rows, head ranges), 256 threads: the angles' sines and cosines once a block, then a warp a head, a lane the channels 64 j + 2 lane and the next, the next head's on their way.
 // A channel's partner is in another register or lane where rotary / 2 is a power of two from 2 on, else it comes by way of shared memory. Bound: the instructions of a head, then HBM: 2,048
 // rows of 24/4 heads of 256 (101 MB) took 25 us at 320 instructions a head, 21 at 250, a block's start among them.
+//
+// A cache of e4m3 (CACHE_E4M3): a head's keys, and its values, of a token are codes times one scale, max |y| / 448 (448 is the largest code; at least 2^-100, so that a head of zeros divides
+// by something), code = y / scale rounded to nearest even. The scales are fp32 [page][kv head][token in page]. Queries are bf16.
 struct SplPagedRows { const void *q, *k, *v; long long q_ld, k_ld, v_ld; };
+struct SplPagedScales { float *k, *v; };
+#define SPL_SCALE_MIN 7.888609052210118e-31f      // 2^-100
+enum { SPL_CACHE_F16 = 0, SPL_CACHE_BF16, SPL_CACHE_E4M3 };
+__device__ __forceinline__ uint16_t spl_pack_e4m3(float lo, float hi) {
+    uint16_t v;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;\n" : "=h"(v) : "f"(hi), "f"(lo));
+    return v;
+}
 
-template <int TYPE, bool BF16, int HD>
+template <int TYPE, int CACHE, int HD>
 __global__ void __launch_bounds__(256, 5)
 spl_paged_append_kernel(SplPagedRows in, const uint16_t *__restrict__ q_norm, const uint16_t *__restrict__ k_norm, const double *__restrict__ turns,
-                        SplPagedTables t, SplPagedShape s, float eps, uint16_t *q_out, uint16_t *k_cache, uint16_t *v_cache) {
+                        SplPagedTables t, SplPagedShape s, float eps, uint16_t *q_out, void *k_cache, void *v_cache, SplPagedScales scales) {
+    constexpr bool BF16 = CACHE != SPL_CACHE_F16, E4M3 = CACHE == SPL_CACHE_E4M3;
+    constexpr int CELL = E4M3 ? 1 : 2;           // bytes an element of the cache
     constexpr int J = HD / 64, SIZE = TYPE == 0 ? 4 : 2;
     __shared__ __align__(16) float2 turn[128];   // (cos, sin) of channel pair i
     __shared__ float2 vector[8][32 * J];
@@ -86,12 +99,14 @@ spl_paged_append_kernel(SplPagedRows in, const uint16_t *__restrict__ q_norm, co
     __syncthreads();
     const bool square = (half & (half - 1)) == 0 && half > 1;
     const size_t place = size_t(page) * s.page_stride + size_t(position % s.page_tokens) * s.token_stride + 2 * lane;
-    uint16_t *q_to = q_out + size_t(row) * s.heads * HD + 2 * lane, *k_to = k_cache + place, *v_to = v_cache + place;
+    uint16_t *q_to = q_out + size_t(row) * s.heads * HD + 2 * lane;
+    char *k_to = static_cast<char *>(k_cache) + place * CELL, *v_to = static_cast<char *>(v_cache) + place * CELL;
+    const size_t scale_place = size_t(page) * s.kv_heads * s.page_tokens + position % s.page_tokens;
     const uint16_t *held = nullptr;              // the weight in registers: a warp's queries come first, then its keys
     float2 w[J];
     for (int n = begin; n < last; n += 8) {
         const int k = n - s.heads, v = k - s.kv_heads;
-        uint16_t *dst = k < 0 ? q_to + n * HD : v < 0 ? k_to + size_t(k) * s.head_stride : v_to + size_t(v) * s.head_stride;
+        char *dst = k < 0 ? reinterpret_cast<char *>(q_to + n * HD) : v < 0 ? k_to + size_t(k) * s.head_stride * CELL : v_to + size_t(v) * s.head_stride * CELL;
         float2 x[J];
 #pragma unroll
         for (int j = 0; j < J; ++j) x[j] = ahead[j];
@@ -142,8 +157,18 @@ spl_paged_append_kernel(SplPagedRows in, const uint16_t *__restrict__ q_norm, co
                 for (int j = 0; j < J; ++j) x[j] = make_float2(turned(64 * j + 2 * lane, x[j].x), turned(64 * j + 2 * lane + 1, x[j].y));
             }
         }
+        if (E4M3 && k >= 0) {
+            float most = 0.0f;
 #pragma unroll
-        for (int j = 0; j < J; ++j) *reinterpret_cast<uint32_t *>(dst + 64 * j) = spl_pack16<BF16>(x[j].x, x[j].y);
+            for (int j = 0; j < J; ++j) most = fmaxf(most, fmaxf(fabsf(x[j].x), fabsf(x[j].y)));
+            const float scale = fmaxf(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most))) * (1.0f / 448.0f), SPL_SCALE_MIN), inv = 1.0f / scale;      // (numbers of one sign order as their bits do)
+            if (lane == 0) (v < 0 ? scales.k : scales.v)[scale_place + size_t(v < 0 ? k : v) * s.page_tokens] = scale;
+#pragma unroll
+            for (int j = 0; j < J; ++j) *reinterpret_cast<uint16_t *>(dst + 64 * j) = spl_pack_e4m3(x[j].x * inv, x[j].y * inv);
+            continue;
+        }
+#pragma unroll
+        for (int j = 0; j < J; ++j) *reinterpret_cast<uint32_t *>(dst + 128 * j) = spl_pack16<BF16>(x[j].x, x[j].y);
     }
 }
 
@@ -714,7 +739,7 @@ spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
                 spl_tc_fence_before();
                 spl_paged_pair_barrier(quarter);              // the sums in shared memory are read before the next piece's
             }
-            if (it.slot >= 0) {
+            if (it.merge >= 0) {
                 // Whichever block is the last to leave a piece of these rows joins them, in the order of the pieces whoever it is.
                 __threadfence();
                 spl_named_barrier<5, 256>();
@@ -737,4 +762,71 @@ spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
     __syncthreads();
     spl_tc_fence_after();
     if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512) : "memory");
+}
+
+// ---- the pieces of a shared batch joined ----------------------------------------------------------
+// o = sum_n 2^(m_n - m) O_n / sum_n 2^(m_n - m) l_n over the pieces of a row: those of the prefix that its sequences met together, and those of its own tokens. A piece of the prefix
+// holds rows of many sequences, so no block of the attention is the last of all that a row waits for; here the rows are dealt to warps, whoever's they are.
+// A warp a row and 128 channels (64 of a head of 64): lane n looks up piece n's sums for all. Bound: L2, what the attention just left there.
+struct SplPagedCombine {
+    const int *work_count; const int2 *work;         // (record, its first of four (row, channels))
+    const SplPagedRecord *records;
+    const float *partial; const float2 *partial_ml;
+    void *out; int out_f32;
+};
+template <int HD, bool BF16>
+__global__ void __launch_bounds__(128)
+spl_paged_combine_kernel(SplPagedCombine a, SplPagedShape s) {
+    constexpr int CHUNKS = (HD + 127) / 128, VEC = HD / CHUNKS / 32;      // channels a lane
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, count = __ldg(a.work_count);
+    bool waited = false;
+    for (int w = blockIdx.x; w < count; w += gridDim.x) {
+        const int2 work = __ldg(a.work + w);
+        const SplPagedRecord rec = a.records[work.x];
+        if (!waited) { spl_grid_begin(); waited = true; }                  // (the tables were copied in front of the attention)
+        const int job = work.y + warp, r = job / CHUNKS, pieces = rec.a_pieces + rec.b_pieces;
+        if (r >= rec.count) continue;
+        const int channel = job % CHUNKS * 128 + VEC * lane;
+        float acc[VEC], m = -INFINITY, sum = 0.0f;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) acc[e] = 0.0f;
+        for (int n0 = 0; n0 < pieces; n0 += 32) {
+            const int n = n0 + lane;
+            const int at = (n < rec.a_pieces ? rec.a_first + n * rec.a_step : rec.b_first + (n - rec.a_pieces) * rec.b_step) + r;
+            const float2 ml = n < pieces ? __ldcg(a.partial_ml + at) : make_float2(-INFINITY, 0.0f);
+            const float now = fmaxf(m, spl_warp_max(ml.x));
+            if (now == -INFINITY) continue;
+            const float f = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - now), old = exp2f(m - now);      // (a piece of whose tokens this row sees none)
+            sum = sum * old + f * ml.y;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) acc[e] *= old;
+            m = now;
+            const int here = min(32, pieces - n0);
+            for (int u0 = 0; u0 < here; u0 += 8) {                         // eight on their way
+                float v[8][VEC];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    const float *from = a.partial + size_t(__shfl_sync(0xffffffffu, at, min(u0 + u, here - 1))) * HD + channel;
+                    if constexpr (VEC == 4) { const float4 x = __ldcg(reinterpret_cast<const float4 *>(from)); v[u][0] = x.x; v[u][1] = x.y; v[u][2] = x.z; v[u][3] = x.w; }
+                    else { const float2 x = __ldcg(reinterpret_cast<const float2 *>(from)); v[u][0] = x.x; v[u][1] = x.y; }
+                }
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    const float g = __shfl_sync(0xffffffffu, f, min(u0 + u, here - 1));
+                    if (u0 + u >= here || g == 0.0f) continue;
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) acc[e] += g * v[u][e];
+                }
+            }
+        }
+        const float inv = 1.0f / spl_warp_sum(sum);
+        const int x = rec.q0 + r, row = x / s.group;
+        const size_t place = (size_t(rec.row0 + row) * s.heads + rec.kv_head * s.group + x - row * s.group) * HD + channel;
+#pragma unroll
+        for (int e = 0; e < VEC; e += 2) {
+            if (a.out_f32) *reinterpret_cast<float2 *>(static_cast<float *>(a.out) + place + e) = make_float2(acc[e] * inv, acc[e + 1] * inv);
+            else *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(a.out) + place + e) = spl_pack16<BF16>(acc[e] * inv, acc[e + 1] * inv);
+        }
+    }
+    if (!waited) spl_grid_begin();
 }

@@ -5,6 +5,7 @@
 #include <new>
 
 #include "spl_paged.cuh"
+#include "spl_paged_e4m3.cuh"
 #include "spl_sample.cuh"
 
 // A call leaves the calling thread's current device as it was.
@@ -26,7 +27,7 @@ struct spl_paged {
     SplEncodeTiled encode = nullptr;
     // Device tables in one block, filled from one of two pinned blocks (the other's copy may still be on its way): the row count, block_begin, the pieces that have arrived of each merge
     // (none), the blocks' first items, the rows' sequences and positions, the plan's items, the page table. Places do not depend on the batch, so a captured graph finds the next one's.
-    size_t words = 0, begin_at = 16, arrived_at = 0, starts_at = 0, batch_at = 0, items_at = 0, table_at = 0;
+    size_t words = 0, begin_at = 16, arrived_at = 0, starts_at = 0, batch_at = 0, lengths_at = 0, items_at = 0, table_at = 0;
     SplPagedPlan plan;
     // Partial sums of query rows whose tokens several blocks share.
     int slot_rows = 0;
@@ -36,9 +37,18 @@ struct spl_paged {
     cudaEvent_t copied[2] = {};
     int turn = 0;
     double *turns = nullptr;
+    // What a batch with groups is dealt by, made by the first of them, and from then on filled by every batch (a captured graph may hold either form): the count of joining work, the
+    // plan's block_begin, starts and items, the records, the work. Partial sums by the row.
+    struct Shared {
+        size_t words = 0, begin_at = 16, starts_at = 0, items_at = 0, records_at = 0, work_at = 0;
+        int *dev = nullptr, *host[2] = {};
+        float *partial = nullptr;
+        float2 *partial_ml = nullptr;
+        SplPagedPlan plan;
+    } shared;
     // The batch that was set last.
-    int rows = 0;
-    bool ready = false, shared_write = false;
+    int rows = 0, combine_work = 0;
+    bool ready = false, shared_write = false, joint = false;
     std::vector<uint8_t> written;      // scratch of the check for pages that two sequences would write
 
     SplPagedTables tables() const {
@@ -69,7 +79,8 @@ static spl_status paged_create(spl_engine *e, const spl_paged_config *cp, spl_pa
     p->arrived_at = p->begin_at + (blocks + 1 + 3) / 4 * 4;
     p->starts_at = p->arrived_at + (blocks + 3) / 4 * 4;
     p->batch_at = p->starts_at + blocks * (sizeof(SplPagedItem) / 4);
-    p->items_at = (p->batch_at + size_t(c.max_rows) * 2 + 3) / 4 * 4;
+    p->lengths_at = p->batch_at + size_t(c.max_rows) * 2;
+    p->items_at = (p->lengths_at + size_t(c.max_sequences) + 3) / 4 * 4;
     p->table_at = p->items_at + items * (sizeof(SplPagedItem) / 4);
     p->words = p->table_at + size_t(p->max_pages) * c.max_sequences;
     p->written.assign(size_t(c.pages), 0);
@@ -97,7 +108,8 @@ static spl_status paged_create(spl_engine *e, const spl_paged_config *cp, spl_pa
 }
 
 static void paged_release(spl_paged *p) {
-    cudaFree(p->tables_dev);
+    cudaFree(p->tables_dev); cudaFree(p->shared.dev);
+    if (p->shared.host[0]) cudaFreeHost(p->shared.host[0]);
     if (p->tables_host[0]) cudaFreeHost(p->tables_host[0]);
     for (cudaEvent_t event : p->copied) if (event) cudaEventDestroy(event);
     delete p;
@@ -105,7 +117,50 @@ static void paged_release(spl_paged *p) {
 
 static cudaStream_t paged_stream(const spl_engine *e, void *stream) { return stream ? static_cast<cudaStream_t>(stream) : e->stream; }
 
-static spl_status paged_batch(spl_paged *p, int32_t sequences, const int32_t *rows, const int32_t *lengths, const int32_t *table, int32_t table_ld, cudaStream_t stream) {
+// The device and pinned memory of batches with groups.
+static spl_status paged_shared_create(spl_paged *p) {
+    spl_engine *e = p->e;
+    spl_paged::Shared &sh = p->shared;
+    if (sh.dev) return SPL_OK;
+    const size_t blocks = size_t(e->sms), item = sizeof(SplPagedItem) / 4;
+    sh.starts_at = sh.begin_at + (blocks + 1 + 3) / 4 * 4;
+    sh.items_at = sh.starts_at + blocks * item;
+    sh.records_at = sh.items_at + size_t(spl_paged_shared_items_max(p->c, e->sms)) * item;
+    sh.work_at = sh.records_at + size_t(spl_paged_records_max(p->c, e->sms)) * (sizeof(SplPagedRecord) / 4);
+    sh.words = sh.work_at + size_t(spl_paged_combine_max(p->c, e->sms)) * 2;
+    const size_t table_bytes = (sh.words * 4 + 255) / 256 * 256, partial_rows = size_t(spl_paged_partial_rows_max(p->c, e->sms));
+    int *host = nullptr;
+    SPL_CUDA(cudaMallocHost(reinterpret_cast<void **>(&host), sh.words * 8));
+    unsigned char *block = nullptr;
+    const cudaError_t made = cudaMalloc(reinterpret_cast<void **>(&block), table_bytes + partial_rows * (size_t(p->c.head_dim) * 4 + sizeof(float2)));
+    if (made != cudaSuccess) { cudaFreeHost(host); SPL_CUDA(made); }
+    sh.host[0] = host; sh.host[1] = host + sh.words;
+    sh.partial = reinterpret_cast<float *>(block + table_bytes);
+    sh.partial_ml = reinterpret_cast<float2 *>(sh.partial + partial_rows * p->c.head_dim);
+    sh.dev = reinterpret_cast<int *>(block);
+    return SPL_OK;
+}
+
+// The plan with groups, in the words of pinned block `turn`: how many are used.
+static size_t paged_shared_fill(spl_paged *p, int turn, int32_t sequences, const int32_t *rows, const int32_t *lengths, const SplPagedGroups &groups) {
+    spl_paged::Shared &sh = p->shared;
+    const SplPagedPlan &plan = sh.plan;
+    spl_paged_plan(p->c, p->e->sms, sequences, rows, lengths, sh.plan, &groups);
+    int *w = sh.host[turn], work = 0;
+    std::memcpy(w + sh.begin_at, plan.block_begin.data(), plan.block_begin.size() * 4);
+    std::memcpy(w + sh.starts_at, plan.starts.data(), plan.starts.size() * sizeof(SplPagedItem));
+    std::memcpy(w + sh.items_at, plan.items.data(), plan.items.size() * sizeof(SplPagedItem));
+    std::memcpy(w + sh.records_at, plan.records.data(), plan.records.size() * sizeof(SplPagedRecord));
+    const int chunks = (p->c.head_dim + 127) / 128;
+    for (size_t r = 0; r < plan.records.size(); ++r)
+        for (int job = 0; job < plan.records[r].count * chunks; job += 4, ++work) { w[sh.work_at + 2 * work] = int(r); w[sh.work_at + 2 * work + 1] = job; }
+    std::memset(w, 0, 16 * 4);
+    w[0] = work;
+    p->combine_work = work;
+    return sh.work_at + 2 * size_t(work);
+}
+
+static spl_status paged_batch(spl_paged *p, int32_t sequences, const int32_t *rows, const int32_t *lengths, const int32_t *table, int32_t table_ld, const SplPagedGroups &groups, cudaStream_t stream) {
     spl_engine *e = p->e;
     const spl_paged_config &c = p->c;
     std::string why;
@@ -115,6 +170,11 @@ static spl_status paged_batch(spl_paged *p, int32_t sequences, const int32_t *ro
     cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
     SPL_CUDA(cudaStreamIsCapturing(stream, &capture));
     if (capture != cudaStreamCaptureStatusNone) return e->fail(SPL_ERR_INVALID_ARGUMENT, "spl_paged_batch: a batch is set outside a capture");
+    if (groups.count) {
+        if (!spl_paged_groups_check(c, sequences, rows, lengths, table, table_ld, groups, &why)) return e->fail(SPL_ERR_INVALID_ROWS, "spl_paged_batch_shared: " + why);
+        const spl_status made = paged_shared_create(p);
+        if (made != SPL_OK) { cudaGetLastError(); return made; }
+    }
     int64_t total = 0;
     for (int s = 0; s < sequences; ++s) total += rows[s];
     spl_paged_plan(c, e->sms, sequences, rows, lengths, p->plan);
@@ -129,6 +189,7 @@ static spl_status paged_batch(spl_paged *p, int32_t sequences, const int32_t *ro
     std::memcpy(w + p->items_at, p->plan.items.data(), p->plan.items.size() * sizeof(SplPagedItem));
     int *row_sequence = w + p->batch_at, *row_position = row_sequence + c.max_rows, *pages = w + p->table_at;
     int longest = 1;
+    std::memcpy(w + p->lengths_at, lengths, size_t(sequences) * 4);
     for (int s = 0, r = 0; s < sequences; ++s) {
         for (int i = 0; i < rows[s]; ++i, ++r) { row_sequence[r] = s; row_position[r] = lengths[s] - rows[s] + i; }
         const int used = (lengths[s] + c.page_tokens - 1) / c.page_tokens;
@@ -138,23 +199,29 @@ static spl_status paged_batch(spl_paged *p, int32_t sequences, const int32_t *ro
     const size_t planned = p->items_at + p->plan.items.size() * (sizeof(SplPagedItem) / 4), pitch = size_t(p->max_pages) * 4;
     SPL_CUDA(cudaMemcpyAsync(p->tables_dev, w, planned * 4, cudaMemcpyHostToDevice, stream));
     SPL_CUDA(cudaMemcpy2DAsync(p->tables_dev + p->table_at, pitch, pages, pitch, size_t(longest) * 4, size_t(sequences), cudaMemcpyHostToDevice, stream));
+    if (p->shared.dev) {
+        const size_t used = paged_shared_fill(p, turn, sequences, rows, lengths, groups);
+        SPL_CUDA(cudaMemcpyAsync(p->shared.dev, p->shared.host[turn], used * 4, cudaMemcpyHostToDevice, stream));
+    }
+    p->joint = p->shared.dev && p->shared.plan.joint;
     SPL_CUDA(cudaEventRecord(p->copied[turn], stream));
     p->turn ^= 1;
     p->rows = int(total); p->shared_write = shared; p->ready = true;
     return SPL_OK;
 }
 
-template <int TYPE, int HD> static void launch_append_dim(const spl_paged *p, const SplPagedRows &in, const uint16_t *q_norm, const uint16_t *k_norm, uint16_t *q, uint16_t *k, uint16_t *v, cudaStream_t stream) {
+struct SplPagedOut { uint16_t *q; void *k, *v; SplPagedScales scales; };
+template <int TYPE, int HD> static void launch_append_dim(const spl_paged *p, const SplPagedRows &in, const uint16_t *q_norm, const uint16_t *k_norm, const SplPagedOut &out, cudaStream_t stream) {
     // A warp a head of a row; few rows are spread over more blocks.
     const int vectors = p->c.heads + 2 * p->c.kv_heads, most = (vectors + 7) / 8;
     const dim3 grid(p->rows, std::max(1, std::min(most, (2 * p->e->sms + p->rows - 1) / p->rows)));
-    launch_step(p->c.dtype == SPL_BF16 ? spl_paged_append_kernel<TYPE, true, HD> : spl_paged_append_kernel<TYPE, false, HD>, grid, dim3(256), 0, stream, in, q_norm, k_norm, (const double *)p->turns,
-                p->tables(), p->shape, p->e->g.eps, q, k, v);
+    launch_step(p->c.dtype == SPL_E4M3 ? spl_paged_append_kernel<TYPE, SPL_CACHE_E4M3, HD> : p->c.dtype == SPL_BF16 ? spl_paged_append_kernel<TYPE, SPL_CACHE_BF16, HD> : spl_paged_append_kernel<TYPE, SPL_CACHE_F16, HD>,
+                grid, dim3(256), 0, stream, in, q_norm, k_norm, (const double *)p->turns, p->tables(), p->shape, p->e->g.eps, out.q, out.k, out.v, out.scales);
 }
-template <int TYPE> static void launch_append(const spl_paged *p, const SplPagedRows &in, const uint16_t *q_norm, const uint16_t *k_norm, uint16_t *q, uint16_t *k, uint16_t *v, cudaStream_t stream) {
-    if (p->c.head_dim == 64) launch_append_dim<TYPE, 64>(p, in, q_norm, k_norm, q, k, v, stream);
-    else if (p->c.head_dim == 128) launch_append_dim<TYPE, 128>(p, in, q_norm, k_norm, q, k, v, stream);
-    else launch_append_dim<TYPE, 256>(p, in, q_norm, k_norm, q, k, v, stream);
+template <int TYPE> static void launch_append(const spl_paged *p, const SplPagedRows &in, const uint16_t *q_norm, const uint16_t *k_norm, const SplPagedOut &out, cudaStream_t stream) {
+    if (p->c.head_dim == 64) launch_append_dim<TYPE, 64>(p, in, q_norm, k_norm, out, stream);
+    else if (p->c.head_dim == 128) launch_append_dim<TYPE, 128>(p, in, q_norm, k_norm, out, stream);
+    else launch_append_dim<TYPE, 256>(p, in, q_norm, k_norm, out, stream);
 }
 
 // The cache as a tensor (channel in block, token in page, block of 64 channels, kv head, page) for the copies of values, in boxes of all channels by a page's tokens (at most a
@@ -190,11 +257,11 @@ static int sample_blocks(const spl_engine *e, int rows, int limit) {
     return best;
 }
 
-static spl_status launch_sample(spl_engine *e, const SplSampleArgs &args, int rows, cudaStream_t stream) {
+static spl_status launch_sample(spl_engine *e, const SplSampleArgs &args, int rows, cudaStream_t stream, bool verify = false) {
     const int blocks = sample_blocks(e, rows, args.limit);
     const bool held = blocks * SPL_SAMPLE_STRETCH >= args.limit;      // a block's share fits its shared memory
-    void (*kernel)(SplSampleArgs) = held ? spl_sample_kernel<true> : spl_sample_kernel<false>;
-    const size_t smem = sizeof(SplSampleShared) + (held ? size_t(((args.limit + blocks - 1) / blocks + 31) / 32 * 32) * 4 : 0);      // a block's stretch, as the kernel forms it
+    void (*kernel)(SplSampleArgs) = verify ? (held ? spl_sample_kernel<true, true> : spl_sample_kernel<false, true>) : held ? spl_sample_kernel<true, false> : spl_sample_kernel<false, false>;
+    const size_t smem = sizeof(SplSampleShared) + (verify ? spl_verify_bytes() : 0) + (held ? size_t(((args.limit + blocks - 1) / blocks + 31) / 32 * 32) * 4 : 0);      // a block's stretch, as the kernel forms it
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(blocks, rows); cfg.blockDim = dim3(1024); cfg.dynamicSmemBytes = smem; cfg.stream = stream;
     cudaLaunchAttribute attr[2];
@@ -205,7 +272,84 @@ static spl_status launch_sample(spl_engine *e, const SplSampleArgs &args, int ro
     return check_launch(e, "sampling");
 }
 
+// Four warps a block; a graph's replay may have other work than the batch it was captured with, so the blocks go round.
+static void launch_combine(const spl_paged *p, const SplPagedCombine &j, cudaStream_t stream) {
+    const dim3 grid(std::max(1, std::min(p->combine_work, 4 * p->e->sms)));
+    const int hd = p->c.head_dim;
+    const bool bf16 = p->c.dtype != SPL_F16;
+    launch_step(hd == 64 ? (bf16 ? spl_paged_combine_kernel<64, true> : spl_paged_combine_kernel<64, false>) : hd == 128 ? (bf16 ? spl_paged_combine_kernel<128, true> : spl_paged_combine_kernel<128, false>) :
+                (bf16 ? spl_paged_combine_kernel<256, true> : spl_paged_combine_kernel<256, false>), grid, dim3(128), 0, stream, j, p->shape);
+}
+
 static bool misaligned(const void *p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes != 0; }
+
+static spl_status paged_append(spl_paged *p, const char *name, bool scaled, int32_t type, const void *device_q, int64_t q_ld, const void *device_k, int64_t k_ld, const void *device_v, int64_t v_ld,
+                               const spl_tensor *q_norm, const spl_tensor *k_norm, const SplPagedOut &out, void *stream) {
+    if (!device_q || !device_k || !device_v || !out.q || !out.k || !out.v) return SPL_ERR_INVALID_ARGUMENT;
+    spl_engine *e = p->e;
+    SPL_NOT_IN_FLIGHT(e);
+    const spl_paged_config &c = p->c;
+    auto refuse = [&](const char *text) { return e->fail(SPL_ERR_INVALID_ARGUMENT, std::string(name) + text); };
+    if (scaled != (c.dtype == SPL_E4M3)) return refuse(scaled ? "the cache has no scales" : "the cache has scales");
+    if (!p->ready) return refuse("no batch is set");
+    if (p->shared_write) return refuse("two sequences of the batch would write to one page");
+    if (type != SPL_F32 && type != SPL_F16 && type != SPL_BF16) return refuse("rows are fp32, fp16 or bf16");
+    const int64_t q_width = int64_t(c.heads) * c.head_dim, kv_width = int64_t(c.kv_heads) * c.head_dim;
+    if (q_ld < q_width || k_ld < kv_width || v_ld < kv_width || q_ld % 2 || k_ld % 2 || v_ld % 2) return refuse("row strides must be even and hold the heads");
+    const size_t pair = type == SPL_F32 ? 8 : 4;
+    if (misaligned(device_q, pair) || misaligned(device_k, pair) || misaligned(device_v, pair)) return refuse("rows begin on a boundary of two elements");
+    if (misaligned(out.q, 16) || misaligned(out.k, 16) || misaligned(out.v, 16)) return refuse("queries and cache begin on a 16-byte boundary");
+    if (misaligned(out.scales.k, 16) || misaligned(out.scales.v, 16)) return refuse("scales begin on a 16-byte boundary");
+    if ((q_norm && (!q_norm->vec || q_norm->count != c.head_dim)) || (k_norm && (!k_norm->vec || k_norm->count != c.head_dim))) return refuse("a norm weight is a vector of head_dim elements");
+    const SplDeviceScope scope(e->device);
+    const SplPagedRows in{device_q, device_k, device_v, q_ld, k_ld, v_ld};
+    const uint16_t *qw = q_norm ? q_norm->vec : nullptr, *kw = k_norm ? k_norm->vec : nullptr;
+    if (type == SPL_F32) launch_append<0>(p, in, qw, kw, out, paged_stream(e, stream));
+    else if (type == SPL_F16) launch_append<1>(p, in, qw, kw, out, paged_stream(e, stream));
+    else launch_append<2>(p, in, qw, kw, out, paged_stream(e, stream));
+    return check_launch(e, "spl_paged_append");
+}
+
+static spl_status paged_attend(spl_paged *p, const char *name, bool scaled, const void *device_q, const void *device_k_cache, const void *device_v_cache, const float *k_scale, const float *v_scale,
+                               int32_t out_type, void *device_out, void *stream) {
+    if (!device_q || !device_k_cache || !device_v_cache || !device_out) return SPL_ERR_INVALID_ARGUMENT;
+    spl_engine *e = p->e;
+    SPL_NOT_IN_FLIGHT(e);
+    const spl_paged_config &c = p->c;
+    auto refuse = [&](const char *text) { return e->fail(SPL_ERR_INVALID_ARGUMENT, std::string(name) + text); };
+    if (scaled != (c.dtype == SPL_E4M3)) return refuse(scaled ? "the cache has no scales" : "the cache has scales");
+    if (!p->ready) return refuse("no batch is set");
+    const int own_type = scaled ? SPL_BF16 : c.dtype;
+    if (out_type != SPL_F32 && out_type != own_type) return refuse("outputs are fp32 or of the queries' type");
+    if (misaligned(device_q, 16) || misaligned(device_k_cache, 16) || misaligned(device_v_cache, 16) || misaligned(device_out, 16)) return refuse("all buffers begin on a 16-byte boundary");
+    if (misaligned(k_scale, 16) || misaligned(v_scale, 16)) return refuse("scales begin on a 16-byte boundary");
+    const SplDeviceScope scope(e->device);
+    cudaStream_t st = paged_stream(e, stream);
+    // A batch whose sequences meet a prefix together has tables, partial sums by the row and a joining kernel of its own.
+    const spl_paged::Shared &sh = p->shared;
+    const bool joint = p->joint;
+    const int *tables = joint ? sh.dev : p->tables_dev;
+    const SplPagedAttend a{static_cast<const uint16_t *>(device_q), device_out, out_type == SPL_F32, reinterpret_cast<const SplPagedItem *>(tables + (joint ? sh.starts_at : p->starts_at)),
+                           reinterpret_cast<const SplPagedItem *>(tables + (joint ? sh.items_at : p->items_at)), tables + (joint ? sh.begin_at : p->begin_at), p->tables_dev + p->arrived_at,
+                           joint ? sh.partial : p->partial, joint ? sh.partial_ml : p->partial_ml, joint ? 1 : p->slot_rows, e->tc_error};
+    if (scaled) {
+        const SplPagedAttendE4m3 x{a.q, static_cast<const unsigned char *>(device_k_cache), static_cast<const unsigned char *>(device_v_cache), k_scale, v_scale, device_out, a.out_f32, p->tables_dev + p->lengths_at};
+        const dim3 grid((p->rows * c.heads + 7) / 8);
+        launch_step(c.head_dim == 64 ? spl_paged_attend_e4m3_kernel<64> : c.head_dim == 128 ? spl_paged_attend_e4m3_kernel<128> : spl_paged_attend_e4m3_kernel<256>, grid, dim3(256), 0, st, p->tables(), p->shape, x);
+        return check_launch(e, "spl_paged_attend_scaled");
+    }
+    CUtensorMap k_map, v_map;
+    if (!paged_map(p, device_k_cache, false, &k_map) || !paged_map(p, device_v_cache, true, &v_map)) return refuse("the driver takes no tensor map of this cache");
+    const bool bf16 = c.dtype == SPL_BF16;
+    if (c.head_dim == 64) { if (bf16) launch_attend<64, true>(p, k_map, v_map, a, st); else launch_attend<64, false>(p, k_map, v_map, a, st); }
+    else if (c.head_dim == 128) { if (bf16) launch_attend<128, true>(p, k_map, v_map, a, st); else launch_attend<128, false>(p, k_map, v_map, a, st); }
+    else { if (bf16) launch_attend<256, true>(p, k_map, v_map, a, st); else launch_attend<256, false>(p, k_map, v_map, a, st); }
+    if (joint) {
+        const SplPagedCombine j{sh.dev, reinterpret_cast<const int2 *>(sh.dev + sh.work_at), reinterpret_cast<const SplPagedRecord *>(sh.dev + sh.records_at), sh.partial, sh.partial_ml, device_out, a.out_f32};
+        launch_combine(p, j, st);
+    }
+    return check_launch(e, "spl_paged_attend");
+}
 
 extern "C" {
 
@@ -235,60 +379,41 @@ void spl_paged_destroy(spl_paged *p) {
 }
 
 spl_status spl_paged_batch(spl_paged *p, int32_t sequences, const int32_t *rows, const int32_t *lengths, const int32_t *page_table, int32_t table_ld, void *stream) {
-    if (!p || !rows || !lengths || !page_table || table_ld < 0) return SPL_ERR_INVALID_ARGUMENT;
+    return spl_paged_batch_shared(p, sequences, rows, lengths, page_table, table_ld, 0, nullptr, nullptr, stream);
+}
+
+spl_status spl_paged_batch_shared(spl_paged *p, int32_t sequences, const int32_t *rows, const int32_t *lengths, const int32_t *page_table, int32_t table_ld, int32_t groups, const int32_t *group_sequences,
+                                  const int32_t *group_tokens, void *stream) {
+    if (!p || !rows || !lengths || !page_table || table_ld < 0 || groups < 0 || (groups && (!group_sequences || !group_tokens))) return SPL_ERR_INVALID_ARGUMENT;
     spl_engine *e = p->e;
     SPL_NOT_IN_FLIGHT(e);
     const SplDeviceScope scope(e->device);
-    try { return paged_batch(p, sequences, rows, lengths, page_table, table_ld, paged_stream(e, stream)); }
+    try { return paged_batch(p, sequences, rows, lengths, page_table, table_ld, SplPagedGroups{groups, group_sequences, group_tokens}, paged_stream(e, stream)); }
     catch (const std::bad_alloc &) { return SPL_ERR_ALLOCATION_FAILED; }
 }
 
 spl_status spl_paged_append(spl_paged *p, int32_t type, const void *device_q, int64_t q_ld, const void *device_k, int64_t k_ld, const void *device_v, int64_t v_ld,
                             const spl_tensor *q_norm, const spl_tensor *k_norm, void *device_q_out, void *device_k_cache, void *device_v_cache, void *stream) {
-    if (!p || !device_q || !device_k || !device_v || !device_q_out || !device_k_cache || !device_v_cache) return SPL_ERR_INVALID_ARGUMENT;
-    spl_engine *e = p->e;
-    SPL_NOT_IN_FLIGHT(e);
-    const spl_paged_config &c = p->c;
-    auto refuse = [&](const char *text) { return e->fail(SPL_ERR_INVALID_ARGUMENT, std::string("spl_paged_append: ") + text); };
-    if (!p->ready) return refuse("no batch is set");
-    if (p->shared_write) return refuse("two sequences of the batch would write to one page");
-    if (type != SPL_F32 && type != SPL_F16 && type != SPL_BF16) return refuse("rows are fp32, fp16 or bf16");
-    const int64_t q_width = int64_t(c.heads) * c.head_dim, kv_width = int64_t(c.kv_heads) * c.head_dim;
-    if (q_ld < q_width || k_ld < kv_width || v_ld < kv_width || q_ld % 2 || k_ld % 2 || v_ld % 2) return refuse("row strides must be even and hold the heads");
-    const size_t pair = type == SPL_F32 ? 8 : 4;
-    if (misaligned(device_q, pair) || misaligned(device_k, pair) || misaligned(device_v, pair)) return refuse("rows begin on a boundary of two elements");
-    if (misaligned(device_q_out, 16) || misaligned(device_k_cache, 16) || misaligned(device_v_cache, 16)) return refuse("queries and cache begin on a 16-byte boundary");
-    if ((q_norm && (!q_norm->vec || q_norm->count != c.head_dim)) || (k_norm && (!k_norm->vec || k_norm->count != c.head_dim))) return refuse("a norm weight is a vector of head_dim elements");
-    const SplDeviceScope scope(e->device);
-    const SplPagedRows in{device_q, device_k, device_v, q_ld, k_ld, v_ld};
-    const uint16_t *qw = q_norm ? q_norm->vec : nullptr, *kw = k_norm ? k_norm->vec : nullptr;
-    uint16_t *q = static_cast<uint16_t *>(device_q_out), *k = static_cast<uint16_t *>(device_k_cache), *v = static_cast<uint16_t *>(device_v_cache);
-    if (type == SPL_F32) launch_append<0>(p, in, qw, kw, q, k, v, paged_stream(e, stream));
-    else if (type == SPL_F16) launch_append<1>(p, in, qw, kw, q, k, v, paged_stream(e, stream));
-    else launch_append<2>(p, in, qw, kw, q, k, v, paged_stream(e, stream));
-    return check_launch(e, "spl_paged_append");
+    if (!p) return SPL_ERR_INVALID_ARGUMENT;
+    return paged_append(p, "spl_paged_append: ", false, type, device_q, q_ld, device_k, k_ld, device_v, v_ld, q_norm, k_norm, {static_cast<uint16_t *>(device_q_out), device_k_cache, device_v_cache, {nullptr, nullptr}}, stream);
+}
+
+spl_status spl_paged_append_scaled(spl_paged *p, int32_t type, const void *device_q, int64_t q_ld, const void *device_k, int64_t k_ld, const void *device_v, int64_t v_ld, const spl_tensor *q_norm,
+                                   const spl_tensor *k_norm, void *device_q_out, void *device_k_cache, void *device_v_cache, float *device_k_scale, float *device_v_scale, void *stream) {
+    if (!p || !device_k_scale || !device_v_scale) return SPL_ERR_INVALID_ARGUMENT;
+    return paged_append(p, "spl_paged_append_scaled: ", true, type, device_q, q_ld, device_k, k_ld, device_v, v_ld, q_norm, k_norm,
+                        {static_cast<uint16_t *>(device_q_out), device_k_cache, device_v_cache, {device_k_scale, device_v_scale}}, stream);
 }
 
 spl_status spl_paged_attend(spl_paged *p, const void *device_q, const void *device_k_cache, const void *device_v_cache, int32_t out_type, void *device_out, void *stream) {
-    if (!p || !device_q || !device_k_cache || !device_v_cache || !device_out) return SPL_ERR_INVALID_ARGUMENT;
-    spl_engine *e = p->e;
-    SPL_NOT_IN_FLIGHT(e);
-    const spl_paged_config &c = p->c;
-    auto refuse = [&](const char *text) { return e->fail(SPL_ERR_INVALID_ARGUMENT, std::string("spl_paged_attend: ") + text); };
-    if (!p->ready) return refuse("no batch is set");
-    if (out_type != SPL_F32 && out_type != c.dtype) return refuse("outputs are fp32 or of the cache's type");
-    if (misaligned(device_q, 16) || misaligned(device_k_cache, 16) || misaligned(device_v_cache, 16) || misaligned(device_out, 16)) return refuse("all buffers begin on a 16-byte boundary");
-    const SplDeviceScope scope(e->device);
-    CUtensorMap k_map, v_map;
-    if (!paged_map(p, device_k_cache, false, &k_map) || !paged_map(p, device_v_cache, true, &v_map)) return refuse("the driver takes no tensor map of this cache");
-    const SplPagedAttend a{static_cast<const uint16_t *>(device_q), device_out, out_type == SPL_F32, reinterpret_cast<const SplPagedItem *>(p->tables_dev + p->starts_at),
-                           reinterpret_cast<const SplPagedItem *>(p->tables_dev + p->items_at), p->tables_dev + p->begin_at, p->tables_dev + p->arrived_at, p->partial, p->partial_ml, p->slot_rows, e->tc_error};
-    cudaStream_t st = paged_stream(e, stream);
-    const bool bf16 = c.dtype == SPL_BF16;
-    if (c.head_dim == 64) { if (bf16) launch_attend<64, true>(p, k_map, v_map, a, st); else launch_attend<64, false>(p, k_map, v_map, a, st); }
-    else if (c.head_dim == 128) { if (bf16) launch_attend<128, true>(p, k_map, v_map, a, st); else launch_attend<128, false>(p, k_map, v_map, a, st); }
-    else { if (bf16) launch_attend<256, true>(p, k_map, v_map, a, st); else launch_attend<256, false>(p, k_map, v_map, a, st); }
-    return check_launch(e, "spl_paged_attend");
+    if (!p) return SPL_ERR_INVALID_ARGUMENT;
+    return paged_attend(p, "spl_paged_attend: ", false, device_q, device_k_cache, device_v_cache, nullptr, nullptr, out_type, device_out, stream);
+}
+
+spl_status spl_paged_attend_scaled(spl_paged *p, const void *device_q, const void *device_k_cache, const void *device_v_cache, const float *device_k_scale, const float *device_v_scale, int32_t out_type,
+                                   void *device_out, void *stream) {
+    if (!p || !device_k_scale || !device_v_scale) return SPL_ERR_INVALID_ARGUMENT;
+    return paged_attend(p, "spl_paged_attend_scaled: ", true, device_q, device_k_cache, device_v_cache, device_k_scale, device_v_scale, out_type, device_out, stream);
 }
 
 spl_status spl_pass_sample(spl_engine *e, const float *device_logits, int32_t rows, int64_t ld, int32_t vocab_limit, const float *device_temperature, const int32_t *device_top_k,
@@ -300,6 +425,24 @@ spl_status spl_pass_sample(spl_engine *e, const float *device_logits, int32_t ro
     const SplDeviceScope scope(e->device);
     const SplSampleArgs args{device_logits, ld, vocab_limit, device_temperature, device_top_k, device_top_p, device_min_p, device_uniform, device_ids};
     return launch_sample(e, args, rows, paged_stream(e, stream));
+}
+
+spl_status spl_pass_verify(spl_engine *e, const float *device_logits, int32_t sequences, int32_t rows, int64_t ld, int32_t vocab_limit, const int32_t *device_first, const int32_t *device_drafts, int32_t candidates,
+                           const int32_t *device_candidates, const float *device_probabilities, const float *device_temperature, const int32_t *device_top_k, const float *device_top_p, const float *device_min_p,
+                           const float *device_uniform, int32_t *device_ids, int32_t *device_accepted, int32_t *device_next, void *stream) {
+    if (!e || !device_logits || !device_first || !device_drafts || !device_uniform || !device_ids || !device_accepted || !device_next) return SPL_ERR_INVALID_ARGUMENT;
+    SPL_NOT_IN_FLIGHT(e);
+    if (sequences < 1 || rows < 1 || rows > 65535 || sequences > 65535) return e->fail(SPL_ERR_INVALID_ROWS, "spl_pass_verify: the number of sequences or rows is outside 1 ... 65535");
+    if (vocab_limit < 1 || vocab_limit > SPL_SAMPLE_VOCAB || ld < vocab_limit) return e->fail(SPL_ERR_INVALID_ARGUMENT, "spl_pass_verify: vocab_limit must be 1 ... 524288 and at most the rows' stride");
+    if (candidates < 0 || candidates > SPL_VERIFY_CANDIDATES || (candidates && (!device_candidates || !device_probabilities)))
+        return e->fail(SPL_ERR_INVALID_ARGUMENT, "spl_pass_verify: a token was picked from at most 64 candidates, with their probabilities (0: it was the only choice)");
+    const SplDeviceScope scope(e->device);
+    cudaStream_t st = paged_stream(e, stream);
+    const SplSampleArgs args{device_logits, ld, vocab_limit, device_temperature, device_top_k, device_top_p, device_min_p, device_uniform, device_ids, device_drafts, candidates, device_candidates, device_probabilities};
+    const spl_status launched = launch_sample(e, args, rows, st, true);
+    if (launched != SPL_OK) return launched;
+    launch_step(spl_verify_count_kernel, dim3((sequences + 3) / 4), dim3(128), 0, st, device_first, int(sequences), int(rows), (const int *)device_ids, device_accepted, device_next);
+    return check_launch(e, "spl_pass_verify");
 }
 
 spl_status spl_sample(spl_engine *e, int32_t vocab_limit, const spl_sampling *settings, const float *uniform, int32_t *ids) {
@@ -328,7 +471,12 @@ spl_status spl_sample(spl_engine *e, int32_t vocab_limit, const spl_sampling *se
 // Host arithmetic, no device needed.
 spl_status spl_paged_check(const spl_paged_config *config, int32_t sequences, const int32_t *rows, const int32_t *lengths, const int32_t *page_table, int32_t table_ld, int32_t *shared_write,
                            char *message, size_t message_bytes) {
-    if (!config || (sequences && (!rows || !lengths || !page_table)) || table_ld < 0) return SPL_ERR_INVALID_ARGUMENT;
+    return spl_paged_check_shared(config, sequences, rows, lengths, page_table, table_ld, 0, nullptr, nullptr, shared_write, message, message_bytes);
+}
+
+spl_status spl_paged_check_shared(const spl_paged_config *config, int32_t sequences, const int32_t *rows, const int32_t *lengths, const int32_t *page_table, int32_t table_ld, int32_t groups,
+                                  const int32_t *group_sequences, const int32_t *group_tokens, int32_t *shared_write, char *message, size_t message_bytes) {
+    if (!config || (sequences && (!rows || !lengths || !page_table)) || table_ld < 0 || groups < 0 || (groups && (!group_sequences || !group_tokens))) return SPL_ERR_INVALID_ARGUMENT;
     auto say = [&](const std::string &text) { if (message && message_bytes) { const size_t n = std::min(message_bytes - 1, text.size()); std::memcpy(message, text.data(), n); message[n] = 0; } };
     say("");
     try {
@@ -337,7 +485,8 @@ spl_status spl_paged_check(const spl_paged_config *config, int32_t sequences, co
         std::vector<uint8_t> written;
         std::string why;
         bool shared = false;
-        const spl_status s = spl_paged_batch_check(*config, sequences, rows, lengths, page_table, table_ld, written, &shared, &why);
+        spl_status s = spl_paged_batch_check(*config, sequences, rows, lengths, page_table, table_ld, written, &shared, &why);
+        if (s == SPL_OK && groups && !spl_paged_groups_check(*config, sequences, rows, lengths, page_table, table_ld, SplPagedGroups{groups, group_sequences, group_tokens}, &why)) s = SPL_ERR_INVALID_ROWS;
         say(why);
         if (s == SPL_OK && shared_write) *shared_write = shared;
         return s;
@@ -359,6 +508,26 @@ spl_status spl_debug_paged_plan(const spl_paged_config *config, int32_t blocks, 
             if (it.merge >= 0) std::memcpy(merges + 8 * it.merge, merge, sizeof merge);
         }
         *item_count = int32_t(plan.items.size()); *merge_count = plan.merges;
+        return SPL_OK;
+    } catch (const std::bad_alloc &) { return SPL_ERR_ALLOCATION_FAILED; }
+}
+
+spl_status spl_debug_paged_plan_shared(const spl_paged_config *config, int32_t blocks, int32_t sequences, const int32_t *rows, const int32_t *lengths, int32_t groups, const int32_t *group_sequences,
+                                       const int32_t *group_tokens, int32_t *block_begin, int32_t *items, int32_t items_capacity, int32_t *item_count, int32_t *records, int32_t records_capacity,
+                                       int32_t *record_count, int64_t *partial_rows, int32_t *joint) {
+    if (!config || !rows || !lengths || !block_begin || !items || !item_count || !records || !record_count || !partial_rows || !joint || blocks < 1 || sequences < 1 || groups < 0 ||
+        (groups && (!group_sequences || !group_tokens)) || spl_paged_config_error(*config)) return SPL_ERR_INVALID_ARGUMENT;
+    try {
+        SplPagedPlan plan;
+        const SplPagedGroups g{groups, group_sequences, group_tokens};
+        spl_paged_plan(*config, blocks, sequences, rows, lengths, plan, &g);
+        if (plan.items.size() > size_t(std::max(items_capacity, 0)) || plan.records.size() > size_t(std::max(records_capacity, 0))) return SPL_ERR_ALLOCATION_FAILED;
+        std::memcpy(block_begin, plan.block_begin.data(), plan.block_begin.size() * 4);
+        for (size_t i = 0; i < plan.items.size(); ++i) std::memcpy(items + 8 * i, &plan.items[i], 8 * 4);
+        for (size_t i = 0; i < plan.records.size(); ++i) std::memcpy(records + 10 * i, &plan.records[i], 10 * 4);
+        *item_count = int32_t(plan.items.size()); *record_count = int32_t(plan.records.size()); *partial_rows = plan.partial_rows; *joint = plan.joint;
+        if (plan.items.size() > size_t(spl_paged_shared_items_max(*config, blocks)) || plan.records.size() > size_t(spl_paged_records_max(*config, blocks)) ||
+            plan.partial_rows > spl_paged_partial_rows_max(*config, blocks)) return SPL_ERR_DEVICE;      // (what the object sets aside)
         return SPL_OK;
     } catch (const std::bad_alloc &) { return SPL_ERR_ALLOCATION_FAILED; }
 }

@@ -17,12 +17,23 @@
 // its first new one.
 struct alignas(16) SplPagedItem { int32_t sequence, row0, kv_head, q0, q_count, tile_begin, tile_end, slot, length, base, merge, pieces, slot0, reserved[3]; };
 
+// Rows of a shared batch whose partial sums a kernel of its own joins: `count` packed rows from q0 on of the sequence whose rows begin at row0. Row i's
+// sums of piece n lie at row a_first + n * a_step + i of the partial sums (a_pieces of them), and at b_first + n * b_step + i.
+struct alignas(16) SplPagedRecord { int32_t row0, q0, kv_head, count, a_first, a_step, a_pieces, b_first, b_step, b_pieces, reserved[2]; };
+
 struct SplPagedPlan {
     std::vector<SplPagedItem> items;
     std::vector<int32_t> block_begin;         // [blocks + 1]: a block's items
     std::vector<SplPagedItem> starts;         // [blocks]: a block's first item (none: no tiles)
     int merges = 0;
+    // Of a batch planned with groups (the items' slots are rows of the partial sums, and no block joins): what is joined behind the attention.
+    std::vector<SplPagedRecord> records;
+    int64_t partial_rows = 0;
+    bool joint = false;                       // some sequences meet a prefix together
 };
+
+// Which sequences of a batch share their first pages: group g is the next sequences[g] sequences, tokens[g] tokens each.
+struct SplPagedGroups { int32_t count; const int32_t *sequences, *tokens; };
 
 // Most items that a configuration's batches come to: a block's boundary cuts at most one tile of query rows.
 inline int64_t spl_paged_items_max(const spl_paged_config &c, int blocks) {
@@ -36,11 +47,12 @@ inline int spl_paged_first_token(const spl_paged_config &c, int position) { retu
 inline const char *spl_paged_config_error(const spl_paged_config &c) {
     if (c.head_dim != 64 && c.head_dim != 128 && c.head_dim != 256) return "heads are 64, 128 or 256 channels wide";
     if (c.heads < 1 || c.kv_heads < 1 || c.heads % c.kv_heads || c.heads > 1024 || c.heads / c.kv_heads > 64) return "heads must be a multiple of kv_heads, at most 1024 and 64 a kv head";
-    if (c.dtype != SPL_F16 && c.dtype != SPL_BF16) return "the cache holds fp16 or bf16";
+    if (c.dtype != SPL_F16 && c.dtype != SPL_BF16 && c.dtype != SPL_E4M3) return "the cache holds fp16, bf16 or e4m3";
     if (c.page_tokens != 16 && c.page_tokens != 32 && c.page_tokens != 64 && c.page_tokens != 128 && c.page_tokens != 256) return "pages hold 16, 32, 64, 128 or 256 tokens";
     if (c.pages < 1) return "no pages";
     const int64_t d = c.head_dim, ps = c.page_stride, hs = c.head_stride, ts = c.token_stride, most = int64_t(1) << 38;
-    if (ps % 8 || hs % 8 || ts % 8) return "strides must be multiples of 8 elements";
+    const int unit = c.dtype == SPL_E4M3 ? 16 : 8;
+    if (ps % unit || hs % unit || ts % unit) return "strides must be multiples of 16 bytes";
     if (ps <= 0 || hs <= 0 || ts <= 0 || ps > most || hs > most || ts > most || ps > (int64_t(1) << 50) / c.pages) return "strides are out of range";
     const bool token_inside = ts >= d && hs >= ts * c.page_tokens && ps >= hs * c.kv_heads, head_inside = hs >= d && ts >= hs * c.kv_heads && ps >= ts * c.page_tokens;
     if (!token_inside && !head_inside) return "strides must be those of [page][kv head][token][channel] or [page][token][kv head][channel], rows not overlapping";
@@ -86,6 +98,24 @@ inline spl_status spl_paged_batch_check(const spl_paged_config &c, int32_t seque
     return SPL_OK;
 }
 
+// Whether a batch's groups are taken: whole pages of tokens that lie in front of every member's new rows, in the same pages.
+inline bool spl_paged_groups_check(const spl_paged_config &c, int32_t sequences, const int32_t *rows, const int32_t *lengths, const int32_t *table, int32_t table_ld, const SplPagedGroups &groups, std::string *why) {
+    int64_t at = 0;
+    for (int g = 0; g < groups.count; ++g) {
+        const std::string name = "group " + std::to_string(g);
+        const int64_t n = groups.sequences[g], tokens = groups.tokens[g];
+        if (n < 1 || at + n > sequences) { *why = name + " has more sequences than are left, or none"; return false; }
+        if (tokens < 0 || tokens % c.page_tokens) { *why = name + " does not share whole pages"; return false; }
+        for (int64_t s = at; s < at + n; ++s) {
+            if (tokens > int64_t(lengths[s]) - rows[s]) { *why = name + " shares more tokens than sequence " + std::to_string(s) + " has in front of its new rows"; return false; }
+            for (int64_t i = 0; i < tokens / c.page_tokens; ++i)
+                if (table[size_t(s) * table_ld + i] != table[size_t(at) * table_ld + i]) { *why = "page " + std::to_string(i) + " of sequence " + std::to_string(s) + " is not that of its group's first"; return false; }
+        }
+        at += n;
+    }
+    return true;
+}
+
 // The tiles of all (sequence, kv head, 128 packed rows) in a line, cut in one stretch a block of equal cost. In tiles: a piece costs its tiles and
 // SPL_PAGED_PIECE_COST more (the first keys' way, the output), and a piece of a cut unit what leaving and joining partial sums takes, which goes by the rows.
 // Units of many rows are cut only into pieces that are worth it. (Whole units, longest first, leave the last round of blocks idle for prompts and most of the GPU for
@@ -106,63 +136,124 @@ inline int64_t spl_paged_take(int64_t t, int64_t left, int64_t stretch, int q_co
     }
     return left == stretch ? t : 0;                             // not worth a cut: whole, in a block of its own at the worst
 }
-inline void spl_paged_plan(const spl_paged_config &c, int blocks, int32_t sequences, const int32_t *rows, const int32_t *lengths, SplPagedPlan &plan) {
+// With groups, the sequences of a run (consecutive members of a group, none with more packed rows than a block takes) meet the whole tiles of their prefix
+// together: their rows lie one behind the other, so they are the rows of one sequence over the prefix, in blocks of 128 packed rows whoever's they are; each sequence's own
+// tokens are units of their own, and both leave partial sums (O, m, l) that spl_paged_combine_kernel joins. (Sequences of more packed rows read the prefix once for 128 of them as it is.)
+// That pays where the tiles saved are more than the joining, some SPL_PAGED_JOINT_COST tiles a block.
+#define SPL_PAGED_JOINT_COST 1
+struct SplPagedUnit { SplPagedItem item; bool joint; int run, prefix; };      // run: its run of sequences or -1; prefix: the first of its run's prefix units of its kv head
+inline void spl_paged_plan(const spl_paged_config &c, int blocks, int32_t sequences, const int32_t *rows, const int32_t *lengths, SplPagedPlan &plan, const SplPagedGroups *groups = nullptr) {
     const int group = c.heads / c.kv_heads, tile = SPL_PAGED_TILE;
     std::vector<SplPagedItem> &units = plan.items;
-    std::vector<SplPagedItem> whole;
+    std::vector<SplPagedUnit> whole;
     int64_t tiles = 0;
-    int longest = 0;
-    for (int s = 0, row0 = 0; s < sequences; row0 += rows[s], ++s)
+    auto add = [&](const SplPagedUnit &u) { tiles += u.item.tile_end - u.item.tile_begin; whole.push_back(u); };
+    auto add_sequence = [&](int s, int row0, int skip, int run, int first_prefix, int prefix_step) {
         for (int h = 0; h < c.kv_heads; ++h)
             for (int q0 = 0; q0 < rows[s] * group; q0 += tile) {
                 const int count = std::min(tile, rows[s] * group - q0), base = lengths[s] - rows[s];
                 const int first = spl_paged_first_token(c, base + q0 / group), last = c.causal ? base + (q0 + count - 1) / group + 1 : lengths[s];
-                const SplPagedItem u{s, row0, h, q0, count, first / tile, (last + tile - 1) / tile, -1, lengths[s], base, -1, 1, 0, {0, 0, 0}};
-                tiles += u.tile_end - u.tile_begin;
-                longest = std::max(longest, u.tile_end - u.tile_begin);
-                whole.push_back(u);
+                add({SplPagedItem{s, row0, h, q0, count, std::max(first / tile, skip), (last + tile - 1) / tile, -1, lengths[s], base, -1, 1, 0, {0, 0, 0}}, run >= 0, run, first_prefix + h * prefix_step});
             }
+    };
+    plan.joint = false;
+    std::vector<int> run_row0;
+    int s = 0, row0 = 0;
+    auto pass_over = [&]() { add_sequence(s, row0, 0, -1, 0, 0); row0 += rows[s]; ++s; };
+    for (int g = 0; groups && g < groups->count; ++g) {
+        const int end = s + groups->sequences[g], prefix = c.window > 0 ? 0 : groups->tokens[g] / tile;
+        while (s < end) {
+            // The longest run from here on, and whether it pays.
+            int run_end = s, members = 0;
+            int64_t packed = 0;
+            while (run_end < end && int64_t(rows[run_end]) * group <= tile) { packed += rows[run_end] * group; members += rows[run_end] > 0; ++run_end; }
+            const int64_t joint_units = (packed + tile - 1) / tile;
+            if (members < 2 || int64_t(c.kv_heads) * prefix * (members - joint_units) <= int64_t(blocks) * SPL_PAGED_JOINT_COST) {
+                do pass_over(); while (s < run_end);
+                continue;
+            }
+            const int run = int(run_row0.size()), first_prefix = int(whole.size());
+            run_row0.push_back(row0);
+            plan.joint = true;
+            for (int h = 0; h < c.kv_heads; ++h)
+                for (int64_t q0 = 0; q0 < packed; q0 += tile)
+                    add({SplPagedItem{s, row0, h, int(q0), int(std::min<int64_t>(tile, packed - q0)), 0, prefix, -1, prefix * tile, prefix * tile, -1, 1, 0, {0, 0, 0}}, true, -1, 0});
+            for (; s < run_end; row0 += rows[s], ++s) add_sequence(s, row0, prefix, run, first_prefix, int(joint_units));
+        }
+    }
+    while (s < sequences) pass_over();
     // The least stretch that makes do with the blocks there are.
     auto blocks_for = [&](int64_t stretch) {
         int64_t used = 1, left = stretch;
-        for (const SplPagedItem &u : whole)
-            for (int64_t t = u.tile_end - u.tile_begin, all = t; t > 0;) {
-                const int64_t take = spl_paged_take(t, left, stretch, u.q_count, t < all);
+        for (const SplPagedUnit &u : whole)
+            for (int64_t t = u.item.tile_end - u.item.tile_begin, all = t; t > 0;) {
+                const int64_t take = spl_paged_take(t, left, stretch, u.item.q_count, t < all || u.joint);
                 if (take < 0) return int64_t(blocks) + 1;
                 if (!take) { if (++used > blocks) return used; left = stretch; continue; }
-                left -= take + SPL_PAGED_PIECE_COST + (take < all ? spl_paged_cut_cost(u.q_count) : 0);
+                left -= take + SPL_PAGED_PIECE_COST + (take < all || u.joint ? spl_paged_cut_cost(u.item.q_count) : 0);
                 t -= take;
             }
         return used;
     };
     int64_t low = SPL_PAGED_PIECE_COST + 1, high = std::max<int64_t>(low, tiles + int64_t(whole.size()) * (SPL_PAGED_PIECE_COST + 2));
     while (low < high) { const int64_t mid = (low + high) / 2; if (blocks_for(mid) <= blocks) high = mid; else low = mid + 1; }
-    units.clear(); plan.merges = 0;
+    units.clear(); plan.merges = 0; plan.records.clear(); plan.partial_rows = 0;
     plan.block_begin.assign(1, 0);
     int64_t left = low;
     int slots = 0;
-    for (const SplPagedItem &u : whole) {
+    std::vector<std::pair<int32_t, int32_t>> left_at;      // with groups: each unit's first row of partial sums, and its pieces
+    for (const SplPagedUnit &one : whole) {
+        const SplPagedItem &u = one.item;
         const size_t piece0 = units.size();
         const int all = u.tile_end - u.tile_begin;
         for (int t = u.tile_begin; t < u.tile_end;) {
-            const int take = int(spl_paged_take(u.tile_end - t, left, low, u.q_count, t > u.tile_begin));
+            const int take = int(spl_paged_take(u.tile_end - t, left, low, u.q_count, t > u.tile_begin || one.joint));
             if (!take) { plan.block_begin.push_back(int32_t(units.size())); left = low; continue; }
             SplPagedItem piece = u;
             piece.tile_begin = t; piece.tile_end = t + take;
             units.push_back(piece);
-            left -= take + SPL_PAGED_PIECE_COST + (take < all ? spl_paged_cut_cost(u.q_count) : 0);
+            left -= take + SPL_PAGED_PIECE_COST + (take < all || one.joint ? spl_paged_cut_cost(u.q_count) : 0);
             t += take;
         }
         const int pieces = int(units.size() - piece0);
-        if (pieces > 1) {
+        if (groups) {
+            left_at.push_back({int32_t(plan.partial_rows), pieces});
+            if (pieces > 1 || one.joint)
+                for (size_t i = piece0; i < units.size(); ++i) { units[i].slot = int32_t(plan.partial_rows); plan.partial_rows += u.q_count; }
+        } else if (pieces > 1) {
             for (size_t i = piece0; i < units.size(); ++i) { units[i].slot = slots + int(i - piece0); units[i].slot0 = slots; units[i].pieces = pieces; units[i].merge = plan.merges; }
             slots += pieces; ++plan.merges;
+        }
+    }
+    for (size_t i = 0; i < left_at.size(); ++i) {
+        const SplPagedUnit &one = whole[i];
+        const SplPagedItem &u = one.item;
+        const auto [first, pieces] = left_at[i];
+        if (one.run < 0) {
+            if (!one.joint && pieces > 1) plan.records.push_back({u.row0, u.q0, u.kv_head, u.q_count, first, u.q_count, pieces, 0, 0, 0, {0, 0}});
+            continue;
+        }
+        // A sequence's rows may lie in two of the run's blocks of packed rows.
+        const int begin = (u.row0 - run_row0[one.run]) * group;
+        for (int q = begin; q < begin + u.q_count;) {
+            const int end = std::min(begin + u.q_count, (q / tile + 1) * tile), joint = one.prefix + q / tile;
+            plan.records.push_back({u.row0, q - begin, u.kv_head, end - q, left_at[joint].first + q % tile, whole[joint].item.q_count, left_at[joint].second, first + q - begin, u.q_count, pieces, {0, 0}});
+            q = end;
         }
     }
     plan.block_begin.resize(size_t(blocks) + 1, int32_t(units.size()));
     plan.block_begin[blocks] = int32_t(units.size());
     plan.starts.assign(size_t(blocks), SplPagedItem{});
     for (int b = 0; b < blocks; ++b) if (plan.block_begin[b] < plan.block_begin[b + 1]) plan.starts[b] = units[plan.block_begin[b]];
+}
+// Most items, records and rows of partial sums that a plan with groups comes to: the joint rows once over the prefix and once over their own tokens, and each block's boundary cuts at most one
+// unit; a sequence's rows are in one record a kv head and tile, or in two.
+inline int64_t spl_paged_joint_rows_max(const spl_paged_config &c) { return std::min(int64_t(c.max_rows) * c.heads, int64_t(c.max_sequences) * SPL_PAGED_TILE * c.kv_heads); }
+inline int64_t spl_paged_shared_items_max(const spl_paged_config &c, int blocks) { return 2 * spl_paged_items_max(c, blocks); }
+inline int64_t spl_paged_records_max(const spl_paged_config &c, int blocks) { return 2 * spl_paged_items_max(c, blocks); }
+inline int64_t spl_paged_partial_rows_max(const spl_paged_config &c, int blocks) { return 2 * spl_paged_joint_rows_max(c) + int64_t(blocks) * 2 * SPL_PAGED_TILE; }
+inline int64_t spl_paged_combine_max(const spl_paged_config &c, int blocks) {      // of blocks of the joining kernel's work, four (row, channels) each
+    return (spl_paged_joint_rows_max(c) + int64_t(blocks) * SPL_PAGED_TILE) * ((c.head_dim + 127) / 128) / 4 + spl_paged_records_max(c, blocks);
 }
 // Slots that a plan of `blocks` stretches takes at most: a unit is cut only where a block ends, and each such cut makes two pieces of one.
 inline int spl_paged_slots_max(int blocks) { return 2 * blocks; }

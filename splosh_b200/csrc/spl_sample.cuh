@@ -20,10 +20,18 @@
 #define SPL_SAMPLE_UNIT 17592186044416.0       // 2^44
 #define SPL_SAMPLE_VOCAB (1 << 19)
 
+//
+// Drafted tokens tested (spl_sample_kernel<HELD, true>): with p = w / W over what stays (W its sum) and q the drafter's probabilities, a row's drafted token d stays where u0 q(d) < p(d);
+// otherwise the row draws from max(p - q, 0), in the same order (from p where that is nothing). In whole numbers p W is w and q W rounds to one, so the sums of what is left are those of w less
+// min(w, q W) at the drafter's candidates (SPL_VERIFY_CANDIDATES at most): the bins, the lists and their running sums are sampling's, with the candidates' shares taken off.
+#define SPL_VERIFY_CANDIDATES 64
 struct SplSampleArgs {
     const float *logits; long long ld; int limit;
     const float *temperature; const int *top_k; const float *top_p, *min_p, *uniform;      // per row; null: 1, all, 1, 0
     int *ids;
+    // Drafted tokens tested: per row the token (negative: none), its `candidates` and their probabilities (0: the token was the only choice); uniform then has two numbers a row, for the test and the draw, and
+    // ids is -1 where the token stays.
+    const int *drafts; int candidates; const int *candidate_ids; const float *probabilities;
 };
 
 __device__ __forceinline__ float spl_topk_value(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key); }
@@ -91,6 +99,14 @@ enum { SPL_SAMPLE_DONE = 0, SPL_SAMPLE_FINISH, SPL_SAMPLE_CUT, SPL_SAMPLE_END, S
 
 struct SplSampleRow { float t, p, u, m, bin_scale; SplSampleWeigh w; unsigned long long least; int k; };
 
+// The first block's drafted token and its drafter's candidates: entry (0: not a value that may be picked, or listed before), probability, what is taken off its weight; the token itself is the last one.
+struct SplVerifyShared {
+    unsigned long long entry[SPL_VERIFY_CANDIDATES + 1], off[SPL_VERIFY_CANDIDATES + 1], left;
+    float q[SPL_VERIFY_CANDIDATES + 1];
+    int bin[SPL_VERIFY_CANDIDATES + 1], count, stays;
+    float u0;
+};
+
 __device__ __forceinline__ unsigned long long spl_sample_entry(uint32_t key, uint32_t index) { return (unsigned long long)key << 32 | uint32_t(~index); }
 
 // Sum over the block's threads before this one (exclusive), and of all in *total.
@@ -153,8 +169,45 @@ __device__ __forceinline__ unsigned long long spl_sample_target(float fraction, 
     return fraction > 0.0f ? min(sum, (unsigned long long)ceil(double(fraction) * double(sum))) : 0ull;
 }
 
+// What stays weighs `sum`, and stays(entry) says whether a value does: the test of the drafted token, what its drafter's candidates take off, and what is left (all threads get it).
+template <typename Stays>
+__device__ __forceinline__ unsigned long long spl_verify_resolve(SplVerifyShared &ve, const SplSampleRow &r, unsigned long long sum, Stays &&stays) {
+    __syncthreads();
+    const int tid = threadIdx.x;
+    if (tid < ve.count) {
+        const unsigned long long entry = ve.entry[tid], w = entry != 0ull && stays(entry) ? spl_sample_weight(spl_topk_value(uint32_t(entry >> 32)), r.w) : 0ull;
+        const double q = double(ve.q[tid]), share = q * double(sum);
+        if (tid == ve.count - 1) ve.stays = double(ve.u0) * q * double(sum) < double(w);
+        // (The last one, the token itself, is among the candidates where it has a probability; without candidates it is the only one.)
+        ve.off[tid] = (tid == ve.count - 1 && ve.count > 1) || !(share > 0.0) ? 0ull : share >= double(w) ? w : (unsigned long long)__double2ll_rn(share);
+    }
+    __syncthreads();
+    if (tid < 32) {
+        unsigned long long off = 0ull;
+        for (int i = tid; i < ve.count; i += 32) off += ve.off[i];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) off += __shfl_xor_sync(0xffffffffu, off, o);
+        if (off >= sum) for (int i = tid; i < ve.count; i += 32) ve.off[i] = 0ull;      // nothing is left: the target's own
+        if (tid == 0) ve.left = off >= sum ? sum : sum - off;
+    }
+    __syncthreads();
+    return ve.left;
+}
+// What has been taken off down to an entry of the order, or to the end of a bin.
+__device__ __forceinline__ unsigned long long spl_verify_off(const SplVerifyShared &ve, unsigned long long entry) {
+    unsigned long long off = 0ull;
+    for (int i = 0; i < ve.count; ++i) if (ve.entry[i] >= entry) off += ve.off[i];
+    return off;
+}
+__device__ __forceinline__ unsigned long long spl_verify_off_bins(const SplVerifyShared &ve, int bin) {
+    unsigned long long off = 0ull;
+    for (int i = 0; i < ve.count; ++i) if (ve.bin[i] <= bin) off += ve.off[i];
+    return off;
+}
+
 // Places found on the row itself, eight bits of the keys at a time, by one block.
-__device__ __noinline__ void spl_sample_slow(const SplSampleArgs &a, const SplSampleRow &r, SplSampleShared &sh, int row) {
+template <bool VERIFY>
+__device__ __noinline__ void spl_sample_slow(const SplSampleArgs &a, const SplSampleRow &r, SplSampleShared &sh, int row, SplVerifyShared *ve) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const float *x = a.logits + size_t(row) * a.ld;
     unsigned long long *mass = sh.sums;
@@ -164,7 +217,7 @@ __device__ __noinline__ void spl_sample_slow(const SplSampleArgs &a, const SplSa
     unsigned long long cut_ties = ~0ull, least = 0ull;
     // The place in the order where the running count (by_count) or the running weight reaches `target` (at least the first place):
     // its key, and how many of the key's values the prefix takes.
-    auto find = [&](bool by_count, unsigned long long target, uint32_t *key_out, unsigned long long *ties_out) {
+    auto find = [&](bool by_count, unsigned long long target, uint32_t *key_out, unsigned long long *ties_out, bool left = false) {      // left: of what the candidates leave
         uint32_t prefix = 0u;
         unsigned long long before = 0ull;
         for (int shift = 24; shift >= 0; shift -= 8) {
@@ -197,6 +250,9 @@ __device__ __noinline__ void spl_sample_slow(const SplSampleArgs &a, const SplSa
                     unsigned long long here = mass[d];
                     // The key that an earlier cut goes through keeps only its lowest indices.
                     if (shift == 0 && (prefix << 8 | uint32_t(d)) == cut_key && count[d] > cut_ties) here = mass[d] / count[d] * cut_ties;
+                    if constexpr (VERIFY) {
+                        if (left) for (int i = 0; i < ve->count; ++i) if (uint32_t(ve->entry[i] >> 32) >> shift == (shift == 24 ? uint32_t(d) : prefix << 8 | uint32_t(d))) here -= ve->off[i];
+                    }
                     last = d;
                     sh.value[0] = sum;
                     sum += here;
@@ -242,23 +298,54 @@ __device__ __noinline__ void spl_sample_slow(const SplSampleArgs &a, const SplSa
         if (key > cut_key || ties < cut_ties) { cut_key = key; cut_ties = ties; }
     }
     least = r.least;
+    // f(index, its number among the values of `key`, from one on) for each of these in order, by the block; the number of them so far goes to `enough`, which ends the walk.
+    auto walk = [&](uint32_t key, auto &&f, auto &&enough) {
+        unsigned long long seen = 0ull;
+        for (int base = 0; base < a.limit; base += 1024) {
+            const int i = base + tid;
+            const bool hit = i < a.limit && spl_topk_key(x[i]) == key;
+            const unsigned int votes = __ballot_sync(0xffffffffu, hit);
+            __syncthreads();
+            if (lane == 0) warp_count[warp] = __popc(votes);
+            __syncthreads();
+            unsigned int before = 0u, all = 0u;
+            for (int w = 0; w < 32; ++w) { if (w < warp) before += warp_count[w]; all += warp_count[w]; }
+            if (hit) f(i, seen + before + __popc(votes & ((1u << lane) - 1u)) + 1u);
+            seen += all;
+            if (enough(seen)) return;
+        }
+    };
     uint32_t pick_key; unsigned long long pick_tie;
+    if constexpr (VERIFY) {
+        // The last index of the cut's ties that stays, where a candidate may be one of them.
+        __syncthreads();
+        if (tid == 0) sh.found = 0xffffffffu;
+        __syncthreads();
+        if (cut_ties != ~0ull) walk(cut_key, [&](int i, unsigned long long n) { if (n == cut_ties) sh.found = unsigned(i); }, [&](unsigned long long seen) { return seen >= cut_ties; });
+        __syncthreads();
+        const unsigned long long last = spl_sample_entry(cut_key, sh.found);
+        const unsigned long long sum = total(), rest = spl_verify_resolve(*ve, r, sum, [&](unsigned long long e) { return e >= last && spl_sample_weight(spl_topk_value(uint32_t(e >> 32)), r.w) >= least; });
+        if (ve->stays) { if (tid == 0) a.ids[row] = -1; return; }
+        const unsigned long long target = spl_sample_target(r.u, rest);
+        find(false, target, &pick_key, &pick_tie, true);
+        // What the order leaves in front of the key's values, and the first of these that reaches the target.
+        __syncthreads();
+        const unsigned long long before = sh.value[0], each = spl_sample_weight(spl_topk_value(pick_key), r.w);
+        bool done = false;
+        walk(pick_key, [&](int i, unsigned long long n) {
+            const unsigned long long entry = spl_sample_entry(pick_key, uint32_t(i));
+            unsigned long long run = before + n * each, own = each;
+            for (int c = 0; c < ve->count; ++c) {
+                if (uint32_t(ve->entry[c] >> 32) == pick_key && ve->entry[c] >= entry) run -= ve->off[c];
+                if (ve->entry[c] == entry) own -= ve->off[c];
+            }
+            if (target <= before ? n == 1ull : run >= target && run - own < target) a.ids[row] = i;
+        }, [&](unsigned long long) { return done; });
+        return;
+    }
     find(false, spl_sample_target(r.u, total()), &pick_key, &pick_tie);
     // The pick_tie-th lowest index of pick_key: the block walks the row in order.
-    unsigned long long seen = 0ull;
-    for (int base = 0; base < a.limit; base += 1024) {
-        const int i = base + tid;
-        const bool hit = i < a.limit && spl_topk_key(x[i]) == pick_key;
-        const unsigned int votes = __ballot_sync(0xffffffffu, hit);
-        __syncthreads();
-        if (lane == 0) warp_count[warp] = __popc(votes);
-        __syncthreads();
-        unsigned int before = 0u, all = 0u;
-        for (int w = 0; w < 32; ++w) { if (w < warp) before += warp_count[w]; all += warp_count[w]; }
-        if (hit && seen + before + __popc(votes & ((1u << lane) - 1u)) + 1u == pick_tie) a.ids[row] = i;
-        seen += all;
-        if (seen >= pick_tie) return;
-    }
+    walk(pick_key, [&](int i, unsigned long long n) { if (n == pick_tie) a.ids[row] = i; }, [&](unsigned long long seen) { return seen >= pick_tie; });
 }
 
 // The first block: the blocks' lists into its own, sorted, with running sums of weights that begin at `base`. Returns the entries, or -1 where
@@ -337,8 +424,10 @@ __device__ __forceinline__ int spl_sample_sorted(SplSampleShared &sh, cooperativ
     return int(n);
 }
 
+__host__ __device__ constexpr size_t spl_verify_bytes() { return (sizeof(SplVerifyShared) + 127) / 128 * 128; }
+
 // Grid (blocks a row, rows) in clusters of a row's blocks, 1,024 threads.
-template <bool HELD>
+template <bool HELD, bool VERIFY>
 __global__ void __launch_bounds__(1024, 1)
 spl_sample_kernel(SplSampleArgs a) {
     namespace cg = cooperative_groups;
@@ -348,7 +437,8 @@ spl_sample_kernel(SplSampleArgs a) {
     const int row = blockIdx.y, rank = blockIdx.x, blocks = gridDim.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const float *x = a.logits + size_t(row) * a.ld;
     const int stretch = ((a.limit + blocks - 1) / blocks + 31) / 32 * 32, begin = rank * stretch, end = min(a.limit, begin + stretch);
-    float *held = reinterpret_cast<float *>(spl_sample_raw + sizeof(SplSampleShared));
+    SplVerifyShared &ve = *reinterpret_cast<SplVerifyShared *>(spl_sample_raw + sizeof(SplSampleShared));
+    float *held = reinterpret_cast<float *>(spl_sample_raw + sizeof(SplSampleShared) + (VERIFY ? spl_verify_bytes() : 0));
     const float *mine = x + begin;
     const int count = max(0, end - begin);
     asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");      // (a block's shared memory may be reached when it has begun)
@@ -376,10 +466,32 @@ spl_sample_kernel(SplSampleArgs a) {
         }
     };
     SplSampleRow r;
-    r.t = a.temperature ? a.temperature[row] : 1.0f; r.p = a.top_p ? a.top_p[row] : 1.0f; r.u = a.uniform[row];
+    r.t = a.temperature ? a.temperature[row] : 1.0f; r.p = a.top_p ? a.top_p[row] : 1.0f; r.u = a.uniform[VERIFY ? 2 * row + 1 : row];
     // (At an infinite temperature every weight is one, or none beside an infinite value: min-p takes nothing away.)
     r.m = a.min_p && a.min_p[row] > 0.0f && r.t < INFINITY ? fminf(a.min_p[row], 1.0f) : 0.0f; r.k = a.top_k ? a.top_k[row] : 0;
     r.least = r.m > 0.0f ? (unsigned long long)ceil(double(r.m) * SPL_SAMPLE_UNIT) : 0ull;
+
+    if constexpr (VERIFY) {
+        // The drafted token and its candidates, their logits on the way beside the row's.
+        const int draft = a.drafts[row];
+        if (rank == 0 && tid <= SPL_VERIFY_CANDIDATES) {
+            const int n = draft < 0 ? 0 : a.candidates + 1;      // (without candidates the token alone, at probability one)
+            int id = -1;
+            float q = 0.0f;
+            if (tid < n) {
+                const int *ids = a.candidate_ids + size_t(row) * a.candidates;
+                id = tid < a.candidates ? ids[tid] : draft;
+                q = a.candidates ? 0.0f : 1.0f;
+                bool again = false;
+                for (int i = 0; i < min(tid, a.candidates); ++i) if (ids[i] == id) { if (tid == a.candidates) { q = a.probabilities[size_t(row) * a.candidates + i]; break; } again = true; }
+                if (tid < a.candidates) q = a.probabilities[size_t(row) * a.candidates + tid];
+                const uint32_t key = id >= 0 && id < a.limit ? spl_topk_key(x[id]) : 0u;
+                ve.entry[tid] = key == 0u || again ? 0ull : spl_sample_entry(key, uint32_t(id));
+                ve.q[tid] = q;
+            }
+            if (tid == 0) { ve.count = n; ve.u0 = a.uniform[2 * row]; ve.stays = 0; }
+        }
+    }
 
     // The largest value and its lowest index.
     {
@@ -414,6 +526,11 @@ spl_sample_kernel(SplSampleArgs a) {
     for (int b = 1; b < blocks; ++b) top = max(top, sh.best[b]);
     const bool nothing = (top >> 32) == 0ull;          // id 0, as an untouched slot of a top-k
     if (nothing || !(r.t > 0.0f)) {
+        if constexpr (VERIFY) {
+            // All the weight is the largest value's.
+            if (rank == 0 && tid == 0) a.ids[row] = nothing ? 0 : ve.count && ve.entry[ve.count - 1] == top && ve.u0 * ve.q[ve.count - 1] < 1.0f ? -1 : int32_t(~uint32_t(top));
+            return;
+        }
         if (rank == 0 && tid == 0) a.ids[row] = nothing ? 0 : int32_t(~uint32_t(top));
         return;
     }
@@ -427,6 +544,7 @@ spl_sample_kernel(SplSampleArgs a) {
     auto bin_of = [&](float value) {
         return __float_as_int(fminf(fmaf(-0.5f, value, half_max) * r.bin_scale, float(SPL_SAMPLE_BINS - 1)) + 8388608.0f) & (SPL_SAMPLE_BINS - 1);
     };
+    if constexpr (VERIFY) { if (rank == 0 && tid < ve.count) ve.bin[tid] = ve.entry[tid] ? bin_of(spl_topk_value(uint32_t(ve.entry[tid] >> 32))) : SPL_SAMPLE_BINS; }
     unsigned long long cut = 0ull;                     // entries below it are out
     // The values of the bins [first, last] and [also_first, also_last] (in front of them; none where also_first is negative) into the block's list.
     auto set_aside = [&](int first, int last, int also_first, int also_last) {
@@ -507,8 +625,15 @@ spl_sample_kernel(SplSampleArgs a) {
                         __syncthreads();
                         stay = int(sh.found);
                     }
-                    const int pick = spl_sample_place(sh, stay, spl_sample_target(r.u, sh.sums[stay - 1]));
-                    if (tid == 0) a.ids[row] = int32_t(~uint32_t(sh.list[pick]));
+                    if constexpr (VERIFY) {
+                        const unsigned long long last = sh.list[stay - 1], left = spl_verify_resolve(ve, r, sh.sums[stay - 1], [&](unsigned long long e) { return e >= last; });
+                        for (int i = tid; i < stay; i += 1024) sh.sums[i] -= spl_verify_off(ve, sh.list[i]);
+                        const int pick = spl_sample_place(sh, stay, spl_sample_target(r.u, left));
+                        if (tid == 0) a.ids[row] = ve.stays ? -1 : int32_t(~uint32_t(sh.list[pick]));
+                    } else {
+                        const int pick = spl_sample_place(sh, stay, spl_sample_target(r.u, sh.sums[stay - 1]));
+                        if (tid == 0) a.ids[row] = int32_t(~uint32_t(sh.list[pick]));
+                    }
                     decide(SPL_SAMPLE_DONE, 0, 0, 0ull);
                 }
             }
@@ -560,7 +685,8 @@ spl_sample_kernel(SplSampleArgs a) {
                 if (p_bin > m1) { c0 = m0; c1 = m1; p_bin = SPL_SAMPLE_BINS; }      // top-p's place comes later
                 else if (p_bin >= m0) { c0 = m0; c1 = m1; }
             }
-            if (c1 >= 0) {
+            if (VERIFY && c1 >= 0) decide(SPL_SAMPLE_END, c0, c1, cut);      // (what the candidates leave is known when what stays is)
+            else if (c1 >= 0) {
                 // Whatever of the bins [c0, c1] stays, the draw mostly lies in one and the same bin, or one of a few: set aside with them, it is found in the same list. (With one bin
                 // alone a fifth of the rows of a vocabulary of 248,077 needed another turn.)
                 const unsigned long long least_sum = c0 ? sh.sums[c0 - 1] : 0ull;
@@ -568,8 +694,16 @@ spl_sample_kernel(SplSampleArgs a) {
                 if (d0 < c0 && min(d1, c0 - 1) - d0 < 8) { also = d0; also_last = min(d1, c0 - 1); }
                 decide(SPL_SAMPLE_END, c0, c1, cut, also, also_last);
             } else {
-                const int b = spl_sample_place(sh, SPL_SAMPLE_BINS, spl_sample_target(r.u, all));
-                decide(SPL_SAMPLE_DRAW, b, b, cut);
+                unsigned long long left = all;
+                if constexpr (VERIFY) {
+                    left = spl_verify_resolve(ve, r, all, [&](unsigned long long e) { return e >= cut && bin_of(spl_topk_value(uint32_t(e >> 32))) < SPL_SAMPLE_BINS - 1; });
+                    for (int i = tid; i < SPL_SAMPLE_BINS; i += 1024) sh.sums[i] -= spl_verify_off_bins(ve, i);
+                }
+                const unsigned long long target = spl_sample_target(r.u, left);
+                const int b = spl_sample_place(sh, SPL_SAMPLE_BINS, target);
+                all = left;
+                if (VERIFY && ve.stays) { if (tid == 0) a.ids[row] = -1; decide(SPL_SAMPLE_DONE, 0, 0, 0ull); }
+                else decide(SPL_SAMPLE_DRAW, b, b, cut);
             }
         }
         cluster.sync();
@@ -615,13 +749,21 @@ spl_sample_kernel(SplSampleArgs a) {
                         __syncthreads();
                         stay = int(sh.found);
                     }
-                    target = spl_sample_target(r.u, stay > front ? sh.sums[stay - 1] : base);
+                    unsigned long long left = stay > front ? sh.sums[stay - 1] : base, first = base;
+                    if constexpr (VERIFY) {
+                        const unsigned long long last = stay > 0 ? sh.list[stay - 1] : ~0ull;
+                        left = spl_verify_resolve(ve, r, left, [&](unsigned long long e) { return e >= cut && (e >= last || bin_of(spl_topk_value(uint32_t(e >> 32))) < c0); });
+                        first -= c0 ? spl_verify_off_bins(ve, c0 - 1) : 0ull;
+                        for (int i = tid; i < stay; i += 1024) sh.sums[i] -= spl_verify_off(ve, sh.list[i]);
+                    }
+                    target = spl_sample_target(r.u, left);
                     int from = -1, to = stay;
                     unsigned long long shift = 0ull;
-                    if (target > base || base == 0ull) from = front;
+                    if (target > first || base == 0ull) from = front;
                     else if (also >= 0 && target > also_base && target <= also_base + also_sum) { from = 0; to = front; shift = base - also_sum - also_base; }
                     else if (also == 0) { from = 0; to = front; shift = base - also_sum; }      // a target of nothing: the first value
-                    if (from >= 0) {
+                    if (VERIFY && ve.stays) { if (tid == 0) a.ids[row] = -1; decide(SPL_SAMPLE_DONE, 0, 0, 0ull); }
+                    else if (from >= 0) {
                         __syncthreads();
                         if (tid == 0) sh.found = unsigned(to - 1);
                         __syncthreads();
@@ -631,7 +773,10 @@ spl_sample_kernel(SplSampleArgs a) {
                         decide(SPL_SAMPLE_DONE, 0, 0, 0ull);
                     } else {
                         __syncthreads();
-                        for (int i = tid; i < SPL_SAMPLE_BINS; i += 1024) sh.sums[i] = kept[i];
+                        for (int i = tid; i < SPL_SAMPLE_BINS; i += 1024) {
+                            if constexpr (VERIFY) sh.sums[i] = kept[i] - spl_verify_off_bins(ve, i);
+                            else sh.sums[i] = kept[i];
+                        }
                         const int b = spl_sample_place(sh, SPL_SAMPLE_BINS, target);
                         decide(SPL_SAMPLE_DRAW, b, b, cut);
                     }
@@ -647,6 +792,7 @@ spl_sample_kernel(SplSampleArgs a) {
                 const int n = spl_sample_sorted(sh, cluster, blocks, r, b ? kept[b - 1] : 0ull);
                 if (n < 0) decide(SPL_SAMPLE_SLOW, 0, 0, 0ull);
                 else {
+                    if constexpr (VERIFY) for (int i = tid; i < n; i += 1024) sh.sums[i] -= spl_verify_off(ve, sh.list[i]);
                     const int pick = spl_sample_place(sh, n, target);
                     if (tid == 0) a.ids[row] = int32_t(~uint32_t(sh.list[pick]));
                     decide(SPL_SAMPLE_DONE, 0, 0, 0ull);
@@ -656,5 +802,21 @@ spl_sample_kernel(SplSampleArgs a) {
             step = sh.step;
         }
     }
-    if (step == SPL_SAMPLE_SLOW && rank == 0) spl_sample_slow(a, r, sh, row);
+    if (step == SPL_SAMPLE_SLOW && rank == 0) spl_sample_slow<VERIFY>(a, r, sh, row, &ve);
+}
+
+// A sequence's rows [first[s], first[s + 1]): how many of its drafted tokens stay, the rows in front of the first whose token does not, and that row's token (-1: they all stay). A warp a sequence.
+__global__ void __launch_bounds__(128)
+spl_verify_count_kernel(const int *first, int sequences, int rows, const int *ids, int *accepted, int *next) {
+    const int s = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const int begin = s < sequences ? min(max(first[s], 0), rows) : 0, end = s < sequences ? min(max(first[s + 1], begin), rows) : 0;
+    spl_grid_begin();
+    if (s >= sequences) return;
+    int stop = end, token = -1;
+    for (int r0 = begin; r0 < end; r0 += 32) {
+        const int id = r0 + lane < end ? ids[r0 + lane] : -1;
+        const unsigned int votes = __ballot_sync(0xffffffffu, id >= 0);
+        if (votes) { stop = r0 + __ffs(votes) - 1; token = __shfl_sync(0xffffffffu, id, __ffs(votes) - 1); break; }
+    }
+    if (lane == 0) { accepted[s] = stop - begin; next[s] = token; }
 }

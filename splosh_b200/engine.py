@@ -248,6 +248,12 @@ def lib():
             "spl_paged_create": (i32, [vp, vp, C.POINTER(vp)]),
             "spl_paged_destroy": (None, [vp]),
             "spl_paged_batch": (i32, [vp, i32, vp, vp, vp, i32, vp]),
+            "spl_pass_verify": (i32, [vp, vp, i32, i32, C.c_int64, i32, vp, vp, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp]),
+            "spl_paged_batch_shared": (i32, [vp, i32, vp, vp, vp, i32, i32, vp, vp, vp]),
+            "spl_paged_append_scaled": (i32, [vp, i32, vp, C.c_int64, vp, C.c_int64, vp, C.c_int64, vp, vp, vp, vp, vp, vp, vp, vp]),
+            "spl_paged_attend_scaled": (i32, [vp, vp, vp, vp, vp, vp, i32, vp, vp]),
+            "spl_paged_check_shared": (i32, [vp, i32, vp, vp, vp, i32, i32, vp, vp, vp, C.c_char_p, C.c_size_t]),
+            "spl_debug_paged_plan_shared": (i32, [vp, i32, i32, vp, vp, i32, vp, vp, vp, vp, i32, vp, vp, i32, vp, vp, vp]),
             "spl_paged_append": (i32, [vp, i32, vp, C.c_int64, vp, C.c_int64, vp, C.c_int64, vp, vp, vp, vp, vp, vp]),
             "spl_paged_attend": (i32, [vp, vp, vp, vp, i32, vp, vp]),
             "spl_paged_check": (i32, [vp, i32, vp, vp, vp, i32, vp, C.c_char_p, C.c_size_t]),
@@ -543,6 +549,13 @@ class Engine:
         """A token a row from fp32 logits on the device (spl_pass_sample); the settings are addresses of one value a row, or None."""
         self._check(lib().spl_pass_sample(self.handle, device_logits, rows, ld, vocab_limit, temperature, top_k, top_p, min_p, device_uniform, device_ids,
                                           stream_handle(stream)))
+
+    def pass_verify(self, device_logits, sequences, rows, ld, vocab_limit, device_first, device_drafts, device_uniform, device_ids, device_accepted, device_next, candidates=0, candidate_ids=None,
+                    probabilities=None, temperature=None, top_k=None, top_p=None, min_p=None, stream=None):
+        """Drafted tokens tested against the target's logits (spl_pass_verify): sequence s has the rows first[s] ... first[s + 1], a row the token drafted to follow it (negative: none) out of `candidates` with their
+        probabilities (0: it was the only choice), two uniform numbers, and settings as pass_sample's. A row's id is -1 where its token stays, else the token in its place; accepted and next are each sequence's."""
+        self._check(lib().spl_pass_verify(self.handle, device_logits, sequences, rows, ld, vocab_limit, device_first, device_drafts, candidates, candidate_ids, probabilities, temperature, top_k, top_p, min_p,
+                                          device_uniform, device_ids, device_accepted, device_next, stream_handle(stream)))
 
     def pass_wait(self):
         self._check(lib().spl_pass_wait(self.handle))
