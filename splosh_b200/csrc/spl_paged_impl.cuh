@@ -27,7 +27,7 @@ struct spl_paged {
     SplEncodeTiled encode = nullptr;
     // Device tables in one block, filled from one of two pinned blocks (the other's copy may still be on its way): the row count, block_begin, the pieces that have arrived of each merge
     // (none), the blocks' first items, the rows' sequences and positions, the plan's items, the page table. Places do not depend on the batch, so a captured graph finds the next one's.
-    size_t words = 0, begin_at = 16, arrived_at = 0, starts_at = 0, batch_at = 0, lengths_at = 0, items_at = 0, table_at = 0;
+    size_t words = 0, begin_at = 16, arrived_at = 0, starts_at = 0, batch_at = 0, items_at = 0, table_at = 0;
     SplPagedPlan plan;
     // Partial sums of query rows whose tokens several blocks share.
     int slot_rows = 0;
@@ -47,7 +47,7 @@ struct spl_paged {
         SplPagedPlan plan;
     } shared;
     // The batch that was set last.
-    int rows = 0, combine_work = 0;
+    int rows = 0, combine_work = 0, packed = 0;      // packed: the most packed rows a sequence has
     bool ready = false, shared_write = false, joint = false;
     std::vector<uint8_t> written;      // scratch of the check for pages that two sequences would write
 
@@ -66,8 +66,17 @@ template <int HD> static bool paged_configure_dim() {
     return cudaFuncSetAttribute(spl_paged_attend_kernel<HD, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess &&
            cudaFuncSetAttribute(spl_paged_attend_kernel<HD, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess;
 }
+template <int HD, int N> static bool paged_configure_narrow() {
+    return cudaFuncSetAttribute(spl_paged_attend_e4m3_narrow_kernel<HD, N>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(spl_paged8n_smem_bytes(HD, N))) == cudaSuccess;
+}
+template <int HD> static bool paged_configure_e4m3() {
+    if constexpr (HD >= 128) { if (!paged_configure_narrow<HD, 16>() || !paged_configure_narrow<HD, 32>() || !paged_configure_narrow<HD, 48>()) return false; }
+    return cudaFuncSetAttribute(spl_paged_attend_e4m3_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(spl_paged8_smem_bytes(HD))) == cudaSuccess;
+}
 // (The opt-in is a property of the current device.)
-static bool paged_configure(int head_dim) { return head_dim == 64 ? paged_configure_dim<64>() : head_dim == 128 ? paged_configure_dim<128>() : paged_configure_dim<256>(); }
+static bool paged_configure(int head_dim, bool e4m3) {
+    if (e4m3) return head_dim == 64 ? paged_configure_e4m3<64>() : head_dim == 128 ? paged_configure_e4m3<128>() : paged_configure_e4m3<256>();     return head_dim == 64 ? paged_configure_dim<64>() : head_dim == 128 ? paged_configure_dim<128>() : paged_configure_dim<256>();
+}
 
 static spl_status paged_create(spl_engine *e, const spl_paged_config *cp, spl_paged *p) {
     const spl_paged_config &c = p->c = *cp;
@@ -79,8 +88,7 @@ static spl_status paged_create(spl_engine *e, const spl_paged_config *cp, spl_pa
     p->arrived_at = p->begin_at + (blocks + 1 + 3) / 4 * 4;
     p->starts_at = p->arrived_at + (blocks + 3) / 4 * 4;
     p->batch_at = p->starts_at + blocks * (sizeof(SplPagedItem) / 4);
-    p->lengths_at = p->batch_at + size_t(c.max_rows) * 2;
-    p->items_at = (p->lengths_at + size_t(c.max_sequences) + 3) / 4 * 4;
+    p->items_at = (p->batch_at + size_t(c.max_rows) * 2 + 3) / 4 * 4;
     p->table_at = p->items_at + items * (sizeof(SplPagedItem) / 4);
     p->words = p->table_at + size_t(p->max_pages) * c.max_sequences;
     p->written.assign(size_t(c.pages), 0);
@@ -101,7 +109,7 @@ static spl_status paged_create(spl_engine *e, const spl_paged_config *cp, spl_pa
     SPL_CUDA(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &encode, 12000, cudaEnableDefault, &found));
     if (found != cudaDriverEntryPointSuccess || !encode) return e->fail(SPL_ERR_UNSUPPORTED_DEVICE, "spl_paged_create: the driver has no tensor maps");
     p->encode = reinterpret_cast<SplEncodeTiled>(encode);
-    if (!paged_configure(c.head_dim)) return e->fail(SPL_ERR_UNSUPPORTED_DEVICE, "spl_paged_create: the kernel's shared-memory opt-in failed");
+    if (!paged_configure(c.head_dim, c.dtype == SPL_E4M3)) return e->fail(SPL_ERR_UNSUPPORTED_DEVICE, "spl_paged_create: the kernel's shared-memory opt-in failed");
     double turns[128] = {};
     for (int i = 0; i < c.rotary_dim / 2; ++i) turns[i] = std::pow(double(c.rope_theta), -2.0 * i / c.rotary_dim) / 6.283185307179586476925;
     return upload(e, p->turns, turns, sizeof turns);
@@ -189,7 +197,6 @@ static spl_status paged_batch(spl_paged *p, int32_t sequences, const int32_t *ro
     std::memcpy(w + p->items_at, p->plan.items.data(), p->plan.items.size() * sizeof(SplPagedItem));
     int *row_sequence = w + p->batch_at, *row_position = row_sequence + c.max_rows, *pages = w + p->table_at;
     int longest = 1;
-    std::memcpy(w + p->lengths_at, lengths, size_t(sequences) * 4);
     for (int s = 0, r = 0; s < sequences; ++s) {
         for (int i = 0; i < rows[s]; ++i, ++r) { row_sequence[r] = s; row_position[r] = lengths[s] - rows[s] + i; }
         const int used = (lengths[s] + c.page_tokens - 1) / c.page_tokens;
@@ -206,6 +213,8 @@ static spl_status paged_batch(spl_paged *p, int32_t sequences, const int32_t *ro
     p->joint = p->shared.dev && p->shared.plan.joint;
     SPL_CUDA(cudaEventRecord(p->copied[turn], stream));
     p->turn ^= 1;
+    p->packed = 0;
+    for (int s = 0; s < sequences; ++s) p->packed = std::max(p->packed, int(std::min<int64_t>(int64_t(rows[s]) * p->shape.group, 1 << 30)));
     p->rows = int(total); p->shared_write = shared; p->ready = true;
     return SPL_OK;
 }
@@ -224,10 +233,21 @@ template <int TYPE> static void launch_append(const spl_paged *p, const SplPaged
     else launch_append_dim<TYPE, 256>(p, in, q_norm, k_norm, out, stream);
 }
 
+// Whether the batch's attention over a cache of e4m3 runs in its transposed form: few packed rows a sequence, none of them met together with others'.
+static bool paged_narrow(const spl_paged *p) { return p->c.dtype == SPL_E4M3 && p->c.head_dim >= 128 && !p->joint && p->packed <= SPL_PAGED8_NARROW; }
 // The cache as a tensor (channel in block, token in page, block of 64 channels, kv head, page) for the copies of values, in boxes of all channels by a page's tokens (at most a
 // chunk's), or of keys: of a page's tokens (at most a tile's) by 64 channels, or by a chunk's where the box is a tile's tokens.
 static bool paged_map(const spl_paged *p, const void *cache, bool values, CUtensorMap *map) {
     const spl_paged_config &c = p->c;
+    if (c.dtype == SPL_E4M3) {
+        values = values && !paged_narrow(p);      // (there the values come in the keys' boxes)
+        // In bytes, blocks of 128 channels (all of 64): boxes of a block by a page's tokens (at most a tile's) of keys, of all blocks by a page's tokens (at most a chunk's) of values.
+        const cuuint64_t row = cuuint64_t(std::min(c.head_dim, 128)), blocks = cuuint64_t(c.head_dim) / row, dims[5] = {row, cuuint64_t(c.page_tokens), blocks, cuuint64_t(c.kv_heads), cuuint64_t(c.pages)};
+        const cuuint64_t strides[4] = {cuuint64_t(c.token_stride), row, cuuint64_t(c.head_stride), cuuint64_t(c.page_stride)};
+        const cuuint32_t box[5] = {cuuint32_t(row), cuuint32_t(std::min(c.page_tokens, values ? spl_paged8_v_tokens(c.head_dim) : SPL_PAGED_TILE)), values ? cuuint32_t(blocks) : 1u, 1, 1}, steps[5] = {1, 1, 1, 1, 1};
+        return p->encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 5, const_cast<void *>(cache), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         row == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : values ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    }
     const cuuint64_t d = cuuint64_t(c.head_dim), dims[5] = {64, cuuint64_t(c.page_tokens), d / 64, cuuint64_t(c.kv_heads), cuuint64_t(c.pages)};
     const cuuint64_t strides[4] = {cuuint64_t(c.token_stride) * 2, 128, cuuint64_t(c.head_stride) * 2, cuuint64_t(c.page_stride) * 2};
     const int chunk = spl_paged_chunk(c.head_dim), tokens = std::min(c.page_tokens, values ? chunk / (2 * c.head_dim) : SPL_PAGED_TILE);
@@ -239,6 +259,18 @@ static bool paged_map(const spl_paged *p, const void *cache, bool values, CUtens
 
 template <int HD, bool BF16> static void launch_attend(const spl_paged *p, const CUtensorMap &k_map, const CUtensorMap &v_map, const SplPagedAttend &a, cudaStream_t stream) {
     launch_step(spl_paged_attend_kernel<HD, BF16>, dim3(p->e->sms), dim3(SPL_PAGED_THREADS), spl_paged_smem_bytes(HD), stream, k_map, v_map, p->tables(), p->shape, a);
+}
+
+template <int HD> static void launch_attend_e4m3(const spl_paged *p, const CUtensorMap &k_map, const CUtensorMap &v_map, const SplPagedAttend &a, const SplPagedScaled &scales, cudaStream_t stream) {
+    if constexpr (HD >= 128) {
+        if (paged_narrow(p)) {
+            const int n = p->packed <= 16 ? 16 : p->packed <= 32 ? 32 : 48;
+            launch_step(n == 16 ? spl_paged_attend_e4m3_narrow_kernel<HD, 16> : n == 32 ? spl_paged_attend_e4m3_narrow_kernel<HD, 32> : spl_paged_attend_e4m3_narrow_kernel<HD, 48>, dim3(p->e->sms), dim3(384),
+                        spl_paged8n_smem_bytes(HD, n), stream, k_map, v_map, p->tables(), p->shape, a, scales);
+            return;
+        }
+    }
+    launch_step(spl_paged_attend_e4m3_kernel<HD>, dim3(p->e->sms), dim3(SPL_PAGED8_THREADS), spl_paged8_smem_bytes(HD), stream, k_map, v_map, p->tables(), p->shape, a, scales);
 }
 
 // The blocks of a row's cluster: a wave of clusters costs some 14 us of meetings and sorting whatever a block's share, and 19 us for 32,768 values a block (they fit
@@ -332,16 +364,15 @@ static spl_status paged_attend(spl_paged *p, const char *name, bool scaled, cons
     const SplPagedAttend a{static_cast<const uint16_t *>(device_q), device_out, out_type == SPL_F32, reinterpret_cast<const SplPagedItem *>(tables + (joint ? sh.starts_at : p->starts_at)),
                            reinterpret_cast<const SplPagedItem *>(tables + (joint ? sh.items_at : p->items_at)), tables + (joint ? sh.begin_at : p->begin_at), p->tables_dev + p->arrived_at,
                            joint ? sh.partial : p->partial, joint ? sh.partial_ml : p->partial_ml, joint ? 1 : p->slot_rows, e->tc_error};
-    if (scaled) {
-        const SplPagedAttendE4m3 x{a.q, static_cast<const unsigned char *>(device_k_cache), static_cast<const unsigned char *>(device_v_cache), k_scale, v_scale, device_out, a.out_f32, p->tables_dev + p->lengths_at};
-        const dim3 grid((p->rows * c.heads + 7) / 8);
-        launch_step(c.head_dim == 64 ? spl_paged_attend_e4m3_kernel<64> : c.head_dim == 128 ? spl_paged_attend_e4m3_kernel<128> : spl_paged_attend_e4m3_kernel<256>, grid, dim3(256), 0, st, p->tables(), p->shape, x);
-        return check_launch(e, "spl_paged_attend_scaled");
-    }
     CUtensorMap k_map, v_map;
     if (!paged_map(p, device_k_cache, false, &k_map) || !paged_map(p, device_v_cache, true, &v_map)) return refuse("the driver takes no tensor map of this cache");
     const bool bf16 = c.dtype == SPL_BF16;
-    if (c.head_dim == 64) { if (bf16) launch_attend<64, true>(p, k_map, v_map, a, st); else launch_attend<64, false>(p, k_map, v_map, a, st); }
+    if (scaled) {
+        const SplPagedScaled scales{k_scale, v_scale};
+        if (c.head_dim == 64) launch_attend_e4m3<64>(p, k_map, v_map, a, scales, st);
+        else if (c.head_dim == 128) launch_attend_e4m3<128>(p, k_map, v_map, a, scales, st);
+        else launch_attend_e4m3<256>(p, k_map, v_map, a, scales, st);
+    } else if (c.head_dim == 64) { if (bf16) launch_attend<64, true>(p, k_map, v_map, a, st); else launch_attend<64, false>(p, k_map, v_map, a, st); }
     else if (c.head_dim == 128) { if (bf16) launch_attend<128, true>(p, k_map, v_map, a, st); else launch_attend<128, false>(p, k_map, v_map, a, st); }
     else { if (bf16) launch_attend<256, true>(p, k_map, v_map, a, st); else launch_attend<256, false>(p, k_map, v_map, a, st); }
     if (joint) {

@@ -113,17 +113,33 @@ def test_scores_far_apart_and_a_maximum_that_keeps_rising(engine):
     check(scene, attend(engine, scene, "f32"), "f32")
 
 
-@pytest.mark.parametrize("spread", [8.0, 20.0])
-def test_values_of_very_different_sizes(engine, spread):
+def test_values_of_very_different_sizes(engine):
     """Scales of values that span many powers of two, scales of zero among them: every row's own largest products count, whatever others' are."""
-    scene = Scene(int(spread), 4, 2, 128, [3, 60, 1], [300, 200, 1000], page_tokens=32)
+    scene = Scene(8, 4, 2, 128, [3, 60, 1], [300, 200, 1000], page_tokens=32)
     g = torch.Generator().manual_seed(5)
     for s, (_, _, _, v_scale) in enumerate(scene.tokens):
-        v_scale.copy_((v_scale * torch.exp2(spread * torch.randn(v_scale.shape, generator=g, dtype=torch.float64))).float().double())
+        v_scale.copy_((v_scale * torch.exp2(8.0 * torch.randn(v_scale.shape, generator=g, dtype=torch.float64))).float().double())
         v_scale[::7] = 0.0
         for i in range(-(-v_scale.shape[0] // 32)):
             part = v_scale[i * 32:(i + 1) * 32]
             scene.vs[scene.table[s, i], :, :part.shape[0]] = part.transpose(0, 1).float().cuda()
+    check(scene, attend(engine, scene, "f32"), "f32")
+
+
+def test_value_scales_out_of_range(engine):
+    """Negative ones and those above 2^40 are no numbers for whoever sees their token; at 2^40 and beside zeros all is as defined, and the smallest count as 2^-60."""
+    scene = Scene(9, 4, 2, 128, [140], [140], page_tokens=64)
+    good = attend(engine, scene, "f32")
+    for value in (-1.0, -1e-30, 1.1e12, float("inf")):
+        scene.vs[scene.table[0, 1], 0, 6] = value               # token 70 of the first kv head
+        out = attend(engine, scene, "f32")
+        assert out[70:, :2].isnan().all() and torch.equal(out[:, 2:], good[:, 2:])
+    for value, as_if in ((2.0 ** 40, 2.0 ** 40), (0.0, 2.0 ** -60), (1e-38, 2.0 ** -60), (2.0 ** -61, 2.0 ** -60)):
+        scene.vs[scene.table[0, 1], 0, 6] = value
+        scene.tokens[0][3][70, 0] = as_if
+        check(scene, attend(engine, scene, "f32"), "f32")
+    scene.vs[scene.vs.isfinite()] = 0.0
+    scene.tokens[0][3][:] = 2.0 ** -60
     check(scene, attend(engine, scene, "f32"), "f32")
 
 
