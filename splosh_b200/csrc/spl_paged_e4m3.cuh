@@ -72,13 +72,26 @@ template <typename Op> __device__ __forceinline__ float spl_paged8_reduce(const 
     const float a = op(high ? v[2] : v[0], __shfl_xor_sync(0xffffffffu, high ? v[0] : v[2], 2)), b = op(high ? v[3] : v[1], __shfl_xor_sync(0xffffffffu, high ? v[1] : v[3], 2));
     return op(odd ? b : a, __shfl_xor_sync(0xffffffffu, odd ? a : b, 1));
 }
-// The four warps of 32 rows: barriers 1 to 4.
-__device__ __forceinline__ void spl_paged8_barrier(int quarter) {
-    if (quarter == 0) spl_named_barrier<1, 128>();
-    else if (quarter == 1) spl_named_barrier<2, 128>();
-    else if (quarter == 2) spl_named_barrier<3, 128>();
+// Four warps meet: barriers 1 to 4; and whether any of their threads says so.
+__device__ __forceinline__ void spl_paged8_barrier(int which) {
+    if (which == 0) spl_named_barrier<1, 128>();
+    else if (which == 1) spl_named_barrier<2, 128>();
+    else if (which == 2) spl_named_barrier<3, 128>();
     else spl_named_barrier<4, 128>();
 }
+template <int ID> __device__ __forceinline__ bool spl_named_barrier_or(bool mine) {
+    uint32_t any;
+    asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.or.pred q, %2, 128, p;\n selp.u32 %0, 1, 0, q;\n}\n" : "=r"(any) : "r"(uint32_t(mine)), "n"(ID) : "memory");
+    return any;
+}
+__device__ __forceinline__ bool spl_paged8_barrier_or(int which, bool mine) {
+    return which == 0 ? spl_named_barrier_or<1>(mine) : which == 1 ? spl_named_barrier_or<2>(mine) : which == 2 ? spl_named_barrier_or<3>(mine) : spl_named_barrier_or<4>(mine);
+}
+// A row's P are 2^(y + offset), offset = 7 - reference. While no y + offset of a tile is above SPL_PAGED8_MOST the reference may stay, and nobody looks for a maximum; a row that has seen nothing has an offset that takes any number above that.
+#define SPL_PAGED8_MOST 15.0f
+#define SPL_PAGED8_UNSEEN 1.0e30f
+__device__ __forceinline__ float spl_lg2(float x) { float y; asm("lg2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x)); return y; }
+__device__ __forceinline__ float spl_rcp(float x) { float y; asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x)); return y; }
 
 template <int HD>
 __global__ void __launch_bounds__(SPL_PAGED8_THREADS, 1)
@@ -264,7 +277,7 @@ spl_paged_attend_e4m3_kernel(const __grid_constant__ CUtensorMap k_map, const __
             float *to = scale_ring + (tile % NS) * 3 * 128 + mine;
             const bool there = x.place >= 0;
             const float v = x.v >= 0.0f && x.v <= SPL_PAGED8_SCALE_MOST ? fmaxf(x.v, SPL_PAGED8_SCALE_LEAST) : __int_as_float(0x7fffffff);
-            to[0] = there ? x.k : 0.0f; to[128] = there ? log2f(v) : 0.0f; to[256] = there ? 1.0f / v : 0.0f;
+            to[0] = there ? x.k : 0.0f; to[128] = there ? spl_lg2(v) : 0.0f; to[256] = there ? spl_rcp(v) : 0.0f;
             __syncwarp();
             if (lane == 0) spl_mbar_arrive(&scaled[tile % NS]);
         };
@@ -393,7 +406,7 @@ spl_paged_attend_e4m3_kernel(const __grid_constant__ CUtensorMap k_map, const __
             float ref = -INFINITY, c[4], offset[4];
             float2 sum[4];
 #pragma unroll
-            for (int n = 0; n < 4; ++n) { c[n] = 0.0f; offset[n] = PBIAS; sum[n] = make_float2(0.0f, 0.0f); }      // a row that has seen nothing yet: all its y are -inf
+            for (int n = 0; n < 4; ++n) { c[n] = 0.0f; offset[n] = SPL_PAGED8_UNSEEN; sum[n] = make_float2(0.0f, 0.0f); }
             for (; tile < tile_end; ++tile, ++tiles) {
                 const int buf = tiles & 1;
                 wait(&scaled[tiles % NS], tiles / NS, 73);
@@ -437,19 +450,22 @@ spl_paged_attend_e4m3_kernel(const __grid_constant__ CUtensorMap k_map, const __
                         }
                     }
                     float most[4];
+                    bool over = false;
 #pragma unroll
                     for (int n = 0; n < 4; ++n) {
                         const uint32_t *z = x + n / 2 * 16 + n % 2 * 2;
                         most[n] = fmaxf(__uint_as_float(z[0]), __uint_as_float(z[1]));
 #pragma unroll
                         for (int j = 1; j < 4; ++j) most[n] = fmaxf(most[n], fmaxf(__uint_as_float(z[4 * j]), __uint_as_float(z[4 * j + 1])));
+                        over |= most[n] + offset[n] > SPL_PAGED8_MOST;
                     }
-                    float *others = xmax + buf * 4 * 128 + own;
-                    others[part * 128] = spl_paged8_reduce(most, lane, [](float u, float v) { return fmaxf(u, v); });
-                    spl_paged8_barrier(quarter);
-                    const float m = fmaxf(fmaxf(others[0], others[128]), fmaxf(others[256], others[384]));
-                    const bool raise = m > ref + SPL_PAGED_HEADROOM;
-                    if (__any_sync(0xffffffffu, raise)) {
+                    if (spl_paged8_barrier_or(quarter, over)) {
+                        // Some rows' references rise to their maxima: over the four lanes that share a row, then over the four warps.
+                        float *others = xmax + buf * 4 * 128 + own;
+                        others[part * 128] = spl_paged8_reduce(most, lane, [](float u, float v) { return fmaxf(u, v); });
+                        spl_paged8_barrier(quarter);
+                        const float m = fmaxf(fmaxf(others[0], others[128]), fmaxf(others[256], others[384]));
+                        const bool raise = m > ref + (SPL_PAGED8_MOST - PBIAS);
                         const float old = raise ? exp2f(ref - m) : 1.0f;
                         if (tile > tile_begin) {
                             // The product before has to be done with these sums; the next waits for this warp's probabilities.
@@ -466,7 +482,7 @@ spl_paged_attend_e4m3_kernel(const __grid_constant__ CUtensorMap k_map, const __
                             }
                         }
                         if (raise) ref = m;
-                        const float now = (ref == -INFINITY ? 0.0f : -ref) + PBIAS;
+                        const float now = ref == -INFINITY ? SPL_PAGED8_UNSEEN : PBIAS - ref;
 #pragma unroll
                         for (int n = 0; n < 4; ++n) {
                             const float f = __shfl_sync(0xffffffffu, old, (lane & 28) + n);
@@ -568,16 +584,23 @@ spl_paged_attend_e4m3_kernel(const __grid_constant__ CUtensorMap k_map, const __
 // A piece of at most 48 packed rows (single tokens, verify blocks) would leave most of the rows above empty, and has no rows to spread a tile's conversion over. Here the cache is the A operand of both products, as it
 // lies there, and the rows are columns:
 //   S^T[128 tokens x 2 N]       = K [hi; lo]^T            A = K (tokens by channels), B = the N queries' two parts, so that K is read once; a score is the sum of two columns
-//   O^T[128 channels x 3 N]    += V^T [P1; P2; P3]        A = V (a block of 128 channels), B = P in three parts, K-major: a row of 128 tokens for each row and part
+//   O^T[128 channels x 3 N]    += V^T [P1; P2; P3]        A = V (a block of 128 channels), B = P in three parts: units of sixteen columns of one part, sixteen bytes a token, token after token
 // P is a number in fp16, of which e5m2 is the upper byte: P1 is that byte, P2 the upper byte of what it leaves, P3 that of what both leave, rounded: nine significant bits or more over all of fp16's range. The parts' sums are
-// columns of their own and are added at the piece's end.
-// A softmax thread has a token, and half of the columns (warps 0-3 the first half, 4-7 the second): the token's scales are its own registers, a row's maximum is a reduction over lanes (redux) and four warps, its sum stays
-// in the threads until the piece's end. Warps 8 and 11 copy, 9 and 10 issue the products.
+// columns of their own and are added at the piece's end. (A unit is the operand's layout without a swizzle, its columns the inner dimension: a thread stores its part of a unit at once. With a row of 128 tokens for each column a
+// tile's probabilities were 48 one-byte stores a thread and half of the softmax's time.)
+// A softmax thread has a token, and 8 or 16 of the columns (groups of four warps share these out): the token's scales, which came with its keys, are its own registers, a row's maximum, where one is wanted, is a reduction over lanes (redux) and
+// four warps, its sum stays in the threads until the piece's end. The last four warps copy keys, issue the scores' and the sums' products, copy values.
 // A tile of 128 tokens by 256 channels is 64 KB from memory (some 2,700 cycles at an SM's share); the products take 400 cycles of the tensor cores with 16 rows.
 #define SPL_PAGED8_NARROW 48            // packed rows at most
-__host__ __device__ constexpr int spl_paged8n_ring(int n) { return n == 16 ? 6 : 5; }      // chunks of 128 tokens by 128 channels, of keys and of values
+__host__ __device__ constexpr int spl_paged8n_groups(int n) { return n == 48 ? 3 : 2; }
+__host__ __device__ constexpr int spl_paged8n_threads(int n) { return 128 * spl_paged8n_groups(n) + 128; }
+// Chunks of 128 tokens by 128 channels, of keys and of values.
+__host__ __device__ constexpr int spl_paged8n_ring_k(int n) { return n == 16 ? 6 : 5; }
+__host__ __device__ constexpr int spl_paged8n_ring_v(int n) { return n == 16 ? 6 : n == 32 ? 5 : 4; }
+// Tiles of scales. Those of tile j come with its first keys, which waited for the scores of tile j - ring / blocks or a later one, and these for the softmax of the tile two before.
+__host__ __device__ constexpr int spl_paged8n_scales(int hd, int n) { return (spl_paged8n_ring_k(n) * 128 + hd - 1) / hd + 2; }
 __host__ __device__ constexpr size_t spl_paged8n_smem_bytes(int hd, int n) {
-    return size_t(2 * spl_paged8n_ring(n)) * 16384 + size_t(2) * n * hd /* Q */ + size_t(2) * 3 * n * 128 /* P */ + 1024 /* joins */ + size_t(2 + 8) * n * 4 /* factors, maxima */ + 512 /* barriers */;
+    return size_t(spl_paged8n_ring_k(n) + spl_paged8n_ring_v(n)) * 16384 + size_t(2) * n * hd /* Q */ + size_t(2) * 3 * n * 128 /* P */ + size_t(spl_paged8n_scales(hd, n)) * 1024 + size_t(2 + 8) * n * 4 /* factors, maxima */ + 512 /* barriers */;
 }
 __device__ __forceinline__ void spl_tc_ld8_later(uint32_t *r, uint32_t taddr) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(taddr));
@@ -600,31 +623,37 @@ __device__ __forceinline__ uint32_t spl_half2_sub(uint32_t a, uint32_t b) {
     return *reinterpret_cast<const uint32_t *>(&d);
 }
 
+// Columns inner, without a swizzle: sixteen columns (bytes) of a token, eight tokens 128 bytes, the next eight behind them; the next sixteen columns 2,048 bytes on.
+__device__ __forceinline__ uint64_t spl_paged8n_p_desc(uint32_t addr) {
+    return uint64_t((addr & 0x3FFFFu) >> 4) | uint64_t(128 >> 4) << 16 | uint64_t(2048 >> 4) << 32 | uint64_t(1) << 46;
+}
+
 template <int HD, int N>
-__global__ void __launch_bounds__(384, 1)
+__global__ void __launch_bounds__(spl_paged8n_threads(N), 1)
 spl_paged_attend_e4m3_narrow_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, SplPagedTables t, SplPagedShape s, SplPagedAttend a, SplPagedScaled scales) {
-    constexpr int RING = spl_paged8n_ring(N), BLOCKS = HD / 128, H = N / 2, CHUNK = 16384, PBYTES = 3 * N * 128;      // H: a softmax thread's columns
+    constexpr int NK = spl_paged8n_ring_k(N), NV = spl_paged8n_ring_v(N), NS = spl_paged8n_scales(HD, N), BLOCKS = HD / 128, GROUPS = spl_paged8n_groups(N), H = N / GROUPS, CHUNK = 16384, PBYTES = 3 * N * 128;      // H: a softmax thread's columns
+    constexpr int SOFTMAX = 4 * GROUPS, COPY_K = SOFTMAX, SCORES = COPY_K + 1, SUMS = COPY_K + 2, COPY_V = COPY_K + 3;
     constexpr float PBIAS = 7.0f;
     extern __shared__ __align__(1024) unsigned char spl_paged8n_raw[];
     if (spl_smem_addr(spl_paged8n_raw) % 1024) { if (threadIdx.x == 0) a.error_flag[0] = 299; return; }
-    unsigned char *ring = spl_paged8n_raw, *v_ring = ring + RING * CHUNK, *q_tile = v_ring + RING * CHUNK, *p_tile = q_tile + 2 * N * HD;
-    float *scratch = reinterpret_cast<float *>(p_tile + 2 * PBYTES), *factor = scratch + 256, *xmax = factor + 2 * N;      // [item parity][column]; [tile parity][quarter of the tokens][column]
+    unsigned char *ring = spl_paged8n_raw, *v_ring = ring + NK * CHUNK, *q_tile = v_ring + NV * CHUNK, *p_tile = q_tile + 2 * N * HD;
+    float *scale_ring = reinterpret_cast<float *>(p_tile + 2 * PBYTES), *factor = scale_ring + NS * 256, *xmax = factor + 2 * N;      // [tile % NS][keys', values'][token]; [item parity][column]; [tile parity][quarter of the tokens][column]
     uint64_t *bars = reinterpret_cast<uint64_t *>(xmax + 8 * N);
-    uint64_t *full_k = bars, *empty_k = full_k + RING, *full_v = empty_k + RING, *empty_v = full_v + RING, *s_full = empty_v + RING, *p_full = s_full + 2, *o_done = p_full + 2, *q_full = o_done + 2, *drained = q_full + 1;
+    uint64_t *full_k = bars, *empty_k = full_k + NK, *full_v = empty_k + NK, *empty_v = full_v + NV, *scaled = empty_v + NV, *s_full = scaled + NS, *p_full = s_full + 2, *o_done = p_full + 2, *q_full = o_done + 2, *drained = q_full + 1;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drained + 2);
     volatile int *abort = reinterpret_cast<volatile int *>(tmem_slot + 1), *joins = abort + 1;
     auto uniform = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
     const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
 
     if (tid == 0) {
-        for (int i = 0; i < 4 * RING; ++i) spl_mbar_init(&bars[i], 1);
-        for (int i = 0; i < 2; ++i) { spl_mbar_init(&s_full[i], 1); spl_mbar_init(&p_full[i], 8); spl_mbar_init(&o_done[i], 1); }
-        spl_mbar_init(q_full, 8); spl_mbar_init(&drained[0], 1); spl_mbar_init(&drained[1], 1);
+        for (int i = 0; i < 2 * NK + 2 * NV + NS; ++i) spl_mbar_init(&bars[i], 1);
+        for (int i = 0; i < 2; ++i) { spl_mbar_init(&s_full[i], 1); spl_mbar_init(&p_full[i], SOFTMAX); spl_mbar_init(&o_done[i], 1); }
+        spl_mbar_init(q_full, SOFTMAX); spl_mbar_init(&drained[0], 1); spl_mbar_init(&drained[1], 1);
         *abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
-    if (tid == 256) { spl_tma_prefetch(&k_map); spl_tma_prefetch(&v_map); }
-    if (warp == 9) {
+    if (tid == 32 * COPY_K) { spl_tma_prefetch(&k_map); spl_tma_prefetch(&v_map); }
+    if (warp == SCORES) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(spl_smem_addr(tmem_slot)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
     }
@@ -645,7 +674,7 @@ spl_paged_attend_e4m3_narrow_kernel(const __grid_constant__ CUtensorMap k_map, c
     };
     auto inside_page = [&](int tile) { return s.page_tokens > 128 ? (tile & 1) * 128 : 0; };
     auto present = [&](const SplPagedItem &it, int tile) { return (min(128, it.length - tile * 128) + box - 1) / box; };
-    const bool copies = warp == 8 || warp == 11, keys = warp == 8;
+    const bool copies = warp == COPY_K || warp == COPY_V, keys = warp == COPY_K;
     const CUtensorMap *map = keys ? &k_map : &v_map;
     const int first_page = copies && item0 < item1 ? page_of(first_item, first_item.tile_begin) : 0;
     if (copies && item0 < item1) {
@@ -667,31 +696,45 @@ spl_paged_attend_e4m3_narrow_kernel(const __grid_constant__ CUtensorMap k_map, c
     if (copies) {
         uint64_t *full = keys ? full_k : full_v, *empty = keys ? empty_k : empty_v;
         unsigned char *to = keys ? ring : v_ring;
-        int n = 0, st = 0;
+        const int slots = keys ? NK : NV;
+        int n = 0, st = 0, tiles = 0;
         SplPagedItem it = first_item;
         int page = first_page;
         for (int i = item0; i < item1 && ok; ++i) {
             if (i > item0) { it = a.items[i]; page = page_of(it, it.tile_begin); }
-            for (int tile = it.tile_begin; tile < it.tile_end && ok; ++tile) {
+            for (int tile = it.tile_begin; tile < it.tile_end && ok; ++tile, ++tiles) {
                 const int ahead = page_of(it, tile + 1), inside = inside_page(tile), there = present(it, tile);
-                for (int c = 0; c < BLOCKS && wait(&empty[st], n / RING + 1, 60); ++c) {
+                for (int c = 0; c < BLOCKS && wait(&empty[st], n / slots + 1, 60); ++c) {
+                    if (keys && c == 0) {
+                        // The tile's scales, as many as there are pages for.
+                        const int sl = tiles % NS;
+                        if (lane == 0) spl_mbar_expect_tx(&scaled[sl], uint32_t(there) * box * 8);
+                        __syncwarp();
+                        if (lane < there) {
+                            const size_t at = (size_t(page) * s.kv_heads + it.kv_head) * s.page_tokens + inside;
+                            spl_bulk_g2s(scale_ring + sl * 256 + lane * box, scales.k + at, box * 4, &scaled[sl]);
+                            spl_bulk_g2s(scale_ring + sl * 256 + 128 + lane * box, scales.v + at, box * 4, &scaled[sl]);
+                        }
+                    }
                     if (lane == 0) spl_mbar_expect_tx(&full[st], uint32_t(there) * box * 128);
                     __syncwarp();
                     if (lane < there) spl_tma_load5(to + st * CHUNK + lane * box * 128, map, 0, inside, c, it.kv_head, page, &full[st]);
-                    ++n; st = st + 1 == RING ? 0 : st + 1;
+                    ++n; st = st + 1 == slots ? 0 : st + 1;
                 }
                 page = ahead;
             }
         }
         // Nothing may still be on its way into the block's shared memory when it is handed on.
-        for (int z = 0; z < RING && z < n; ++z) spl_mbar_wait(&full[z], ((z + (n - 1 - z) / RING * RING) / RING) & 1);
-    } else if (warp == 9 || warp == 10) {
+        for (int z = 0; z < slots && z < n; ++z) spl_mbar_wait(&full[z], ((z + (n - 1 - z) / slots * slots) / slots) & 1);
+        const int copied = (n + BLOCKS - 1) / BLOCKS;
+        if (keys) for (int z = 0; z < NS && z < copied; ++z) spl_mbar_wait(&scaled[z], ((z + (copied - 1 - z) / NS * NS) / NS) & 1);
+    } else if (warp == SCORES || warp == SUMS) {
         const uint32_t elected = spl_elect_one() ? 1u : 0u;
-        const bool scores = warp == 9;
-        // Scores: e4m3 by e4m3, both K-major. Sums: A = V, e4m3 with its channels (M) in rows of the tokens, B = P, e5m2 (format 1), K-major.
-        constexpr uint32_t s_idesc = spl_tc_idesc(2 * N), o_idesc = spl_tc_idesc(3 * N) | 1u << 10 | 1u << 15;
+        const bool scores = warp == SCORES;
+        // Scores: e4m3 by e4m3, both K-major. Sums: A = V, e4m3 with its channels (M) in rows of the tokens, B = P, e5m2 (format 1), its columns (N) in the tokens' sixteen bytes.
+        constexpr uint32_t s_idesc = spl_tc_idesc(2 * N), o_idesc = spl_tc_idesc(3 * N) | 1u << 10 | 1u << 15 | 1u << 16;
         const uint64_t k_desc = spl_tc_desc_sw128(spl_smem_addr(ring)), q_desc = spl_tc_desc_sw128(spl_smem_addr(q_tile)), v_desc = spl_tc_desc_mn_sw128(spl_smem_addr(v_ring), CHUNK),
-                       p_desc = spl_tc_desc_sw128(spl_smem_addr(p_tile));
+                       p_desc = spl_paged8n_p_desc(spl_smem_addr(p_tile));
         int n = 0, tiles = 0;
         for (int i = item0; i < item1 && ok; ++i) {
             const SplPagedItem it = a.items[i];
@@ -700,12 +743,12 @@ spl_paged_attend_e4m3_narrow_kernel(const __grid_constant__ CUtensorMap k_map, c
                 if (!wait(q_full, i - item0, 63)) break;
                 for (int tile = 0; tile < count && ok; ++tile) {
                     const int at = tiles + tile;
-                    if (!wait(&full_k[n % RING], n / RING, 62)) break;
-                    if (at >= 2 && !wait(&p_full[at & 1], (at - 2) >> 1, 61)) break;      // tile at - 2's scores have been read
+                    if (!wait(&full_k[n % NK], n / NK, 62)) break;
+                    if (at >= 2 && !wait(&o_done[at & 1], (at - 2) >> 1, 61)) break;      // tile at - 2's scores have been read, and its P: whoever sees these scores may write over that
 #pragma unroll
                     for (int c = 0; c < BLOCKS; ++c, ++n) {
-                        const int st = n % RING;
-                        if (c > 0 && !wait(&full_k[st], n / RING, 62)) break;
+                        const int st = n % NK;
+                        if (c > 0 && !wait(&full_k[st], n / NK, 62)) break;
                         spl_tc_fence_after();
 #pragma unroll
                         for (int ks = 0; ks < 4; ++ks)
@@ -719,8 +762,8 @@ spl_paged_attend_e4m3_narrow_kernel(const __grid_constant__ CUtensorMap k_map, c
                 for (int tile = 0; tile < count && ok; ++tile) {
                     const int at = tiles + tile, token0 = (tile_begin + tile) * 128, from = max(0, from_all - token0), to = min(128, to_all - token0), k0 = from / 32, k1 = (to + 31) / 32;
                     for (int c = 0; c < BLOCKS && ok; ++c, ++n) {
-                        const int st = n % RING;
-                        if (!wait(&full_v[st], n / RING, 65)) break;
+                        const int st = n % NV;
+                        if (!wait(&full_v[st], n / NV, 65)) break;
                         if (from % 32 || to % 32) {
                             // Values of unseen tokens in the first and last groups of 32: zero, whatever the cache holds there (0 x NaN is no number).
                             const int before = from % 32, after = (32 - to % 32) % 32;
@@ -734,7 +777,7 @@ spl_paged_attend_e4m3_narrow_kernel(const __grid_constant__ CUtensorMap k_map, c
                         if (c == 0 && !wait(&p_full[at & 1], at >> 1, 64)) break;
                         spl_tc_fence_after();
                         for (int ks = k0; ks < k1; ++ks)      // (the piece's first product overwrites what the sums held)
-                            spl_tc_mma8_ss_if(elected, tmem_o + c * 3 * N, v_desc + uint64_t((st * CHUNK + ks * 4096) >> 4), p_desc + uint64_t(((at & 1) * PBYTES + ks * 32) >> 4), o_idesc, tile > 0 || ks > k0 ? 1u : 0u);
+                            spl_tc_mma8_ss_if(elected, tmem_o + c * 3 * N, v_desc + uint64_t((st * CHUNK + ks * 4096) >> 4), p_desc + uint64_t(((at & 1) * PBYTES + ks * 512) >> 4), o_idesc, tile > 0 || ks > k0 ? 1u : 0u);
                         spl_tc_commit_if(elected, &empty_v[st]);
                         if (c == BLOCKS - 1) spl_tc_commit_if(elected, &o_done[at & 1]);
                     }
@@ -745,99 +788,94 @@ spl_paged_attend_e4m3_narrow_kernel(const __grid_constant__ CUtensorMap k_map, c
         // No product may still read shared or write tensor memory when they are handed on.
         spl_tc_commit_if(elected, &drained[scores ? 0 : 1]);
         spl_mbar_wait(&drained[scores ? 0 : 1], 0);
-    } else if (warp < 8) {
+    } else {
         // ---- softmax: token `mine` of a tile, the columns [n0, n0 + H).
-        const int quarter = warp & 3, half = warp >> 2, mine = quarter * 32 + lane, n0 = half * H;
+        const int quarter = warp & 3, group = warp >> 2, mine = quarter * 32 + lane, n0 = group * H;
         const uint32_t lanes = uint32_t(quarter * 32) << 16;
         const uint32_t per_group = (65536u + s.group - 1) / s.group;      // x / group = x * per_group >> 16 for x below 192
-        auto barrier = [&]() { if (half == 0) spl_named_barrier<1, 128>(); else spl_named_barrier<2, 128>(); };
         // A piece's queries: rows n of the operand the upper parts, N + n the rest; columns without a query are zeros.
-        auto bring_q = [&](const SplPagedItem &it, int parity) {
-            const int row0 = it.row0 + it.q0 / s.group, head0 = it.q0 % s.group, pieces = it.q_count * (HD / 8);
-#pragma unroll 1
-            for (int base = 0; base < N * (HD / 8); base += 2 * 256) {
-                uint4 v[2];
+        constexpr int PIECES = N * (HD / 8), EACH = (PIECES + 32 * SOFTMAX - 1) / (32 * SOFTMAX);      // sixteen bytes of queries; a thread's
+        auto load_q = [&](const SplPagedItem &it, uint4 (&v)[EACH]) {
+            const int row0 = it.row0 + it.q0 / s.group, head0 = it.q0 % s.group;
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const int idx = base + u * 256 + tid, x = head0 + idx / (HD / 8), row = int(x * per_group >> 16);
-                    v[u] = make_uint4(0u, 0u, 0u, 0u);
-                    if (idx < pieces) v[u] = *reinterpret_cast<const uint4 *>(a.q + (size_t(row0 + row) * s.heads + it.kv_head * s.group + (x - row * s.group)) * HD + idx % (HD / 8) * 8);
+            for (int u = 0; u < EACH; ++u) {
+                const int idx = u * 32 * SOFTMAX + tid, x = head0 + idx / (HD / 8), row = int(x * per_group >> 16);
+                v[u] = make_uint4(0u, 0u, 0u, 0u);
+                if (idx < it.q_count * (HD / 8)) v[u] = *reinterpret_cast<const uint4 *>(a.q + (size_t(row0 + row) * s.heads + it.kv_head * s.group + (x - row * s.group)) * HD + idx % (HD / 8) * 8);
+            }
+        };
+        // (Held in registers over a tile they would be the softmax's: the next piece's come to L1 while the last tile runs.)
+        auto ask_q = [&](const SplPagedItem &it) {
+            const int row0 = it.row0 + it.q0 / s.group, head0 = it.q0 % s.group;
+#pragma unroll
+            for (int u = 0; u < EACH; ++u) {
+                const int idx = u * 32 * SOFTMAX + tid, x = head0 + idx / (HD / 8), row = int(x * per_group >> 16);
+                if (idx % 8 == 0 && idx < it.q_count * (HD / 8)) asm volatile("prefetch.global.L1 [%0];\n" ::"l"(a.q + (size_t(row0 + row) * s.heads + it.kv_head * s.group + (x - row * s.group)) * HD + idx % (HD / 8) * 8));
+            }
+        };
+        auto place_q = [&](const uint4 (&v)[EACH], int q_count, int parity) {
+#pragma unroll
+            for (int u = 0; u < EACH; ++u) {
+                const int idx = u * 32 * SOFTMAX + tid, piece = idx % (HD / 8), n = idx / (HD / 8);
+                const uint32_t w[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+                uint32_t most = 0u;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) most = max(most, max(w[e] & 0x7fffu, w[e] >> 16 & 0x7fffu));
+#pragma unroll
+                for (int o = HD / 16; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+                const int up = min(261 - int(most >> 7), 253);      // (as above)
+                const float f = __uint_as_float(uint32_t(up) << 23);
+                uint16_t hi[4], lo[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float2 x = spl_unpack16<true>(w[e]), y = make_float2(x.x * f, x.y * f);
+                    hi[e] = spl_pack_e4m3(y.x, y.y);
+                    const uint32_t back = spl_halves_of_e4m3(hi[e]);
+                    const float2 z = __half22float2(*reinterpret_cast<const __half2 *>(&back));
+                    lo[e] = spl_pack_e4m3(y.x - z.x, y.y - z.y);
                 }
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    if (base + u * 256 >= N * (HD / 8)) break;
-                    const int idx = base + u * 256 + tid, piece = idx % (HD / 8), n = idx / (HD / 8);
-                    const uint32_t w[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
-                    uint32_t most = 0u;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) most = max(most, max(w[e] & 0x7fffu, w[e] >> 16 & 0x7fffu));
-#pragma unroll
-                    for (int o = HD / 16; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-                    const int up = min(261 - int(most >> 7), 253);      // (as above)
-                    const float f = __uint_as_float(uint32_t(up) << 23);
-                    uint16_t hi[4], lo[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float2 x = spl_unpack16<true>(w[e]), y = make_float2(x.x * f, x.y * f);
-                        hi[e] = spl_pack_e4m3(y.x, y.y);
-                        const uint32_t back = spl_halves_of_e4m3(hi[e]);
-                        const float2 z = __half22float2(*reinterpret_cast<const __half2 *>(&back));
-                        lo[e] = spl_pack_e4m3(y.x - z.x, y.y - z.y);
-                    }
-                    const int place = (piece >> 4) * (2 * N * 128) + n * 128 + (((piece >> 1 & 7) ^ (n & 7)) * 16) + (piece & 1) * 8;
-                    *reinterpret_cast<uint2 *>(q_tile + place) = make_uint2(hi[0] | uint32_t(hi[1]) << 16, hi[2] | uint32_t(hi[3]) << 16);
-                    *reinterpret_cast<uint2 *>(q_tile + N * 128 + place) = make_uint2(lo[0] | uint32_t(lo[1]) << 16, lo[2] | uint32_t(lo[3]) << 16);
-                    if (piece == 0) factor[parity * N + n] = n >= it.q_count ? 0.0f : most >= 0x7f80u ? __int_as_float(0x7fffffff) : s.scale * 1.4426950408889634f * __uint_as_float(uint32_t(254 - up) << 23);
-                }
+                if (PIECES % (32 * SOFTMAX) && n >= N) continue;
+                const int place = (piece >> 4) * (2 * N * 128) + n * 128 + (((piece >> 1 & 7) ^ (n & 7)) * 16) + (piece & 1) * 8;
+                *reinterpret_cast<uint2 *>(q_tile + place) = make_uint2(hi[0] | uint32_t(hi[1]) << 16, hi[2] | uint32_t(hi[3]) << 16);
+                *reinterpret_cast<uint2 *>(q_tile + N * 128 + place) = make_uint2(lo[0] | uint32_t(lo[1]) << 16, lo[2] | uint32_t(lo[3]) << 16);
+                if (piece == 0) factor[parity * N + n] = n >= q_count ? 0.0f : most >= 0x7f80u ? __int_as_float(0x7fffffff) : s.scale * 1.4426950408889634f * __uint_as_float(uint32_t(254 - up) << 23);
             }
             spl_fence_proxy_async();
             spl_tc_fence_before();
             __syncwarp();
             if (lane == 0) spl_mbar_arrive(q_full);
         };
-        // The token's scales: its page looked up two tiles and they one tile before they are wanted. place: among the page's scales, negative where no row sees the token.
-        struct Ahead { int page, place; float k, v; };
-        int cursor = item0, tile_at = 0, tile_last = 0, sequence_at = 0, place_at = 0, from = 0, to = 0;
-        const int page_log = 31 - __clz(s.page_tokens);
-        auto enter = [&](const SplPagedItem &it) { tile_at = it.tile_begin; tile_last = it.tile_end; sequence_at = it.sequence; place_at = it.kv_head * s.page_tokens; from = seen_first(it); to = seen_last(it); };
-        auto look = [&]() {
-            Ahead x{0, -1, 0.0f, 0.0f};
-            if (cursor >= item1) return x;
-            const int token = tile_at * 128 + mine;
-            if (token >= from && token < to) { x.place = place_at + (token & (s.page_tokens - 1)); x.page = __ldcg(t.table + size_t(sequence_at) * s.max_pages + (token >> page_log)); }
-            if (++tile_at == tile_last && ++cursor < item1) enter(a.items[cursor]);
-            return x;
-        };
-        auto bring = [&](Ahead &x) {
-            if (x.place < 0) return;
-            const size_t at = size_t(x.page) * (s.kv_heads * s.page_tokens) + x.place;
-            x.k = __ldcg(scales.k + at); x.v = __ldcg(scales.v + at);
-        };
-        Ahead next{}, later{};
-        if (item0 < item1) { enter(first_item); next = look(); later = look(); bring(next); bring_q(first_item, 0); }
-        // The bytes of this token in the rows of P, but for the swizzle's part that goes by the row.
-        const int p_chunk = (quarter * 2 + (lane >> 4)) * 16, p_byte = lane & 15;
+        if (item0 < item1) {
+            uint4 q[EACH];
+            load_q(first_item, q);
+            place_q(q, first_item.q_count, 0);
+        }
         int tiles = 0;
         for (int i = item0; i < item1; ++i) {
-            const SplPagedItem it = a.items[i];
-            auto place_of = [&](int n) { return it.base + it.q0 / s.group + int((it.q0 % s.group + min(n, it.q_count - 1)) * per_group >> 16); };
-            const int seen_by_all = spl_paged_first(s, place_of(N)), unseen_by_some = spl_paged_last(s, place_of(0), it.length);
-            float ref = -INFINITY, c[H], offset[H], sum[H];      // ref: of column n0 + lane
+            // (What the tiles do not need of the item is looked up again where it is wanted.)
+            int seen_by_all, unseen_by_some, tile, tile_begin, tile_end, from, to, row_at, head_at, last_row;
+            {
+                const SplPagedItem it = a.items[i];
+                row_at = it.base + it.q0 / s.group; head_at = it.q0 % s.group; last_row = it.q_count - 1;
+                seen_by_all = spl_paged_first(s, row_at + int(uint32_t(head_at + last_row) * per_group >> 16)); unseen_by_some = spl_paged_last(s, row_at, it.length);
+                tile = tile_begin = it.tile_begin; tile_end = it.tile_end; from = seen_first(it); to = seen_last(it);
+            }
+            float ref = -INFINITY;                                   // of column n0 + lane
+            float2 c[H / 2], offset[H / 2], sum[H / 2];              // of two columns
 #pragma unroll
-            for (int n = 0; n < H; ++n) { c[n] = 0.0f; offset[n] = PBIAS; sum[n] = 0.0f; }      // a row that has seen nothing yet: all its y are -inf
-            for (int tile = it.tile_begin; tile < it.tile_end; ++tile, ++tiles) {
+            for (int n = 0; n < H / 2; ++n) { c[n] = sum[n] = make_float2(0.0f, 0.0f); offset[n] = make_float2(SPL_PAGED8_UNSEEN, SPL_PAGED8_UNSEEN); }
+            for (; tile < tile_end; ++tile, ++tiles) {
                 const int buf = tiles & 1;
-                const Ahead now = next;
-                next = later;
-                bring(next);
-                later = look();
-                const bool there = now.place >= 0;
-                const float v = now.v >= 0.0f && now.v <= SPL_PAGED8_SCALE_MOST ? fmaxf(now.v, SPL_PAGED8_SCALE_LEAST) : __int_as_float(0x7fffffff);
-                const float k = there ? now.k : 0.0f, l = there ? log2f(v) : 0.0f, inv = there ? 1.0f / v : 0.0f;
+                if (tile + 1 == tile_end && i + 1 < item1) ask_q(a.items[i + 1]);
+                wait(&scaled[tiles % NS], tiles / NS, 70);
+                const float *mine_of = scale_ring + tiles % NS * 256 + mine;
+                const bool there = tile * 128 + mine >= from && tile * 128 + mine < to;      // (what no row sees is masked)
+                const float given = mine_of[128], v = given >= 0.0f && given <= SPL_PAGED8_SCALE_MOST ? fmaxf(given, SPL_PAGED8_SCALE_LEAST) : __int_as_float(0x7fffffff);
+                const float k = there ? mine_of[0] : 0.0f, l = there ? spl_lg2(v) : 0.0f, inv = there ? spl_rcp(v) : 0.0f;
                 wait(&s_full[buf], tiles >> 1, 66);
-                if (tile == it.tile_begin) {                         // (all of the queries were there before the scores)
+                if (tile == tile_begin) {                            // (all of the queries were there before the scores)
 #pragma unroll
-                    for (int n = 0; n < H; ++n) c[n] = factor[((i - item0) & 1) * N + n0 + n];
+                    for (int n = 0; n < H / 2; ++n) c[n] = *reinterpret_cast<const float2 *>(factor + ((i - item0) & 1) * N + n0 + 2 * n);
                 }
                 spl_tc_fence_after();
                 uint32_t x[2 * H];
@@ -846,63 +884,82 @@ spl_paged_attend_e4m3_narrow_kernel(const __grid_constant__ CUtensorMap k_map, c
                 for (int n = 0; n < H; n += 8) { spl_tc_ld8_later(x + n, at + n); spl_tc_ld8_later(x + H + n, at + N + n); }
                 spl_tc_ld_done_of<2 * H>(x);
                 // y = score ks c + log2 vs.
-                float y[H];
+                auto two = [](const uint32_t *v) { return make_float2(__uint_as_float(v[0]), __uint_as_float(v[1])); };
+                float2 y[H / 2];
 #pragma unroll
-                for (int n = 0; n < H; ++n) y[n] = fmaf((__uint_as_float(x[n]) + __uint_as_float(x[H + n])) * k, c[n], l);
+                for (int n = 0; n < H / 2; ++n) y[n] = spl_fma2(spl_mul2(spl_add2(two(x + 2 * n), two(x + H + 2 * n)), make_float2(k, k)), c[n], make_float2(l, l));
                 if (tile * 128 < seen_by_all || tile * 128 + 128 > unseen_by_some) {
-                    const int token = tile * 128 + mine;
+                    const int token = tile * 128 + mine, length = a.items[i].length;
+                    auto hidden = [&](int n) {
+                        const int position = row_at + int(uint32_t(head_at + min(n0 + n, last_row)) * per_group >> 16);
+                        return token < spl_paged_first(s, position) || token >= spl_paged_last(s, position, length);
+                    };
 #pragma unroll
-                    for (int n = 0; n < H; ++n) {
-                        const int position = place_of(n0 + n);
-                        if (token < spl_paged_first(s, position) || token >= spl_paged_last(s, position, it.length)) y[n] = -INFINITY;
-                    }
+                    for (int n = 0; n < H / 2; ++n) { if (hidden(2 * n)) y[n].x = -INFINITY; if (hidden(2 * n + 1)) y[n].y = -INFINITY; }
                 }
-                // The columns' maxima: over the warp's tokens, then over the four warps'; lane n has column n0 + n's.
-                float m = -INFINITY;
+                float most = -INFINITY;
 #pragma unroll
-                for (int n = 0; n < H; ++n) { const float most = spl_redux_max(y[n]); if (lane == n) m = most; }
-                float *others = xmax + buf * 4 * N + n0 + lane;
-                if (lane < H) others[quarter * N] = m;
-                barrier();
-                if (lane < H) m = fmaxf(fmaxf(others[0], others[N]), fmaxf(others[2 * N], others[3 * N]));
-                const bool raise = lane < H && m > ref + SPL_PAGED_HEADROOM;
-                if (__any_sync(0xffffffffu, raise)) {
+                for (int n = 0; n < H / 2; ++n) { const float2 z = spl_add2(y[n], offset[n]); most = fmaxf(most, fmaxf(z.x, z.y)); }
+                if (spl_paged8_barrier_or(group, most > SPL_PAGED8_MOST)) {
+                    // Some columns' references rise to their maxima: over the warp's tokens, then over the four warps'; lane n has column n0 + n's.
+                    float m = -INFINITY;
+#pragma unroll
+                    for (int n = 0; n < H; ++n) { const float all = spl_redux_max(n % 2 ? y[n / 2].y : y[n / 2].x); if (lane == n) m = all; }
+                    float *others = xmax + buf * 4 * N + n0 + lane;
+                    if (lane < H) others[quarter * N] = m;
+                    spl_paged8_barrier(group);
+                    if (lane < H) m = fmaxf(fmaxf(others[0], others[N]), fmaxf(others[2 * N], others[3 * N]));
+                    const bool raise = lane < H && m > ref + (SPL_PAGED8_MOST - PBIAS);
                     const float old = raise ? exp2f(ref - m) : 1.0f;
                     if (raise) ref = m;
-                    const float shift = (ref == -INFINITY ? 0.0f : -ref) + PBIAS;
-                    float f[H];
+                    const float shift = ref == -INFINITY ? SPL_PAGED8_UNSEEN : PBIAS - ref;
 #pragma unroll
-                    for (int n = 0; n < H; ++n) { f[n] = __shfl_sync(0xffffffffu, old, n); sum[n] *= f[n]; offset[n] = __shfl_sync(0xffffffffu, shift, n); }
-                    if (tile > it.tile_begin) {
+                    for (int n = 0; n < H / 2; ++n) {
+                        sum[n] = spl_mul2(sum[n], make_float2(__shfl_sync(0xffffffffu, old, 2 * n), __shfl_sync(0xffffffffu, old, 2 * n + 1)));
+                        offset[n] = make_float2(__shfl_sync(0xffffffffu, shift, 2 * n), __shfl_sync(0xffffffffu, shift, 2 * n + 1));
+                    }
+                    if (tile > tile_begin) {
                         // The product before has to be done with these sums; the next waits for this warp's probabilities.
                         wait(&o_done[(tiles - 1) & 1], (tiles - 1) >> 1, 67);
                         spl_tc_fence_after();
+#pragma unroll 1
+                        for (int n = 0; n < H; n += 8) {
+                            float f[8];
 #pragma unroll
-                        for (int n = 0; n < H; n += 8)
+                            for (int j = 0; j < 8; ++j) f[j] = __shfl_sync(0xffffffffu, old, n + j);
 #pragma unroll 1
                             for (int b = 0; b < 3 * BLOCKS; ++b) {
                                 uint32_t o[8];
                                 spl_tc_ld8_later(o, tmem_o + lanes + b * N + n0 + n);
                                 spl_tc_ld_done_of<8>(o);
 #pragma unroll
-                                for (int j = 0; j < 8; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f[n + j]);
+                                for (int j = 0; j < 8; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f[j]);
                                 spl_tc_st8_later(tmem_o + lanes + b * N + n0 + n, o);
                             }
+                        }
                         spl_tc_st_wait();
                     }
                 }
-                if (tiles >= 2) wait(&o_done[buf], (tiles - 2) >> 1, 69);      // P of tile - 2 has been read
-                unsigned char *to_p = p_tile + buf * PBYTES + n0 * 128 + p_byte;
+                // (P of tile - 2 has been read: its scores' place was free for these.)
+                uint32_t part[3][H / 4];
 #pragma unroll
-                for (int n = 0; n < H; n += 2) {
-                    const float e0 = spl_ex2(y[n] + offset[n]), e1 = spl_ex2(y[n + 1] + offset[n + 1]);
-                    sum[n] = fmaf(e0, inv, sum[n]); sum[n + 1] = fmaf(e1, inv, sum[n + 1]);
-                    const uint32_t p = spl_pack16<false>(e0, e1), p1 = p & 0xff00ff00u, rest = spl_half2_sub(p, p1), p2 = rest & 0xff00ff00u;
-                    const uint32_t p3 = spl_e5m2_of_halves(spl_half2_sub(rest, p2));
-                    unsigned char *at0 = to_p + n * 128 + (p_chunk ^ (n0 + n & 7) * 16), *at1 = to_p + (n + 1) * 128 + (p_chunk ^ (n0 + n + 1 & 7) * 16);
-                    at0[0] = (unsigned char)(p1 >> 8); at1[0] = (unsigned char)(p1 >> 24);
-                    at0[N * 128] = (unsigned char)(p2 >> 8); at1[N * 128] = (unsigned char)(p2 >> 24);
-                    at0[2 * N * 128] = (unsigned char)p3; at1[2 * N * 128] = (unsigned char)(p3 >> 8);
+                for (int n = 0; n < H / 4; ++n) {
+                    uint32_t p[2], rest[2], low[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float2 z = spl_add2(y[2 * n + e], offset[2 * n + e]), w = make_float2(spl_ex2(z.x), spl_ex2(z.y));
+                        sum[2 * n + e] = spl_fma2(w, make_float2(inv, inv), sum[2 * n + e]);
+                        p[e] = spl_pack16<false>(w.x, w.y);
+                        rest[e] = spl_half2_sub(p[e], p[e] & 0xff00ff00u);
+                        low[e] = spl_e5m2_of_halves(spl_half2_sub(rest[e], rest[e] & 0xff00ff00u));
+                    }
+                    part[0][n] = __byte_perm(p[0], p[1], 0x7531); part[1][n] = __byte_perm(rest[0], rest[1], 0x7531); part[2][n] = low[0] | low[1] << 16;
+                }
+                unsigned char *to_p = p_tile + buf * PBYTES + n0 / 16 * 2048 + mine * 16 + n0 % 16;
+#pragma unroll
+                for (int e = 0; e < 3; ++e) {
+                    if constexpr (H == 16) *reinterpret_cast<uint4 *>(to_p + e * (N / 16) * 2048) = make_uint4(part[e][0], part[e][1], part[e][2], part[e][3]);
+                    else *reinterpret_cast<uint2 *>(to_p + e * (N / 16) * 2048) = make_uint2(part[e][0], part[e][1]);
                 }
                 spl_fence_proxy_async();
                 spl_tc_fence_before();
@@ -910,16 +967,33 @@ spl_paged_attend_e4m3_narrow_kernel(const __grid_constant__ CUtensorMap k_map, c
                 if (lane == 0) spl_mbar_arrive(&p_full[buf]);
             }
             // The next piece's queries: all scores of this one have been seen, so its own are no longer read. (The sums are overwritten by a product that waits for this warp.)
-            if (i + 1 < item1) bring_q(a.items[i + 1], (i + 1 - item0) & 1);
+            if (i + 1 < item1) {
+                uint4 q[EACH];
+                load_q(a.items[i + 1], q);
+                place_q(q, a.items[i + 1].q_count, (i + 1 - item0) & 1);
+            }
+            const SplPagedItem it = a.items[i];
             // The piece's sums.
             wait(&o_done[(tiles - 1) & 1], (tiles - 1) >> 1, 68);
             spl_tc_fence_after();
-            float all = 0.0f;
+            // Over the lanes: at each step half of the columns stay, and the other half's sums go to the lane that keeps these; lanes that end up with the same column have the same sum.
+            int column = 0;
+            float sums[H];
 #pragma unroll
-            for (int n = 0; n < H; ++n) { const float of_warp = spl_warp_sum(sum[n]); if (lane == n) all = of_warp; }
-            float *others = xmax + (tiles & 1) * 4 * N + n0 + lane;      // (where the maxima of the tile before the last were: nobody reads those any more)
-            if (lane < H) others[quarter * N] = all;
-            barrier();
+            for (int n = 0; n < H / 2; ++n) { sums[2 * n] = sum[n].x; sums[2 * n + 1] = sum[n].y; }
+#pragma unroll
+            for (int o = 16, left = H; o > 0; o >>= 1) {
+                if (left > 1) {
+                    left /= 2;
+                    const bool up = lane & o;
+                    if (up) column += left;
+#pragma unroll
+                    for (int n = 0; n < left; ++n) { const float keep = up ? sums[left + n] : sums[n], give = up ? sums[n] : sums[left + n]; sums[n] = keep + __shfl_xor_sync(0xffffffffu, give, o); }
+                } else sums[0] += __shfl_xor_sync(0xffffffffu, sums[0], o);
+            }
+            float all = 0.0f, *others = xmax + (tiles & 1) * 4 * N + n0 + lane;      // (where the maxima of the tile before the last were: nobody reads those any more)
+            others[quarter * N + column - lane] = sums[0];
+            spl_paged8_barrier(group);
             if (lane < H) all = (others[0] + others[N]) + (others[2 * N] + others[3 * N]);
             const float inv = it.slot < 0 ? 1.0f / all : 1.0f;
             const int row0 = it.row0 + it.q0 / s.group, head0 = it.q0 % s.group;
@@ -945,21 +1019,21 @@ spl_paged_attend_e4m3_narrow_kernel(const __grid_constant__ CUtensorMap k_map, c
                 }
             if (it.slot >= 0 && quarter == 0 && lane < H && n0 + lane < it.q_count) a.partial_ml[slot_row + lane] = make_float2(ref, all);
             spl_tc_fence_before();
-            barrier();                                               // the sums in shared memory are read before the next piece's
+            spl_paged8_barrier(group);                                               // the sums in shared memory are read before the next piece's
             if (it.merge >= 0) {
                 // Whichever block is the last to leave a piece of these rows joins them, in the order of the pieces whoever it is.
                 __threadfence();
-                spl_named_barrier<5, 256>();
+                spl_named_barrier<6, 32 * SOFTMAX>();
                 if (tid == 0) {
                     const bool last = atomicAdd(&a.arrived[it.merge], 1) == it.pieces - 1;
                     if (last) a.arrived[it.merge] = 0;         // for the next launch
                     *joins = last;
                 }
-                spl_named_barrier<5, 256>();
+                spl_named_barrier<6, 32 * SOFTMAX>();
                 if (*joins) {
                     __threadfence();
-                    spl_paged_join<HD, true>(s, a, it, row0, head0, per_group, scratch);
-                    spl_named_barrier<5, 256>();
+                    if (warp < 8) spl_paged_join<HD, true>(s, a, it, row0, head0, per_group, reinterpret_cast<float *>(p_tile));      // (the piece's products have read P)
+                    spl_named_barrier<6, 32 * SOFTMAX>();
                 }
             }
         }
@@ -967,5 +1041,5 @@ spl_paged_attend_e4m3_narrow_kernel(const __grid_constant__ CUtensorMap k_map, c
     spl_tc_fence_before();
     __syncthreads();
     spl_tc_fence_after();
-    if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512) : "memory");
+    if (warp == SCORES) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512) : "memory");
 }

@@ -265,7 +265,7 @@ template <int HD> static void launch_attend_e4m3(const spl_paged *p, const CUten
     if constexpr (HD >= 128) {
         if (paged_narrow(p)) {
             const int n = p->packed <= 16 ? 16 : p->packed <= 32 ? 32 : 48;
-            launch_step(n == 16 ? spl_paged_attend_e4m3_narrow_kernel<HD, 16> : n == 32 ? spl_paged_attend_e4m3_narrow_kernel<HD, 32> : spl_paged_attend_e4m3_narrow_kernel<HD, 48>, dim3(p->e->sms), dim3(384),
+            launch_step(n == 16 ? spl_paged_attend_e4m3_narrow_kernel<HD, 16> : n == 32 ? spl_paged_attend_e4m3_narrow_kernel<HD, 32> : spl_paged_attend_e4m3_narrow_kernel<HD, 48>, dim3(p->e->sms), dim3(spl_paged8n_threads(n)),
                         spl_paged8n_smem_bytes(HD, n), stream, k_map, v_map, p->tables(), p->shape, a, scales);
             return;
         }
