@@ -122,14 +122,16 @@ inline bool spl_paged_groups_check(const spl_paged_config &c, int32_t sequences,
 // decode steps of few sequences; stretches that cut everything spent 25 of 47 us on joining 1-tile pieces of 128 rows in a step of six decoding sessions and a
 // 301-token prompt.)
 #define SPL_PAGED_PIECE_COST 2
-inline int spl_paged_cut_cost(int q_count) { return q_count <= 16 ? 0 : q_count <= 64 ? 1 : 2; }
-inline int spl_paged_cut_least(int q_count) { return q_count <= 16 ? 1 : q_count <= 64 ? 3 : 5; }      // tiles a piece
+inline int spl_paged_cut_cost(int q_count, bool by_rows = false) { return q_count <= 16 ? 0 : q_count <= (by_rows ? 96 : 64) ? 1 : 2; }
+inline int spl_paged_cut_least(int q_count, bool by_rows = false) { return q_count <= 16 ? 1 : q_count > (by_rows ? 96 : 64) ? 5 : by_rows ? 2 : 3; }      // tiles a piece
+// With groups (by_rows) a kernel of its own joins, and pieces of up to 96 rows may be smaller: the 72 packed rows of twelve sequences over 8,192 shared tokens 32.9 -> 25.0 us; the same rule for 128
+// packed rows (eight verify blocks over 20,992 shared tokens) took 61.5 us instead of 55.6.
 // What a block that has `left` of its stretch takes of the `t` tiles left of a unit (cut: some have gone to another block): 0, some, or all; -1: the stretch is too short
 // for this unit's pieces.
-inline int64_t spl_paged_take(int64_t t, int64_t left, int64_t stretch, int q_count, bool cut) {
-    const int64_t piece = SPL_PAGED_PIECE_COST + (cut ? spl_paged_cut_cost(q_count) : 0);
+inline int64_t spl_paged_take(int64_t t, int64_t left, int64_t stretch, int q_count, bool cut, bool by_rows = false) {
+    const int64_t piece = SPL_PAGED_PIECE_COST + (cut ? spl_paged_cut_cost(q_count, by_rows) : 0);
     if (t + piece <= left) return t;
-    const int64_t least = spl_paged_cut_least(q_count), some = left - SPL_PAGED_PIECE_COST - spl_paged_cut_cost(q_count);
+    const int64_t least = spl_paged_cut_least(q_count, by_rows), some = left - SPL_PAGED_PIECE_COST - spl_paged_cut_cost(q_count, by_rows);
     if (t >= 2 * least) {
         if (some >= least) return std::min(some, t - least);    // (a rest is a piece, too)
         return left == stretch ? -1 : 0;
@@ -187,10 +189,10 @@ inline void spl_paged_plan(const spl_paged_config &c, int blocks, int32_t sequen
         int64_t used = 1, left = stretch;
         for (const SplPagedUnit &u : whole)
             for (int64_t t = u.item.tile_end - u.item.tile_begin, all = t; t > 0;) {
-                const int64_t take = spl_paged_take(t, left, stretch, u.item.q_count, t < all || u.joint);
+                const int64_t take = spl_paged_take(t, left, stretch, u.item.q_count, t < all || u.joint, groups);
                 if (take < 0) return int64_t(blocks) + 1;
                 if (!take) { if (++used > blocks) return used; left = stretch; continue; }
-                left -= take + SPL_PAGED_PIECE_COST + (take < all || u.joint ? spl_paged_cut_cost(u.item.q_count) : 0);
+                left -= take + SPL_PAGED_PIECE_COST + (take < all || u.joint ? spl_paged_cut_cost(u.item.q_count, groups) : 0);
                 t -= take;
             }
         return used;
@@ -207,12 +209,12 @@ inline void spl_paged_plan(const spl_paged_config &c, int blocks, int32_t sequen
         const size_t piece0 = units.size();
         const int all = u.tile_end - u.tile_begin;
         for (int t = u.tile_begin; t < u.tile_end;) {
-            const int take = int(spl_paged_take(u.tile_end - t, left, low, u.q_count, t > u.tile_begin || one.joint));
+            const int take = int(spl_paged_take(u.tile_end - t, left, low, u.q_count, t > u.tile_begin || one.joint, groups));
             if (!take) { plan.block_begin.push_back(int32_t(units.size())); left = low; continue; }
             SplPagedItem piece = u;
             piece.tile_begin = t; piece.tile_end = t + take;
             units.push_back(piece);
-            left -= take + SPL_PAGED_PIECE_COST + (take < all || one.joint ? spl_paged_cut_cost(u.q_count) : 0);
+            left -= take + SPL_PAGED_PIECE_COST + (take < all || one.joint ? spl_paged_cut_cost(u.q_count, groups) : 0);
             t += take;
         }
         const int pieces = int(units.size() - piece0);
