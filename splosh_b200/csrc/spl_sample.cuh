@@ -205,6 +205,18 @@ __device__ __forceinline__ unsigned long long spl_verify_off_bins(const SplVerif
     return off;
 }
 
+// The running sums of the bins (kept[], as they were) less what the candidates take off, in sums[].
+__device__ __forceinline__ void spl_verify_left(SplSampleShared &sh, const SplVerifyShared &ve, const unsigned long long *kept) {
+    const int tid = threadIdx.x;
+    __syncthreads();
+    for (int i = tid; i < SPL_SAMPLE_BINS; i += 1024) sh.sums[i] = kept[i] - (i ? kept[i - 1] : 0ull);
+    __syncthreads();
+    if (tid < ve.count && ve.off[tid]) atomicAdd(&sh.sums[ve.bin[tid]], 0ull - ve.off[tid]);
+    __syncthreads();
+    unsigned long long all;
+    spl_sample_running(sh, &all);
+}
+
 // Places found on the row itself, eight bits of the keys at a time, by one block.
 template <bool VERIFY>
 __device__ __noinline__ void spl_sample_slow(const SplSampleArgs &a, const SplSampleRow &r, SplSampleShared &sh, int row, SplVerifyShared *ve) {
@@ -471,25 +483,19 @@ spl_sample_kernel(SplSampleArgs a) {
     r.m = a.min_p && a.min_p[row] > 0.0f && r.t < INFINITY ? fminf(a.min_p[row], 1.0f) : 0.0f; r.k = a.top_k ? a.top_k[row] : 0;
     r.least = r.m > 0.0f ? (unsigned long long)ceil(double(r.m) * SPL_SAMPLE_UNIT) : 0ull;
 
+    // The drafted token and its candidates: one a thread of the first block's, the token itself behind them (without candidates alone, at probability one).
+    int drafted = -1, v_count = 0, v_id = -1;
+    float v_q = 0.0f;
     if constexpr (VERIFY) {
-        // The drafted token and its candidates, their logits on the way beside the row's.
-        const int draft = a.drafts[row];
         if (rank == 0 && tid <= SPL_VERIFY_CANDIDATES) {
-            const int n = draft < 0 ? 0 : a.candidates + 1;      // (without candidates the token alone, at probability one)
-            int id = -1;
-            float q = 0.0f;
-            if (tid < n) {
-                const int *ids = a.candidate_ids + size_t(row) * a.candidates;
-                id = tid < a.candidates ? ids[tid] : draft;
-                q = a.candidates ? 0.0f : 1.0f;
-                bool again = false;
-                for (int i = 0; i < min(tid, a.candidates); ++i) if (ids[i] == id) { if (tid == a.candidates) { q = a.probabilities[size_t(row) * a.candidates + i]; break; } again = true; }
-                if (tid < a.candidates) q = a.probabilities[size_t(row) * a.candidates + tid];
-                const uint32_t key = id >= 0 && id < a.limit ? spl_topk_key(x[id]) : 0u;
-                ve.entry[tid] = key == 0u || again ? 0ull : spl_sample_entry(key, uint32_t(id));
-                ve.q[tid] = q;
+            drafted = a.drafts[row];
+            v_count = drafted < 0 ? 0 : a.candidates + 1;
+            if (tid < a.candidates) { v_id = a.candidate_ids[size_t(row) * a.candidates + tid]; v_q = a.probabilities[size_t(row) * a.candidates + tid]; }
+            if (tid < v_count) {
+                if (tid == a.candidates) v_id = drafted;
+                ve.bin[tid] = v_id; ve.q[tid] = tid < a.candidates ? v_q : a.candidates ? 0.0f : 1.0f;
             }
-            if (tid == 0) { ve.count = n; ve.u0 = a.uniform[2 * row]; ve.stays = 0; }
+            if (tid == 0) { ve.count = v_count; ve.u0 = a.uniform[2 * row]; ve.stays = 0; }
         }
     }
 
@@ -517,6 +523,16 @@ spl_sample_kernel(SplSampleArgs a) {
             best = sh.warp_sum[lane];
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+        }
+        if constexpr (VERIFY) {
+            // Their places in the order (0: no value that may be picked, or listed before); the token's probability is the first of its entries'. (The row has just passed by: its values are near.)
+            if (rank == 0 && tid < v_count) {
+                const uint32_t own = v_id >= 0 && v_id < a.limit ? spl_topk_key(x[v_id]) : 0u;
+                bool again = false;
+                for (int i = 0; i < min(tid, a.candidates); ++i)
+                    if (ve.bin[i] == v_id) { if (tid == a.candidates) { ve.q[tid] = ve.q[i]; break; } again = true; }
+                ve.entry[tid] = own == 0u || again ? 0ull : spl_sample_entry(own, uint32_t(v_id));
+            }
         }
         asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
         if (warp == 0 && lane < blocks) cluster.map_shared_rank(&sh, lane)->best[rank] = best;
@@ -685,8 +701,32 @@ spl_sample_kernel(SplSampleArgs a) {
                 if (p_bin > m1) { c0 = m0; c1 = m1; p_bin = SPL_SAMPLE_BINS; }      // top-p's place comes later
                 else if (p_bin >= m0) { c0 = m0; c1 = m1; }
             }
-            if (VERIFY && c1 >= 0) decide(SPL_SAMPLE_END, c0, c1, cut);      // (what the candidates leave is known when what stays is)
-            else if (c1 >= 0) {
+            if (VERIFY && c1 >= 0) {
+                // What stays weighs between the bins in front and those with them; where the draw lies if the candidates take off what they would of the one and what they might of the other. (Only a guess at the bins to
+                // bring along: the draw is looked for where it is, and has a turn of its own if it is elsewhere.)
+                bool sure = false;
+                if (c0 > 0) {
+                    const unsigned long long low = sh.sums[c0 - 1], high = sh.sums[c1];
+                    // A token in front of these bins whose test does not depend on where in them it ends: it stays, and nothing else is asked.
+                    if (ve.count && tid == 0) {
+                        const unsigned long long entry = ve.entry[ve.count - 1];
+                        sh.found = entry && entry >= cut && ve.bin[ve.count - 1] < c0 && double(ve.u0) * double(ve.q[ve.count - 1]) * double(high) < double(spl_sample_weight(spl_topk_value(uint32_t(entry >> 32)), r.w));
+                    }
+                    __syncthreads();
+                    sure = ve.count && sh.found;
+                    __syncthreads();
+                    if (!sure) {
+                        spl_verify_resolve(ve, r, low, [&](unsigned long long e) { return e >= cut && bin_of(spl_topk_value(uint32_t(e >> 32))) < c0; });
+                        const unsigned long long off = spl_verify_off_bins(ve, c0 - 1), extra = (unsigned long long)(double(off) * (double(high - low) / double(low))) + 64ull;
+                        spl_verify_left(sh, ve, keep);
+                        const int d0 = spl_sample_place(sh, SPL_SAMPLE_BINS, spl_sample_target(r.u, low - min(low, off + extra + (high - low)))),
+                                  d1 = spl_sample_place(sh, SPL_SAMPLE_BINS, spl_sample_target(r.u, high - min(high, off)) + extra);
+                        if (d0 < c0 && min(d1, c0 - 1) - d0 < 8) { also = d0; also_last = max(d0, min(d1, c0 - 1)); }
+                    }
+                }
+                if (sure) { if (tid == 0) a.ids[row] = -1; decide(SPL_SAMPLE_DONE, 0, 0, 0ull); }
+                else decide(SPL_SAMPLE_END, c0, c1, cut, also, also_last);
+            } else if (c1 >= 0) {
                 // Whatever of the bins [c0, c1] stays, the draw mostly lies in one and the same bin, or one of a few: set aside with them, it is found in the same list. (With one bin
                 // alone a fifth of the rows of a vocabulary of 248,077 needed another turn.)
                 const unsigned long long least_sum = c0 ? sh.sums[c0 - 1] : 0ull;
@@ -697,7 +737,7 @@ spl_sample_kernel(SplSampleArgs a) {
                 unsigned long long left = all;
                 if constexpr (VERIFY) {
                     left = spl_verify_resolve(ve, r, all, [&](unsigned long long e) { return e >= cut && bin_of(spl_topk_value(uint32_t(e >> 32))) < SPL_SAMPLE_BINS - 1; });
-                    for (int i = tid; i < SPL_SAMPLE_BINS; i += 1024) sh.sums[i] -= spl_verify_off_bins(ve, i);
+                    spl_verify_left(sh, ve, keep);
                 }
                 const unsigned long long target = spl_sample_target(r.u, left);
                 const int b = spl_sample_place(sh, SPL_SAMPLE_BINS, target);
@@ -759,8 +799,10 @@ spl_sample_kernel(SplSampleArgs a) {
                     target = spl_sample_target(r.u, left);
                     int from = -1, to = stay;
                     unsigned long long shift = 0ull;
+                    unsigned long long also_from = also_base, also_to = also_base + also_sum;
+                    if constexpr (VERIFY) { if (also >= 0) { also_from -= also ? spl_verify_off_bins(ve, also - 1) : 0ull; also_to -= spl_verify_off_bins(ve, also_last); } }
                     if (target > first || base == 0ull) from = front;
-                    else if (also >= 0 && target > also_base && target <= also_base + also_sum) { from = 0; to = front; shift = base - also_sum - also_base; }
+                    else if (also >= 0 && target > also_from && target <= also_to) { from = 0; to = front; shift = base - also_sum - also_base; }
                     else if (also == 0) { from = 0; to = front; shift = base - also_sum; }      // a target of nothing: the first value
                     if (VERIFY && ve.stays) { if (tid == 0) a.ids[row] = -1; decide(SPL_SAMPLE_DONE, 0, 0, 0ull); }
                     else if (from >= 0) {
@@ -773,10 +815,8 @@ spl_sample_kernel(SplSampleArgs a) {
                         decide(SPL_SAMPLE_DONE, 0, 0, 0ull);
                     } else {
                         __syncthreads();
-                        for (int i = tid; i < SPL_SAMPLE_BINS; i += 1024) {
-                            if constexpr (VERIFY) sh.sums[i] = kept[i] - spl_verify_off_bins(ve, i);
-                            else sh.sums[i] = kept[i];
-                        }
+                        if constexpr (VERIFY) spl_verify_left(sh, ve, kept);
+                        else for (int i = tid; i < SPL_SAMPLE_BINS; i += 1024) sh.sums[i] = kept[i];
                         const int b = spl_sample_place(sh, SPL_SAMPLE_BINS, target);
                         decide(SPL_SAMPLE_DRAW, b, b, cut);
                     }
