@@ -8,8 +8,8 @@
 //   O += P V       in fp16, which holds every code exactly. Four warps turn the values of a chunk into fp16 on their way to the products (V as 8-bit operand would want P in 8 bits, too: a weight below
 //                  2^-17 of the row's largest would be lost, and many tokens of small weight are not a small matter).
 // The value scales go into the exponent: y_t = log2 of p_t vs_t = x_t + log2 vs_t has the running reference, so that P = 2^(y - ref) uses fp16's range for what counts in the row's sum, whatever the
-// sizes of values that do not (a running maximum of x alone would leave tokens of small values in the subnormals beside one of large ones); the denominator adds P / vs. The conversion warps bring each
-// token's ks, log2 vs and 1 / vs a tile ahead.
+// sizes of values that do not (a running maximum of x alone would leave tokens of small values in the subnormals beside one of large ones); the denominator adds P / vs. The warp that copies keys writes each
+// token's ks, log2 vs and 1 / vs beside them.
 // Values behind the sequence's last token and in front of every row's window are zeros in fp16, whatever the cache holds there.
 #pragma once
 #include "spl_paged.cuh"
@@ -18,11 +18,12 @@
 #define SPL_PAGED8_THREADS (32 * (SPL_PAGED8_SOFTMAX + 8))
 __host__ __device__ constexpr int spl_paged8_k_chunk(int hd) { return hd == 64 ? 8192 : 16384; }          // 128 tokens by up to 128 channels
 __host__ __device__ constexpr int spl_paged8_v_tokens(int hd) { return hd == 256 ? 64 : 128; }            // a chunk of values: tokens by all channels
-__host__ __device__ constexpr int spl_paged8_ring_k(int hd) { return hd == 64 ? 6 : hd == 128 ? 4 : 3; }
-__host__ __device__ constexpr int spl_paged8_ring_v(int hd) { return hd == 64 ? 6 : hd == 128 ? 3 : 2; }
-__host__ __device__ constexpr int spl_paged8_ring_w(int hd) { return hd == 64 ? 3 : 2; }                  // chunks of values in fp16
-// Tiles of scales. Those of tile i + 1 are written when tile i - 1 has been converted, which waited for a place among the chunks in fp16: for the product, and so the softmax, of tile i - 1 - ring_w (or a later one).
-__host__ __device__ constexpr int spl_paged8_scales(int hd) { return spl_paged8_ring_w(hd) + 2; }
+__host__ __device__ constexpr int spl_paged8_ring_k(int hd) { return hd == 64 ? 6 : hd == 128 ? 5 : 3; }
+// Chunks of values, as they lie and in fp16: even numbers, for two pairs of warps take turns at them and a pair has to meet every phase of its places' barriers.
+__host__ __device__ constexpr int spl_paged8_ring_v(int hd) { return hd == 64 ? 6 : 2; }
+__host__ __device__ constexpr int spl_paged8_ring_w(int hd) { return hd == 64 ? 4 : 2; }
+// Tiles of scales. Those of tile j are written behind its first keys, which waited for the scores of the tile a ring before, and these for the softmax of the tile two before that.
+__host__ __device__ constexpr int spl_paged8_scales(int hd) { return (spl_paged8_ring_k(hd) + (hd == 256 ? 1 : 0)) / (hd == 256 ? 2 : 1) + 2; }
 __host__ __device__ constexpr size_t spl_paged8_smem_bytes(int hd) {
     return size_t(hd) * 256 /* Q, two parts */ + size_t(spl_paged8_ring_k(hd)) * spl_paged8_k_chunk(hd) + size_t(spl_paged8_ring_v(hd) + 2 * spl_paged8_ring_w(hd)) * spl_paged8_v_tokens(hd) * hd +
            spl_paged8_scales(hd) * 3 * 512 + 2 * 512 /* the rows' factors */ + 2 * 4 * 512 /* maxima, sums */ + 512 /* barriers */;
@@ -116,9 +117,9 @@ spl_paged_attend_e4m3_kernel(const __grid_constant__ CUtensorMap k_map, const __
 
     if (tid == 0) {
         for (int i = 0; i < NK; ++i) { spl_mbar_init(&full_k[i], 1); spl_mbar_init(&empty_k[i], 1); }
-        for (int i = 0; i < NV; ++i) { spl_mbar_init(&full_v[i], 1); spl_mbar_init(&empty_v[i], 4); }
-        for (int i = 0; i < NW; ++i) { spl_mbar_init(&full_w[i], 4); spl_mbar_init(&empty_w[i], 1); }
-        for (int i = 0; i < NS; ++i) spl_mbar_init(&scaled[i], 4);
+        for (int i = 0; i < NV; ++i) { spl_mbar_init(&full_v[i], 1); spl_mbar_init(&empty_v[i], 2); }
+        for (int i = 0; i < NW; ++i) { spl_mbar_init(&full_w[i], 2); spl_mbar_init(&empty_w[i], 1); }
+        for (int i = 0; i < NS; ++i) spl_mbar_init(&scaled[i], 1);
         for (int i = 0; i < 2; ++i) { spl_mbar_init(&s_full[i], 1); spl_mbar_init(&p_full[i], SPL_PAGED8_SOFTMAX); spl_mbar_init(&o_done[i], 1); }
         spl_mbar_init(q_full, SPL_PAGED8_SOFTMAX); spl_mbar_init(&drained[0], 1); spl_mbar_init(&drained[1], 1);
         *abort = 0;
@@ -164,9 +165,12 @@ spl_paged_attend_e4m3_kernel(const __grid_constant__ CUtensorMap k_map, const __
     }
     spl_grid_begin();
     // Waits and what gives them up: as in spl_paged_attend_kernel.
-    bool ok = true;
-    auto gave_up = [&](int code) { ok = false; if (!*abort && lane == 0) { spl_note_wait(a.error_flag, code, 0); a.error_flag[0] = 200 + warp; } *abort = 1; };
-    auto wait = [&](uint64_t *bar, int phase, int code) { if (ok && !spl_mbar_wait_warp(bar, phase & 1, const_cast<const int *>(abort))) gave_up(code); return ok; };
+    int ok = 1;
+    auto gave_up = [&](int code) { ok = 0; if (!*abort && lane == 0) { spl_note_wait(a.error_flag, code, 0); a.error_flag[0] = 200 + warp; } *abort = 1; };
+    auto wait = [&](uint64_t *bar, int phase, int code) { if (ok && !spl_mbar_wait_warp(bar, phase & 1, const_cast<const int *>(abort))) gave_up(code); return ok != 0; };
+    // The softmax's waits: the empty statement keeps the compiler from making a second loop for the case that a wait has run out. With the loop twice as large its instructions came too late: 2,048 rows over
+    // 8,192 tokens of 32/8 heads of 128 took 671 us instead of 390. (The products' loops are faster without it.)
+    auto meet = [&](uint64_t *bar, int phase, int code) { wait(bar, phase, code); asm volatile("" : "+r"(ok)); };
     // Tokens that some row of a piece sees.
     auto seen_first = [&](const SplPagedItem &it) { return spl_paged_first(s, it.base + it.q0 / s.group); };
     auto seen_last = [&](const SplPagedItem &it) { return spl_paged_last(s, it.base + (it.q0 + it.q_count - 1) / s.group, it.length); };
@@ -176,12 +180,13 @@ spl_paged_attend_e4m3_kernel(const __grid_constant__ CUtensorMap k_map, const __
         const bool keys = warp == COPY_K;
         uint64_t *full = keys ? full_k : full_v, *empty = keys ? empty_k : empty_v;
         const int slots = keys ? NK : NV;
-        int n = 0, st = 0;
+        int n = 0, st = 0, tiles = 0;
         SplPagedItem it = first_item;
         int page = first_page;
         for (int i = item0; i < item1 && ok; ++i) {
             if (i > item0) { it = a.items[i]; page = page_of(it, it.tile_begin); }
-            for (int tile = it.tile_begin; tile < it.tile_end && ok; ++tile) {
+            const int seen0 = seen_first(it), seen1 = seen_last(it);
+            for (int tile = it.tile_begin; tile < it.tile_end && ok; ++tile, ++tiles) {
                 const int ahead = page_of(it, tile + 1), inside = inside_page(tile);
                 for (int c = 0; c < (keys ? KPARTS : VPARTS) && wait(&empty[st], (n / slots) + 1, 60); ++c) {
                     const int there = keys ? key_boxes(it, tile) : value_boxes(it, tile, c), from = keys ? page : value_page(page, c);
@@ -192,6 +197,28 @@ spl_paged_attend_e4m3_kernel(const __grid_constant__ CUtensorMap k_map, const __
                         else spl_tma_load5(v_ring + st * VCHUNK + lane * vbox * HD, &v_map, 0, inside + (c * vboxes + lane) % per_page * vbox, 0, it.kv_head, from, &full[st]);
                     }
                     ++n; st = st + 1 == slots ? 0 : st + 1;
+                    if (keys && c == 0) {
+                        // The tile's scales, four tokens a lane (of one page); what no row sees is masked.
+                        const int mine = 4 * lane, token = tile * 128 + mine;
+                        const size_t at = (size_t(__shfl_sync(0xffffffffu, page, mine / box)) * s.kv_heads + it.kv_head) * s.page_tokens + inside + mine % box;
+                        float k[4] = {0.0f, 0.0f, 0.0f, 0.0f}, l[4] = {0.0f, 0.0f, 0.0f, 0.0f}, inv[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        if (token + 4 > seen0 && token < seen1) {
+                            const float4 ks = __ldcg(reinterpret_cast<const float4 *>(scales.k + at)), vs = __ldcg(reinterpret_cast<const float4 *>(scales.v + at));
+                            const float given_k[4] = {ks.x, ks.y, ks.z, ks.w}, given_v[4] = {vs.x, vs.y, vs.z, vs.w};
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                if (token + e < seen0 || token + e >= seen1) continue;
+                                const float v = given_v[e] >= 0.0f && given_v[e] <= SPL_PAGED8_SCALE_MOST ? fmaxf(given_v[e], SPL_PAGED8_SCALE_LEAST) : __int_as_float(0x7fffffff);
+                                k[e] = given_k[e]; l[e] = spl_lg2(v); inv[e] = spl_rcp(v);
+                            }
+                        }
+                        float *put = scale_ring + (tiles % NS) * 3 * 128 + mine;
+                        *reinterpret_cast<float4 *>(put) = make_float4(k[0], k[1], k[2], k[3]);
+                        *reinterpret_cast<float4 *>(put + 128) = make_float4(l[0], l[1], l[2], l[3]);
+                        *reinterpret_cast<float4 *>(put + 256) = make_float4(inv[0], inv[1], inv[2], inv[3]);
+                        __syncwarp();
+                        if (lane == 0) spl_mbar_arrive(&scaled[tiles % NS]);
+                    }
                 }
                 page = ahead;
             }
@@ -249,86 +276,47 @@ spl_paged_attend_e4m3_kernel(const __grid_constant__ CUtensorMap k_map, const __
         spl_tc_commit_if(elected, &drained[first_product ? 0 : 1]);
         spl_mbar_wait(&drained[first_product ? 0 : 1], 0);
     } else if (warp >= CONVERT) {
-        // ---- values into fp16, and the scales of a tile ahead: thread `mine` has the tile's token of that number, its page looked up two tiles and its scales one tile before they are wanted.
-        const int mine = (warp - CONVERT) * 32 + lane;
-        struct Ahead { int page, place; float k, v; };      // place: of the token among its page's scales, negative where no row sees it
-        int cursor = item0, tile_at = 0, tile_last = 0, pages_at = 0, place_at = 0, from = 0, to = 0;
-        auto enter = [&](const SplPagedItem &it) {
-            tile_at = it.tile_begin; tile_last = it.tile_end; pages_at = it.sequence; place_at = it.kv_head * s.page_tokens; from = seen_first(it); to = seen_last(it);
-        };
-        if (item0 < item1) enter(first_item);
-        const int page_log = 31 - __clz(s.page_tokens);
-        // The cursor's tile with its page, and the cursor one on.
-        auto look = [&]() {
-            Ahead x{0, -1, 0.0f, 0.0f};
-            if (cursor >= item1) return x;
-            const int token = tile_at * 128 + mine;
-            if (token >= from && token < to) { x.place = place_at + (token & (s.page_tokens - 1)); x.page = __ldcg(t.table + size_t(pages_at) * s.max_pages + (token >> page_log)); }
-            if (++tile_at == tile_last && ++cursor < item1) enter(a.items[cursor]);
-            return x;
-        };
-        auto bring = [&](Ahead &x) {
-            if (x.place < 0) return;
-            const size_t at = size_t(x.page) * (s.kv_heads * s.page_tokens) + x.place;
-            x.k = __ldcg(scales.k + at); x.v = __ldcg(scales.v + at);
-        };
-        auto write = [&](const Ahead &x, int tile) {
-            // (What no row sees is masked.)
-            float *to = scale_ring + (tile % NS) * 3 * 128 + mine;
-            const bool there = x.place >= 0;
-            const float v = x.v >= 0.0f && x.v <= SPL_PAGED8_SCALE_MOST ? fmaxf(x.v, SPL_PAGED8_SCALE_LEAST) : __int_as_float(0x7fffffff);
-            to[0] = there ? x.k : 0.0f; to[128] = there ? spl_lg2(v) : 0.0f; to[256] = there ? spl_rcp(v) : 0.0f;
-            __syncwarp();
-            if (lane == 0) spl_mbar_arrive(&scaled[tile % NS]);
-        };
-        Ahead next{}, later{};
-        if (item0 < item1) {
-            Ahead now = look();
-            next = look(); later = look();
-            bring(now); bring(next);
-            write(now, 0);
-        }
+        // ---- values into fp16, two warps a chunk, the other two the next.
         // A quarter of a warp turns 64 channels of two tokens a step: four lanes a token, 16 channels each. The tokens of a pair differ by 5 in the low three bits of their number, so that neither the
-        // reads (16-byte pieces of swizzled rows) nor the writes (two pieces a lane) of a quarter meet in a bank.
-        // A warp keeps to one block of 64 channels where there are as many as warps divide by; its steps go through the chunk's groups of eight tokens.
-        constexpr int GROUPS = HD / 64, EIGHTS = 4 / GROUPS, STEPS = VT / 8 / EIGHTS;
-        const int low = lane >> 3, pair_token = (lane & 4) ? low ^ 5 : low, quarter = lane & 3, group = (warp - CONVERT) % GROUPS, eight0 = (warp - CONVERT) / GROUPS, vlog = 31 - __clz(vbox);
-        const int read_at = HD == 64 ? pair_token * 64 + quarter * 16 : (group >> 1) * vbox * 128 + pair_token * 128 + (((group & 1) * 4 + quarter) ^ pair_token) * 16;
-        const int write_at = group * (VT * 128) + pair_token * 128, write_lo = ((2 * quarter) ^ pair_token) * 16;
-        int n = 0, tiles = 0;
+        // reads (16-byte pieces of swizzled rows) nor the writes (two pieces a lane) of a quarter meet in a bank. A warp has half of the channels where there are blocks of 64 to share, else half of the tokens.
+        constexpr int GROUPS = HD / 64, EACH = GROUPS > 1 ? GROUPS / 2 : 1, EIGHTS = GROUPS > 1 ? 1 : 2, STEPS = VT / 8 / EIGHTS;
+        const int side = (warp - CONVERT) & 1, low = lane >> 3, pair_token = (lane & 4) ? low ^ 5 : low, quarter = lane & 3, eight0 = GROUPS > 1 ? 0 : side, vlog = 31 - __clz(vbox);
+        const int write_lo = ((2 * quarter) ^ pair_token) * 16;
+        int n = 0;
         for (int i = item0; i < item1 && ok; ++i) {
             int tile, last_tile, from, to;
             { const SplPagedItem it = a.items[i]; tile = it.tile_begin; last_tile = it.tile_end; from = seen_first(it); to = seen_last(it); }
-            for (; tile < last_tile && ok; ++tile, ++tiles) {
-                write(next, tiles + 1);          // (behind the block's last tile nobody waits for it)
-                next = later;
-                bring(next);
-                later = look();
+            for (; tile < last_tile && ok; ++tile) {
                 for (int c = 0; c < VPARTS && ok; ++c, ++n) {
+                    if ((n & 1) != (warp - CONVERT) >> 1) continue;
                     const int st = n % NV, sw = n % NW;
                     if (!wait(&full_v[st], n / NV, 71) || !wait(&empty_w[sw], n / NW + 1, 72)) break;
                     const int base = tile * 128 + c * VT;
                     const bool whole = base >= from && base + VT <= to;
-                    const unsigned char *src = v_ring + st * VCHUNK + read_at;
-                    unsigned char *dst = w_ring + sw * WCHUNK + write_at;
+#pragma unroll 1
+                    for (int e = 0; e < EACH; ++e) {
+                        const int group = GROUPS > 1 ? side * EACH + e : 0;
+                        const unsigned char *src = v_ring + st * VCHUNK + (HD == 64 ? pair_token * 64 + quarter * 16 : (group >> 1) * vbox * 128 + pair_token * 128 + (((group & 1) * 4 + quarter) ^ pair_token) * 16);
+                        unsigned char *dst = w_ring + sw * WCHUNK + group * (VT * 128) + pair_token * 128;
 #pragma unroll
-                    for (int z0 = 0; z0 < STEPS; z0 += 4) {
-                        uint4 codes[4];
+                        for (int z0 = 0; z0 < STEPS; z0 += 4) {
+                            uint4 codes[4];
 #pragma unroll
-                        for (int z = 0; z < 4; ++z) {
-                            const int token = (eight0 + (z0 + z) * EIGHTS) * 8;
-                            codes[z] = *reinterpret_cast<const uint4 *>(src + (token >> vlog) * (vbox * HD) + (token & (vbox - 1)) * ROW);
-                            if (!whole && (base + token + pair_token < from || base + token + pair_token >= to)) codes[z] = make_uint4(0u, 0u, 0u, 0u);
-                        }
+                            for (int z = 0; z < 4; ++z) {
+                                const int token = (eight0 + (z0 + z) * EIGHTS) * 8;
+                                codes[z] = *reinterpret_cast<const uint4 *>(src + (token >> vlog) * (vbox * HD) + (token & (vbox - 1)) * ROW);
+                                if (!whole && (base + token + pair_token < from || base + token + pair_token >= to)) codes[z] = make_uint4(0u, 0u, 0u, 0u);
+                            }
 #pragma unroll
-                        for (int z = 0; z < 4; ++z) {
-                            const uint32_t w[4] = {codes[z].x, codes[z].y, codes[z].z, codes[z].w};
-                            uint32_t h[8];
+                            for (int z = 0; z < 4; ++z) {
+                                const uint32_t w[4] = {codes[z].x, codes[z].y, codes[z].z, codes[z].w};
+                                uint32_t h[8];
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) { h[2 * e] = spl_halves_of_e4m3(uint16_t(w[e])); h[2 * e + 1] = spl_halves_of_e4m3(uint16_t(w[e] >> 16)); }
-                            unsigned char *row = dst + (eight0 + (z0 + z) * EIGHTS) * 1024;
-                            *reinterpret_cast<uint4 *>(row + write_lo) = make_uint4(h[0], h[1], h[2], h[3]);
-                            *reinterpret_cast<uint4 *>(row + (write_lo ^ 16)) = make_uint4(h[4], h[5], h[6], h[7]);
+                                for (int d = 0; d < 4; ++d) { h[2 * d] = spl_halves_of_e4m3(uint16_t(w[d])); h[2 * d + 1] = spl_halves_of_e4m3(uint16_t(w[d] >> 16)); }
+                                unsigned char *row = dst + (eight0 + (z0 + z) * EIGHTS) * 1024;
+                                *reinterpret_cast<uint4 *>(row + write_lo) = make_uint4(h[0], h[1], h[2], h[3]);
+                                *reinterpret_cast<uint4 *>(row + (write_lo ^ 16)) = make_uint4(h[4], h[5], h[6], h[7]);
+                            }
                         }
                     }
                     spl_fence_proxy_async();
@@ -409,8 +397,8 @@ spl_paged_attend_e4m3_kernel(const __grid_constant__ CUtensorMap k_map, const __
             for (int n = 0; n < 4; ++n) { c[n] = 0.0f; offset[n] = SPL_PAGED8_UNSEEN; sum[n] = make_float2(0.0f, 0.0f); }
             for (; tile < tile_end; ++tile, ++tiles) {
                 const int buf = tiles & 1;
-                wait(&scaled[tiles % NS], tiles / NS, 73);
-                wait(&s_full[buf], tiles >> 1, 66);
+                meet(&scaled[tiles % NS], tiles / NS, 73);
+                meet(&s_full[buf], tiles >> 1, 66);
                 if (busy) {
                     if (tile == tile_begin) {                        // (all of the queries were there before the scores)
 #pragma unroll
@@ -470,7 +458,7 @@ spl_paged_attend_e4m3_kernel(const __grid_constant__ CUtensorMap k_map, const __
                         if (tile > tile_begin) {
                             // The product before has to be done with these sums; the next waits for this warp's probabilities.
                             const float of_mine = __shfl_sync(0xffffffffu, old, of_row);
-                            wait(&o_done[(tiles - 1) & 1], (tiles - 1) >> 1, 67);
+                            meet(&o_done[(tiles - 1) & 1], (tiles - 1) >> 1, 67);
                             spl_tc_fence_after();
 #pragma unroll 1
                             for (int o = 0; o < HD / 4; o += 16) {
@@ -514,7 +502,7 @@ spl_paged_attend_e4m3_kernel(const __grid_constant__ CUtensorMap k_map, const __
             // The next piece's queries: all scores of this one have been seen, so its own are no longer read. (O is overwritten by a product that waits for this warp.)
             if (i + 1 < item1) bring_q(a.items[i + 1], (i + 1 - item0) & 1);
             // The piece's sums.
-            wait(&o_done[(tiles - 1) & 1], (tiles - 1) >> 1, 68);
+            meet(&o_done[(tiles - 1) & 1], (tiles - 1) >> 1, 68);
             const SplPagedItem it = a.items[i];
             const int row0 = it.row0 + it.q0 / s.group, mine = it.q0 % s.group + min(r, it.q_count - 1), row = int(mine * per_group >> 16), head = it.kv_head * s.group + mine - row * s.group;
             const size_t slot_row = size_t(it.slot) * a.slot_rows + r;
@@ -686,9 +674,12 @@ spl_paged_attend_e4m3_narrow_kernel(const __grid_constant__ CUtensorMap k_map, c
         }
     }
     spl_grid_begin();
-    bool ok = true;
-    auto gave_up = [&](int code) { ok = false; if (!*abort && lane == 0) { spl_note_wait(a.error_flag, code, 0); a.error_flag[0] = 200 + warp; } *abort = 1; };
-    auto wait = [&](uint64_t *bar, int phase, int code) { if (ok && !spl_mbar_wait_warp(bar, phase & 1, const_cast<const int *>(abort))) gave_up(code); return ok; };
+    int ok = 1;
+    auto gave_up = [&](int code) { ok = 0; if (!*abort && lane == 0) { spl_note_wait(a.error_flag, code, 0); a.error_flag[0] = 200 + warp; } *abort = 1; };
+    auto wait = [&](uint64_t *bar, int phase, int code) { if (ok && !spl_mbar_wait_warp(bar, phase & 1, const_cast<const int *>(abort))) gave_up(code); return ok != 0; };
+    // The softmax's waits: the empty statement keeps the compiler from making a second loop for the case that a wait has run out. With the loop twice as large its instructions came too late: 2,048 rows over
+    // 8,192 tokens of 32/8 heads of 128 took 671 us instead of 390. (The products' loops are faster without it.)
+    auto meet = [&](uint64_t *bar, int phase, int code) { wait(bar, phase, code); asm volatile("" : "+r"(ok)); };
     // Tokens that some row of a piece sees.
     auto seen_first = [&](const SplPagedItem &it) { return spl_paged_first(s, it.base + it.q0 / s.group); };
     auto seen_last = [&](const SplPagedItem &it) { return spl_paged_last(s, it.base + (it.q0 + it.q_count - 1) / s.group, it.length); };
@@ -867,12 +858,12 @@ spl_paged_attend_e4m3_narrow_kernel(const __grid_constant__ CUtensorMap k_map, c
             for (; tile < tile_end; ++tile, ++tiles) {
                 const int buf = tiles & 1;
                 if (tile + 1 == tile_end && i + 1 < item1) ask_q(a.items[i + 1]);
-                wait(&scaled[tiles % NS], tiles / NS, 70);
+                meet(&scaled[tiles % NS], tiles / NS, 70);
                 const float *mine_of = scale_ring + tiles % NS * 256 + mine;
                 const bool there = tile * 128 + mine >= from && tile * 128 + mine < to;      // (what no row sees is masked)
                 const float given = mine_of[128], v = given >= 0.0f && given <= SPL_PAGED8_SCALE_MOST ? fmaxf(given, SPL_PAGED8_SCALE_LEAST) : __int_as_float(0x7fffffff);
                 const float k = there ? mine_of[0] : 0.0f, l = there ? spl_lg2(v) : 0.0f, inv = there ? spl_rcp(v) : 0.0f;
-                wait(&s_full[buf], tiles >> 1, 66);
+                meet(&s_full[buf], tiles >> 1, 66);
                 if (tile == tile_begin) {                            // (all of the queries were there before the scores)
 #pragma unroll
                     for (int n = 0; n < H / 2; ++n) c[n] = *reinterpret_cast<const float2 *>(factor + ((i - item0) & 1) * N + n0 + 2 * n);
@@ -920,7 +911,7 @@ spl_paged_attend_e4m3_narrow_kernel(const __grid_constant__ CUtensorMap k_map, c
                     }
                     if (tile > tile_begin) {
                         // The product before has to be done with these sums; the next waits for this warp's probabilities.
-                        wait(&o_done[(tiles - 1) & 1], (tiles - 1) >> 1, 67);
+                        meet(&o_done[(tiles - 1) & 1], (tiles - 1) >> 1, 67);
                         spl_tc_fence_after();
 #pragma unroll 1
                         for (int n = 0; n < H; n += 8) {
@@ -974,7 +965,7 @@ spl_paged_attend_e4m3_narrow_kernel(const __grid_constant__ CUtensorMap k_map, c
             }
             const SplPagedItem it = a.items[i];
             // The piece's sums.
-            wait(&o_done[(tiles - 1) & 1], (tiles - 1) >> 1, 68);
+            meet(&o_done[(tiles - 1) & 1], (tiles - 1) >> 1, 68);
             spl_tc_fence_after();
             // Over the lanes: at each step half of the columns stay, and the other half's sums go to the lane that keeps these; lanes that end up with the same column have the same sum.
             int column = 0;
