@@ -579,7 +579,6 @@ spl_paged_attend_e4m3_kernel(const __grid_constant__ CUtensorMap k_map, const __
 // A softmax thread has a token, and 8 or 16 of the columns (groups of four warps share these out): the token's scales, which came with its keys, are its own registers, a row's maximum, where one is wanted, is a reduction over lanes (redux) and
 // four warps, its sum stays in the threads until the piece's end. The last four warps copy keys, issue the scores' and the sums' products, copy values.
 // A tile of 128 tokens by 256 channels is 64 KB from memory (some 2,700 cycles at an SM's share); the products take 400 cycles of the tensor cores with 16 rows.
-#define SPL_PAGED8_NARROW 48            // packed rows at most
 __host__ __device__ constexpr int spl_paged8n_groups(int n) { return n == 48 ? 3 : 2; }
 __host__ __device__ constexpr int spl_paged8n_threads(int n) { return 128 * spl_paged8n_groups(n) + 128; }
 // Chunks of 128 tokens by 128 channels, of keys and of values.

@@ -233,8 +233,8 @@ template <int TYPE> static void launch_append(const spl_paged *p, const SplPaged
     else launch_append_dim<TYPE, 256>(p, in, q_norm, k_norm, out, stream);
 }
 
-// Whether the batch's attention over a cache of e4m3 runs in its transposed form: few packed rows a sequence, none of them met together with others'.
-static bool paged_narrow(const spl_paged *p) { return p->c.dtype == SPL_E4M3 && p->c.head_dim >= 128 && !p->joint && p->packed <= SPL_PAGED8_NARROW; }
+// Whether the batch's attention runs in the transposed form.
+static bool paged_narrow(const spl_paged *p) { return p->joint ? spl_paged_joint_narrow(p->c, p->packed) : spl_paged_narrow(p->c, p->packed); }
 // The cache as a tensor (channel in block, token in page, block of 64 channels, kv head, page) for the copies of values, in boxes of all channels by a page's tokens (at most a
 // chunk's), or of keys: of a page's tokens (at most a tile's) by 64 channels, or by a chunk's where the box is a tile's tokens.
 static bool paged_map(const spl_paged *p, const void *cache, bool values, CUtensorMap *map) {
@@ -264,7 +264,8 @@ template <int HD, bool BF16> static void launch_attend(const spl_paged *p, const
 template <int HD> static void launch_attend_e4m3(const spl_paged *p, const CUtensorMap &k_map, const CUtensorMap &v_map, const SplPagedAttend &a, const SplPagedScaled &scales, cudaStream_t stream) {
     if constexpr (HD >= 128) {
         if (paged_narrow(p)) {
-            const int n = p->packed <= 16 ? 16 : p->packed <= 32 ? 32 : 48;
+            // (Over a prefix, several sequences' rows: as many as the batch has.)
+            const int packed = p->joint ? std::min(p->rows * p->shape.group, SPL_PAGED8_NARROW) : p->packed, n = packed <= 16 ? 16 : packed <= 32 ? 32 : 48;
             launch_step(n == 16 ? spl_paged_attend_e4m3_narrow_kernel<HD, 16> : n == 32 ? spl_paged_attend_e4m3_narrow_kernel<HD, 32> : spl_paged_attend_e4m3_narrow_kernel<HD, 48>, dim3(p->e->sms), dim3(spl_paged8n_threads(n)),
                         spl_paged8n_smem_bytes(HD, n), stream, k_map, v_map, p->tables(), p->shape, a, scales);
             return;

@@ -10,6 +10,7 @@
 #include "../../include/splosh_cuda.h"
 
 #define SPL_PAGED_TILE 128            // tokens a tile; packed query rows a block
+#define SPL_PAGED8_NARROW 48          // packed rows at most of attention over a cache of e4m3 in its transposed form
 
 // A block's piece of work: packed query rows [q0, q0 + q_count) of a sequence (packed row i is the sequence's new token i / group, head i % group of
 // the kv head) against the tokens [tile_begin * 128, tile_end * 128). slot >= 0: the piece is one of several of its rows and leaves
@@ -122,10 +123,11 @@ inline bool spl_paged_groups_check(const spl_paged_config &c, int32_t sequences,
 // decode steps of few sequences; stretches that cut everything spent 25 of 47 us on joining 1-tile pieces of 128 rows in a step of six decoding sessions and a
 // 301-token prompt.)
 #define SPL_PAGED_PIECE_COST 2
-inline int spl_paged_cut_cost(int q_count, bool by_rows = false) { return q_count <= 16 ? 0 : q_count <= (by_rows ? 96 : 64) ? 1 : 2; }
-inline int spl_paged_cut_least(int q_count, bool by_rows = false) { return q_count <= 16 ? 1 : q_count > (by_rows ? 96 : 64) ? 5 : by_rows ? 2 : 3; }      // tiles a piece
-// With groups (by_rows) a kernel of its own joins, and pieces of up to 96 rows may be smaller: the 72 packed rows of twelve sequences over 8,192 shared tokens 32.9 -> 25.0 us; the same rule for 128
-// packed rows (eight verify blocks over 20,992 shared tokens) took 61.5 us instead of 55.6.
+// With groups (by_rows) a kernel of its own joins, and pieces may be smaller: the 72 packed rows of twelve sequences over 8,192 shared tokens 32.9 -> 25.0 us. A piece of 128 rows counts for four tiles more
+// there (its partial sums), so that pieces get small only where a block's stretch is short: six verify blocks of 24 rows over 1,024 shared tokens 27.2 -> 17.5 us, sixteen 30.3 -> 22.0, and eight of 48 over
+// 20,992 stay at 55.7 (61.5 where such pieces counted for one tile).
+inline int spl_paged_cut_cost(int q_count, bool by_rows = false) { return q_count <= 16 ? 0 : by_rows ? (q_count <= 96 ? 1 : 4) : q_count <= 64 ? 1 : 2; }
+inline int spl_paged_cut_least(int q_count, bool by_rows = false) { return q_count <= 16 ? 1 : by_rows ? 2 : q_count > 64 ? 5 : 3; }      // tiles a piece
 // What a block that has `left` of its stretch takes of the `t` tiles left of a unit (cut: some have gone to another block): 0, some, or all; -1: the stretch is too short
 // for this unit's pieces.
 inline int64_t spl_paged_take(int64_t t, int64_t left, int64_t stretch, int q_count, bool cut, bool by_rows = false) {
@@ -141,8 +143,23 @@ inline int64_t spl_paged_take(int64_t t, int64_t left, int64_t stretch, int q_co
 // With groups, the sequences of a run (consecutive members of a group, none with more packed rows than a block takes) meet the whole tiles of their prefix
 // together: their rows lie one behind the other, so they are the rows of one sequence over the prefix, in blocks of 128 packed rows whoever's they are; each sequence's own
 // tokens are units of their own, and both leave partial sums (O, m, l) that spl_paged_combine_kernel joins. (Sequences of more packed rows read the prefix once for 128 of them as it is.)
-// That pays where the tiles saved are more than the joining, some SPL_PAGED_JOINT_COST tiles a block.
-#define SPL_PAGED_JOINT_COST 1
+// Over a cache of e4m3 the rows that meet a prefix together take the transposed form, 48 a block, where a sequence has up to 36 of them, and the form of 128 where two sequences' do not fit 48 any more by much
+// (heads of 256, 24 on 4: four sequences of 24 packed rows over 20,992 shared tokens 35.2 us in the former and 38.4 in the latter, of 36 43.9 and 54.2, two of 48 57.5 and 37.9).
+// Both go by the most packed rows that a sequence has, so a graph that holds one form is right for every batch of its rows.
+#define SPL_PAGED8_JOINT_NARROW 36
+inline bool spl_paged_narrow(const spl_paged_config &c, int64_t packed) { return c.dtype == SPL_E4M3 && c.head_dim >= 128 && packed <= SPL_PAGED8_NARROW; }
+inline bool spl_paged_joint_narrow(const spl_paged_config &c, int64_t packed) { return spl_paged_narrow(c, packed) && packed <= SPL_PAGED8_JOINT_NARROW; }
+// Meeting together pays where the tiles saved are more than the joining: so many a block for one more launch and the pieces' first keys, and one for so many rows of heads that leave and join sums. Measured with
+// heads of 256, 24 of them on 4, together and apart:
+//   tiles of one cost      six sequences of one row over 1,024 shared tokens 15.2 and 13.7 us, over 4,096 17.7 and 21.8; sixteen of four rows over 512 21.5 and 19.7, over 1,024 22.0 and 23.0;
+//                          48 of four over 256 35.7 and 30.3, over 512 35.6 and 36.6;
+//   transposed, both       (apart it is quick where sequences find the same keys in L2, most of all with up to 16 packed rows) six of one row over 4,096 19.4 and 15.7, sixteen over 2,048 19.2 and 19.3;
+//                          two of four rows over 8,192 23.0 and 32.7, sixteen over 2,048 30.6 and 25.0, over 8,192 46.9 and 56.9, 48 over 2,048 63.7 and 55.7;
+//   transposed apart only  two of eight rows over 20,992 37.9 and 57.6, eight over 4,096 38.9 and 34.5, over 20,992 71.1 and 83.2, 24 over 4,096 74.9 and 56.7.
+inline bool spl_paged_joint_pays(const spl_paged_config &c, int64_t saved, int blocks, int64_t rows_of_heads, int64_t most) {
+    if (spl_paged_joint_narrow(c, most)) return saved > int64_t(blocks) * (most <= 16 ? 4 : 1) + rows_of_heads / 3;
+    return saved > blocks + (spl_paged_narrow(c, most) ? rows_of_heads : rows_of_heads / 10);
+}
 struct SplPagedUnit { SplPagedItem item; bool joint; int run, prefix; };      // run: its run of sequences or -1; prefix: the first of its run's prefix units of its kv head
 inline void spl_paged_plan(const spl_paged_config &c, int blocks, int32_t sequences, const int32_t *rows, const int32_t *lengths, SplPagedPlan &plan, const SplPagedGroups *groups = nullptr) {
     const int group = c.heads / c.kv_heads, tile = SPL_PAGED_TILE;
@@ -159,6 +176,9 @@ inline void spl_paged_plan(const spl_paged_config &c, int blocks, int32_t sequen
             }
     };
     plan.joint = false;
+    int64_t most = 0;
+    for (int i = 0; i < sequences; ++i) most = std::max(most, int64_t(rows[i]) * group);
+    const int width = spl_paged_joint_narrow(c, most) ? SPL_PAGED8_NARROW : tile;
     std::vector<int> run_row0;
     int s = 0, row0 = 0;
     auto pass_over = [&]() { add_sequence(s, row0, 0, -1, 0, 0); row0 += rows[s]; ++s; };
@@ -169,8 +189,8 @@ inline void spl_paged_plan(const spl_paged_config &c, int blocks, int32_t sequen
             int run_end = s, members = 0;
             int64_t packed = 0;
             while (run_end < end && int64_t(rows[run_end]) * group <= tile) { packed += rows[run_end] * group; members += rows[run_end] > 0; ++run_end; }
-            const int64_t joint_units = (packed + tile - 1) / tile;
-            if (members < 2 || int64_t(c.kv_heads) * prefix * (members - joint_units) <= int64_t(blocks) * SPL_PAGED_JOINT_COST) {
+            const int64_t joint_units = (packed + width - 1) / width;
+            if (members < 2 || !spl_paged_joint_pays(c, int64_t(c.kv_heads) * prefix * (members - joint_units), blocks, packed * c.kv_heads, most)) {
                 do pass_over(); while (s < run_end);
                 continue;
             }
@@ -178,8 +198,8 @@ inline void spl_paged_plan(const spl_paged_config &c, int blocks, int32_t sequen
             run_row0.push_back(row0);
             plan.joint = true;
             for (int h = 0; h < c.kv_heads; ++h)
-                for (int64_t q0 = 0; q0 < packed; q0 += tile)
-                    add({SplPagedItem{s, row0, h, int(q0), int(std::min<int64_t>(tile, packed - q0)), 0, prefix, -1, prefix * tile, prefix * tile, -1, 1, 0, {0, 0, 0}}, true, -1, 0});
+                for (int64_t q0 = 0; q0 < packed; q0 += width)
+                    add({SplPagedItem{s, row0, h, int(q0), int(std::min<int64_t>(width, packed - q0)), 0, prefix, -1, prefix * tile, prefix * tile, -1, 1, 0, {0, 0, 0}}, true, -1, 0});
             for (; s < run_end; row0 += rows[s], ++s) add_sequence(s, row0, prefix, run, first_prefix, int(joint_units));
         }
     }
@@ -189,10 +209,10 @@ inline void spl_paged_plan(const spl_paged_config &c, int blocks, int32_t sequen
         int64_t used = 1, left = stretch;
         for (const SplPagedUnit &u : whole)
             for (int64_t t = u.item.tile_end - u.item.tile_begin, all = t; t > 0;) {
-                const int64_t take = spl_paged_take(t, left, stretch, u.item.q_count, t < all || u.joint, groups);
+                const int64_t take = spl_paged_take(t, left, stretch, u.item.q_count, t < all || u.joint, plan.joint);
                 if (take < 0) return int64_t(blocks) + 1;
                 if (!take) { if (++used > blocks) return used; left = stretch; continue; }
-                left -= take + SPL_PAGED_PIECE_COST + (take < all || u.joint ? spl_paged_cut_cost(u.item.q_count, groups) : 0);
+                left -= take + SPL_PAGED_PIECE_COST + (take < all || u.joint ? spl_paged_cut_cost(u.item.q_count, plan.joint) : 0);
                 t -= take;
             }
         return used;
@@ -209,12 +229,12 @@ inline void spl_paged_plan(const spl_paged_config &c, int blocks, int32_t sequen
         const size_t piece0 = units.size();
         const int all = u.tile_end - u.tile_begin;
         for (int t = u.tile_begin; t < u.tile_end;) {
-            const int take = int(spl_paged_take(u.tile_end - t, left, low, u.q_count, t > u.tile_begin || one.joint, groups));
+            const int take = int(spl_paged_take(u.tile_end - t, left, low, u.q_count, t > u.tile_begin || one.joint, plan.joint));
             if (!take) { plan.block_begin.push_back(int32_t(units.size())); left = low; continue; }
             SplPagedItem piece = u;
             piece.tile_begin = t; piece.tile_end = t + take;
             units.push_back(piece);
-            left -= take + SPL_PAGED_PIECE_COST + (take < all || one.joint ? spl_paged_cut_cost(u.q_count, groups) : 0);
+            left -= take + SPL_PAGED_PIECE_COST + (take < all || one.joint ? spl_paged_cut_cost(u.q_count, plan.joint) : 0);
             t += take;
         }
         const int pieces = int(units.size() - piece0);
@@ -238,8 +258,8 @@ inline void spl_paged_plan(const spl_paged_config &c, int blocks, int32_t sequen
         // A sequence's rows may lie in two of the run's blocks of packed rows.
         const int begin = (u.row0 - run_row0[one.run]) * group;
         for (int q = begin; q < begin + u.q_count;) {
-            const int end = std::min(begin + u.q_count, (q / tile + 1) * tile), joint = one.prefix + q / tile;
-            plan.records.push_back({u.row0, q - begin, u.kv_head, end - q, left_at[joint].first + q % tile, whole[joint].item.q_count, left_at[joint].second, first + q - begin, u.q_count, pieces, {0, 0}});
+            const int end = std::min(begin + u.q_count, (q / width + 1) * width), joint = one.prefix + q / width;
+            plan.records.push_back({u.row0, q - begin, u.kv_head, end - q, left_at[joint].first + q % width, whole[joint].item.q_count, left_at[joint].second, first + q - begin, u.q_count, pieces, {0, 0}});
             q = end;
         }
     }

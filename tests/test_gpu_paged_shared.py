@@ -14,7 +14,7 @@ pytestmark = pytest.mark.gpu
 
 def joint(scene):
     return debug_paged_plan_shared(scene.rows, scene.lengths, scene.groups, heads=scene.heads, kv_heads=scene.kv_heads, head_dim=scene.head_dim, pages=1, page_tokens=256, window=scene.window,
-                                   causal=scene.causal, max_sequences=len(scene.rows), max_rows=scene.total, max_context=1 << 20)[4]
+                                   causal=scene.causal, dtype=scene.dtype, max_sequences=len(scene.rows), max_rows=scene.total, max_context=1 << 20)[4]
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16", "e4m3"])
@@ -32,7 +32,8 @@ def test_types_and_head_shapes(engine, dtype, heads, kv_heads, head_dim, out_dty
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("dtype", ["bf16", "e4m3"])
 def test_blocks_of_rows_that_straddle_two_units(engine, rows, causal, dtype):
-    scene = Scene(rows, 12, 2, 128, [rows] * 20, [4096 + rows + 11 * i for i in range(20)], page_tokens=128, dtype=dtype, causal=causal, groups=[(20, 4096)])
+    shared = {1: 4096, 3: 4096, 8: 12288, 16: 8192}[rows]
+    scene = Scene(rows, 12, 2, 128, [rows] * 20, [shared + rows + 11 * i for i in range(20)], page_tokens=128, dtype=dtype, causal=causal, groups=[(20, shared)])
     assert joint(scene)
     check(scene, attend(engine, scene, "f32"), "f32")
 
@@ -49,6 +50,17 @@ def test_several_groups_prompts_among_them_and_sequences_of_their_own(engine, dt
     check(scene, attend(engine, scene, "f32"), "f32")
 
 
+@pytest.mark.parametrize("rows,heads,kv_heads,shared", [(1, 8, 2, 8192), (1, 12, 2, 8192), (2, 8, 8, 4096), (4, 24, 4, 4096), (6, 24, 4, 16384), (7, 12, 2, 16384), (8, 32, 4, 8192)])
+@pytest.mark.parametrize("head_dim", [128, 256])
+def test_both_forms_over_a_cache_of_e4m3(engine, rows, heads, kv_heads, shared, head_dim):
+    """Four to 64 packed rows a sequence, two to nine sequences: joint rows of 16, 32, 48 and 128 a block, full and not."""
+    for n in (2, 5, 9):
+        scene = Scene(rows + n, heads, kv_heads, head_dim, [rows] * n, [shared + rows + 77 * i for i in range(n)], page_tokens=64, dtype="e4m3", groups=[(n, shared)])
+        if joint(scene):
+            check(scene, attend(engine, scene, "f32"), "f32")
+    assert joint(scene)
+
+
 def test_a_window_leaves_a_prefix_to_each_sequence(engine):
     scene = Scene(4, 8, 2, 128, [1] * 12, [1024 + 1 + 9 * i for i in range(12)], page_tokens=64, dtype="bf16", window=1000, groups=[(12, 1024)])
     assert not joint(scene)
@@ -58,7 +70,7 @@ def test_a_window_leaves_a_prefix_to_each_sequence(engine):
 @pytest.mark.parametrize("dtype", ["bf16", "e4m3"])
 def test_rows_whose_weight_lies_on_one_side(engine, dtype):
     """Rows whose prefix has all the weight and rows whose own tokens have: the joining goes by the largest score of both."""
-    scene = Scene(6, 8, 2, 128, [2] * 16, [2048 + 2 + 17 * i for i in range(16)], page_tokens=128, dtype=dtype, groups=[(16, 2048)])
+    scene = Scene(6, 8, 2, 128, [2] * 16, [4096 + 2 + 17 * i for i in range(16)], page_tokens=128, dtype=dtype, groups=[(16, 4096)])
     assert joint(scene)
     scene.q = (scene.q.float() * torch.tensor([20.0, 0.01, 5.0, 1.0] * 8)[:, None, None]).to(TYPES[scene.q_type])
     scene.dq.copy_(scene.q)
@@ -67,7 +79,7 @@ def test_rows_whose_weight_lies_on_one_side(engine, dtype):
 
 def test_runs_are_equal_to_the_bit(engine):
     for dtype in ("bf16", "e4m3"):
-        scene = Scene(2, 24, 4, 256, [1] * 9 + [8] * 3, [2304 + 8 + 100 * i for i in range(12)], page_tokens=256, dtype=dtype, groups=[(12, 2304)])
+        scene = Scene(2, 24, 4, 256, [1] * 9 + [8] * 3, [4608 + 8 + 100 * i for i in range(12)], page_tokens=256, dtype=dtype, groups=[(12, 4608)])
         assert joint(scene)
         first = attend(engine, scene)
         paged = scene.paged(engine, S.PagedAttention)
@@ -83,7 +95,7 @@ def test_graphs_captured_with_groups_and_without_follow_any_batch(engine, dtype)
         own = [shared + 1 + (31 * (n + i)) % 300 for n in range(12)]
         held = sum(-(-n // 64) for n in own) - (shared // 64 * 11 if groups else 0)
         return Scene(40 + i, 12, 4, 128, rows, own, page_tokens=64, dtype=dtype, groups=[(12, shared)] if groups else [], spare_pages=pages - held)
-    scenes = [make(0, 256, False), make(1, 2048, True), make(2, 256, False), make(3, 3072, True), make(4, 64, True)]
+    scenes = [make(0, 256, False), make(1, 2048, True), make(2, 256, False), make(3, 2944, True), make(4, 64, True)]
     assert [joint(s) for s in scenes] == [False, True, False, True, False]
     paged = scenes[0].paged(engine, S.PagedAttention, max_context=4096)
     q, k, v, ks, vs = (torch.empty_like(x) for x in (scenes[0].dq, scenes[0].k, scenes[0].v, scenes[0].ks, scenes[0].vs))

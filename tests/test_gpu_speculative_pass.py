@@ -1,4 +1,4 @@
-"""A speculating server's decode step over tensors of the caller's own, whole: eight sequences behind one prompt, their verify blocks appended to an e4m3 cache, attended with the prompt's pages read once for all, the target's
+"""A speculating server's decode step over tensors of the caller's own, whole: twelve sequences behind one prompt, their verify blocks appended to an e4m3 cache, attended with the prompt's pages read once for all, the target's
 head, and the drafted tokens tested on the device. Against a plain 64-bit forward, against batches without groups, and captured into a graph."""
 import numpy as np
 import pytest
@@ -12,7 +12,7 @@ from test_gpu_own_pass import DIM, HEADS, KV, LAYERS, ROT, THETA, TOLERANCE, Mod
 
 pytestmark = pytest.mark.gpu
 
-PAGE, PAGES, PROMPT, SEQUENCES, BLOCK = 32, 80, 1536, 8, 4
+PAGE, PAGES, PROMPT, SEQUENCES, BLOCK = 32, 132, 2944, 12, 5
 # Keys and values are rounded to e4m3: independent relative errors of at most 2^-4 / sqrt(3) = 3.6e-2 (root mean square) of each, in two layers: 2 x 3.6e-2 of what the attention adds, which is at most all of the logits;
 # beside what the 16-bit roundings do.
 QUANTISED = 7.2e-2 + TOLERANCE
@@ -85,20 +85,20 @@ def test_a_decode_step_of_a_speculating_server(model):
     paged = model.paged(SEQUENCES, 64)
     for a in range(0, PROMPT, 64):                              # the prompt once, in the first sequence's pages
         model.step(paged, prompt[a:a + 64], [64], [a + 64], table[:1])
-    own = [rng.integers(0, model.g.vocab, 5 + 7 * s) for s in range(SEQUENCES)]
+    own = [rng.integers(0, model.g.vocab, 5 + 5 * s) for s in range(SEQUENCES)]
     for s in range(1, SEQUENCES):                               # what each has added since
         held = len(own[s]) - 1
         model.step(paged, own[s][:held], [held], [PROMPT + held], table[s:s + 1])
     held = len(own[0]) - 1
     model.step(paged, own[0][:held], [held], [PROMPT + held], table[:1])
-    # A block: the last token and three drafted ones.
+    # A block: the last token and four drafted ones.
     drafts = rng.integers(0, model.g.vocab, (SEQUENCES, BLOCK - 1))
     blocks = [np.concatenate([own[s][-1:], drafts[s]]) for s in range(SEQUENCES)]
     rows, lengths = [BLOCK] * SEQUENCES, [PROMPT + len(own[s]) - 1 + BLOCK for s in range(SEQUENCES)]
     drafted = np.concatenate([np.concatenate([drafts[s], [-1]]) for s in range(SEQUENCES)])
     u = rng.random((len(drafted), 2)).astype(np.float32)
     groups = [(SEQUENCES, PROMPT)]
-    assert debug_paged_plan_shared(rows, lengths, groups, heads=HEADS, kv_heads=KV, head_dim=DIM, pages=1, page_tokens=PAGE, max_sequences=SEQUENCES, max_rows=64, max_context=PAGE * PAGES)[4]
+    assert debug_paged_plan_shared(rows, lengths, groups, heads=HEADS, kv_heads=KV, head_dim=DIM, dtype="e4m3", pages=1, page_tokens=PAGE, max_sequences=SEQUENCES, max_rows=64, max_context=PAGE * PAGES)[4]
     # First with candidates that mean nothing, to see the logits; then as a drafter that knows them would have it.
     some = (np.tile(np.arange(8), (len(drafted), 1)), np.full((len(drafted), 8), 0.125, np.float32))
     logits, *_ = model.verify_step(paged, np.concatenate(blocks), rows, lengths, table, groups, drafted, some, u)
@@ -130,8 +130,9 @@ def test_append_attention_and_the_drafts_test_in_a_graph(model):
     """The three calls on a stream of the caller's, captured once and replayed while the sequences grow behind their common pages: the same bits as calls made one by one."""
     rng = np.random.default_rng(4)
     order = rng.permutation(PAGES).astype(np.int32)
-    table = np.stack([np.concatenate([order[:48], order[48 + 3 * s:51 + 3 * s]]) for s in range(SEQUENCES)])
-    width, n = (HEADS + 2 * KV) * DIM, 4 * SEQUENCES
+    shared = PROMPT // PAGE
+    table = np.stack([np.concatenate([order[:shared], order[shared + 3 * s:shared + 3 * (s + 1)]]) for s in range(SEQUENCES)])
+    width, n = (HEADS + 2 * KV) * DIM, BLOCK * SEQUENCES
     start = torch.randn((2, PAGES, KV, PAGE, DIM), device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)).to(torch.float8_e4m3fn).view(torch.uint8)
     states = []
     for graph_form in (False, True):
@@ -140,7 +141,7 @@ def test_append_attention_and_the_drafts_test_in_a_graph(model):
         k, v = start[0].clone(), start[1].clone()
         ks, vs = (torch.full((PAGES, KV, PAGE), 0.02, device="cuda") for _ in range(2))
         qkv, q, out = torch.zeros((n, width), device="cuda"), torch.zeros((n, HEADS, DIM), device="cuda", dtype=torch.bfloat16), torch.zeros((n, HEADS * DIM), device="cuda")
-        first, drafts = torch.arange(0, n + 1, 4, device="cuda", dtype=torch.int32), torch.zeros(n, device="cuda", dtype=torch.int32)
+        first, drafts = torch.arange(0, n + 1, BLOCK, device="cuda", dtype=torch.int32), torch.zeros(n, device="cuda", dtype=torch.int32)
         u, ids = torch.zeros((n, 2), device="cuda"), torch.zeros(n + 2 * SEQUENCES, device="cuda", dtype=torch.int32)
         stream = torch.cuda.Stream()
         torch.cuda.synchronize()
@@ -152,7 +153,7 @@ def test_append_attention_and_the_drafts_test_in_a_graph(model):
             model.engine.pass_verify(out.data_ptr(), SEQUENCES, n, HEADS * DIM, HEADS * DIM, first.data_ptr(), drafts.data_ptr(), u.data_ptr(), ids.data_ptr(), ids[n:].data_ptr(), ids[n + SEQUENCES:].data_ptr(),
                                      stream=stream.cuda_stream)
         def batch(t):
-            paged.batch([4] * SEQUENCES, [1536 + 4 * (t + 1) + s for s in range(SEQUENCES)], table, groups=[(SEQUENCES, 1536)], stream=stream.cuda_stream)
+            paged.batch([BLOCK] * SEQUENCES, [PROMPT + BLOCK * (t + 1) + s for s in range(SEQUENCES)], table, groups=[(SEQUENCES, PROMPT)], stream=stream.cuda_stream)
         batch(0)
         graph = torch.cuda.CUDAGraph()
         if graph_form:

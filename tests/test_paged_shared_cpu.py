@@ -107,3 +107,19 @@ def test_a_prefix_is_read_once_for_128_packed_rows():
     assert max(load) <= 2 * tiles / 148 + 4
     # Two sequences that share too little to be worth it.
     assert not debug_paged_plan_shared([1] * 2, [300] * 2, [(2, 256)], heads=24, kv_heads=4, head_dim=256, pages=1, max_sequences=2, max_rows=2, max_context=1 << 16)[4]
+
+
+def test_over_a_cache_of_e4m3_few_rows_meet_a_prefix_48_at_a_time():
+    """Two verify blocks of four rows, six heads a kv head, over 16,384 shared tokens: their 48 packed rows are one block's. With a sequence of seven rows (42 packed) beside them the batch's form has 128."""
+    config = dict(heads=24, kv_heads=4, head_dim=256, dtype="e4m3", pages=1, max_sequences=16, max_rows=128, max_context=1 << 16)
+    for rows, width in (([4] * 6, 48), ([4] * 6 + [7], 128), ([1] * 16, 48)):
+        begin, items, records, _, joint = debug_paged_plan_shared(rows, [16384 + 300] * len(rows), [(len(rows), 16384)], **config)
+        assert joint
+        packed = 6 * sum(rows)
+        over = [(int(i[3]), int(i[4])) for i in items if i[6] <= 128]
+        assert set(over) <= {(q, min(width, packed - q)) for q in range(0, packed, width)}
+        assert sum(int(i[6] - i[5]) for i in items if i[6] <= 128) == 4 * 128 * -(-packed // width)
+        joined = np.zeros((sum(rows) * 6, 4), int)
+        for row0, q0, h, count, *_ in records.tolist():
+            joined[6 * row0 + q0:6 * row0 + q0 + count, h] += 1
+        assert (joined == 1).all()
