@@ -37,18 +37,20 @@ struct spl_paged {
     cudaEvent_t copied[2] = {};
     int turn = 0;
     double *turns = nullptr;
-    // What a batch with groups is dealt by, made by the first of them, and from then on filled by every batch (a captured graph may hold either form): the count of joining work, the
-    // plan's block_begin, starts and items, the records, the work. Partial sums by the row.
-    struct Shared {
+    // What a batch is dealt by whose pieces a kernel of its own joins: the count of joining work, the plan's block_begin, starts and items, the records, the work; partial sums by the row.
+    struct ByRows {
         size_t words = 0, begin_at = 16, starts_at = 0, items_at = 0, records_at = 0, work_at = 0;
         int *dev = nullptr, *host[2] = {};
         float *partial = nullptr;
         float2 *partial_ml = nullptr;
         SplPagedPlan plan;
-    } shared;
+        int work = 0;
+    };
+    // Of batches with groups, made by the first of them, and from then on filled by every batch (a captured graph may hold either form); of batches without that are joined so, which their rows decide.
+    ByRows shared, split;
     // The batch that was set last.
-    int rows = 0, combine_work = 0, packed = 0;      // packed: the most packed rows a sequence has
-    bool ready = false, shared_write = false, joint = false;
+    int rows = 0, packed = 0;      // packed: the most packed rows a sequence has
+    bool ready = false, shared_write = false, joint = false, by_rows = false;      // joint: some sequences meet a prefix together; by_rows: in `split`
     std::vector<uint8_t> written;      // scratch of the check for pages that two sequences would write
 
     SplPagedTables tables() const {
@@ -75,7 +77,31 @@ template <int HD> static bool paged_configure_e4m3() {
 }
 // (The opt-in is a property of the current device.)
 static bool paged_configure(int head_dim, bool e4m3) {
-    if (e4m3) return head_dim == 64 ? paged_configure_e4m3<64>() : head_dim == 128 ? paged_configure_e4m3<128>() : paged_configure_e4m3<256>();     return head_dim == 64 ? paged_configure_dim<64>() : head_dim == 128 ? paged_configure_dim<128>() : paged_configure_dim<256>();
+    if (e4m3) return head_dim == 64 ? paged_configure_e4m3<64>() : head_dim == 128 ? paged_configure_e4m3<128>() : paged_configure_e4m3<256>();
+    return head_dim == 64 ? paged_configure_dim<64>() : head_dim == 128 ? paged_configure_dim<128>() : paged_configure_dim<256>();
+}
+
+// The device and pinned memory of plans of so many items, records, joining work and rows of partial sums.
+static spl_status paged_by_rows_create(spl_paged *p, spl_paged::ByRows &t, int64_t items, int64_t records, int64_t work, int64_t partial_rows) {
+    spl_engine *e = p->e;
+    if (t.dev) return SPL_OK;
+    const size_t blocks = size_t(e->sms), item = sizeof(SplPagedItem) / 4;
+    t.starts_at = t.begin_at + (blocks + 1 + 3) / 4 * 4;
+    t.items_at = t.starts_at + blocks * item;
+    t.records_at = t.items_at + size_t(items) * item;
+    t.work_at = t.records_at + size_t(records) * (sizeof(SplPagedRecord) / 4);
+    t.words = t.work_at + size_t(work) * 2;
+    const size_t table_bytes = (t.words * 4 + 255) / 256 * 256;
+    int *host = nullptr;
+    SPL_CUDA(cudaMallocHost(reinterpret_cast<void **>(&host), t.words * 8));
+    unsigned char *block = nullptr;
+    const cudaError_t made = cudaMalloc(reinterpret_cast<void **>(&block), table_bytes + size_t(partial_rows) * (size_t(p->c.head_dim) * 4 + sizeof(float2)));
+    if (made != cudaSuccess) { cudaFreeHost(host); SPL_CUDA(made); }
+    t.host[0] = host; t.host[1] = host + t.words;
+    t.partial = reinterpret_cast<float *>(block + table_bytes);
+    t.partial_ml = reinterpret_cast<float2 *>(t.partial + size_t(partial_rows) * p->c.head_dim);
+    t.dev = reinterpret_cast<int *>(block);
+    return SPL_OK;
 }
 
 static spl_status paged_create(spl_engine *e, const spl_paged_config *cp, spl_paged *p) {
@@ -110,14 +136,18 @@ static spl_status paged_create(spl_engine *e, const spl_paged_config *cp, spl_pa
     if (found != cudaDriverEntryPointSuccess || !encode) return e->fail(SPL_ERR_UNSUPPORTED_DEVICE, "spl_paged_create: the driver has no tensor maps");
     p->encode = reinterpret_cast<SplEncodeTiled>(encode);
     if (!paged_configure(c.head_dim, c.dtype == SPL_E4M3)) return e->fail(SPL_ERR_UNSUPPORTED_DEVICE, "spl_paged_create: the kernel's shared-memory opt-in failed");
+    if (c.dtype == SPL_E4M3 && int64_t(c.max_rows) * p->shape.group > 16) {
+        const spl_status made = paged_by_rows_create(p, p->split, int64_t(items), int64_t(items), spl_paged_split_combine_max(c, e->sms), spl_paged_split_rows_max(c, e->sms));
+        if (made != SPL_OK) return made;
+    }
     double turns[128] = {};
     for (int i = 0; i < c.rotary_dim / 2; ++i) turns[i] = std::pow(double(c.rope_theta), -2.0 * i / c.rotary_dim) / 6.283185307179586476925;
     return upload(e, p->turns, turns, sizeof turns);
 }
 
 static void paged_release(spl_paged *p) {
-    cudaFree(p->tables_dev); cudaFree(p->shared.dev);
-    if (p->shared.host[0]) cudaFreeHost(p->shared.host[0]);
+    cudaFree(p->tables_dev);
+    for (spl_paged::ByRows *t : {&p->shared, &p->split}) { cudaFree(t->dev); if (t->host[0]) cudaFreeHost(t->host[0]); }
     if (p->tables_host[0]) cudaFreeHost(p->tables_host[0]);
     for (cudaEvent_t event : p->copied) if (event) cudaEventDestroy(event);
     delete p;
@@ -125,47 +155,21 @@ static void paged_release(spl_paged *p) {
 
 static cudaStream_t paged_stream(const spl_engine *e, void *stream) { return stream ? static_cast<cudaStream_t>(stream) : e->stream; }
 
-// The device and pinned memory of batches with groups.
-static spl_status paged_shared_create(spl_paged *p) {
-    spl_engine *e = p->e;
-    spl_paged::Shared &sh = p->shared;
-    if (sh.dev) return SPL_OK;
-    const size_t blocks = size_t(e->sms), item = sizeof(SplPagedItem) / 4;
-    sh.starts_at = sh.begin_at + (blocks + 1 + 3) / 4 * 4;
-    sh.items_at = sh.starts_at + blocks * item;
-    sh.records_at = sh.items_at + size_t(spl_paged_shared_items_max(p->c, e->sms)) * item;
-    sh.work_at = sh.records_at + size_t(spl_paged_records_max(p->c, e->sms)) * (sizeof(SplPagedRecord) / 4);
-    sh.words = sh.work_at + size_t(spl_paged_combine_max(p->c, e->sms)) * 2;
-    const size_t table_bytes = (sh.words * 4 + 255) / 256 * 256, partial_rows = size_t(spl_paged_partial_rows_max(p->c, e->sms));
-    int *host = nullptr;
-    SPL_CUDA(cudaMallocHost(reinterpret_cast<void **>(&host), sh.words * 8));
-    unsigned char *block = nullptr;
-    const cudaError_t made = cudaMalloc(reinterpret_cast<void **>(&block), table_bytes + partial_rows * (size_t(p->c.head_dim) * 4 + sizeof(float2)));
-    if (made != cudaSuccess) { cudaFreeHost(host); SPL_CUDA(made); }
-    sh.host[0] = host; sh.host[1] = host + sh.words;
-    sh.partial = reinterpret_cast<float *>(block + table_bytes);
-    sh.partial_ml = reinterpret_cast<float2 *>(sh.partial + partial_rows * p->c.head_dim);
-    sh.dev = reinterpret_cast<int *>(block);
-    return SPL_OK;
-}
-
-// The plan with groups, in the words of pinned block `turn`: how many are used.
-static size_t paged_shared_fill(spl_paged *p, int turn, int32_t sequences, const int32_t *rows, const int32_t *lengths, const SplPagedGroups &groups) {
-    spl_paged::Shared &sh = p->shared;
-    const SplPagedPlan &plan = sh.plan;
-    spl_paged_plan(p->c, p->e->sms, sequences, rows, lengths, sh.plan, &groups);
-    int *w = sh.host[turn], work = 0;
-    std::memcpy(w + sh.begin_at, plan.block_begin.data(), plan.block_begin.size() * 4);
-    std::memcpy(w + sh.starts_at, plan.starts.data(), plan.starts.size() * sizeof(SplPagedItem));
-    std::memcpy(w + sh.items_at, plan.items.data(), plan.items.size() * sizeof(SplPagedItem));
-    std::memcpy(w + sh.records_at, plan.records.data(), plan.records.size() * sizeof(SplPagedRecord));
+// The plan, in the words of pinned block `turn`: how many are used.
+static size_t paged_by_rows_fill(const spl_paged *p, spl_paged::ByRows &t, int turn) {
+    const SplPagedPlan &plan = t.plan;
+    int *w = t.host[turn], work = 0;
+    std::memcpy(w + t.begin_at, plan.block_begin.data(), plan.block_begin.size() * 4);
+    std::memcpy(w + t.starts_at, plan.starts.data(), plan.starts.size() * sizeof(SplPagedItem));
+    std::memcpy(w + t.items_at, plan.items.data(), plan.items.size() * sizeof(SplPagedItem));
+    std::memcpy(w + t.records_at, plan.records.data(), plan.records.size() * sizeof(SplPagedRecord));
     const int chunks = (p->c.head_dim + 127) / 128;
     for (size_t r = 0; r < plan.records.size(); ++r)
-        for (int job = 0; job < plan.records[r].count * chunks; job += 4, ++work) { w[sh.work_at + 2 * work] = int(r); w[sh.work_at + 2 * work + 1] = job; }
+        for (int job = 0; job < plan.records[r].count * chunks; job += 4, ++work) { w[t.work_at + 2 * work] = int(r); w[t.work_at + 2 * work + 1] = job; }
     std::memset(w, 0, 16 * 4);
     w[0] = work;
-    p->combine_work = work;
-    return sh.work_at + 2 * size_t(work);
+    t.work = work;
+    return t.work_at + 2 * size_t(work);
 }
 
 static spl_status paged_batch(spl_paged *p, int32_t sequences, const int32_t *rows, const int32_t *lengths, const int32_t *table, int32_t table_ld, const SplPagedGroups &groups, cudaStream_t stream) {
@@ -180,21 +184,27 @@ static spl_status paged_batch(spl_paged *p, int32_t sequences, const int32_t *ro
     if (capture != cudaStreamCaptureStatusNone) return e->fail(SPL_ERR_INVALID_ARGUMENT, "spl_paged_batch: a batch is set outside a capture");
     if (groups.count) {
         if (!spl_paged_groups_check(c, sequences, rows, lengths, table, table_ld, groups, &why)) return e->fail(SPL_ERR_INVALID_ROWS, "spl_paged_batch_shared: " + why);
-        const spl_status made = paged_shared_create(p);
+        const spl_status made = paged_by_rows_create(p, p->shared, spl_paged_shared_items_max(c, e->sms), spl_paged_records_max(c, e->sms), spl_paged_combine_max(c, e->sms), spl_paged_partial_rows_max(c, e->sms));
         if (made != SPL_OK) { cudaGetLastError(); return made; }
     }
-    int64_t total = 0;
-    for (int s = 0; s < sequences; ++s) total += rows[s];
-    spl_paged_plan(c, e->sms, sequences, rows, lengths, p->plan);
+    int64_t total = 0, packed = 0;
+    for (int s = 0; s < sequences; ++s) { total += rows[s]; packed = std::max(packed, int64_t(rows[s]) * p->shape.group); }
+    // (Only the plan that is launched by has to be right; a graph of these rows takes the same one.)
+    const bool by_rows = spl_paged_split(c, packed);
+    const SplPagedGroups none{0, nullptr, nullptr};
+    if (by_rows) spl_paged_plan(c, e->sms, sequences, rows, lengths, p->split.plan, &none);
+    else spl_paged_plan(c, e->sms, sequences, rows, lengths, p->plan);
+    if (p->shared.dev) spl_paged_plan(c, e->sms, sequences, rows, lengths, p->shared.plan, &groups);
     const int turn = p->turn;
     SPL_CUDA(cudaEventSynchronize(p->copied[turn]));      // this block's last copy
     int *w = p->tables_host[turn];
     std::memset(w, 0, 16 * 4);
     w[0] = int(total);
-    std::memcpy(w + p->begin_at, p->plan.block_begin.data(), p->plan.block_begin.size() * 4);
+    const SplPagedPlan empty, &plan = by_rows ? empty : p->plan;
+    std::memcpy(w + p->begin_at, plan.block_begin.data(), plan.block_begin.size() * 4);
     std::memset(w + p->arrived_at, 0, size_t(e->sms) * 4);
-    std::memcpy(w + p->starts_at, p->plan.starts.data(), p->plan.starts.size() * sizeof(SplPagedItem));
-    std::memcpy(w + p->items_at, p->plan.items.data(), p->plan.items.size() * sizeof(SplPagedItem));
+    std::memcpy(w + p->starts_at, plan.starts.data(), plan.starts.size() * sizeof(SplPagedItem));
+    std::memcpy(w + p->items_at, plan.items.data(), plan.items.size() * sizeof(SplPagedItem));
     int *row_sequence = w + p->batch_at, *row_position = row_sequence + c.max_rows, *pages = w + p->table_at;
     int longest = 1;
     for (int s = 0, r = 0; s < sequences; ++s) {
@@ -203,18 +213,17 @@ static spl_status paged_batch(spl_paged *p, int32_t sequences, const int32_t *ro
         if (used) std::memcpy(pages + size_t(s) * p->max_pages, table + size_t(s) * table_ld, size_t(used) * 4);
         longest = std::max(longest, used);
     }
-    const size_t planned = p->items_at + p->plan.items.size() * (sizeof(SplPagedItem) / 4), pitch = size_t(p->max_pages) * 4;
+    const size_t planned = p->items_at + plan.items.size() * (sizeof(SplPagedItem) / 4), pitch = size_t(p->max_pages) * 4;
     SPL_CUDA(cudaMemcpyAsync(p->tables_dev, w, planned * 4, cudaMemcpyHostToDevice, stream));
     SPL_CUDA(cudaMemcpy2DAsync(p->tables_dev + p->table_at, pitch, pages, pitch, size_t(longest) * 4, size_t(sequences), cudaMemcpyHostToDevice, stream));
-    if (p->shared.dev) {
-        const size_t used = paged_shared_fill(p, turn, sequences, rows, lengths, groups);
-        SPL_CUDA(cudaMemcpyAsync(p->shared.dev, p->shared.host[turn], used * 4, cudaMemcpyHostToDevice, stream));
+    for (spl_paged::ByRows *t : {&p->shared, &p->split}) {
+        if (t == &p->shared ? !t->dev : !by_rows) continue;
+        const size_t used = paged_by_rows_fill(p, *t, turn);
+        SPL_CUDA(cudaMemcpyAsync(t->dev, t->host[turn], used * 4, cudaMemcpyHostToDevice, stream));
     }
-    p->joint = p->shared.dev && p->shared.plan.joint;
     SPL_CUDA(cudaEventRecord(p->copied[turn], stream));
     p->turn ^= 1;
-    p->packed = 0;
-    for (int s = 0; s < sequences; ++s) p->packed = std::max(p->packed, int(std::min<int64_t>(int64_t(rows[s]) * p->shape.group, 1 << 30)));
+    p->joint = p->shared.dev && p->shared.plan.joint; p->by_rows = by_rows; p->packed = int(std::min<int64_t>(packed, 1 << 30));
     p->rows = int(total); p->shared_write = shared; p->ready = true;
     return SPL_OK;
 }
@@ -233,14 +242,12 @@ template <int TYPE> static void launch_append(const spl_paged *p, const SplPaged
     else launch_append_dim<TYPE, 256>(p, in, q_norm, k_norm, out, stream);
 }
 
-// Whether the batch's attention runs in the transposed form.
-static bool paged_narrow(const spl_paged *p) { return p->joint ? spl_paged_joint_narrow(p->c, p->packed) : spl_paged_narrow(p->c, p->packed); }
 // The cache as a tensor (channel in block, token in page, block of 64 channels, kv head, page) for the copies of values, in boxes of all channels by a page's tokens (at most a
 // chunk's), or of keys: of a page's tokens (at most a tile's) by 64 channels, or by a chunk's where the box is a tile's tokens.
 static bool paged_map(const spl_paged *p, const void *cache, bool values, CUtensorMap *map) {
     const spl_paged_config &c = p->c;
     if (c.dtype == SPL_E4M3) {
-        values = values && !paged_narrow(p);      // (there the values come in the keys' boxes)
+        values = values && !spl_paged_narrow(p->c, p->packed);      // (there the values come in the keys' boxes)
         // In bytes, blocks of 128 channels (all of 64): boxes of a block by a page's tokens (at most a tile's) of keys, of all blocks by a page's tokens (at most a chunk's) of values.
         const cuuint64_t row = cuuint64_t(std::min(c.head_dim, 128)), blocks = cuuint64_t(c.head_dim) / row, dims[5] = {row, cuuint64_t(c.page_tokens), blocks, cuuint64_t(c.kv_heads), cuuint64_t(c.pages)};
         const cuuint64_t strides[4] = {cuuint64_t(c.token_stride), row, cuuint64_t(c.head_stride), cuuint64_t(c.page_stride)};
@@ -263,7 +270,7 @@ template <int HD, bool BF16> static void launch_attend(const spl_paged *p, const
 
 template <int HD> static void launch_attend_e4m3(const spl_paged *p, const CUtensorMap &k_map, const CUtensorMap &v_map, const SplPagedAttend &a, const SplPagedScaled &scales, cudaStream_t stream) {
     if constexpr (HD >= 128) {
-        if (paged_narrow(p)) {
+        if (spl_paged_narrow(p->c, p->packed)) {
             // (Over a prefix, several sequences' rows: as many as the batch has.)
             const int packed = p->joint ? std::min(p->rows * p->shape.group, SPL_PAGED8_NARROW) : p->packed, n = packed <= 16 ? 16 : packed <= 32 ? 32 : 48;
             launch_step(n == 16 ? spl_paged_attend_e4m3_narrow_kernel<HD, 16> : n == 32 ? spl_paged_attend_e4m3_narrow_kernel<HD, 32> : spl_paged_attend_e4m3_narrow_kernel<HD, 48>, dim3(p->e->sms), dim3(spl_paged8n_threads(n)),
@@ -306,8 +313,8 @@ static spl_status launch_sample(spl_engine *e, const SplSampleArgs &args, int ro
 }
 
 // Four warps a block; a graph's replay may have other work than the batch it was captured with, so the blocks go round.
-static void launch_combine(const spl_paged *p, const SplPagedCombine &j, cudaStream_t stream) {
-    const dim3 grid(std::max(1, std::min(p->combine_work, 4 * p->e->sms)));
+static void launch_combine(const spl_paged *p, int work, const SplPagedCombine &j, cudaStream_t stream) {
+    const dim3 grid(std::max(1, std::min(work, 4 * p->e->sms)));
     const int hd = p->c.head_dim;
     const bool bf16 = p->c.dtype != SPL_F16;
     launch_step(hd == 64 ? (bf16 ? spl_paged_combine_kernel<64, true> : spl_paged_combine_kernel<64, false>) : hd == 128 ? (bf16 ? spl_paged_combine_kernel<128, true> : spl_paged_combine_kernel<128, false>) :
@@ -358,13 +365,12 @@ static spl_status paged_attend(spl_paged *p, const char *name, bool scaled, cons
     if (misaligned(k_scale, 16) || misaligned(v_scale, 16)) return refuse("scales begin on a 16-byte boundary");
     const SplDeviceScope scope(e->device);
     cudaStream_t st = paged_stream(e, stream);
-    // A batch whose sequences meet a prefix together has tables, partial sums by the row and a joining kernel of its own.
-    const spl_paged::Shared &sh = p->shared;
-    const bool joint = p->joint;
-    const int *tables = joint ? sh.dev : p->tables_dev;
-    const SplPagedAttend a{static_cast<const uint16_t *>(device_q), device_out, out_type == SPL_F32, reinterpret_cast<const SplPagedItem *>(tables + (joint ? sh.starts_at : p->starts_at)),
-                           reinterpret_cast<const SplPagedItem *>(tables + (joint ? sh.items_at : p->items_at)), tables + (joint ? sh.begin_at : p->begin_at), p->tables_dev + p->arrived_at,
-                           joint ? sh.partial : p->partial, joint ? sh.partial_ml : p->partial_ml, joint ? 1 : p->slot_rows, e->tc_error};
+    // Tables, partial sums by the row and a joining kernel of its own, or the attention's own joins.
+    const spl_paged::ByRows *const t = p->joint ? &p->shared : p->by_rows ? &p->split : nullptr;
+    const int *tables = t ? t->dev : p->tables_dev;
+    const SplPagedAttend a{static_cast<const uint16_t *>(device_q), device_out, out_type == SPL_F32, reinterpret_cast<const SplPagedItem *>(tables + (t ? t->starts_at : p->starts_at)),
+                           reinterpret_cast<const SplPagedItem *>(tables + (t ? t->items_at : p->items_at)), tables + (t ? t->begin_at : p->begin_at), p->tables_dev + p->arrived_at,
+                           t ? t->partial : p->partial, t ? t->partial_ml : p->partial_ml, t ? 1 : p->slot_rows, e->tc_error};
     CUtensorMap k_map, v_map;
     if (!paged_map(p, device_k_cache, false, &k_map) || !paged_map(p, device_v_cache, true, &v_map)) return refuse("the driver takes no tensor map of this cache");
     const bool bf16 = c.dtype == SPL_BF16;
@@ -376,9 +382,9 @@ static spl_status paged_attend(spl_paged *p, const char *name, bool scaled, cons
     } else if (c.head_dim == 64) { if (bf16) launch_attend<64, true>(p, k_map, v_map, a, st); else launch_attend<64, false>(p, k_map, v_map, a, st); }
     else if (c.head_dim == 128) { if (bf16) launch_attend<128, true>(p, k_map, v_map, a, st); else launch_attend<128, false>(p, k_map, v_map, a, st); }
     else { if (bf16) launch_attend<256, true>(p, k_map, v_map, a, st); else launch_attend<256, false>(p, k_map, v_map, a, st); }
-    if (joint) {
-        const SplPagedCombine j{sh.dev, reinterpret_cast<const int2 *>(sh.dev + sh.work_at), reinterpret_cast<const SplPagedRecord *>(sh.dev + sh.records_at), sh.partial, sh.partial_ml, device_out, a.out_f32};
-        launch_combine(p, j, st);
+    if (t) {
+        const SplPagedCombine j{t->dev, reinterpret_cast<const int2 *>(t->dev + t->work_at), reinterpret_cast<const SplPagedRecord *>(t->dev + t->records_at), t->partial, t->partial_ml, device_out, a.out_f32};
+        launch_combine(p, t->work, j, st);
     }
     return check_launch(e, "spl_paged_attend");
 }

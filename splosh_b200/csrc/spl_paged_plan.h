@@ -143,23 +143,22 @@ inline int64_t spl_paged_take(int64_t t, int64_t left, int64_t stretch, int q_co
 // With groups, the sequences of a run (consecutive members of a group, none with more packed rows than a block takes) meet the whole tiles of their prefix
 // together: their rows lie one behind the other, so they are the rows of one sequence over the prefix, in blocks of 128 packed rows whoever's they are; each sequence's own
 // tokens are units of their own, and both leave partial sums (O, m, l) that spl_paged_combine_kernel joins. (Sequences of more packed rows read the prefix once for 128 of them as it is.)
-// Over a cache of e4m3 the rows that meet a prefix together take the transposed form, 48 a block, where a sequence has up to 36 of them, and the form of 128 where two sequences' do not fit 48 any more by much
-// (heads of 256, 24 on 4: four sequences of 24 packed rows over 20,992 shared tokens 35.2 us in the former and 38.4 in the latter, of 36 43.9 and 54.2, two of 48 57.5 and 37.9).
-// Both go by the most packed rows that a sequence has, so a graph that holds one form is right for every batch of its rows.
-#define SPL_PAGED8_JOINT_NARROW 36
+// Over a cache of e4m3 a batch takes the transposed form by the most packed rows that a sequence has, also where sequences meet a prefix together (48 rows a block then), so a graph that holds one form is right for
+// every batch of its rows.
 inline bool spl_paged_narrow(const spl_paged_config &c, int64_t packed) { return c.dtype == SPL_E4M3 && c.head_dim >= 128 && packed <= SPL_PAGED8_NARROW; }
-inline bool spl_paged_joint_narrow(const spl_paged_config &c, int64_t packed) { return spl_paged_narrow(c, packed) && packed <= SPL_PAGED8_JOINT_NARROW; }
+// And over such a cache the pieces of a batch whose sequences have more than 16 packed rows, but at most a block's, are joined by the kernel of its own, groups or not. In and behind the attention: heads of 256
+// (24 on 4), one verify block of eight rows over 1,000, 4,000 and 32,000 tokens 22.2 and 15.7, 39.2 and 17.0, 82.7 and 31.2 us, one of sixteen over 4,000 66.9 and 22.1, eight of eight over 39,000 135.7 and 123.6;
+// heads of 64 (16 on 2), eight of sixteen over 3,600 45.8 and 18.9; 32 sequences, of which few are cut, the same. Prompts: 300 rows over 300 tokens 19.7 and 22.8, 2,048 over 8,192 1,358 and 1,396. (With
+// up to 16 rows a piece's join is short: the launch would cost more.)
+inline bool spl_paged_split(const spl_paged_config &c, int64_t packed) { return c.dtype == SPL_E4M3 && packed > 16 && packed <= SPL_PAGED_TILE; }
 // Meeting together pays where the tiles saved are more than the joining: so many a block for one more launch and the pieces' first keys, and one for so many rows of heads that leave and join sums. Measured with
 // heads of 256, 24 of them on 4, together and apart:
-//   tiles of one cost      six sequences of one row over 1,024 shared tokens 15.2 and 13.7 us, over 4,096 17.7 and 21.8; sixteen of four rows over 512 21.5 and 19.7, over 1,024 22.0 and 23.0;
-//                          48 of four over 256 35.7 and 30.3, over 512 35.6 and 36.6;
-//   transposed, both       (apart it is quick where sequences find the same keys in L2, most of all with up to 16 packed rows) six of one row over 4,096 19.4 and 15.7, sixteen over 2,048 19.2 and 19.3;
-//                          two of four rows over 8,192 23.0 and 32.7, sixteen over 2,048 30.6 and 25.0, over 8,192 46.9 and 56.9, 48 over 2,048 63.7 and 55.7;
-//   transposed apart only  two of eight rows over 20,992 37.9 and 57.6, eight over 4,096 38.9 and 34.5, over 20,992 71.1 and 83.2, 24 over 4,096 74.9 and 56.7.
-inline bool spl_paged_joint_pays(const spl_paged_config &c, int64_t saved, int blocks, int64_t rows_of_heads, int64_t most) {
-    if (spl_paged_joint_narrow(c, most)) return saved > int64_t(blocks) * (most <= 16 ? 4 : 1) + rows_of_heads / 3;
-    return saved > blocks + (spl_paged_narrow(c, most) ? rows_of_heads : rows_of_heads / 10);
-}
+//   in 16 bits    six sequences of one row over 1,024 shared tokens 15.2 and 13.7 us, over 4,096 17.7 and 21.8; sixteen of four rows over 512 21.5 and 19.7, over 1,024 22.0 and 23.0;
+//                 48 of four over 256 35.7 and 30.3, over 512 35.6 and 36.6;
+//   transposed    (apart it is quick where sequences find the same keys in L2) six of one row over 4,096 19.4 and 15.7, sixteen over 2,048 19.2 and 19.3, 48 over 1,024 31.1 and 31.2; two of four rows over
+//                 20,992 28.1 and 27.0, four 35.3 and 36.1, eight 46.9 and 59.0; 24 of four over 4,096 47.4 and 50.0, 24 of six 63.2 and 58.5;
+//   e4m3, wide    eight of sixteen rows over 4,096 53.7 and 45.5, over 20,992 116 and 126.
+inline bool spl_paged_joint_pays(int64_t saved, int blocks, int64_t rows_of_heads, bool narrow) { return saved > int64_t(blocks) * (narrow ? 4 : 1) + rows_of_heads / (narrow ? 3 : 10); }
 struct SplPagedUnit { SplPagedItem item; bool joint; int run, prefix; };      // run: its run of sequences or -1; prefix: the first of its run's prefix units of its kv head
 inline void spl_paged_plan(const spl_paged_config &c, int blocks, int32_t sequences, const int32_t *rows, const int32_t *lengths, SplPagedPlan &plan, const SplPagedGroups *groups = nullptr) {
     const int group = c.heads / c.kv_heads, tile = SPL_PAGED_TILE;
@@ -178,7 +177,7 @@ inline void spl_paged_plan(const spl_paged_config &c, int blocks, int32_t sequen
     plan.joint = false;
     int64_t most = 0;
     for (int i = 0; i < sequences; ++i) most = std::max(most, int64_t(rows[i]) * group);
-    const int width = spl_paged_joint_narrow(c, most) ? SPL_PAGED8_NARROW : tile;
+    const int width = spl_paged_narrow(c, most) ? SPL_PAGED8_NARROW : tile;
     std::vector<int> run_row0;
     int s = 0, row0 = 0;
     auto pass_over = [&]() { add_sequence(s, row0, 0, -1, 0, 0); row0 += rows[s]; ++s; };
@@ -190,7 +189,7 @@ inline void spl_paged_plan(const spl_paged_config &c, int blocks, int32_t sequen
             int64_t packed = 0;
             while (run_end < end && int64_t(rows[run_end]) * group <= tile) { packed += rows[run_end] * group; members += rows[run_end] > 0; ++run_end; }
             const int64_t joint_units = (packed + width - 1) / width;
-            if (members < 2 || !spl_paged_joint_pays(c, int64_t(c.kv_heads) * prefix * (members - joint_units), blocks, packed * c.kv_heads, most)) {
+            if (members < 2 || !spl_paged_joint_pays(int64_t(c.kv_heads) * prefix * (members - joint_units), blocks, packed * c.kv_heads, width < tile)) {
                 do pass_over(); while (s < run_end);
                 continue;
             }
@@ -204,15 +203,16 @@ inline void spl_paged_plan(const spl_paged_config &c, int blocks, int32_t sequen
         }
     }
     while (s < sequences) pass_over();
+    const bool by_rows = plan.joint || (groups && spl_paged_split(c, most));
     // The least stretch that makes do with the blocks there are.
     auto blocks_for = [&](int64_t stretch) {
         int64_t used = 1, left = stretch;
         for (const SplPagedUnit &u : whole)
             for (int64_t t = u.item.tile_end - u.item.tile_begin, all = t; t > 0;) {
-                const int64_t take = spl_paged_take(t, left, stretch, u.item.q_count, t < all || u.joint, plan.joint);
+                const int64_t take = spl_paged_take(t, left, stretch, u.item.q_count, t < all || u.joint, by_rows);
                 if (take < 0) return int64_t(blocks) + 1;
                 if (!take) { if (++used > blocks) return used; left = stretch; continue; }
-                left -= take + SPL_PAGED_PIECE_COST + (take < all || u.joint ? spl_paged_cut_cost(u.item.q_count, plan.joint) : 0);
+                left -= take + SPL_PAGED_PIECE_COST + (take < all || u.joint ? spl_paged_cut_cost(u.item.q_count, by_rows) : 0);
                 t -= take;
             }
         return used;
@@ -229,12 +229,12 @@ inline void spl_paged_plan(const spl_paged_config &c, int blocks, int32_t sequen
         const size_t piece0 = units.size();
         const int all = u.tile_end - u.tile_begin;
         for (int t = u.tile_begin; t < u.tile_end;) {
-            const int take = int(spl_paged_take(u.tile_end - t, left, low, u.q_count, t > u.tile_begin || one.joint, plan.joint));
+            const int take = int(spl_paged_take(u.tile_end - t, left, low, u.q_count, t > u.tile_begin || one.joint, by_rows));
             if (!take) { plan.block_begin.push_back(int32_t(units.size())); left = low; continue; }
             SplPagedItem piece = u;
             piece.tile_begin = t; piece.tile_end = t + take;
             units.push_back(piece);
-            left -= take + SPL_PAGED_PIECE_COST + (take < all || one.joint ? spl_paged_cut_cost(u.q_count, plan.joint) : 0);
+            left -= take + SPL_PAGED_PIECE_COST + (take < all || one.joint ? spl_paged_cut_cost(u.q_count, by_rows) : 0);
             t += take;
         }
         const int pieces = int(units.size() - piece0);
@@ -277,5 +277,8 @@ inline int64_t spl_paged_partial_rows_max(const spl_paged_config &c, int blocks)
 inline int64_t spl_paged_combine_max(const spl_paged_config &c, int blocks) {      // of blocks of the joining kernel's work, four (row, channels) each
     return (spl_paged_joint_rows_max(c) + int64_t(blocks) * SPL_PAGED_TILE) * ((c.head_dim + 127) / 128) / 4 + spl_paged_records_max(c, blocks);
 }
+// The same of a plan without groups whose pieces the kernel of its own joins: a block's boundary cuts at most one unit, and each cut makes two pieces of one.
+inline int64_t spl_paged_split_rows_max(const spl_paged_config &c, int blocks) { return int64_t(blocks) * 2 * std::min<int64_t>(SPL_PAGED_TILE, int64_t(c.max_rows) * (c.heads / c.kv_heads)); }
+inline int64_t spl_paged_split_combine_max(const spl_paged_config &c, int blocks) { return spl_paged_split_rows_max(c, blocks) / 2 * ((c.head_dim + 127) / 128) / 4 + spl_paged_items_max(c, blocks); }
 // Slots that a plan of `blocks` stretches takes at most: a unit is cut only where a block ends, and each such cut makes two pieces of one.
 inline int spl_paged_slots_max(int blocks) { return 2 * blocks; }

@@ -28,11 +28,11 @@ def test_types_and_head_shapes(engine, dtype, heads, kv_heads, head_dim, out_dty
     check(scene, attend(engine, scene, out), out)
 
 
-@pytest.mark.parametrize("rows", [1, 3, 8, 16])
+@pytest.mark.parametrize("rows", [1, 3, 6, 16])
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("dtype", ["bf16", "e4m3"])
 def test_blocks_of_rows_that_straddle_two_units(engine, rows, causal, dtype):
-    shared = {1: 4096, 3: 4096, 8: 12288, 16: 8192}[rows]
+    shared = {1: 4096, 3: 8192, 6: 20480, 16: 8192}[rows]
     scene = Scene(rows, 12, 2, 128, [rows] * 20, [shared + rows + 11 * i for i in range(20)], page_tokens=128, dtype=dtype, causal=causal, groups=[(20, shared)])
     assert joint(scene)
     check(scene, attend(engine, scene, "f32"), "f32")
@@ -50,7 +50,7 @@ def test_several_groups_prompts_among_them_and_sequences_of_their_own(engine, dt
     check(scene, attend(engine, scene, "f32"), "f32")
 
 
-@pytest.mark.parametrize("rows,heads,kv_heads,shared", [(1, 8, 2, 8192), (1, 12, 2, 8192), (2, 8, 8, 4096), (4, 24, 4, 4096), (6, 24, 4, 16384), (7, 12, 2, 16384), (8, 32, 4, 8192)])
+@pytest.mark.parametrize("rows,heads,kv_heads,shared", [(1, 8, 2, 8192), (1, 12, 2, 8192), (2, 8, 8, 4096), (4, 24, 4, 8192), (6, 24, 4, 20480), (5, 8, 2, 20480), (8, 32, 4, 8192)])
 @pytest.mark.parametrize("head_dim", [128, 256])
 def test_both_forms_over_a_cache_of_e4m3(engine, rows, heads, kv_heads, shared, head_dim):
     """Four to 64 packed rows a sequence, two to nine sequences: joint rows of 16, 32, 48 and 128 a block, full and not."""
@@ -87,19 +87,19 @@ def test_runs_are_equal_to_the_bit(engine):
             assert torch.equal(first, attend(engine, scene, stream=stream)) and torch.equal(first, attend(engine, scene, stream=stream, paged=paged))
 
 
-@pytest.mark.parametrize("dtype", ["bf16", "e4m3"])
-def test_graphs_captured_with_groups_and_without_follow_any_batch(engine, dtype):
+@pytest.mark.parametrize("dtype,each,long,longer", [("bf16", 1, 2048, 2944), ("e4m3", 1, 2048, 2944), ("e4m3", 8, 6144, 8192), ("e4m3", 30, 6528, 8192)])
+def test_graphs_captured_with_groups_and_without_follow_any_batch(engine, dtype, each, long, longer):
     """One object, a graph captured before any group, one captured with a prefix met together: both replayed behind batches of either kind."""
-    rows, pages = [1] * 12, 200
+    rows, pages = [each] * 12, 290
     def make(i, shared, groups):
-        own = [shared + 1 + (31 * (n + i)) % 300 for n in range(12)]
+        own = [shared + each + (31 * (n + i)) % 300 for n in range(12)]
         held = sum(-(-n // 64) for n in own) - (shared // 64 * 11 if groups else 0)
         return Scene(40 + i, 12, 4, 128, rows, own, page_tokens=64, dtype=dtype, groups=[(12, shared)] if groups else [], spare_pages=pages - held)
-    scenes = [make(0, 256, False), make(1, 2048, True), make(2, 256, False), make(3, 2944, True), make(4, 64, True)]
+    scenes = [make(0, 256, False), make(1, long, True), make(2, 256, False), make(3, longer, True), make(4, 64, True)]
     assert [joint(s) for s in scenes] == [False, True, False, True, False]
-    paged = scenes[0].paged(engine, S.PagedAttention, max_context=4096)
+    paged = scenes[0].paged(engine, S.PagedAttention, max_context=longer + 512)
     q, k, v, ks, vs = (torch.empty_like(x) for x in (scenes[0].dq, scenes[0].k, scenes[0].v, scenes[0].ks, scenes[0].vs))
-    out = torch.zeros((2, 12, 12, 128), device="cuda")
+    out = torch.zeros((2, 12 * each, 12, 128), device="cuda")
     scales = {"k_scale": ks.data_ptr(), "v_scale": vs.data_ptr()} if dtype == "e4m3" else {}
     stream = torch.cuda.Stream()
     graphs = []

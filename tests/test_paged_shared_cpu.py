@@ -46,14 +46,15 @@ def random_batch(rng):
     return group * kv_heads, kv_heads, rows, lengths, groups, int(rng.choice([0, 0, 0, 200])), bool(rng.random() < 0.7)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "e4m3"])
 @pytest.mark.parametrize("seed", range(80))
-def test_every_row_meets_every_tile_once_and_is_joined_from_all_its_pieces(seed):
+def test_every_row_meets_every_tile_once_and_is_joined_from_all_its_pieces(seed, dtype):
     rng = np.random.default_rng(seed)
     heads, kv_heads, rows, lengths, groups, window, causal = random_batch(rng)
     if not any(rows):
         rows[0] = 1; lengths[0] += 1
     blocks, group = int(rng.choice([1, 3, 148])), heads // kv_heads
-    config = dict(heads=heads, kv_heads=kv_heads, head_dim=128, pages=1, page_tokens=256, window=window, causal=causal, max_sequences=len(rows), max_rows=max(sum(rows), 1), max_context=1 << 20)
+    config = dict(heads=heads, kv_heads=kv_heads, head_dim=128, dtype=dtype, pages=1, page_tokens=256, window=window, causal=causal, max_sequences=len(rows), max_rows=max(sum(rows), 1), max_context=1 << 20)
     begin, items, records, partial_rows, joint = debug_paged_plan_shared(rows, lengths, groups, blocks=blocks, **config)
     assert begin[0] == 0 and begin[-1] == len(items) and (np.diff(begin) >= 0).all()
     starts = np.concatenate([[0], np.cumsum(rows)])
@@ -92,7 +93,9 @@ def test_every_row_meets_every_tile_once_and_is_joined_from_all_its_pieces(seed)
     assert not joined
     if window or not any(n > 1 and t >= 128 for n, t in groups):
         assert not joint
-    if not joint:
+    if not joint and dtype == "e4m3" and 16 < max(rows) * group <= 128:
+        assert partial_rows <= 2 * blocks * min(128, sum(rows) * group)       # what is set aside for batches without groups
+    elif not joint:
         plain = debug_paged_plan(rows, lengths, blocks=blocks, **config)[1]
         assert (plain[:, :7] == items[:, :7]).all()
 
@@ -110,15 +113,15 @@ def test_a_prefix_is_read_once_for_128_packed_rows():
 
 
 def test_over_a_cache_of_e4m3_few_rows_meet_a_prefix_48_at_a_time():
-    """Two verify blocks of four rows, six heads a kv head, over 16,384 shared tokens: their 48 packed rows are one block's. With a sequence of seven rows (42 packed) beside them the batch's form has 128."""
+    """Two verify blocks of four rows, six heads a kv head, over 20,480 shared tokens: their 48 packed rows are one block's. With a sequence of nine rows (54 packed) beside them the batch's form has 128."""
     config = dict(heads=24, kv_heads=4, head_dim=256, dtype="e4m3", pages=1, max_sequences=16, max_rows=128, max_context=1 << 16)
-    for rows, width in (([4] * 6, 48), ([4] * 6 + [7], 128), ([1] * 16, 48)):
-        begin, items, records, _, joint = debug_paged_plan_shared(rows, [16384 + 300] * len(rows), [(len(rows), 16384)], **config)
+    for rows, width in (([4] * 6, 48), ([4] * 6 + [9], 128), ([1] * 16, 48)):
+        begin, items, records, _, joint = debug_paged_plan_shared(rows, [20480 + 300] * len(rows), [(len(rows), 20480)], **config)
         assert joint
         packed = 6 * sum(rows)
-        over = [(int(i[3]), int(i[4])) for i in items if i[6] <= 128]
+        over = [(int(i[3]), int(i[4])) for i in items if i[6] <= 160]
         assert set(over) <= {(q, min(width, packed - q)) for q in range(0, packed, width)}
-        assert sum(int(i[6] - i[5]) for i in items if i[6] <= 128) == 4 * 128 * -(-packed // width)
+        assert sum(int(i[6] - i[5]) for i in items if i[6] <= 160) == 4 * 160 * -(-packed // width)
         joined = np.zeros((sum(rows) * 6, 4), int)
         for row0, q0, h, count, *_ in records.tolist():
             joined[6 * row0 + q0:6 * row0 + q0 + count, h] += 1
