@@ -480,7 +480,7 @@ spl_status spl_paged_attend_scaled(spl_paged *paged, const void *device_q, const
                                    void *device_out, void *stream);
 /* spl_paged_batch for sequences that begin with the same tokens (a system prompt, continuations of one prompt): group g is the batch's next group_sequences[g] sequences, whose first group_tokens[g] tokens
  * lie in the same pages (whole pages, in front of every member's new rows, the same entries of the page table; SPL_ERR_INVALID_ROWS otherwise). Sequences behind the last group share nothing. attend then reads
- * the whole tiles of 128 tokens of a shared prefix once for up to 128 packed rows (a row's heads that share a kv head) of its group instead of once a sequence, where that saves more than the joining costs: without a window, for sequences of at most 128
+ * the whole tiles of 128 tokens of a shared prefix once for up to 128 packed rows (a row's heads that share a kv head; 48 over a cache of SPL_E4M3 with heads of 128 or 256 and at most 48 a sequence) of its group instead of once a sequence, where that saves more than the joining costs: without a window, for sequences of at most 128
  * packed rows. The results are the same to the rounding of fp32 sums. The first call sets device memory aside for it (two partial sums a packed row); a graph captured before or after may be replayed after batches with
  * groups and without. */
 spl_status spl_paged_batch_shared(spl_paged *paged, int32_t sequences, const int32_t *rows, const int32_t *lengths, const int32_t *page_table, int32_t table_ld, int32_t groups, const int32_t *group_sequences,

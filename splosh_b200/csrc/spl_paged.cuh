@@ -764,8 +764,8 @@ spl_paged_attend_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
     if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512) : "memory");
 }
 
-// ---- the pieces of a shared batch joined ----------------------------------------------------------
-// o = sum_n 2^(m_n - m) O_n / sum_n 2^(m_n - m) l_n over the pieces of a row: those of the prefix that its sequences met together, and those of its own tokens. A piece of the prefix
+// ---- the pieces of a batch joined by rows -----------------------------------------------------------
+// o = sum_n 2^(m_n - m) O_n / sum_n 2^(m_n - m) l_n over the pieces of a row: those of the prefix that its sequences met together, where some did, and those of its own tokens. A piece of the prefix
 // holds rows of many sequences, so no block of the attention is the last of all that a row waits for; here the rows are dealt to warps, whoever's they are.
 // A warp a row and 128 channels (64 of a head of 64): lane n looks up piece n's sums for all. Bound: L2, what the attention just left there.
 struct SplPagedCombine {
@@ -795,7 +795,7 @@ spl_paged_combine_kernel(SplPagedCombine a, SplPagedShape s) {
             const int at = (n < rec.a_pieces ? rec.a_first + n * rec.a_step : rec.b_first + (n - rec.a_pieces) * rec.b_step) + r;
             const float2 ml = n < pieces ? __ldcg(a.partial_ml + at) : make_float2(-INFINITY, 0.0f);
             const float now = fmaxf(m, spl_warp_max(ml.x));
-            if (now == -INFINITY) continue;
+            if (now == -INFINITY) { sum += ml.y; continue; }                // (pieces of no tokens that this row sees: zeros, or scores that are no numbers)
             const float f = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - now), old = exp2f(m - now);      // (a piece of whose tokens this row sees none)
             sum = sum * old + f * ml.y;
 #pragma unroll

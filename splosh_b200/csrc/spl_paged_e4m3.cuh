@@ -5,8 +5,8 @@
 //   S = Q K^T      in 8 bits, K as it lies in the cache. A bf16 query is the sum of two e4m3 (four significant bits each) once its row is scaled by the power of two that puts its largest
 //                  channel in [128, 256): both are rows of the A operand's tile, and a tile's scores are 2 HD / 32 instructions of 32 channels, as long as a 16-bit product's HD / 16. What is lost is
 //                  below 2^-17 of the row's largest channel.
-//   O += P V       in fp16, which holds every code exactly. Four warps turn the values of a chunk into fp16 on their way to the products (V as 8-bit operand would want P in 8 bits, too: a weight below
-//                  2^-17 of the row's largest would be lost, and many tokens of small weight are not a small matter).
+//   O += P V       in fp16, which holds every code exactly. Two pairs of warps turn the values of a chunk into fp16 on their way to the products, each every second chunk (V as 8-bit operand would want P in 8 bits, too: a
+//                  weight below 2^-17 of the row's largest would be lost, and many tokens of small weight are not a small matter).
 // The value scales go into the exponent: y_t = log2 of p_t vs_t = x_t + log2 vs_t has the running reference, so that P = 2^(y - ref) uses fp16's range for what counts in the row's sum, whatever the
 // sizes of values that do not (a running maximum of x alone would leave tokens of small values in the subnormals beside one of large ones); the denominator adds P / vs. The warp that copies keys writes each
 // token's ks, log2 vs and 1 / vs beside them.
@@ -22,6 +22,7 @@ __host__ __device__ constexpr int spl_paged8_ring_k(int hd) { return hd == 64 ? 
 // Chunks of values, as they lie and in fp16: even numbers, for two pairs of warps take turns at them and a pair has to meet every phase of its places' barriers.
 __host__ __device__ constexpr int spl_paged8_ring_v(int hd) { return hd == 64 ? 6 : 2; }
 __host__ __device__ constexpr int spl_paged8_ring_w(int hd) { return hd == 64 ? 4 : 2; }
+static_assert(spl_paged8_ring_v(64) % 2 == 0 && spl_paged8_ring_v(128) % 2 == 0 && spl_paged8_ring_v(256) % 2 == 0 && spl_paged8_ring_w(64) % 2 == 0 && spl_paged8_ring_w(128) % 2 == 0 && spl_paged8_ring_w(256) % 2 == 0, "");
 // Tiles of scales. Those of tile j are written behind its first keys, which waited for the scores of the tile a ring before, and these for the softmax of the tile two before that.
 __host__ __device__ constexpr int spl_paged8_scales(int hd) { return (spl_paged8_ring_k(hd) + (hd == 256 ? 1 : 0)) / (hd == 256 ? 2 : 1) + 2; }
 __host__ __device__ constexpr size_t spl_paged8_smem_bytes(int hd) {

@@ -152,3 +152,17 @@ def test_a_group_that_is_refused_leaves_the_batch(engine):
     paged.attend(scene.dq.data_ptr(), scene.k.data_ptr(), scene.v.data_ptr(), out.data_ptr(), out_dtype="f32")
     engine.pass_wait()
     assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "e4m3"])
+@pytest.mark.parametrize("each,shared", [(1, 8192), (8, 12288), (30, 8192)])
+def test_a_key_that_is_no_number_in_a_prefix_reaches_who_sees_it(engine, dtype, each, shared):
+    """Keys of the first kv head of one token, and of all tokens: the rows' heads on it are NaN, those on the second are not."""
+    scene = Scene(9, 6, 2, 128, [each] * 12, [shared + each + 19 * i for i in range(12)], page_tokens=64, dtype=dtype, groups=[(12, shared)])
+    assert joint(scene)
+    k = scene.k.view(torch.uint8) if dtype == "e4m3" else scene.k
+    for pages in (scene.table[0, 3:4], scene.table[:, :]):
+        pages = torch.from_numpy(np.unique(pages[pages >= 0])).cuda().long()
+        k[pages, 0, 5 if len(pages) == 1 else slice(None), 7] = 0x7f if dtype == "e4m3" else float("nan")
+        out = attend(engine, scene, "f32")
+        assert torch.isnan(out[:, :3]).all() and torch.isfinite(out[:, 3:]).all()
