@@ -136,7 +136,7 @@ static spl_status paged_create(spl_engine *e, const spl_paged_config *cp, spl_pa
     if (found != cudaDriverEntryPointSuccess || !encode) return e->fail(SPL_ERR_UNSUPPORTED_DEVICE, "spl_paged_create: the driver has no tensor maps");
     p->encode = reinterpret_cast<SplEncodeTiled>(encode);
     if (!paged_configure(c.head_dim, c.dtype == SPL_E4M3)) return e->fail(SPL_ERR_UNSUPPORTED_DEVICE, "spl_paged_create: the kernel's shared-memory opt-in failed");
-    if (c.dtype == SPL_E4M3 && int64_t(c.max_rows) * p->shape.group > 16) {
+    if (spl_paged_split(c, std::min<int64_t>(int64_t(c.max_rows) * p->shape.group, SPL_PAGED_TILE))) {      // (some batch is joined so)
         const spl_status made = paged_by_rows_create(p, p->split, int64_t(items), int64_t(items), spl_paged_split_combine_max(c, e->sms), spl_paged_split_rows_max(c, e->sms));
         if (made != SPL_OK) return made;
     }

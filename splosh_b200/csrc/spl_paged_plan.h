@@ -146,11 +146,12 @@ inline int64_t spl_paged_take(int64_t t, int64_t left, int64_t stretch, int q_co
 // Over a cache of e4m3 a batch takes the transposed form by the most packed rows that a sequence has, also where sequences meet a prefix together (48 rows a block then), so a graph that holds one form is right for
 // every batch of its rows.
 inline bool spl_paged_narrow(const spl_paged_config &c, int64_t packed) { return c.dtype == SPL_E4M3 && c.head_dim >= 128 && packed <= SPL_PAGED8_NARROW; }
-// And over such a cache the pieces of a batch whose sequences have more than 16 packed rows, but at most a block's, are joined by the kernel of its own, groups or not. In and behind the attention: heads of 256
-// (24 on 4), one verify block of eight rows over 1,000, 4,000 and 32,000 tokens 22.2 and 15.7, 39.2 and 17.0, 82.7 and 31.2 us, one of sixteen over 4,000 66.9 and 22.1, eight of eight over 39,000 135.7 and 123.6;
-// heads of 64 (16 on 2), eight of sixteen over 3,600 45.8 and 18.9; 32 sequences, of which few are cut, the same. Prompts: 300 rows over 300 tokens 19.7 and 22.8, 2,048 over 8,192 1,358 and 1,396. (With
-// up to 16 rows a piece's join is short: the launch would cost more.)
-inline bool spl_paged_split(const spl_paged_config &c, int64_t packed) { return c.dtype == SPL_E4M3 && packed > 16 && packed <= SPL_PAGED_TILE; }
+// And over such a cache the pieces of a batch whose sequences have more than 8 packed rows, but at most a block's, are joined by the kernel of its own, groups or not. In and behind the attention: heads of 256
+// (24 on 4), two rows over 4,000 tokens 27.7 and 16.5 us, eight of two over 7,200 35.8 and 31.5, one verify block of eight rows over 1,000, 4,000 and 32,000 22.2 and 15.7, 39.2 and 17.0, 82.7 and 31.2, one of sixteen
+// over 4,000 66.9 and 22.1, eight of eight over 39,000 135.7 and 123.6; heads of 64 (16 on 2), eight of sixteen over 3,600 45.8 and 18.9; 32 sequences, of which few are cut, the same. With fewer rows a piece's join
+// is short and the launch counts: one row over 1,000 tokens 10.0 and 11.5, over 4,000 14.4 and 14.5, twelve over 900 12.8 and 13.2, 32 over 2,700 41.6 and 42.5. Prompts: 300 rows over 300 tokens 19.7 and 22.8,
+// 2,048 over 8,192 1,358 and 1,396.
+inline bool spl_paged_split(const spl_paged_config &c, int64_t packed) { return c.dtype == SPL_E4M3 && packed > 8 && packed <= SPL_PAGED_TILE; }
 // Meeting together pays where the tiles saved are more than the joining: so many a block for one more launch and the pieces' first keys, and one for so many rows of heads that leave and join sums. Measured with
 // heads of 256, 24 of them on 4, together and apart:
 //   in 16 bits    six sequences of one row over 1,024 shared tokens 15.2 and 13.7 us, over 4,096 17.7 and 21.8; sixteen of four rows over 512 21.5 and 19.7, over 1,024 22.0 and 23.0;
