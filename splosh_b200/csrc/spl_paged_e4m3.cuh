@@ -1011,7 +1011,7 @@ spl_paged_attend_e4m3_narrow_kernel(const __grid_constant__ CUtensorMap k_map, c
             if (it.slot >= 0 && quarter == 0 && lane < H && n0 + lane < it.q_count) a.partial_ml[slot_row + lane] = make_float2(ref, all);
             spl_tc_fence_before();
             spl_paged8_barrier(group);                                               // the sums in shared memory are read before the next piece's
-            if (it.merge >= 0) {
+            if (N == 16 && it.merge >= 0) {                // (more rows are joined by rows)
                 // Whichever block is the last to leave a piece of these rows joins them, in the order of the pieces whoever it is.
                 __threadfence();
                 spl_named_barrier<6, 32 * SOFTMAX>();

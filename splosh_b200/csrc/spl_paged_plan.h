@@ -144,7 +144,9 @@ inline int64_t spl_paged_take(int64_t t, int64_t left, int64_t stretch, int q_co
 // together: their rows lie one behind the other, so they are the rows of one sequence over the prefix, in blocks of 128 packed rows whoever's they are; each sequence's own
 // tokens are units of their own, and both leave partial sums (O, m, l) that spl_paged_combine_kernel joins. (Sequences of more packed rows read the prefix once for 128 of them as it is.)
 // Over a cache of e4m3 a batch takes the transposed form by the most packed rows that a sequence has, also where sequences meet a prefix together (48 rows a block then), so a graph that holds one form is right for
-// every batch of its rows.
+// every batch of its rows. Transposed and wide, before pieces were joined by rows: heads of 256 (24 on 4), eight sequences of about 6,000 tokens with 6, 12, 24, 36 and 48 packed rows 27.7 and 51.4, 31.2 and 54.7, 40.4 and
+// 56.1, 48.3 and 65.0, 51.2 and 67.9 us; of 128 (32 on 8), with 8, 16, 32 and 48 21.5 and 35.0, 23.9 and 38.7, 30.6 and 37.0, 37.6 and 47.7. (For 64 rows the sums of three parts
+// and two blocks of channels, 384 columns of tensor memory, and two tiles' scores, 256, are more than its 512.)
 inline bool spl_paged_narrow(const spl_paged_config &c, int64_t packed) { return c.dtype == SPL_E4M3 && c.head_dim >= 128 && packed <= SPL_PAGED8_NARROW; }
 // And over such a cache the pieces of a batch whose sequences have more than 8 packed rows, but at most a block's, are joined by the kernel of its own, groups or not. In and behind the attention: heads of 256
 // (24 on 4), two rows over 4,000 tokens 27.7 and 16.5 us, eight of two over 7,200 35.8 and 31.5, one verify block of eight rows over 1,000, 4,000 and 32,000 22.2 and 15.7, 39.2 and 17.0, 82.7 and 31.2, one of sixteen
