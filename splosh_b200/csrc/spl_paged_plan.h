@@ -276,7 +276,7 @@ inline void spl_paged_plan(const spl_paged_config &c, int blocks, int32_t sequen
 inline int64_t spl_paged_joint_rows_max(const spl_paged_config &c) { return std::min(int64_t(c.max_rows) * c.heads, int64_t(c.max_sequences) * SPL_PAGED_TILE * c.kv_heads); }
 inline int64_t spl_paged_shared_items_max(const spl_paged_config &c, int blocks) { return 2 * spl_paged_items_max(c, blocks); }
 inline int64_t spl_paged_records_max(const spl_paged_config &c, int blocks) { return 2 * spl_paged_items_max(c, blocks); }
-inline int64_t spl_paged_partial_rows_max(const spl_paged_config &c, int blocks) { return 2 * spl_paged_joint_rows_max(c) + int64_t(blocks) * 2 * SPL_PAGED_TILE; }
+inline int64_t spl_paged_partial_rows_max(const spl_paged_config &c, int blocks) { return 2 * spl_paged_joint_rows_max(c) + int64_t(blocks) * 2 * std::min<int64_t>(SPL_PAGED_TILE, int64_t(c.max_rows) * (c.heads / c.kv_heads)); }
 inline int64_t spl_paged_combine_max(const spl_paged_config &c, int blocks) {      // of blocks of the joining kernel's work, four (row, channels) each
     return (spl_paged_joint_rows_max(c) + int64_t(blocks) * SPL_PAGED_TILE) * ((c.head_dim + 127) / 128) / 4 + spl_paged_records_max(c, blocks);
 }
