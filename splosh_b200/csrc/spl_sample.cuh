@@ -708,6 +708,7 @@ spl_sample_kernel(SplSampleArgs a) {
                 if (c0 > 0) {
                     const unsigned long long low = sh.sums[c0 - 1], high = sh.sums[c1];
                     // A token in front of these bins whose test does not depend on where in them it ends: it stays, and nothing else is asked.
+                    __syncthreads();                   // (all have read the place of top-p's end)
                     if (ve.count && tid == 0) {
                         const unsigned long long entry = ve.entry[ve.count - 1];
                         sh.found = entry && entry >= cut && ve.bin[ve.count - 1] < c0 && double(ve.u0) * double(ve.q[ve.count - 1]) * double(high) < double(spl_sample_weight(spl_topk_value(uint32_t(entry >> 32)), r.w));
