@@ -284,6 +284,7 @@ struct SplPagedAttend {
 
 // The pieces of a tile of query rows joined by 256 threads: o = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s. First m and 1 / sum of every row, to shared memory (`scratch`,
 // 256 floats); then the sums, four channels a thread, as many on their way as there are registers for: UP groups of 1024 channels times UN pieces.
+// A piece whose reference is -inf has none of a row's tokens, or only such whose scores are no numbers (a maximum passes over those): its O is left out, its sum, 0 or NaN, is not.
 template <int HD, bool BF16, int UP, int UN>
 __device__ __forceinline__ void spl_paged_join_sums(const SplPagedShape &s, const SplPagedAttend &a, const SplPagedItem &it, int row0, int head0, uint32_t per_group, const float *scratch) {
     const int fours = it.q_count * (HD / 4);
@@ -308,7 +309,7 @@ __device__ __forceinline__ void spl_paged_join_sums(const SplPagedShape &s, cons
 #pragma unroll
                 for (int n = 0; n < UN; ++n) {
                     const int r = min(base + u * 256, fours - 1) / (HD / 4);
-                    if (n0 + n >= it.pieces || ref[u][n] == -INFINITY) continue;      // (a piece of whose tokens this row sees none)
+                    if (n0 + n >= it.pieces || ref[u][n] == -INFINITY) continue;      // (its sum decides)
                     const float f = exp2f(ref[u][n] - scratch[r]);
                     acc[u].x += f * v[u][n].x; acc[u].y += f * v[u][n].y; acc[u].z += f * v[u][n].z; acc[u].w += f * v[u][n].w;
                 }
@@ -349,14 +350,19 @@ __device__ __forceinline__ void spl_paged_join(const SplPagedShape &s, const Spl
             float now = m;
 #pragma unroll
             for (int n = 0; n < 8; ++n) if (n0 + n < it.pieces) now = fmaxf(now, ml[n].x);
-            if (now == -INFINITY) continue;
+            if (now == -INFINITY) {
+#pragma unroll
+                for (int n = 0; n < 8; ++n) if (n0 + n < it.pieces) sum += ml[n].y;
+                continue;
+            }
             const float old = exp2f(m - now);
             sum *= old;
 #pragma unroll
             for (int j = 0; j < HD / 64; ++j) { acc[j].x *= old; acc[j].y *= old; }
 #pragma unroll
             for (int n = 0; n < 8; ++n) {
-                if (n0 + n >= it.pieces || ml[n].x == -INFINITY) continue;      // (a piece of whose tokens this row sees none)
+                if (n0 + n >= it.pieces) continue;
+                if (ml[n].x == -INFINITY) { sum += ml[n].y; continue; }
                 const float f = exp2f(ml[n].x - now);
                 sum += f * ml[n].y;
 #pragma unroll
@@ -382,14 +388,14 @@ __device__ __forceinline__ void spl_paged_join(const SplPagedShape &s, const Spl
             const float m = fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x));
             float sum = 0.0f;
 #pragma unroll
-            for (int n = 0; n < 4; ++n) if (ml[n].x > -INFINITY) sum += exp2f(ml[n].x - m) * ml[n].y;
+            for (int n = 0; n < 4; ++n) sum += ml[n].x > -INFINITY ? exp2f(ml[n].x - m) * ml[n].y : ml[n].y;
             scratch[r] = m; scratch[128 + r] = 1.0f / sum;
         }
     } else for (int r = warp; r < it.q_count; r += 8) {       // a warp a row
         float m = -INFINITY, sum = 0.0f;
         for (int n = lane; n < it.pieces; n += 32) m = fmaxf(m, at(n, r).x);
         m = spl_warp_max(m);
-        for (int n = lane; n < it.pieces; n += 32) { const float2 ml = at(n, r); if (ml.x > -INFINITY) sum += exp2f(ml.x - m) * ml.y; }
+        for (int n = lane; n < it.pieces; n += 32) { const float2 ml = at(n, r); sum += ml.x > -INFINITY ? exp2f(ml.x - m) * ml.y : ml.y; }
         sum = spl_warp_sum(sum);
         if (lane == 0) { scratch[r] = m; scratch[128 + r] = 1.0f / sum; }
     }

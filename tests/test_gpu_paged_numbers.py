@@ -1,0 +1,61 @@
+"""Attention over a paged cache where numbers end: what is no number in tokens whose pieces are joined. Wherever a sequence is cut, a row answers as in one piece."""
+import pytest
+import torch
+
+from more_reference import Scene
+from splosh_b200.paged import debug_paged_plan
+from test_gpu_paged_e4m3 import attend, engine      # noqa: F401  (the fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+def spoil(scene, sequence, tokens, which, kv_head=0, channel=5):
+    """NaN in keys or values (one channel of a code or number) or scales of these tokens of a sequence."""
+    for token in tokens:
+        at = (int(scene.table[sequence, token // scene.page_tokens]), kv_head, token % scene.page_tokens)
+        if which in ("ks", "vs"):
+            getattr(scene, which)[at] = float("nan")
+        elif scene.dtype == "e4m3":
+            getattr(scene, which).view(torch.uint8)[at + (channel,)] = 0x7f
+        else:
+            getattr(scene, which)[at + (channel,)] = float("nan")
+
+
+def last_pieces(scene):
+    """The first token of each (kv head, tile of rows)'s last piece of the first sequence, and how many it is cut into."""
+    items = debug_paged_plan(scene.rows, scene.lengths, heads=scene.heads, kv_heads=scene.kv_heads, head_dim=scene.head_dim, pages=1, page_tokens=256, dtype=scene.dtype, max_sequences=len(scene.rows),
+                             max_rows=scene.total, max_context=1 << 20)[1]
+    items = items[items[:, 0] == 0]
+    count = {}
+    for it in items:
+        key = tuple(it[2:4])
+        count[key] = (max(count.get(key, (0, 0))[0], int(it[5])), count.get(key, (0, 0))[1] + 1)
+    return count
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "e4m3"])
+@pytest.mark.parametrize("heads,kv_heads,head_dim,rows,length", [
+    (4, 1, 128, 1, 129), (4, 1, 128, 1, 257), (8, 2, 128, 1, 385), (24, 4, 256, 1, 1025), (2, 1, 64, 1, 129), (8, 1, 256, 1, 2177),        # up to eight packed rows: the newest token alone in the last piece
+    (8, 2, 64, 2, 9001), (2, 1, 128, 4, 20000),
+    (12, 2, 256, 3, 1300), (16, 1, 128, 4, 1300), (16, 1, 64, 1, 4097), (24, 4, 256, 8, 4000),                                              # nine to 128
+    (6, 1, 256, 30, 8000), (8, 1, 128, 40, 3000), (4, 1, 64, 200, 5000)])                                                                  # more
+def test_a_piece_of_tokens_that_are_no_numbers_is_not_lost(engine, dtype, heads, kv_heads, head_dim, rows, length):
+    """All that a row sees in its last piece is NaN: the row is, and no other sequence or kv head."""
+    scene = Scene(length + rows, heads, kv_heads, head_dim, [rows, 1], [length, 200], page_tokens=64, dtype=dtype)
+    good = attend(engine, scene, "f32")
+    pieces = last_pieces(scene)
+    assert max(n for _, n in pieces.values()) > 1
+    start = min(128 * tile for tile, _ in pieces.values())
+    group = heads // kv_heads
+    keep = {w: getattr(scene, w).view(torch.uint8).clone() for w in ("k", "v")}, scene.ks.clone(), scene.vs.clone()
+    for which in ("k", "v") + (("ks", "vs") if dtype == "e4m3" else ()):
+        for w in ("k", "v"):
+            getattr(scene, w).view(torch.uint8).copy_(keep[0][w])
+        scene.ks.copy_(keep[1]); scene.vs.copy_(keep[2])
+        spoil(scene, 0, range(start, length), which)
+        out = attend(engine, scene, "f32")
+        sees = torch.arange(rows) + length - rows >= start
+        assert sees.any()
+        wrong = out[:rows][sees.cuda()][:, :group]
+        assert (wrong[..., 5] if which == "v" else wrong).isnan().all(), which
+        assert torch.equal(out[:rows, group:], good[:rows, group:]) and torch.equal(out[rows:], good[rows:])
