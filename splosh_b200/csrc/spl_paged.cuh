@@ -802,7 +802,8 @@ spl_paged_combine_kernel(SplPagedCombine a, SplPagedShape s) {
             const float2 ml = n < pieces ? __ldcg(a.partial_ml + at) : make_float2(-INFINITY, 0.0f);
             const float now = fmaxf(m, spl_warp_max(ml.x));
             if (now == -INFINITY) { sum += ml.y; continue; }                // (pieces of no tokens that this row sees: zeros, or scores that are no numbers)
-            const float f = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - now), old = exp2f(m - now);      // (a piece of whose tokens this row sees none)
+            const float f = exp2f(ml.x - now), old = exp2f(m - now);
+            const unsigned int seen = __ballot_sync(0xffffffffu, ml.x != -INFINITY);      // (a piece of whose tokens this row sees none is left out; one whose factor is nothing is not: 0 x NaN is none)
             sum = sum * old + f * ml.y;
 #pragma unroll
             for (int e = 0; e < VEC; ++e) acc[e] *= old;
@@ -819,7 +820,7 @@ spl_paged_combine_kernel(SplPagedCombine a, SplPagedShape s) {
 #pragma unroll
                 for (int u = 0; u < 8; ++u) {
                     const float g = __shfl_sync(0xffffffffu, f, min(u0 + u, here - 1));
-                    if (u0 + u >= here || g == 0.0f) continue;
+                    if (!(seen >> (u0 + u) & 1u)) continue;
 #pragma unroll
                     for (int e = 0; e < VEC; ++e) acc[e] += g * v[u][e];
                 }

@@ -59,3 +59,25 @@ def test_a_piece_of_tokens_that_are_no_numbers_is_not_lost(engine, dtype, heads,
         wrong = out[:rows][sees.cuda()][:, :group]
         assert (wrong[..., 5] if which == "v" else wrong).isnan().all(), which
         assert torch.equal(out[:rows, group:], good[:rows, group:]) and torch.equal(out[rows:], good[rows:])
+
+
+@pytest.mark.parametrize("dtype,heads,kv_heads,head_dim,rows,length,shared", [
+    ("e4m3", 8, 1, 128, 2, 2000, 0), ("e4m3", 24, 4, 256, 8, 8000, 0), ("e4m3", 16, 2, 64, 8, 8000, 0), ("e4m3", 24, 4, 256, 1, 4400, 4096), ("bf16", 24, 4, 256, 1, 4400, 4096), ("fp16", 16, 2, 64, 1, 4400, 4096),
+    ("bf16", 4, 1, 128, 1, 2000, 0), ("bf16", 6, 1, 256, 30, 8000, 0)])
+def test_a_value_that_is_no_number_in_a_piece_of_vanishing_weight(engine, dtype, heads, kv_heads, head_dim, rows, length, shared):
+    """Scores of the first tile in hundreds: the other pieces' factors are 0, and 0 times NaN is none."""
+    n = 12 if shared else 1
+    scene = Scene(rows + length, heads, kv_heads, head_dim, [rows] * n, [length + 3 * i for i in range(n)], page_tokens=64, dtype=dtype, groups=[(n, shared)] if shared else ())
+    pages = scene.table[0, :2].tolist()
+    if dtype == "e4m3":
+        scene.ks[pages] *= 400.0
+    else:
+        scene.k[pages] *= 400.0
+    good = attend(engine, scene, "f32")
+    assert good.isfinite().all()
+    spoil(scene, 0, [length - rows], "v")
+    out = attend(engine, scene, "f32")
+    group = heads // kv_heads
+    assert out[:rows, :group, 5].isnan().all()
+    out[:rows, :group, 5] = good[:rows, :group, 5]
+    assert torch.equal(out, good)
