@@ -416,7 +416,8 @@ spl_status spl_pass_sample(spl_engine *engine, const float *device_logits, int32
  * with candidates 0 the token was its only choice (a continuation found in the text, or a greedy drafter's). Settings are one a row as spl_pass_sample's and make the target's distribution p: the weights of what stays over their sum;
  * uniform [rows][2] in [0, 1).
  *   ids[rows]       -1 where uniform[0] * q(draft) < p(draft), q the draft's probability (0 where it is not a candidate); otherwise the token that takes its place: spl_sample's draw with uniform[1], in its order, from
- *                   max(p - q, 0) over the sum of that, or from p where nothing is left of it. A row without a draft draws from p.
+ *                   max(p - q, 0) over the sum of that, or from p where nothing is left of it. A row without a draft draws from p. (A uniform[1] of 0 takes the first token of which something is left;
+ *                   spl_speculative_resolve takes the first of all there, as SpeculativeSampling.resolve does.)
  *   accepted, next  [sequences] the rows in front of the sequence's first whose id is not -1, and that id (-1: all are)
  * Every row is answered, those behind a refused token, too. What spl_sample says of weights, of NaN and infinities, of ties and of rows that take milliseconds holds here; q is rounded to whole units of 2^-44 of the
  * largest weight, as p is. Queued on `stream`; may be captured. */

@@ -169,6 +169,9 @@ __device__ __forceinline__ unsigned long long spl_sample_target(float fraction, 
     return fraction > 0.0f ? min(sum, (unsigned long long)ceil(double(fraction) * double(sum))) : 0ull;
 }
 
+// The same in what the drafter's candidates leave, which has places of no weight in front: a fraction of zero takes the first that has any.
+__device__ __forceinline__ unsigned long long spl_verify_target(float fraction, unsigned long long left) { return max(1ull, spl_sample_target(fraction, left)); }
+
 // What stays weighs `sum`, and stays(entry) says whether a value does: the test of the drafted token, what its drafter's candidates take off, and what is left (all threads get it).
 template <typename Stays>
 __device__ __forceinline__ unsigned long long spl_verify_resolve(SplVerifyShared &ve, const SplSampleRow &r, unsigned long long sum, Stays &&stays) {
@@ -338,7 +341,7 @@ __device__ __noinline__ void spl_sample_slow(const SplSampleArgs &a, const SplSa
         const unsigned long long last = spl_sample_entry(cut_key, sh.found);
         const unsigned long long sum = total(), rest = spl_verify_resolve(*ve, r, sum, [&](unsigned long long e) { return e >= last && spl_sample_weight(spl_topk_value(uint32_t(e >> 32)), r.w) >= least; });
         if (ve->stays) { if (tid == 0) a.ids[row] = -1; return; }
-        const unsigned long long target = spl_sample_target(r.u, rest);
+        const unsigned long long target = spl_verify_target(r.u, rest);
         find(false, target, &pick_key, &pick_tie, true);
         // What the order leaves in front of the key's values, and the first of these that reaches the target.
         __syncthreads();
@@ -351,7 +354,7 @@ __device__ __noinline__ void spl_sample_slow(const SplSampleArgs &a, const SplSa
                 if (uint32_t(ve->entry[c] >> 32) == pick_key && ve->entry[c] >= entry) run -= ve->off[c];
                 if (ve->entry[c] == entry) own -= ve->off[c];
             }
-            if (target <= before ? n == 1ull : run >= target && run - own < target) a.ids[row] = i;
+            if (run >= target && run - own < target) a.ids[row] = i;
         }, [&](unsigned long long) { return done; });
         return;
     }
@@ -644,7 +647,7 @@ spl_sample_kernel(SplSampleArgs a) {
                     if constexpr (VERIFY) {
                         const unsigned long long last = sh.list[stay - 1], left = spl_verify_resolve(ve, r, sh.sums[stay - 1], [&](unsigned long long e) { return e >= last; });
                         for (int i = tid; i < stay; i += 1024) sh.sums[i] -= spl_verify_off(ve, sh.list[i]);
-                        const int pick = spl_sample_place(sh, stay, spl_sample_target(r.u, left));
+                        const int pick = spl_sample_place(sh, stay, spl_verify_target(r.u, left));
                         if (tid == 0) a.ids[row] = ve.stays ? -1 : int32_t(~uint32_t(sh.list[pick]));
                     } else {
                         const int pick = spl_sample_place(sh, stay, spl_sample_target(r.u, sh.sums[stay - 1]));
@@ -740,7 +743,7 @@ spl_sample_kernel(SplSampleArgs a) {
                     left = spl_verify_resolve(ve, r, all, [&](unsigned long long e) { return e >= cut && bin_of(spl_topk_value(uint32_t(e >> 32))) < SPL_SAMPLE_BINS - 1; });
                     spl_verify_left(sh, ve, keep);
                 }
-                const unsigned long long target = spl_sample_target(r.u, left);
+                const unsigned long long target = VERIFY ? spl_verify_target(r.u, left) : spl_sample_target(r.u, left);
                 const int b = spl_sample_place(sh, SPL_SAMPLE_BINS, target);
                 all = left;
                 if (VERIFY && ve.stays) { if (tid == 0) a.ids[row] = -1; decide(SPL_SAMPLE_DONE, 0, 0, 0ull); }
@@ -750,7 +753,7 @@ spl_sample_kernel(SplSampleArgs a) {
         cluster.sync();
         step = sh.step;
         const unsigned long long *kept = reinterpret_cast<const unsigned long long *>(sh.lo);
-        unsigned long long target = rank == 0 && step == SPL_SAMPLE_DRAW ? spl_sample_target(r.u, all) : 0ull;
+        unsigned long long target = rank == 0 && step == SPL_SAMPLE_DRAW ? VERIFY ? spl_verify_target(r.u, all) : spl_sample_target(r.u, all) : 0ull;
         while (step == SPL_SAMPLE_END) {                                               // (twice at most)
             set_aside(sh.first_bin, sh.last_bin, sh.also_first, sh.also_last);
             if (rank == 0) {
@@ -797,14 +800,14 @@ spl_sample_kernel(SplSampleArgs a) {
                         first -= c0 ? spl_verify_off_bins(ve, c0 - 1) : 0ull;
                         for (int i = tid; i < stay; i += 1024) sh.sums[i] -= spl_verify_off(ve, sh.list[i]);
                     }
-                    target = spl_sample_target(r.u, left);
+                    target = VERIFY ? spl_verify_target(r.u, left) : spl_sample_target(r.u, left);
                     int from = -1, to = stay;
                     unsigned long long shift = 0ull;
                     unsigned long long also_from = also_base, also_to = also_base + also_sum;
                     if constexpr (VERIFY) { if (also >= 0) { also_from -= also ? spl_verify_off_bins(ve, also - 1) : 0ull; also_to -= spl_verify_off_bins(ve, also_last); } }
                     if (target > first || base == 0ull) from = front;
                     else if (also >= 0 && target > also_from && target <= also_to) { from = 0; to = front; shift = base - also_sum - also_base; }
-                    else if (also == 0) { from = 0; to = front; shift = base - also_sum; }      // a target of nothing: the first value
+                    else if (!VERIFY && also == 0) { from = 0; to = front; shift = base - also_sum; }      // a target of nothing: the first value
                     if (VERIFY && ve.stays) { if (tid == 0) a.ids[row] = -1; decide(SPL_SAMPLE_DONE, 0, 0, 0ull); }
                     else if (from >= 0) {
                         __syncthreads();
