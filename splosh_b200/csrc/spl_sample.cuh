@@ -546,8 +546,8 @@ spl_sample_kernel(SplSampleArgs a) {
     const bool nothing = (top >> 32) == 0ull;          // id 0, as an untouched slot of a top-k
     if (nothing || !(r.t > 0.0f)) {
         if constexpr (VERIFY) {
-            // All the weight is the largest value's.
-            if (rank == 0 && tid == 0) a.ids[row] = nothing ? 0 : ve.count && ve.entry[ve.count - 1] == top && ve.u0 * ve.q[ve.count - 1] < 1.0f ? -1 : int32_t(~uint32_t(top));
+            // All the weight is the largest value's. (The product in 64 bits, where it is exact: a probability a step above one times a number a step below one is below one.)
+            if (rank == 0 && tid == 0) a.ids[row] = nothing ? 0 : ve.count && ve.entry[ve.count - 1] == top && double(ve.u0) * double(ve.q[ve.count - 1]) < 1.0 ? -1 : int32_t(~uint32_t(top));
             return;
         }
         if (rank == 0 && tid == 0) a.ids[row] = nothing ? 0 : int32_t(~uint32_t(top));

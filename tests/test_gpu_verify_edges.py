@@ -1,4 +1,4 @@
-"""The test of drafted tokens where its definition or its threads can go apart: what the threads of a block decide by, and uniform numbers at their ends."""
+"""The test of drafted tokens where its definition or its threads can go apart: what the threads of a block decide by, and uniform numbers and probabilities at their ends."""
 import numpy as np
 import pytest
 
@@ -48,3 +48,15 @@ def test_a_second_number_of_zero_takes_the_first_token_with_something_left(engin
         for u in (tiny, zero):
             got, _, _ = device(engine, x, width, [rows], drafts, candidates, settings, u)
             assert np.array_equal(got, want), (got.tolist(), want.tolist())
+
+
+def test_the_largest_value_alone_beside_probabilities_above_one(engine):
+    """Temperature 0: a token stays while its number times its drafter's probability is below one, in exact arithmetic. (A drafter's rounded probabilities may pass one by a step.)"""
+    x = np.zeros((4, 50), np.float32)
+    x[:, 17] = 1.0
+    drafts = np.full(4, 17)
+    step = np.float32(2.0 ** -23)
+    p = np.array([[1 + step], [1 + step], [1.0], [1 + 2 * step]], np.float32)
+    u = np.array([[1 - step, 0.5], [BELOW, 0.5], [BELOW, 0.5], [1 - 2 * step, 0.5]], np.float32)      # 1 - 2^-46, above 1, below 1, 1 - 2^-44
+    got, accepted, following = device(engine, x, 50, [1, 1, 1, 1], drafts, (np.full((4, 1), 17), p), (0.0, None, None, None), u)
+    assert got.tolist() == [-1, 17, -1, -1] and accepted.tolist() == [1, 0, 1, 1] and following.tolist() == [-1, 17, -1, -1]
