@@ -473,7 +473,7 @@ spl_status spl_paged_append(spl_paged *paged, int32_t type, const void *device_q
 spl_status spl_paged_attend(spl_paged *paged, const void *device_q, const void *device_k_cache, const void *device_v_cache, int32_t out_type, void *device_out, void *stream);
 /* A cache of SPL_E4M3: a token's keys of one kv head are head_dim codes times one scale, its values likewise, at half the memory and traffic of 16 bits. The scales are the caller's, fp32 [pages][kv_heads][page_tokens]
  * for keys and for values, on 16-byte boundaries. append takes scale = max |y| / 448 over the head's channels (at least 2^-100) and code = y * (1 / scale), in fp32, to nearest even, y what spl_paged_append
- * would round to 16 bits; a head that holds an infinity or NaN is NaN for whoever sees its token. attend's queries and 16-bit outputs are bf16, its scores q.k * scale and sums fp32; a probability times its token's value
+ * would round to 16 bits; a head that holds an infinity or NaN is NaN for whoever sees its token. attend's queries and 16-bit outputs are bf16, its scores q.k * scale (times log2 e within fp32's range) and sums fp32; a probability times its token's value
  * scale is rounded to fp16, relative to the row's largest such product; attend takes value scales below 2^-60 as 2^-60, and negative ones and those above 2^40 as NaN. In all else they are spl_paged_append and spl_paged_attend, which refuse a cache with scales as these refuse one without. */
 spl_status spl_paged_append_scaled(spl_paged *paged, int32_t type, const void *device_q, int64_t q_ld, const void *device_k, int64_t k_ld, const void *device_v, int64_t v_ld, const spl_tensor *q_norm,
                                    const spl_tensor *k_norm, void *device_q_out, void *device_k_cache, void *device_v_cache, float *device_k_scale, float *device_v_scale, void *stream);

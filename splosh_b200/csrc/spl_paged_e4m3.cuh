@@ -89,9 +89,9 @@ template <int ID> __device__ __forceinline__ bool spl_named_barrier_or(bool mine
 __device__ __forceinline__ bool spl_paged8_barrier_or(int which, bool mine) {
     return which == 0 ? spl_named_barrier_or<1>(mine) : which == 1 ? spl_named_barrier_or<2>(mine) : which == 2 ? spl_named_barrier_or<3>(mine) : spl_named_barrier_or<4>(mine);
 }
-// A row's P are 2^(y + offset), offset = 7 - reference. While no y + offset of a tile is above SPL_PAGED8_MOST the reference may stay, and nobody looks for a maximum; a row that has seen nothing has an offset that takes any number above that.
+// A row's P are 2^(y + offset), offset = 7 - reference. While no y + offset of a tile is above SPL_PAGED8_MOST the reference may stay, and nobody looks for a maximum; a row that has seen nothing has an offset that takes any number above that: the largest of fp32, so that scores far below zero raise it, too.
 #define SPL_PAGED8_MOST 15.0f
-#define SPL_PAGED8_UNSEEN 1.0e30f
+#define SPL_PAGED8_UNSEEN 3.402823466e38f
 __device__ __forceinline__ float spl_lg2(float x) { float y; asm("lg2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ float spl_rcp(float x) { float y; asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x)); return y; }
 

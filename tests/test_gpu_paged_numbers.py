@@ -1,4 +1,4 @@
-"""Attention over a paged cache where numbers end: what is no number in tokens whose pieces are joined. Wherever a sequence is cut, a row answers as in one piece."""
+"""Attention over a paged cache where numbers end: what is no number in tokens whose pieces are joined, and scores near the ends of fp32. Wherever a sequence is cut, a row answers as in one piece."""
 import pytest
 import torch
 
@@ -81,3 +81,40 @@ def test_a_value_that_is_no_number_in_a_piece_of_vanishing_weight(engine, dtype,
     assert out[:rows, :group, 5].isnan().all()
     out[:rows, :group, 5] = good[:rows, :group, 5]
     assert torch.equal(out, good)
+
+
+def aligned(scene, scale_of, query):
+    """Every key of the first sequence is the same vector, every query that vector times `query`; the keys' scales are scale_of(token)."""
+    heads, kv_heads, dim = scene.heads, scene.kv_heads, scene.head_dim
+    g = torch.Generator().manual_seed(9)
+    direction = torch.where(torch.rand(dim, generator=g) < 0.5, -1.0, 1.0)
+    scene.q[:] = (query * direction).to(torch.bfloat16)
+    scene.dq.copy_(scene.q)
+    scene.k.view(torch.uint8).copy_(direction.to(torch.float8_e4m3fn).view(torch.uint8).cuda().expand(scene.k.shape))
+    for token in range(scene.lengths[0]):
+        scene.ks[int(scene.table[0, token // scene.page_tokens]), :, token % scene.page_tokens] = scale_of(token)
+
+
+SHAPES = [(4, 1, 128, 1), (24, 4, 256, 1), (8, 2, 256, 4), (12, 1, 128, 4), (8, 1, 64, 1), (32, 2, 128, 5), (8, 1, 256, 40)]
+
+
+def one_weight(engine, heads, kv_heads, head_dim, rows, length, best, query, least):
+    """All scores far below zero (or above), one of them the largest by far: its token's value comes out, however the sequence is cut. The weight is exactly one, so the value is off by the roundings of its scale's
+    reciprocal, of that one's and of the product with it: 2^-21 is more than these."""
+    rows = min(rows, length)
+    best = min(best, length - rows)
+    scene = Scene(length, heads, kv_heads, head_dim, [rows], [length], page_tokens=64)
+    # (Negative scores: the smallest scale's is the largest.)
+    aligned(scene, lambda token: least if token == best else 4.0 * least if query < 0 else 0.25 * least, query)
+    assert 1e30 < abs(query) * head_dim ** 0.5 * 1.44 * least and abs(query) * head_dim * 4.0 * least < 3.0e38
+    out = attend(engine, scene, "f32").double().cpu()
+    _, _, values, v_scale = scene.tokens[0]
+    want = (values[best] * v_scale[best, :, None]).repeat_interleave(heads // kv_heads, 0)[None]
+    assert ((out - want).abs() <= 2.0 ** -21 * want.abs()).all()
+
+
+@pytest.mark.parametrize("heads,kv_heads,head_dim,rows", SHAPES)
+@pytest.mark.parametrize("length,best", [(40, 0), (129, 128), (300, 130), (2000, 7), (2000, 1500)])
+@pytest.mark.parametrize("query,least", [(-1.0, 1e30), (-1.0, 1e32), (1.0, 1e31)])
+def test_scores_far_below_zero(engine, heads, kv_heads, head_dim, rows, length, best, query, least):
+    one_weight(engine, heads, kv_heads, head_dim, rows, length, best, query, least)
