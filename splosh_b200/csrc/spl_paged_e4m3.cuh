@@ -412,14 +412,14 @@ spl_paged_attend_e4m3_kernel(const __grid_constant__ CUtensorMap k_map, const __
                     spl_tc_ld_rows(x, at + part * 32);
                     spl_tc_ld_rows(x + 16, at + (16u << 16) + part * 32);
                     spl_tc_ld_done(x);
-                    // y = score ks c + log2 vs.
+                    // y = score c ks + log2 vs. (In this order: score c is the row's own size times codes, while score ks could pass fp32's range where y does not.)
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const float2 k = k2[4 * j], l = l2[4 * j];
 #pragma unroll
                         for (int n = 0; n < 4; ++n) {
                             uint32_t *z = x + n / 2 * 16 + 4 * j + n % 2 * 2;
-                            const float2 y = spl_fma2(spl_mul2(make_float2(__uint_as_float(z[0]), __uint_as_float(z[1])), k), make_float2(c[n], c[n]), l);
+                            const float2 y = spl_fma2(spl_mul2(make_float2(__uint_as_float(z[0]), __uint_as_float(z[1])), make_float2(c[n], c[n])), k, l);
                             z[0] = __float_as_uint(y.x); z[1] = __float_as_uint(y.y);
                         }
                     }
@@ -874,11 +874,11 @@ spl_paged_attend_e4m3_narrow_kernel(const __grid_constant__ CUtensorMap k_map, c
 #pragma unroll
                 for (int n = 0; n < H; n += 8) { spl_tc_ld8_later(x + n, at + n); spl_tc_ld8_later(x + H + n, at + N + n); }
                 spl_tc_ld_done_of<2 * H>(x);
-                // y = score ks c + log2 vs.
+                // y = score c ks + log2 vs (in this order, as above).
                 auto two = [](const uint32_t *v) { return make_float2(__uint_as_float(v[0]), __uint_as_float(v[1])); };
                 float2 y[H / 2];
 #pragma unroll
-                for (int n = 0; n < H / 2; ++n) y[n] = spl_fma2(spl_mul2(spl_add2(two(x + 2 * n), two(x + H + 2 * n)), make_float2(k, k)), c[n], make_float2(l, l));
+                for (int n = 0; n < H / 2; ++n) y[n] = spl_fma2(spl_mul2(spl_add2(two(x + 2 * n), two(x + H + 2 * n)), c[n]), make_float2(k, k), make_float2(l, l));
                 if (tile * 128 < seen_by_all || tile * 128 + 128 > unseen_by_some) {
                     const int token = tile * 128 + mine, length = a.items[i].length;
                     auto hidden = [&](int n) {

@@ -118,3 +118,11 @@ def one_weight(engine, heads, kv_heads, head_dim, rows, length, best, query, lea
 @pytest.mark.parametrize("query,least", [(-1.0, 1e30), (-1.0, 1e32), (1.0, 1e31)])
 def test_scores_far_below_zero(engine, heads, kv_heads, head_dim, rows, length, best, query, least):
     one_weight(engine, heads, kv_heads, head_dim, rows, length, best, query, least)
+
+
+@pytest.mark.parametrize("heads,kv_heads,head_dim,rows", SHAPES)
+@pytest.mark.parametrize("length,best", [(40, 0), (300, 130), (2000, 1500)])
+@pytest.mark.parametrize("query,least", [(-2.0 ** -20, 1e36), (2.0 ** -10, 1e36), (2.0 ** -20, 1e37)])
+def test_scales_of_keys_near_the_end_of_fp32(engine, heads, kv_heads, head_dim, rows, length, best, query, least):
+    """Keys whose scores with these queries are ordinary fp32 numbers, although their products with the queries' codes would not be."""
+    one_weight(engine, heads, kv_heads, head_dim, rows, length, best, query, least)
