@@ -555,6 +555,13 @@ spl_status spl_debug_paged_plan_shared(const spl_paged_config *config, int32_t b
                                        int32_t *record_count, int64_t *partial_rows, int32_t *joint) {
     if (!config || !rows || !lengths || !block_begin || !items || !item_count || !records || !record_count || !partial_rows || !joint || blocks < 1 || sequences < 1 || groups < 0 ||
         (groups && (!group_sequences || !group_tokens)) || spl_paged_config_error(*config)) return SPL_ERR_INVALID_ARGUMENT;
+    // (No pages here: of what spl_paged_batch_shared checks, what the plan goes by.)
+    for (int i = 0; i < sequences; ++i) if (rows[i] < 0 || lengths[i] < rows[i]) return SPL_ERR_INVALID_ROWS;
+    int64_t at = 0;
+    for (int g = 0; g < groups; ++g) {
+        if (group_sequences[g] < 1 || at + group_sequences[g] > sequences || group_tokens[g] < 0) return SPL_ERR_INVALID_ROWS;
+        for (int64_t end = at + group_sequences[g]; at < end; ++at) if (group_tokens[g] > lengths[at] - rows[at]) return SPL_ERR_INVALID_ROWS;
+    }
     try {
         SplPagedPlan plan;
         const SplPagedGroups g{groups, group_sequences, group_tokens};
