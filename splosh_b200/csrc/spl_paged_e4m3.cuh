@@ -574,8 +574,9 @@ spl_paged_attend_e4m3_kernel(const __grid_constant__ CUtensorMap k_map, const __
 // lies there, and the rows are columns:
 //   S^T[128 tokens x 2 N]       = K [hi; lo]^T            A = K (tokens by channels), B = the N queries' two parts, so that K is read once; a score is the sum of two columns
 //   O^T[128 channels x 3 N]    += V^T [P1; P2; P3]        A = V (a block of 128 channels), B = P in three parts: units of sixteen columns of one part, sixteen bytes a token, token after token
-// P is a number in fp16, of which e5m2 is the upper byte: P1 is that byte, P2 the upper byte of what it leaves, P3 that of what both leave, rounded: nine significant bits or more over all of fp16's range. The parts' sums are
-// columns of their own and are added at the piece's end. (A unit is the operand's layout without a swizzle, its columns the inner dimension: a thread stores its part of a unit at once. With a row of 128 tokens for each column a
+// P is a number in fp16 of at most 2^15, of which e5m2 is the upper byte: P1 is P rounded to that (three significant bits), P2 sixteen times what that leaves, rounded likewise, P3 sixteen times what that leaves. What is left
+// has either sign and at most an eighth of the part's size, so three parts hold the eleven bits; with the factors of sixteen also of the subnormals, down to fp16's own 2^-24: P1 + P2 / 16 + P3 / 256 is P, exactly, for all of
+// them. The parts' sums are columns of their own and are added at the piece's end. (A unit is the operand's layout without a swizzle, its columns the inner dimension: a thread stores its part of a unit at once. With a row of 128 tokens for each column a
 // tile's probabilities were 48 one-byte stores a thread and half of the softmax's time.)
 // A softmax thread has a token, and 8 or 16 of the columns (groups of four warps share these out): the token's scales, which came with its keys, are its own registers, a row's maximum, where one is wanted, is a reduction over lanes (redux) and
 // four warps, its sum stays in the threads until the piece's end. The last four warps copy keys, issue the scores' and the sums' products, copy values.
@@ -606,8 +607,11 @@ __device__ __forceinline__ uint16_t spl_e5m2_of_halves(uint32_t v) {
     asm("cvt.rn.satfinite.e5m2x2.f16x2 %0, %1;\n" : "=h"(d) : "r"(v));
     return d;
 }
-__device__ __forceinline__ uint32_t spl_half2_sub(uint32_t a, uint32_t b) {
-    const __half2 d = __hsub2(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&b));
+// Two halves rounded to their upper bytes (a carry raises the exponent, as it should). What is no number becomes -0: what it leaves is none, and so the last part.
+__device__ __forceinline__ uint32_t spl_halves_to_e5m2(uint32_t v) { return (v + 0x00800080u) & 0xff00ff00u; }
+// Sixteen times what they leave.
+__device__ __forceinline__ uint32_t spl_half2_left16(uint32_t a, uint32_t b) {
+    const __half2 d = __hmul2(__hsub2(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&b)), __float2half2_rn(16.0f));
     return *reinterpret_cast<const uint32_t *>(&d);
 }
 
@@ -935,14 +939,16 @@ spl_paged_attend_e4m3_narrow_kernel(const __grid_constant__ CUtensorMap k_map, c
                 uint32_t part[3][H / 4];
 #pragma unroll
                 for (int n = 0; n < H / 4; ++n) {
-                    uint32_t p[2], rest[2], low[2];
+                    uint32_t p[2], rest[2], low[2];      // the parts, the first two in the upper bytes of halves
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         const float2 z = spl_add2(y[2 * n + e], offset[2 * n + e]), w = make_float2(spl_ex2(z.x), spl_ex2(z.y));
                         sum[2 * n + e] = spl_fma2(w, make_float2(inv, inv), sum[2 * n + e]);
-                        p[e] = spl_pack16<false>(w.x, w.y);
-                        rest[e] = spl_half2_sub(p[e], p[e] & 0xff00ff00u);
-                        low[e] = spl_e5m2_of_halves(spl_half2_sub(rest[e], rest[e] & 0xff00ff00u));
+                        const uint32_t whole = spl_pack16<false>(w.x, w.y);
+                        p[e] = spl_halves_to_e5m2(whole);
+                        const uint32_t left = spl_half2_left16(whole, p[e]);
+                        rest[e] = spl_halves_to_e5m2(left);
+                        low[e] = spl_e5m2_of_halves(spl_half2_left16(left, rest[e]));
                     }
                     part[0][n] = __byte_perm(p[0], p[1], 0x7531); part[1][n] = __byte_perm(rest[0], rest[1], 0x7531); part[2][n] = low[0] | low[1] << 16;
                 }
@@ -999,7 +1005,7 @@ spl_paged_attend_e4m3_narrow_kernel(const __grid_constant__ CUtensorMap k_map, c
                     spl_tc_ld_done_of<24>(o);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        const float value = (__uint_as_float(o[j]) + __uint_as_float(o[8 + j]) + __uint_as_float(o[16 + j])) * __shfl_sync(0xffffffffu, inv, n + j);
+                        const float value = fmaf(__uint_as_float(o[16 + j]), 1.0f / 256.0f, fmaf(__uint_as_float(o[8 + j]), 1.0f / 16.0f, __uint_as_float(o[j]))) * __shfl_sync(0xffffffffu, inv, n + j);
                         const int x = head0 + n0 + n + j, row = int(x * per_group >> 16), channel = b * 128 + mine;
                         if (n0 + n + j >= it.q_count) continue;
                         const size_t place = (size_t(row0 + row) * s.heads + it.kv_head * s.group + x - row * s.group) * HD + channel;
