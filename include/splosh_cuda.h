@@ -473,7 +473,8 @@ spl_status spl_paged_append(spl_paged *paged, int32_t type, const void *device_q
 spl_status spl_paged_attend(spl_paged *paged, const void *device_q, const void *device_k_cache, const void *device_v_cache, int32_t out_type, void *device_out, void *stream);
 /* A cache of SPL_E4M3: a token's keys of one kv head are head_dim codes times one scale, its values likewise, at half the memory and traffic of 16 bits. The scales are the caller's, fp32 [pages][kv_heads][page_tokens]
  * for keys and for values, on 16-byte boundaries. append takes scale = max |y| / 448 over the head's channels (at least 2^-100) and code = y * (1 / scale), in fp32, to nearest even, y what spl_paged_append
- * would round to 16 bits; a head that holds an infinity or NaN is NaN for whoever sees its token. attend's queries and 16-bit outputs are bf16, its scores q.k * scale (times log2 e within fp32's range) and sums fp32; a probability times its token's value
+ * would round to 16 bits; for whoever sees its token a head that holds an infinity is NaN, and keys that hold a NaN are; a NaN among values is one in its own channel. attend's queries and 16-bit outputs are bf16 (a channel
+ * below 2^-7 of its row's largest is off by up to 2^-17 of that), its scores q.k * scale (times log2 e within fp32's range) and sums fp32; a probability times its token's value
  * scale is rounded to fp16, relative to the row's largest such product; attend takes value scales below 2^-60 as 2^-60, and negative ones and those above 2^40 as NaN. In all else they are spl_paged_append and spl_paged_attend, which refuse a cache with scales as these refuse one without. */
 spl_status spl_paged_append_scaled(spl_paged *paged, int32_t type, const void *device_q, int64_t q_ld, const void *device_k, int64_t k_ld, const void *device_v, int64_t v_ld, const spl_tensor *q_norm,
                                    const spl_tensor *k_norm, void *device_q_out, void *device_k_cache, void *device_v_cache, float *device_k_scale, float *device_v_scale, void *stream);
@@ -481,8 +482,8 @@ spl_status spl_paged_attend_scaled(spl_paged *paged, const void *device_q, const
                                    void *device_out, void *stream);
 /* spl_paged_batch for sequences that begin with the same tokens (a system prompt, continuations of one prompt): group g is the batch's next group_sequences[g] sequences, whose first group_tokens[g] tokens
  * lie in the same pages (whole pages, in front of every member's new rows, the same entries of the page table; SPL_ERR_INVALID_ROWS otherwise). Sequences behind the last group share nothing. attend then reads
- * the whole tiles of 128 tokens of a shared prefix once for up to 128 packed rows (a row's heads that share a kv head; 48 over a cache of SPL_E4M3 with heads of 128 or 256 and at most 48 a sequence) of its group instead of once a sequence, where that saves more than the joining costs: without a window, for sequences of at most 128
- * packed rows. The results are the same to the rounding of fp32 sums. The first call sets device memory aside for it (two partial sums a packed row); a graph captured before or after may be replayed after batches with
+ * the whole tiles of 128 tokens of a shared prefix once for up to 128 packed rows (a row's heads that share a kv head; 48 over a cache of SPL_E4M3 with heads of 128 or 256 and at most 48 a sequence) of its group instead of once a sequence, where a rule expects that to save more than the joining costs: without a window, for sequences of at most 128
+ * packed rows. (The rule was set by heads of 256. In batches of 10 to 35 us with heads of 64 and 128 it saves up to half, and costs up to 7 us in some with few rows a kv head; a batch without groups is never dealt so.) The results are the same to the rounding of fp32 sums. The first call sets device memory aside for it (two partial sums a packed row); a graph captured before or after may be replayed after batches with
  * groups and without. */
 spl_status spl_paged_batch_shared(spl_paged *paged, int32_t sequences, const int32_t *rows, const int32_t *lengths, const int32_t *page_table, int32_t table_ld, int32_t groups, const int32_t *group_sequences,
                                   const int32_t *group_tokens, void *stream);

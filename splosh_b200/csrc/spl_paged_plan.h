@@ -143,7 +143,8 @@ inline int64_t spl_paged_take(int64_t t, int64_t left, int64_t stretch, int q_co
 // With groups, the sequences of a run (consecutive members of a group, none with more packed rows than a block takes) meet the whole tiles of their prefix
 // together: their rows lie one behind the other, so they are the rows of one sequence over the prefix, in blocks of 128 packed rows whoever's they are; each sequence's own
 // tokens are units of their own, and both leave partial sums (O, m, l) that spl_paged_combine_kernel joins. (Sequences of more packed rows read the prefix once for 128 of them as it is.)
-// Over a cache of e4m3 a batch takes the transposed form by the most packed rows that a sequence has, also where sequences meet a prefix together (48 rows a block then), so a graph that holds one form is right for
+// Over a cache of e4m3 a batch takes the transposed form by the most packed rows that a sequence has (so a prompt's rows, or one block of 54 packed, take it from all: six decode rows over 6,000 tokens of 24/4 heads of 256
+// 21.6 us, 301 prompt rows 19.6, in one batch 60.4, where 16 bits take 38.2; nine blocks of eight rows 41.1, with one of nine rows among them 63.2; twelve decode rows and a block of eight rows 45.2, of nine 78.9), also where sequences meet a prefix together (48 rows a block then), so a graph that holds one form is right for
 // every batch of its rows. Transposed and wide, before pieces were joined by rows: heads of 256 (24 on 4), eight sequences of about 6,000 tokens with 6, 12, 24, 36 and 48 packed rows 27.7 and 51.4, 31.2 and 54.7, 40.4 and
 // 56.1, 48.3 and 65.0, 51.2 and 67.9 us; of 128 (32 on 8), with 8, 16, 32 and 48 21.5 and 35.0, 23.9 and 38.7, 30.6 and 37.0, 37.6 and 47.7. (For 64 rows the sums of three parts
 // and two blocks of channels, 384 columns of tensor memory, and two tiles' scores, 256, are more than its 512.)
@@ -152,7 +153,7 @@ inline bool spl_paged_narrow(const spl_paged_config &c, int64_t packed) { return
 // (24 on 4), two rows over 4,000 tokens 27.7 and 16.5 us, eight of two over 7,200 35.8 and 31.5, one verify block of eight rows over 1,000, 4,000 and 32,000 22.2 and 15.7, 39.2 and 17.0, 82.7 and 31.2, one of sixteen
 // over 4,000 66.9 and 22.1, eight of eight over 39,000 135.7 and 123.6; heads of 64 (16 on 2), eight of sixteen over 3,600 45.8 and 18.9; 32 sequences, of which few are cut, the same. With fewer rows a piece's join
 // is short and the launch counts: one row over 1,000 tokens 10.0 and 11.5, over 4,000 14.4 and 14.5, twelve over 900 12.8 and 13.2, 32 over 2,700 41.6 and 42.5. Prompts: 300 rows over 300 tokens 19.7 and 22.8,
-// 2,048 over 8,192 1,358 and 1,396.
+// 2,048 over 26,624 1,358 and 1,396. (Here and below of three sets of data in turn.)
 inline bool spl_paged_split(const spl_paged_config &c, int64_t packed) { return c.dtype == SPL_E4M3 && packed > 8 && packed <= SPL_PAGED_TILE; }
 // Meeting together pays where the tiles saved are more than the joining: so many a block for one more launch and the pieces' first keys, and one for so many rows of heads that leave and join sums. Measured with
 // heads of 256, 24 of them on 4, together and apart:
@@ -161,6 +162,14 @@ inline bool spl_paged_split(const spl_paged_config &c, int64_t packed) { return 
 //   transposed    (apart it is quick where sequences find the same keys in L2) six of one row over 4,096 19.4 and 15.7, sixteen over 2,048 19.2 and 19.3, 48 over 1,024 31.1 and 31.2; two of four rows over
 //                 20,992 28.1 and 27.0, four 35.3 and 36.1, eight 46.9 and 59.0; 24 of four over 4,096 47.4 and 50.0, 24 of six 63.2 and 58.5;
 //   e4m3, wide    eight of sixteen rows over 4,096 53.7 and 45.5, over 20,992 116 and 126.
+// A tile counts the same whatever its channels, though one of 64 is a quarter of the bytes and a join is not. Other heads, together and apart, where the rule deals them together:
+//   32 on 8 of 128, 16 bits   six of one row over 1,024 11.8 and 13.1, sixteen over 1,024 14.1 and 20.1, 48 over 1,024 27.1 and 53.6; sixteen of four over 512 18.3 and 15.2, over 2,048 19.8 and 29.8;
+//     transposed              two of one row over 16,384 17.4 and 25.1, six over 4,096 14.8 and 19.1, sixteen over 1,024 22.4 and 16.0, over 2,048 23.8 and 23.0; six of four over 4,096 23.6 and 20.2, sixteen over 2,048
+//                             32.1 and 25.5;
+//   32 on 8 of 64             16 bits sixteen of one row over 1,024 12.8 and 19.2, of four over 512 16.3 and 13.9, over 2,048 18.3 and 27.0; e4m3 15.8 and 29.8, 21.6 and 23.0, 25.6 and 48.1;
+//   16 on 2 of 64             16 bits two of one row over 16,384 20.6 and 16.1, sixteen over 2,048 16.2 and 13.8, 48 over 1,024 16.3 and 18.1, two of four over 16,384 20.8 and 25.6; e4m3 sixteen of one over 1,024 20.0
+//                             and 15.0, 48 over 1,024 21.1 and 25.8.
+// So with eight packed rows a sequence or fewer on two kv heads, and transposed with 128 channels, it takes the slower of the two in places.
 inline bool spl_paged_joint_pays(int64_t saved, int blocks, int64_t rows_of_heads, bool narrow) { return saved > int64_t(blocks) * (narrow ? 4 : 1) + rows_of_heads / (narrow ? 3 : 10); }
 struct SplPagedUnit { SplPagedItem item; bool joint; int run, prefix; };      // run: its run of sequences or -1; prefix: the first of its run's prefix units of its kv head
 inline void spl_paged_plan(const spl_paged_config &c, int blocks, int32_t sequences, const int32_t *rows, const int32_t *lengths, SplPagedPlan &plan, const SplPagedGroups *groups = nullptr) {
